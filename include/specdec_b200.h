@@ -32,6 +32,8 @@
  *   specdec_lmhead_argmax        <- logits = x @ embed_tokens.weight.T (model_self.py:857)
  *                                   followed by the executors' argmax (spec_dec.py:230-236,
  *                                   fast_spec_dec.py:246-249), fused: no logits are written
+ *   specdec_*_int8               <- no counterpart (the reference's linear layers are bf16):
+ *                                   8-bit activations and weights for the decoder's projections
  */
 #ifndef SPECDEC_B200_H_
 #define SPECDEC_B200_H_
@@ -352,6 +354,48 @@ int specdec_swiglu(const void* gate, const void* up, void* out, int32_t dtype, i
  * bf16(bf16(silu(g)) * u) with silu from the hardware exponential and reciprocal (at most
  * one bf16 ulp from specdec_swiglu); inter % 8 == 0, 16-byte aligned rows. */
 int specdec_swiglu_packed(const void* gate_up, void* out, int64_t rows, int64_t inter, specdec_stream_t stream);
+
+/*
+ * 8-bit linear layers: rows of activations (and of weights) as int8 codes with one f32 scale
+ * a row, and the product of two such matrices.
+ *
+ *   int8(v) of a row v:  m = max(max|v|, 2^-100);  scale = m / 127;  code = rint(v * (127 / m))
+ *
+ * in fp32, ties to even.  A row that holds an infinity or a NaN gets scale NaN and codes 0
+ * (everything computed from it is NaN).  Activations are f32 or bf16 (`dtype`), rows
+ * `x_stride` elements apart with contiguous columns; code rows are `codes_stride` bytes apart.
+ * rows == 0 launches nothing.  A weight (out_features, width) quantised by rows has the scale
+ * for each output channel that specdec_linear_int8 takes.
+ */
+/* codes = int8(x) */
+int specdec_quantize_int8(const void* x, int64_t x_stride, void* codes, int64_t codes_stride, float* scale,
+                          int32_t dtype, int64_t rows, int32_t width, specdec_stream_t stream);
+/* s = x + residual (s = x without one);  codes = int8(s / sqrt(mean(s^2) + eps) * weight) in fp32 from the
+   unrounded sum; summed receives s rounded to the input type.  residual and summed are both given or both
+   NULL; summed may be x or residual (same stride). */
+int specdec_rmsnorm_int8(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                         const void* weight, float eps, void* summed, int64_t summed_stride, void* codes,
+                         int64_t codes_stride, float* scale, int32_t dtype, int64_t rows, int32_t hidden,
+                         specdec_stream_t stream);
+/* codes = int8(silu(gate) * up), a row of gate_up holding gate (inter values), then up (inter values) */
+int specdec_swiglu_int8(const void* gate_up, int64_t x_stride, void* codes, int64_t codes_stride, float* scale,
+                        int32_t dtype, int64_t rows, int32_t inter, specdec_stream_t stream);
+/* out = code * scale, rounded to `dtype` */
+int specdec_dequantize_int8(const void* codes, int64_t codes_stride, const float* scale, void* out,
+                            int64_t out_stride, int32_t dtype, int64_t rows, int32_t width, specdec_stream_t stream);
+/*
+ * out[r][n] = (sum_k a[r][k] w[n][k]) * a_scale[r] * w_scale[n] + bias[n]
+ * a (rows, width), w (out_features, width) int8 codes, 16-byte aligned, row strides multiples of 16 bytes
+ * (what lies between a row's end and its stride is never used); scales and the optional bias f32; out f32 or
+ * bf16 (`out_dtype`), rows `out_stride` elements apart.  The sum is exact (width <= 131072), the rest fp32
+ * with one rounding to the output type.  rows <= 2^21.
+ * weight_ready 1: the caller promises that the work right before the call on the stream does not write w, so
+ * the kernel may load it while that work finishes.  status (optional): SPECDEC_STATUS_TIMEOUT.
+ */
+int specdec_linear_int8(const void* a, int64_t a_stride, const float* a_scale, const void* w, int64_t w_stride,
+                        const float* w_scale, const float* bias, void* out, int64_t out_stride, int32_t out_dtype,
+                        int64_t rows, int32_t width, int32_t out_features, int32_t weight_ready, int32_t* status,
+                        specdec_stream_t stream);
 
 /* Diagnostics. */
 /* Tensor-core self-check (no counterpart in the reference): one CTA computes, with

@@ -207,6 +207,17 @@ SIGNATURES = {
     "specdec_attention_fp8v": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _sz,
                                               _vp]),
     "specdec_lmhead_argmax": (ctypes.c_int, [_vp, _vp]),
+    "specdec_quantize_int8": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _vp]),
+    "specdec_rmsnorm_int8": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, _i64, _vp, ctypes.c_float, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _vp],
+    ),
+    "specdec_swiglu_int8": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _vp]),
+    "specdec_dequantize_int8": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i32, _i64, _i32, _vp]),
+    "specdec_linear_int8": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _vp],
+    ),
     "specdec_last_error": (ctypes.c_char_p, []),
     "specdec_abi_version": (ctypes.c_int, []),
     "specdec_launch_count": (_i64, []),

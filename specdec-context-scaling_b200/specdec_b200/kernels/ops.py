@@ -8,7 +8,8 @@ C ABI -- so ``backend`` must be ``"cuda"``; any other value raises
 
 Beyond the reference's four ops this module exposes the paged decode path:
 ``paged_attention``, ``ragged_plan``, ``append_kv``, ``greedy_accept`` and
-``trim_lengths``.
+``trim_lengths``; and the 8-bit linear path: ``rmsnorm_int8``, ``quantize_int8``,
+``swiglu_int8``, ``linear_int8`` and ``dequantize_int8``.
 """
 
 from __future__ import annotations
@@ -549,4 +550,146 @@ def trim_lengths(cur_len, new_len, out=None, status=None):
     rc = _lib_handle().specdec_trim(cur_len.data_ptr(), new_len.data_ptr(), out.data_ptr(), int(cur_len.numel()),
                                     _ptr(status), _stream())
     _lib.check(rc, "trim")
+    return out
+
+
+# ---------------------------------------------------------------------------- 8-bit linear path
+def _raw_stream(t: torch.Tensor) -> int:
+    """The current stream of ``t``'s device, which has to be the current device."""
+    if not t.is_cuda:
+        raise RuntimeError("tensors must be CUDA")
+    dev = t.get_device()
+    if dev != torch._C._cuda_getDevice():
+        raise RuntimeError(f"tensor is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _int8_rows_out(x: torch.Tensor, width: int, codes, scale):
+    """Check ``x`` (rows, .) f32 / bf16; its dtype code and the codes (rows, width) and scale (rows,)
+    to write.  New codes have a row stride that is a multiple of 16 bytes, as linear_int8 reads them."""
+    code = _dtype_code(x)
+    if code < 0 or x.dim() != 2 or x.stride(1) != 1 and x.shape[1] != 1:
+        raise ValueError("x must be (rows, width) float32 or bfloat16 with contiguous columns")
+    rows = x.shape[0]
+    if codes is None:
+        stride = (width + 15) & ~15
+        codes = torch.empty((rows, stride), dtype=torch.int8, device=x.device)
+        if stride != width:
+            codes = codes[:, :width]
+    elif codes.dtype != torch.int8 or codes.shape != (rows, width) or codes.stride(1) != 1 or not codes.is_cuda:
+        raise ValueError("codes must be int8 (rows, width) with contiguous columns")
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    elif scale.dtype != torch.float32 or scale.shape != (rows,) or not scale.is_contiguous() or not scale.is_cuda:
+        raise ValueError("scale must be contiguous float32 (rows,)")
+    return code, codes, scale
+
+
+def quantize_int8(x, *, codes=None, scale=None):
+    """Rows of ``x`` (rows, width) f32 / bf16 as int8 codes with one f32 scale a row:
+    m = max(max|x|, 2^-100), scale = m / 127, code = rint(x * (127 / m)).  Returns (codes, scale);
+    a row with an infinity or a NaN gets scale NaN and codes 0.  Rows of a weight (out_features,
+    width) give the codes and the per-channel scale that ``linear_int8`` takes."""
+    stream = _raw_stream(x)
+    code, codes, scale = _int8_rows_out(x, x.shape[-1], codes, scale)
+    rows, width = x.shape
+    rc = _lib_handle().specdec_quantize_int8(x.data_ptr(), x.stride(0), codes.data_ptr(), codes.stride(0),
+                                             scale.data_ptr(), code, rows, width, stream)
+    _lib.check(rc, "quantize_int8")
+    return codes, scale
+
+
+def rmsnorm_int8(x, weight, eps: float = 1e-6, *, residual=None, summed=None, codes=None, scale=None):
+    """s = x + residual (s = x without one), then int8 rows of s / sqrt(mean(s^2) + eps) * weight,
+    all in fp32 from the unrounded sum.  Returns (codes, scale, summed): ``summed`` is s in x's dtype
+    (None without a residual); it may be given as x or residual, to update that in place."""
+    stream = _raw_stream(x)
+    code, codes, scale = _int8_rows_out(x, x.shape[-1], codes, scale)
+    rows, hidden = x.shape
+    if weight.dtype != x.dtype or weight.shape != (hidden,) or not weight.is_contiguous() or not weight.is_cuda:
+        raise ValueError("weight must be contiguous (hidden,) of x's dtype")
+    r_ptr = s_ptr = None
+    r_stride = s_stride = hidden
+    if residual is not None:
+        if summed is None:
+            summed = torch.empty((rows, hidden), dtype=x.dtype, device=x.device)
+        for t in (residual, summed):
+            if t.dtype != x.dtype or t.shape != x.shape or t.stride(1) != 1 and hidden != 1 or not t.is_cuda:
+                raise ValueError("residual and summed must be (rows, hidden) of x's dtype with contiguous columns")
+        r_ptr, r_stride, s_ptr, s_stride = residual.data_ptr(), residual.stride(0), summed.data_ptr(), summed.stride(0)
+    elif summed is not None:
+        raise ValueError("summed is written only with a residual")
+    rc = _lib_handle().specdec_rmsnorm_int8(x.data_ptr(), x.stride(0), r_ptr, r_stride, weight.data_ptr(), eps, s_ptr,
+                                            s_stride, codes.data_ptr(), codes.stride(0), scale.data_ptr(), code, rows,
+                                            hidden, stream)
+    _lib.check(rc, "rmsnorm_int8")
+    return codes, scale, summed
+
+
+def swiglu_int8(gate_up, *, codes=None, scale=None):
+    """int8 rows of silu(gate) * up, in fp32, of a fused (rows, 2 inter) projection.  Returns (codes, scale)."""
+    stream = _raw_stream(gate_up)
+    if gate_up.dim() != 2 or gate_up.shape[1] % 2:
+        raise ValueError("gate_up must be (rows, 2 inter)")
+    rows, inter = gate_up.shape[0], gate_up.shape[1] // 2
+    code, codes, scale = _int8_rows_out(gate_up, inter, codes, scale)
+    rc = _lib_handle().specdec_swiglu_int8(gate_up.data_ptr(), gate_up.stride(0), codes.data_ptr(), codes.stride(0),
+                                           scale.data_ptr(), code, rows, inter, stream)
+    _lib.check(rc, "swiglu_int8")
+    return codes, scale
+
+
+def dequantize_int8(codes, scale, *, out=None, dtype=torch.bfloat16):
+    """codes * scale of int8 rows, in ``dtype`` (f32 or bf16) or into ``out``."""
+    stream = _raw_stream(codes)
+    if codes.dtype != torch.int8 or codes.dim() != 2 or codes.stride(1) != 1 and codes.shape[1] != 1:
+        raise ValueError("codes must be int8 (rows, width) with contiguous columns")
+    rows, width = codes.shape
+    if scale.dtype != torch.float32 or scale.shape != (rows,) or not scale.is_contiguous() or not scale.is_cuda:
+        raise ValueError("scale must be contiguous float32 (rows,)")
+    if out is None:
+        out = torch.empty((rows, width), dtype=dtype, device=codes.device)
+    code = _dtype_code(out)
+    if code < 0 or out.shape != (rows, width) or out.stride(1) != 1 and width != 1 or not out.is_cuda:
+        raise ValueError("out must be (rows, width) float32 or bfloat16 with contiguous columns")
+    rc = _lib_handle().specdec_dequantize_int8(codes.data_ptr(), codes.stride(0), scale.data_ptr(), out.data_ptr(),
+                                               out.stride(0), code, rows, width, stream)
+    _lib.check(rc, "dequantize_int8")
+    return out
+
+
+def linear_int8(codes, scale, weight_codes, weight_scale, *, bias=None, out=None, out_dtype=torch.bfloat16,
+                weight_ready: bool = False, status=None):
+    """out[r, n] = (sum_k codes[r, k] weight_codes[n, k]) * scale[r] * weight_scale[n] + bias[n].
+
+    ``codes`` (rows, width) and ``weight_codes`` (out_features, width) are int8 with 16-byte aligned rows
+    (as ``quantize_int8`` lays them out), ``scale``, ``weight_scale`` and ``bias`` f32, ``out`` f32 or bf16.
+    The integer sum is exact; the rest is fp32, rounded once.  ``weight_ready``: the caller promises that the
+    work right before this call on the stream does not write ``weight_codes``, so they may be loaded early."""
+    stream = _raw_stream(codes)
+    if codes.dtype != torch.int8 or weight_codes.dtype != torch.int8 or codes.dim() != 2 or weight_codes.dim() != 2:
+        raise ValueError("codes (rows, width) and weight_codes (out_features, width) must be 2-D int8")
+    rows, width = codes.shape
+    n = weight_codes.shape[0]
+    if weight_codes.shape[1] != width or (codes.stride(1) != 1 or weight_codes.stride(1) != 1) and width != 1:
+        raise ValueError("codes and weight_codes must share a contiguous width")
+    f32 = torch.float32
+    if scale.dtype != f32 or scale.shape != (rows,) or not scale.is_contiguous():
+        raise ValueError("scale must be contiguous float32 (rows,)")
+    if weight_scale.dtype != f32 or weight_scale.shape != (n,) or not weight_scale.is_contiguous():
+        raise ValueError("weight_scale must be contiguous float32 (out_features,)")
+    if bias is not None and (bias.dtype != f32 or bias.shape != (n,) or not bias.is_contiguous() or not bias.is_cuda):
+        raise ValueError("bias must be contiguous float32 (out_features,)")
+    if not (scale.is_cuda and weight_codes.is_cuda and weight_scale.is_cuda):
+        raise RuntimeError("tensors must be CUDA")
+    if out is None:
+        out = torch.empty((rows, n), dtype=out_dtype, device=codes.device)
+    code = _dtype_code(out)
+    if code < 0 or out.shape != (rows, n) or out.stride(1) != 1 and n != 1 or not out.is_cuda:
+        raise ValueError("out must be (rows, out_features) float32 or bfloat16 with contiguous columns")
+    rc = _lib_handle().specdec_linear_int8(
+        codes.data_ptr(), codes.stride(0), scale.data_ptr(), weight_codes.data_ptr(), weight_codes.stride(0),
+        weight_scale.data_ptr(), _ptr(bias), out.data_ptr(), out.stride(0), code, rows, width, n,
+        1 if weight_ready else 0, _ptr(status), stream)
+    _lib.check(rc, "linear_int8")
     return out
