@@ -1,70 +1,524 @@
 // int8_linear.cu -- linear layer over 8-bit activations and weights:
 //   y[r][n] = (sum_k a[r][k] w[n][k]) * a_scale[r] * w_scale[n] + bias[n]
-// The integer sum is exact: |sum| <= K 127^2 < 2^31 for K <= 131072.  Scales and bias are
-// applied in fp32 and the result is rounded once to the output type.
+// The integer sum is exact: |sum| <= K 127^2 < 2^31 for K <= 131072, in any order.  Scales and
+// bias are applied in fp32 and the result is rounded once to the output type.
 //
-// One block per 64 x 64 outputs, 64 codes of K at a time through shared memory, four
-// products per dot-product instruction.
+// The weight is the M operand: a tile is 128 output channels by up to 256 rows ("tokens") of a,
+// so a call of a few tokens wastes only columns of a narrow N, and an accumulator lane is an
+// output channel: a warp stores 32 neighbouring channels of one token at a time, whatever the
+// alignment of the output.
+//
+// linear_int8_kernel, 192 threads:
+//   warp 4    producer: TMA loads of the W tile [128 channels][128 codes] and the a tile
+//             [tokens][128 codes] of each 128-code chunk of K (128-byte swizzle, K-major; the
+//             ragged ends of K, N and the rows are filled with zeros by the TMA unit) into a
+//             ring of 4 to 12 stages;
+//   warp 5    one lane issues tcgen05.mma kind::i8 (K 32) into one of two TMEM accumulators,
+//             so a tile's epilogue overlaps the next tile's products;
+//   warps 0-3 epilogue: lane = channel, columns = tokens.
+// CG = 2: two CTAs on one 256-channel tile (cta_group::2).  Each loads its own 128 channels and
+// half of the tokens, so a chunk costs a CTA 128 + tokens / 2 rows of loads instead of
+// 128 + tokens; the pair's first CTA issues the products.
+// splits > 1 (CG = 1): a cluster of `splits` CTAs shares one tile, each taking a share of the
+// chunks of K, and adds up the integer partial sums through distributed shared memory.
+#include <cudaTypedefs.h>
+
 #include "sd_common.cuh"
 #include "sd_internal.h"
+#include "umma.cuh"
 
 namespace sd {
 
 constexpr int kMaxWidth = 131072;
 constexpr int kMaxRows = 1 << 21;
+constexpr int kLinThreads = 192;
+constexpr int kLinChunk = 128;                   // codes of K per stage
+constexpr int kLinCh = 128;                      // channels per CTA
+constexpr int kLinWTile = kLinCh * kLinChunk;    // 16 KB
+constexpr int kLinMaxStages = 12;
+constexpr int kLinRing = 216 * 1024;
+constexpr int kLinMaxTokens = 256;
 
 struct LinParams {
-  const int8_t* a;
-  const int8_t* w;
   const float* a_scale;
   const float* w_scale;
   const float* bias;
   void* out;
-  int64_t a_stride, w_stride, out_stride;
-  int32_t rows, width, n;
+  int64_t out_stride;
+  int32_t rows, n, chunks;
+  int32_t tokens;    // tokens of a tile (the MMA's N)
+  int32_t ch_tiles;  // tiles along the channels
+  int32_t units;     // tiles of the call
+  int32_t splits, stages, tmem_cols, weight_ready, vec_out;
+  int32_t* status;
 };
 
-// four codes of row `row` from column k on (zero past the row's end and past the last row)
-SD_DEV int load4(const int8_t* p, int64_t stride, int row, int rows, int k, int width) {
-  if (row >= rows || k >= width) return 0;
-  const int8_t* q = p + row * stride + k;
-  if (k + 4 <= width) return *reinterpret_cast<const int*>(q);
-  uint32_t v = 0;
-  for (int i = 0; k + i < width; ++i) v |= static_cast<uint32_t>(static_cast<uint8_t>(q[i])) << (8 * i);
-  return static_cast<int>(v);
+// ---------------------------------------------------------------- PTX of this kernel
+// instruction descriptor of kind::i8: signed x signed -> s32, both operands K-major
+SD_DEV uint32_t idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+template <int CG>
+SD_DEV void mma_i8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  const uint32_t acc = accumulate ? 1u : 0u;
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// arrive on `bar` (of both CTAs of a pair) when the MMAs issued so far are complete
+template <int CG>
+SD_DEV void commit_mma(uint64_t* bar) {
+  if constexpr (CG == 1)
+    umma::commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+template <int CG>
+SD_DEV void tmem_alloc_cg(uint32_t* result, uint32_t ncols) {
+  if constexpr (CG == 1) {
+    umma::tmem_alloc(result, ncols);
+    umma::tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(result)),
+                 "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+}
+template <int CG>
+SD_DEV void tmem_dealloc_cg(uint32_t taddr, uint32_t ncols) {
+  if constexpr (CG == 1)
+    umma::tmem_dealloc(taddr, ncols);
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// 2-D tile load; CG = 2: `bar` may be the barrier of the pair's other CTA
+template <int CG>
+SD_DEV void tma_codes(void* dst, const CUtensorMap* map, int32_t k, int32_t row, uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(k), "r"(row), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(k), "r"(row), "r"(bar)
+        : "memory");
+}
+// arrive on a barrier of another CTA of the cluster (or on one's own, by its cluster address)
+SD_DEV void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+SD_DEV void tmem_ld16_s32(uint32_t ta, int32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(ta));
+}
+// wait for this thread's TMEM loads; `v` may be used from here on
+SD_DEV void tmem_wait_ld16(int32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::"memory");
+}
+SD_DEV int4 dsmem_ld4_s32(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) linear_int8_kernel(const LinParams p) {
-  __shared__ int sa[64][17], sw[64][17];
-  const int r0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  const int tr = (threadIdx.x >> 4) * 4, tn = (threadIdx.x & 15) * 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < p.width; k0 += 64) {
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-      sa[i >> 4][i & 15] = load4(p.a, p.a_stride, r0 + (i >> 4), p.rows, k0 + (i & 15) * 4, p.width);
-      sw[i >> 4][i & 15] = load4(p.w, p.w_stride, n0 + (i >> 4), p.n, k0 + (i & 15) * 4, p.width);
-    }
-    __syncthreads();
+SD_DEV void store_out(T* p, float v) {
+  if constexpr (sizeof(T) == 4)
+    *p = v;
+  else
+    *p = __float2bfloat16_rn(v);
+}
+SD_DEV float scaled(int32_t acc, float sa, float sw, float b) {
+  return __fmaf_rn(__fmul_rn(static_cast<float>(acc), sa), sw, b);
+}
+
+// 16 tokens of one channel, from token c of the tile on: scaled, rounded, stored.  All scales are
+// read and all results formed before the first store, so nothing waits behind a store.
+template <typename T, bool GUARD>
+SD_DEV void store_tokens(const int32_t (&v)[16], const float* s_scale, float sw, float bias, T* o, int64_t stride,
+                         int ntok) {
+  float sa[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
+  for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(sa + i) = *reinterpret_cast<const float4*>(s_scale + i);
+  float y[16];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 16; ++i) y[i] = scaled(v[i], sa[i], sw, bias);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sa[tr + i][k], sw[tn + j][k], acc[i][j]);
-    __syncthreads();
+  for (int i = 0; i < 16; ++i) {
+    if (!GUARD || i < ntok) store_out(o, y[i]);
+    o += stride;
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int r = r0 + tr + i, n = n0 + tn + j;
-      if (r >= p.rows || n >= p.n) continue;
-      const float y = static_cast<float>(acc[i][j]) * p.a_scale[r] * p.w_scale[n] + (p.bias ? p.bias[n] : 0.f);
-      T* o = static_cast<T*>(p.out) + r * p.out_stride + n;
-      if constexpr (sizeof(T) == 4)
-        *o = y;
-      else
-        *o = __float2bfloat16_rn(y);
+}
+
+// ---------------------------------------------------------------- the kernel
+template <int CG, typename T>
+__global__ void __launch_bounds__(kLinThreads, 1)
+    linear_int8_kernel(const LinParams p, const __grid_constant__ CUtensorMap amap,
+                       const __grid_constant__ CUtensorMap wmap) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[kLinMaxStages], empty[kLinMaxStages], acc_full[2], acc_empty[2], fin_bar;
+  __shared__ uint32_t tmem_base;
+  __shared__ __align__(16) float s_scale[4][kLinMaxTokens];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int csize = CG == 2 ? 2 : p.splits;
+  const int rank = csize > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int unit0 = blockIdx.x / csize, unit_step = gridDim.x / csize;
+  if (tid == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4 * CG);
+    }
+    mbar_init(&fin_bar, 1);
+    fence_barrier_init();
+  }
+  if (warp == 4 && lane == 0) {
+    prefetch_tmap(&amap);
+    prefetch_tmap(&wmap);
+  }
+  if (warp == 5) tmem_alloc_cg<CG>(&tmem_base, p.tmem_cols);
+  umma::fence_before_sync();
+  if (CG == 2)
+    cluster_sync();  // the partner's barriers are signalled from here on
+  else
+    __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tbase = tmem_base;
+  const int a_rows = p.tokens / CG;  // rows of a this CTA loads
+  const int stage_bytes = kLinWTile + a_rows * kLinChunk;
+  // this CTA's share of the chunks of K
+  const int k_begin = CG == 2 ? 0 : static_cast<int>(static_cast<int64_t>(p.chunks) * rank / csize);
+  const int k_end = CG == 2 ? p.chunks : static_cast<int>(static_cast<int64_t>(p.chunks) * (rank + 1) / csize);
+
+  if (warp == 4) {
+    // ---- producer
+    int g = 0;
+    bool stop = false;
+    bool waited = false;
+    for (int u = unit0; u < p.units && !stop; u += unit_step) {
+      const int tt = u / p.ch_tiles, ct = u - tt * p.ch_tiles;
+      const int ch0 = (ct * CG + (CG == 2 ? rank : 0)) * kLinCh;
+      const int tok0 = tt * p.tokens + (CG == 2 ? rank * a_rows : 0);
+      int k = k_begin;
+      if (!waited) {
+        // the first stages' weights go out before the preceding kernel is over, if they may
+        const int ahead = min(p.stages, k_end - k_begin);
+        if (lane == 0) {
+          if (!p.weight_ready) grid_dep_wait();
+          for (int i = 0; i < ahead; ++i) {
+            const uint32_t bar = CG == 2 ? dsmem_addr(smem_u32(&full[i]), 0) : smem_u32(&full[i]);
+            if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[i], CG * stage_bytes);
+            tma_codes<CG>(smem + i * stage_bytes, &wmap, (k + i) * kLinChunk, ch0, bar);
+          }
+          if (p.weight_ready) grid_dep_wait();
+          grid_dep_launch();
+          for (int i = 0; i < ahead; ++i) {
+            const uint32_t bar = CG == 2 ? dsmem_addr(smem_u32(&full[i]), 0) : smem_u32(&full[i]);
+            tma_codes<CG>(smem + i * stage_bytes + kLinWTile, &amap, (k + i) * kLinChunk, tok0, bar);
+          }
+        }
+        __syncwarp();
+        k += ahead;
+        g = ahead;
+        waited = true;
+      }
+      for (; k < k_end; ++k, ++g) {
+        const int s = g % p.stages;
+        if (g >= p.stages && !warp_wait(&empty[s], ((g / p.stages) - 1) & 1)) {
+          if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+          stop = true;
+          break;
+        }
+        if (lane == 0) {
+          uint8_t* st = smem + s * stage_bytes;
+          const uint32_t bar = CG == 2 ? dsmem_addr(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
+          if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[s], CG * stage_bytes);
+          tma_codes<CG>(st, &wmap, k * kLinChunk, ch0, bar);
+          tma_codes<CG>(st + kLinWTile, &amap, k * kLinChunk, tok0, bar);
+        }
+        __syncwarp();
+      }
+    }
+    // every stage's last use is over before the CTA leaves (bounded)
+    for (int i = max(0, g - p.stages); i < g && !stop; ++i) stop = !warp_wait(&empty[i % p.stages], (i / p.stages) & 1);
+  } else if (warp == 5) {
+    // ---- MMA issuer
+    if (lane == 0 && rank % CG == 0) {
+      const uint32_t idesc = idesc_i8(kLinCh * CG, p.tokens);
+      int g = 0, ui = 0;
+      bool ok = true;
+      for (int u = unit0; u < p.units && ok; u += unit_step, ++ui) {
+        const int b = ui & 1;
+        // accumulator b is free once the epilogue has read unit ui - 2
+        if (ui >= 2 && !mbar_wait(&acc_empty[b], ((ui >> 1) - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        umma::fence_after_sync();
+        const uint32_t d = umma::taddr(tbase, 0, b * (p.tmem_cols / 2));
+        for (int k = k_begin; k < k_end; ++k, ++g) {
+          const int s = g % p.stages;
+          if (!mbar_wait(&full[s], (g / p.stages) & 1)) {
+            ok = false;
+            break;
+          }
+          umma::fence_after_sync();
+          const uint32_t wa = smem_u32(smem + s * stage_bytes), aa = wa + kLinWTile;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_i8_ss<CG>(d, umma::desc_kmajor_sw128(wa + kk * 32), umma::desc_kmajor_sw128(aa + kk * 32), idesc,
+                          k > k_begin || kk > 0);
+          commit_mma<CG>(&empty[s]);
+        }
+        if (!ok) break;
+        commit_mma<CG>(&acc_full[b]);
+      }
+      if (!ok) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      if constexpr (CG == 1) {
+        umma::commit(&fin_bar);
+        (void)mbar_wait(&fin_bar, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- epilogue: lane = channel, columns = tokens
+    grid_dep_wait();
+    T* out = static_cast<T*>(p.out);
+    int ui = 0;
+    for (int u = unit0; u < p.units; u += unit_step, ++ui) {
+      const int tt = u / p.ch_tiles, ct = u - tt * p.ch_tiles;
+      const int b = ui & 1;
+      const int n = (ct * CG + (CG == 2 ? rank : 0)) * kLinCh + warp * 32 + lane;
+      const int tok0 = tt * p.tokens, ntok = min(p.tokens, p.rows - tok0);
+      float sw = 0.f, bias = 0.f;
+      if (p.splits == 1) {
+        if (n < p.n) {
+          sw = p.w_scale[n];
+          if (p.bias) bias = p.bias[n];
+        }
+        __syncwarp();
+        for (int c = lane; c < ntok; c += 32) s_scale[warp][c] = p.a_scale[tok0 + c];
+        __syncwarp();
+      }
+      if (!warp_wait(&acc_full[b], (ui >> 1) & 1)) {
+        if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+        break;
+      }
+      umma::fence_after_sync();
+      const uint32_t ta = umma::taddr(tbase, warp * 32, b * (p.tmem_cols / 2));
+      if (p.splits == 1) {
+        T* o = out + tok0 * p.out_stride + n;
+        const bool whole = ntok == p.tokens && n - lane + 32 <= p.n;
+        const int mine = n < p.n ? ntok : 0;  // tokens this lane stores
+        // the next 16 columns are on their way while these are scaled and stored
+        int32_t v[2][16];
+        tmem_ld16_s32(ta, v[0]);
+#pragma unroll 1
+        for (int c = 0; c < p.tokens; c += 32) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int cc = c + 16 * h;
+            if (cc >= p.tokens) break;
+            tmem_wait_ld16(v[h]);
+            if (cc + 16 < p.tokens) tmem_ld16_s32(ta + cc + 16, v[1 - h]);
+            if (whole)
+              store_tokens<T, false>(v[h], &s_scale[warp][cc], sw, bias, o + cc * p.out_stride, p.out_stride, 16);
+            else
+              store_tokens<T, true>(v[h], &s_scale[warp][cc], sw, bias, o + cc * p.out_stride, p.out_stride, mine - cc);
+          }
+        }
+      } else {
+        // the partial sums take the ring's place: every product that read it is complete
+        int32_t* part = reinterpret_cast<int32_t*>(smem) + warp * 32 + lane;
+#pragma unroll 1
+        for (int c = 0; c < p.tokens; c += 16) {
+          int32_t v[16];
+          tmem_ld16_s32(ta + c, v);
+          tmem_wait_ld16(v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) part[(c + i) * kLinCh] = v[i];
+        }
+      }
+      umma::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2)
+          mbar_arrive_cluster(dsmem_addr(smem_u32(&acc_empty[b]), 0));
+        else
+          mbar_arrive(&acc_empty[b]);
+      }
+    }
+  }
+
+  umma::fence_before_sync();
+  __syncwarp();
+  if (csize > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  if (warp == 5) {
+    umma::fence_after_sync();
+    tmem_dealloc_cg<CG>(tbase, p.tmem_cols);
+  }
+  if (CG == 1 && csize > 1) {
+    // token columns are dealt over the cluster; a warp sums one token's 128 channels
+    grid_dep_wait();
+    const int tt = unit0 / p.ch_tiles, ct = unit0 - tt * p.ch_tiles;
+    const int n = ct * kLinCh + lane * 4;
+    const int tok0 = tt * p.tokens, ntok = min(p.tokens, p.rows - tok0);
+    float sw[4] = {}, bias[4] = {};
+    for (int j = 0; j < 4; ++j)
+      if (n + j < p.n) {
+        sw[j] = p.w_scale[n + j];
+        if (p.bias) bias[j] = p.bias[n + j];
+      }
+    const uint32_t mine = smem_u32(smem) + lane * 16;
+    for (int c = rank + csize * warp; c < ntok; c += csize * (kLinThreads / 32)) {
+      const float sa = p.a_scale[tok0 + c];
+      int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 8
+      for (int r = 0; r < csize; ++r) {
+        const int4 v = dsmem_ld4_s32(dsmem_addr(mine + c * (kLinCh * 4), r));
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      }
+      const float y[4] = {scaled(sum.x, sa, sw[0], bias[0]), scaled(sum.y, sa, sw[1], bias[1]),
+                          scaled(sum.z, sa, sw[2], bias[2]), scaled(sum.w, sa, sw[3], bias[3])};
+      T* o = static_cast<T*>(p.out) + (tok0 + c) * p.out_stride + n;
+      if (p.vec_out && n + 4 <= p.n) {
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
+        else
+          *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+      } else {
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.n) store_out(o + j, y[j]);
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // the peers have read this CTA's shared memory
+  }
+}
+
+// ---------------------------------------------------------------- host
+static int encode_codes(CUtensorMap* map, const void* base, int64_t width, int64_t rows, int64_t stride, int box_rows) {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  if (fn == nullptr) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) != cudaSuccess ||
+        qres != cudaDriverEntryPointSuccess)
+      return fail(SPECDEC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
+  const cuuint32_t box[2] = {kLinChunk, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SPECDEC_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return SPECDEC_OK;
+}
+
+struct LinShape {
+  int cg, tokens, splits;
+};
+
+// Launch shape by an estimate of the clocks a call takes: waves of tiles over the SMs, each tile
+// its chunks of K times the larger of the products' time (128 x 128 x 32 per 64 clocks and SM)
+// and the loads' (64 bytes per clock and SM), plus what starting and ending a tile costs.
+static LinShape pick_shape(int rows, int n, int chunks, int sms) {
+  LinShape best = {1, 16, 1};
+  double best_cost = 1e30;
+  const int ch1 = (n + kLinCh - 1) / kLinCh, ch2 = (n + 2 * kLinCh - 1) / (2 * kLinCh);
+  for (int tokens = 16; tokens <= kLinMaxTokens; tokens += 16) {
+    const int tt = (rows + tokens - 1) / tokens;
+    for (int splits = 1; splits <= 8; splits *= 2) {
+      if (splits > 1 && (chunks < 2 * splits || ch1 * tt * splits > sms)) break;
+      const int waves = (ch1 * tt * splits + sms - 1) / sms;
+      const double tile = ((chunks + splits - 1) / splits) * 2.0 * (kLinCh + tokens) + 800.0;
+      const double cost = waves * tile + (splits > 1 ? 1500.0 + 8.0 * tokens : 4.0 * tokens);
+      if (cost < best_cost) best_cost = cost, best = {1, tokens, splits};
+    }
+    if (tokens % 32 == 0) {
+      const int waves = (ch2 * tt + sms / 2 - 1) / (sms / 2);
+      const double tile = chunks * (tokens >= kLinMaxTokens ? 2.0 * tokens : 256.0 + tokens) + 800.0;
+      const double cost = waves * tile + 4.0 * tokens;
+      if (cost < best_cost) best_cost = cost, best = {2, tokens, 1};
+    }
+    if (tokens >= rows) break;
+  }
+  return best;
+}
+
+template <int CG, typename T>
+static int launch_linear(const LinParams& p, const CUtensorMap& amap, const CUtensorMap& wmap, int grid, int smem,
+                         cudaStream_t st) {
+  static bool attr_set[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (!attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(linear_int8_kernel<CG, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kLinRing + 1024);
+    if (e != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "linear_int8: %s", cudaGetErrorString(e));
+    attr_set[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kLinThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const int cluster = CG == 2 ? 2 : p.splits;
+  if (cluster > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_int8_kernel<CG, T>, p, amap, wmap);
+  if (e != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "linear_int8_kernel launch: %s", cudaGetErrorString(e));
+  return after_launch("linear_int8_kernel");
 }
 
 }  // namespace sd
@@ -76,8 +530,6 @@ extern "C" int specdec_linear_int8(const void* a, int64_t a_stride, const float*
                                    int64_t out_stride, int32_t out_dtype, int64_t rows, int32_t width,
                                    int32_t out_features, int32_t weight_ready, int32_t* status,
                                    specdec_stream_t stream) {
-  (void)weight_ready;
-  (void)status;
   if (rows < 0 || rows > kMaxRows) return fail(SPECDEC_ERR_INVALID, "linear_int8: row count out of range");
   if (width <= 0 || width > kMaxWidth)
     return fail(SPECDEC_ERR_INVALID, "linear_int8: width must be in 1 .. %d", kMaxWidth);
@@ -87,19 +539,51 @@ extern "C" int specdec_linear_int8(const void* a, int64_t a_stride, const float*
     return fail(SPECDEC_ERR_INVALID, "linear_int8 writes float32 or bfloat16");
   if (rows == 0) return SPECDEC_OK;
   if (!a || !a_scale || !w || !w_scale || !out) return fail(SPECDEC_ERR_INVALID, "linear_int8: tensors must be CUDA");
+  // the stride of a single row is of no account
+  if (rows == 1) a_stride = (width + 15) & ~15, out_stride = out_features;
+  if (out_features == 1) w_stride = (width + 15) & ~15;
   if (a_stride < width || w_stride < width || out_stride < out_features)
     return fail(SPECDEC_ERR_INVALID, "linear_int8: a row stride is smaller than its row");
   if ((a_stride | w_stride) & 15)
     return fail(SPECDEC_ERR_INVALID, "linear_int8: the row strides of the codes must be multiples of 16");
   if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w)) & 15u)
     return fail(SPECDEC_ERR_INVALID, "linear_int8: the codes must be 16-byte aligned");
-  LinParams p = {static_cast<const int8_t*>(a), static_cast<const int8_t*>(w), a_scale, w_scale, bias, out, a_stride,
-                 w_stride, out_stride, static_cast<int32_t>(rows), width, out_features};
-  const dim3 grid(static_cast<unsigned>((out_features + 63) / 64), static_cast<unsigned>((rows + 63) / 64));
+  const int sms = device_sm_count();
+  LinParams p = {};
+  p.a_scale = a_scale;
+  p.w_scale = w_scale;
+  p.bias = bias;
+  p.out = out;
+  p.out_stride = out_stride;
+  p.rows = static_cast<int32_t>(rows);
+  p.n = out_features;
+  p.chunks = (width + kLinChunk - 1) / kLinChunk;
+  const LinShape shape = pick_shape(p.rows, p.n, p.chunks, sms);
+  p.tokens = shape.tokens;
+  p.splits = shape.splits;
+  p.ch_tiles = (p.n + shape.cg * kLinCh - 1) / (shape.cg * kLinCh);
+  const int64_t units = static_cast<int64_t>(p.ch_tiles) * ((p.rows + p.tokens - 1) / p.tokens);
+  if (units > (1 << 30)) return fail(SPECDEC_ERR_INVALID, "linear_int8: too many outputs");
+  p.units = static_cast<int32_t>(units);
+  p.weight_ready = weight_ready;
+  p.status = status;
+  const int esize = out_dtype == SPECDEC_F32 ? 4 : 2;
+  p.vec_out = (reinterpret_cast<uintptr_t>(out) % (4 * esize)) == 0 && out_stride % 4 == 0;
+  const int stage = kLinWTile + p.tokens / shape.cg * kLinChunk;
+  p.stages = kLinRing / stage < kLinMaxStages ? kLinRing / stage : kLinMaxStages;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < 2 * p.tokens) p.tmem_cols *= 2;
+  CUtensorMap amap, wmap;
+  if (int rc = encode_codes(&amap, a, width, rows, a_stride, p.tokens / shape.cg)) return rc;
+  if (int rc = encode_codes(&wmap, w, width, out_features, w_stride, kLinCh)) return rc;
+  const int smem = p.stages * stage + 1024;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (out_dtype == SPECDEC_F32)
-    linear_int8_kernel<float><<<grid, 256, 0, st>>>(p);
-  else
-    linear_int8_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
-  return after_launch("linear_int8_kernel");
+  if (shape.cg == 2) {
+    const int grid = 2 * (p.units < sms / 2 ? p.units : sms / 2);
+    return out_dtype == SPECDEC_F32 ? launch_linear<2, float>(p, amap, wmap, grid, smem, st)
+                                    : launch_linear<2, __nv_bfloat16>(p, amap, wmap, grid, smem, st);
+  }
+  const int grid = p.splits > 1 ? p.units * p.splits : (p.units < sms ? p.units : sms);
+  return out_dtype == SPECDEC_F32 ? launch_linear<1, float>(p, amap, wmap, grid, smem, st)
+                                  : launch_linear<1, __nv_bfloat16>(p, amap, wmap, grid, smem, st);
 }
