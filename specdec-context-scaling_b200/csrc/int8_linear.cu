@@ -59,6 +59,16 @@ SD_DEV uint32_t idesc_i8(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
          (static_cast<uint32_t>(M >> 4) << 24);
 }
+// One lane of a converged warp.  The loops around it stay warp-uniform, so descriptors, barriers and
+// loop counters live in uniform registers (the tcgen05 operands): a loop inside `if (lane == 0)`
+// moved every operand there first and took 590 clocks a chunk instead of
+SD_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
 template <int CG>
 SD_DEV void mma_i8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
   const uint32_t acc = accumulate ? 1u : 0u;
@@ -184,7 +194,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                        const __grid_constant__ CUtensorMap wmap) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kLinMaxStages], empty[kLinMaxStages], acc_full[2], acc_empty[2], fin_bar;
+  __shared__ uint64_t full[kLinMaxStages], empty[kLinMaxStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
   __shared__ __align__(16) float s_scale[4][kLinMaxTokens];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -200,7 +210,6 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 4 * CG);
     }
-    mbar_init(&fin_bar, 1);
     fence_barrier_init();
   }
   if (warp == 4 && lane == 0) {
@@ -223,7 +232,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 
   if (warp == 4) {
     // ---- producer
-    int g = 0;
+    int s = 0;              // next stage to fill, and the parity of its last use's end
+    uint32_t parity = 1;    // (a fresh barrier reads as "phase 1 is over")
     bool stop = false;
     bool waited = false;
     for (int u = unit0; u < p.units && !stop; u += unit_step) {
@@ -234,7 +244,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       if (!waited) {
         // the first stages' weights go out before the preceding kernel is over, if they may
         const int ahead = min(p.stages, k_end - k_begin);
-        if (lane == 0) {
+        if (elect_one()) {
           if (!p.weight_ready) grid_dep_wait();
           for (int i = 0; i < ahead; ++i) {
             const uint32_t bar = CG == 2 ? dsmem_addr(smem_u32(&full[i]), 0) : smem_u32(&full[i]);
@@ -250,17 +260,17 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         }
         __syncwarp();
         k += ahead;
-        g = ahead;
+        s = ahead;
+        if (s == p.stages) s = 0, parity = 0;
         waited = true;
       }
-      for (; k < k_end; ++k, ++g) {
-        const int s = g % p.stages;
-        if (g >= p.stages && !warp_wait(&empty[s], ((g / p.stages) - 1) & 1)) {
+      for (; k < k_end; ++k) {
+        if (!warp_wait(&empty[s], parity)) {
           if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
           stop = true;
           break;
         }
-        if (lane == 0) {
+        if (elect_one()) {
           uint8_t* st = smem + s * stage_bytes;
           const uint32_t bar = CG == 2 ? dsmem_addr(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
           if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[s], CG * stage_bytes);
@@ -268,49 +278,58 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           tma_codes<CG>(st + kLinWTile, &amap, k * kLinChunk, tok0, bar);
         }
         __syncwarp();
+        if (++s == p.stages) s = 0, parity ^= 1;
       }
     }
-    // every stage's last use is over before the CTA leaves (bounded)
-    for (int i = max(0, g - p.stages); i < g && !stop; ++i) stop = !warp_wait(&empty[i % p.stages], (i / p.stages) & 1);
+    // every stage's last use is over before the CTA leaves (bounded; unused stages pass at once)
+    for (int i = 0; i < p.stages && !stop; ++i) {
+      stop = !warp_wait(&empty[s], parity);
+      if (++s == p.stages) s = 0, parity ^= 1;
+    }
   } else if (warp == 5) {
     // ---- MMA issuer
-    if (lane == 0 && rank % CG == 0) {
+    if (rank % CG == 0) {
       const uint32_t idesc = idesc_i8(kLinCh * CG, p.tokens);
-      int g = 0, ui = 0;
+      const uint32_t ring = smem_u32(smem);
+      int s = 0, ui = 0;
+      uint32_t parity = 0;
       bool ok = true;
+      bool ready = false;  // stage s was seen full already
       for (int u = unit0; u < p.units && ok; u += unit_step, ++ui) {
         const int b = ui & 1;
         // accumulator b is free once the epilogue has read unit ui - 2
-        if (ui >= 2 && !mbar_wait(&acc_empty[b], ((ui >> 1) - 1) & 1)) {
+        if (ui >= 2 && !warp_wait(&acc_empty[b], ((ui >> 1) - 1) & 1)) {
           ok = false;
           break;
         }
         umma::fence_after_sync();
         const uint32_t d = umma::taddr(tbase, 0, b * (p.tmem_cols / 2));
-        for (int k = k_begin; k < k_end; ++k, ++g) {
-          const int s = g % p.stages;
-          if (!mbar_wait(&full[s], (g / p.stages) & 1)) {
+        for (int k = k_begin; k < k_end; ++k) {
+          if (!__all_sync(0xffffffffu, ready) && !warp_wait(&full[s], parity)) {
             ok = false;
             break;
           }
           umma::fence_after_sync();
-          const uint32_t wa = smem_u32(smem + s * stage_bytes), aa = wa + kLinWTile;
+          // the next stage's barrier is read while this stage's products are issued
+          const int s1 = s + 1 == p.stages ? 0 : s + 1;
+          const uint32_t parity1 = s1 == 0 ? parity ^ 1 : parity;
+          ready = mbar_test(&full[s1], parity1);
+          // 32 codes further along K are 32 bytes, 2 in the descriptor's address field
+          const uint64_t wd = umma::desc_kmajor_sw128(ring + s * stage_bytes);
+          const uint64_t ad = umma::desc_kmajor_sw128(ring + s * stage_bytes + kLinWTile);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_i8_ss<CG>(d, umma::desc_kmajor_sw128(wa + kk * 32), umma::desc_kmajor_sw128(aa + kk * 32), idesc,
-                          k > k_begin || kk > 0);
-          commit_mma<CG>(&empty[s]);
+            for (int kk = 0; kk < 4; ++kk)
+              mma_i8_ss<CG>(d, wd + 2 * kk, ad + 2 * kk, idesc, k > k_begin || kk > 0);
+            commit_mma<CG>(&empty[s]);
+            if (k + 1 == k_end) commit_mma<CG>(&acc_full[b]);
+          }
+          s = s1;
+          parity = parity1;
         }
-        if (!ok) break;
-        commit_mma<CG>(&acc_full[b]);
       }
-      if (!ok) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-      if constexpr (CG == 1) {
-        umma::commit(&fin_bar);
-        (void)mbar_wait(&fin_bar, 0);
-      }
+      if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
     }
-    __syncwarp();
   } else {
     // ---- epilogue: lane = channel, columns = tokens
     grid_dep_wait();
