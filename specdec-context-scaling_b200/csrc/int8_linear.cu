@@ -8,14 +8,14 @@
 // output channel: a warp stores 32 neighbouring channels of one token at a time, whatever the
 // alignment of the output.
 //
-// linear_int8_kernel, 192 threads:
-//   warp 4    producer: TMA loads of the W tile [128 channels][128 codes] and the a tile
+// linear_int8_kernel, 320 threads:
+//   warp 8    producer: TMA loads of the W tile [128 channels][128 codes] and the a tile
 //             [tokens][128 codes] of each 128-code chunk of K (128-byte swizzle, K-major; the
 //             ragged ends of K, N and the rows are filled with zeros by the TMA unit) into a
 //             ring of 4 to 12 stages;
-//   warp 5    one lane issues tcgen05.mma kind::i8 (K 32) into one of two TMEM accumulators,
+//   warp 9    one lane issues tcgen05.mma kind::i8 (K 32) into one of two TMEM accumulators,
 //             so a tile's epilogue overlaps the next tile's products;
-//   warps 0-3 epilogue: lane = channel, columns = tokens.
+//   warps 0-7 epilogue: lane = channel, columns = tokens.
 // CG = 2: two CTAs on one 256-channel tile (cta_group::2).  Each loads its own 128 channels and
 // half of the tokens, so a chunk costs a CTA 128 + tokens / 2 rows of loads instead of
 // 128 + tokens; the pair's first CTA issues the products.
@@ -31,7 +31,8 @@ namespace sd {
 
 constexpr int kMaxWidth = 131072;
 constexpr int kMaxRows = 1 << 21;
-constexpr int kLinThreads = 192;
+constexpr int kLinEpiWarps = 8;
+constexpr int kLinThreads = 32 * (kLinEpiWarps + 2);
 constexpr int kLinChunk = 128;                   // codes of K per stage
 constexpr int kLinCh = 128;                      // channels per CTA
 constexpr int kLinWTile = kLinCh * kLinChunk;    // 16 KB
@@ -132,9 +133,11 @@ SD_DEV void tma_codes(void* dst, const CUtensorMap* map, int32_t k, int32_t row,
         "l"(reinterpret_cast<uint64_t>(map)), "r"(k), "r"(row), "r"(bar)
         : "memory");
 }
-// arrive on a barrier of another CTA of the cluster (or on one's own, by its cluster address)
+// Arrive on a barrier of another CTA of the cluster (or on one's own, by its cluster address).  It
+// hands back an accumulator whose reads are complete (tcgen05.wait::ld), no memory: a release at
+// cluster scope would first wait for all of the warp's output stores.
 SD_DEV void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 SD_DEV void tmem_ld16_s32(uint32_t ta, int32_t (&v)[16]) {
   asm volatile(
@@ -196,7 +199,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kLinMaxStages], empty[kLinMaxStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
-  __shared__ __align__(16) float s_scale[4][kLinMaxTokens];
+  __shared__ __align__(16) float s_scale[kLinEpiWarps][kLinMaxTokens / 2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int csize = CG == 2 ? 2 : p.splits;
   const int rank = csize > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -208,15 +211,15 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4 * CG);
+      mbar_init(&acc_empty[b], kLinEpiWarps * CG);
     }
     fence_barrier_init();
   }
-  if (warp == 4 && lane == 0) {
+  if (warp == kLinEpiWarps && lane == 0) {
     prefetch_tmap(&amap);
     prefetch_tmap(&wmap);
   }
-  if (warp == 5) tmem_alloc_cg<CG>(&tmem_base, p.tmem_cols);
+  if (warp == kLinEpiWarps + 1) tmem_alloc_cg<CG>(&tmem_base, p.tmem_cols);
   umma::fence_before_sync();
   if (CG == 2)
     cluster_sync();  // the partner's barriers are signalled from here on
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   const int k_begin = CG == 2 ? 0 : static_cast<int>(static_cast<int64_t>(p.chunks) * rank / csize);
   const int k_end = CG == 2 ? p.chunks : static_cast<int>(static_cast<int64_t>(p.chunks) * (rank + 1) / csize);
 
-  if (warp == 4) {
+  if (warp == kLinEpiWarps) {
     // ---- producer
     int s = 0;              // next stage to fill, and the parity of its last use's end
     uint32_t parity = 1;    // (a fresh barrier reads as "phase 1 is over")
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       stop = !warp_wait(&empty[s], parity);
       if (++s == p.stages) s = 0, parity ^= 1;
     }
-  } else if (warp == 5) {
+  } else if (warp == kLinEpiWarps + 1) {
     // ---- MMA issuer
     if (rank % CG == 0) {
       const uint32_t idesc = idesc_i8(kLinCh * CG, p.tokens);
@@ -331,14 +334,16 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
     }
   } else {
-    // ---- epilogue: lane = channel, columns = tokens
+    // ---- epilogue: lane = channel, columns = tokens; two warps share a lane quarter, each half the tokens
     grid_dep_wait();
     T* out = static_cast<T*>(p.out);
+    const int quarter = warp & 3, batches = p.tokens / 16;
+    const int c0 = (warp >> 2) * (batches / 2) * 16, c1 = warp >= 4 ? p.tokens : batches / 2 * 16;
     int ui = 0;
     for (int u = unit0; u < p.units; u += unit_step, ++ui) {
       const int tt = u / p.ch_tiles, ct = u - tt * p.ch_tiles;
       const int b = ui & 1;
-      const int n = (ct * CG + (CG == 2 ? rank : 0)) * kLinCh + warp * 32 + lane;
+      const int n = (ct * CG + (CG == 2 ? rank : 0)) * kLinCh + quarter * 32 + lane;
       const int tok0 = tt * p.tokens, ntok = min(p.tokens, p.rows - tok0);
       float sw = 0.f, bias = 0.f;
       if (p.splits == 1) {
@@ -347,7 +352,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           if (p.bias) bias = p.bias[n];
         }
         __syncwarp();
-        for (int c = lane; c < ntok; c += 32) s_scale[warp][c] = p.a_scale[tok0 + c];
+        for (int c = c0 + lane; c < min(c1, ntok); c += 32) s_scale[warp][c - c0] = p.a_scale[tok0 + c];
         __syncwarp();
       }
       if (!warp_wait(&acc_full[b], (ui >> 1) & 1)) {
@@ -355,33 +360,34 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         break;
       }
       umma::fence_after_sync();
-      const uint32_t ta = umma::taddr(tbase, warp * 32, b * (p.tmem_cols / 2));
+      const uint32_t ta = umma::taddr(tbase, quarter * 32, b * (p.tmem_cols / 2));
       if (p.splits == 1) {
-        T* o = out + tok0 * p.out_stride + n;
-        const bool whole = ntok == p.tokens && n - lane + 32 <= p.n;
+        T* o = out + (tok0 + c0) * p.out_stride + n;
+        const bool whole = c1 <= ntok && n - lane + 32 <= p.n;
         const int mine = n < p.n ? ntok : 0;  // tokens this lane stores
         // the next 16 columns are on their way while these are scaled and stored
         int32_t v[2][16];
-        tmem_ld16_s32(ta, v[0]);
+        if (c0 < c1) tmem_ld16_s32(ta + c0, v[0]);
 #pragma unroll 1
-        for (int c = 0; c < p.tokens; c += 32) {
+        for (int c = c0; c < c1; c += 32) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int cc = c + 16 * h;
-            if (cc >= p.tokens) break;
+            if (cc >= c1) break;
             tmem_wait_ld16(v[h]);
-            if (cc + 16 < p.tokens) tmem_ld16_s32(ta + cc + 16, v[1 - h]);
+            if (cc + 16 < c1) tmem_ld16_s32(ta + cc + 16, v[1 - h]);
+            T* oc = o + (cc - c0) * p.out_stride;
             if (whole)
-              store_tokens<T, false>(v[h], &s_scale[warp][cc], sw, bias, o + cc * p.out_stride, p.out_stride, 16);
+              store_tokens<T, false>(v[h], &s_scale[warp][cc - c0], sw, bias, oc, p.out_stride, 16);
             else
-              store_tokens<T, true>(v[h], &s_scale[warp][cc], sw, bias, o + cc * p.out_stride, p.out_stride, mine - cc);
+              store_tokens<T, true>(v[h], &s_scale[warp][cc - c0], sw, bias, oc, p.out_stride, mine - cc);
           }
         }
       } else {
         // the partial sums take the ring's place: every product that read it is complete
-        int32_t* part = reinterpret_cast<int32_t*>(smem) + warp * 32 + lane;
+        int32_t* part = reinterpret_cast<int32_t*>(smem) + quarter * 32 + lane;
 #pragma unroll 1
-        for (int c = 0; c < p.tokens; c += 16) {
+        for (int c = c0; c < c1; c += 16) {
           int32_t v[16];
           tmem_ld16_s32(ta + c, v);
           tmem_wait_ld16(v);
@@ -406,7 +412,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     cluster_sync();
   else
     __syncthreads();
-  if (warp == 5) {
+  if (warp == kLinEpiWarps + 1) {
     umma::fence_after_sync();
     tmem_dealloc_cg<CG>(tbase, p.tmem_cols);
   }
