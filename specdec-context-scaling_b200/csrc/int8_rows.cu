@@ -17,6 +17,7 @@
 namespace sd {
 
 constexpr float kInt8Max = 127.f;
+constexpr int kInt8MaxRow = 1 << 24;
 constexpr float kInt8Floor = 7.888609052210118e-31f;  // 2^-100
 
 template <typename T>
@@ -58,87 +59,239 @@ struct RowArgs {
   int32_t width;
 };
 
-// rint(y) for |y| < 2^22 in the low byte of the sum with 1.5 * 2^23
-SD_DEV int8_t code_of(float v, float inv) {
-  return static_cast<int8_t>(__float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.f)) & 0xFFu);
+// rint(y) for |y| < 2^22 in the low byte of the sum with 1.5 * 2^23 (a product and a sum, each
+// rounded: the codes are those of the formula in IEEE fp32)
+SD_DEV uint32_t code_of(float v, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.f)); }
+
+// silu with the hardware exponential and division: within 2^-20 of the exact value for |g| < 16,
+// under the fp32 rounding of the codes' quotients; 0 where exp(-g) overflows
+SD_DEV float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+
+// N consecutive values (N = 1, or 16 bytes of them), widened to fp32
+template <typename T, int N>
+SD_DEV void load_values(const T* p, float (&v)[N]) {
+  if constexpr (N == 1) {
+    v[0] = widen<T>(*p);
+  } else {
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = widen<T>(e[k]);
+  }
+}
+template <typename T, int N>
+SD_DEV void store_values(T* p, const float (&v)[N]) {
+  if constexpr (N == 1) {
+    *p = narrow<T>(v[0]);
+  } else {
+    uint4 raw;
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int k = 0; k < N; ++k) e[k] = narrow<T>(v[k]);
+    *reinterpret_cast<uint4*>(p) = raw;
+  }
+}
+SD_DEV uint32_t pack_codes(const float* v, float inv) {
+  const uint32_t lo = __byte_perm(code_of(v[0], inv), code_of(v[1], inv), 0x0040);
+  const uint32_t hi = __byte_perm(code_of(v[2], inv), code_of(v[3], inv), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+template <int N>
+SD_DEV void store_codes(int8_t* p, const float (&v)[N], float inv) {
+  if constexpr (N == 1)
+    *p = static_cast<int8_t>(code_of(v[0], inv) & 0xFFu);
+  else if constexpr (N == 4)
+    *reinterpret_cast<uint32_t*>(p) = pack_codes(v, inv);
+  else
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_codes(v, inv), pack_codes(v + 4, inv));
 }
 
-// Block-wide reductions (sum; maximum that keeps a NaN), the result in every thread.
-template <bool SUM>
-SD_DEV float block_reduce(float v, float* part) {
+// Reductions over the G threads of a row (sum; maximum that keeps a NaN), the result in every
+// thread.  `part`: one word per warp, used by one reduction only (G > 32: a row per block).
+template <int G, bool SUM>
+SD_DEV float row_reduce(float v, float* part) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float w = __shfl_xor_sync(0xffffffffu, v, o);
     v = SUM ? v + w : amax_nan(v, w);
   }
-  __syncthreads();  // the previous use of `part` is over
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = part[0];
-  for (int k = 1; k < (blockDim.x >> 5); ++k) v = SUM ? v + part[k] : amax_nan(v, part[k]);
-  return v;
-}
-
-template <typename T, int OP>
-SD_DEV float row_value(const RowArgs& a, int64_t row, int i) {
-  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-  const float v = widen<T>(x[i]);
-  if (OP == kRowSwiglu) return v / (1.f + expf(-v)) * widen<T>(x[a.width + i]);
-  if (OP == kRowNorm && a.residual)
-    return v + widen<T>(static_cast<const T*>(a.residual)[row * a.r_stride + i]);
-  return v;
-}
-
-template <typename T, int OP>
-__global__ void __launch_bounds__(256) int8_rows_kernel(const RowArgs a) {
-  __shared__ float part[8];
-  const int64_t row = blockIdx.x;
-  float inv_rms = 1.f;
-  const T* w = static_cast<const T*>(a.weight);
-  if (OP == kRowNorm) {
-    float ss = 0.f;
-    for (int i = threadIdx.x; i < a.width; i += blockDim.x) {
-      const float v = row_value<T, OP>(a, row, i);
-      ss += v * v;
+  if constexpr (G > 32) {
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = part[threadIdx.x & (G / 32 - 1)];
+#pragma unroll
+    for (int o = G / 64; o > 0; o >>= 1) {
+      const float w = __shfl_xor_sync(0xffffffffu, v, o);
+      v = SUM ? v + w : amax_nan(v, w);
     }
-    ss = block_reduce<true>(ss, part);
-    inv_rms = __fdiv_rn(1.f, __fsqrt_rn(ss / static_cast<float>(a.width) + a.eps));
+  }
+  return v;
+}
+
+// N values of row `row` from column i on: what is quantised, before the norm's factors
+template <typename T, int OP, int N>
+SD_DEV void row_values(const RowArgs& a, int64_t row, int i, float (&v)[N]) {
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride + i;
+  load_values<T, N>(x, v);
+  if constexpr (OP == kRowSwiglu) {
+    float u[N];
+    load_values<T, N>(x + a.width, u);
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = silu_mul(v[k], u[k]);
+  }
+  if constexpr (OP == kRowNorm)
+    if (a.residual) {
+      float r[N];
+      load_values<T, N>(static_cast<const T*>(a.residual) + row * a.r_stride + i, r);
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] += r[k];
+    }
+}
+SD_DEV float inv_rms_of(const RowArgs& a, float ss) {
+  return __fdiv_rn(1.f, __fsqrt_rn(ss / static_cast<float>(a.width) + a.eps));
+}
+struct RowScale {
+  float inv, scale;  // inv = 0 and scale NaN for a row that is not finite
+};
+SD_DEV RowScale row_scale(float m) {
+  if (!(m <= 3.4028234663852886e38f)) return {0.f, __int_as_float(0x7FC00000)};
+  m = fmaxf(m, kInt8Floor);
+  return {__fdiv_rn(kInt8Max, m), __fdiv_rn(m, kInt8Max)};
+}
+
+// G threads a row (32: eight rows a block, no block-wide step; else a row per block), each with up
+// to CH pieces of N values held in registers as fp32 between the passes: a row is read once, and
+// the only waits are the reductions (two for the norm, one else).
+template <typename T, int OP, int G, int N, int CH>
+__global__ void __launch_bounds__(G == 32 ? 256 : G) int8_rows_kernel(const RowArgs a) {
+  __shared__ float part[2][G == 32 ? 1 : G / 32];
+  const int t = threadIdx.x & (G - 1);
+  const int64_t row = G == 32 ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  grid_dep_wait();  // launched programmatically: x is the preceding work's output
+  grid_dep_launch();
+  if (G == 32 && row >= a.rows) return;
+  float v[CH][N];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = (t + G * c) * N;
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[c][k] = 0.f;
+    if (i < a.width) row_values<T, OP, N>(a, row, i, v[c]);
   }
   float m = 0.f;
-  for (int i = threadIdx.x; i < a.width; i += blockDim.x) {
-    float v = row_value<T, OP>(a, row, i);
-    if (OP == kRowNorm) v = v * inv_rms * widen<T>(w[i]);
-    m = amax_nan(m, fabsf(v));
-  }
-  m = block_reduce<false>(m, part);
-  const bool finite = m <= 3.4028234663852886e38f;  // false for NaN, too
-  m = fmaxf(m, kInt8Floor);
-  const float inv = __fdiv_rn(kInt8Max, m);
-  for (int i = threadIdx.x; i < a.width; i += blockDim.x) {
-    float v = row_value<T, OP>(a, row, i);
-    if (OP == kRowNorm) {
-      if (a.summed) static_cast<T*>(a.summed)[row * a.s_stride + i] = narrow<T>(v);
-      v = v * inv_rms * widen<T>(w[i]);
+  if constexpr (OP == kRowNorm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int k = 0; k < N; ++k) ss += v[c][k] * v[c][k];
+    const float inv_rms = inv_rms_of(a, row_reduce<G, true>(ss, part[0]));
+    T* summed = static_cast<T*>(a.summed);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = (t + G * c) * N;
+      if (i < a.width) {
+        if (summed) store_values<T, N>(summed + row * a.s_stride + i, v[c]);
+        float w[N];
+        load_values<T, N>(static_cast<const T*>(a.weight) + i, w);
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[c][k] = v[c][k] * inv_rms * w[k];
+      }
     }
-    a.codes[row * a.c_stride + i] = finite ? code_of(v, inv) : int8_t(0);
   }
-  if (threadIdx.x == 0) a.scale[row] = finite ? __fdiv_rn(m, kInt8Max) : __int_as_float(0x7FC00000);
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int k = 0; k < N; ++k) m = amax_nan(m, fabsf(v[c][k]));
+  const RowScale s = row_scale(row_reduce<G, false>(m, part[1]));
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = (t + G * c) * N;
+    if (i < a.width) {
+      if (s.inv == 0.f)
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[c][k] = 0.f;
+      store_codes<N>(a.codes + row * a.c_stride + i, v[c], s.inv);
+    }
+  }
+  if (t == 0) a.scale[row] = s.scale;
 }
 
-template <typename T>
+// Rows too long for the registers of a block: read again in each pass.
+template <typename T, int OP>
+__global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowArgs a) {
+  __shared__ float part[2][32];
+  const int64_t row = blockIdx.x;
+  grid_dep_wait();
+  grid_dep_launch();
+  const T* w = static_cast<const T*>(a.weight);
+  float inv_rms = 1.f, m = 0.f, v[1];
+  if (OP == kRowNorm) {
+    float ss = 0.f;
+    for (int i = threadIdx.x; i < a.width; i += 1024) {
+      row_values<T, OP, 1>(a, row, i, v);
+      ss += v[0] * v[0];
+    }
+    inv_rms = inv_rms_of(a, row_reduce<1024, true>(ss, part[0]));
+  }
+  for (int i = threadIdx.x; i < a.width; i += 1024) {
+    row_values<T, OP, 1>(a, row, i, v);
+    if (OP == kRowNorm) v[0] = v[0] * inv_rms * widen<T>(w[i]);
+    m = amax_nan(m, fabsf(v[0]));
+  }
+  const RowScale s = row_scale(row_reduce<1024, false>(m, part[1]));
+  for (int i = threadIdx.x; i < a.width; i += 1024) {
+    row_values<T, OP, 1>(a, row, i, v);
+    if (OP == kRowNorm) {
+      if (a.summed) static_cast<T*>(a.summed)[row * a.s_stride + i] = narrow<T>(v[0]);
+      v[0] = v[0] * inv_rms * widen<T>(w[i]);
+    }
+    if (s.inv == 0.f) v[0] = 0.f;
+    store_codes<1>(a.codes + row * a.c_stride + i, v, s.inv);
+  }
+  if (threadIdx.x == 0) a.scale[row] = s.scale;
+}
+
+// code * scale: a warp per row and 1024 columns, 16 codes a lane and load where the rows allow it
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t* __restrict__ codes, int64_t c_stride,
                                                               const float* __restrict__ scale, T* __restrict__ out,
-                                                              int64_t o_stride, int width) {
-  const int64_t row = blockIdx.x;
+                                                              int64_t o_stride, int64_t rows, int width) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  grid_dep_wait();
+  grid_dep_launch();
+  if (row >= rows) return;
   const float s = scale[row];
-  for (int i = threadIdx.x; i < width; i += blockDim.x)
-    out[row * o_stride + i] = narrow<T>(static_cast<float>(codes[row * c_stride + i]) * s);
+  const int8_t* c = codes + row * c_stride;
+  T* o = out + row * o_stride;
+  const int begin = blockIdx.y * 1024, end = min(width, begin + 1024);
+  if constexpr (VEC) {
+    constexpr int kOut = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = begin + (j * 32 + lane) * 16;
+      if (i >= end) break;
+      const uint4 raw = *reinterpret_cast<const uint4*>(c + i);
+      const int8_t* e = reinterpret_cast<const int8_t*>(&raw);
+#pragma unroll
+      for (int k = 0; k < 16; k += kOut) {
+        float v[kOut];
+#pragma unroll
+        for (int q = 0; q < kOut; ++q) v[q] = static_cast<float>(e[k + q]) * s;
+        store_values<T, kOut>(o + i + k, v);
+      }
+    }
+  } else {
+    for (int i = begin + lane; i < end; i += 32) o[i] = narrow<T>(static_cast<float>(c[i]) * s);
+  }
 }
 
 static int check_rows(const char* what, const void* x, int64_t x_stride, int64_t need, const void* codes,
                       int64_t c_stride, const void* scale, int32_t dtype, int64_t rows, int32_t width) {
   if (rows < 0 || rows > 0x7fffffff) return fail(SPECDEC_ERR_INVALID, "%s: row count out of range", what);
   if (width <= 0) return fail(SPECDEC_ERR_INVALID, "%s: empty row", what);
+  if (width > kInt8MaxRow) return fail(SPECDEC_ERR_INVALID, "%s: row longer than %d", what, kInt8MaxRow);
   if (dtype != SPECDEC_F32 && dtype != SPECDEC_BF16)
     return fail(SPECDEC_ERR_INVALID, "%s supports float32 and bfloat16", what);
   if (rows == 0) return SPECDEC_OK;
@@ -148,13 +301,59 @@ static int check_rows(const char* what, const void* x, int64_t x_stride, int64_t
   return SPECDEC_OK;
 }
 
+template <typename T, int OP, int G, int N, int CH>
+static int launch_rows_as(const char* what, const RowArgs& a, cudaStream_t st) {
+  const int64_t blocks = G == 32 ? (a.rows + 7) / 8 : a.rows;
+  return launch_pdl(what, int8_rows_kernel<T, OP, G, N, CH>, dim3(static_cast<unsigned>(blocks)),
+                    dim3(G == 32 ? 256 : G), 0, st, a);
+}
+
+// Threads a row: with at least eight rows an SM a warp takes a row as long as 8 pieces of 16 bytes a
+// lane hold it (no block-wide waits, the most loads in flight a thread); fewer rows are spread over a
+// block each, a piece a thread, which is the shortest chain from the first load to the last store.
+template <typename T, int OP>
+static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool many = a.rows >= 8 * device_sm_count();
+  uintptr_t bits = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.residual) |
+                   reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.summed);
+  bits |= static_cast<uintptr_t>(a.x_stride | a.r_stride | a.s_stride) * sizeof(T);
+  const bool vec = bits % 16 == 0 && a.width % V == 0 &&
+                   (reinterpret_cast<uintptr_t>(a.codes) | static_cast<uintptr_t>(a.c_stride)) % V == 0;
+  if (vec) {
+    const int need = a.width / V;
+    if (many && need <= 64) return launch_rows_as<T, OP, 32, V, 2>(what, a, st);
+    if (many && need <= 128) return launch_rows_as<T, OP, 32, V, 4>(what, a, st);
+    if (many && need <= 256) return launch_rows_as<T, OP, 32, V, 8>(what, a, st);
+    if (need <= 256) return launch_rows_as<T, OP, 256, V, 1>(what, a, st);
+    if (!many && need <= 1024) return launch_rows_as<T, OP, 1024, V, 1>(what, a, st);
+    if (many && need <= 1024) return launch_rows_as<T, OP, 256, V, 4>(what, a, st);
+    if (many && need <= 2048) return launch_rows_as<T, OP, 256, V, 8>(what, a, st);
+    if (need <= 4096) return launch_rows_as<T, OP, 1024, V, 4>(what, a, st);
+  } else {
+    if (many && a.width <= 256) return launch_rows_as<T, OP, 32, 1, 8>(what, a, st);
+    if (many && a.width <= 1024) return launch_rows_as<T, OP, 32, 1, 32>(what, a, st);
+    if (a.width <= 2048) return launch_rows_as<T, OP, 256, 1, 8>(what, a, st);
+    if (many && a.width <= 8192) return launch_rows_as<T, OP, 256, 1, 32>(what, a, st);
+    if (a.width <= 32768) return launch_rows_as<T, OP, 1024, 1, 32>(what, a, st);
+  }
+  return launch_pdl(what, int8_long_rows_kernel<T, OP>, dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st, a);
+}
 template <int OP>
 static int launch_rows(const char* what, const RowArgs& a, int32_t dtype, cudaStream_t st) {
-  if (dtype == SPECDEC_F32)
-    int8_rows_kernel<float, OP><<<static_cast<unsigned>(a.rows), 256, 0, st>>>(a);
-  else
-    int8_rows_kernel<__nv_bfloat16, OP><<<static_cast<unsigned>(a.rows), 256, 0, st>>>(a);
-  return after_launch(what);
+  return dtype == SPECDEC_F32 ? launch_rows_t<float, OP>(what, a, st) : launch_rows_t<__nv_bfloat16, OP>(what, a, st);
+}
+
+template <typename T>
+static int launch_dequantize(const int8_t* codes, int64_t c_stride, const float* scale, T* out, int64_t o_stride,
+                             int64_t rows, int32_t width, cudaStream_t st) {
+  const bool vec = (reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(out) |
+                    static_cast<uintptr_t>(c_stride) | static_cast<uintptr_t>(o_stride) * sizeof(T) |
+                    static_cast<uintptr_t>(width)) %
+                       16 == 0;
+  const dim3 grid(static_cast<unsigned>((rows + 7) / 8), static_cast<unsigned>((width + 1023) / 1024));
+  return launch_pdl("dequantize_int8", vec ? dequantize_int8_kernel<T, true> : dequantize_int8_kernel<T, false>, grid,
+                    dim3(256), 0, st, codes, c_stride, scale, out, o_stride, rows, width);
 }
 
 }  // namespace sd
@@ -230,12 +429,8 @@ extern "C" int specdec_dequantize_int8(const void* codes, int64_t codes_stride, 
     return rc;
   if (rows == 0) return SPECDEC_OK;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const unsigned grid = static_cast<unsigned>(rows);
-  if (dtype == SPECDEC_F32)
-    dequantize_int8_kernel<float><<<grid, 256, 0, st>>>(static_cast<const int8_t*>(codes), codes_stride, scale,
-                                                        static_cast<float*>(out), out_stride, width);
-  else
-    dequantize_int8_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const int8_t*>(codes), codes_stride, scale,
-                                                                static_cast<__nv_bfloat16*>(out), out_stride, width);
-  return after_launch("dequantize_int8");
+  const int8_t* c = static_cast<const int8_t*>(codes);
+  return dtype == SPECDEC_F32
+             ? launch_dequantize(c, codes_stride, scale, static_cast<float*>(out), out_stride, rows, width, st)
+             : launch_dequantize(c, codes_stride, scale, static_cast<__nv_bfloat16*>(out), out_stride, rows, width, st);
 }

@@ -22,6 +22,7 @@ def _quantize(lib, x=P, xs=64, c=P, cs=64, s=P, dtype=1, rows=4, width=64):
     (dict(rows=-1), "row count out of range"),
     (dict(rows=1 << 31), "row count out of range"),
     (dict(width=0), "empty row"),
+    (dict(width=(1 << 24) + 1, xs=1 << 25, cs=1 << 25), "row longer than"),
     (dict(dtype=2), "supports float32 and bfloat16"),
     (dict(x=None), "must be CUDA"),
     (dict(c=None), "must be CUDA"),
