@@ -41,7 +41,8 @@ SD_DEV __nv_bfloat16 narrow<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-enum RowOp { kRowQuantize = 0, kRowSwiglu = 1, kRowNorm = 2 };
+constexpr int kWarpRows = 4;
+enum RowOp { kRowQuantize = 0, kRowSwiglu = 1, kRowNorm = 2, kRowNormAdd = 3 };  // Add: with a residual
 
 struct RowArgs {
   const void* x;
@@ -63,33 +64,40 @@ struct RowArgs {
 // rounded: the codes are those of the formula in IEEE fp32)
 SD_DEV uint32_t code_of(float v, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.f)); }
 
-// silu with the hardware exponential and division: within 2^-20 of the exact value for |g| < 16,
-// under the fp32 rounding of the codes' quotients; 0 where exp(-g) overflows
-SD_DEV float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// max that returns NaN when an operand is one (fmaxf drops it)
+SD_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
-// N consecutive values (N = 1, or 16 bytes of them), widened to fp32
+// silu(g) * u with the hardware exponential and reciprocal: for |g| < 16 within 2^-19 of the exact
+// value, far under what decides a code; -0 where exp(-g) overflows
+SD_DEV float silu_mul(float g, float u) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(g * -1.4426950408889634f)));
+  return g * r * u;
+}
+
+// N consecutive values (N = 1, or 16 bytes of them) as they lie in memory
 template <typename T, int N>
-SD_DEV void load_values(const T* p, float (&v)[N]) {
-  if constexpr (N == 1) {
-    v[0] = widen<T>(*p);
-  } else {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = widen<T>(e[k]);
-  }
+struct Piece {
+  T e[N];
+};
+template <typename T>
+struct alignas(16) Piece<T, 16 / sizeof(T)> {
+  T e[16 / sizeof(T)];
+};
+template <typename T, int N>
+SD_DEV Piece<T, N> load_piece(const T* p) {
+  return *reinterpret_cast<const Piece<T, N>*>(p);
 }
 template <typename T, int N>
 SD_DEV void store_values(T* p, const float (&v)[N]) {
-  if constexpr (N == 1) {
-    *p = narrow<T>(v[0]);
-  } else {
-    uint4 raw;
-    T* e = reinterpret_cast<T*>(&raw);
+  Piece<T, N> raw;
 #pragma unroll
-    for (int k = 0; k < N; ++k) e[k] = narrow<T>(v[k]);
-    *reinterpret_cast<uint4*>(p) = raw;
-  }
+  for (int k = 0; k < N; ++k) raw.e[k] = narrow<T>(v[k]);
+  *reinterpret_cast<Piece<T, N>*>(p) = raw;
 }
 SD_DEV uint32_t pack_codes(const float* v, float inv) {
   const uint32_t lo = __byte_perm(code_of(v[0], inv), code_of(v[1], inv), 0x0040);
@@ -113,7 +121,7 @@ SD_DEV float row_reduce(float v, float* part) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = SUM ? v + w : amax_nan(v, w);
+    v = SUM ? v + w : max_nan(v, w);
   }
   if constexpr (G > 32) {
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
@@ -122,30 +130,27 @@ SD_DEV float row_reduce(float v, float* part) {
 #pragma unroll
     for (int o = G / 64; o > 0; o >>= 1) {
       const float w = __shfl_xor_sync(0xffffffffu, v, o);
-      v = SUM ? v + w : amax_nan(v, w);
+      v = SUM ? v + w : max_nan(v, w);
     }
   }
   return v;
 }
 
-// N values of row `row` from column i on: what is quantised, before the norm's factors
-template <typename T, int OP, int N>
-SD_DEV void row_values(const RowArgs& a, int64_t row, int i, float (&v)[N]) {
-  const T* x = static_cast<const T*>(a.x) + row * a.x_stride + i;
-  load_values<T, N>(x, v);
-  if constexpr (OP == kRowSwiglu) {
-    float u[N];
-    load_values<T, N>(x + a.width, u);
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = silu_mul(v[k], u[k]);
-  }
-  if constexpr (OP == kRowNorm)
-    if (a.residual) {
-      float r[N];
-      load_values<T, N>(static_cast<const T*>(a.residual) + row * a.r_stride + i, r);
-#pragma unroll
-      for (int k = 0; k < N; ++k) v[k] += r[k];
-    }
+// What is quantised, before the norm's factors, from the values x and (second half of a gate|up row,
+// or the residual) y
+template <int OP>
+SD_DEV float row_value(float x, float y) {
+  if (OP == kRowSwiglu) return silu_mul(x, y);
+  return OP == kRowNormAdd ? x + y : x;
+}
+template <int OP>
+constexpr bool kTwoInputs = OP == kRowSwiglu || OP == kRowNormAdd;
+template <int OP>
+constexpr bool kIsNorm = OP == kRowNorm || OP == kRowNormAdd;
+template <typename T, int OP>
+SD_DEV const T* second_row(const RowArgs& a, int64_t row) {
+  if (OP == kRowSwiglu) return static_cast<const T*>(a.x) + row * a.x_stride + a.width;
+  return static_cast<const T*>(a.residual) + row * a.r_stride;
 }
 SD_DEV float inv_rms_of(const RowArgs& a, float ss) {
   return __fdiv_rn(1.f, __fsqrt_rn(ss / static_cast<float>(a.width) + a.eps));
@@ -159,60 +164,68 @@ SD_DEV RowScale row_scale(float m) {
   return {__fdiv_rn(kInt8Max, m), __fdiv_rn(m, kInt8Max)};
 }
 
-// G threads a row (32: eight rows a block, no block-wide step; else a row per block), each with up
+// G threads a row (32: kWarpRows rows a block, no block-wide step; else a row per block), each with up
 // to CH pieces of N values held in registers as fp32 between the passes: a row is read once, and
 // the only waits are the reductions (two for the norm, one else).
 template <typename T, int OP, int G, int N, int CH>
-__global__ void __launch_bounds__(G == 32 ? 256 : G) int8_rows_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) int8_rows_kernel(const RowArgs a) {
   __shared__ float part[2][G == 32 ? 1 : G / 32];
   const int t = threadIdx.x & (G - 1);
-  const int64_t row = G == 32 ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t row = G == 32 ? static_cast<int64_t>(blockIdx.x) * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
   grid_dep_wait();  // launched programmatically: x is the preceding work's output
   grid_dep_launch();
   if (G == 32 && row >= a.rows) return;
-  float v[CH][N];
+  // every load of the row is under way before the first value is used
+  const T* xr = static_cast<const T*>(a.x) + row * a.x_stride;
+  const T* yr = second_row<T, OP>(a, row);
+  Piece<T, N> px[CH] = {}, py[CH] = {};
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int i = (t + G * c) * N;
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[c][k] = 0.f;
-    if (i < a.width) row_values<T, OP, N>(a, row, i, v[c]);
+    if (i < a.width) px[c] = load_piece<T, N>(xr + i);
+    if (kTwoInputs<OP> && i < a.width) py[c] = load_piece<T, N>(yr + i);
   }
+  float v[CH][N];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[c][k] = row_value<OP>(widen<T>(px[c].e[k]), widen<T>(py[c].e[k]));
   float m = 0.f;
-  if constexpr (OP == kRowNorm) {
+  if constexpr (kIsNorm<OP>) {
     float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int k = 0; k < N; ++k) ss += v[c][k] * v[c][k];
     const float inv_rms = inv_rms_of(a, row_reduce<G, true>(ss, part[0]));
-    T* summed = static_cast<T*>(a.summed);
+    const T* w = static_cast<const T*>(a.weight);
+    T* summed = static_cast<T*>(a.summed) + row * a.s_stride;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int i = (t + G * c) * N;
-      if (i < a.width) {
-        if (summed) store_values<T, N>(summed + row * a.s_stride + i, v[c]);
-        float w[N];
-        load_values<T, N>(static_cast<const T*>(a.weight) + i, w);
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[c][k] = v[c][k] * inv_rms * w[k];
-      }
+      if (i < a.width) px[c] = load_piece<T, N>(w + i);
+      if (OP == kRowNormAdd && i < a.width) store_values<T, N>(summed + i, v[c]);
     }
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[c][k] = v[c][k] * inv_rms * widen<T>(px[c].e[k]);
   }
 #pragma unroll
   for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int k = 0; k < N; ++k) m = amax_nan(m, fabsf(v[c][k]));
+    for (int k = 0; k < N; ++k) m = max_nan(m, fabsf(v[c][k]));
   const RowScale s = row_scale(row_reduce<G, false>(m, part[1]));
+  if (s.inv == 0.f) {  // the same for the whole row: its codes are 0, whatever it holds
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[c][k] = 0.f;
+  }
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int i = (t + G * c) * N;
-    if (i < a.width) {
-      if (s.inv == 0.f)
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[c][k] = 0.f;
-      store_codes<N>(a.codes + row * a.c_stride + i, v[c], s.inv);
-    }
+    if (i < a.width) store_codes<N>(a.codes + row * a.c_stride + i, v[c], s.inv);
   }
   if (t == 0) a.scale[row] = s.scale;
 }
@@ -224,28 +237,29 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowArgs a) {
   const int64_t row = blockIdx.x;
   grid_dep_wait();
   grid_dep_launch();
+  const T* xr = static_cast<const T*>(a.x) + row * a.x_stride;
+  const T* yr = second_row<T, OP>(a, row);
   const T* w = static_cast<const T*>(a.weight);
-  float inv_rms = 1.f, m = 0.f, v[1];
-  if (OP == kRowNorm) {
+  const auto value = [&](int i) { return row_value<OP>(widen<T>(xr[i]), kTwoInputs<OP> ? widen<T>(yr[i]) : 0.f); };
+  float inv_rms = 1.f, m = 0.f;
+  if (kIsNorm<OP>) {
     float ss = 0.f;
     for (int i = threadIdx.x; i < a.width; i += 1024) {
-      row_values<T, OP, 1>(a, row, i, v);
-      ss += v[0] * v[0];
+      const float v = value(i);
+      ss += v * v;
     }
     inv_rms = inv_rms_of(a, row_reduce<1024, true>(ss, part[0]));
   }
   for (int i = threadIdx.x; i < a.width; i += 1024) {
-    row_values<T, OP, 1>(a, row, i, v);
-    if (OP == kRowNorm) v[0] = v[0] * inv_rms * widen<T>(w[i]);
-    m = amax_nan(m, fabsf(v[0]));
+    float v = value(i);
+    if (kIsNorm<OP>) v = v * inv_rms * widen<T>(w[i]);
+    m = max_nan(m, fabsf(v));
   }
   const RowScale s = row_scale(row_reduce<1024, false>(m, part[1]));
   for (int i = threadIdx.x; i < a.width; i += 1024) {
-    row_values<T, OP, 1>(a, row, i, v);
-    if (OP == kRowNorm) {
-      if (a.summed) static_cast<T*>(a.summed)[row * a.s_stride + i] = narrow<T>(v[0]);
-      v[0] = v[0] * inv_rms * widen<T>(w[i]);
-    }
+    float v[1] = {value(i)};
+    if (OP == kRowNormAdd) static_cast<T*>(a.summed)[row * a.s_stride + i] = narrow<T>(v[0]);
+    if (kIsNorm<OP>) v[0] = v[0] * inv_rms * widen<T>(w[i]);
     if (s.inv == 0.f) v[0] = 0.f;
     store_codes<1>(a.codes + row * a.c_stride + i, v, s.inv);
   }
@@ -303,9 +317,9 @@ static int check_rows(const char* what, const void* x, int64_t x_stride, int64_t
 
 template <typename T, int OP, int G, int N, int CH>
 static int launch_rows_as(const char* what, const RowArgs& a, cudaStream_t st) {
-  const int64_t blocks = G == 32 ? (a.rows + 7) / 8 : a.rows;
+  const int64_t blocks = G == 32 ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows;
   return launch_pdl(what, int8_rows_kernel<T, OP, G, N, CH>, dim3(static_cast<unsigned>(blocks)),
-                    dim3(G == 32 ? 256 : G), 0, st, a);
+                    dim3(G == 32 ? 32 * kWarpRows : G), 0, st, a);
 }
 
 // Threads a row: with at least eight rows an SM a warp takes a row as long as 8 pieces of 16 bytes a
@@ -324,17 +338,25 @@ static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
     const int need = a.width / V;
     if (many && need <= 64) return launch_rows_as<T, OP, 32, V, 2>(what, a, st);
     if (many && need <= 128) return launch_rows_as<T, OP, 32, V, 4>(what, a, st);
+    if (many && need <= 192) return launch_rows_as<T, OP, 32, V, 6>(what, a, st);
     if (many && need <= 256) return launch_rows_as<T, OP, 32, V, 8>(what, a, st);
+    if (many && need <= 384 && V == 4) return launch_rows_as<T, OP, 32, V, 48 / V>(what, a, st);
     if (need <= 256) return launch_rows_as<T, OP, 256, V, 1>(what, a, st);
     if (!many && need <= 1024) return launch_rows_as<T, OP, 1024, V, 1>(what, a, st);
+    if (many && need <= 512) return launch_rows_as<T, OP, 128, V, 4>(what, a, st);
+    if (many && need <= 640) return launch_rows_as<T, OP, 128, V, 5>(what, a, st);
+    if (many && need <= 768) return launch_rows_as<T, OP, 256, V, 3>(what, a, st);
     if (many && need <= 1024) return launch_rows_as<T, OP, 256, V, 4>(what, a, st);
+    if (many && need <= 1280) return launch_rows_as<T, OP, 256, V, 5>(what, a, st);
     if (many && need <= 2048) return launch_rows_as<T, OP, 256, V, 8>(what, a, st);
+    if (need <= 2048) return launch_rows_as<T, OP, 1024, V, 2>(what, a, st);
     if (need <= 4096) return launch_rows_as<T, OP, 1024, V, 4>(what, a, st);
   } else {
     if (many && a.width <= 256) return launch_rows_as<T, OP, 32, 1, 8>(what, a, st);
-    if (many && a.width <= 1024) return launch_rows_as<T, OP, 32, 1, 32>(what, a, st);
+    if (many && a.width <= 512) return launch_rows_as<T, OP, 32, 1, 16>(what, a, st);
+    if (a.width <= 1024) return launch_rows_as<T, OP, 256, 1, 4>(what, a, st);
     if (a.width <= 2048) return launch_rows_as<T, OP, 256, 1, 8>(what, a, st);
-    if (many && a.width <= 8192) return launch_rows_as<T, OP, 256, 1, 32>(what, a, st);
+    if (a.width <= 8192) return launch_rows_as<T, OP, 1024, 1, 8>(what, a, st);
     if (a.width <= 32768) return launch_rows_as<T, OP, 1024, 1, 32>(what, a, st);
   }
   return launch_pdl(what, int8_long_rows_kernel<T, OP>, dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st, a);
@@ -419,7 +441,9 @@ extern "C" int specdec_rmsnorm_int8(const void* x, int64_t x_stride, const void*
   a.scale = scale;
   a.rows = rows;
   a.width = hidden;
-  return launch_rows<kRowNorm>("rmsnorm_int8", a, dtype, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return residual ? launch_rows<kRowNormAdd>("rmsnorm_int8", a, dtype, st)
+                  : launch_rows<kRowNorm>("rmsnorm_int8", a, dtype, st);
 }
 
 extern "C" int specdec_dequantize_int8(const void* codes, int64_t codes_stride, const float* scale, void* out,
