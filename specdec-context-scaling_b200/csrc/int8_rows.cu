@@ -114,14 +114,14 @@ SD_DEV void store_codes(int8_t* p, const float (&v)[N], float inv) {
     *reinterpret_cast<uint2*>(p) = make_uint2(pack_codes(v, inv), pack_codes(v + 4, inv));
 }
 
-// Reductions over the G threads of a row (sum; maximum that keeps a NaN), the result in every
-// thread.  `part`: one word per warp, used by one reduction only (G > 32: a row per block).
+// Sum of squares and largest magnitude of a row over the G threads that hold it, in every thread (the
+// maximum keeps a NaN).  `part`: a pair per warp, used once between two block-wide barriers.
 template <int G, bool SUM>
-SD_DEV float row_reduce(float v, float* part) {
+SD_DEV float2 row_reduce(float2 v, float2* part) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = SUM ? v + w : max_nan(v, w);
+    if (SUM) v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y = max_nan(v.y, __shfl_xor_sync(0xffffffffu, v.y, o));
   }
   if constexpr (G > 32) {
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
@@ -129,8 +129,8 @@ SD_DEV float row_reduce(float v, float* part) {
     v = part[threadIdx.x & (G / 32 - 1)];
 #pragma unroll
     for (int o = G / 64; o > 0; o >>= 1) {
-      const float w = __shfl_xor_sync(0xffffffffu, v, o);
-      v = SUM ? v + w : max_nan(v, w);
+      if (SUM) v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y = max_nan(v.y, __shfl_xor_sync(0xffffffffu, v.y, o));
     }
   }
   return v;
@@ -152,24 +152,36 @@ SD_DEV const T* second_row(const RowArgs& a, int64_t row) {
   if (OP == kRowSwiglu) return static_cast<const T*>(a.x) + row * a.x_stride + a.width;
   return static_cast<const T*>(a.residual) + row * a.r_stride;
 }
-SD_DEV float inv_rms_of(const RowArgs& a, float ss) {
-  return __fdiv_rn(1.f, __fsqrt_rn(ss / static_cast<float>(a.width) + a.eps));
-}
+// The norm's y = s * weight / rms is kept as z = s * weight until the one reduction of a row has given
+// both the sum of s^2 and the largest |z|; 1 / rms then joins the factors of the codes and the scale.
 struct RowScale {
-  float inv, scale;  // inv = 0 and scale NaN for a row that is not finite
+  float rms, inv, scale;  // code = rint(z * rms * inv); inv = 0 and scale NaN for a row that is not finite
 };
-SD_DEV RowScale row_scale(float m) {
-  if (!(m <= 3.4028234663852886e38f)) return {0.f, __int_as_float(0x7FC00000)};
-  m = fmaxf(m, kInt8Floor);
-  return {__fdiv_rn(kInt8Max, m), __fdiv_rn(m, kInt8Max)};
+template <int OP>
+SD_DEV RowScale row_scale(const RowArgs& a, float2 r) {
+  RowScale s;
+  s.rms = 1.f;
+  if (kIsNorm<OP>) {
+    s.rms = __fdiv_rn(1.f, __fsqrt_rn(r.x / static_cast<float>(a.width) + a.eps));
+    r.y *= s.rms;
+  }
+  if (!(r.y <= 3.4028234663852886e38f)) {
+    s.rms = s.inv = 0.f;
+    s.scale = __int_as_float(0x7FC00000);
+    return s;
+  }
+  const float m = fmaxf(r.y, kInt8Floor);
+  s.inv = __fdiv_rn(kInt8Max, m);
+  s.scale = __fdiv_rn(m, kInt8Max);
+  return s;
 }
 
 // G threads a row (32: kWarpRows rows a block, no block-wide step; else a row per block), each with up
-// to CH pieces of N values held in registers as fp32 between the passes: a row is read once, and
-// the only waits are the reductions (two for the norm, one else).
+// to CH pieces of N values held in registers as fp32 from the load to the store: a row is read once,
+// and the only wait is the reduction.
 template <typename T, int OP, int G, int N, int CH>
 __global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) int8_rows_kernel(const RowArgs a) {
-  __shared__ float part[2][G == 32 ? 1 : G / 32];
+  __shared__ float2 part[G == 32 ? 1 : G / 32];
   const int t = threadIdx.x & (G - 1);
   const int64_t row = G == 32 ? static_cast<int64_t>(blockIdx.x) * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
   grid_dep_wait();  // launched programmatically: x is the preceding work's output
@@ -178,6 +190,7 @@ __global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) int8_rows_kernel
   // every load of the row is under way before the first value is used
   const T* xr = static_cast<const T*>(a.x) + row * a.x_stride;
   const T* yr = second_row<T, OP>(a, row);
+  const T* w = static_cast<const T*>(a.weight);
   Piece<T, N> px[CH] = {}, py[CH] = {};
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
@@ -186,36 +199,26 @@ __global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) int8_rows_kernel
     if (kTwoInputs<OP> && i < a.width) py[c] = load_piece<T, N>(yr + i);
   }
   float v[CH][N];
+  float2 r = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+  for (int c = 0; c < CH; ++c) {
+    const int i = (t + G * c) * N;
 #pragma unroll
     for (int k = 0; k < N; ++k) v[c][k] = row_value<OP>(widen<T>(px[c].e[k]), widen<T>(py[c].e[k]));
-  float m = 0.f;
-  if constexpr (kIsNorm<OP>) {
-    float ss = 0.f;
+    if constexpr (kIsNorm<OP>) {
+      if (OP == kRowNormAdd && i < a.width)
+        store_values<T, N>(static_cast<T*>(a.summed) + row * a.s_stride + i, v[c]);
+      if (i < a.width) py[c] = load_piece<T, N>(w + i);
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int k = 0; k < N; ++k) ss += v[c][k] * v[c][k];
-    const float inv_rms = inv_rms_of(a, row_reduce<G, true>(ss, part[0]));
-    const T* w = static_cast<const T*>(a.weight);
-    T* summed = static_cast<T*>(a.summed) + row * a.s_stride;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int i = (t + G * c) * N;
-      if (i < a.width) px[c] = load_piece<T, N>(w + i);
-      if (OP == kRowNormAdd && i < a.width) store_values<T, N>(summed + i, v[c]);
+      for (int k = 0; k < N; ++k) {
+        r.x += v[c][k] * v[c][k];
+        v[c][k] *= widen<T>(py[c].e[k]);
+      }
     }
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int k = 0; k < N; ++k) v[c][k] = v[c][k] * inv_rms * widen<T>(px[c].e[k]);
+    for (int k = 0; k < N; ++k) r.y = max_nan(r.y, fabsf(v[c][k]));
   }
-#pragma unroll
-  for (int c = 0; c < CH; ++c)
-#pragma unroll
-    for (int k = 0; k < N; ++k) m = max_nan(m, fabsf(v[c][k]));
-  const RowScale s = row_scale(row_reduce<G, false>(m, part[1]));
+  const RowScale s = row_scale<OP>(a, row_reduce<G, kIsNorm<OP>>(r, part));
   if (s.inv == 0.f) {  // the same for the whole row: its codes are 0, whatever it holds
 #pragma unroll
     for (int c = 0; c < CH; ++c)
@@ -225,15 +228,195 @@ __global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) int8_rows_kernel
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int i = (t + G * c) * N;
+    if constexpr (kIsNorm<OP>)
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[c][k] *= s.rms;
     if (i < a.width) store_codes<N>(a.codes + row * a.c_stride + i, v[c], s.inv);
   }
   if (t == 0) a.scale[row] = s.scale;
 }
 
-// Rows too long for the registers of a block: read again in each pass.
+// Rows of any alignment, or too long for registers, through shared memory.  W warps work on a row (1:
+// eight independent warps a block, each with rings of its own; 8: the whole block), and the copies of
+// the next rows are always under way (cp.async.bulk into a ring of `slots` rows), so neither the
+// reduction nor the arithmetic leaves HBM idle.  A copy takes the 16-byte granules inside the row;
+// the up to 7 values at each end of an unaligned row are loaded by lanes one row ahead.  VEC: every
+// row and output is 16-byte aligned, values move in 16-byte pieces, and silu's results take their
+// inputs' place in the ring; else a lane takes every 32nd value.
+constexpr int kStreamThreads = 256;
+constexpr int kStreamSlots = 4;
+constexpr int kStreamSmem = 200 * 1024;
+template <typename T, int OP, int W, bool VEC>
+__global__ void __launch_bounds__(kStreamThreads) int8_stream_rows_kernel(const RowArgs a, int slots, int piece_bytes) {
+  constexpr int kGroups = 8 / W, kThreads = 32 * W, kStreams = kTwoInputs<OP> ? 2 : 1;
+  constexpr int kN = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ uint64_t full[kGroups][kStreamSlots];
+  __shared__ float2 part[2][W];
+  __shared__ int late;  // W = 8: a thread's wait gave up
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = W == 1 ? warp : 0, t = W == 1 ? lane : threadIdx.x;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+  uint8_t* mine = ring + group * slots * kStreams * piece_bytes;
+  if (t == 0) {
+    for (int s = 0; s < slots; ++s) mbar_init(&full[group][s], 1);
+    fence_barrier_init();
+    if (W > 1) late = 0;
+  }
+  __syncthreads();
+  grid_dep_wait();
+  grid_dep_launch();
+
+  const T* streams[2] = {static_cast<const T*>(a.x), nullptr};
+  const int64_t strides[2] = {a.x_stride, OP == kRowSwiglu ? a.x_stride : a.r_stride};
+  if (kTwoInputs<OP>) streams[1] = second_row<T, OP>(a, 0);
+  const auto row_ptr = [&](int k, int64_t row) { return reinterpret_cast<uintptr_t>(streams[k] + row * strides[k]); };
+  const auto slot_ptr = [&](int k, int slot) { return mine + (slot * kStreams + k) * piece_bytes; };
+  // the granules inside row `row`, by one thread
+  const auto copy_row = [&](int64_t row, int slot) {
+    uint32_t bytes[2] = {0, 0};
+    for (int k = 0; k < kStreams; ++k) {
+      const uintptr_t p = row_ptr(k, row), lo = (p + 15) & ~uintptr_t(15);
+      const uintptr_t hi = (p + static_cast<uintptr_t>(a.width) * sizeof(T)) & ~uintptr_t(15);
+      if (hi > lo) bytes[k] = static_cast<uint32_t>(hi - lo);
+    }
+    fence_proxy_async();  // the slot's last use was by ordinary loads and stores
+    mbar_arrive_expect_tx(&full[group][slot], bytes[0] + bytes[1]);
+    for (int k = 0; k < kStreams; ++k) {
+      const uintptr_t p = row_ptr(k, row), lo = (p + 15) & ~uintptr_t(15);
+      if (bytes[k])
+        bulk_g2s(slot_ptr(k, slot) + (lo - (p & ~uintptr_t(15))), reinterpret_cast<const void*>(lo), bytes[k],
+                 &full[group][slot]);
+    }
+  };
+  // the values of `row` outside its granules, one a lane (16 lanes a stream): index, or -1
+  const auto end_index = [&](int64_t row) {
+    const int k = lane >> 4, l = lane & 15;
+    if (k >= kStreams) return -1;
+    const uintptr_t p = row_ptr(k, row), lo = (p + 15) & ~uintptr_t(15);
+    const uintptr_t end = p + static_cast<uintptr_t>(a.width) * sizeof(T), hi = end & ~uintptr_t(15);
+    const int head = min(a.width, static_cast<int>((lo - p) / sizeof(T)));
+    const int tail = hi >= lo ? static_cast<int>((end - hi) / sizeof(T)) : 0;
+    return l < head ? l : l < head + tail ? a.width - tail + (l - head) : -1;
+  };
+  const auto load_end = [&](int64_t row, int at) { return at < 0 ? T(0.f) : reinterpret_cast<const T*>(row_ptr(lane >> 4, row))[at]; };
+  const auto store_end = [&](int64_t row, int slot, int at, T v) {
+    const int k = lane >> 4;
+    if (at >= 0) reinterpret_cast<T*>(slot_ptr(k, slot) + (row_ptr(k, row) & 15))[at] = v;
+  };
+
+  if (t == 0)
+    for (int s = 0; s < slots - (W > 1); ++s)
+      if (row0 + s * step < a.rows) copy_row(row0 + s * step, s);
+  const bool ends = !VEC && (W == 1 || warp == 0);
+  if (ends && row0 < a.rows) {
+    const int at = end_index(row0);
+    store_end(row0, 0, at, load_end(row0, at));
+  }
+  if (W > 1)
+    __syncthreads();
+  else
+    __syncwarp();
+
+  int slot = 0;
+  uint32_t parity = 0, odd = 0;
+  for (int64_t row = row0; row < a.rows; row += step, odd ^= 1) {
+    const int next_slot = slot + 1 == slots ? 0 : slot + 1;
+    // the next row's ends are on their way while this row is worked on
+    int at = -1;
+    T end_value = T(0.f);
+    if (ends && row + step < a.rows) {
+      at = end_index(row + step);
+      end_value = load_end(row + step, at);
+    }
+    bool ok = mbar_wait(&full[group][slot], parity);
+    if (W == 1)
+      ok = __all_sync(0xffffffffu, ok);
+    else if (!ok)
+      late = 1;
+    const T* x = reinterpret_cast<const T*>(slot_ptr(0, slot) + (row_ptr(0, row) & 15));
+    const T* y = kStreams == 2 ? reinterpret_cast<const T*>(slot_ptr(1, slot) + (row_ptr(1, row) & 15)) : x;
+    const T* w = static_cast<const T*>(a.weight);
+    float2 r = make_float2(0.f, 0.f);
+    const auto values = [&](int i, float (&v)[kN]) {
+      const Piece<T, kN> px = load_piece<T, kN>(x + i), py = load_piece<T, kN>(y + i);
+#pragma unroll
+      for (int k = 0; k < kN; ++k) v[k] = row_value<OP>(widen<T>(px.e[k]), widen<T>(py.e[k]));
+    };
+    const auto weigh = [&](int i, float (&v)[kN]) {
+      const Piece<T, kN> pw = load_piece<T, kN>(w + i);
+#pragma unroll
+      for (int k = 0; k < kN; ++k) v[k] *= widen<T>(pw.e[k]);
+    };
+    constexpr int kUnroll = VEC ? 2 : 8;
+#pragma unroll kUnroll
+    for (int i = t * kN; i < a.width; i += kThreads * kN) {
+      float v[kN];
+      values(i, v);
+      if constexpr (OP == kRowNormAdd) store_values<T, kN>(static_cast<T*>(a.summed) + row * a.s_stride + i, v);
+      if constexpr (OP == kRowSwiglu && VEC) {
+        // fp32 results in the inputs' place: the piece of x, then (bf16) the piece of y
+        constexpr int kPer = 4;
+        *reinterpret_cast<float4*>(const_cast<T*>(x + i)) = make_float4(v[0], v[1], v[2], v[3]);
+        if constexpr (kN > kPer)
+          *reinterpret_cast<float4*>(const_cast<T*>(y + i)) = make_float4(v[kN - 4], v[kN - 3], v[kN - 2], v[kN - 1]);
+      }
+      if constexpr (kIsNorm<OP>) {
+#pragma unroll
+        for (int k = 0; k < kN; ++k) r.x += v[k] * v[k];
+        weigh(i, v);
+      }
+#pragma unroll
+      for (int k = 0; k < kN; ++k) r.y = max_nan(r.y, fabsf(v[k]));
+    }
+    if (ends) store_end(row + step, next_slot, at, end_value);
+    if (ends || (OP == kRowSwiglu && VEC)) fence_proxy_async();  // before a later copy into these bytes
+    r = row_reduce<kThreads, kIsNorm<OP>>(r, part[odd]);
+    if (W > 1) ok = late == 0;
+    if (!ok) {
+      // copies that did not land within the wait's limit: what is left is marked, the others are awaited
+      // (bounded, too), and the block ends
+      if (t == 0) {
+        for (int64_t left = row; left < a.rows; left += step) a.scale[left] = __int_as_float(0x7FC00000);
+        for (int i = 0; i < slots; ++i) (void)mbar_wait(&full[group][(slot + i) % slots], slot + i < slots ? parity : parity ^ 1);
+      }
+      break;
+    }
+    if (W > 1 && t == 0 && row + (slots - 1) * step < a.rows) {
+      // past the barrier of this row's reduction nobody reads the previous row's slot
+      copy_row(row + (slots - 1) * step, slot == 0 ? slots - 1 : slot - 1);
+    }
+    const RowScale s = row_scale<OP>(a, r);
+#pragma unroll kUnroll
+    for (int i = t * kN; i < a.width; i += kThreads * kN) {
+      float v[kN];
+      if constexpr (OP == kRowSwiglu && VEC) {
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(x + i);
+        if constexpr (kN > 4) *reinterpret_cast<float4*>(v + kN - 4) = *reinterpret_cast<const float4*>(y + i);
+      } else {
+        values(i, v);
+      }
+      if constexpr (kIsNorm<OP>) weigh(i, v);
+#pragma unroll
+      for (int k = 0; k < kN; ++k) v[k] = s.inv == 0.f ? 0.f : v[k] * s.rms;
+      store_codes<kN>(a.codes + row * a.c_stride + i, v, s.inv);
+    }
+    if (t == 0) a.scale[row] = s.scale;
+    if (W == 1) {
+      __syncwarp();
+      if (lane == 0 && row + slots * step < a.rows) copy_row(row + slots * step, slot);
+      __syncwarp();
+    }
+    if (next_slot == 0) parity ^= 1;
+    slot = next_slot;
+  }
+}
+
+// Rows too long for a ring in shared memory: read again in each pass.
 template <typename T, int OP>
 __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowArgs a) {
-  __shared__ float part[2][32];
+  __shared__ float2 part[32];
   const int64_t row = blockIdx.x;
   grid_dep_wait();
   grid_dep_launch();
@@ -241,26 +424,21 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowArgs a) {
   const T* yr = second_row<T, OP>(a, row);
   const T* w = static_cast<const T*>(a.weight);
   const auto value = [&](int i) { return row_value<OP>(widen<T>(xr[i]), kTwoInputs<OP> ? widen<T>(yr[i]) : 0.f); };
-  float inv_rms = 1.f, m = 0.f;
-  if (kIsNorm<OP>) {
-    float ss = 0.f;
-    for (int i = threadIdx.x; i < a.width; i += 1024) {
-      const float v = value(i);
-      ss += v * v;
-    }
-    inv_rms = inv_rms_of(a, row_reduce<1024, true>(ss, part[0]));
-  }
+  float2 r = make_float2(0.f, 0.f);
   for (int i = threadIdx.x; i < a.width; i += 1024) {
     float v = value(i);
-    if (kIsNorm<OP>) v = v * inv_rms * widen<T>(w[i]);
-    m = max_nan(m, fabsf(v));
+    if (kIsNorm<OP>) {
+      r.x += v * v;
+      v *= widen<T>(w[i]);
+    }
+    r.y = max_nan(r.y, fabsf(v));
   }
-  const RowScale s = row_scale(row_reduce<1024, false>(m, part[1]));
+  const RowScale s = row_scale<OP>(a, row_reduce<1024, kIsNorm<OP>>(r, part));
   for (int i = threadIdx.x; i < a.width; i += 1024) {
     float v[1] = {value(i)};
     if (OP == kRowNormAdd) static_cast<T*>(a.summed)[row * a.s_stride + i] = narrow<T>(v[0]);
-    if (kIsNorm<OP>) v[0] = v[0] * inv_rms * widen<T>(w[i]);
-    if (s.inv == 0.f) v[0] = 0.f;
+    if (kIsNorm<OP>) v[0] *= widen<T>(w[i]);
+    v[0] = s.inv == 0.f ? 0.f : v[0] * s.rms;
     store_codes<1>(a.codes + row * a.c_stride + i, v, s.inv);
   }
   if (threadIdx.x == 0) a.scale[row] = s.scale;
@@ -322,9 +500,46 @@ static int launch_rows_as(const char* what, const RowArgs& a, cudaStream_t st) {
                     dim3(G == 32 ? 32 * kWarpRows : G), 0, st, a);
 }
 
-// Threads a row: with at least eight rows an SM a warp takes a row as long as 8 pieces of 16 bytes a
-// lane hold it (no block-wide waits, the most loads in flight a thread); fewer rows are spread over a
-// block each, a piece a thread, which is the shortest chain from the first load to the last store.
+template <typename T, int OP, int W, bool VEC>
+static int launch_stream_as(const char* what, const RowArgs& a, int slots, int piece, cudaStream_t st) {
+  const int smem = 8 / W * slots * piece * (kTwoInputs<OP> ? 2 : 1);
+  auto* kern = int8_stream_rows_kernel<T, OP, W, VEC>;
+  static bool attr_set[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (!attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamSmem);
+    if (e != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    attr_set[dev] = true;
+  }
+  int per_sm = 220 * 1024 / (smem + 2048);  // blocks that fit an SM's shared memory, four at most
+  per_sm = per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm;
+  const int64_t need = (a.rows + 8 / W - 1) / (8 / W);
+  const int64_t most = static_cast<int64_t>(device_sm_count()) * per_sm;
+  return launch_pdl(what, kern, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kStreamThreads),
+                    static_cast<size_t>(smem), st, a, slots, piece);
+}
+template <typename T, int OP>
+static int launch_stream(const char* what, const RowArgs& a, bool vec, cudaStream_t st) {
+  // a row's granules, and room for its ends when it is not aligned
+  const int piece = (static_cast<int>(sizeof(T)) * a.width + 15) / 16 * 16 + (vec ? 0 : 16);
+  const int row = piece * (kTwoInputs<OP> ? 2 : 1);
+  if (row <= 8 * 1024) {
+    // a warp per row, two rows of each of eight warps under way
+    return vec ? launch_stream_as<T, OP, 1, true>(what, a, 2, piece, st)
+               : launch_stream_as<T, OP, 1, false>(what, a, 2, piece, st);
+  }
+  int slots = (kStreamSmem / 2 + 8 * 1024) / row;
+  if (slots < 3) slots = kStreamSmem / row;
+  if (slots > kStreamSlots) slots = kStreamSlots;
+  return vec ? launch_stream_as<T, OP, 8, true>(what, a, slots, piece, st)
+             : launch_stream_as<T, OP, 8, false>(what, a, slots, piece, st);
+}
+
+// Which kernel takes the rows.  `many` (eight rows an SM): a warp a row in registers while 64 values a
+// lane hold it, through shared memory otherwise.  Fewer rows are spread over a block each, one to four
+// pieces a thread, which is the shortest chain from the first load to the last store; unaligned rows
+// likewise, by single values.
 template <typename T, int OP>
 static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
@@ -334,31 +549,27 @@ static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
   bits |= static_cast<uintptr_t>(a.x_stride | a.r_stride | a.s_stride) * sizeof(T);
   const bool vec = bits % 16 == 0 && a.width % V == 0 &&
                    (reinterpret_cast<uintptr_t>(a.codes) | static_cast<uintptr_t>(a.c_stride)) % V == 0;
-  if (vec) {
-    const int need = a.width / V;
-    if (many && need <= 64) return launch_rows_as<T, OP, 32, V, 2>(what, a, st);
-    if (many && need <= 128) return launch_rows_as<T, OP, 32, V, 4>(what, a, st);
-    if (many && need <= 192) return launch_rows_as<T, OP, 32, V, 6>(what, a, st);
-    if (many && need <= 256) return launch_rows_as<T, OP, 32, V, 8>(what, a, st);
-    if (many && need <= 384 && V == 4) return launch_rows_as<T, OP, 32, V, 48 / V>(what, a, st);
+  const int need = vec ? a.width / V : a.width;
+  if (many && vec) {
+    if (need <= 64) return launch_rows_as<T, OP, 32, V, 2>(what, a, st);
+    if (need <= 128) return launch_rows_as<T, OP, 32, V, 4>(what, a, st);
+    if (need <= 192) return launch_rows_as<T, OP, 32, V, 6>(what, a, st);
+    if (need <= 256) return launch_rows_as<T, OP, 32, V, 8>(what, a, st);
+    if (V == 4 && need <= 384) return launch_rows_as<T, OP, 32, V, 48 / V>(what, a, st);
+  }
+  if (!many && vec) {
     if (need <= 256) return launch_rows_as<T, OP, 256, V, 1>(what, a, st);
-    if (!many && need <= 1024) return launch_rows_as<T, OP, 1024, V, 1>(what, a, st);
-    if (many && need <= 512) return launch_rows_as<T, OP, 128, V, 4>(what, a, st);
-    if (many && need <= 640) return launch_rows_as<T, OP, 128, V, 5>(what, a, st);
-    if (many && need <= 768) return launch_rows_as<T, OP, 256, V, 3>(what, a, st);
-    if (many && need <= 1024) return launch_rows_as<T, OP, 256, V, 4>(what, a, st);
-    if (many && need <= 1280) return launch_rows_as<T, OP, 256, V, 5>(what, a, st);
-    if (many && need <= 2048) return launch_rows_as<T, OP, 256, V, 8>(what, a, st);
+    if (need <= 1024) return launch_rows_as<T, OP, 1024, V, 1>(what, a, st);
     if (need <= 2048) return launch_rows_as<T, OP, 1024, V, 2>(what, a, st);
     if (need <= 4096) return launch_rows_as<T, OP, 1024, V, 4>(what, a, st);
-  } else {
-    if (many && a.width <= 256) return launch_rows_as<T, OP, 32, 1, 8>(what, a, st);
-    if (many && a.width <= 512) return launch_rows_as<T, OP, 32, 1, 16>(what, a, st);
-    if (a.width <= 1024) return launch_rows_as<T, OP, 256, 1, 4>(what, a, st);
-    if (a.width <= 2048) return launch_rows_as<T, OP, 256, 1, 8>(what, a, st);
-    if (a.width <= 8192) return launch_rows_as<T, OP, 1024, 1, 8>(what, a, st);
-    if (a.width <= 32768) return launch_rows_as<T, OP, 1024, 1, 32>(what, a, st);
   }
+  if (!many && !vec) {
+    if (need <= 1024) return launch_rows_as<T, OP, 256, 1, 4>(what, a, st);
+    if (need <= 8192) return launch_rows_as<T, OP, 1024, 1, 8>(what, a, st);
+  }
+  // three rows in the ring: the one at work, the next, and the one whose ends are being written
+  if (3 * (static_cast<int64_t>(a.width) * sizeof(T) + 32) * (kTwoInputs<OP> ? 2 : 1) <= kStreamSmem)
+    return launch_stream<T, OP>(what, a, vec, st);
   return launch_pdl(what, int8_long_rows_kernel<T, OP>, dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st, a);
 }
 template <int OP>
