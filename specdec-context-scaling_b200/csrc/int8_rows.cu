@@ -71,6 +71,19 @@ SD_DEV float max_nan(float a, float b) {
   return r;
 }
 
+// the largest magnitude of `m` and N values, two values an instruction (sm_100's three-operand maximum)
+template <int N>
+SD_DEV float amax_values(float m, const float (&v)[N]) {
+  if constexpr (N == 1) {
+    return max_nan(m, fabsf(v[0]));
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; k += 2)
+      asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(v[k]), "f"(v[k + 1]));
+    return m;
+  }
+}
+
 // silu(g) * u with the hardware exponential and reciprocal: for |g| < 16 within 2^-19 of the exact
 // value, far under what decides a code; -0 where exp(-g) overflows
 SD_DEV float silu_mul(float g, float u) {
@@ -215,8 +228,7 @@ __global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) int8_rows_kernel
         v[c][k] *= widen<T>(py[c].e[k]);
       }
     }
-#pragma unroll
-    for (int k = 0; k < N; ++k) r.y = max_nan(r.y, fabsf(v[c][k]));
+    r.y = amax_values(r.y, v[c]);
   }
   const RowScale s = row_scale<OP>(a, row_reduce<G, kIsNorm<OP>>(r, part));
   if (s.inv == 0.f) {  // the same for the whole row: its codes are 0, whatever it holds
@@ -236,29 +248,50 @@ __global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) int8_rows_kernel
   if (t == 0) a.scale[row] = s.scale;
 }
 
-// Rows of any alignment, or too long for registers, through shared memory.  W warps work on a row (1:
-// eight independent warps a block, each with rings of its own; 8: the whole block), and the copies of
-// the next rows are always under way (cp.async.bulk into a ring of `slots` rows), so neither the
-// reduction nor the arithmetic leaves HBM idle.  A copy takes the 16-byte granules inside the row;
-// the up to 7 values at each end of an unaligned row are loaded by lanes one row ahead.  VEC: every
-// row and output is 16-byte aligned, values move in 16-byte pieces, and silu's results take their
-// inputs' place in the ring; else a lane takes every 32nd value.
-constexpr int kStreamThreads = 256;
+// 16 bytes from `sh` (a multiple of sizeof(T), the same for a warp) bytes into a pair of granules.  A
+// branch picks the words: selecting them took three times the instructions, and this is what bounds an
+// unaligned row.
+template <typename T>
+SD_DEV uint4 shift_granules(const uint4* g, uint32_t sh) {
+  const uint4 a = g[0], b = g[1];
+  uint32_t w0, w1, w2, w3, w4;
+  switch (sh >> 2) {
+    case 0: w0 = a.x, w1 = a.y, w2 = a.z, w3 = a.w, w4 = b.x; break;
+    case 1: w0 = a.y, w1 = a.z, w2 = a.w, w3 = b.x, w4 = b.y; break;
+    case 2: w0 = a.z, w1 = a.w, w2 = b.x, w3 = b.y, w4 = b.z; break;
+    default: w0 = a.w, w1 = b.x, w2 = b.y, w3 = b.z, w4 = b.w; break;
+  }
+  if (sizeof(T) == 4) return make_uint4(w0, w1, w2, w3);
+  const uint32_t bits = (sh & 2) * 8;
+  return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                    __funnelshift_r(w3, w4, bits));
+}
+
+// Rows of any alignment, or too long for the registers of a few warps, through shared memory: W warps
+// work on a row (1: eight independent warps a block with a ring each; 4 to 16: the block), and the
+// copies of the next rows are always under way (cp.async.bulk into a ring of `slots` rows), so neither
+// the reduction nor the arithmetic leaves HBM idle.  A copy takes the 16-byte granules inside the row;
+// the values at the two ends of an unaligned row are loaded by lanes, one row ahead.  A thread holds up
+// to stream_pieces(W) pieces of 16 bytes a row from the ring to the store.  VEC: all rows are 16-byte
+// aligned and whole pieces; else a piece is shifted out of two granules of the ring, and the values past
+// the last whole piece are taken by a lane each.  Outputs and weight are aligned either way.
 constexpr int kStreamSlots = 4;
 constexpr int kStreamSmem = 200 * 1024;
+constexpr int stream_threads(int W) { return W == 1 ? 256 : 32 * W; }
+constexpr int stream_pieces(int W) { return W == 1 ? 4 : 5; }
 template <typename T, int OP, int W, bool VEC>
-__global__ void __launch_bounds__(kStreamThreads) int8_stream_rows_kernel(const RowArgs a, int slots, int piece_bytes) {
-  constexpr int kGroups = 8 / W, kThreads = 32 * W, kStreams = kTwoInputs<OP> ? 2 : 1;
-  constexpr int kN = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+__global__ void __launch_bounds__(stream_threads(W)) int8_stream_rows_kernel(const RowArgs a, int slots, int row_bytes) {
+  constexpr int kGroups = W == 1 ? 8 : 1, kThreads = 32 * W, kStreams = kTwoInputs<OP> ? 2 : 1;
+  constexpr int kN = 16 / static_cast<int>(sizeof(T)), kCh = stream_pieces(W);
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t full[kGroups][kStreamSlots];
   __shared__ float2 part[2][W];
-  __shared__ int late;  // W = 8: a thread's wait gave up
+  __shared__ int late;  // W > 1: a thread's wait gave up
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = W == 1 ? warp : 0, t = W == 1 ? lane : threadIdx.x;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kGroups + group;
-  uint8_t* mine = ring + group * slots * kStreams * piece_bytes;
+  uint8_t* mine = ring + group * slots * kStreams * row_bytes;
   if (t == 0) {
     for (int s = 0; s < slots; ++s) mbar_init(&full[group][s], 1);
     fence_barrier_init();
@@ -268,29 +301,30 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_rows_kernel(const 
   grid_dep_wait();
   grid_dep_launch();
 
-  const T* streams[2] = {static_cast<const T*>(a.x), nullptr};
-  const int64_t strides[2] = {a.x_stride, OP == kRowSwiglu ? a.x_stride : a.r_stride};
-  if (kTwoInputs<OP>) streams[1] = second_row<T, OP>(a, 0);
-  const auto row_ptr = [&](int k, int64_t row) { return reinterpret_cast<uintptr_t>(streams[k] + row * strides[k]); };
-  const auto slot_ptr = [&](int k, int slot) { return mine + (slot * kStreams + k) * piece_bytes; };
+  const auto row_ptr = [&](int k, int64_t row) {
+    return reinterpret_cast<uintptr_t>(k == 0 ? static_cast<const T*>(a.x) + row * a.x_stride : second_row<T, OP>(a, row));
+  };
+  const auto slot_ptr = [&](int k, int slot) { return mine + (slot * kStreams + k) * row_bytes; };
   // the granules inside row `row`, by one thread
   const auto copy_row = [&](int64_t row, int slot) {
+    uintptr_t lo[2];
     uint32_t bytes[2] = {0, 0};
+#pragma unroll
     for (int k = 0; k < kStreams; ++k) {
-      const uintptr_t p = row_ptr(k, row), lo = (p + 15) & ~uintptr_t(15);
+      const uintptr_t p = row_ptr(k, row);
+      lo[k] = (p + 15) & ~uintptr_t(15);
       const uintptr_t hi = (p + static_cast<uintptr_t>(a.width) * sizeof(T)) & ~uintptr_t(15);
-      if (hi > lo) bytes[k] = static_cast<uint32_t>(hi - lo);
+      if (hi > lo[k]) bytes[k] = static_cast<uint32_t>(hi - lo[k]);
     }
-    fence_proxy_async();  // the slot's last use was by ordinary loads and stores
+    fence_proxy_async();  // the ends of the slot's last row were written by ordinary stores
     mbar_arrive_expect_tx(&full[group][slot], bytes[0] + bytes[1]);
-    for (int k = 0; k < kStreams; ++k) {
-      const uintptr_t p = row_ptr(k, row), lo = (p + 15) & ~uintptr_t(15);
+#pragma unroll
+    for (int k = 0; k < kStreams; ++k)
       if (bytes[k])
-        bulk_g2s(slot_ptr(k, slot) + (lo - (p & ~uintptr_t(15))), reinterpret_cast<const void*>(lo), bytes[k],
-                 &full[group][slot]);
-    }
+        bulk_g2s(slot_ptr(k, slot) + (lo[k] - (row_ptr(k, row) & ~uintptr_t(15))), reinterpret_cast<const void*>(lo[k]),
+                 bytes[k], &full[group][slot]);
   };
-  // the values of `row` outside its granules, one a lane (16 lanes a stream): index, or -1
+  // the values of `row` outside its granules, one a lane (16 lanes an input): index, or -1
   const auto end_index = [&](int64_t row) {
     const int k = lane >> 4, l = lane & 15;
     if (k >= kStreams) return -1;
@@ -300,10 +334,20 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_rows_kernel(const 
     const int tail = hi >= lo ? static_cast<int>((end - hi) / sizeof(T)) : 0;
     return l < head ? l : l < head + tail ? a.width - tail + (l - head) : -1;
   };
-  const auto load_end = [&](int64_t row, int at) { return at < 0 ? T(0.f) : reinterpret_cast<const T*>(row_ptr(lane >> 4, row))[at]; };
+  const auto load_end = [&](int64_t row, int at) {
+    return at < 0 ? T(0.f) : reinterpret_cast<const T*>(row_ptr(lane >> 4, row))[at];
+  };
   const auto store_end = [&](int64_t row, int slot, int at, T v) {
     const int k = lane >> 4;
     if (at >= 0) reinterpret_cast<T*>(slot_ptr(k, slot) + (row_ptr(k, row) & 15))[at] = v;
+  };
+  // 16 bytes from value i on of input k of the row in `slot`
+  const auto piece = [&](int k, int slot, uint32_t sh, int i) {
+    Piece<T, kN> p;
+    const uint4* g = reinterpret_cast<const uint4*>(slot_ptr(k, slot)) + i / kN;
+    const uint4 raw = VEC ? g[0] : shift_granules<T>(g, sh);
+    *reinterpret_cast<uint4*>(&p) = raw;
+    return p;
   };
 
   if (t == 0)
@@ -319,6 +363,9 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_rows_kernel(const 
   else
     __syncwarp();
 
+  const T* w = static_cast<const T*>(a.weight);
+  const int whole = a.width / kN * kN;                                   // values in whole pieces
+  const int tail = !VEC && t < a.width - whole ? whole + t : -1;         // this thread's value past them
   int slot = 0;
   uint32_t parity = 0, odd = 0;
   for (int64_t row = row0; row < a.rows; row += step, odd ^= 1) {
@@ -335,43 +382,43 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_rows_kernel(const 
       ok = __all_sync(0xffffffffu, ok);
     else if (!ok)
       late = 1;
-    const T* x = reinterpret_cast<const T*>(slot_ptr(0, slot) + (row_ptr(0, row) & 15));
-    const T* y = kStreams == 2 ? reinterpret_cast<const T*>(slot_ptr(1, slot) + (row_ptr(1, row) & 15)) : x;
-    const T* w = static_cast<const T*>(a.weight);
+    const uint32_t shx = VEC ? 0 : static_cast<uint32_t>(row_ptr(0, row) & 15);
+    const uint32_t shy = VEC || kStreams == 1 ? 0 : static_cast<uint32_t>(row_ptr(1, row) & 15);
+    float v[kCh][kN], tv[1] = {0.f};
     float2 r = make_float2(0.f, 0.f);
-    const auto values = [&](int i, float (&v)[kN]) {
-      const Piece<T, kN> px = load_piece<T, kN>(x + i), py = load_piece<T, kN>(y + i);
 #pragma unroll
-      for (int k = 0; k < kN; ++k) v[k] = row_value<OP>(widen<T>(px.e[k]), widen<T>(py.e[k]));
-    };
-    const auto weigh = [&](int i, float (&v)[kN]) {
-      const Piece<T, kN> pw = load_piece<T, kN>(w + i);
+    for (int c = 0; c < kCh; ++c) {
+      const int i = (t + kThreads * c) * kN;
+      if (i >= whole) break;
+      const Piece<T, kN> px = piece(0, slot, shx, i), py = kStreams == 2 ? piece(1, slot, shy, i) : px;
 #pragma unroll
-      for (int k = 0; k < kN; ++k) v[k] *= widen<T>(pw.e[k]);
-    };
-    constexpr int kUnroll = VEC ? 2 : 8;
-#pragma unroll kUnroll
-    for (int i = t * kN; i < a.width; i += kThreads * kN) {
-      float v[kN];
-      values(i, v);
-      if constexpr (OP == kRowNormAdd) store_values<T, kN>(static_cast<T*>(a.summed) + row * a.s_stride + i, v);
-      if constexpr (OP == kRowSwiglu && VEC) {
-        // fp32 results in the inputs' place: the piece of x, then (bf16) the piece of y
-        constexpr int kPer = 4;
-        *reinterpret_cast<float4*>(const_cast<T*>(x + i)) = make_float4(v[0], v[1], v[2], v[3]);
-        if constexpr (kN > kPer)
-          *reinterpret_cast<float4*>(const_cast<T*>(y + i)) = make_float4(v[kN - 4], v[kN - 3], v[kN - 2], v[kN - 1]);
-      }
+      for (int k = 0; k < kN; ++k) v[c][k] = row_value<OP>(widen<T>(px.e[k]), widen<T>(py.e[k]));
+      if constexpr (OP == kRowNormAdd)
+        store_values<T, kN>(static_cast<T*>(a.summed) + row * a.s_stride + i, v[c]);
       if constexpr (kIsNorm<OP>) {
+        const Piece<T, kN> pw = load_piece<T, kN>(w + i);
 #pragma unroll
-        for (int k = 0; k < kN; ++k) r.x += v[k] * v[k];
-        weigh(i, v);
+        for (int k = 0; k < kN; ++k) {
+          r.x += v[c][k] * v[c][k];
+          v[c][k] *= widen<T>(pw.e[k]);
+        }
       }
-#pragma unroll
-      for (int k = 0; k < kN; ++k) r.y = max_nan(r.y, fabsf(v[k]));
+      r.y = amax_values(r.y, v[c]);
     }
-    if (ends) store_end(row + step, next_slot, at, end_value);
-    if (ends || (OP == kRowSwiglu && VEC)) fence_proxy_async();  // before a later copy into these bytes
+    if (tail >= 0) {
+      const auto at_tail = [&](int k, uint32_t sh) { return widen<T>(reinterpret_cast<const T*>(slot_ptr(k, slot) + sh)[tail]); };
+      tv[0] = row_value<OP>(at_tail(0, shx), kStreams == 2 ? at_tail(1, shy) : 0.f);
+      if constexpr (OP == kRowNormAdd) static_cast<T*>(a.summed)[row * a.s_stride + tail] = narrow<T>(tv[0]);
+      if constexpr (kIsNorm<OP>) {
+        r.x += tv[0] * tv[0];
+        tv[0] *= widen<T>(w[tail]);
+      }
+      r.y = amax_values(r.y, tv);
+    }
+    if (ends) {
+      store_end(row + step, next_slot, at, end_value);
+      fence_proxy_async();  // before a later copy into these bytes
+    }
     r = row_reduce<kThreads, kIsNorm<OP>>(r, part[odd]);
     if (W > 1) ok = late == 0;
     if (!ok) {
@@ -379,35 +426,38 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_rows_kernel(const 
       // (bounded, too), and the block ends
       if (t == 0) {
         for (int64_t left = row; left < a.rows; left += step) a.scale[left] = __int_as_float(0x7FC00000);
-        for (int i = 0; i < slots; ++i) (void)mbar_wait(&full[group][(slot + i) % slots], slot + i < slots ? parity : parity ^ 1);
+        for (int i = 0; i < slots; ++i)
+          (void)mbar_wait(&full[group][(slot + i) % slots], slot + i < slots ? parity : parity ^ 1);
       }
       break;
     }
-    if (W > 1 && t == 0 && row + (slots - 1) * step < a.rows) {
-      // past the barrier of this row's reduction nobody reads the previous row's slot
-      copy_row(row + (slots - 1) * step, slot == 0 ? slots - 1 : slot - 1);
+    // W > 1: past the barrier of this row's reduction nobody reads the previous row's slot; W = 1: the
+    // shuffles of the reduction come after every lane's reads of this row's
+    if (t == 0) {
+      if (W > 1 && row + (slots - 1) * step < a.rows)
+        copy_row(row + (slots - 1) * step, slot == 0 ? slots - 1 : slot - 1);
+      if (W == 1 && row + slots * step < a.rows) copy_row(row + slots * step, slot);
     }
     const RowScale s = row_scale<OP>(a, r);
-#pragma unroll kUnroll
-    for (int i = t * kN; i < a.width; i += kThreads * kN) {
-      float v[kN];
-      if constexpr (OP == kRowSwiglu && VEC) {
-        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(x + i);
-        if constexpr (kN > 4) *reinterpret_cast<float4*>(v + kN - 4) = *reinterpret_cast<const float4*>(y + i);
-      } else {
-        values(i, v);
-      }
-      if constexpr (kIsNorm<OP>) weigh(i, v);
+    int8_t* codes = a.codes + row * a.c_stride;
 #pragma unroll
-      for (int k = 0; k < kN; ++k) v[k] = s.inv == 0.f ? 0.f : v[k] * s.rms;
-      store_codes<kN>(a.codes + row * a.c_stride + i, v, s.inv);
+    for (int c = 0; c < kCh; ++c) {
+      const int i = (t + kThreads * c) * kN;
+      if (i >= whole) break;
+      if (s.inv == 0.f)
+#pragma unroll
+        for (int k = 0; k < kN; ++k) v[c][k] = 0.f;
+      if constexpr (kIsNorm<OP>)
+#pragma unroll
+        for (int k = 0; k < kN; ++k) v[c][k] *= s.rms;
+      store_codes<kN>(codes + i, v[c], s.inv);
+    }
+    if (tail >= 0) {
+      tv[0] = s.inv == 0.f ? 0.f : tv[0] * s.rms;
+      store_codes<1>(codes + tail, tv, s.inv);
     }
     if (t == 0) a.scale[row] = s.scale;
-    if (W == 1) {
-      __syncwarp();
-      if (lane == 0 && row + slots * step < a.rows) copy_row(row + slots * step, slot);
-      __syncwarp();
-    }
+    if (W == 1) __syncwarp();
     if (next_slot == 0) parity ^= 1;
     slot = next_slot;
   }
@@ -501,8 +551,9 @@ static int launch_rows_as(const char* what, const RowArgs& a, cudaStream_t st) {
 }
 
 template <typename T, int OP, int W, bool VEC>
-static int launch_stream_as(const char* what, const RowArgs& a, int slots, int piece, cudaStream_t st) {
-  const int smem = 8 / W * slots * piece * (kTwoInputs<OP> ? 2 : 1);
+static int launch_stream_as(const char* what, const RowArgs& a, int slots, int row_bytes, cudaStream_t st) {
+  constexpr int kGroups = W == 1 ? 8 : 1;
+  const int smem = kGroups * slots * row_bytes * (kTwoInputs<OP> ? 2 : 1);
   auto* kern = int8_stream_rows_kernel<T, OP, W, VEC>;
   static bool attr_set[64] = {};
   int dev = 0;
@@ -512,43 +563,50 @@ static int launch_stream_as(const char* what, const RowArgs& a, int slots, int p
     if (e != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
     attr_set[dev] = true;
   }
-  int per_sm = 220 * 1024 / (smem + 2048);  // blocks that fit an SM's shared memory, four at most
-  per_sm = per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm;
-  const int64_t need = (a.rows + 8 / W - 1) / (8 / W);
+  // blocks that fit an SM's shared memory, and 1024 threads
+  int per_sm = 220 * 1024 / (smem + 2048);
+  per_sm = per_sm < 1 ? 1 : per_sm > 1024 / stream_threads(W) ? 1024 / stream_threads(W) : per_sm;
+  const int64_t need = (a.rows + kGroups - 1) / kGroups;
   const int64_t most = static_cast<int64_t>(device_sm_count()) * per_sm;
-  return launch_pdl(what, kern, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kStreamThreads),
-                    static_cast<size_t>(smem), st, a, slots, piece);
+  return launch_pdl(what, kern, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(stream_threads(W)),
+                    static_cast<size_t>(smem), st, a, slots, row_bytes);
 }
+// SPECDEC_ERR_UNSUPPORTED when three rows do not fit the ring (the one at work, the next, and the one
+// whose ends are being written)
 template <typename T, int OP>
 static int launch_stream(const char* what, const RowArgs& a, bool vec, cudaStream_t st) {
-  // a row's granules, and room for its ends when it is not aligned
-  const int piece = (static_cast<int>(sizeof(T)) * a.width + 15) / 16 * 16 + (vec ? 0 : 16);
-  const int row = piece * (kTwoInputs<OP> ? 2 : 1);
-  if (row <= 8 * 1024) {
-    // a warp per row, two rows of each of eight warps under way
-    return vec ? launch_stream_as<T, OP, 1, true>(what, a, 2, piece, st)
-               : launch_stream_as<T, OP, 1, false>(what, a, 2, piece, st);
-  }
-  int slots = (kStreamSmem / 2 + 8 * 1024) / row;
-  if (slots < 3) slots = kStreamSmem / row;
+  constexpr int kStreams = kTwoInputs<OP> ? 2 : 1;
+  const int64_t bytes = (static_cast<int64_t>(sizeof(T)) * a.width + 15) / 16 * 16 + (vec ? 0 : 32);
+  const int64_t pieces = (a.width + 16 / static_cast<int>(sizeof(T)) - 1) / (16 / static_cast<int>(sizeof(T)));
+  if (pieces > 512 * stream_pieces(16) || 3 * kStreams * bytes > kStreamSmem) return SPECDEC_ERR_UNSUPPORTED;
+  const int row = static_cast<int>(bytes);
+  if (!vec && pieces <= 32 * stream_pieces(1)) return launch_stream_as<T, OP, 1, false>(what, a, 2, row, st);
+  if (!vec && pieces <= 128 * stream_pieces(4)) return launch_stream_as<T, OP, 4, false>(what, a, kStreamSlots, row, st);
+  int slots = (kStreamSmem / 2 + 8 * 1024) / (row * kStreams);  // two blocks an SM, if they have three rows each
+  if (slots < 3) slots = kStreamSmem / (row * kStreams);
   if (slots > kStreamSlots) slots = kStreamSlots;
-  return vec ? launch_stream_as<T, OP, 8, true>(what, a, slots, piece, st)
-             : launch_stream_as<T, OP, 8, false>(what, a, slots, piece, st);
+  if (pieces <= 256 * stream_pieces(8))
+    return vec ? launch_stream_as<T, OP, 8, true>(what, a, slots, row, st)
+               : launch_stream_as<T, OP, 8, false>(what, a, slots, row, st);
+  return vec ? launch_stream_as<T, OP, 16, true>(what, a, slots, row, st)
+             : launch_stream_as<T, OP, 16, false>(what, a, slots, row, st);
 }
 
-// Which kernel takes the rows.  `many` (eight rows an SM): a warp a row in registers while 64 values a
-// lane hold it, through shared memory otherwise.  Fewer rows are spread over a block each, one to four
-// pieces a thread, which is the shortest chain from the first load to the last store; unaligned rows
-// likewise, by single values.
+// Which kernel takes the rows.  `many` (eight rows an SM): aligned rows in the registers of a warp, or
+// of four, while they hold it; others through shared memory.  Fewer rows are spread over a block each,
+// one to four pieces a thread, which is the shortest chain from the first load to the last store;
+// unaligned ones likewise, by single values, and so are rows whose outputs are not aligned.
 template <typename T, int OP>
 static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool many = a.rows >= 8 * device_sm_count();
-  uintptr_t bits = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.residual) |
-                   reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.summed);
-  bits |= static_cast<uintptr_t>(a.x_stride | a.r_stride | a.s_stride) * sizeof(T);
-  const bool vec = bits % 16 == 0 && a.width % V == 0 &&
-                   (reinterpret_cast<uintptr_t>(a.codes) | static_cast<uintptr_t>(a.c_stride)) % V == 0;
+  const uintptr_t out_bits = reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.summed) |
+                             static_cast<uintptr_t>(a.s_stride) * sizeof(T);
+  const bool out_vec = out_bits % 16 == 0 &&
+                       (reinterpret_cast<uintptr_t>(a.codes) | static_cast<uintptr_t>(a.c_stride)) % V == 0;
+  const uintptr_t in_bits = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.residual) |
+                            static_cast<uintptr_t>(a.x_stride | a.r_stride) * sizeof(T);
+  const bool vec = out_vec && in_bits % 16 == 0 && a.width % V == 0;
   const int need = vec ? a.width / V : a.width;
   if (many && vec) {
     if (need <= 64) return launch_rows_as<T, OP, 32, V, 2>(what, a, st);
@@ -556,6 +614,7 @@ static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
     if (need <= 192) return launch_rows_as<T, OP, 32, V, 6>(what, a, st);
     if (need <= 256) return launch_rows_as<T, OP, 32, V, 8>(what, a, st);
     if (V == 4 && need <= 384) return launch_rows_as<T, OP, 32, V, 48 / V>(what, a, st);
+    if (need <= 640) return launch_rows_as<T, OP, 128, V, 5>(what, a, st);
   }
   if (!many && vec) {
     if (need <= 256) return launch_rows_as<T, OP, 256, V, 1>(what, a, st);
@@ -563,13 +622,10 @@ static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
     if (need <= 2048) return launch_rows_as<T, OP, 1024, V, 2>(what, a, st);
     if (need <= 4096) return launch_rows_as<T, OP, 1024, V, 4>(what, a, st);
   }
-  if (!many && !vec) {
-    if (need <= 1024) return launch_rows_as<T, OP, 256, 1, 4>(what, a, st);
-    if (need <= 8192) return launch_rows_as<T, OP, 1024, 1, 8>(what, a, st);
-  }
-  // three rows in the ring: the one at work, the next, and the one whose ends are being written
-  if (3 * (static_cast<int64_t>(a.width) * sizeof(T) + 32) * (kTwoInputs<OP> ? 2 : 1) <= kStreamSmem)
-    return launch_stream<T, OP>(what, a, vec, st);
+  if (out_vec && (many || vec || need > 8192))
+    if (const int rc = launch_stream<T, OP>(what, a, vec, st); rc != SPECDEC_ERR_UNSUPPORTED) return rc;
+  if (a.width <= 1024) return launch_rows_as<T, OP, 256, 1, 4>(what, a, st);
+  if (a.width <= 8192) return launch_rows_as<T, OP, 1024, 1, 8>(what, a, st);
   return launch_pdl(what, int8_long_rows_kernel<T, OP>, dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st, a);
 }
 template <int OP>

@@ -611,8 +611,11 @@ def rmsnorm_int8(x, weight, eps: float = 1e-6, *, residual=None, summed=None, co
     r_ptr = s_ptr = None
     r_stride = s_stride = hidden
     if residual is not None:
-        if summed is None:
-            summed = torch.empty((rows, hidden), dtype=x.dtype, device=x.device)
+        if summed is None:  # rows on 16-byte boundaries, so the next call on it reads aligned rows
+            stride = (hidden + 7) & ~7
+            summed = x.new_empty((rows, stride))
+            if stride != hidden:
+                summed = summed[:, :hidden]
         for t in (residual, summed):
             if t.dtype != x.dtype or t.shape != x.shape or t.stride(1) != 1 and hidden != 1 or not t.is_cuda:
                 raise ValueError("residual and summed must be (rows, hidden) of x's dtype with contiguous columns")
