@@ -276,9 +276,9 @@ SD_DEV uint4 shift_granules(const uint4* g, uint32_t sh) {
 // aligned and whole pieces; else a piece is shifted out of two granules of the ring, and the values past
 // the last whole piece are taken by a lane each.  Outputs and weight are aligned either way.
 constexpr int kStreamSlots = 4;
-constexpr int kStreamSmem = 200 * 1024;
+constexpr int kStreamSmem = 222 * 1024;
 constexpr int stream_threads(int W) { return W == 1 ? 256 : 32 * W; }
-constexpr int stream_pieces(int W) { return W == 1 ? 4 : 5; }
+constexpr int stream_pieces(int W) { return W == 1 ? 7 : 5; }
 template <typename T, int OP, int W, bool VEC>
 __global__ void __launch_bounds__(stream_threads(W)) int8_stream_rows_kernel(const RowArgs a, int slots, int row_bytes) {
   constexpr int kGroups = W == 1 ? 8 : 1, kThreads = 32 * W, kStreams = kTwoInputs<OP> ? 2 : 1;
@@ -304,50 +304,47 @@ __global__ void __launch_bounds__(stream_threads(W)) int8_stream_rows_kernel(con
   const auto row_ptr = [&](int k, int64_t row) {
     return reinterpret_cast<uintptr_t>(k == 0 ? static_cast<const T*>(a.x) + row * a.x_stride : second_row<T, OP>(a, row));
   };
+  const uint32_t width_bytes = static_cast<uint32_t>(a.width) * sizeof(T);
+  // bytes of row `row` of input k into its first granule
+  const uint32_t base0 = static_cast<uint32_t>(row_ptr(0, 0)), base1 = kStreams == 2 ? static_cast<uint32_t>(row_ptr(1, 0)) : 0;
+  const uint32_t pitch0 = static_cast<uint32_t>(a.x_stride) * sizeof(T);
+  const uint32_t pitch1 = static_cast<uint32_t>(OP == kRowSwiglu ? a.x_stride : a.r_stride) * sizeof(T);
+  const auto row_shift = [&](int k, int64_t row) {
+    return VEC ? 0u : ((k == 0 ? base0 : base1) + static_cast<uint32_t>(row) * (k == 0 ? pitch0 : pitch1)) & 15u;
+  };
   const auto slot_ptr = [&](int k, int slot) { return mine + (slot * kStreams + k) * row_bytes; };
   // the granules inside row `row`, by one thread
   const auto copy_row = [&](int64_t row, int slot) {
-    uintptr_t lo[2];
-    uint32_t bytes[2] = {0, 0};
+    uint32_t skip[2], bytes[2] = {0, 0};
 #pragma unroll
     for (int k = 0; k < kStreams; ++k) {
-      const uintptr_t p = row_ptr(k, row);
-      lo[k] = (p + 15) & ~uintptr_t(15);
-      const uintptr_t hi = (p + static_cast<uintptr_t>(a.width) * sizeof(T)) & ~uintptr_t(15);
-      if (hi > lo[k]) bytes[k] = static_cast<uint32_t>(hi - lo[k]);
+      const uint32_t sh = row_shift(k, row);
+      skip[k] = (16 - sh) & 15;
+      if (width_bytes > skip[k]) bytes[k] = (width_bytes - skip[k]) & ~15u;
     }
     fence_proxy_async();  // the ends of the slot's last row were written by ordinary stores
     mbar_arrive_expect_tx(&full[group][slot], bytes[0] + bytes[1]);
 #pragma unroll
     for (int k = 0; k < kStreams; ++k)
       if (bytes[k])
-        bulk_g2s(slot_ptr(k, slot) + (lo[k] - (row_ptr(k, row) & ~uintptr_t(15))), reinterpret_cast<const void*>(lo[k]),
+        bulk_g2s(slot_ptr(k, slot) + (skip[k] ? 16 : 0), reinterpret_cast<const void*>(row_ptr(k, row) + skip[k]),
                  bytes[k], &full[group][slot]);
   };
   // the values of `row` outside its granules, one a lane (16 lanes an input): index, or -1
+  const int end_input = lane >> 4;
   const auto end_index = [&](int64_t row) {
-    const int k = lane >> 4, l = lane & 15;
-    if (k >= kStreams) return -1;
-    const uintptr_t p = row_ptr(k, row), lo = (p + 15) & ~uintptr_t(15);
-    const uintptr_t end = p + static_cast<uintptr_t>(a.width) * sizeof(T), hi = end & ~uintptr_t(15);
-    const int head = min(a.width, static_cast<int>((lo - p) / sizeof(T)));
-    const int tail = hi >= lo ? static_cast<int>((end - hi) / sizeof(T)) : 0;
+    if (end_input >= kStreams) return -1;
+    const int l = lane & 15;
+    const uint32_t sh = row_shift(end_input, row);
+    const int head = min(a.width, static_cast<int>(((16 - sh) & 15) / sizeof(T)));
+    const int tail = sh != 0 && sh + width_bytes < 16 ? 0 : static_cast<int>(((sh + width_bytes) & 15) / sizeof(T));
     return l < head ? l : l < head + tail ? a.width - tail + (l - head) : -1;
   };
   const auto load_end = [&](int64_t row, int at) {
-    return at < 0 ? T(0.f) : reinterpret_cast<const T*>(row_ptr(lane >> 4, row))[at];
+    return at < 0 ? T(0.f) : reinterpret_cast<const T*>(row_ptr(end_input, row))[at];
   };
   const auto store_end = [&](int64_t row, int slot, int at, T v) {
-    const int k = lane >> 4;
-    if (at >= 0) reinterpret_cast<T*>(slot_ptr(k, slot) + (row_ptr(k, row) & 15))[at] = v;
-  };
-  // 16 bytes from value i on of input k of the row in `slot`
-  const auto piece = [&](int k, int slot, uint32_t sh, int i) {
-    Piece<T, kN> p;
-    const uint4* g = reinterpret_cast<const uint4*>(slot_ptr(k, slot)) + i / kN;
-    const uint4 raw = VEC ? g[0] : shift_granules<T>(g, sh);
-    *reinterpret_cast<uint4*>(&p) = raw;
-    return p;
+    if (at >= 0) reinterpret_cast<T*>(slot_ptr(end_input, slot) + row_shift(end_input, row))[at] = v;
   };
 
   if (t == 0)
@@ -382,15 +379,22 @@ __global__ void __launch_bounds__(stream_threads(W)) int8_stream_rows_kernel(con
       ok = __all_sync(0xffffffffu, ok);
     else if (!ok)
       late = 1;
-    const uint32_t shx = VEC ? 0 : static_cast<uint32_t>(row_ptr(0, row) & 15);
-    const uint32_t shy = VEC || kStreams == 1 ? 0 : static_cast<uint32_t>(row_ptr(1, row) & 15);
+    const uint32_t shx = row_shift(0, row), shy = kStreams == 2 ? row_shift(1, row) : 0;
+    const uint8_t *xs = slot_ptr(0, slot), *ys = slot_ptr(kStreams - 1, slot);
+    // 16 bytes from value i on of an input's row
+    const auto piece = [&](const uint8_t* at, uint32_t sh, int i) {
+      Piece<T, kN> p;
+      const uint4* g = reinterpret_cast<const uint4*>(at + i * sizeof(T));
+      *reinterpret_cast<uint4*>(&p) = VEC ? g[0] : shift_granules<T>(g, sh);
+      return p;
+    };
     float v[kCh][kN], tv[1] = {0.f};
     float2 r = make_float2(0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < kCh; ++c) {
       const int i = (t + kThreads * c) * kN;
       if (i >= whole) break;
-      const Piece<T, kN> px = piece(0, slot, shx, i), py = kStreams == 2 ? piece(1, slot, shy, i) : px;
+      const Piece<T, kN> px = piece(xs, shx, i), py = kStreams == 2 ? piece(ys, shy, i) : px;
 #pragma unroll
       for (int k = 0; k < kN; ++k) v[c][k] = row_value<OP>(widen<T>(px.e[k]), widen<T>(py.e[k]));
       if constexpr (OP == kRowNormAdd)
@@ -406,8 +410,8 @@ __global__ void __launch_bounds__(stream_threads(W)) int8_stream_rows_kernel(con
       r.y = amax_values(r.y, v[c]);
     }
     if (tail >= 0) {
-      const auto at_tail = [&](int k, uint32_t sh) { return widen<T>(reinterpret_cast<const T*>(slot_ptr(k, slot) + sh)[tail]); };
-      tv[0] = row_value<OP>(at_tail(0, shx), kStreams == 2 ? at_tail(1, shy) : 0.f);
+      const auto at_tail = [&](const uint8_t* at, uint32_t sh) { return widen<T>(reinterpret_cast<const T*>(at + sh)[tail]); };
+      tv[0] = row_value<OP>(at_tail(xs, shx), kStreams == 2 ? at_tail(ys, shy) : 0.f);
       if constexpr (OP == kRowNormAdd) static_cast<T*>(a.summed)[row * a.s_stride + tail] = narrow<T>(tv[0]);
       if constexpr (kIsNorm<OP>) {
         r.x += tv[0] * tv[0];
@@ -494,11 +498,15 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowArgs a) {
   if (threadIdx.x == 0) a.scale[row] = s.scale;
 }
 
-// code * scale: a warp per row and 1024 columns, 16 codes a lane and load where the rows allow it
+// code * scale: a warp per row and 1024 columns.  VEC: 16 codes a lane and load.  Else the outputs'
+// alignment leads: a lane stores the 16 aligned bytes of outputs from value i on, its codes shifted out
+// of the words around them, and the values before the first and after the last such piece (at most 26)
+// are one lane's each.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t* __restrict__ codes, int64_t c_stride,
                                                               const float* __restrict__ scale, T* __restrict__ out,
                                                               int64_t o_stride, int64_t rows, int width) {
+  constexpr int kOut = 16 / static_cast<int>(sizeof(T));
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   grid_dep_wait();
@@ -507,9 +515,8 @@ __global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t* __re
   const float s = scale[row];
   const int8_t* c = codes + row * c_stride;
   T* o = out + row * o_stride;
-  const int begin = blockIdx.y * 1024, end = min(width, begin + 1024);
   if constexpr (VEC) {
-    constexpr int kOut = 16 / sizeof(T);
+    const int begin = blockIdx.y * 1024, end = min(width, begin + 1024);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int i = begin + (j * 32 + lane) * 16;
@@ -525,7 +532,31 @@ __global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t* __re
       }
     }
   } else {
-    for (int i = begin + lane; i < end; i += 32) o[i] = narrow<T>(static_cast<float>(c[i]) * s);
+    // pieces end 4 codes before the row does, so that the words around their codes are the row's
+    int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(o) & 15)) & 15) / static_cast<int>(sizeof(T));
+    if (head < 4 && (reinterpret_cast<uintptr_t>(c) & 3)) head += kOut;  // nor before its first code
+    const int pieces = max(0, width - head - 4) / kOut, most = 1024 / kOut;
+    const int last = min(pieces, static_cast<int>(blockIdx.y + 1) * most);
+    for (int j = blockIdx.y * most + lane; j < last; j += 32) {
+      const int i = head + j * kOut;
+      const uintptr_t at = reinterpret_cast<uintptr_t>(c + i);
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+      const uint32_t bits = static_cast<uint32_t>(at & 3) * 8;
+      uint32_t raw[kOut / 4 + 1];
+#pragma unroll
+      for (int q = 0; q <= kOut / 4; ++q) raw[q] = words[q];
+      float v[kOut];
+#pragma unroll
+      for (int q = 0; q < kOut; ++q) {
+        const uint32_t word = __funnelshift_r(raw[q / 4], raw[q / 4 + 1], bits);
+        v[q] = static_cast<float>(static_cast<int8_t>(word >> (8 * (q % 4)))) * s;
+      }
+      store_values<T, kOut>(o + i, v);
+    }
+    if (blockIdx.y == 0) {
+      const int first = min(head, width), i = lane < first ? lane : head + pieces * kOut + lane - first;
+      if (i < width) o[i] = narrow<T>(static_cast<float>(c[i]) * s);
+    }
   }
 }
 
