@@ -458,6 +458,113 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   }
 }
 
+// ---------------------------------------------------------------- a few rows
+// A call of up to 32 rows is bound by reading W once and by the chain of latencies around that.  Here a
+// block takes 16 output channels and its warps a share of K each, straight from global memory into
+// mma.sync fragments: no ring, barriers or TMEM to set up.  (The tcgen05 kernel took 4.2 us at
+// 5 x 1536 x 2048 and 6.7 us at 5 x 8960 x 1536.)
+// mma.sync m16n8k32 multiplies in any order of K, so a lane's 16 consecutive codes of a row are its
+// fragments of two products: lane (g, t) holds codes 16 t .. 16 t + 15 of channels g and g + 8 and of
+// token g in each step of 64 codes.  Channels and tokens past the end read as zero.
+constexpr int kFewRows = 32;
+constexpr int kFewCh = 16;
+constexpr int kFewStep = 64;
+constexpr int kFewAhead = 4;  // steps whose loads of a are under way together (of W: 4, or all of a warp's share up to 9)
+
+struct FewParams {
+  const int8_t* a;
+  const int8_t* w;
+  const float* a_scale;
+  const float* w_scale;
+  const float* bias;
+  void* out;
+  int64_t a_stride, w_stride, out_stride;
+  int32_t rows, n, width, weight_ready;
+};
+
+// codes k .. k + 15 of a row of `width` (16-byte aligned); zero past its end
+SD_DEV uint4 load_codes16(const int8_t* row, int k, int width) {
+  if (k + 16 <= width) return *reinterpret_cast<const uint4*>(row + k);
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (k < width) {
+    uint32_t* words = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < 15; ++i)
+      if (k + i < width) words[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + i])) << (8 * (i % 4));
+  }
+  return v;
+}
+SD_DEV void mma_m16n8k32(int32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int NB, int WARPS, int AHEAD, typename T>
+__global__ void __launch_bounds__(32 * WARPS) linear_int8_few_kernel(const FewParams p) {
+  __shared__ int32_t part[WARPS][NB * 8][kFewCh + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * kFewCh;
+  const int steps = (p.width + kFewStep - 1) / kFewStep;
+  const int s_begin = steps * warp / WARPS, s_end = steps * (warp + 1) / WARPS;
+  const int8_t* w0 = p.w + static_cast<int64_t>(n0 + g) * p.w_stride;
+  const int8_t* w1 = w0 + 8 * p.w_stride;
+  const bool has0 = n0 + g < p.n, has1 = n0 + g + 8 < p.n;
+  int32_t d[NB][4] = {};
+  if (!p.weight_ready) grid_dep_wait();
+  bool waited = !p.weight_ready;
+  for (int s = s_begin; s < s_end || !waited; s += AHEAD) {
+    uint4 wa[AHEAD], wb[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = s + j < s_end ? (s + j) * kFewStep + t * 16 : p.width;
+      wa[j] = has0 ? load_codes16(w0, k, p.width) : make_uint4(0, 0, 0, 0);
+      wb[j] = has1 ? load_codes16(w1, k, p.width) : make_uint4(0, 0, 0, 0);
+    }
+    if (!waited) {
+      grid_dep_wait();
+      waited = true;
+    }
+#pragma unroll
+    for (int h = 0; h < AHEAD; h += kFewAhead) {
+      uint4 x[NB][kFewAhead];
+#pragma unroll
+      for (int j = 0; j < kFewAhead && h + j < AHEAD; ++j) {
+        const int k = s + h + j < s_end ? (s + h + j) * kFewStep + t * 16 : p.width;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          x[b][j] = b * 8 + g < p.rows ? load_codes16(p.a + static_cast<int64_t>(b * 8 + g) * p.a_stride, k, p.width)
+                                       : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < kFewAhead && h + j < AHEAD; ++j)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint4 &c0 = wa[h + j], &c1 = wb[h + j];
+          mma_m16n8k32(d[b], c0.x, c1.x, c0.y, c1.y, x[b][j].x, x[b][j].y);
+          mma_m16n8k32(d[b], c0.z, c1.z, c0.w, c1.w, x[b][j].z, x[b][j].w);
+        }
+    }
+  }
+  grid_dep_launch();
+  // accumulator: channels g (d0, d1) and g + 8 (d2, d3), tokens 2 t and 2 t + 1
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[warp][b * 8 + 2 * t + (i & 1)][g + (i >> 1) * 8] = d[b][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < NB * 8 * kFewCh; i += 32 * WARPS) {
+    const int row = i / kFewCh, n = n0 + i % kFewCh;
+    if (row >= p.rows || n >= p.n) continue;
+    int32_t sum = 0;
+#pragma unroll
+    for (int j = 0; j < WARPS; ++j) sum += part[j][row][i % kFewCh];
+    store_out(static_cast<T*>(p.out) + row * p.out_stride + n,
+              scaled(sum, p.a_scale[row], p.w_scale[n], p.bias ? p.bias[n] : 0.f));
+  }
+}
+
 // ---------------------------------------------------------------- host
 static int encode_codes(CUtensorMap* map, const void* base, int64_t width, int64_t rows, int64_t stride, int box_rows) {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -581,6 +688,27 @@ static int launch_linear(const LinParams& p, const CUtensorMap& amap, const CUte
   return after_launch("linear_int8_kernel");
 }
 
+// Up to 8 rows always (5 x 1536 x 17920: 5.7 us, 6.9 in the tcgen05 kernel); with more, each block reads
+// more of a, and the tcgen05 kernel is ahead once a block an SM does not cover the channels (16 x 1536 x
+// 17920: 8.8 and 7.1 us; 16 x 8960 x 1536: 6.0 and 6.8) or, past 16 rows, K is long (32 x 1536 x 2048: 3.4
+// and 5.0 us; 32 x 8960 x 1536: 8.2 and 7.5).
+static bool few_rows(int64_t rows, int width, int n) {
+  if (rows <= 8) return true;
+  return rows <= kFewRows && n <= kFewCh * device_sm_count() && (rows <= 16 || width <= 2048);
+}
+template <int NB, int WARPS, int AHEAD, typename T>
+static int launch_few_as(const FewParams& p, cudaStream_t st) {
+  return launch_pdl("linear_int8_few_kernel", linear_int8_few_kernel<NB, WARPS, AHEAD, T>,
+                    dim3(static_cast<unsigned>((p.n + kFewCh - 1) / kFewCh)), dim3(32 * WARPS), 0, st, p);
+}
+template <int NB, typename T>
+static int launch_few(const FewParams& p, cudaStream_t st) {
+  // a warp's share of K as far as it can be under way at once: 4 steps (K <= 2048), 5 or 9
+  if (p.width <= 8 * kFewAhead * kFewStep) return launch_few_as<NB, 8, 4, T>(p, st);
+  if (NB > 1 || p.width <= 16 * 5 * kFewStep) return launch_few_as<NB, 16, NB == 1 ? 5 : 4, T>(p, st);
+  return launch_few_as<1, 16, 9, T>(p, st);
+}
+
 }  // namespace sd
 
 using namespace sd;
@@ -608,6 +736,16 @@ extern "C" int specdec_linear_int8(const void* a, int64_t a_stride, const float*
     return fail(SPECDEC_ERR_INVALID, "linear_int8: the row strides of the codes must be multiples of 16");
   if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w)) & 15u)
     return fail(SPECDEC_ERR_INVALID, "linear_int8: the codes must be 16-byte aligned");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (few_rows(rows, width, out_features)) {
+    const FewParams f = {static_cast<const int8_t*>(a), static_cast<const int8_t*>(w), a_scale, w_scale, bias, out,
+                         a_stride, w_stride, out_stride, static_cast<int32_t>(rows), out_features, width, weight_ready};
+    if (out_dtype == SPECDEC_F32)
+      return rows <= 8 ? launch_few<1, float>(f, st) : rows <= 16 ? launch_few<2, float>(f, st) : launch_few<4, float>(f, st);
+    return rows <= 8    ? launch_few<1, __nv_bfloat16>(f, st)
+           : rows <= 16 ? launch_few<2, __nv_bfloat16>(f, st)
+                        : launch_few<4, __nv_bfloat16>(f, st);
+  }
   const int sms = device_sm_count();
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
@@ -640,7 +778,6 @@ extern "C" int specdec_linear_int8(const void* a, int64_t a_stride, const float*
   if (int rc = encode_codes(&amap, a, width, rows, a_stride, p.tokens / shape.cg)) return rc;
   if (int rc = encode_codes(&wmap, w, width, out_features, w_stride, kLinCh)) return rc;
   const int smem = p.stages * stage + 1024;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (shape.cg == 2) {
     const int grid = 2 * (p.units < sms / 2 ? p.units : sms / 2);
     return out_dtype == SPECDEC_F32 ? launch_linear<2, float>(p, amap, wmap, grid, smem, dev, st)
