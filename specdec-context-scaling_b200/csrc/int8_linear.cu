@@ -37,7 +37,7 @@ constexpr int kLinChunk = 128;                   // codes of K per stage
 constexpr int kLinCh = 128;                      // channels per CTA
 constexpr int kLinWTile = kLinCh * kLinChunk;    // 16 KB
 constexpr int kLinMaxStages = 12;
-constexpr int kLinRing = 216 * 1024;
+constexpr int kLinRing = 204 * 1024;
 constexpr int kLinMaxTokens = 256;
 
 struct LinParams {
@@ -50,7 +50,9 @@ struct LinParams {
   int32_t tokens;    // tokens of a tile (the MMA's N)
   int32_t ch_tiles;  // tiles along the channels
   int32_t units;     // tiles of the call
-  int32_t splits, stages, tmem_cols, weight_ready, vec_out;
+  int32_t splits, stages, tmem_cols, weight_ready;
+  int32_t vec_out;  // four outputs of a row can be stored at once
+  int32_t rows16;   // rows of the output are 16-byte aligned and whole 16-byte pieces
   int32_t* status;
 };
 
@@ -152,6 +154,24 @@ SD_DEV void tmem_wait_ld16(int32_t (&v)[16]) {
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
                  "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::"memory");
 }
+// 32 lanes x 16 columns as two halves of 16 lanes (16x256b): v[8 h + 4 j + 2 q + e] is lane
+// 16 h + 8 q + T / 4, column 8 j + 2 (T % 4) + e of thread T -- the fragments of 8 x 8 matrices that
+// stmatrix takes
+SD_DEV void tmem_ld_fragments(uint32_t ta, int32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(ta));
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(ta + (16u << 16)));
+}
+// four 8 x 8 matrices of 16-bit values, stored transposed: lane 8 i + k gives the address of column k of
+// matrix i
+SD_DEV void stmatrix_trans(uint32_t addr, uint32_t m0, uint32_t m1, uint32_t m2, uint32_t m3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(m0), "r"(m1),
+               "r"(m2), "r"(m3)
+               : "memory");
+}
 SD_DEV int4 dsmem_ld4_s32(uint32_t addr) {
   int4 v;
   asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
@@ -190,6 +210,37 @@ SD_DEV void store_tokens(const int32_t (&v)[16], const float* s_scale, float sw,
   }
 }
 
+// bf16 results of 32 channels x 16 tokens, held as fragments, to 64 consecutive bytes of each token's row
+// by way of 1 KB of shared memory: eight tokens a store instead of half of one, and 4.4 instructions a value
+// where one store a token took 11, which bound the kernel at short K (8192 x 896 x 9728:
+SD_DEV void store_fragments(const int32_t (&v)[16], const float* s_scale, const float (&sw)[4], const float (&bias)[4],
+                            uint8_t* stage, __nv_bfloat16* o, int64_t stride, int ntok, int nch) {
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  const float2 sa[2] = {*reinterpret_cast<const float2*>(s_scale + 2 * t),
+                        *reinterpret_cast<const float2*>(s_scale + 8 + 2 * t)};
+  __syncwarp();  // the stage's previous contents are read
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t m[4];  // (tokens 0-7, channels 0-7), (tokens 0-7, channels 8-15), then tokens 8-15
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        m[2 * j + q] = pack_bf16(scaled(v[8 * h + 4 * j + 2 * q], sa[j].x, sw[2 * h + q], bias[2 * h + q]),
+                                 scaled(v[8 * h + 4 * j + 2 * q + 1], sa[j].y, sw[2 * h + q], bias[2 * h + q]));
+    // rows of 64 bytes, 16-byte chunk c of token k at chunk c ^ (k / 2 % 4): no bank conflicts either way
+    const int token = (lane >> 4) * 8 + (lane & 7), chunk = 2 * h + ((lane >> 3) & 1);
+    stmatrix_trans(smem_u32(stage + token * 64 + ((chunk ^ ((token >> 1) & 3)) << 4)), m[0], m[1], m[2], m[3]);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int token = 8 * j + (lane >> 2);
+    const uint4 row = *reinterpret_cast<const uint4*>(stage + token * 64 + ((t ^ ((token >> 1) & 3)) << 4));
+    if (token < ntok && 8 * t < nch) *reinterpret_cast<uint4*>(o + token * stride + 8 * t) = row;
+  }
+}
+
 // ---------------------------------------------------------------- the kernel
 template <int CG, typename T>
 __global__ void __launch_bounds__(kLinThreads, 1)
@@ -200,6 +251,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   __shared__ uint64_t full[kLinMaxStages], empty[kLinMaxStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
   __shared__ __align__(16) float s_scale[kLinEpiWarps][kLinMaxTokens / 2];
+  __shared__ __align__(128) uint8_t s_stage[kLinEpiWarps][1024];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int csize = CG == 2 ? 2 : p.splits;
   const int rank = csize > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -345,11 +397,17 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       const int b = ui & 1;
       const int n = (ct * CG + (CG == 2 ? rank : 0)) * kLinCh + quarter * 32 + lane;
       const int tok0 = tt * p.tokens, ntok = min(p.tokens, p.rows - tok0);
-      float sw = 0.f, bias = 0.f;
+      // fragments: this thread's channels are T / 4 + {0, 8, 16, 24} of the quarter's, else lane T's
+      const bool fragments = sizeof(T) == 2 && p.rows16;
+      float sw[4] = {}, bias[4] = {};
       if (p.splits == 1) {
-        if (n < p.n) {
-          sw = p.w_scale[n];
-          if (p.bias) bias = p.bias[n];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int nj = fragments ? n - lane + (lane >> 2) + 8 * j : n;
+          if ((fragments || j == 0) && nj < p.n) {
+            sw[j] = p.w_scale[nj];
+            if (p.bias) bias[j] = p.bias[nj];
+          }
         }
         __syncwarp();
         for (int c = c0 + lane; c < min(c1, ntok); c += 32) s_scale[warp][c - c0] = p.a_scale[tok0 + c];
@@ -361,7 +419,25 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       }
       umma::fence_after_sync();
       const uint32_t ta = umma::taddr(tbase, quarter * 32, b * (p.tmem_cols / 2));
-      if (p.splits == 1) {
+      if (p.splits == 1 && fragments) {
+        if constexpr (sizeof(T) == 2) {
+          T* o = out + (tok0 + c0) * p.out_stride + (n - lane);
+          int32_t v[2][16];
+          if (c0 < c1) tmem_ld_fragments(ta + c0, v[0]);
+#pragma unroll 1
+          for (int c = c0; c < c1; c += 32) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int cc = c + 16 * h;
+              if (cc >= c1) break;
+              tmem_wait_ld16(v[h]);
+              if (cc + 16 < c1) tmem_ld_fragments(ta + cc + 16, v[1 - h]);
+              store_fragments(v[h], &s_scale[warp][cc - c0], sw, bias, s_stage[warp], o + (cc - c0) * p.out_stride,
+                              p.out_stride, ntok - cc, p.n - (n - lane));
+            }
+          }
+        }
+      } else if (p.splits == 1) {
         T* o = out + (tok0 + c0) * p.out_stride + n;
         const bool whole = c1 <= ntok && n - lane + 32 <= p.n;
         const int mine = n < p.n ? ntok : 0;  // tokens this lane stores
@@ -378,9 +454,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             if (cc + 16 < c1) tmem_ld16_s32(ta + cc + 16, v[1 - h]);
             T* oc = o + (cc - c0) * p.out_stride;
             if (whole)
-              store_tokens<T, false>(v[h], &s_scale[warp][cc - c0], sw, bias, oc, p.out_stride, 16);
+              store_tokens<T, false>(v[h], &s_scale[warp][cc - c0], sw[0], bias[0], oc, p.out_stride, 16);
             else
-              store_tokens<T, true>(v[h], &s_scale[warp][cc - c0], sw, bias, oc, p.out_stride, mine - cc);
+              store_tokens<T, true>(v[h], &s_scale[warp][cc - c0], sw[0], bias[0], oc, p.out_stride, mine - cc);
           }
         }
       } else {
@@ -770,6 +846,7 @@ extern "C" int specdec_linear_int8(const void* a, int64_t a_stride, const float*
   p.status = status;
   const int esize = out_dtype == SPECDEC_F32 ? 4 : 2;
   p.vec_out = (reinterpret_cast<uintptr_t>(out) % (4 * esize)) == 0 && out_stride % 4 == 0;
+  p.rows16 = (reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(out_stride * esize) | static_cast<uintptr_t>(out_features) * esize) % 16 == 0;
   const int stage = kLinWTile + p.tokens / shape.cg * kLinChunk;
   p.stages = kLinRing / stage < kLinMaxStages ? kLinRing / stage : kLinMaxStages;
   p.tmem_cols = 32;
