@@ -210,14 +210,32 @@ SD_DEV void store_tokens(const int32_t (&v)[16], const float* s_scale, float sw,
   }
 }
 
+// two fp32 products / sums at once (sm_100's packed arithmetic; each is the scalar operation's result)
+SD_DEV uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+SD_DEV uint32_t scaled_pair(int32_t a0, int32_t a1, uint64_t sa, uint64_t sw, uint64_t bias) {
+  uint64_t y = pair_of(static_cast<float>(a0), static_cast<float>(a1));
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(y) : "l"(sa));
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(y) : "l"(sw), "l"(bias));
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(y));
+  return pack_bf16(lo, hi);
+}
+
 // bf16 results of 32 channels x 16 tokens, held as fragments, to 64 consecutive bytes of each token's row
-// by way of 1 KB of shared memory: eight tokens a store instead of half of one, and 4.4 instructions a value
-// where one store a token took 11, which bound the kernel at short K (8192 x 896 x 9728:
-SD_DEV void store_fragments(const int32_t (&v)[16], const float* s_scale, const float (&sw)[4], const float (&bias)[4],
-                            uint8_t* stage, __nv_bfloat16* o, int64_t stride, int ntok, int nch) {
+// by way of 1 KB of shared memory: eight tokens a store instead of half of one.  `put`: this lane's
+// address for stmatrix, `get`: for reading back; o: this lane's 16 bytes of tokens lane / 4 and, `half`
+// further, lane / 4 + 8.  At short K it is the issue of these instructions that bounds the kernel.
+template <bool GUARD>
+SD_DEV void store_fragments(const int32_t (&v)[16], const float* s_scale, const uint64_t (&sw)[4],
+                            const uint64_t (&bias)[4], uint32_t put, const uint8_t* get, uint8_t* o, int64_t half,
+                            int ntok, bool ch_ok) {
   const int lane = threadIdx.x & 31, t = lane & 3;
-  const float2 sa[2] = {*reinterpret_cast<const float2*>(s_scale + 2 * t),
-                        *reinterpret_cast<const float2*>(s_scale + 8 + 2 * t)};
+  const uint64_t sa[2] = {*reinterpret_cast<const uint64_t*>(s_scale + 2 * t),
+                          *reinterpret_cast<const uint64_t*>(s_scale + 8 + 2 * t)};
   __syncwarp();  // the stage's previous contents are read
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -226,19 +244,14 @@ SD_DEV void store_fragments(const int32_t (&v)[16], const float* s_scale, const 
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int q = 0; q < 2; ++q)
-        m[2 * j + q] = pack_bf16(scaled(v[8 * h + 4 * j + 2 * q], sa[j].x, sw[2 * h + q], bias[2 * h + q]),
-                                 scaled(v[8 * h + 4 * j + 2 * q + 1], sa[j].y, sw[2 * h + q], bias[2 * h + q]));
-    // rows of 64 bytes, 16-byte chunk c of token k at chunk c ^ (k / 2 % 4): no bank conflicts either way
-    const int token = (lane >> 4) * 8 + (lane & 7), chunk = 2 * h + ((lane >> 3) & 1);
-    stmatrix_trans(smem_u32(stage + token * 64 + ((chunk ^ ((token >> 1) & 3)) << 4)), m[0], m[1], m[2], m[3]);
+        m[2 * j + q] = scaled_pair(v[8 * h + 4 * j + 2 * q], v[8 * h + 4 * j + 2 * q + 1], sa[j], sw[2 * h + q],
+                                   bias[2 * h + q]);
+    stmatrix_trans(put ^ (h * 32u), m[0], m[1], m[2], m[3]);
   }
   __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int token = 8 * j + (lane >> 2);
-    const uint4 row = *reinterpret_cast<const uint4*>(stage + token * 64 + ((t ^ ((token >> 1) & 3)) << 4));
-    if (token < ntok && 8 * t < nch) *reinterpret_cast<uint4*>(o + token * stride + 8 * t) = row;
-  }
+  const uint4 r0 = *reinterpret_cast<const uint4*>(get), r1 = *reinterpret_cast<const uint4*>(get + 512);
+  if (!GUARD || (ch_ok && (lane >> 2) < ntok)) *reinterpret_cast<uint4*>(o) = r0;
+  if (!GUARD || (ch_ok && (lane >> 2) + 8 < ntok)) *reinterpret_cast<uint4*>(o + half) = r1;
 }
 
 // ---------------------------------------------------------------- the kernel
@@ -391,37 +404,63 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     T* out = static_cast<T*>(p.out);
     const int quarter = warp & 3, batches = p.tokens / 16;
     const int c0 = (warp >> 2) * (batches / 2) * 16, c1 = warp >= 4 ? p.tokens : batches / 2 * 16;
+    // fragments: this thread's channels are T / 4 + {0, 8, 16, 24} of the quarter's, else lane T's
+    const bool fragments = sizeof(T) == 2 && p.rows16;
+    // lane 8 i + k of stmatrix stores token 8 (i / 2) + k, 16-byte chunk i % 2 (+ 2 in the second half) of its
+    // 64 bytes, at chunk c ^ (token / 2 % 4): no bank conflicts either way
+    const int put_token = (lane >> 4) * 8 + (lane & 7);
+    const uint32_t put = smem_u32(s_stage[warp]) + put_token * 64 + ((((lane >> 3) & 1) ^ ((put_token >> 1) & 3)) << 4);
+    const uint8_t* get = s_stage[warp] + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+    int tt = unit0 / p.ch_tiles, ct = unit0 - tt * p.ch_tiles;
+    const int step_tt = unit_step / p.ch_tiles, step_ct = unit_step - step_tt * p.ch_tiles;
+    // a tile's scales are loaded while the tile before it is worked on
+    float sw_next[4], bias_next[4], sa_next[4];
+    const auto load_scales = [&]() {
+      const int nq = (ct * CG + (CG == 2 ? rank : 0)) * kLinCh + quarter * 32;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int nj = fragments ? nq + (lane >> 2) + 8 * j : nq + lane, c = c0 + lane + 32 * j;
+        const bool used = nj < p.n && (fragments || j == 0);
+        sw_next[j] = used ? p.w_scale[nj] : 0.f;
+        bias_next[j] = used && p.bias ? p.bias[nj] : 0.f;
+        sa_next[j] = c < c1 && tt * p.tokens + c < p.rows ? p.a_scale[tt * p.tokens + c] : 0.f;
+      }
+    };
+    if (p.splits == 1 && unit0 < p.units) load_scales();
     int ui = 0;
     for (int u = unit0; u < p.units; u += unit_step, ++ui) {
-      const int tt = u / p.ch_tiles, ct = u - tt * p.ch_tiles;
       const int b = ui & 1;
-      const int n = (ct * CG + (CG == 2 ? rank : 0)) * kLinCh + quarter * 32 + lane;
+      const int nq = (ct * CG + (CG == 2 ? rank : 0)) * kLinCh + quarter * 32, n = nq + lane;
       const int tok0 = tt * p.tokens, ntok = min(p.tokens, p.rows - tok0);
-      // fragments: this thread's channels are T / 4 + {0, 8, 16, 24} of the quarter's, else lane T's
-      const bool fragments = sizeof(T) == 2 && p.rows16;
-      float sw[4] = {}, bias[4] = {};
-      if (p.splits == 1) {
+      const float sw0 = sw_next[0], bias0 = bias_next[0];
+      uint64_t sw[4], bias[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int nj = fragments ? n - lane + (lane >> 2) + 8 * j : n;
-          if ((fragments || j == 0) && nj < p.n) {
-            sw[j] = p.w_scale[nj];
-            if (p.bias) bias[j] = p.bias[nj];
-          }
-        }
-        __syncwarp();
-        for (int c = c0 + lane; c < min(c1, ntok); c += 32) s_scale[warp][c - c0] = p.a_scale[tok0 + c];
+      for (int j = 0; j < 4; ++j) {
+        sw[j] = pair_of(sw_next[j], sw_next[j]);
+        bias[j] = pair_of(bias_next[j], bias_next[j]);
+      }
+      if (p.splits == 1) {
+        __syncwarp();  // the previous tile's scales are read
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s_scale[warp][lane + 32 * j] = sa_next[j];
         __syncwarp();
       }
+      tt += step_tt;
+      ct += step_ct;
+      if (ct >= p.ch_tiles) ct -= p.ch_tiles, ++tt;
+      if (p.splits == 1 && u + unit_step < p.units) load_scales();
       if (!warp_wait(&acc_full[b], (ui >> 1) & 1)) {
         if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
         break;
       }
       umma::fence_after_sync();
       const uint32_t ta = umma::taddr(tbase, quarter * 32, b * (p.tmem_cols / 2));
+      const bool whole = c1 <= ntok && nq + 32 <= p.n;
       if (p.splits == 1 && fragments) {
         if constexpr (sizeof(T) == 2) {
-          T* o = out + (tok0 + c0) * p.out_stride + (n - lane);
+          uint8_t* o = reinterpret_cast<uint8_t*>(out + (tok0 + c0 + (lane >> 2)) * p.out_stride + nq + 8 * (lane & 3));
+          const int64_t half = 8 * p.out_stride * static_cast<int64_t>(sizeof(T));
+          const bool ch_ok = nq + 8 * (lane & 3) < p.n;
           int32_t v[2][16];
           if (c0 < c1) tmem_ld_fragments(ta + c0, v[0]);
 #pragma unroll 1
@@ -431,17 +470,20 @@ __global__ void __launch_bounds__(kLinThreads, 1)
               const int cc = c + 16 * h;
               if (cc >= c1) break;
               tmem_wait_ld16(v[h]);
+              // the next 16 columns are on their way while these are scaled and stored
               if (cc + 16 < c1) tmem_ld_fragments(ta + cc + 16, v[1 - h]);
-              store_fragments(v[h], &s_scale[warp][cc - c0], sw, bias, s_stage[warp], o + (cc - c0) * p.out_stride,
-                              p.out_stride, ntok - cc, p.n - (n - lane));
+              const float* sa = &s_scale[warp][cc - c0];
+              if (whole)
+                store_fragments<false>(v[h], sa, sw, bias, put, get, o, half, 16, true);
+              else
+                store_fragments<true>(v[h], sa, sw, bias, put, get, o, half, ntok - cc, ch_ok);
+              o += 2 * half;
             }
           }
         }
       } else if (p.splits == 1) {
         T* o = out + (tok0 + c0) * p.out_stride + n;
-        const bool whole = c1 <= ntok && n - lane + 32 <= p.n;
         const int mine = n < p.n ? ntok : 0;  // tokens this lane stores
-        // the next 16 columns are on their way while these are scaled and stored
         int32_t v[2][16];
         if (c0 < c1) tmem_ld16_s32(ta + c0, v[0]);
 #pragma unroll 1
@@ -454,9 +496,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             if (cc + 16 < c1) tmem_ld16_s32(ta + cc + 16, v[1 - h]);
             T* oc = o + (cc - c0) * p.out_stride;
             if (whole)
-              store_tokens<T, false>(v[h], &s_scale[warp][cc - c0], sw[0], bias[0], oc, p.out_stride, 16);
+              store_tokens<T, false>(v[h], &s_scale[warp][cc - c0], sw0, bias0, oc, p.out_stride, 16);
             else
-              store_tokens<T, true>(v[h], &s_scale[warp][cc - c0], sw[0], bias[0], oc, p.out_stride, mine - cc);
+              store_tokens<T, true>(v[h], &s_scale[warp][cc - c0], sw0, bias0, oc, p.out_stride, mine - cc);
           }
         }
       } else {
