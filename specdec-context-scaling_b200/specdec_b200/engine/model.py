@@ -17,6 +17,13 @@ Per layer of a decode / verify step (rows = packed query rows of all sequences):
 Prefill (the whole prompt at once) uses torch's fused causal attention for the
 prompt block and appends the prompt's K/V into the pages; decode never does.
 
+With ``weights="int8"`` the projections run on 8-bit weights and activations (one scale for
+each output channel and each token), in a decode / verify step and in the prompt pass:
+  x (+ the previous projection), int8(rmsnorm(x))  specdec_rmsnorm_int8
+  qkv, o, gate|up and down projections             specdec_linear_int8
+  int8(o), int8(silu(gate) up)                     specdec_quantize_int8, specdec_swiglu_int8
+Attention, the cache, the embedding and the LM head are the same as with bf16 weights.
+
 Weights come from a state dict with the reference's parameter names
 (``embed_tokens.weight``, ``layers.{i}.self_attn.q_proj.weight`` ...), so a
 reference QwenLM's weights load directly, or from a seeded random init.
@@ -92,12 +99,32 @@ def _e4m3_round_trip(v: torch.Tensor) -> torch.Tensor:
 
 
 @dataclass
+class Int8Linear:
+    """A projection's weight as int8 codes with one f32 scale for each output channel; applied to int8 rows."""
+
+    codes: torch.Tensor  # int8 (out_features, width), rows on 16-byte boundaries
+    scale: torch.Tensor  # f32 (out_features,)
+    bias: torch.Tensor | None  # f32 (out_features,)
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor, bias: torch.Tensor | None = None) -> "Int8Linear":
+        """Quantise a (out_features, width) weight.  The weight is final on every stream when this returns, so
+        a call may load it ahead of the work before it (``weight_ready``)."""
+        codes, scale = ops.quantize_int8(weight)
+        torch.cuda.current_stream(weight.device).synchronize()
+        return cls(codes, scale, None if bias is None else bias.float())
+
+    def __call__(self, codes: torch.Tensor, scale: torch.Tensor, status: torch.Tensor | None = None) -> torch.Tensor:
+        return ops.linear_int8(codes, scale, self.codes, self.scale, bias=self.bias, weight_ready=True, status=status)
+
+
+@dataclass
 class _Layer:
-    w_qkv: torch.Tensor
+    w_qkv: torch.Tensor | Int8Linear
     b_qkv: torch.Tensor | None
-    w_o: torch.Tensor
-    w_gu: torch.Tensor  # gate_proj and up_proj stacked: (2 inter, hidden)
-    w_down: torch.Tensor
+    w_o: torch.Tensor | Int8Linear
+    w_gu: torch.Tensor | Int8Linear  # gate_proj and up_proj stacked: (2 inter, hidden)
+    w_down: torch.Tensor | Int8Linear
     ln1: torch.Tensor
     ln2: torch.Tensor
 
@@ -139,8 +166,11 @@ class StepLayout:
 class PagedModel:
     """Decoder weights in fused, layout-ready form plus the batched paged forward."""
 
-    def __init__(self, cfg: ModelConfig, state: dict, device="cuda", dtype=torch.bfloat16):
+    def __init__(self, cfg: ModelConfig, state: dict, device="cuda", dtype=torch.bfloat16, *, weights: str = "bf16"):
+        if weights not in ("bf16", "int8"):
+            raise ValueError(f"weights must be 'bf16' or 'int8', got {weights!r}")
         self.cfg = cfg
+        self.int8 = weights == "int8"
         self.device = torch.device(device)
 
         def get(k):
@@ -156,6 +186,13 @@ class PagedModel:
             b_qkv = None
             if (a + "q_proj.bias") in state:
                 b_qkv = torch.cat([get(a + "q_proj.bias"), get(a + "k_proj.bias"), get(a + "v_proj.bias")])
+            if self.int8:
+                self.layers.append(_Layer(
+                    Int8Linear.from_weight(w_qkv, b_qkv), None, Int8Linear.from_weight(get(a + "o_proj.weight")),
+                    Int8Linear.from_weight(torch.cat([get(p + "mlp.gate_proj.weight"), get(p + "mlp.up_proj.weight")])),
+                    Int8Linear.from_weight(get(p + "mlp.down_proj.weight")),
+                    get(p + "input_layernorm.weight"), get(p + "post_attention_layernorm.weight")))
+                continue
             self.layers.append(_Layer(w_qkv.contiguous(), None if b_qkv is None else b_qkv.contiguous(),
                                       get(a + "o_proj.weight"),
                                       torch.cat([get(p + "mlp.gate_proj.weight"), get(p + "mlp.up_proj.weight")]),
@@ -165,8 +202,8 @@ class PagedModel:
                                                                dtype=torch.float32) / cfg.head_dim))
 
     @classmethod
-    def random(cls, cfg: ModelConfig, seed: int, device="cuda") -> "PagedModel":
-        return cls(cfg, random_state(cfg, seed, device), device)
+    def random(cls, cfg: ModelConfig, seed: int, device="cuda", *, weights: str = "bf16") -> "PagedModel":
+        return cls(cfg, random_state(cfg, seed, device), device, weights=weights)
 
     def new_cache(self, num_seqs: int, capacity: int, v_dtype: str = "bf16") -> PagedKVCache:
         c = self.cfg
@@ -183,9 +220,12 @@ class PagedModel:
 
     def _qkv(self, L: _Layer, h: torch.Tensor, cos, sin):
         """Packed rows -> q (1, H, rows, D) and k (1, KV, rows, D) after RoPE, v (KV, rows, D)."""
-        c = self.cfg
-        rows = h.shape[0]
         qkv = torch.addmm(L.b_qkv, h, L.w_qkv.t()) if L.b_qkv is not None else h @ L.w_qkv.t()
+        return self._split_qkv(qkv, cos, sin)
+
+    def _split_qkv(self, qkv: torch.Tensor, cos, sin):
+        c = self.cfg
+        rows = qkv.shape[0]
         qkv = qkv.view(rows, c.heads + 2 * c.kv_heads, c.head_dim)
         q = ops.apply_rope(qkv[:, :c.heads].transpose(0, 1).unsqueeze(0), cos, sin)
         k = ops.apply_rope(qkv[:, c.heads:c.heads + c.kv_heads].transpose(0, 1).unsqueeze(0), cos, sin)
@@ -197,6 +237,18 @@ class PagedModel:
         added by the down GEMM (in place on x)."""
         h = ops.rmsnorm(x, L.ln2, self.cfg.eps)
         return x.addmm_(ops.swiglu_packed(h @ L.w_gu.t()), L.w_down.t())
+
+    def _mlp_int8(self, L: _Layer, x: torch.Tensor, delta: torch.Tensor, status=None) -> torch.Tensor:
+        """x += delta (the attention's projection) in place; returns down(silu(gate(h)) * up(h)), h = rmsnorm(x),
+        which the next norm adds to x."""
+        codes, scale, _ = ops.rmsnorm_int8(x, L.ln2, self.cfg.eps, residual=delta, summed=x)
+        return L.w_down(*ops.swiglu_int8(L.w_gu(codes, scale, status)), status)
+
+    def _norm_int8(self, L: _Layer, x: torch.Tensor, delta: torch.Tensor | None):
+        """x += delta (the previous layer's MLP; None in the first layer) in place; int8(rmsnorm(x))."""
+        codes, scale, _ = ops.rmsnorm_int8(x, L.ln1, self.cfg.eps, residual=delta,
+                                           summed=None if delta is None else x)
+        return codes, scale
 
     def logits(self, hidden_rows: torch.Tensor) -> torch.Tensor:
         """Tied LM head (model_self.py:857): (n, hidden) -> (n, vocab)."""
@@ -223,9 +275,13 @@ class PagedModel:
         # attention writes every row of each sequence's q_len; padding rows stay unset
         # (meaningless, never stored, never mixed into other rows)
         o = torch.empty(rows, c.heads, c.head_dim, dtype=x.dtype, device=x.device)
+        delta = None  # int8: the previous layer's MLP output, added to x by the next norm
         for li, L in enumerate(self.layers):
-            h = ops.rmsnorm(x, L.ln1, c.eps)
-            qkv = torch.addmm(L.b_qkv, h, L.w_qkv.t()) if L.b_qkv is not None else h @ L.w_qkv.t()
+            if self.int8:
+                qkv = L.w_qkv(*self._norm_int8(L, x, delta), status)
+            else:
+                h = ops.rmsnorm(x, L.ln1, c.eps)
+                qkv = torch.addmm(L.b_qkv, h, L.w_qkv.t()) if L.b_qkv is not None else h @ L.w_qkv.t()
             # rotated q, and rotated k + v appended to the cache, in one launch
             ops.rope_append(qkv.view(rows, c.heads + 2 * c.kv_heads, c.head_dim), cos, sin, cache, li,
                             num_q_heads=c.heads, row0=layout.q_row0, n_new=layout.q_len, pos0=layout.pos0,
@@ -234,8 +290,14 @@ class PagedModel:
             # is this step's new tokens, so the history may be loaded early
             ops.paged_attention(q, cache, li, layout.batch, out=o, workspace=workspace, reuse_plan=li > 0,
                                 status=status, history_ready=li > 0)
-            x.addmm_(o.view(rows, c.heads * c.head_dim), L.w_o.t())
-            x = self._mlp(L, x)
+            if self.int8:
+                delta = L.w_o(*ops.quantize_int8(o.view(rows, c.heads * c.head_dim)), status)
+                delta = self._mlp_int8(L, x, delta, status)
+            else:
+                x.addmm_(o.view(rows, c.heads * c.head_dim), L.w_o.t())
+                x = self._mlp(L, x)
+        if delta is not None:
+            x.add_(delta)
         return ops.rmsnorm(x, self.norm, c.eps)
 
     def prefill(self, ids: torch.Tensor, cache: PagedKVCache, seq0: int, *, need_logits: bool = True,
@@ -257,9 +319,12 @@ class PagedModel:
         x = self.embed[ids.reshape(-1).long()]
         cos, sin = self._cos_sin(torch.arange(P, device=dev).repeat(n))
         n_rep = c.heads // c.kv_heads
+        delta = None
         for li, L in enumerate(self.layers):
-            h = ops.rmsnorm(x, L.ln1, c.eps)
-            q, k, v = self._qkv(L, h, cos, sin)
+            if self.int8:
+                q, k, v = self._split_qkv(L.w_qkv(*self._norm_int8(L, x, delta), status), cos, sin)
+            else:
+                q, k, v = self._qkv(L, ops.rmsnorm(x, L.ln1, c.eps), cos, sin)
             ops.append_kv(k[0].transpose(0, 1), v.transpose(0, 1), cache, li, row0=row0, n_new=n_new, pos0=pos0,
                           max_new=P, status=status)
             if cache.v_dtype == "e4m3":
@@ -271,11 +336,17 @@ class PagedModel:
             k4 = k[0].view(c.kv_heads, n, P, c.head_dim).transpose(0, 1).repeat_interleave(n_rep, dim=1)
             v4 = v.view(c.kv_heads, n, P, c.head_dim).transpose(0, 1).repeat_interleave(n_rep, dim=1)
             o = F.scaled_dot_product_attention(q4, k4, v4, is_causal=True, scale=1.0 / math.sqrt(c.head_dim))
-            x = x + o.transpose(1, 2).reshape(rows, c.heads * c.head_dim) @ L.w_o.t()
-            x = self._mlp(L, x)
+            o = o.transpose(1, 2).reshape(rows, c.heads * c.head_dim)
+            if self.int8:
+                delta = self._mlp_int8(L, x, L.w_o(*ops.quantize_int8(o), status), status)
+            else:
+                x = x + o @ L.w_o.t()
+                x = self._mlp(L, x)
         cache.lengths.copy_(torch.where(inside, torch.full_like(seqs, P), cache.lengths))
         cache.host_lengths = None
         if not need_logits:
             return None
+        if delta is not None:
+            x.add_(delta)
         last = x.view(n, P, -1)[:, -1]
         return self.logits(ops.rmsnorm(last.contiguous(), self.norm, c.eps))

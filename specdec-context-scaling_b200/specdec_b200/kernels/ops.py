@@ -554,35 +554,68 @@ def trim_lengths(cur_len, new_len, out=None, status=None):
 
 
 # ---------------------------------------------------------------------------- 8-bit linear path
-def _raw_stream(t: torch.Tensor) -> int:
-    """The current stream of ``t``'s device, which has to be the current device."""
-    if not t.is_cuda:
-        raise RuntimeError("tensors must be CUDA")
+# These calls take a few microseconds of GPU time each in a decode step, so their checks read every
+# attribute once and the library and stream are looked up directly.
+_BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
+_int8_lib = None
+
+
+def _int8_call(t: torch.Tensor):
+    """(library, device index, its current stream) for a call on ``t``, whose device has to be the current one."""
+    global _int8_lib
     dev = t.get_device()
+    if dev < 0:
+        raise RuntimeError("tensors must be CUDA")
     if dev != torch._C._cuda_getDevice():
         raise RuntimeError(f"tensor is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch._C._cuda_getCurrentRawStream(dev)
+    if _int8_lib is None:
+        _int8_lib = _lib_handle()
+    return _int8_lib, dev, torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _int8_rows_out(x: torch.Tensor, width: int, codes, scale):
-    """Check ``x`` (rows, .) f32 / bf16; its dtype code and the codes (rows, width) and scale (rows,)
-    to write.  New codes have a row stride that is a multiple of 16 bytes, as linear_int8 reads them."""
-    code = _dtype_code(x)
-    if code < 0 or x.dim() != 2 or x.stride(1) != 1 and x.shape[1] != 1:
-        raise ValueError("x must be (rows, width) float32 or bfloat16 with contiguous columns")
-    rows = x.shape[0]
+def _on_device(dev: int, *tensors) -> None:
+    for t in tensors:
+        if t.get_device() != dev:
+            raise RuntimeError("tensors must be CUDA, all on one device")
+
+
+def _rows_of(x: torch.Tensor, what: str):
+    """(dtype code, rows, width, row stride) of f32 / bf16 rows with contiguous columns."""
+    dt = x.dtype
+    code = _lib.BF16 if dt is _BF16 else _lib.F32 if dt is _F32 else -1
+    if code < 0 or x.dim() != 2:
+        raise ValueError(f"{what} must be 2-D float32 or bfloat16")
+    rows, width = x.shape
+    st, sc = x.stride()
+    if sc != 1 and width != 1:
+        raise ValueError(f"{what} must have contiguous columns")
+    return code, rows, width, st if rows != 1 else width
+
+
+def _int8_out(x, dev: int, rows: int, width: int, codes, scale):
+    """The codes (rows, width), their row stride and the scale (rows,) to write.  New codes have a row
+    stride that is a multiple of 16 bytes, as linear_int8 reads them."""
     if codes is None:
         stride = (width + 15) & ~15
-        codes = torch.empty((rows, stride), dtype=torch.int8, device=x.device)
+        codes = x.new_empty((rows, stride), dtype=_I8)
         if stride != width:
             codes = codes[:, :width]
-    elif codes.dtype != torch.int8 or codes.shape != (rows, width) or codes.stride(1) != 1 or not codes.is_cuda:
-        raise ValueError("codes must be int8 (rows, width) with contiguous columns")
+    else:
+        _on_device(dev, codes)
+        if codes.dtype is not _I8 or codes.shape != (rows, width) or codes.stride(1) != 1 and width != 1:
+            raise ValueError("codes must be int8 (rows, width) with contiguous columns")
+        stride = codes.stride(0) if rows != 1 else width
     if scale is None:
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    elif scale.dtype != torch.float32 or scale.shape != (rows,) or not scale.is_contiguous() or not scale.is_cuda:
-        raise ValueError("scale must be contiguous float32 (rows,)")
-    return code, codes, scale
+        scale = x.new_empty(rows, dtype=_F32)
+    else:
+        _check_scale(scale, dev, rows, "scale")
+    return codes, stride, scale
+
+
+def _check_scale(scale, dev: int, n: int, what: str) -> None:
+    _on_device(dev, scale)
+    if scale.dtype is not _F32 or scale.dim() != 1 or scale.shape[0] != n or not scale.is_contiguous():
+        raise ValueError(f"{what} must be contiguous float32 ({n},)")
 
 
 def quantize_int8(x, *, codes=None, scale=None):
@@ -590,74 +623,98 @@ def quantize_int8(x, *, codes=None, scale=None):
     m = max(max|x|, 2^-100), scale = m / 127, code = rint(x * (127 / m)).  Returns (codes, scale);
     a row with an infinity or a NaN gets scale NaN and codes 0.  Rows of a weight (out_features,
     width) give the codes and the per-channel scale that ``linear_int8`` takes."""
-    stream = _raw_stream(x)
-    code, codes, scale = _int8_rows_out(x, x.shape[-1], codes, scale)
-    rows, width = x.shape
-    rc = _lib_handle().specdec_quantize_int8(x.data_ptr(), x.stride(0), codes.data_ptr(), codes.stride(0),
-                                             scale.data_ptr(), code, rows, width, stream)
-    _lib.check(rc, "quantize_int8")
+    lib, dev, stream = _int8_call(x)
+    code, rows, width, xs = _rows_of(x, "x")
+    codes, cs, scale = _int8_out(x, dev, rows, width, codes, scale)
+    rc = lib.specdec_quantize_int8(x.data_ptr(), xs, codes.data_ptr(), cs, scale.data_ptr(), code, rows, width, stream)
+    if rc:
+        _lib.check(rc, "quantize_int8")
     return codes, scale
 
 
 def rmsnorm_int8(x, weight, eps: float = 1e-6, *, residual=None, summed=None, codes=None, scale=None):
     """s = x + residual (s = x without one), then int8 rows of s / sqrt(mean(s^2) + eps) * weight,
     all in fp32 from the unrounded sum.  Returns (codes, scale, summed): ``summed`` is s in x's dtype
-    (None without a residual); it may be given as x or residual, to update that in place."""
-    stream = _raw_stream(x)
-    code, codes, scale = _int8_rows_out(x, x.shape[-1], codes, scale)
-    rows, hidden = x.shape
-    if weight.dtype != x.dtype or weight.shape != (hidden,) or not weight.is_contiguous() or not weight.is_cuda:
+    (None without a residual); it may be given as x or residual, to update that in place.  A row whose
+    sum of squares passes fp32's largest number counts as not finite (scale NaN, codes 0)."""
+    lib, dev, stream = _int8_call(x)
+    code, rows, hidden, xs = _rows_of(x, "x")
+    if weight.dtype is not x.dtype or weight.dim() != 1 or weight.shape[0] != hidden or not weight.is_contiguous():
         raise ValueError("weight must be contiguous (hidden,) of x's dtype")
     r_ptr = s_ptr = None
-    r_stride = s_stride = hidden
-    if residual is not None:
+    rs = ss = hidden
+    if residual is None:
+        if summed is not None:
+            raise ValueError("summed is written only with a residual")
+        _on_device(dev, weight)
+    else:
         if summed is None:  # rows on 16-byte boundaries, so the next call on it reads aligned rows
-            stride = (hidden + 7) & ~7
-            summed = x.new_empty((rows, stride))
-            if stride != hidden:
+            ss = (hidden + 7) & ~7
+            summed = x.new_empty((rows, ss))
+            if ss != hidden:
                 summed = summed[:, :hidden]
-        for t in (residual, summed):
-            if t.dtype != x.dtype or t.shape != x.shape or t.stride(1) != 1 and hidden != 1 or not t.is_cuda:
-                raise ValueError("residual and summed must be (rows, hidden) of x's dtype with contiguous columns")
-        r_ptr, r_stride, s_ptr, s_stride = residual.data_ptr(), residual.stride(0), summed.data_ptr(), summed.stride(0)
-    elif summed is not None:
-        raise ValueError("summed is written only with a residual")
-    rc = _lib_handle().specdec_rmsnorm_int8(x.data_ptr(), x.stride(0), r_ptr, r_stride, weight.data_ptr(), eps, s_ptr,
-                                            s_stride, codes.data_ptr(), codes.stride(0), scale.data_ptr(), code, rows,
-                                            hidden, stream)
-    _lib.check(rc, "rmsnorm_int8")
+        else:
+            ss = _like_x(summed, x)
+        rs = _like_x(residual, x)
+        _on_device(dev, weight, residual, summed)
+        r_ptr, s_ptr = residual.data_ptr(), summed.data_ptr()
+    codes, cs, scale = _int8_out(x, dev, rows, hidden, codes, scale)
+    rc = lib.specdec_rmsnorm_int8(x.data_ptr(), xs, r_ptr, rs, weight.data_ptr(), eps, s_ptr, ss, codes.data_ptr(), cs,
+                                  scale.data_ptr(), code, rows, hidden, stream)
+    if rc:
+        _lib.check(rc, "rmsnorm_int8")
     return codes, scale, summed
+
+
+def _like_x(t, x) -> int:
+    """Row stride of ``t``, which has to have x's dtype and shape and contiguous columns."""
+    if t.dtype is not x.dtype or t.shape != x.shape or t.stride(1) != 1 and t.shape[1] != 1:
+        raise ValueError("residual and summed must be (rows, hidden) of x's dtype with contiguous columns")
+    return t.stride(0) if t.shape[0] != 1 else t.shape[1]
 
 
 def swiglu_int8(gate_up, *, codes=None, scale=None):
     """int8 rows of silu(gate) * up, in fp32, of a fused (rows, 2 inter) projection.  Returns (codes, scale)."""
-    stream = _raw_stream(gate_up)
-    if gate_up.dim() != 2 or gate_up.shape[1] % 2:
+    lib, dev, stream = _int8_call(gate_up)
+    code, rows, width, xs = _rows_of(gate_up, "gate_up")
+    if width % 2:
         raise ValueError("gate_up must be (rows, 2 inter)")
-    rows, inter = gate_up.shape[0], gate_up.shape[1] // 2
-    code, codes, scale = _int8_rows_out(gate_up, inter, codes, scale)
-    rc = _lib_handle().specdec_swiglu_int8(gate_up.data_ptr(), gate_up.stride(0), codes.data_ptr(), codes.stride(0),
-                                           scale.data_ptr(), code, rows, inter, stream)
-    _lib.check(rc, "swiglu_int8")
+    inter = width // 2
+    codes, cs, scale = _int8_out(gate_up, dev, rows, inter, codes, scale)
+    rc = lib.specdec_swiglu_int8(gate_up.data_ptr(), xs, codes.data_ptr(), cs, scale.data_ptr(), code, rows, inter,
+                                 stream)
+    if rc:
+        _lib.check(rc, "swiglu_int8")
     return codes, scale
+
+
+def _check_codes(codes, what: str):
+    """(rows, width, row stride) of int8 rows with contiguous columns."""
+    if codes.dtype is not _I8 or codes.dim() != 2:
+        raise ValueError(f"{what} must be 2-D int8")
+    rows, width = codes.shape
+    st, sc = codes.stride()
+    if sc != 1 and width != 1:
+        raise ValueError(f"{what} must have contiguous columns")
+    return rows, width, st
 
 
 def dequantize_int8(codes, scale, *, out=None, dtype=torch.bfloat16):
     """codes * scale of int8 rows, in ``dtype`` (f32 or bf16) or into ``out``."""
-    stream = _raw_stream(codes)
-    if codes.dtype != torch.int8 or codes.dim() != 2 or codes.stride(1) != 1 and codes.shape[1] != 1:
-        raise ValueError("codes must be int8 (rows, width) with contiguous columns")
-    rows, width = codes.shape
-    if scale.dtype != torch.float32 or scale.shape != (rows,) or not scale.is_contiguous() or not scale.is_cuda:
-        raise ValueError("scale must be contiguous float32 (rows,)")
+    lib, dev, stream = _int8_call(codes)
+    rows, width, cs = _check_codes(codes, "codes")
+    _check_scale(scale, dev, rows, "scale")
     if out is None:
-        out = torch.empty((rows, width), dtype=dtype, device=codes.device)
-    code = _dtype_code(out)
-    if code < 0 or out.shape != (rows, width) or out.stride(1) != 1 and width != 1 or not out.is_cuda:
-        raise ValueError("out must be (rows, width) float32 or bfloat16 with contiguous columns")
-    rc = _lib_handle().specdec_dequantize_int8(codes.data_ptr(), codes.stride(0), scale.data_ptr(), out.data_ptr(),
-                                               out.stride(0), code, rows, width, stream)
-    _lib.check(rc, "dequantize_int8")
+        out = scale.new_empty((rows, width), dtype=dtype)
+    else:
+        _on_device(dev, out)
+    code, o_rows, o_width, os = _rows_of(out, "out")
+    if o_rows != rows or o_width != width:
+        raise ValueError("out must be (rows, width)")
+    rc = lib.specdec_dequantize_int8(codes.data_ptr(), cs if rows != 1 else width, scale.data_ptr(), out.data_ptr(),
+                                     os, code, rows, width, stream)
+    if rc:
+        _lib.check(rc, "dequantize_int8")
     return out
 
 
@@ -668,31 +725,30 @@ def linear_int8(codes, scale, weight_codes, weight_scale, *, bias=None, out=None
     ``codes`` (rows, width) and ``weight_codes`` (out_features, width) are int8 with 16-byte aligned rows
     (as ``quantize_int8`` lays them out), ``scale``, ``weight_scale`` and ``bias`` f32, ``out`` f32 or bf16.
     The integer sum is exact; the rest is fp32, rounded once.  ``weight_ready``: the caller promises that the
-    work right before this call on the stream does not write ``weight_codes``, so they may be loaded early."""
-    stream = _raw_stream(codes)
-    if codes.dtype != torch.int8 or weight_codes.dtype != torch.int8 or codes.dim() != 2 or weight_codes.dim() != 2:
-        raise ValueError("codes (rows, width) and weight_codes (out_features, width) must be 2-D int8")
-    rows, width = codes.shape
-    n = weight_codes.shape[0]
-    if weight_codes.shape[1] != width or (codes.stride(1) != 1 or weight_codes.stride(1) != 1) and width != 1:
+    work right before this call on the stream does not write ``weight_codes``, so they may be loaded early.
+    ``status``: a device int32 that receives the library's status bits (a wait that timed out)."""
+    lib, dev, stream = _int8_call(codes)
+    rows, width, cs = _check_codes(codes, "codes")
+    n, w_width, ws = _check_codes(weight_codes, "weight_codes")
+    if w_width != width:
         raise ValueError("codes and weight_codes must share a contiguous width")
-    f32 = torch.float32
-    if scale.dtype != f32 or scale.shape != (rows,) or not scale.is_contiguous():
-        raise ValueError("scale must be contiguous float32 (rows,)")
-    if weight_scale.dtype != f32 or weight_scale.shape != (n,) or not weight_scale.is_contiguous():
-        raise ValueError("weight_scale must be contiguous float32 (out_features,)")
-    if bias is not None and (bias.dtype != f32 or bias.shape != (n,) or not bias.is_contiguous() or not bias.is_cuda):
-        raise ValueError("bias must be contiguous float32 (out_features,)")
-    if not (scale.is_cuda and weight_codes.is_cuda and weight_scale.is_cuda):
-        raise RuntimeError("tensors must be CUDA")
+    _check_scale(scale, dev, rows, "scale")
+    _check_scale(weight_scale, dev, n, "weight_scale")
+    b_ptr = None
+    if bias is not None:
+        _check_scale(bias, dev, n, "bias")
+        b_ptr = bias.data_ptr()
     if out is None:
-        out = torch.empty((rows, n), dtype=out_dtype, device=codes.device)
-    code = _dtype_code(out)
-    if code < 0 or out.shape != (rows, n) or out.stride(1) != 1 and n != 1 or not out.is_cuda:
-        raise ValueError("out must be (rows, out_features) float32 or bfloat16 with contiguous columns")
-    rc = _lib_handle().specdec_linear_int8(
-        codes.data_ptr(), codes.stride(0), scale.data_ptr(), weight_codes.data_ptr(), weight_codes.stride(0),
-        weight_scale.data_ptr(), _ptr(bias), out.data_ptr(), out.stride(0), code, rows, width, n,
-        1 if weight_ready else 0, _ptr(status), stream)
-    _lib.check(rc, "linear_int8")
+        out = scale.new_empty((rows, n), dtype=out_dtype)
+        _on_device(dev, weight_codes)
+    else:
+        _on_device(dev, weight_codes, out)
+    code, o_rows, o_n, os = _rows_of(out, "out")
+    if o_rows != rows or o_n != n:
+        raise ValueError("out must be (rows, out_features)")
+    rc = lib.specdec_linear_int8(codes.data_ptr(), cs, scale.data_ptr(), weight_codes.data_ptr(), ws,
+                                 weight_scale.data_ptr(), b_ptr, out.data_ptr(), os, code, rows, width, n,
+                                 1 if weight_ready else 0, _ptr(status), stream)
+    if rc:
+        _lib.check(rc, "linear_int8")
     return out
