@@ -597,7 +597,7 @@ def _int8_out(x, dev: int, rows: int, width: int, codes, scale):
     stride that is a multiple of 16 bytes, as linear_int8 reads them."""
     if codes is None:
         stride = (width + 15) & ~15
-        codes = x.new_empty((rows, stride), dtype=_I8)
+        codes = torch.empty(rows, stride, dtype=_I8, device=x.device)
         if stride != width:
             codes = codes[:, :width]
     else:
@@ -606,15 +606,16 @@ def _int8_out(x, dev: int, rows: int, width: int, codes, scale):
             raise ValueError("codes must be int8 (rows, width) with contiguous columns")
         stride = codes.stride(0) if rows != 1 else width
     if scale is None:
-        scale = x.new_empty(rows, dtype=_F32)
+        scale = torch.empty(rows, dtype=_F32, device=x.device)
     else:
         _check_scale(scale, dev, rows, "scale")
     return codes, stride, scale
 
 
 def _check_scale(scale, dev: int, n: int, what: str) -> None:
-    _on_device(dev, scale)
-    if scale.dtype is not _F32 or scale.dim() != 1 or scale.shape[0] != n or not scale.is_contiguous():
+    if scale.get_device() != dev:
+        raise RuntimeError("tensors must be CUDA, all on one device")
+    if scale.dtype is not _F32 or scale.shape != (n,) or not scale.is_contiguous():
         raise ValueError(f"{what} must be contiguous float32 ({n},)")
 
 
@@ -650,7 +651,7 @@ def rmsnorm_int8(x, weight, eps: float = 1e-6, *, residual=None, summed=None, co
     else:
         if summed is None:  # rows on 16-byte boundaries, so the next call on it reads aligned rows
             ss = (hidden + 7) & ~7
-            summed = x.new_empty((rows, ss))
+            summed = torch.empty(rows, ss, dtype=x.dtype, device=x.device)
             if ss != hidden:
                 summed = summed[:, :hidden]
         else:
@@ -699,18 +700,31 @@ def _check_codes(codes, what: str):
     return rows, width, st
 
 
+def _new_out(like, rows: int, width: int, dtype):
+    """A new f32 / bf16 (rows, width) on ``like``'s device, its dtype code and row stride."""
+    code = _lib.BF16 if dtype is _BF16 else _lib.F32 if dtype is _F32 else -1
+    if code < 0:
+        raise ValueError("out must be float32 or bfloat16")
+    return torch.empty(rows, width, dtype=dtype, device=like.device), code, width
+
+
+def _given_out(out, dev: int, rows: int, width: int):
+    _on_device(dev, out)
+    code, o_rows, o_width, stride = _rows_of(out, "out")
+    if o_rows != rows or o_width != width:
+        raise ValueError(f"out must be ({rows}, {width})")
+    return code, stride
+
+
 def dequantize_int8(codes, scale, *, out=None, dtype=torch.bfloat16):
     """codes * scale of int8 rows, in ``dtype`` (f32 or bf16) or into ``out``."""
     lib, dev, stream = _int8_call(codes)
     rows, width, cs = _check_codes(codes, "codes")
     _check_scale(scale, dev, rows, "scale")
     if out is None:
-        out = scale.new_empty((rows, width), dtype=dtype)
+        out, code, os = _new_out(scale, rows, width, dtype)
     else:
-        _on_device(dev, out)
-    code, o_rows, o_width, os = _rows_of(out, "out")
-    if o_rows != rows or o_width != width:
-        raise ValueError("out must be (rows, width)")
+        code, os = _given_out(out, dev, rows, width)
     rc = lib.specdec_dequantize_int8(codes.data_ptr(), cs if rows != 1 else width, scale.data_ptr(), out.data_ptr(),
                                      os, code, rows, width, stream)
     if rc:
@@ -738,14 +752,12 @@ def linear_int8(codes, scale, weight_codes, weight_scale, *, bias=None, out=None
     if bias is not None:
         _check_scale(bias, dev, n, "bias")
         b_ptr = bias.data_ptr()
+    if weight_codes.get_device() != dev:
+        raise RuntimeError("tensors must be CUDA, all on one device")
     if out is None:
-        out = scale.new_empty((rows, n), dtype=out_dtype)
-        _on_device(dev, weight_codes)
+        out, code, os = _new_out(scale, rows, n, out_dtype)
     else:
-        _on_device(dev, weight_codes, out)
-    code, o_rows, o_n, os = _rows_of(out, "out")
-    if o_rows != rows or o_n != n:
-        raise ValueError("out must be (rows, out_features)")
+        code, os = _given_out(out, dev, rows, n)
     rc = lib.specdec_linear_int8(codes.data_ptr(), cs, scale.data_ptr(), weight_codes.data_ptr(), ws,
                                  weight_scale.data_ptr(), b_ptr, out.data_ptr(), os, code, rows, width, n,
                                  1 if weight_ready else 0, _ptr(status), stream)
