@@ -364,14 +364,16 @@ int specdec_swiglu_packed(const void* gate_up, void* out, int64_t rows, int64_t 
  * in fp32, ties to even.  A row that holds an infinity or a NaN gets scale NaN and codes 0
  * (everything computed from it is NaN).  Activations are f32 or bf16 (`dtype`), rows
  * `x_stride` elements apart with contiguous columns; code rows are `codes_stride` bytes apart.
- * rows == 0 launches nothing.  A weight (out_features, width) quantised by rows has the scale
+ * rows == 0 launches nothing; a row has at most 2^24 values.  A row whose loads do not arrive within a
+ * second (every device wait of this library is bounded) gets scale NaN, too.  A weight (out_features, width) quantised by rows has the scale
  * for each output channel that specdec_linear_int8 takes.
  */
 /* codes = int8(x) */
 int specdec_quantize_int8(const void* x, int64_t x_stride, void* codes, int64_t codes_stride, float* scale,
                           int32_t dtype, int64_t rows, int32_t width, specdec_stream_t stream);
 /* s = x + residual (s = x without one);  codes = int8(s / sqrt(mean(s^2) + eps) * weight) in fp32 from the
-   unrounded sum; summed receives s rounded to the input type.  residual and summed are both given or both
+   unrounded sum; summed receives s rounded to the input type.  A row whose sum of squares passes fp32's
+   largest number counts as not finite.  residual and summed are both given or both
    NULL; summed may be x or residual (same stride). */
 int specdec_rmsnorm_int8(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                          const void* weight, float eps, void* summed, int64_t summed_stride, void* codes,

@@ -3,22 +3,27 @@
 // The integer sum is exact: |sum| <= K 127^2 < 2^31 for K <= 131072, in any order.  Scales and
 // bias are applied in fp32 and the result is rounded once to the output type.
 //
-// The weight is the M operand: a tile is 128 output channels by up to 256 rows ("tokens") of a,
-// so a call of a few tokens wastes only columns of a narrow N, and an accumulator lane is an
-// output channel: a warp stores 32 neighbouring channels of one token at a time, whatever the
-// alignment of the output.
+// Two kernels (few_rows):
 //
-// linear_int8_kernel, 320 threads:
+// linear_int8_few_kernel, up to 8 rows, and up to 32 where that is ahead: bound by reading W once.
+// Its comment is beside it.
+//
+// linear_int8_kernel, on the fifth-generation tensor cores, 320 threads.  The weight is the M operand:
+// a tile is 128 output channels by up to 256 rows ("tokens") of a, so a call of few tokens wastes only
+// columns of a narrow N, and an accumulator lane is an output channel.
 //   warp 8    producer: TMA loads of the W tile [128 channels][128 codes] and the a tile
 //             [tokens][128 codes] of each 128-code chunk of K (128-byte swizzle, K-major; the
 //             ragged ends of K, N and the rows are filled with zeros by the TMA unit) into a
-//             ring of 4 to 12 stages;
+//             ring of 4 to 11 stages;
 //   warp 9    one lane issues tcgen05.mma kind::i8 (K 32) into one of two TMEM accumulators,
 //             so a tile's epilogue overlaps the next tile's products;
-//   warps 0-7 epilogue: lane = channel, columns = tokens.
+//   warps 0-7 epilogue: scales, bias, rounding and stores, two warps to a lane quarter.
 // CG = 2: two CTAs on one 256-channel tile (cta_group::2).  Each loads its own 128 channels and
-// half of the tokens, so a chunk costs a CTA 128 + tokens / 2 rows of loads instead of
-// 128 + tokens; the pair's first CTA issues the products.
+// half of the tokens, so a chunk costs a CTA 128 + tokens / 2 rows of loads where one CTA alone
+// pays 128 + tokens; the pair's first CTA issues the products.  L2 delivers about 64 bytes a clock
+// and SM, which a 256 x 256 pair needs exactly at the products' full rate: 8192^3 runs at 3.2-3.3
+// POP/s, twice the bf16 rate of the library's product (3.29).  With K = 1536 and 17920 channels the
+// output (1.2 GB for 32768 rows) shares L2 with those loads: 617-700 us, 2.6-2.9 POP/s.
 // splits > 1 (CG = 1): a cluster of `splits` CTAs shares one tile, each taking a share of the
 // chunks of K, and adds up the integer partial sums through distributed shared memory.
 #include <cudaTypedefs.h>
@@ -64,7 +69,7 @@ SD_DEV uint32_t idesc_i8(int M, int N) {
 }
 // One lane of a converged warp.  The loops around it stay warp-uniform, so descriptors, barriers and
 // loop counters live in uniform registers (the tcgen05 operands): a loop inside `if (lane == 0)`
-// moved every operand there first and took 590 clocks a chunk instead of
+// moved every operand there first, and cost 6 % of the whole at 8192^3 (398 and 375 us).
 SD_DEV bool elect_one() {
   uint32_t p;
   asm volatile(
@@ -192,8 +197,9 @@ SD_DEV float scaled(int32_t acc, float sa, float sw, float b) {
   return __fmaf_rn(__fmul_rn(static_cast<float>(acc), sa), sw, b);
 }
 
-// 16 tokens of one channel, from token c of the tile on: scaled, rounded, stored.  All scales are
-// read and all results formed before the first store, so nothing waits behind a store.
+// 16 tokens of one channel (lane = channel, any alignment, f32 or bf16): scaled, rounded, stored, 32
+// neighbouring channels of a token at a time.  All scales are read and all results formed before the
+// first store, so nothing waits behind a store (one by one: 1.9 times the time at 32768 x 1536 x 17920).
 template <typename T, bool GUARD>
 SD_DEV void store_tokens(const int32_t (&v)[16], const float* s_scale, float sw, float bias, T* o, int64_t stride,
                          int ntok) {
@@ -228,7 +234,8 @@ SD_DEV uint32_t scaled_pair(int32_t a0, int32_t a1, uint64_t sa, uint64_t sw, ui
 // bf16 results of 32 channels x 16 tokens, held as fragments, to 64 consecutive bytes of each token's row
 // by way of 1 KB of shared memory: eight tokens a store instead of half of one.  `put`: this lane's
 // address for stmatrix, `get`: for reading back; o: this lane's 16 bytes of tokens lane / 4 and, `half`
-// further, lane / 4 + 8.  At short K it is the issue of these instructions that bounds the kernel.
+// further, lane / 4 + 8.  At short K the epilogue bounds the kernel: with one 2-byte store a token and
+// a tile's scales loaded at its start, 8192 x 896 x 9728 took 72 us; so, 62.
 template <bool GUARD>
 SD_DEV void store_fragments(const int32_t (&v)[16], const float* s_scale, const uint64_t (&sw)[4],
                             const uint64_t (&bias)[4], uint32_t put, const uint8_t* get, uint8_t* o, int64_t half,
@@ -261,7 +268,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                        const __grid_constant__ CUtensorMap wmap) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kLinMaxStages], empty[kLinMaxStages], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[kLinMaxStages], empty[kLinMaxStages], acc_full[2], acc_empty[2], given_up;
   __shared__ uint32_t tmem_base;
   __shared__ __align__(16) float s_scale[kLinEpiWarps][kLinMaxTokens / 2];
   __shared__ __align__(128) uint8_t s_stage[kLinEpiWarps][1024];
@@ -278,6 +285,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], kLinEpiWarps * CG);
     }
+    mbar_init(&given_up, 1);
     fence_barrier_init();
   }
   if (warp == kLinEpiWarps && lane == 0) {
@@ -349,11 +357,12 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         if (++s == p.stages) s = 0, parity ^= 1;
       }
     }
-    // every stage's last use is over before the CTA leaves (bounded; unused stages pass at once)
-    for (int i = 0; i < p.stages && !stop; ++i) {
-      stop = !warp_wait(&empty[s], parity);
-      if (++s == p.stages) s = 0, parity ^= 1;
-    }
+    // every stage's last use is over before the CTA leaves (bounded; unused stages pass at once) ...
+    for (int i = 0, at = s; i < p.stages && !stop; ++i, at = at + 1 == p.stages ? 0 : at + 1)
+      stop = !warp_wait(&empty[at], at < s ? parity ^ 1 : parity);
+    // ... or, after a wait that gave up, at least the copies under way have landed
+    for (int i = 0; i < p.stages && stop && (CG == 1 || rank == 0); ++i)
+      (void)warp_wait(&full[i], i < s ? parity ^ 1 : parity);
   } else if (warp == kLinEpiWarps + 1) {
     // ---- MMA issuer
     if (rank % CG == 0) {
@@ -396,7 +405,14 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           parity = parity1;
         }
       }
-      if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      if (!ok) {  // the products issued so far end before TMEM is given back
+        if (elect_one()) {
+          raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+          commit_mma<CG>(&given_up);
+        }
+        __syncwarp();
+        (void)warp_wait(&given_up, 0);
+      }
     }
   } else {
     // ---- epilogue: lane = channel, columns = tokens; two warps share a lane quarter, each half the tokens
