@@ -623,14 +623,20 @@ static int launch_stream(const char* what, const RowArgs& a, bool vec, cudaStrea
              : launch_stream_as<T, OP, 16, false>(what, a, slots, row, st);
 }
 
-// Which kernel takes the rows.  `many` (eight rows an SM): aligned rows in the registers of a warp, or
-// of four, while they hold it; others through shared memory.  Fewer rows are spread over a block each,
-// one to four pieces a thread, which is the shortest chain from the first load to the last store;
-// unaligned ones likewise, by single values, and so are rows whose outputs are not aligned.
+// Which kernel takes the rows; measured for bf16 rows of 896, 1536, 4864 and 8960 values, 5 to 32768 of
+// them.  Aligned rows that a few warps can hold: a warp, or two to eight, a row, three to six pieces a
+// thread, which keeps the most loads in flight (a block of 1024 threads a row: 3.3 us for 5 rows of
+// swiglu's 8960, 13.5 for 600; 256 threads: 2.5 and 7.3; 32768 rows of swiglu's 1536: 49 us with a warp a
+// row, 39 with two); short rows in small number are spread as wide as they go, a piece a thread (`few`:
+// under eight rows an SM).  Longer ones, swiglu's long ones in large
+// number (its arithmetic hides behind the ring's copies: 8192 x 8960 62 us, 95 in registers) and unaligned
+// ones in large number through shared memory; unaligned rows in small number by single values, a block a
+// row, and so are rows whose outputs are not aligned.
 template <typename T, int OP>
 static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool many = a.rows >= 8 * device_sm_count();
+  const int64_t sms = device_sm_count();
+  const bool few = a.rows < 8 * sms, two = kTwoInputs<OP>;
   const uintptr_t out_bits = reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.summed) |
                              static_cast<uintptr_t>(a.s_stride) * sizeof(T);
   const bool out_vec = out_bits % 16 == 0 &&
@@ -639,21 +645,19 @@ static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
                             static_cast<uintptr_t>(a.x_stride | a.r_stride) * sizeof(T);
   const bool vec = out_vec && in_bits % 16 == 0 && a.width % V == 0;
   const int need = vec ? a.width / V : a.width;
-  if (many && vec) {
-    if (need <= 64) return launch_rows_as<T, OP, 32, V, 2>(what, a, st);
-    if (need <= 128) return launch_rows_as<T, OP, 32, V, 4>(what, a, st);
-    if (need <= 192) return launch_rows_as<T, OP, 32, V, 6>(what, a, st);
-    if (need <= 256) return launch_rows_as<T, OP, 32, V, 8>(what, a, st);
-    if (V == 4 && need <= 384) return launch_rows_as<T, OP, 32, V, 48 / V>(what, a, st);
+  if (vec) {
+    if (need <= 64 && !few) return launch_rows_as<T, OP, 32, V, 2>(what, a, st);
+    if (need <= 128) return few ? launch_rows_as<T, OP, 128, V, 1>(what, a, st) : launch_rows_as<T, OP, 32, V, 4>(what, a, st);
+    if (need <= 256 && a.rows <= 2 * sms) return launch_rows_as<T, OP, 256, V, 1>(what, a, st);
+    if (need <= 192) return few || two ? launch_rows_as<T, OP, 64, V, 3>(what, a, st) : launch_rows_as<T, OP, 32, V, 6>(what, a, st);
+    if (need <= 256) return few || two ? launch_rows_as<T, OP, 128, V, 2>(what, a, st) : launch_rows_as<T, OP, 32, V, 8>(what, a, st);
+    if (need <= 384 && V == 4 && !few && !two) return launch_rows_as<T, OP, 32, V, 48 / V>(what, a, st);
+    if (need <= 384) return launch_rows_as<T, OP, 128, V, 3>(what, a, st);
     if (need <= 640) return launch_rows_as<T, OP, 128, V, 5>(what, a, st);
+    if (need <= 768) return launch_rows_as<T, OP, 256, V, 3>(what, a, st);
+    if (need <= 1280 && (few || OP != kRowSwiglu)) return launch_rows_as<T, OP, 256, V, 5>(what, a, st);
   }
-  if (!many && vec) {
-    if (need <= 256) return launch_rows_as<T, OP, 256, V, 1>(what, a, st);
-    if (need <= 1024) return launch_rows_as<T, OP, 1024, V, 1>(what, a, st);
-    if (need <= 2048) return launch_rows_as<T, OP, 1024, V, 2>(what, a, st);
-    if (need <= 4096) return launch_rows_as<T, OP, 1024, V, 4>(what, a, st);
-  }
-  if (out_vec && (many || vec || need > 8192))
+  if (out_vec && (vec || need > 8192 || a.rows > (need > 1024 ? 1 : 4) * sms))
     if (const int rc = launch_stream<T, OP>(what, a, vec, st); rc != SPECDEC_ERR_UNSUPPORTED) return rc;
   if (a.width <= 1024) return launch_rows_as<T, OP, 256, 1, 4>(what, a, st);
   if (a.width <= 8192) return launch_rows_as<T, OP, 1024, 1, 8>(what, a, st);
