@@ -81,6 +81,48 @@ def test_quantize_is_bit_exact(rows, width, pad, dtype):
         assert torch.equal(values, (codes.float() * scale[:, None]).to(out_dtype))
 
 
+# enough rows for the kernels that take a warp or more a row, and for the ring in shared memory
+MANY = [(1300, 500), (1300, 896), (1300, 1536), (1200, 2048), (1200, 2500), (1200, 4864), (1200, 6000), (1200, 8960),
+        (1300, 101), (1300, 1001), (300, 1537), (1200, 1792), (400, 2501), (200, 6001), (160, 11003), (1190, 12000),
+        (4, 16001), (4, 26001)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("op", ["quantize", "rmsnorm", "rmsnorm_add", "rmsnorm_add_in_place", "swiglu"])
+@pytest.mark.parametrize("rows,width", MANY)
+def test_many_rows(rows, width, op, dtype):
+    """Every operator at sizes that other kernels take than the few rows above; rows are padded by 0 to 9
+    values, so that those of the two inputs start at every alignment."""
+    ops = _ops()
+    g = _gen(rows + width)
+    pad = [int(torch.randint(0, 10, (1,), generator=g)) * (width % 2) for _ in range(2)]
+    if op == "swiglu":
+        x = (torch.randn(rows, 2 * width + pad[0], generator=g) * 2).clamp(-12, 12).to(dtype).cuda()[:, :2 * width]
+        codes, scale = ops.swiglu_int8(x)
+        return _assert_codes(codes, scale, o8.swiglu_rows(x), 2.0 ** -19)
+    x = _hidden(rows, width, dtype, 2 * rows + width, pad[0])
+    x[rows // 2, width - 1] = float("nan")
+    x[rows // 3] = 0
+    keep = torch.arange(rows, device="cuda") != rows // 2
+    if op == "quantize":
+        codes, scale = ops.quantize_int8(x)
+        want_codes, want_scale = o8.quantize_rows_f32(x.float().cpu().numpy())
+        assert np.array_equal(codes.cpu().numpy(), want_codes)
+        assert np.array_equal(scale.cpu().numpy(), want_scale, equal_nan=True)
+        values = ops.dequantize_int8(codes, scale, dtype=dtype)
+        assert torch.equal(values[keep], (codes.float() * scale[:, None]).to(dtype)[keep])
+        return
+    r = _hidden(rows, width, dtype, 3 * rows + width, pad[1]) if "add" in op else None
+    w = (torch.rand(width, generator=g) + 0.5).to(dtype).cuda()
+    y, _ = o8.rmsnorm_rows(x, w, 1e-6, r)
+    want = None if r is None else (x.float() + r.float()).to(dtype)
+    codes, scale, summed = ops.rmsnorm_int8(x, w, 1e-6, residual=r, summed=r if "place" in op else None)
+    assert torch.isnan(scale[rows // 2]) and (codes[rows // 2] == 0).all()
+    if r is not None:
+        assert torch.equal(summed[keep], want[keep])
+    _assert_codes(codes[keep], scale[keep], y[keep], ((width / 32 + 16) / 2 + 8) * U)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("width", [8, 100, 1536, 20000])
 def test_quantize_special_rows(width, dtype):
