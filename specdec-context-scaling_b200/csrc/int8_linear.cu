@@ -635,68 +635,111 @@ SD_DEV void mma_m16n8k32(int32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Products of one step of 64 codes: this lane's codes of channels g and g + 8, and of token 8 b + g.
+template <int NB>
+SD_DEV void few_step(int32_t (&d)[NB][4], const uint4& c0, const uint4& c1, const uint4 (&x)[NB]) {
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    mma_m16n8k32(d[b], c0.x, c1.x, c0.y, c1.y, x[b].x, x[b].y);
+    mma_m16n8k32(d[b], c0.z, c1.z, c0.w, c1.w, x[b].z, x[b].w);
+  }
+}
+// The warps' partial sums of 16 channels meet in shared memory; the block's threads scale and store them.
+template <int NB, int WARPS, typename T>
+SD_DEV void few_finish(const FewParams& p, const int32_t (&d)[NB][4], int32_t (*part)[NB * 8][kFewCh + 1], int n0) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  // accumulator: channels g (d0, d1) and g + 8 (d2, d3), tokens 2 t and 2 t + 1
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[warp][b * 8 + 2 * t + (i & 1)][g + (i >> 1) * 8] = d[b][i];
+  // this thread's first output's scales are on their way while the block meets
+  const int row0 = threadIdx.x / kFewCh, n = n0 + threadIdx.x % kFewCh;
+  const bool mine = row0 < NB * 8 && row0 < p.rows && n < p.n;
+  const float sw = mine ? p.w_scale[n] : 0.f, bias = mine && p.bias ? p.bias[n] : 0.f;
+  float sa = mine ? p.a_scale[row0] : 0.f;
+  __syncthreads();
+  for (int row = row0; row < NB * 8 && row < p.rows && n < p.n; row += 2 * WARPS) {
+    int32_t sum = 0;
+#pragma unroll
+    for (int j = 0; j < WARPS; ++j) sum += part[j][row][threadIdx.x % kFewCh];
+    if (row != row0) sa = p.a_scale[row];
+    store_out(static_cast<T*>(p.out) + row * p.out_stride + n, scaled(sum, sa, sw, bias));
+  }
+}
+
+// A warp's share of K is at most AHEAD steps: all its loads are under way at once, those of W before the
+// preceding kernel is over if they may.
 template <int NB, int WARPS, int AHEAD, typename T>
-__global__ void __launch_bounds__(32 * WARPS) linear_int8_few_kernel(const FewParams p) {
+__global__ void __launch_bounds__(32 * WARPS, AHEAD <= 3 && NB == 1 ? 4 : 1) linear_int8_few_kernel(const FewParams p) {
+  __shared__ int32_t part[WARPS][NB * 8][kFewCh + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * kFewCh;
+  const int steps = (p.width + kFewStep - 1) / kFewStep;
+  const int s_begin = steps * warp / WARPS, s_end = steps * (warp + 1) / WARPS;
+  // first code of step j of this lane (past the row's end: zeros)
+  const auto code = [&](int j) { return s_begin + j < s_end ? (s_begin + j) * kFewStep + t * 16 : p.width; };
+  const int8_t* w0 = p.w + static_cast<int64_t>(n0 + g) * p.w_stride;
+  uint4 wa[AHEAD], wb[AHEAD], x[AHEAD][NB];
+  if (!p.weight_ready) grid_dep_wait();
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) {
+    wa[j] = n0 + g < p.n ? load_codes16(w0, code(j), p.width) : make_uint4(0, 0, 0, 0);
+    wb[j] = n0 + g + 8 < p.n ? load_codes16(w0 + 8 * p.w_stride, code(j), p.width) : make_uint4(0, 0, 0, 0);
+  }
+  if (p.weight_ready) grid_dep_wait();
+  grid_dep_launch();
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      x[j][b] = b * 8 + g < p.rows ? load_codes16(p.a + static_cast<int64_t>(b * 8 + g) * p.a_stride, code(j), p.width)
+                                   : make_uint4(0, 0, 0, 0);
+  int32_t d[NB][4] = {};
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) few_step<NB>(d, wa[j], wb[j], x[j]);
+  few_finish<NB, WARPS, T>(p, d, part, n0);
+}
+
+// The same for a longer K: a warp's share in turns of AHEAD steps.
+template <int NB, int WARPS, int AHEAD, typename T>
+__global__ void __launch_bounds__(32 * WARPS) linear_int8_few_long_kernel(const FewParams p) {
   __shared__ int32_t part[WARPS][NB * 8][kFewCh + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * kFewCh;
   const int steps = (p.width + kFewStep - 1) / kFewStep;
   const int s_begin = steps * warp / WARPS, s_end = steps * (warp + 1) / WARPS;
   const int8_t* w0 = p.w + static_cast<int64_t>(n0 + g) * p.w_stride;
-  const int8_t* w1 = w0 + 8 * p.w_stride;
   const bool has0 = n0 + g < p.n, has1 = n0 + g + 8 < p.n;
   int32_t d[NB][4] = {};
   if (!p.weight_ready) grid_dep_wait();
   bool waited = !p.weight_ready;
   for (int s = s_begin; s < s_end || !waited; s += AHEAD) {
+    const auto code = [&](int j) { return s + j < s_end ? (s + j) * kFewStep + t * 16 : p.width; };
     uint4 wa[AHEAD], wb[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const int k = s + j < s_end ? (s + j) * kFewStep + t * 16 : p.width;
-      wa[j] = has0 ? load_codes16(w0, k, p.width) : make_uint4(0, 0, 0, 0);
-      wb[j] = has1 ? load_codes16(w1, k, p.width) : make_uint4(0, 0, 0, 0);
+      wa[j] = has0 ? load_codes16(w0, code(j), p.width) : make_uint4(0, 0, 0, 0);
+      wb[j] = has1 ? load_codes16(w0 + 8 * p.w_stride, code(j), p.width) : make_uint4(0, 0, 0, 0);
     }
-    if (!waited) {
-      grid_dep_wait();
-      waited = true;
-    }
+    if (!waited) grid_dep_wait();
+    if (s == s_begin) grid_dep_launch();
+    waited = true;
 #pragma unroll
     for (int h = 0; h < AHEAD; h += kFewAhead) {
-      uint4 x[NB][kFewAhead];
-#pragma unroll
-      for (int j = 0; j < kFewAhead && h + j < AHEAD; ++j) {
-        const int k = s + h + j < s_end ? (s + h + j) * kFewStep + t * 16 : p.width;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-          x[b][j] = b * 8 + g < p.rows ? load_codes16(p.a + static_cast<int64_t>(b * 8 + g) * p.a_stride, k, p.width)
-                                       : make_uint4(0, 0, 0, 0);
-      }
+      uint4 x[kFewAhead][NB];
 #pragma unroll
       for (int j = 0; j < kFewAhead && h + j < AHEAD; ++j)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const uint4 &c0 = wa[h + j], &c1 = wb[h + j];
-          mma_m16n8k32(d[b], c0.x, c1.x, c0.y, c1.y, x[b][j].x, x[b][j].y);
-          mma_m16n8k32(d[b], c0.z, c1.z, c0.w, c1.w, x[b][j].z, x[b][j].w);
-        }
+        for (int b = 0; b < NB; ++b)
+          x[j][b] = b * 8 + g < p.rows
+                        ? load_codes16(p.a + static_cast<int64_t>(b * 8 + g) * p.a_stride, code(h + j), p.width)
+                        : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < kFewAhead && h + j < AHEAD; ++j) few_step<NB>(d, wa[h + j], wb[h + j], x[j]);
     }
   }
-  grid_dep_launch();
-  // accumulator: channels g (d0, d1) and g + 8 (d2, d3), tokens 2 t and 2 t + 1
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) part[warp][b * 8 + 2 * t + (i & 1)][g + (i >> 1) * 8] = d[b][i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < NB * 8 * kFewCh; i += 32 * WARPS) {
-    const int row = i / kFewCh, n = n0 + i % kFewCh;
-    if (row >= p.rows || n >= p.n) continue;
-    int32_t sum = 0;
-#pragma unroll
-    for (int j = 0; j < WARPS; ++j) sum += part[j][row][i % kFewCh];
-    store_out(static_cast<T*>(p.out) + row * p.out_stride + n,
-              scaled(sum, p.a_scale[row], p.w_scale[n], p.bias ? p.bias[n] : 0.f));
-  }
+  few_finish<NB, WARPS, T>(p, d, part, n0);
 }
 
 // ---------------------------------------------------------------- host
@@ -835,12 +878,21 @@ static int launch_few_as(const FewParams& p, cudaStream_t st) {
   return launch_pdl("linear_int8_few_kernel", linear_int8_few_kernel<NB, WARPS, AHEAD, T>,
                     dim3(static_cast<unsigned>((p.n + kFewCh - 1) / kFewCh)), dim3(32 * WARPS), 0, st, p);
 }
+template <int NB, int AHEAD, typename T>
+static int launch_few_long(const FewParams& p, cudaStream_t st) {
+  return launch_pdl("linear_int8_few_long_kernel", linear_int8_few_long_kernel<NB, 16, AHEAD, T>,
+                    dim3(static_cast<unsigned>((p.n + kFewCh - 1) / kFewCh)), dim3(512), 0, st, p);
+}
 template <int NB, typename T>
 static int launch_few(const FewParams& p, cudaStream_t st) {
-  // a warp's share of K as far as it can be under way at once: 4 steps (K <= 2048), 5 or 9
-  if (p.width <= 8 * kFewAhead * kFewStep) return launch_few_as<NB, 8, 4, T>(p, st);
-  if (NB > 1 || p.width <= 16 * 5 * kFewStep) return launch_few_as<NB, 16, NB == 1 ? 5 : 4, T>(p, st);
-  return launch_few_as<1, 16, 9, T>(p, st);
+  // a warp's share of K as far as it can be under way at once: 2 to 4 steps in a block of 8 warps, 5 or 9 in
+  // one of 16
+  const int steps = (p.width + kFewStep - 1) / kFewStep;
+  if (steps <= 16) return launch_few_as<NB, 8, 2, T>(p, st);
+  if (steps <= 24) return launch_few_as<NB, 8, 3, T>(p, st);
+  if (steps <= 32) return launch_few_as<NB, 8, 4, T>(p, st);
+  if (NB > 1 || steps <= 80) return launch_few_long<NB, NB == 1 ? 5 : 4, T>(p, st);
+  return launch_few_long<1, 9, T>(p, st);
 }
 
 }  // namespace sd
