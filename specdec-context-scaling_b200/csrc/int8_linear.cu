@@ -595,8 +595,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 // ---------------------------------------------------------------- a few rows
 // A call of up to 32 rows is bound by reading W once and by the chain of latencies around that.  Here a
 // block takes 16 output channels and its warps a share of K each, straight from global memory into
-// mma.sync fragments: no ring, barriers or TMEM to set up.  (The tcgen05 kernel took 4.2 us at
-// 5 x 1536 x 2048 and 6.7 us at 5 x 8960 x 1536.)
+// mma.sync fragments: no ring, barriers or TMEM to set up, and a small enough block that the next kernel
+// on the stream starts beside it.  5 x 1536 x 2048 takes 1.7 us (4.2 in the tcgen05 kernel); 5 x 1536 x
+// 17920 4.7 us from L2, 6.1 from HBM (4.5 TB/s), where the waves of blocks over the SMs bound it.
 // mma.sync m16n8k32 multiplies in any order of K, so a lane's 16 consecutive codes of a row are its
 // fragments of two products: lane (g, t) holds codes 16 t .. 16 t + 15 of channels g and g + 8 and of
 // token g in each step of 64 codes.  Channels and tokens past the end read as zero.
@@ -865,13 +866,15 @@ static int launch_linear(const LinParams& p, const CUtensorMap& amap, const CUte
   return after_launch("linear_int8_kernel");
 }
 
-// Up to 8 rows always (5 x 1536 x 17920: 5.7 us, 6.9 in the tcgen05 kernel); with more, each block reads
-// more of a, and the tcgen05 kernel is ahead once a block an SM does not cover the channels (16 x 1536 x
-// 17920: 8.8 and 7.1 us; 16 x 8960 x 1536: 6.0 and 6.8) or, past 16 rows, K is long (32 x 1536 x 2048: 3.4
-// and 5.0 us; 32 x 8960 x 1536: 8.2 and 7.5).
+// Up to 8 rows always (5 x 1536 x 17920: 4.7 us, 6.9 in the tcgen05 kernel).  With more, each block reads
+// more of a, and the tcgen05 kernel is ahead once there are many blocks an SM or, past 16 rows, K is long
+// (us here and there: 16 x 1536 x 4000 2.9 and 4.9, x 8000 5.0 and 5.0, 16 x 8960 x 1536 5.8 and 6.8;
+// 32 x 1536 x 4000 3.5 and 4.9, x 8000 6.6 and 5.1, 32 x 4864 x 896 5.8 and 4.7).
 static bool few_rows(int64_t rows, int width, int n) {
+  const int per_sm = (n + kFewCh * device_sm_count() - 1) / (kFewCh * device_sm_count());  // blocks
   if (rows <= 8) return true;
-  return rows <= kFewRows && n <= kFewCh * device_sm_count() && (rows <= 16 || width <= 2048);
+  if (rows <= 16) return per_sm <= (width <= 2048 ? 3 : 1);
+  return rows <= kFewRows && width <= 2048 && per_sm <= 2;
 }
 template <int NB, int WARPS, int AHEAD, typename T>
 static int launch_few_as(const FewParams& p, cudaStream_t st) {
@@ -885,14 +888,14 @@ static int launch_few_long(const FewParams& p, cudaStream_t st) {
 }
 template <int NB, typename T>
 static int launch_few(const FewParams& p, cudaStream_t st) {
-  // a warp's share of K as far as it can be under way at once: 2 to 4 steps in a block of 8 warps, 5 or 9 in
-  // one of 16
+  // a warp's share of K as far as registers let it be under way at once: 2 to 4 steps in a block of 8 warps
+  // (K <= 2048), up to 5 or 9 in one of 16
   const int steps = (p.width + kFewStep - 1) / kFewStep;
   if (steps <= 16) return launch_few_as<NB, 8, 2, T>(p, st);
   if (steps <= 24) return launch_few_as<NB, 8, 3, T>(p, st);
   if (steps <= 32) return launch_few_as<NB, 8, 4, T>(p, st);
-  if (NB > 1 || steps <= 80) return launch_few_long<NB, NB == 1 ? 5 : 4, T>(p, st);
-  return launch_few_long<1, 9, T>(p, st);
+  if (steps <= 80) return launch_few_long<NB, NB < 4 ? 5 : 4, T>(p, st);
+  return launch_few_long<NB, NB == 1 ? 9 : NB == 2 ? 6 : 4, T>(p, st);
 }
 
 }  // namespace sd
