@@ -261,6 +261,67 @@ SD_DEV void store_fragments(const int32_t (&v)[16], const float* s_scale, const 
   if (!GUARD || (ch_ok && (lane >> 2) + 8 < ntok)) *reinterpret_cast<uint4*>(o + half) = r1;
 }
 
+// A split tile's partial sums, [token][128 channels] in each CTA's shared memory: CTA `rank` takes every
+// SPLITS-th token, a warp a token, a lane four channels.  16 loads a lane are under way at once: one
+// token's at a time left a microsecond of latency for each.
+template <int SPLITS, typename T>
+SD_DEV void add_partials(const LinParams& p, const uint8_t* smem, int rank, int unit) {
+  constexpr int kAtOnce = 16 / SPLITS, kStep = SPLITS * (kLinThreads / 32);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tt = unit / p.ch_tiles, ct = unit - tt * p.ch_tiles;
+  const int n = ct * kLinCh + lane * 4;
+  const int tok0 = tt * p.tokens, ntok = min(p.tokens, p.rows - tok0);
+  float sw[4] = {}, bias[4] = {};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (n + j < p.n) {
+      sw[j] = p.w_scale[n + j];
+      if (p.bias) bias[j] = p.bias[n + j];
+    }
+  uint32_t from[SPLITS];
+#pragma unroll
+  for (int r = 0; r < SPLITS; ++r) from[r] = dsmem_addr(smem_u32(smem) + lane * 16, r);
+  for (int c0 = rank + SPLITS * warp; c0 < ntok; c0 += kAtOnce * kStep) {
+    int4 v[kAtOnce][SPLITS];
+    float sa[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int c = c0 + i * kStep;
+      if (c < ntok) {
+        sa[i] = p.a_scale[tok0 + c];
+#pragma unroll
+        for (int r = 0; r < SPLITS; ++r) v[i][r] = dsmem_ld4_s32(from[r] + c * (kLinCh * 4));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int c = c0 + i * kStep;
+      if (c >= ntok) break;
+      int4 sum = v[i][0];
+#pragma unroll
+      for (int r = 1; r < SPLITS; ++r) {
+        sum.x += v[i][r].x;
+        sum.y += v[i][r].y;
+        sum.z += v[i][r].z;
+        sum.w += v[i][r].w;
+      }
+      const float y[4] = {scaled(sum.x, sa[i], sw[0], bias[0]), scaled(sum.y, sa[i], sw[1], bias[1]),
+                          scaled(sum.z, sa[i], sw[2], bias[2]), scaled(sum.w, sa[i], sw[3], bias[3])};
+      T* o = static_cast<T*>(p.out) + (tok0 + c) * p.out_stride + n;
+      if (p.vec_out && n + 4 <= p.n) {
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
+        else
+          *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.n) store_out(o + j, y[j]);
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------- the kernel
 template <int CG, typename T>
 __global__ void __launch_bounds__(kLinThreads, 1)
@@ -551,42 +612,13 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     tmem_dealloc_cg<CG>(tbase, p.tmem_cols);
   }
   if (CG == 1 && csize > 1) {
-    // token columns are dealt over the cluster; a warp sums one token's 128 channels
     grid_dep_wait();
-    const int tt = unit0 / p.ch_tiles, ct = unit0 - tt * p.ch_tiles;
-    const int n = ct * kLinCh + lane * 4;
-    const int tok0 = tt * p.tokens, ntok = min(p.tokens, p.rows - tok0);
-    float sw[4] = {}, bias[4] = {};
-    for (int j = 0; j < 4; ++j)
-      if (n + j < p.n) {
-        sw[j] = p.w_scale[n + j];
-        if (p.bias) bias[j] = p.bias[n + j];
-      }
-    const uint32_t mine = smem_u32(smem) + lane * 16;
-    for (int c = rank + csize * warp; c < ntok; c += csize * (kLinThreads / 32)) {
-      const float sa = p.a_scale[tok0 + c];
-      int4 sum = make_int4(0, 0, 0, 0);
-#pragma unroll 8
-      for (int r = 0; r < csize; ++r) {
-        const int4 v = dsmem_ld4_s32(dsmem_addr(mine + c * (kLinCh * 4), r));
-        sum.x += v.x;
-        sum.y += v.y;
-        sum.z += v.z;
-        sum.w += v.w;
-      }
-      const float y[4] = {scaled(sum.x, sa, sw[0], bias[0]), scaled(sum.y, sa, sw[1], bias[1]),
-                          scaled(sum.z, sa, sw[2], bias[2]), scaled(sum.w, sa, sw[3], bias[3])};
-      T* o = static_cast<T*>(p.out) + (tok0 + c) * p.out_stride + n;
-      if (p.vec_out && n + 4 <= p.n) {
-        if constexpr (sizeof(T) == 4)
-          *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
-        else
-          *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-      } else {
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.n) store_out(o + j, y[j]);
-      }
-    }
+    if (csize == 8)
+      add_partials<8, T>(p, smem, rank, unit0);
+    else if (csize == 4)
+      add_partials<4, T>(p, smem, rank, unit0);
+    else
+      add_partials<2, T>(p, smem, rank, unit0);
     __syncwarp();
     cluster_sync();  // the peers have read this CTA's shared memory
   }
