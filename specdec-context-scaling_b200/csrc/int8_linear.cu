@@ -806,11 +806,11 @@ struct LinShape {
 static int resident_clusters(int size, int dev, int sms);
 
 // Launch shape by an estimate of the time of a call in ns.  A 128-code chunk of K costs a CTA the largest
-// of its products (1.3 a token: 128 x 128 x 32 products in 64 clocks), what issuing its loads, waits and
-// products takes (120, and 0.23 a row loaded) and its share of L2's bandwidth (9.2 TB/s); the tiles of a
-// CTA follow one another in waves, each hiding the previous one's epilogue (6 a token); a split adds the
-// exchange of the partial sums.  The figures fit 900 timings of 35 layer shapes (5 to 1280 rows): the
-// chosen shape is within 2 % of the best one on average and 10 % at worst.
+// of its products (1.29 a token: 128 x 128 x 32 products in 64 clocks), what issuing its loads, waits and
+// products takes (126, and 0.25 a row loaded) and its share of L2's bandwidth (9.3 TB/s); the tiles of a
+// CTA follow one another in waves, each hiding the previous one's epilogue (2 a token); a split adds the
+// exchange of the partial sums.  The figures fit 3500 timings of 120 layer shapes (40 to 3500 rows): the
+// chosen shape is within 2 % of the best one on average and 19 % at worst.
 static LinShape pick_shape(int rows, int n, int chunks, int sms, int dev) {
   LinShape best = {1, 16, 1};
   double best_ns = 1e30;
@@ -821,12 +821,13 @@ static LinShape pick_shape(int rows, int n, int chunks, int sms, int dev) {
     const double waves = static_cast<double>((units + slots - 1) / slots);
     const double ctas = static_cast<double>(units < slots ? units : slots) * (cg == 2 ? 2 : splits);
     const double loaded = kLinCh + static_cast<double>(tokens / cg);
-    double chunk = 1.3 * tokens;
-    if (120.0 + 0.23 * loaded > chunk) chunk = 120.0 + 0.23 * loaded;
-    if (ctas * loaded * (kLinChunk / 9200.0) > chunk) chunk = ctas * loaded * (kLinChunk / 9200.0);
-    const double tile = chunk * ((chunks + splits - 1) / splits), epilogue = 6.0 * tokens;
+    double chunk = 1.29 * tokens;
+    if (126.0 + 0.25 * loaded > chunk) chunk = 126.0 + 0.25 * loaded;
+    if (ctas * loaded * (kLinChunk / 9290.0) > chunk) chunk = ctas * loaded * (kLinChunk / 9290.0);
+    const double tile = chunk * ((chunks + splits - 1) / splits), epilogue = 1.95 * tokens;
     double ns = waves * tile + epilogue + (epilogue > tile ? (waves - 1) * (epilogue - tile) : 0.0);
-    if (splits > 1) ns += 1200.0 + 7.0 * tokens + 30.0 * splits;
+    if (splits > 1) ns += 953.0 + 7.0 * tokens + 26.0 * splits;
+    if (cg == 2) ns += 87.0;
     if (ns < best_ns) best_ns = ns, best = {cg, tokens, splits};
   };
   for (int tokens = 16; tokens <= kLinMaxTokens; tokens += tokens < 32 ? 16 : 32) {
