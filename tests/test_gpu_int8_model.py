@@ -1,6 +1,6 @@
 """GPU: the decoder and the SpecDec engine with 8-bit projections (PagedModel(weights="int8")).
 
-The checker is the model-level oracle with every projection replaced by its 8-bit definition (rows and
+The expected values come from the model-level oracle with every projection replaced by its 8-bit definition (rows and
 output channels quantised as in oracle/int8.py, products in fp32), fed like the kernels are: norms in fp32
 from the unrounded sum of the residual and the last projection, SwiGLU in fp32.  What is left between the
 two are fp32 orders of summation and the attention's bf16 roundings, so the logits are held to the bar that
