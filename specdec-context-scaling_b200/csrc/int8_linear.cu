@@ -41,7 +41,7 @@ constexpr int kLinThreads = 32 * (kLinEpiWarps + 2);
 constexpr int kLinChunk = 128;                   // codes of K per stage
 constexpr int kLinCh = 128;                      // channels per CTA
 constexpr int kLinWTile = kLinCh * kLinChunk;    // 16 KB
-constexpr int kLinMaxStages = 12;
+constexpr int kLinMaxStages = 11;
 constexpr int kLinRing = 204 * 1024;
 constexpr int kLinMaxTokens = 256;
 
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 constexpr int kFewRows = 32;
 constexpr int kFewCh = 16;
 constexpr int kFewStep = 64;
-constexpr int kFewAhead = 4;  // steps whose loads of a are under way together (of W: 4, or all of a warp's share up to 9)
+constexpr int kFewAhead = 4;  // steps whose loads of a are under way together (of W: all of a warp's share, or 5 to 9 at a time)
 
 struct FewParams {
   const int8_t* a;
@@ -926,9 +926,11 @@ static int launch_few(const FewParams& p, cudaStream_t st) {
   const int steps = (p.width + kFewStep - 1) / kFewStep;
   if (steps <= 16) return launch_few_as<NB, 8, 2, T>(p, st);
   if (steps <= 24) return launch_few_as<NB, 8, 3, T>(p, st);
-  if (steps <= 32) return launch_few_as<NB, 8, 4, T>(p, st);
-  if (steps <= 80) return launch_few_long<NB, NB < 4 ? 5 : 4, T>(p, st);
-  return launch_few_long<NB, NB == 1 ? 9 : NB == 2 ? 6 : 4, T>(p, st);
+  if (NB == 4 || steps <= 32) return launch_few_as<NB, 8, 4, T>(p, st);  // (few_rows: NB = 4 has K <= 2048)
+  if constexpr (NB < 4) {
+    if (steps <= 80) return launch_few_long<NB, 5, T>(p, st);
+    return launch_few_long<NB, NB == 1 ? 9 : 6, T>(p, st);
+  }
 }
 
 }  // namespace sd
