@@ -25,7 +25,7 @@
 // POP/s, twice the bf16 rate of the library's product (3.29).  With K = 1536 and 17920 channels the
 // output (1.2 GB for 32768 rows) shares L2 with those loads: 617-700 us, 2.6-2.9 POP/s.
 // splits > 1 (CG = 1): a cluster of `splits` CTAs shares one tile, each taking a share of the
-// chunks of K, and adds up the integer partial sums through distributed shared memory.
+// chunks of K and pushing its integer partial sums into the shared memory of the CTA that adds them up.
 #include <cudaTypedefs.h>
 
 #include "sd_common.cuh"
@@ -44,6 +44,7 @@ constexpr int kLinWTile = kLinCh * kLinChunk;    // 16 KB
 constexpr int kLinMaxStages = 11;
 constexpr int kLinRing = 204 * 1024;
 constexpr int kLinMaxTokens = 256;
+constexpr int kLinSplitTokens = 128;             // of a split tile: its partial sums take 512 bytes each
 
 struct LinParams {
   const float* a_scale;
@@ -146,6 +147,19 @@ SD_DEV void tma_codes(void* dst, const CUtensorMap* map, int32_t k, int32_t row,
 SD_DEV void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The same with a release: what this thread wrote, or saw written before a barrier, to that CTA is there.
+SD_DEV void mbar_arrive_release_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+SD_DEV void dsmem_st_s32(uint32_t addr, int32_t v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+// warp_wait that also acquires what other CTAs of the cluster released
+SD_DEV bool warp_wait_cluster(uint64_t* bar, uint32_t parity) {
+  const bool ok = warp_wait(bar, parity);
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  return ok;
+}
 SD_DEV void tmem_ld16_s32(uint32_t ta, int32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -177,15 +191,6 @@ SD_DEV void stmatrix_trans(uint32_t addr, uint32_t m0, uint32_t m1, uint32_t m2,
                "r"(m2), "r"(m3)
                : "memory");
 }
-SD_DEV int4 dsmem_ld4_s32(uint32_t addr) {
-  int4 v;
-  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
 template <typename T>
 SD_DEV void store_out(T* p, float v) {
   if constexpr (sizeof(T) == 4)
@@ -261,13 +266,12 @@ SD_DEV void store_fragments(const int32_t (&v)[16], const float* s_scale, const 
   if (!GUARD || (ch_ok && (lane >> 2) + 8 < ntok)) *reinterpret_cast<uint4*>(o + half) = r1;
 }
 
-// A split tile's partial sums, [token][128 channels] in each CTA's shared memory: CTA `rank` takes every
-// SPLITS-th token, a warp a token, a lane four channels.  16 loads a lane are under way at once: one
-// token's at a time left a microsecond of latency for each.
-template <int SPLITS, typename T>
-SD_DEV void add_partials(const LinParams& p, const uint8_t* smem, int rank, int unit) {
-  constexpr int kAtOnce = 16 / SPLITS, kStep = SPLITS * (kLinThreads / 32);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// A split tile: the CTAs of the cluster have pushed their partial sums of this CTA's tokens (every
+// `splits`-th, from `rank` on) into `got` [split][token][128 channels]; a warp adds up a token, a lane four
+// channels.
+template <typename T>
+SD_DEV void add_partials(const LinParams& p, const int32_t* got, int rank, int unit) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = p.tokens / p.splits;
   const int tt = unit / p.ch_tiles, ct = unit - tt * p.ch_tiles;
   const int n = ct * kLinCh + lane * 4;
   const int tok0 = tt * p.tokens, ntok = min(p.tokens, p.rows - tok0);
@@ -278,46 +282,31 @@ SD_DEV void add_partials(const LinParams& p, const uint8_t* smem, int rank, int 
       sw[j] = p.w_scale[n + j];
       if (p.bias) bias[j] = p.bias[n + j];
     }
-  uint32_t from[SPLITS];
-#pragma unroll
-  for (int r = 0; r < SPLITS; ++r) from[r] = dsmem_addr(smem_u32(smem) + lane * 16, r);
-  for (int c0 = rank + SPLITS * warp; c0 < ntok; c0 += kAtOnce * kStep) {
-    int4 v[kAtOnce][SPLITS];
-    float sa[kAtOnce];
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int c = c0 + i * kStep;
-      if (c < ntok) {
-        sa[i] = p.a_scale[tok0 + c];
-#pragma unroll
-        for (int r = 0; r < SPLITS; ++r) v[i][r] = dsmem_ld4_s32(from[r] + c * (kLinCh * 4));
-      }
+  for (int i = warp; i < share; i += kLinEpiWarps) {
+    const int c = rank + p.splits * i;
+    if (c >= ntok) break;
+    const float sa = p.a_scale[tok0 + c];
+    int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 8
+    for (int r = 0; r < p.splits; ++r) {
+      const int4 v = *reinterpret_cast<const int4*>(got + (r * share + i) * kLinCh + lane * 4);
+      sum.x += v.x;
+      sum.y += v.y;
+      sum.z += v.z;
+      sum.w += v.w;
     }
+    const float y[4] = {scaled(sum.x, sa, sw[0], bias[0]), scaled(sum.y, sa, sw[1], bias[1]),
+                        scaled(sum.z, sa, sw[2], bias[2]), scaled(sum.w, sa, sw[3], bias[3])};
+    T* o = static_cast<T*>(p.out) + (tok0 + c) * p.out_stride + n;
+    if (p.vec_out && n + 4 <= p.n) {
+      if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
+      else
+        *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+    } else {
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int c = c0 + i * kStep;
-      if (c >= ntok) break;
-      int4 sum = v[i][0];
-#pragma unroll
-      for (int r = 1; r < SPLITS; ++r) {
-        sum.x += v[i][r].x;
-        sum.y += v[i][r].y;
-        sum.z += v[i][r].z;
-        sum.w += v[i][r].w;
-      }
-      const float y[4] = {scaled(sum.x, sa[i], sw[0], bias[0]), scaled(sum.y, sa[i], sw[1], bias[1]),
-                          scaled(sum.z, sa[i], sw[2], bias[2]), scaled(sum.w, sa[i], sw[3], bias[3])};
-      T* o = static_cast<T*>(p.out) + (tok0 + c) * p.out_stride + n;
-      if (p.vec_out && n + 4 <= p.n) {
-        if constexpr (sizeof(T) == 4)
-          *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
-        else
-          *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.n) store_out(o + j, y[j]);
-      }
+      for (int j = 0; j < 4; ++j)
+        if (n + j < p.n) store_out(o + j, y[j]);
     }
   }
 }
@@ -329,7 +318,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                        const __grid_constant__ CUtensorMap wmap) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kLinMaxStages], empty[kLinMaxStages], acc_full[2], acc_empty[2], given_up;
+  __shared__ uint64_t full[kLinMaxStages], empty[kLinMaxStages], acc_full[2], acc_empty[2], given_up, partials;
   __shared__ uint32_t tmem_base;
   __shared__ __align__(16) float s_scale[kLinEpiWarps][kLinMaxTokens / 2];
   __shared__ __align__(128) uint8_t s_stage[kLinEpiWarps][1024];
@@ -347,6 +336,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       mbar_init(&acc_empty[b], kLinEpiWarps * CG);
     }
     mbar_init(&given_up, 1);
+    mbar_init(&partials, csize);
     fence_barrier_init();
   }
   if (warp == kLinEpiWarps && lane == 0) {
@@ -355,10 +345,13 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   }
   if (warp == kLinEpiWarps + 1) tmem_alloc_cg<CG>(&tmem_base, p.tmem_cols);
   umma::fence_before_sync();
-  if (CG == 2)
+  __syncwarp();
+  if (CG == 2) {
     cluster_sync();  // the partner's barriers are signalled from here on
-  else
+  } else {
+    if (csize > 1) cluster_arrive();  // partial sums are pushed once every CTA of the cluster is here
     __syncthreads();
+  }
   umma::fence_after_sync();
   const uint32_t tbase = tmem_base;
   const int a_rows = p.tokens / CG;  // rows of a this CTA loads
@@ -424,6 +417,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     // ... or, after a wait that gave up, at least the copies under way have landed
     for (int i = 0; i < p.stages && stop && (CG == 1 || rank == 0); ++i)
       (void)warp_wait(&full[i], i < s ? parity ^ 1 : parity);
+    if (CG == 1 && csize > 1) cluster_wait();
   } else if (warp == kLinEpiWarps + 1) {
     // ---- MMA issuer
     if (rank % CG == 0) {
@@ -475,6 +469,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         (void)warp_wait(&given_up, 0);
       }
     }
+    __syncwarp();
+    if (CG == 1 && csize > 1) cluster_wait();
   } else {
     // ---- epilogue: lane = channel, columns = tokens; two warps share a lane quarter, each half the tokens
     grid_dep_wait();
@@ -504,6 +500,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       }
     };
     if (p.splits == 1 && unit0 < p.units) load_scales();
+    int32_t* got = reinterpret_cast<int32_t*>(smem + p.stages * stage_bytes);  // splits: pushed partial sums
+    if (CG == 1 && csize > 1) cluster_wait();
     int ui = 0;
     for (int u = unit0; u < p.units; u += unit_step, ++ui) {
       const int b = ui & 1;
@@ -579,15 +577,19 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           }
         }
       } else {
-        // the partial sums take the ring's place: every product that read it is complete
-        int32_t* part = reinterpret_cast<int32_t*>(smem) + quarter * 32 + lane;
+        // token c goes to CTA c % splits, as its (c / splits)-th
+        const int log2 = __ffs(p.splits) - 1, share = p.tokens >> log2;
+        const uint32_t mine = smem_u32(got) + (rank * share * kLinCh + quarter * 32 + lane) * 4;
 #pragma unroll 1
         for (int c = c0; c < c1; c += 16) {
           int32_t v[16];
           tmem_ld16_s32(ta + c, v);
           tmem_wait_ld16(v);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) part[(c + i) * kLinCh] = v[i];
+          for (int i = 0; i < 16; ++i) {
+            const int to = (c + i) & (p.splits - 1), at = (c + i) >> log2;
+            dsmem_st_s32(dsmem_addr(mine + at * (kLinCh * 4), to), v[i]);
+          }
         }
       }
       umma::fence_before_sync();
@@ -599,28 +601,27 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           mbar_arrive(&acc_empty[b]);
       }
     }
+    if (CG == 1 && csize > 1) {
+      // this CTA's partial sums are out, whatever became of its waits; then those of the others are in
+      named_bar_sync(1, 32 * kLinEpiWarps);
+      if (threadIdx.x < csize) mbar_arrive_release_cluster(dsmem_addr(smem_u32(&partials), threadIdx.x));
+      __syncwarp();
+      if (warp_wait_cluster(&partials, 0) || warp_wait_cluster(&partials, 0))
+        add_partials<T>(p, got, rank, unit0);
+      else if (lane == 0)
+        raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+    }
   }
 
   umma::fence_before_sync();
   __syncwarp();
-  if (csize > 1)
+  if (CG == 2)
     cluster_sync();
   else
     __syncthreads();
   if (warp == kLinEpiWarps + 1) {
     umma::fence_after_sync();
     tmem_dealloc_cg<CG>(tbase, p.tmem_cols);
-  }
-  if (CG == 1 && csize > 1) {
-    grid_dep_wait();
-    if (csize == 8)
-      add_partials<8, T>(p, smem, rank, unit0);
-    else if (csize == 4)
-      add_partials<4, T>(p, smem, rank, unit0);
-    else
-      add_partials<2, T>(p, smem, rank, unit0);
-    __syncwarp();
-    cluster_sync();  // the peers have read this CTA's shared memory
   }
 }
 
@@ -817,7 +818,7 @@ static LinShape pick_shape(int rows, int n, int chunks, int sms, int dev) {
   const auto consider = [&](int cg, int tokens, int splits) {
     const int64_t units = static_cast<int64_t>((n + cg * kLinCh - 1) / (cg * kLinCh)) * ((rows + tokens - 1) / tokens);
     const int slots = cg == 2 ? sms / 2 : splits > 1 ? resident_clusters(splits, dev, sms) : sms;
-    if (splits > 1 && units > slots) return;
+    if (splits > 1 && (units > slots || tokens > kLinSplitTokens)) return;
     const double waves = static_cast<double>((units + slots - 1) / slots);
     const double ctas = static_cast<double>(units < slots ? units : slots) * (cg == 2 ? 2 : splits);
     const double loaded = kLinCh + static_cast<double>(tokens / cg);
@@ -996,13 +997,15 @@ extern "C" int specdec_linear_int8(const void* a, int64_t a_stride, const float*
   p.vec_out = (reinterpret_cast<uintptr_t>(out) % (4 * esize)) == 0 && out_stride % 4 == 0;
   p.rows16 = (reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(out_stride * esize) | static_cast<uintptr_t>(out_features) * esize) % 16 == 0;
   const int stage = kLinWTile + p.tokens / shape.cg * kLinChunk;
-  p.stages = kLinRing / stage < kLinMaxStages ? kLinRing / stage : kLinMaxStages;
+  const int pushed = p.splits > 1 ? p.tokens * kLinCh * 4 : 0;
+  const int most = (kLinRing - pushed) / stage;
+  p.stages = most < kLinMaxStages ? most : kLinMaxStages;
   p.tmem_cols = 32;
   while (p.tmem_cols < 2 * p.tokens) p.tmem_cols *= 2;
   CUtensorMap amap, wmap;
   if (int rc = encode_codes(&amap, a, width, rows, a_stride, p.tokens / shape.cg)) return rc;
   if (int rc = encode_codes(&wmap, w, width, out_features, w_stride, kLinCh)) return rc;
-  const int smem = p.stages * stage + 1024;
+  const int smem = p.stages * stage + pushed + 1024;
   if (shape.cg == 2) {
     const int grid = 2 * (p.units < sms / 2 ? p.units : sms / 2);
     return out_dtype == SPECDEC_F32 ? launch_linear<2, float>(p, amap, wmap, grid, smem, dev, st)
