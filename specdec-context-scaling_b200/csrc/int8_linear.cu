@@ -808,10 +808,10 @@ static int resident_clusters(int size, int dev, int sms);
 
 // Launch shape by an estimate of the time of a call in ns.  A 128-code chunk of K costs a CTA the largest
 // of its products (1.29 a token: 128 x 128 x 32 products in 64 clocks), what issuing its loads, waits and
-// products takes (126, and 0.25 a row loaded) and its share of L2's bandwidth (9.3 TB/s); the tiles of a
-// CTA follow one another in waves, each hiding the previous one's epilogue (2 a token); a split adds the
-// exchange of the partial sums.  The figures fit 3500 timings of 120 layer shapes (40 to 3500 rows): the
-// chosen shape is within 2 % of the best one on average and 19 % at worst.
+// products takes (108, or 92 in a pair, and 0.43 a row loaded) and its share of L2's bandwidth (9.3 TB/s);
+// the tiles of a CTA follow one another in waves, each hiding the previous one's epilogue (1.35 a token); a
+// pair costs 155 more, a split the exchange of the partial sums.  The figures fit 3000 timings of 120 layer
+// shapes (40 to 3500 rows): the chosen shape is within 2 % of the best one on average and 15 % at worst.
 static LinShape pick_shape(int rows, int n, int chunks, int sms, int dev) {
   LinShape best = {1, 16, 1};
   double best_ns = 1e30;
@@ -823,12 +823,13 @@ static LinShape pick_shape(int rows, int n, int chunks, int sms, int dev) {
     const double ctas = static_cast<double>(units < slots ? units : slots) * (cg == 2 ? 2 : splits);
     const double loaded = kLinCh + static_cast<double>(tokens / cg);
     double chunk = 1.29 * tokens;
-    if (126.0 + 0.25 * loaded > chunk) chunk = 126.0 + 0.25 * loaded;
+    const double issue = (cg == 2 ? 92.0 : 108.0) + 0.43 * loaded;
+    if (issue > chunk) chunk = issue;
     if (ctas * loaded * (kLinChunk / 9290.0) > chunk) chunk = ctas * loaded * (kLinChunk / 9290.0);
-    const double tile = chunk * ((chunks + splits - 1) / splits), epilogue = 1.95 * tokens;
+    const double tile = chunk * ((chunks + splits - 1) / splits), epilogue = 1.35 * tokens;
     double ns = waves * tile + epilogue + (epilogue > tile ? (waves - 1) * (epilogue - tile) : 0.0);
-    if (splits > 1) ns += 953.0 + 7.0 * tokens + 26.0 * splits;
-    if (cg == 2) ns += 87.0;
+    if (splits > 1) ns += 858.0 + 5.1 * tokens + 50.0 * splits;
+    if (cg == 2) ns += 155.0;
     if (ns < best_ns) best_ns = ns, best = {cg, tokens, splits};
   };
   for (int tokens = 16; tokens <= kLinMaxTokens; tokens += tokens < 32 ? 16 : 32) {
