@@ -597,9 +597,10 @@ def _int8_out(x, dev: int, rows: int, width: int, codes, scale):
     stride that is a multiple of 16 bytes, as linear_int8 reads them."""
     if codes is None:
         stride = (width + 15) & ~15
-        codes = torch.empty(rows, stride, dtype=_I8, device=x.device)
-        if stride != width:
-            codes = codes[:, :width]
+        if stride == width:
+            codes = torch.empty(rows, width, dtype=_I8, device=x.device)
+        else:
+            codes = torch.empty_strided((rows, width), (stride, 1), dtype=_I8, device=x.device)
     else:
         _on_device(dev, codes)
         if codes.dtype is not _I8 or codes.shape != (rows, width) or codes.stride(1) != 1 and width != 1:
@@ -651,9 +652,10 @@ def rmsnorm_int8(x, weight, eps: float = 1e-6, *, residual=None, summed=None, co
     else:
         if summed is None:  # rows on 16-byte boundaries, so the next call on it reads aligned rows
             ss = (hidden + 7) & ~7
-            summed = torch.empty(rows, ss, dtype=x.dtype, device=x.device)
-            if ss != hidden:
-                summed = summed[:, :hidden]
+            if ss == hidden:
+                summed = torch.empty(rows, hidden, dtype=x.dtype, device=x.device)
+            else:
+                summed = torch.empty_strided((rows, hidden), (ss, 1), dtype=x.dtype, device=x.device)
         else:
             ss = _like_x(summed, x)
         rs = _like_x(residual, x)
