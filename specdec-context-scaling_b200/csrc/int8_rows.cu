@@ -174,11 +174,13 @@ template <int OP>
 SD_DEV RowScale row_scale(const RowArgs& a, float2 r) {
   RowScale s;
   s.rms = 1.f;
+  bool finite = true;
   if (kIsNorm<OP>) {
+    finite = r.x <= 3.4028234663852886e38f;  // an infinite sum of finite values would make 1 / rms, and the row, zero
     s.rms = __fdiv_rn(1.f, __fsqrt_rn(r.x / static_cast<float>(a.width) + a.eps));
     r.y *= s.rms;
   }
-  if (!(r.y <= 3.4028234663852886e38f)) {
+  if (!finite || !(r.y <= 3.4028234663852886e38f)) {
     s.rms = s.inv = 0.f;
     s.scale = __int_as_float(0x7FC00000);
     return s;

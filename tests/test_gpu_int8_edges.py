@@ -1,0 +1,35 @@
+"""GPU: the 8-bit linear path at the edges of its definitions."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import int8 as o8
+from test_gpu_int8 import _assert_codes, _gen, _hidden, _ops, U
+
+pytestmark = pytest.mark.gpu
+
+
+# registers (aligned, then a few unaligned rows), the ring (aligned, unaligned), rows read twice
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,width", [(5, 1536), (1300, 896), (5, 1001), (6, 6001), (1200, 12000), (1300, 1001),
+                                        (5, 60000)])
+def test_rmsnorm_sum_of_squares_past_fp32(rows, width, residual, dtype):
+    """Finite values whose squares sum past fp32's largest number: scale NaN and codes 0, like a row that is not
+    finite; the rows beside it, one of them just below the limit, are untouched."""
+    x = _hidden(rows, width, dtype, rows + width).clone()
+    x[1] = 1e20            # a square alone passes
+    x[2] = 0
+    x[2, :5] = 1.8e19      # each square (3.24e38) fits, their sum does not
+    x[3] = 0
+    x[3, width // 2] = 1e19  # one square of 1e38: fits
+    r = torch.zeros_like(x) if residual else None
+    w = (torch.rand(width, generator=_gen(3)) + 0.5).to(dtype).cuda()
+    codes, scale, _ = _ops().rmsnorm_int8(x, w, residual=r)
+    assert torch.isnan(scale).nonzero().flatten().tolist() == [1, 2]
+    assert (codes[1:3] == 0).all()
+    keep = torch.tensor([i for i in range(rows) if i not in (1, 2)], device="cuda")
+    y, _ = o8.rmsnorm_rows(x[keep], w, 1e-6)
+    _assert_codes(codes[keep], scale[keep], y, ((width / 32 + 16) / 2 + 8) * U)
