@@ -633,7 +633,11 @@ static int launch_stream(const char* what, const RowArgs& a, bool vec, cudaStrea
 // under eight rows an SM).  Longer ones, swiglu's long ones in large
 // number (its arithmetic hides behind the ring's copies: 8192 x 8960 62 us, 95 in registers) and unaligned
 // ones in large number through shared memory; unaligned rows in small number by single values, a block a
-// row, and so are rows whose outputs are not aligned.
+// row, and so are rows whose outputs are not aligned, and unaligned f32 rows of 897 to 1024 values, which a
+// block of 256 threads still holds while the ring needs four warps each (norm without a residual, 1001 values:
+// 600 rows 3.4 us either way, 2000 5.5 and 7.1 in the ring, 8000 17.2 and 19.6).  Unaligned norms without a
+// residual by single values and in the ring, us: 600 x 501 bf16 3.1 and 2.9, 1000 x 1501 bf16 11.8 and 4.5,
+// 8000 x 1501 bf16 81.6 and 14.9, f32 79.4 and 22.3.
 template <typename T, int OP>
 static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
@@ -659,7 +663,8 @@ static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
     if (need <= 768) return launch_rows_as<T, OP, 256, V, 3>(what, a, st);
     if (need <= 1280 && (few || OP != kRowSwiglu)) return launch_rows_as<T, OP, 256, V, 5>(what, a, st);
   }
-  if (out_vec && (vec || need > 8192 || a.rows > (need > 1024 ? 1 : 4) * sms))
+  const bool held = !vec && a.width <= 1024 && a.width > 32 * stream_pieces(1) * V;
+  if (out_vec && !held && (vec || need > 8192 || a.rows > (need > 1024 ? 1 : 4) * sms))
     if (const int rc = launch_stream<T, OP>(what, a, vec, st); rc != SPECDEC_ERR_UNSUPPORTED) return rc;
   if (a.width <= 1024) return launch_rows_as<T, OP, 256, 1, 4>(what, a, st);
   if (a.width <= 8192) return launch_rows_as<T, OP, 1024, 1, 8>(what, a, st);
@@ -735,11 +740,11 @@ extern "C" int specdec_rmsnorm_int8(const void* x, int64_t x_stride, const void*
   a.x = x;
   a.x_stride = x_stride;
   a.residual = residual;
-  a.r_stride = residual_stride;
+  a.r_stride = residual ? residual_stride : 0;  // of no account without one: they would decide the kernel
   a.weight = weight;
   a.eps = eps;
   a.summed = summed;
-  a.s_stride = summed_stride;
+  a.s_stride = residual ? summed_stride : 0;
   a.codes = static_cast<int8_t*>(codes);
   a.c_stride = codes_stride;
   a.scale = scale;

@@ -33,3 +33,16 @@ def test_rmsnorm_sum_of_squares_past_fp32(rows, width, residual, dtype):
     keep = torch.tensor([i for i in range(rows) if i not in (1, 2)], device="cuda")
     y, _ = o8.rmsnorm_rows(x[keep], w, 1e-6)
     _assert_codes(codes[keep], scale[keep], y, ((width / 32 + 16) / 2 + 8) * U)
+
+
+@pytest.mark.parametrize("rows,width,dtype", [(1300, 1001, torch.bfloat16), (777, 1001, torch.float32),
+                                              (1200, 2501, torch.bfloat16), (300, 6001, torch.float32)])
+def test_rmsnorm_without_residual_is_that_of_a_zero_residual(rows, width, dtype):
+    """The same rows take the same kernel, and so the same order of summation, whether or not there is a residual:
+    equal bits."""
+    ops = _ops()
+    x = _hidden(rows, width, dtype, rows + width)
+    w = (torch.rand(width, generator=_gen(3)) + 0.5).to(dtype).cuda()
+    codes, scale, _ = ops.rmsnorm_int8(x, w)
+    codes0, scale0, _ = ops.rmsnorm_int8(x, w, residual=torch.zeros_like(x))
+    assert torch.equal(scale, scale0) and torch.equal(codes, codes0)
