@@ -419,10 +419,15 @@ int specdec_umma_selftest(const void* k, const void* q, const void* v, const voi
      mode 0: one CTA waits on an mbarrier that nothing arrives on (grid must be 1);
      mode 1: `grid` CTAs (1 .. 8) meet at the grid barrier of the verify kernel expecting
              `n_ctas` arrivals on the zeroed device u64 `counter` (n_ctas > grid times out,
-             n_ctas == grid passes).
+             n_ctas == grid passes);
+     mode 3: mode 0 by a CTA that first lets the next kernel on the stream start (a predecessor that runs on
+             for limit_ns while a programmatically launched successor is already there).
    waited_ns (device u64, may be NULL) receives the time CTA 0 spent in its wait. */
 int specdec_wait_selftest(int32_t mode, void* counter, int32_t n_ctas, int32_t grid, int64_t limit_ns,
                           int32_t* status, void* waited_ns, specdec_stream_t stream);
+/* Limit, 0 .. 1e9 ns, of the device waits in the 8-bit kernels that the calling thread launches from here on, so
+   that their give-up paths can be tested; one second unless set.  0: a wait that is not over at once gives up. */
+int specdec_wait_limit_selftest(int64_t limit_ns);
 const char* specdec_last_error(void);
 int specdec_abi_version(void);
 /* Number of kernels this library launched since load (all entry points). */

@@ -11,6 +11,7 @@
 namespace {
 thread_local char g_last_error[512] = "";
 std::atomic<int64_t> g_launches{0};
+thread_local uint64_t g_wait_limit_ns = 1000000000;
 std::mutex g_sm_mutex;
 int g_sm_count[64] = {0};
 }  // namespace
@@ -32,6 +33,8 @@ int after_launch(const char* what, int n) {
   return SPECDEC_OK;
 }
 
+uint64_t wait_limit_ns() { return g_wait_limit_ns; }
+
 int device_sm_count() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
@@ -47,5 +50,11 @@ int device_sm_count() {
 }  // namespace sd
 
 extern "C" const char* specdec_last_error(void) { return g_last_error; }
+extern "C" int specdec_wait_limit_selftest(int64_t limit_ns) {
+  if (limit_ns < 0 || limit_ns > 1000000000)
+    return sd::fail(SPECDEC_ERR_INVALID, "wait limit must be 0 .. 1 s");
+  g_wait_limit_ns = static_cast<uint64_t>(limit_ns);
+  return SPECDEC_OK;
+}
 extern "C" int specdec_abi_version(void) { return SPECDEC_ABI_VERSION; }
 extern "C" int64_t specdec_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }

@@ -60,6 +60,7 @@ struct LinParams {
   int32_t vec_out;  // four outputs of a row can be stored at once
   int32_t rows16;   // rows of the output are 16-byte aligned and whole 16-byte pieces
   int32_t* status;
+  uint64_t wait_ns;  // limit of a wait
 };
 
 // ---------------------------------------------------------------- PTX of this kernel
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         waited = true;
       }
       for (; k < k_end; ++k) {
-        if (!warp_wait(&empty[s], parity)) {
+        if (!warp_wait(&empty[s], parity, p.wait_ns)) {
           if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
           stop = true;
           break;
@@ -421,6 +422,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   } else if (warp == kLinEpiWarps + 1) {
     // ---- MMA issuer
     if (rank % CG == 0) {
+      grid_dep_wait();  // a is loaded after the preceding kernel is over: the limit of the first wait starts here, too
       const uint32_t idesc = idesc_i8(kLinCh * CG, p.tokens);
       const uint32_t ring = smem_u32(smem);
       int s = 0, ui = 0;
@@ -430,14 +432,14 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       for (int u = unit0; u < p.units && ok; u += unit_step, ++ui) {
         const int b = ui & 1;
         // accumulator b is free once the epilogue has read unit ui - 2
-        if (ui >= 2 && !warp_wait(&acc_empty[b], ((ui >> 1) - 1) & 1)) {
+        if (ui >= 2 && !warp_wait(&acc_empty[b], ((ui >> 1) - 1) & 1, p.wait_ns)) {
           ok = false;
           break;
         }
         umma::fence_after_sync();
         const uint32_t d = umma::taddr(tbase, 0, b * (p.tmem_cols / 2));
         for (int k = k_begin; k < k_end; ++k) {
-          if (!__all_sync(0xffffffffu, ready) && !warp_wait(&full[s], parity)) {
+          if (!__all_sync(0xffffffffu, ready) && !warp_wait(&full[s], parity, p.wait_ns)) {
             ok = false;
             break;
           }
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       ct += step_ct;
       if (ct >= p.ch_tiles) ct -= p.ch_tiles, ++tt;
       if (p.splits == 1 && u + unit_step < p.units) load_scales();
-      if (!warp_wait(&acc_full[b], (ui >> 1) & 1)) {
+      if (!warp_wait(&acc_full[b], (ui >> 1) & 1, p.wait_ns)) {
         if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
         break;
       }
@@ -994,6 +996,7 @@ extern "C" int specdec_linear_int8(const void* a, int64_t a_stride, const float*
   p.units = static_cast<int32_t>(units);
   p.weight_ready = weight_ready;
   p.status = status;
+  p.wait_ns = wait_limit_ns();
   const int esize = out_dtype == SPECDEC_F32 ? 4 : 2;
   p.vec_out = (reinterpret_cast<uintptr_t>(out) % (4 * esize)) == 0 && out_stride % 4 == 0;
   p.rows16 = (reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(out_stride * esize) | static_cast<uintptr_t>(out_features) * esize) % 16 == 0;

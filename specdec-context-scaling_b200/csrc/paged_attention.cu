@@ -1742,7 +1742,8 @@ __global__ void __launch_bounds__(32) wait_selftest_kernel(int mode, unsigned lo
   __syncwarp();
   const uint64_t t0 = globaltimer_ns();
   bool ok = true;
-  if (mode == 0) {
+  if (mode == 3) grid_dep_launch();
+  if (mode != 1) {
     ok = __all_sync(0xffffffffu, mbar_wait(&bar, 0, limit_ns));
   } else if (threadIdx.x == 0) {
     ok = grid_barrier(counter, n_ctas, true, limit_ns);
@@ -1756,12 +1757,12 @@ __global__ void __launch_bounds__(32) wait_selftest_kernel(int mode, unsigned lo
 
 extern "C" int specdec_wait_selftest(int32_t mode, void* counter, int32_t n_ctas, int32_t grid, int64_t limit_ns,
                                      int32_t* status, void* waited_ns, specdec_stream_t stream) {
-  if (mode != 0 && mode != 1) return fail(SPECDEC_ERR_INVALID, "wait self-test mode must be 0 or 1");
+  if (mode != 0 && mode != 1 && mode != 3) return fail(SPECDEC_ERR_INVALID, "wait self-test mode must be 0, 1 or 3");
   if (limit_ns < 1000 || limit_ns > 100000000) return fail(SPECDEC_ERR_INVALID, "wait limit must be 1 us .. 100 ms");
   if (grid < 1 || grid > 8) return fail(SPECDEC_ERR_INVALID, "wait self-test grid must be 1 .. 8 CTAs");
   if (mode == 1 && (counter == nullptr || n_ctas < 1))
     return fail(SPECDEC_ERR_INVALID, "grid-barrier self-test needs a zeroed device counter and n_ctas >= 1");
-  if (mode == 0 && grid != 1) return fail(SPECDEC_ERR_INVALID, "mbarrier self-test runs one CTA");
+  if (mode != 1 && grid != 1) return fail(SPECDEC_ERR_INVALID, "mbarrier self-test runs one CTA");
   sd::wait_selftest_kernel<<<grid, 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       mode, static_cast<unsigned long long*>(counter), static_cast<unsigned>(n_ctas),
       static_cast<uint64_t>(limit_ns), status, static_cast<unsigned long long*>(waited_ns));

@@ -15,6 +15,8 @@ namespace sd {
 int fail(int code, const char* fmt, ...);
 // Checks cudaGetLastError() after a launch; counts `n` launches on success.
 int after_launch(const char* what, int n = 1);
+// Limit of the waits in kernels that this thread launches (specdec_wait_limit_selftest); one second.
+uint64_t wait_limit_ns();
 // SM count of the current device (cached per device).
 int device_sm_count();
 

@@ -218,6 +218,7 @@ SIGNATURES = {
         ctypes.c_int,
         [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _vp],
     ),
+    "specdec_wait_limit_selftest": (ctypes.c_int, [_i64]),
     "specdec_last_error": (ctypes.c_char_p, []),
     "specdec_abi_version": (ctypes.c_int, []),
     "specdec_launch_count": (_i64, []),

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import int8 as o8
-from test_gpu_int8 import _assert_codes, _gen, _hidden, _ops, U
+from test_gpu_int8 import _assert_codes, _codes, _gen, _hidden, _ops, _scales, U
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,39 @@ def test_rmsnorm_without_residual_is_that_of_a_zero_residual(rows, width, dtype)
     codes, scale, _ = ops.rmsnorm_int8(x, w)
     codes0, scale0, _ = ops.rmsnorm_int8(x, w, residual=torch.zeros_like(x))
     assert torch.equal(scale, scale0) and torch.equal(codes, codes0)
+
+
+@pytest.fixture
+def wait_limit():
+    """Sets the limit of the 8-bit kernels' device waits for a test; one second again after it."""
+    from specdec_b200 import _lib
+
+    lib = _lib.load_library()
+    yield lambda ns: _lib.check(lib.specdec_wait_limit_selftest(ns), "wait_limit_selftest")
+    torch.cuda.synchronize()
+    lib.specdec_wait_limit_selftest(1_000_000_000)
+
+
+# a tile for each CTA, more tiles than CTAs (pairs), a split of K, a split over few rows
+@pytest.mark.parametrize("rows,width,n", [(333, 1001, 777), (1280, 1536, 17920), (64, 8960, 1536), (40, 4864, 896)])
+@pytest.mark.parametrize("weight_ready", [False, True])
+def test_linear_behind_a_long_predecessor(rows, width, n, weight_ready, wait_limit):
+    """A kernel that lets its successor start and then runs on for four times the limit of a wait: that time is
+    the predecessor's, and no wait of the product gives up."""
+    from specdec_b200 import _lib
+
+    lib = _lib.load_library()
+    ops = _ops()
+    a, w = _codes(rows, width, 1), _codes(n, width, 2)
+    sa, sw = _scales(rows, 1), _scales(n, 2)
+    want = ops.linear_int8(a, sa, w, sw)
+    status, other = (torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(2))
+    out = torch.full_like(want, 7.0)
+    torch.cuda.synchronize()
+    wait_limit(25_000_000)
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.check(lib.specdec_wait_selftest(3, None, 1, 1, 100_000_000, other.data_ptr(), None, stream), "wait_selftest")
+    ops.linear_int8(a, sa, w, sw, out=out, weight_ready=weight_ready, status=status)
+    torch.cuda.synchronize()
+    assert int(status.item()) == 0 and torch.equal(out, want)
+    assert int(other.item()) == _lib.STATUS_TIMEOUT  # the predecessor did run that long

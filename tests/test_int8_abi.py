@@ -101,3 +101,9 @@ def test_struct_free_signatures_match_the_header():
     for name, n in counts.items():
         res, args = _lib.SIGNATURES[f"specdec_{name}_int8"]
         assert res is ctypes.c_int and len(args) == n
+
+
+def test_wait_limit_refuses_what_is_out_of_range(lib):
+    for ns in (-1, 1_000_000_001):
+        assert lib.specdec_wait_limit_selftest(ns) == 1 and "wait limit must be" in _msg(lib)
+    assert lib.specdec_wait_limit_selftest(1_000_000_000) == 0
