@@ -392,7 +392,8 @@ int specdec_dequantize_int8(const void* codes, int64_t codes_stride, const float
  * bf16 (`out_dtype`), rows `out_stride` elements apart.  The sum is exact (width <= 131072), the rest fp32
  * with one rounding to the output type.  rows <= 2^21.
  * weight_ready 1: the caller promises that the work right before the call on the stream does not write w, so
- * the kernel may load it while that work finishes.  status (optional): SPECDEC_STATUS_TIMEOUT.
+ * the kernel may load it while that work finishes.  status (optional): SPECDEC_STATUS_TIMEOUT, when a device
+ * wait gave up after its second; the outputs it stood for are NaN.
  */
 int specdec_linear_int8(const void* a, int64_t a_stride, const float* a_scale, const void* w, int64_t w_stride,
                         const float* w_scale, const float* bias, void* out, int64_t out_stride, int32_t out_dtype,

@@ -199,6 +199,11 @@ SD_DEV void store_out(T* p, float v) {
   else
     *p = __float2bfloat16_rn(v);
 }
+// NaN for this lane's channel of tokens c0 .. c1 - 1: of a tile whose products did not come
+template <typename T>
+SD_DEV void store_lost(T* o, int64_t stride, int c0, int c1) {
+  for (int c = c0; c < c1; ++c) store_out(o + c * stride, __int_as_float(0x7FC00000));
+}
 SD_DEV float scaled(int32_t acc, float sa, float sw, float b) {
   return __fmaf_rn(__fmul_rn(static_cast<float>(acc), sa), sw, b);
 }
@@ -269,9 +274,9 @@ SD_DEV void store_fragments(const int32_t (&v)[16], const float* s_scale, const 
 
 // A split tile: the CTAs of the cluster have pushed their partial sums of this CTA's tokens (every
 // `splits`-th, from `rank` on) into `got` [split][token][128 channels]; a warp adds up a token, a lane four
-// channels.
+// channels.  `lost`: sums are missing, the results are NaN.
 template <typename T>
-SD_DEV void add_partials(const LinParams& p, const int32_t* got, int rank, int unit) {
+SD_DEV void add_partials(const LinParams& p, const int32_t* got, int rank, int unit, bool lost) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = p.tokens / p.splits;
   const int tt = unit / p.ch_tiles, ct = unit - tt * p.ch_tiles;
   const int n = ct * kLinCh + lane * 4;
@@ -286,7 +291,7 @@ SD_DEV void add_partials(const LinParams& p, const int32_t* got, int rank, int u
   for (int i = warp; i < share; i += kLinEpiWarps) {
     const int c = rank + p.splits * i;
     if (c >= ntok) break;
-    const float sa = p.a_scale[tok0 + c];
+    const float sa = lost ? __int_as_float(0x7FC00000) : p.a_scale[tok0 + c];
     int4 sum = make_int4(0, 0, 0, 0);
 #pragma unroll 8
     for (int r = 0; r < p.splits; ++r) {
@@ -321,6 +326,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kLinMaxStages], empty[kLinMaxStages], acc_full[2], acc_empty[2], given_up, partials;
   __shared__ uint32_t tmem_base;
+  __shared__ int32_t lost;  // splits: partial sums of the tile, of whichever CTA, did not come
   __shared__ __align__(16) float s_scale[kLinEpiWarps][kLinMaxTokens / 2];
   __shared__ __align__(128) uint8_t s_stage[kLinEpiWarps][1024];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -338,6 +344,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     }
     mbar_init(&given_up, 1);
     mbar_init(&partials, csize);
+    lost = 0;
     fence_barrier_init();
   }
   if (warp == kLinEpiWarps && lane == 0) {
@@ -415,9 +422,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     // every stage's last use is over before the CTA leaves (bounded; unused stages pass at once) ...
     for (int i = 0, at = s; i < p.stages && !stop; ++i, at = at + 1 == p.stages ? 0 : at + 1)
       stop = !warp_wait(&empty[at], at < s ? parity ^ 1 : parity);
-    // ... or, after a wait that gave up, at least the copies under way have landed
+    // ... or, after a wait that gave up, at least the copies under way have landed (the first such wait that runs
+    // out, for a stage that the pair's other CTA did not fill, has left time enough for all)
     for (int i = 0; i < p.stages && stop && (CG == 1 || rank == 0); ++i)
-      (void)warp_wait(&full[i], i < s ? parity ^ 1 : parity);
+      if (!warp_wait(&full[i], i < s ? parity ^ 1 : parity)) break;
     if (CG == 1 && csize > 1) cluster_wait();
   } else if (warp == kLinEpiWarps + 1) {
     // ---- MMA issuer
@@ -526,8 +534,18 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       ct += step_ct;
       if (ct >= p.ch_tiles) ct -= p.ch_tiles, ++tt;
       if (p.splits == 1 && u + unit_step < p.units) load_scales();
-      if (!warp_wait(&acc_full[b], (ui >> 1) & 1, p.wait_ns)) {
+      if (!(p.wait_ns ? warp_wait(&acc_full[b], (ui >> 1) & 1, p.wait_ns)
+                      : __all_sync(0xffffffffu, mbar_test(&acc_full[b], (ui >> 1) & 1)))) {
         if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+        if (p.splits > 1) {
+          lost = 1;
+        } else {  // no output of this tile and of those after it is left as it was
+          for (; u < p.units; u += unit_step) {
+            const int t0 = u / p.ch_tiles * p.tokens;
+            const int nl = (u % p.ch_tiles * CG + (CG == 2 ? rank : 0)) * kLinCh + quarter * 32 + lane;
+            if (nl < p.n) store_lost(out + t0 * p.out_stride + nl, p.out_stride, c0, min(c1, p.rows - t0));
+          }
+        }
         break;
       }
       umma::fence_after_sync();
@@ -606,12 +624,16 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     if (CG == 1 && csize > 1) {
       // this CTA's partial sums are out, whatever became of its waits; then those of the others are in
       named_bar_sync(1, 32 * kLinEpiWarps);
-      if (threadIdx.x < csize) mbar_arrive_release_cluster(dsmem_addr(smem_u32(&partials), threadIdx.x));
+      if (threadIdx.x < csize) {
+        if (lost) dsmem_st_s32(dsmem_addr(smem_u32(&lost), threadIdx.x), 1);
+        mbar_arrive_release_cluster(dsmem_addr(smem_u32(&partials), threadIdx.x));
+      }
       __syncwarp();
-      if (warp_wait_cluster(&partials, 0) || warp_wait_cluster(&partials, 0))
-        add_partials<T>(p, got, rank, unit0);
-      else if (lane == 0)
-        raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      // Twice the limit of the one wait that another CTA's push can stand behind, counted from this CTA's own
+      // push: a CTA leaves only when nothing more is pushed to it.
+      const bool in = warp_wait_cluster(&partials, 0) || warp_wait_cluster(&partials, 0);
+      if (!in && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      add_partials<T>(p, got, rank, unit0, !in || lost);
     }
   }
 

@@ -742,7 +742,8 @@ def linear_int8(codes, scale, weight_codes, weight_scale, *, bias=None, out=None
     (as ``quantize_int8`` lays them out), ``scale``, ``weight_scale`` and ``bias`` f32, ``out`` f32 or bf16.
     The integer sum is exact; the rest is fp32, rounded once.  ``weight_ready``: the caller promises that the
     work right before this call on the stream does not write ``weight_codes``, so they may be loaded early.
-    ``status``: a device int32 that receives the library's status bits (a wait that timed out)."""
+    ``status``: a device int32 that receives the library's status bits (a wait that timed out; the outputs it
+    stood for are NaN)."""
     lib, dev, stream = _int8_call(codes)
     rows, width, cs = _check_codes(codes, "codes")
     n, w_width, ws = _check_codes(weight_codes, "weight_codes")

@@ -82,3 +82,32 @@ def test_linear_behind_a_long_predecessor(rows, width, n, weight_ready, wait_lim
     torch.cuda.synchronize()
     assert int(status.item()) == 0 and torch.equal(out, want)
     assert int(other.item()) == _lib.STATUS_TIMEOUT  # the predecessor did run that long
+
+
+# a tile for each CTA, several tiles a CTA (pairs, single CTAs, f32), a split of K, unaligned outputs
+@pytest.mark.parametrize("rows,width,n,out_dtype", [(333, 1001, 777, torch.float32), (1280, 1536, 17920, torch.bfloat16),
+                                                    (1280, 1536, 17920, torch.float32), (4099, 384, 1153, torch.bfloat16),
+                                                    (64, 8960, 1536, torch.bfloat16), (40, 4864, 897, torch.float32)])
+def test_linear_marks_what_its_waits_gave_up_on(rows, width, n, out_dtype, wait_limit):
+    """Waits that give up at once: the status bit is raised, no output keeps what the buffer held before (each is
+    NaN, or the product), nothing beside the output is written, and the next call is right."""
+    from specdec_b200 import _lib
+
+    ops = _ops()
+    a, w = _codes(rows, width, 1), _codes(n, width, 2)
+    sa, sw = _scales(rows, 1), _scales(n, 2)
+    want = ops.linear_int8(a, sa, w, sw, out_dtype=out_dtype)
+    buf = torch.full((rows + 2, n), 7.0, dtype=out_dtype, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    wait_limit(0)
+    out = ops.linear_int8(a, sa, w, sw, out=buf[1:-1], status=status)
+    torch.cuda.synchronize()
+    lost = torch.isnan(out)
+    assert int(status.item()) == _lib.STATUS_TIMEOUT and lost.any()
+    assert torch.equal(out[~lost], want[~lost])
+    assert (buf[0] == 7).all() and (buf[-1] == 7).all()
+    wait_limit(1_000_000_000)
+    status.zero_()
+    assert torch.equal(ops.linear_int8(a, sa, w, sw, out_dtype=out_dtype, status=status), want)
+    assert int(status.item()) == 0
