@@ -365,7 +365,7 @@ int specdec_swiglu_packed(const void* gate_up, void* out, int64_t rows, int64_t 
  * (everything computed from it is NaN).  Activations are f32 or bf16 (`dtype`), rows
  * `x_stride` elements apart with contiguous columns; code rows are `codes_stride` bytes apart.
  * rows == 0 launches nothing; a row has at most 2^24 values.  A row whose loads do not arrive within a
- * second (every device wait of this library is bounded) gets scale NaN, too.  A weight (out_features, width) quantised by rows has the scale
+ * second (every device wait of this library is bounded) gets scale NaN, too, and a sum of NaN.  A weight (out_features, width) quantised by rows has the scale
  * for each output channel that specdec_linear_int8 takes.
  */
 /* codes = int8(x) */
@@ -427,7 +427,8 @@ int specdec_umma_selftest(const void* k, const void* q, const void* v, const voi
 int specdec_wait_selftest(int32_t mode, void* counter, int32_t n_ctas, int32_t grid, int64_t limit_ns,
                           int32_t* status, void* waited_ns, specdec_stream_t stream);
 /* Limit, 0 .. 1e9 ns, of the device waits in the 8-bit kernels that the calling thread launches from here on, so
-   that their give-up paths can be tested; one second unless set.  0: a wait that is not over at once gives up. */
+   that their give-up paths can be tested; one second unless set.  0: linear's waits for what is to be stored give
+   up without looking, and rows that are copied ahead are not copied, so that their waits run out. */
 int specdec_wait_limit_selftest(int64_t limit_ns);
 const char* specdec_last_error(void);
 int specdec_abi_version(void);

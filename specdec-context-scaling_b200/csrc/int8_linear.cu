@@ -534,8 +534,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       ct += step_ct;
       if (ct >= p.ch_tiles) ct -= p.ch_tiles, ++tt;
       if (p.splits == 1 && u + unit_step < p.units) load_scales();
-      if (!(p.wait_ns ? warp_wait(&acc_full[b], (ui >> 1) & 1, p.wait_ns)
-                      : __all_sync(0xffffffffu, mbar_test(&acc_full[b], (ui >> 1) & 1)))) {
+      if (p.wait_ns == 0 || !warp_wait(&acc_full[b], (ui >> 1) & 1, p.wait_ns)) {
         if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
         if (p.splits > 1) {
           lost = 1;

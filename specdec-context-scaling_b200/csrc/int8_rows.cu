@@ -58,6 +58,7 @@ struct RowArgs {
   float* scale;
   int64_t rows;
   int32_t width;
+  int32_t lose;  // of the self-test: no copy is started, every wait for one runs out
 };
 
 // rint(y) for |y| < 2^22 in the low byte of the sum with 1.5 * 2^23 (a product and a sum, each
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(stream_threads(W)) int8_stream_rows_kernel(con
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t full[kGroups][kStreamSlots];
   __shared__ float2 part[2][W];
-  __shared__ int late;  // W > 1: a thread's wait gave up
+  __shared__ uint32_t late;  // W > 1: 1 + `odd` of the row at which a thread's wait gave up (threads may be a row apart)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = W == 1 ? warp : 0, t = W == 1 ? lane : threadIdx.x;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(stream_threads(W)) int8_stream_rows_kernel(con
     if (at >= 0) reinterpret_cast<T*>(slot_ptr(end_input, slot) + row_shift(end_input, row))[at] = v;
   };
 
-  if (t == 0)
+  if (t == 0 && !a.lose)
     for (int s = 0; s < slots - (W > 1); ++s)
       if (row0 + s * step < a.rows) copy_row(row0 + s * step, s);
   const bool ends = !VEC && (W == 1 || warp == 0);
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(stream_threads(W)) int8_stream_rows_kernel(con
     if (W == 1)
       ok = __all_sync(0xffffffffu, ok);
     else if (!ok)
-      late = 1;
+      late = odd + 1;
     const uint32_t shx = row_shift(0, row), shy = kStreams == 2 ? row_shift(1, row) : 0;
     const uint8_t *xs = slot_ptr(0, slot), *ys = slot_ptr(kStreams - 1, slot);
     // 16 bytes from value i on of an input's row
@@ -426,13 +427,19 @@ __global__ void __launch_bounds__(stream_threads(W)) int8_stream_rows_kernel(con
       fence_proxy_async();  // before a later copy into these bytes
     }
     r = row_reduce<kThreads, kIsNorm<OP>>(r, part[odd]);
-    if (W > 1) ok = late == 0;
+    if (W > 1) ok = late != odd + 1;
     if (!ok) {
       // copies that did not land within the wait's limit: what is left is marked, the others are awaited
       // (bounded, too), and the block ends
+      if constexpr (OP == kRowNormAdd) {
+        if (W == 1) __syncwarp();  // this row's sums, of whatever was there, are written
+        for (int64_t left = row; left < a.rows; left += step)
+          for (int i = t; i < a.width; i += kThreads)
+            static_cast<T*>(a.summed)[left * a.s_stride + i] = narrow<T>(__int_as_float(0x7FC00000));
+      }
       if (t == 0) {
         for (int64_t left = row; left < a.rows; left += step) a.scale[left] = __int_as_float(0x7FC00000);
-        for (int i = 0; i < slots; ++i)
+        for (int i = 0; !a.lose && i < slots - (W > 1) && row + i * step < a.rows; ++i)
           (void)mbar_wait(&full[group][(slot + i) % slots], slot + i < slots ? parity : parity ^ 1);
       }
       break;
@@ -697,6 +704,7 @@ extern "C" int specdec_quantize_int8(const void* x, int64_t x_stride, void* code
     return rc;
   if (rows == 0) return SPECDEC_OK;
   RowArgs a = {};
+  a.lose = wait_limit_ns() == 0;
   a.x = x;
   a.x_stride = x_stride;
   a.codes = static_cast<int8_t*>(codes);
@@ -714,6 +722,7 @@ extern "C" int specdec_swiglu_int8(const void* gate_up, int64_t x_stride, void* 
     return rc;
   if (rows == 0) return SPECDEC_OK;
   RowArgs a = {};
+  a.lose = wait_limit_ns() == 0;
   a.x = gate_up;
   a.x_stride = x_stride;
   a.codes = static_cast<int8_t*>(codes);
@@ -737,6 +746,7 @@ extern "C" int specdec_rmsnorm_int8(const void* x, int64_t x_stride, const void*
   if (residual && (residual_stride < hidden || summed_stride < hidden))
     return fail(SPECDEC_ERR_INVALID, "rmsnorm_int8: a row stride is smaller than its row");
   RowArgs a = {};
+  a.lose = wait_limit_ns() == 0;
   a.x = x;
   a.x_stride = x_stride;
   a.residual = residual;

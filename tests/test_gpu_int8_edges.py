@@ -89,8 +89,8 @@ def test_linear_behind_a_long_predecessor(rows, width, n, weight_ready, wait_lim
                                                     (1280, 1536, 17920, torch.float32), (4099, 384, 1153, torch.bfloat16),
                                                     (64, 8960, 1536, torch.bfloat16), (40, 4864, 897, torch.float32)])
 def test_linear_marks_what_its_waits_gave_up_on(rows, width, n, out_dtype, wait_limit):
-    """Waits that give up at once: the status bit is raised, no output keeps what the buffer held before (each is
-    NaN, or the product), nothing beside the output is written, and the next call is right."""
+    """Waits that give up without looking: the status bit is raised, no output keeps what the buffer held before,
+    nothing beside the output is written, and the next call is right."""
     from specdec_b200 import _lib
 
     ops = _ops()
@@ -103,11 +103,45 @@ def test_linear_marks_what_its_waits_gave_up_on(rows, width, n, out_dtype, wait_
     wait_limit(0)
     out = ops.linear_int8(a, sa, w, sw, out=buf[1:-1], status=status)
     torch.cuda.synchronize()
-    lost = torch.isnan(out)
-    assert int(status.item()) == _lib.STATUS_TIMEOUT and lost.any()
-    assert torch.equal(out[~lost], want[~lost])
+    assert int(status.item()) == _lib.STATUS_TIMEOUT and torch.isnan(out).all()
     assert (buf[0] == 7).all() and (buf[-1] == 7).all()
     wait_limit(1_000_000_000)
     status.zero_()
     assert torch.equal(ops.linear_int8(a, sa, w, sw, out_dtype=out_dtype, status=status), want)
     assert int(status.item()) == 0
+
+
+# the ring with a warp, 4, 8 and 16 warps a row; unaligned and aligned rows (a second each: the limit of a wait)
+@pytest.mark.parametrize("rows,width,dtype", [(1300, 501, torch.bfloat16), (1200, 2501, torch.float32),
+                                              (1200, 6001, torch.bfloat16), (1200, 12000, torch.bfloat16)])
+@pytest.mark.parametrize("op", ["swiglu", "rmsnorm_add", "rmsnorm_add_in_place"])
+def test_rows_mark_what_their_waits_gave_up_on(rows, width, dtype, op, wait_limit):
+    """Rows whose copies never come: every row has scale NaN and (with a residual) a sum of NaN, nothing
+    beside the outputs is written, and the next call is right."""
+    ops = _ops()
+    x = _hidden(rows, width * 2 if op == "swiglu" else width, dtype, 1)
+    r = _hidden(rows, width, dtype, 2) if "add" in op else None
+    w = torch.ones(width, dtype=dtype, device="cuda")
+    stride = -(-width // 16) * 16
+
+    def call(x, summed=None):
+        codes = torch.full((rows, stride), 7, dtype=torch.int8, device="cuda")
+        if op == "swiglu":
+            return codes, ops.swiglu_int8(x, codes=codes[:, :width])[1], None
+        return codes, *ops.rmsnorm_int8(x, w, residual=r, summed=summed, codes=codes[:, :width])[1:]
+
+    want = call(x)
+    buf = torch.full((rows, stride), 7.0, dtype=dtype, device="cuda")
+    summed = None if r is None else buf[:, :width]
+    y = x
+    if "place" in op:  # a padded row stride, so that the outputs are aligned
+        y = summed.copy_(x)
+    torch.cuda.synchronize()
+    wait_limit(0)
+    codes, scale, s = call(y, summed)
+    torch.cuda.synchronize()
+    assert torch.isnan(scale).all() and (codes[:, width:] == 7).all() and (buf[:, width:] == 7).all()
+    assert r is None or torch.isnan(s).all()
+    wait_limit(1_000_000_000)
+    for got, ref in zip(call(x), want):
+        assert got is None or torch.equal(got, ref)
