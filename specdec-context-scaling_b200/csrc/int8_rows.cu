@@ -509,12 +509,12 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowArgs a) {
 
 // code * scale: a warp per row and 1024 columns.  VEC: 16 codes a lane and load.  Else the outputs'
 // alignment leads: a lane stores the 16 aligned bytes of outputs from value i on, its codes shifted out
-// of the words around them, and the values before the first and after the last such piece (at most 26)
-// are one lane's each.
+// of the words around them, and the values before the first and after the last such piece (at most 11 each)
+// are one lane's each.  (No __restrict__: codes and scales are written by the preceding kernel, which may
+// still run when this one starts, so their loads must not count as independent of grid_dep_wait.)
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t* __restrict__ codes, int64_t c_stride,
-                                                              const float* __restrict__ scale, T* __restrict__ out,
-                                                              int64_t o_stride, int64_t rows, int width) {
+__global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t* codes, int64_t c_stride, const float* scale,
+                                                              T* out, int64_t o_stride, int64_t rows, int width) {
   constexpr int kOut = 16 / static_cast<int>(sizeof(T));
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
