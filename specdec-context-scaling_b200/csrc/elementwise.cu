@@ -72,11 +72,10 @@ __global__ void __launch_bounds__(256) rmsnorm_kernel(const T* __restrict__ x, c
 
 // bf16 rows of hidden % 8 == 0 (<= 4096): one warp per row, 16-byte vectors kept in
 // registers between the sum of squares (fp32) and the scaling; no block-level sync.
+// (No __restrict__ here and in swiglu_packed_kernel: the input may still be being written when the kernel starts.)
 template <int CH>
-__global__ void __launch_bounds__(256) rmsnorm_warp_kernel(const __nv_bfloat16* __restrict__ x,
-                                                           const __nv_bfloat16* __restrict__ w,
-                                                           __nv_bfloat16* __restrict__ y, int64_t rows, int hidden,
-                                                           float eps) {
+__global__ void __launch_bounds__(256) rmsnorm_warp_kernel(const __nv_bfloat16* x, const __nv_bfloat16* w,
+                                                           __nv_bfloat16* y, int64_t rows, int hidden, float eps) {
   grid_dep_wait();  // launched programmatically: x is the preceding work's output
   grid_dep_launch();
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -159,8 +158,7 @@ __global__ void __launch_bounds__(256) swiglu_kernel(const T* __restrict__ g, co
 
 // SwiGLU of a fused gate|up projection: row r of `gu` holds gate (inter values) then
 // up (inter values); 8 values per thread with 16-byte vectors (inter % 8 == 0).
-__global__ void __launch_bounds__(256) swiglu_packed_kernel(const __nv_bfloat16* __restrict__ gu,
-                                                            __nv_bfloat16* __restrict__ y, int64_t rows,
+__global__ void __launch_bounds__(256) swiglu_packed_kernel(const __nv_bfloat16* gu, __nv_bfloat16* y, int64_t rows,
                                                             int64_t inter) {
   grid_dep_wait();  // launched programmatically: gu is the preceding work's output
   grid_dep_launch();

@@ -36,7 +36,7 @@ def test_kernels_are_found():
             "linear_int8_few_kernel"} <= found
 
 
-@pytest.mark.parametrize("path", [p for p in SOURCES if p.name.startswith("int8")], ids=lambda p: p.name)
+@pytest.mark.parametrize("path", SOURCES, ids=lambda p: p.name)
 def test_early_starters_do_not_promise_unaliased_inputs(path):
     """A kernel that may start while its predecessor runs reads what that one writes: __restrict__ would let the
     compiler load it before, or without regard to, the wait for the predecessor."""
