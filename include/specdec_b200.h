@@ -389,8 +389,8 @@ int specdec_dequantize_int8(const void* codes, int64_t codes_stride, const float
  * out[r][n] = (sum_k a[r][k] w[n][k]) * a_scale[r] * w_scale[n] + bias[n]
  * a (rows, width), w (out_features, width) int8 codes, 16-byte aligned, row strides multiples of 16 bytes
  * (what lies between a row's end and its stride is never used); scales and the optional bias f32; out f32 or
- * bf16 (`out_dtype`), rows `out_stride` elements apart.  The sum is exact (width <= 131072), the rest fp32
- * with one rounding to the output type.  rows <= 2^21.
+ * bf16 (`out_dtype`), rows `out_stride` elements apart.  The sum is exact (width <= 131072; codes -128 .. 127),
+ * the rest fp32 with one rounding to the output type.  rows <= 2^21.
  * weight_ready 1: the caller promises that the work right before the call on the stream does not write w, so
  * the kernel may load it while that work finishes.  status (optional): SPECDEC_STATUS_TIMEOUT, when a device
  * wait gave up after its second; the outputs it stood for are NaN.

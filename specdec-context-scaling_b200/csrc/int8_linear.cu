@@ -1,7 +1,9 @@
 // int8_linear.cu -- linear layer over 8-bit activations and weights:
 //   y[r][n] = (sum_k a[r][k] w[n][k]) * a_scale[r] * w_scale[n] + bias[n]
-// The integer sum is exact: |sum| <= K 127^2 < 2^31 for K <= 131072, in any order.  Scales and
-// bias are applied in fp32 and the result is rounded once to the output type.
+// The integer sum is exact in any order: it lies in -2^31 < sum <= 2^31 for K <= 131072, whatever the codes.
+// +2^31 itself (every product 128^2 at the largest K) converts to fp32 as 2^31 - 1 does: the tensor cores are
+// told to saturate there, and where warps or CTAs add up it wraps to -2^31, which no other sum is (unwrapped).
+// Scales and bias are applied in fp32 and the result is rounded once to the output type.
 //
 // Two kernels (few_rows):
 //
@@ -65,8 +67,8 @@ struct LinParams {
 
 // ---------------------------------------------------------------- PTX of this kernel
 // instruction descriptor of kind::i8: signed x signed -> s32, both operands K-major
-SD_DEV uint32_t idesc_i8(int M, int N) {
-  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
+SD_DEV uint32_t idesc_i8(int M, int N, bool saturate) {
+  return (saturate ? 1u << 3 : 0u) | (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
          (static_cast<uint32_t>(M >> 4) << 24);
 }
 // One lane of a converged warp.  The loops around it stay warp-uniform, so descriptors, barriers and
@@ -204,6 +206,9 @@ template <typename T>
 SD_DEV void store_lost(T* o, int64_t stride, int c0, int c1) {
   for (int c = c0; c < c1; ++c) store_out(o + c * stride, __int_as_float(0x7FC00000));
 }
+// A sum whose conversion to fp32 is that of the sum without wrapping: +2^31, wrapped to -2^31, becomes 2^31 - 1,
+// which converts to 2^31.
+SD_DEV int32_t unwrapped(int32_t sum) { return sum == INT32_MIN ? INT32_MAX : sum; }
 SD_DEV float scaled(int32_t acc, float sa, float sw, float b) {
   return __fmaf_rn(__fmul_rn(static_cast<float>(acc), sa), sw, b);
 }
@@ -292,17 +297,17 @@ SD_DEV void add_partials(const LinParams& p, const int32_t* got, int rank, int u
     const int c = rank + p.splits * i;
     if (c >= ntok) break;
     const float sa = lost ? __int_as_float(0x7FC00000) : p.a_scale[tok0 + c];
-    int4 sum = make_int4(0, 0, 0, 0);
+    uint4 sum = make_uint4(0, 0, 0, 0);
 #pragma unroll 8
     for (int r = 0; r < p.splits; ++r) {
-      const int4 v = *reinterpret_cast<const int4*>(got + (r * share + i) * kLinCh + lane * 4);
+      const uint4 v = *reinterpret_cast<const uint4*>(got + (r * share + i) * kLinCh + lane * 4);
       sum.x += v.x;
       sum.y += v.y;
       sum.z += v.z;
       sum.w += v.w;
     }
-    const float y[4] = {scaled(sum.x, sa, sw[0], bias[0]), scaled(sum.y, sa, sw[1], bias[1]),
-                        scaled(sum.z, sa, sw[2], bias[2]), scaled(sum.w, sa, sw[3], bias[3])};
+    const float y[4] = {scaled(unwrapped(sum.x), sa, sw[0], bias[0]), scaled(unwrapped(sum.y), sa, sw[1], bias[1]),
+                        scaled(unwrapped(sum.z), sa, sw[2], bias[2]), scaled(unwrapped(sum.w), sa, sw[3], bias[3])};
     T* o = static_cast<T*>(p.out) + (tok0 + c) * p.out_stride + n;
     if (p.vec_out && n + 4 <= p.n) {
       if constexpr (sizeof(T) == 4)
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     // ---- MMA issuer
     if (rank % CG == 0) {
       grid_dep_wait();  // a is loaded after the preceding kernel is over: the limit of the first wait starts here, too
-      const uint32_t idesc = idesc_i8(kLinCh * CG, p.tokens);
+      const uint32_t idesc = idesc_i8(kLinCh * CG, p.tokens, p.chunks == kMaxWidth / kLinChunk);
       const uint32_t ring = smem_u32(smem);
       int s = 0, ui = 0;
       uint32_t parity = 0;
@@ -717,11 +722,11 @@ SD_DEV void few_finish(const FewParams& p, const int32_t (&d)[NB][4], int32_t (*
   float sa = mine ? p.a_scale[row0] : 0.f;
   __syncthreads();
   for (int row = row0; row < NB * 8 && row < p.rows && n < p.n; row += 2 * WARPS) {
-    int32_t sum = 0;
+    uint32_t sum = 0;
 #pragma unroll
-    for (int j = 0; j < WARPS; ++j) sum += part[j][row][threadIdx.x % kFewCh];
+    for (int j = 0; j < WARPS; ++j) sum += static_cast<uint32_t>(part[j][row][threadIdx.x % kFewCh]);
     if (row != row0) sa = p.a_scale[row];
-    store_out(static_cast<T*>(p.out) + row * p.out_stride + n, scaled(sum, sa, sw, bias));
+    store_out(static_cast<T*>(p.out) + row * p.out_stride + n, scaled(unwrapped(sum), sa, sw, bias));
   }
 }
 

@@ -740,8 +740,9 @@ def linear_int8(codes, scale, weight_codes, weight_scale, *, bias=None, out=None
 
     ``codes`` (rows, width) and ``weight_codes`` (out_features, width) are int8 with 16-byte aligned rows
     (as ``quantize_int8`` lays them out), ``scale``, ``weight_scale`` and ``bias`` f32, ``out`` f32 or bf16.
-    The integer sum is exact; the rest is fp32, rounded once.  ``weight_ready``: the caller promises that the
-    work right before this call on the stream does not write ``weight_codes``, so they may be loaded early.
+    The integer sum is exact for any codes (width <= 131072); the rest is fp32, rounded once.
+    ``weight_ready``: the caller promises that the work right before this call on the stream does not write
+    ``weight_codes``, so they may be loaded early.
     ``status``: a device int32 that receives the library's status bits (a wait that timed out; the outputs it
     stood for are NaN)."""
     lib, dev, stream = _int8_call(codes)

@@ -145,3 +145,20 @@ def test_rows_mark_what_their_waits_gave_up_on(rows, width, dtype, op, wait_limi
     wait_limit(1_000_000_000)
     for got, ref in zip(call(x), want):
         assert got is None or torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("rows", [1, 12, 24, 40, 300, 3000])
+@pytest.mark.parametrize("width", [131071, 131072])
+def test_linear_sums_of_the_lowest_code(rows, width):
+    """Codes of -128 on both sides: at the largest width the sum is 2^31, one past the largest int32."""
+    a = torch.full((rows, 131072), -128, dtype=torch.int8, device="cuda")[:, :width]
+    w = torch.full((130, 131072), -128, dtype=torch.int8, device="cuda")[:, :width]
+    w[1] = 127
+    w[2] = 0
+    one = torch.ones(rows, device="cuda")
+    for out_dtype in (torch.float32, torch.bfloat16):
+        got = _ops().linear_int8(a, one, w, torch.ones(130, device="cuda"), out_dtype=out_dtype)
+        want = torch.full((rows, 130), float(width * 128 * 128))
+        want[:, 1] = -float(width * 128 * 127)
+        want[:, 2] = 0
+        assert torch.equal(got.cpu(), want.to(out_dtype))  # width * 2^14 and width * 2^7 * 127: exact in fp32
