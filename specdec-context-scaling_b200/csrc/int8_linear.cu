@@ -30,6 +30,8 @@
 // chunks of K and pushing its integer partial sums into the shared memory of the CTA that adds them up.
 #include <cudaTypedefs.h>
 
+#include <atomic>
+
 #include "sd_common.cuh"
 #include "sd_internal.h"
 #include "umma.cuh"
@@ -805,8 +807,11 @@ __global__ void __launch_bounds__(32 * WARPS) linear_int8_few_long_kernel(const 
 }
 
 // ---------------------------------------------------------------- host
+// What a function keeps between calls (an entry point's address, an attribute that was set, an occupancy) is the
+// same whichever thread finds it out; atomics, because several may at once.
 static int encode_codes(CUtensorMap* map, const void* base, int64_t width, int64_t rows, int64_t stride, int box_rows) {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> known{nullptr};
+  PFN_cuTensorMapEncodeTiled_v12000 fn = known.load(std::memory_order_relaxed);
   if (fn == nullptr) {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult qres;
@@ -814,6 +819,7 @@ static int encode_codes(CUtensorMap* map, const void* base, int64_t width, int64
         qres != cudaDriverEntryPointSuccess)
       return fail(SPECDEC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
     fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    known.store(fn, std::memory_order_relaxed);
   }
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
@@ -869,8 +875,8 @@ static LinShape pick_shape(int rows, int n, int chunks, int sms, int dev) {
 }
 
 static int resident_clusters(int size, int dev, int sms) {
-  static int known[64][9] = {};
-  int& n = known[dev][size];
+  static std::atomic<int> known[64][9];  // zeros: not asked yet
+  int n = known[dev][size].load(std::memory_order_relaxed);
   if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(size * sms));
@@ -886,18 +892,19 @@ static int resident_clusters(int size, int dev, int sms) {
     const cudaError_t e = cudaOccupancyMaxActiveClusters(&got, linear_int8_kernel<1, __nv_bfloat16>, &cfg);
     if (e != cudaSuccess) (void)cudaGetLastError();
     n = e == cudaSuccess && got > 0 ? got : sms / (2 * size);
+    known[dev][size].store(n, std::memory_order_relaxed);
   }
   return n;
 }
 
 template <int CG, typename T>
 static int allow_ring(int dev) {
-  static bool set[64] = {};
-  if (!set[dev]) {
+  static std::atomic<bool> set[64];
+  if (!set[dev].load(std::memory_order_acquire)) {
     const cudaError_t e = cudaFuncSetAttribute(linear_int8_kernel<CG, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                kLinRing + 1024);
     if (e != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "linear_int8: %s", cudaGetErrorString(e));
-    set[dev] = true;
+    set[dev].store(true, std::memory_order_release);
   }
   return SPECDEC_OK;
 }

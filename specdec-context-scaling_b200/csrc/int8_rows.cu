@@ -11,6 +11,8 @@
 // kept in fp32, and the sum x + residual is rounded once, when it is stored.
 #include <math.h>
 
+#include <atomic>
+
 #include "sd_common.cuh"
 #include "sd_internal.h"
 
@@ -595,13 +597,13 @@ static int launch_stream_as(const char* what, const RowArgs& a, int slots, int r
   constexpr int kGroups = W == 1 ? 8 : 1;
   const int smem = kGroups * slots * row_bytes * (kTwoInputs<OP> ? 2 : 1);
   auto* kern = int8_stream_rows_kernel<T, OP, W, VEC>;
-  static bool attr_set[64] = {};
+  static std::atomic<bool> attr_set[64];  // threads may be here at once
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-  if (!attr_set[dev]) {
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamSmem);
     if (e != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    attr_set[dev] = true;
+    attr_set[dev].store(true, std::memory_order_release);
   }
   // blocks that fit an SM's shared memory, and 1024 threads
   int per_sm = 220 * 1024 / (smem + 2048);

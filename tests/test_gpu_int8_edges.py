@@ -162,3 +162,41 @@ def test_linear_sums_of_the_lowest_code(rows, width):
         want[:, 1] = -float(width * 128 * 127)
         want[:, 2] = 0
         assert torch.equal(got.cpu(), want.to(out_dtype))  # width * 2^14 and width * 2^7 * 127: exact in fp32
+
+
+def test_first_calls_from_several_threads():
+    """Eight threads of a fresh process make their first calls of the path together, each on a stream of its own."""
+    import subprocess
+    import sys
+
+    from conftest import PKG, ROOT
+
+    code = f"""
+import sys, threading
+sys.path[:0] = [{str(PKG)!r}, {str(ROOT / 'tests')!r}, {str(ROOT)!r}]
+import torch
+from specdec_b200.kernels import ops
+from test_gpu_int8 import _check_linear, _codes, _hidden, _scales
+shapes = [(64, 8960, 300), (40, 4864, 897), (1280, 1536, 600), (333, 1001, 777)]
+data = [(_codes(r, k, 1), _scales(r, 1), _codes(n, k, 2), _scales(n, 2), _hidden(1300, k | 1, torch.bfloat16, 3))
+        for r, k, n in shapes]
+torch.cuda.synchronize()
+start, got = threading.Barrier(8), [None] * 8
+def call(i):
+    a, sa, w, sw, x = data[i % 4]
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        y = ops.linear_int8(a, sa, w, sw)
+        got[i] = y, ops.quantize_int8(x)
+        torch.cuda.current_stream().synchronize()
+threads = [threading.Thread(target=call, args=(i,)) for i in range(8)]
+[t.start() for t in threads]; [t.join() for t in threads]
+for i, (y, (codes, scale)) in enumerate(got):
+    a, sa, w, sw, x = data[i % 4]
+    _check_linear(a, sa, w, sw, None, y)
+    want = ops.quantize_int8(x)
+    assert torch.equal(codes, want[0]) and torch.equal(scale, want[1])
+print("all right")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "all right" in r.stdout, r.stderr[-2000:]

@@ -42,3 +42,12 @@ def test_early_starters_do_not_promise_unaliased_inputs(path):
     compiler load it before, or without regard to, the wait for the predecessor."""
     bad = [name for name, params, body in _kernels(_code(path)) if "grid_dep_wait" in body and "__restrict__" in params]
     assert not bad, bad
+
+
+@pytest.mark.parametrize("path", [p for p in SOURCES if p.name.startswith("int8")], ids=lambda p: p.name)
+def test_state_between_calls_is_shared_safely(path):
+    """Calls from several threads run at once (ctypes releases the interpreter's lock): what a function keeps
+    between calls is atomic or constant."""
+    kept = re.findall(r"^ +static (?!const(?:expr)?\b|_)([^;(]*?)[;={[]", _code(path), flags=re.M)
+    bad = [k for k in kept if not k.startswith("std::atomic<")]
+    assert kept and not bad, bad
