@@ -997,6 +997,10 @@ extern "C" int specdec_linear_int8(const void* a, int64_t a_stride, const float*
     return fail(SPECDEC_ERR_INVALID, "linear_int8: the row strides of the codes must be multiples of 16");
   if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w)) & 15u)
     return fail(SPECDEC_ERR_INVALID, "linear_int8: the codes must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale) | reinterpret_cast<uintptr_t>(bias) |
+       reinterpret_cast<uintptr_t>(status)) % 4 ||
+      reinterpret_cast<uintptr_t>(out) % (out_dtype == SPECDEC_F32 ? 4 : 2))
+    return fail(SPECDEC_ERR_INVALID, "linear_int8: a tensor is not aligned to its elements");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (few_rows(rows, width, out_features)) {
     const FewParams f = {static_cast<const int8_t*>(a), static_cast<const int8_t*>(w), a_scale, w_scale, bias, out,

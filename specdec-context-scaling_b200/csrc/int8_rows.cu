@@ -582,6 +582,8 @@ static int check_rows(const char* what, const void* x, int64_t x_stride, int64_t
   if (!x || !codes || !scale) return fail(SPECDEC_ERR_INVALID, "%s: tensors must be CUDA", what);
   if (x_stride < need || c_stride < width)
     return fail(SPECDEC_ERR_INVALID, "%s: a row stride is smaller than its row", what);
+  if (reinterpret_cast<uintptr_t>(x) % (dtype == SPECDEC_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(scale) % 4)
+    return fail(SPECDEC_ERR_INVALID, "%s: a tensor is not aligned to its elements", what);
   return SPECDEC_OK;
 }
 
@@ -747,6 +749,9 @@ extern "C" int specdec_rmsnorm_int8(const void* x, int64_t x_stride, const void*
     return fail(SPECDEC_ERR_INVALID, "rmsnorm_int8: residual and summed come together");
   if (residual && (residual_stride < hidden || summed_stride < hidden))
     return fail(SPECDEC_ERR_INVALID, "rmsnorm_int8: a row stride is smaller than its row");
+  if ((reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(residual) |
+       reinterpret_cast<uintptr_t>(summed)) % (dtype == SPECDEC_F32 ? 4 : 2))
+    return fail(SPECDEC_ERR_INVALID, "rmsnorm_int8: a tensor is not aligned to its elements");
   RowArgs a = {};
   a.lose = wait_limit_ns() == 0;
   a.x = x;

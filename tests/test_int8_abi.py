@@ -107,3 +107,19 @@ def test_wait_limit_refuses_what_is_out_of_range(lib):
     for ns in (-1, 1_000_000_001):
         assert lib.specdec_wait_limit_selftest(ns) == 1 and "wait limit must be" in _msg(lib)
     assert lib.specdec_wait_limit_selftest(1_000_000_000) == 0
+
+
+@pytest.mark.parametrize("call", [
+    lambda lib: _quantize(lib, x=P + 1), lambda lib: _quantize(lib, x=P + 2, dtype=0), lambda lib: _quantize(lib, s=P + 2),
+    lambda lib: lib.specdec_swiglu_int8(P + 1, 128, P, 64, P, 1, 4, 64, None),
+    lambda lib: lib.specdec_dequantize_int8(P, 64, P, P + 2, 64, 0, 4, 64, None),
+    lambda lib: lib.specdec_rmsnorm_int8(P, 64, P, 64, P + 1, 1e-6, P, 64, P, 64, P, 1, 4, 64, None),
+    lambda lib: lib.specdec_rmsnorm_int8(P, 64, P + 2, 64, P, 1e-6, P, 64, P, 64, P, 0, 4, 64, None),
+    lambda lib: lib.specdec_rmsnorm_int8(P, 64, P, 64, P, 1e-6, P + 1, 64, P, 64, P, 1, 4, 64, None),
+    lambda lib: _linear(lib, sa=P + 2), lambda lib: _linear(lib, sw=P + 1), lambda lib: _linear(lib, out=P + 1),
+    lambda lib: _linear(lib, out=P + 2, dtype=0),
+    lambda lib: lib.specdec_linear_int8(P, 64, P, P, 64, P, P + 2, P, 32, 1, 4, 64, 32, 0, None, None),
+])
+def test_elements_have_to_be_aligned(lib, call):
+    """An address between two elements would fault on the device."""
+    assert call(lib) == 1 and "not aligned to its elements" in _msg(lib)
