@@ -758,6 +758,10 @@ def linear_int8(codes, scale, weight_codes, weight_scale, *, bias=None, out=None
         b_ptr = bias.data_ptr()
     if weight_codes.get_device() != dev:
         raise RuntimeError("tensors must be CUDA, all on one device")
+    if status is not None:
+        _on_device(dev, status)
+        if status.dtype is not torch.int32 or status.numel() < 1:
+            raise ValueError("status must be int32")
     if out is None:
         out, code, os = _new_out(scale, rows, n, out_dtype)
     else:

@@ -200,3 +200,14 @@ print("all right")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "all right" in r.stdout, r.stderr[-2000:]
+
+
+def test_linear_refuses_a_status_the_device_cannot_write():
+    ops = _ops()
+    a, w = _codes(4, 64, 1), _codes(32, 64, 2)
+    sa, sw = _scales(4, 1), _scales(32, 2)
+    with pytest.raises(RuntimeError, match="must be CUDA"):
+        ops.linear_int8(a, sa, w, sw, status=torch.zeros(1, dtype=torch.int32))
+    for status in (torch.zeros(1, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError, match="status must be int32"):
+            ops.linear_int8(a, sa, w, sw, status=status)
