@@ -88,7 +88,8 @@ SD_DEV float amax_values(float m, const float (&v)[N]) {
 }
 
 // silu(g) * u with the hardware exponential and reciprocal: for |g| < 16 within 2^-19 of the exact
-// value, far under what decides a code; -0 where exp(-g) overflows
+// value, far under what decides a code; the exponent's rounding is |g| 2^-24 of it further out, 2^-17 at
+// g = -87, and -0 below, where exp(-g) passes 2^126 (the exact value is under 2^-119 |u|)
 SD_DEV float silu_mul(float g, float u) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(g * -1.4426950408889634f)));
@@ -478,7 +479,8 @@ __global__ void __launch_bounds__(stream_threads(W)) int8_stream_rows_kernel(con
   }
 }
 
-// Rows too long for a ring in shared memory: read again in each pass.
+// Rows too long for a ring in shared memory (a block's registers hold 20480 bf16 values, the ring three rows of 18944
+// and a second input; f32 half as many): read again in each pass, a value a lane and load.  8192 x 28672 bf16: quantise 203 us (108 of bytes), norm 290, with residual 551 (251), swiglu 390 (180).
 template <typename T, int OP>
 __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowArgs a) {
   __shared__ float2 part[32];
@@ -642,9 +644,14 @@ static int launch_stream(const char* what, const RowArgs& a, bool vec, cudaStrea
 // swiglu's 8960, 13.5 for 600; 256 threads: 2.5 and 7.3; 32768 rows of swiglu's 1536: 49 us with a warp a
 // row, 39 with two); short rows in small number are spread as wide as they go, a piece a thread (`few`:
 // under eight rows an SM).  Longer ones, swiglu's long ones in large
-// number (its arithmetic hides behind the ring's copies: 8192 x 8960 62 us, 95 in registers) and unaligned
+// number (its arithmetic hides behind the ring's copies: 8192 x 8960 62 us, 90 in registers) and unaligned
 // ones in large number through shared memory; unaligned rows in small number by single values, a block a
-// row, and so are rows whose outputs are not aligned, and unaligned f32 rows of 897 to 1024 values, which a
+// row, and so are rows whose outputs are not aligned.
+// The thresholds are in pieces of 16 bytes and decide f32, too (registers and ring, us: quantise 8192 x 2048
+// 13.6 and 21.6, norm with residual 8192 x 4096 65.0 and 71.5, swiglu 8192 x 4096 45.6 and 46.1, which is the
+// ring's), but for two: one f32 input in large number keeps a warp a row up to 320 pieces (a warp and four, us:
+// 32768 x 1280 quantise 31.1 and 34.8, norm 35.1 and 37.9; x 1408 34.2 and 35.2, 44.0 and 39.3; x 1536 37.0 and
+// 36.5, 44.2 and 40.7); and single values take unaligned f32 rows of 897 to 1024 values, which a
 // block of 256 threads still holds while the ring needs four warps each (norm without a residual, 1001 values:
 // 600 rows 3.4 us either way, 2000 5.5 and 7.1 in the ring, 8000 17.2 and 19.6).  Unaligned norms without a
 // residual by single values and in the ring, us: 600 x 501 bf16 3.1 and 2.9, 1000 x 1501 bf16 11.8 and 4.5,
@@ -668,7 +675,7 @@ static int launch_rows_t(const char* what, const RowArgs& a, cudaStream_t st) {
     if (need <= 256 && a.rows <= 2 * sms) return launch_rows_as<T, OP, 256, V, 1>(what, a, st);
     if (need <= 192) return few || two ? launch_rows_as<T, OP, 64, V, 3>(what, a, st) : launch_rows_as<T, OP, 32, V, 6>(what, a, st);
     if (need <= 256) return few || two ? launch_rows_as<T, OP, 128, V, 2>(what, a, st) : launch_rows_as<T, OP, 32, V, 8>(what, a, st);
-    if (need <= 384 && V == 4 && !few && !two) return launch_rows_as<T, OP, 32, V, 48 / V>(what, a, st);
+    if (need <= 320 && V == 4 && !few && !two) return launch_rows_as<T, OP, 32, V, 48 / V>(what, a, st);
     if (need <= 384) return launch_rows_as<T, OP, 128, V, 3>(what, a, st);
     if (need <= 640) return launch_rows_as<T, OP, 128, V, 5>(what, a, st);
     if (need <= 768) return launch_rows_as<T, OP, 256, V, 3>(what, a, st);
