@@ -25,7 +25,8 @@
 // pays 128 + tokens; the pair's first CTA issues the products.  L2 delivers about 64 bytes a clock
 // and SM, which a 256 x 256 pair needs exactly at the products' full rate: 8192^3 runs at 3.2-3.3
 // POP/s, twice the bf16 rate of the library's product (3.29).  With K = 1536 and 17920 channels the
-// output (1.2 GB for 32768 rows) shares L2 with those loads: 617-700 us, 2.6-2.9 POP/s.
+// output (1.2 GB for 32768 rows) shares L2 with those loads: 600-735 us, 2.5-3.0 POP/s, by the clock that the
+// power cap leaves.
 // splits > 1 (CG = 1): a cluster of `splits` CTAs shares one tile, each taking a share of the
 // chunks of K and pushing its integer partial sums into the shared memory of the CTA that adds them up.
 #include <cudaTypedefs.h>
@@ -253,7 +254,7 @@ SD_DEV uint32_t scaled_pair(int32_t a0, int32_t a1, uint64_t sa, uint64_t sw, ui
 // by way of 1 KB of shared memory: eight tokens a store instead of half of one.  `put`: this lane's
 // address for stmatrix, `get`: for reading back; o: this lane's 16 bytes of tokens lane / 4 and, `half`
 // further, lane / 4 + 8.  At short K the epilogue bounds the kernel: with one 2-byte store a token and
-// a tile's scales loaded at its start, 8192 x 896 x 9728 took 72 us; so, 62.
+// a tile's scales loaded at its start, 8192 x 896 x 9728 took 72 us; so, 60 to 65.
 template <bool GUARD>
 SD_DEV void store_fragments(const int32_t (&v)[16], const float* s_scale, const uint64_t (&sw)[4],
                             const uint64_t (&bias)[4], uint32_t put, const uint8_t* get, uint8_t* o, int64_t half,

@@ -23,6 +23,10 @@ each output channel and each token), in a decode / verify step and in the prompt
   qkv, o, gate|up and down projections             specdec_linear_int8
   int8(o), int8(silu(gate) up)                     specdec_quantize_int8, specdec_swiglu_int8
 Attention, the cache, the embedding and the LM head are the same as with bf16 weights.
+The o and down projections' results are rounded to bf16 (2^-9 of the value) before the next
+norm adds them to the residual stream, which rounds again: two roundings where the bf16 path's
+addmm has one.  Written as f32 they would double the projection's output and the norm's
+second input, and the codes' own steps (up to 1/254 of a row's maximum) are larger.
 
 Weights come from a state dict with the reference's parameter names
 (``embed_tokens.weight``, ``layers.{i}.self_attn.q_proj.weight`` ...), so a
