@@ -84,7 +84,7 @@ def listed():
         _pages("fork_4", "fork", 2, 2, 128, 64, tokens=300, forks=4),
         # an 8191-token prompt forked to 64 sequences, all target layers
         _pages("fork_64", "fork", 28, 2, 128, 768, tokens=8191, forks=64),
-        # every eighth of the pages moved between sequences, all draft layers
+        # 512 of 1500 pages copied to others, all draft layers
         _pages("copy_512", "copy", 24, 2, 64, 1500, moved=512),
         # a target pool of 1800 pages, half of them free here and there, made dense
         _pages("compact_1800", "compact", 28, 2, 128, 1800, moved=900),
