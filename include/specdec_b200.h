@@ -66,6 +66,7 @@ typedef enum SpecdecResult {
 #define SPECDEC_STATUS_TIMEOUT 0x10      /* a bounded device wait gave up             */
 #define SPECDEC_STATUS_ACCEPT_RANGE 0x20 /* accept: kp outside [1, max_cands]         */
 #define SPECDEC_STATUS_PLAN_MISMATCH 0x40 /* reused plan built for another launch shape */
+#define SPECDEC_STATUS_BAD_GROUP 0x80     /* prefix group: member out of range or listed twice, bad start or length */
 
 typedef enum SpecdecDtype { SPECDEC_F32 = 0, SPECDEC_BF16 = 1, SPECDEC_E4M3 = 2 } SpecdecDtype;
 
@@ -337,6 +338,83 @@ int specdec_attention(const void* q, const void* k, const void* v, void* out, in
 int specdec_attention_fp8v(const void* q, const void* k, const void* v_codes, const float* v_scale, void* out,
                            int32_t B, int32_t H, int32_t KV, int32_t S, int32_t T, int32_t D, void* workspace,
                            size_t workspace_bytes, specdec_stream_t stream);
+
+/*
+ * Causal attention of packed prompts of different lengths, grouped heads, bf16, head_dim 64 or 128, up to 128
+ * query heads a KV head.  Row i of sequence b (query row q_row0[b] + i) sees keys j <= i + (ctx_len[b] - q_len[b]),
+ * key j of sequence b being row kv_row0[b] + j of k and v: a whole prompt has ctx_len == q_len, the next piece
+ * of a long one more keys than rows.  q_len[b] == 0 skips the sequence.  No value of another sequence, of a
+ * later token or behind the last row reaches an output, whatever it holds.  A sequence whose lengths or rows are
+ * out of range (ctx_len < q_len, q_len > max_q_len, rows past q_rows / kv_rows) raises SPECDEC_STATUS_BAD_LENGTH and
+ * writes nothing; rows that belong to no sequence are left as they were.  Replaces the attention of the
+ * reference's prompt pass (specdec/engine/model_self.py:715-775).
+ * q, k, v, out 16-byte aligned, strides multiples of 8 elements; sm_scale positive.
+ * reuse_plan 1: the workspace holds the plan of an earlier call with the same batch (lengths, rows, heads,
+ * num_sms): the layers of one prompt pass.  Calls that share a workspace must not overlap.
+ */
+typedef struct SpecdecPromptArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_stride_tok, q_stride_head;
+  int64_t k_stride_tok, k_stride_head;
+  int64_t v_stride_tok, v_stride_head;
+  int64_t o_stride_tok, o_stride_head;
+  SpecdecBatch batch; /* max_ctx_len is not used */
+  const int32_t* kv_row0; /* [num_seqs] */
+  int64_t q_rows;  /* rows of q and out */
+  int64_t kv_rows; /* rows of k and v */
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  float sm_scale;
+  void* workspace; /* >= specdec_prompt_workspace_bytes(...) bytes, 256-byte aligned, any contents */
+  size_t workspace_bytes;
+  int32_t* status; /* device int32, may be NULL */
+  int32_t reuse_plan;
+  int32_t num_sms; /* SMs the call may use; 0: all */
+} SpecdecPromptArgs;
+
+size_t specdec_prompt_workspace_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                      int32_t max_q_len, int32_t num_sms);
+int specdec_prompt_attention(const SpecdecPromptArgs* args, specdec_stream_t stream);
+
+/*
+ * Paged attention of a batch in which groups of sequences have the same first pages.  The answer is
+ * specdec_paged_attention's (the same mask; decode, verify and longer blocks of new rows); group g's first
+ * prefix_len[g] tokens are read once for all of its members instead of once each.  members[group_start[g] ..
+ * group_start[g + 1] - 1] are the sequences of group g; a sequence is in one group at most, and one that is in none is
+ * attended to alone.  The pages of a group's prefix are taken from the page table of its first member with rows; of
+ * prefix_len only whole pages that every row of the group sees are shared, the rest is read from each member's own
+ * table.  A member out of range or listed twice, a negative prefix or a bad group_start raises
+ * SPECDEC_STATUS_BAD_GROUP (a sequence listed twice counts where it is listed first); bad lengths skip the sequence as
+ * in specdec_prompt_attention.  No counterpart in the reference (batch 1).
+ */
+typedef struct SpecdecSharedPrefixArgs {
+  const void* q; /* bf16 */
+  void* out;     /* bf16 */
+  int64_t q_stride_tok, q_stride_head;
+  int64_t o_stride_tok, o_stride_head;
+  SpecdecBatch batch; /* max_ctx_len is not used */
+  SpecdecPagedKV kv;
+  const int32_t* group_start; /* [num_groups + 1] */
+  const int32_t* members;     /* [num_members] */
+  const int32_t* prefix_len;  /* [num_groups] tokens */
+  int32_t num_groups;
+  int32_t num_members;
+  int64_t q_rows; /* rows of q and out */
+  float sm_scale;
+  void* workspace; /* >= specdec_shared_prefix_workspace_bytes(...) bytes, 256-byte aligned, any contents */
+  size_t workspace_bytes;
+  int32_t* status;
+  int32_t reuse_plan;
+  int32_t num_sms;
+} SpecdecSharedPrefixArgs;
+
+size_t specdec_shared_prefix_workspace_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                                             int32_t head_dim, int32_t max_q_len, int32_t num_groups,
+                                             int32_t num_members, int32_t num_sms);
+int specdec_shared_prefix_attention(const SpecdecSharedPrefixArgs* args, specdec_stream_t stream);
 
 /* RMSNorm over the last dim (fp32 mean of squares; the normalised value is
    rounded to the input dtype before the weight multiply, as model_self.RMSNORM). */

@@ -1011,17 +1011,15 @@ __global__ void __launch_bounds__(128) attn_f32_kernel(const float* __restrict__
 }
 
 // ---------------------------------------------------------------- host side
-static PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
+PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult qres;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
         qres == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }
+      return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    return static_cast<PFN_cuTensorMapEncodeTiled_v12000>(nullptr);
+  }();
   return fn;
 }
 
@@ -1043,7 +1041,7 @@ static int encode_kv_map(CUtensorMap* map, const void* base, int planes, int T, 
 
 // 2-D map over `n_rows` contiguous rows of `row_bytes` bytes (64-bit elements, no
 // swizzle) whose box is one row: the shape tile::gather4 loads fetch four rows of.
-static int encode_rows_map(CUtensorMap* map, const void* base, uint64_t n_rows, uint32_t row_bytes) {
+int encode_rows_map(CUtensorMap* map, const void* base, uint64_t n_rows, uint32_t row_bytes) {
   auto fn = get_encode_fn();
   if (!fn) return fail(SPECDEC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   if (row_bytes % 16 || row_bytes / 8 > 256 || n_rows == 0)

@@ -1,0 +1,1163 @@
+// row_attention.cu -- attention of many query rows against a shared run of keys: whole prompts (packed rows,
+// causal) and batches whose sequences share their first cache pages.
+//
+//   o[r] = sum_j softmax_j(scale q[r] . k[j]) v[j],   j < limit[r]
+//
+// A *unit* is up to 256 query rows of one KV head -- two row tiles of 128, which are TMEM lanes -- against a run of
+// keys.  The query heads of a KV head are rows of their own (row = token * n_rep + head), so a tile holds
+// 128 / n_rep tokens whose causal limits lie close together, and a decode step's few rows share a tile.  In a
+// shared prefix the tokens of all member sequences are the rows of one part; every sequence's own keys are a part of
+// their own with its rows only, and the results of both are joined.
+//
+// Work: parts (prefix groups, then sequences) are cut into units, a unit costs its 128-key blocks plus kUnitCost,
+// and the concatenated costs are cut into equal ranges, one a CTA (plan kernel, one CTA).  A unit that a boundary
+// cuts becomes several items, whose unnormalised rows, maxima and sums go to the workspace and are joined by
+// merge kernels; the others are written to the output at once.
+//
+// One CTA an SM, 12 warps, each role walking the same items:
+//   warps 0-3, 4-7  softmax of row tile 0, 1: a thread owns a row, so maxima and sums need no exchange
+//   warp 8          K/V tiles by TMA into a ring (K 0, V 0, K 1, V 1, ...): packed rows as {64 dims, 128 rows} boxes,
+//                   pages as four-row gathers; both give [dim half][128 keys][128 B] in the 128-byte swizzle
+//   warp 9          MMA issue (one lane), owner of the TMEM
+//   warp 10         query rows of the next item into shared memory, and each row's key limit
+//   warp 11         zeroes the V rows past an item's last key, so that a masked key's zero probability
+//                   never meets what lies behind a sequence (its next one, a page's old contents; NaN x 0)
+// Per block j and tile t:  S_t = Q_t K_j^T (TMEM, fp32) -> P_t = exp2(S_t - m) as bf16 over the same columns
+// -> O_t += P_t V_j (A operand from TMEM).  The two tiles alternate, so one's softmax runs under the other's MMAs.
+// The running maximum moves only when a row's grows by more than 2^8 (then O is rescaled in place); S_t(j) is complete
+// only after O_t(j - 1), both being issued in this order by one lane, so the rescale needs no wait of its own.
+// P is rounded to bf16 (2^-9 of each weight, independent between keys); sums, maxima and O stay fp32.
+#include "sd_common.cuh"
+#include "sd_internal.h"
+#include "umma.cuh"
+
+namespace sd {
+
+constexpr int kRowTile = 128;      // rows of a tile: TMEM lanes
+constexpr int kUnitRows = 256;     // two tiles
+constexpr int kKeyBlock = 128;     // keys of a block
+constexpr int kRowThreads = 384;
+constexpr int kUnitCost = 2;       // what a unit costs beside its blocks (query load, epilogue), in blocks
+constexpr int kMinQuota = 4;       // smallest range of a CTA, in blocks
+constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
+constexpr float kRowRescaleLog2 = 8.f;
+
+enum RowSource { kPacked = 0, kPaged = 1 };
+
+struct alignas(16) RowItem {
+  int32_t src;     // sequence, or ~group
+  int32_t vt0;     // first token of the unit, in the part
+  int32_t n_vt;    // tokens of the part
+  int32_t head;    // KV head
+  int32_t k0, k1;  // keys of this item
+  int32_t slot;    // first workspace row of the partial, or -1: the output itself
+  int32_t nblk;    // blocks (0: nothing to do)
+  int32_t row0;    // sequence: first query row
+  int32_t first;   // sequence: keys before its first new token; group: the prefix
+  int32_t kv;      // packed: first key row; paged: sequence whose page table is read
+  int32_t member0; // group: first member
+};
+static_assert(sizeof(RowItem) == 48, "three 16-byte loads");
+
+struct RowParams {
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  int64_t q_st, q_sh, o_st, o_sh;
+  const int32_t *q_row0, *q_len, *ctx_len, *kv_row0;
+  const int32_t *group_start, *members, *prefix_len;
+  const int32_t* page_table;
+  int64_t q_rows, kv_rows;
+  int32_t B, H, KV, n_rep, tpt, q_max, G, M;
+  int32_t num_pages, max_pages, paged;
+  int32_t grid, compact;        // CTAs of the plan; compact: slots only for cut units
+  int32_t cap_seq, cap_group;   // workspace rows of a sequence's / a group's slot
+  int32_t group_rows;           // workspace rows before the sequences' slots
+  float scale_log2;
+  int32_t* status;
+  // workspace
+  int32_t *cta_first, *cta_last, *cut_unit;     // [grid]
+  int64_t* part_cost;                           // [G + B] starts
+  int32_t* part_units;
+  int32_t *valid_len, *first_member, *seq_group, *seq_vt;  // [B]
+  int32_t *prefix, *group_table;                // [G]
+  int2* member_row;                             // [M] {first query row, tokens}
+  int2* unit_info;                              // [units] {first slot row, pieces}
+  RowItem* items;                               // [units + grid]
+  float2* part_ml;                              // [slot rows] {max (log2), sum}
+  float* part_o;                                // [slot rows][D]
+};
+
+// ---------------------------------------------------------------- plan
+struct PartInfo {
+  int n_vt, k0, first, causal;  // keys k0 .. first + i (causal) or k0 .. first - 1
+};
+SD_DEV PartInfo part_info(const RowParams& p, int part) {
+  PartInfo f;
+  if (part < p.G) {
+    f.k0 = 0;
+    f.first = p.prefix[part];  // 0 where the group is empty or its start bad
+    f.n_vt = f.first > 0 ? (p.group_start[part + 1] - p.group_start[part]) * p.q_max : 0;
+    f.causal = 0;
+  } else {
+    const int b = part - p.G;
+    f.n_vt = p.valid_len[b];
+    f.first = f.n_vt > 0 ? p.ctx_len[b] - f.n_vt : 0;
+    const int g = f.n_vt > 0 ? p.seq_group[b] : -1;
+    f.k0 = g >= 0 ? p.prefix[g] : 0;
+    f.causal = 1;
+  }
+  return f;
+}
+// blocks of the part's unit row r (units of one row have as many for every KV head)
+SD_DEV int unit_blocks(const RowParams& p, const PartInfo& f, int r) {
+  const int end = f.causal ? f.first + min((r + 1) * 2 * p.tpt, f.n_vt) : f.first;
+  return (end - f.k0 + kKeyBlock - 1) / kKeyBlock;
+}
+
+__global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  __shared__ int64_t s_warp[2][32];
+  __shared__ int64_t s_run[2];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nthr = blockDim.x;
+  for (int b = tid; b < p.B; b += nthr) {
+    const int n = p.q_len[b], c = p.ctx_len[b], r0 = p.q_row0[b];
+    int bad = 0;
+    if (n < 0 || n > p.q_max || (n > 0 && (c < n || r0 < 0 || static_cast<int64_t>(r0) + n > p.q_rows)))
+      bad = SPECDEC_STATUS_BAD_LENGTH;
+    else if (n > 0 && p.paged && c > static_cast<int64_t>(p.max_pages) * kPage)
+      bad = SPECDEC_STATUS_PAGE_OVERFLOW;
+    else if (n > 0 && !p.paged && (p.kv_row0[b] < 0 || static_cast<int64_t>(p.kv_row0[b]) + c > p.kv_rows))
+      bad = SPECDEC_STATUS_BAD_LENGTH;
+    if (bad) raise_status(p.status, bad);
+    p.valid_len[b] = bad ? 0 : n;
+    if (p.G > 0) {
+      p.first_member[b] = 0x7fffffff;
+      p.seq_group[b] = -1;
+    } else {
+      p.seq_group[b] = -1;
+    }
+  }
+  for (int c = tid; c < p.grid; c += nthr) {
+    p.cta_first[c] = 0;
+    p.cta_last[c] = -1;
+    p.cut_unit[c] = -1;
+  }
+  if (p.G > 0) {
+    int bad = 0;
+    for (int g = tid; g < p.G; g += nthr) {
+      const int n = p.prefix_len[g], a = p.group_start[g], e = p.group_start[g + 1];
+      bad |= a < 0 || e < a || e > p.M;
+      if (n < 0) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
+      p.prefix[g] = max(n, 0);
+      p.group_table[g] = 0x7fffffff;
+    }
+    // starts that do not ascend within the member list: nobody is in a group, everything is attended to alone
+    bad = __syncthreads_or(bad);
+    if (bad && tid == 0) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
+    const int M = bad ? 0 : p.M;
+    for (int i = tid; i < M; i += nthr) {
+      const int b = p.members[i];
+      if (b < 0 || b >= p.B)
+        raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
+      else
+        atomicMin(&p.first_member[b], i);  // a sequence listed twice counts where it is listed first
+    }
+    __syncthreads();
+    for (int i = tid; i < M; i += nthr) {
+      const int b = p.members[i];
+      int2 mr = make_int2(0, 0);
+      if (b >= 0 && b < p.B) {
+        if (p.first_member[b] != i) {
+          raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
+        } else {
+          int lo = 0, hi = p.G;  // the last group that starts at or before i, and holds it
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (p.group_start[mid] <= i) lo = mid; else hi = mid;
+          }
+          const int gs = p.group_start[lo], ge = p.group_start[lo + 1];
+          if (i >= gs && i < ge) {
+            const int n = p.valid_len[b];
+            p.seq_group[b] = lo;
+            p.seq_vt[b] = (i - gs) * p.q_max;
+            mr = make_int2(p.q_row0[b], n);
+            if (n > 0) {
+              // keys that all of the group's rows see
+              atomicMin(&p.prefix[lo], p.ctx_len[b] - n);
+              atomicMin(&p.group_table[lo], i);
+            }
+          }
+        }
+      }
+      p.member_row[i] = mr;
+    }
+    __syncthreads();
+    for (int g = tid; g < p.G; g += nthr) {
+      const int i = p.group_table[g];
+      p.prefix[g] = i == 0x7fffffff ? 0 : p.prefix[g] / kPage * kPage;  // whole pages
+      p.group_table[g] = i == 0x7fffffff ? 0 : p.members[i];
+    }
+  }
+  __syncthreads();
+  // cost and unit count of every part
+  const int parts = p.G + p.B;
+  for (int part = warp; part < parts; part += nthr / 32) {
+    const PartInfo f = part_info(p, part);
+    const int rows = (f.n_vt + 2 * p.tpt - 1) / (2 * p.tpt);
+    int64_t sum = 0;
+    for (int r = lane; r < rows; r += 32) sum += unit_blocks(p, f, r) + kUnitCost;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+      p.part_cost[part] = sum * p.KV;
+      p.part_units[part] = rows * p.KV;
+    }
+  }
+  if (tid == 0) s_run[0] = s_run[1] = 0;
+  __syncthreads();
+  for (int base = 0; base < parts; base += nthr) {  // exclusive scans, in place
+    const int i = base + tid;
+    int64_t v[2] = {i < parts ? p.part_cost[i] : 0, i < parts ? p.part_units[i] : 0}, x[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      x[q] = v[q];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x[q], o);
+        if (lane >= o) x[q] += y;
+      }
+      if (lane == 31) s_warp[q][warp] = x[q];
+    }
+    __syncthreads();
+    if (warp < 2) {
+      int64_t w = s_warp[warp][lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
+      }
+      s_warp[warp][lane] = w;
+    }
+    __syncthreads();
+    const int64_t run0 = s_run[0], run1 = s_run[1];
+    if (i < parts) {
+      p.part_cost[i] = run0 + (warp ? s_warp[0][warp - 1] : 0) + x[0] - v[0];
+      p.part_units[i] = static_cast<int>(run1 + (warp ? s_warp[1][warp - 1] : 0) + x[1] - v[1]);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      s_run[0] += s_warp[0][31];
+      s_run[1] += s_warp[1][31];
+    }
+    __syncthreads();
+  }
+  const int64_t total = s_run[0];
+  const int64_t quota = max((total + p.grid - 1) / p.grid, static_cast<int64_t>(kMinQuota));
+  // costs pass 32 bits only for prompts of millions of tokens
+  auto cta_of = [&](int64_t at) {
+    return total < 0x7fffffff ? static_cast<int>(at) / static_cast<int>(quota) : static_cast<int>(at / quota);
+  };
+  // items
+  for (int part = warp; part < parts; part += nthr / 32) {
+    const PartInfo f = part_info(p, part);
+    const int rows = (f.n_vt + 2 * p.tpt - 1) / (2 * p.tpt);
+    int64_t start = p.part_cost[part];
+    const int ubase = p.part_units[part];
+    const bool group = part < p.G;
+    const int b = part - p.G;
+    RowItem it;
+    it.src = group ? ~part : b;
+    it.n_vt = f.n_vt;
+    it.row0 = group ? 0 : p.q_row0[b];
+    it.first = f.first;
+    it.kv = group ? p.group_table[part] : (p.paged ? b : p.kv_row0[b]);
+    it.member0 = group ? p.group_start[part] : 0;
+    // a sequence without shared keys writes its uncut rows itself
+    const bool alone = !group && f.k0 == 0;
+    for (int r0 = 0; r0 < rows; r0 += 32) {
+      const int r = r0 + lane;
+      const int nb = r < rows ? unit_blocks(p, f, r) : 0;
+      const int cost = r < rows ? nb + kUnitCost : 0;
+      int64_t x = static_cast<int64_t>(cost) * p.KV;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const int64_t before = x - static_cast<int64_t>(cost) * p.KV;
+      const int64_t chunk = __shfl_sync(0xffffffffu, x, 31);
+      if (r < rows) {
+        it.vt0 = r * 2 * p.tpt;
+        const int end = f.causal ? f.first + min(it.vt0 + 2 * p.tpt, f.n_vt) : f.first;
+        for (int h = 0; h < p.KV; ++h) {
+          const int u = ubase + r * p.KV + h;
+          const int64_t us = start + before + static_cast<int64_t>(h) * cost, ue = us + cost;
+          const int c0 = cta_of(us), c1 = cta_of(ue - 1);
+          it.head = h;
+          // pieces that hold blocks: a CTA whose range ends in the unit's own cost has none
+          const int cb = cta_of(us + kUnitCost);  // first CTA with a block
+          const int pieces = c1 - cb + 1;
+          const int cap = group ? p.cap_group : p.cap_seq;
+          const int slot0 = p.compact ? 2 * cb + 1 : u + cb;
+          const int64_t row0 = (group ? 0 : p.group_rows) + static_cast<int64_t>(slot0) * cap;
+          const bool direct = alone && pieces == 1;
+          p.unit_info[u] = make_int2(static_cast<int>(row0), pieces);
+          if (pieces > 1) p.cut_unit[cb] = u;
+          for (int c = c0; c <= c1; ++c) {
+            const int64_t from = c * quota, to = from + quota;
+            const int a = static_cast<int>(max(from - us - kUnitCost, static_cast<int64_t>(0)));
+            const int e = static_cast<int>(min(to - us - kUnitCost, static_cast<int64_t>(nb)));
+            const int step = c - cb;
+            it.nblk = max(e - a, 0);
+            it.k0 = f.k0 + a * kKeyBlock;
+            it.k1 = min(f.k0 + e * kKeyBlock, end);
+            it.slot = direct ? -1 : static_cast<int>(row0 + static_cast<int64_t>(p.compact && step > 0 ? 2 * step - 1 : step) * cap);
+            p.items[u + c] = it;
+            const int64_t hi = min(to, total) - 1;
+            if (from >= us && from < ue) p.cta_first[c] = u + c;
+            if (hi >= us && hi < ue) p.cta_last[c] = u + c;
+          }
+        }
+      }
+      start += chunk;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- geometry
+template <int D>
+struct RowGeom {
+  static constexpr int KH = D / 64;               // 128-byte dim halves
+  static constexpr int TILE = 16384 * KH;         // one K or V block, one query tile
+  static constexpr int NS = D == 128 ? 5 : 12;    // ring slots (a K or a V block each)
+  static constexpr int RING = 2 * TILE;           // the ring lies behind the two query tiles
+  static constexpr int SMEM = RING + NS * TILE + 1024;
+  static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
+  static_assert(SMEM <= 227 * 1024 - 2048, "shared memory budget, 2 KB of static variables aside");
+};
+
+SD_DEV RowItem load_item(const RowItem* at) {
+  RowItem it;
+  const int4* s = reinterpret_cast<const int4*>(at);
+  int4* d = reinterpret_cast<int4*>(&it);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) d[i] = s[i];
+  return it;
+}
+// blocks of row tile t of an item
+SD_DEV int tile_blocks(const RowParams& p, const RowItem& it, int t) {
+  const int v0 = it.vt0 + t * p.tpt;
+  if (v0 >= it.n_vt) return 0;
+  if (it.src < 0) return it.nblk;
+  const int end = min(it.first + min(v0 + p.tpt, it.n_vt), it.k1);
+  return end <= it.k0 ? 0 : (end - it.k0 + kKeyBlock - 1) / kKeyBlock;
+}
+
+SD_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+SD_DEV void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// 3-D tiled load that stays in L2 as the hardware sees fit (K/V blocks are read again by other CTAs)
+SD_DEV void tma_tile_3d(void* dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
+SD_DEV void tma_rows4(void* dst, const CUtensorMap* map, int32_t r0, int32_t r1, int32_t r2, int32_t r3,
+                      uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// ---------------------------------------------------------------- main kernel
+template <int D, int SRC>
+__global__ void __launch_bounds__(kRowThreads, 1) row_attention_kernel(const RowParams p,
+                                                                       const __grid_constant__ CUtensorMap kmap,
+                                                                       const __grid_constant__ CUtensorMap vmap) {
+  using Geo = RowGeom<D>;
+  constexpr int NS = Geo::NS, KH = Geo::KH;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[NS], empty[NS];
+  __shared__ uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], c_req, v_clean, fin;
+  __shared__ int32_t s_limit[kUnitRows];
+  __shared__ uint32_t s_tmem;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 1 + 8);
+    mbar_init(&c_req, 1);
+    mbar_init(&v_clean, 1);
+    mbar_init(&fin, 1);
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    umma::tmem_alloc(&s_tmem, Geo::TMEM_COLS);
+    umma::tmem_relinquish();
+  }
+  if (warp == 8 && lane == 0) {
+    prefetch_tmap(&kmap);
+    prefetch_tmap(&vmap);
+  }
+  grid_dep_wait();
+  grid_dep_launch();
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  const int i0 = p.cta_first[blockIdx.x], i1 = p.cta_last[blockIdx.x];
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ K/V blocks
+    uint32_t n = 0;  // blocks issued (K and V each count)
+    bool ok = true;
+    for (int i = i0; i <= i1 && ok; ++i) {
+      const RowItem it = load_item(p.items + i);
+      if (it.nblk == 0) continue;
+      const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+      int ids = 0;  // paged: lane l holds the page of keys 16 (32 (j / 4) + l) ..
+      for (int j = 0; j < nb && ok; ++j) {
+        if (SRC == kPaged && (j & 3) == 0) {
+          const int last = (it.k1 - 1) / kPage;
+          const int pg = min(it.k0 / kPage + 8 * j + lane, last);
+          ids = p.page_table[static_cast<int64_t>(it.kv) * p.max_pages + pg];
+          if (ids < 0 || ids >= p.num_pages) {
+            raise_status(p.status, SPECDEC_STATUS_BAD_PAGE);
+            ids = 0;
+          }
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const uint32_t s = n % NS, round = n / NS;
+          if (round > 0 && !warp_wait(&empty[s], (round - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = smem + Geo::RING + s * Geo::TILE;
+          const CUtensorMap* map = kv ? &vmap : &kmap;
+          if (SRC == kPacked) {
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&full[s], Geo::TILE);
+#pragma unroll
+              for (int x = 0; x < KH; ++x)
+                tma_tile_3d(dst + x * 16384, map, x * 64, it.head, it.kv + it.k0 + j * kKeyBlock, &full[s]);
+            }
+          } else {
+            int pg[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pg[e] = __shfl_sync(0xffffffffu, ids, 8 * (j & 3) + e);
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&full[s], Geo::TILE);
+#pragma unroll
+              for (int x = 0; x < KH; ++x)
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                  auto row = [&](int k) { return (pg[k] * p.KV + it.head) * KH + x; };
+                  tma_rows4(dst + x * 16384 + e * 2048, map, row(e), row(e + 1), row(e + 2), row(e + 3), &full[s]);
+                }
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (!ok) {
+      if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      // copies under way land before the CTA leaves
+      for (uint32_t k = n > NS ? n - NS : 0; k < n; ++k) (void)warp_wait(&full[k % NS], (k / NS) & 1);
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issue
+    if (lane == 0) {
+      constexpr uint32_t id_qk = umma::idesc_f16(128, kKeyBlock, true, true, false, false);
+      constexpr uint32_t id_pv = umma::idesc_f16(128, D, true, true, false, true);
+      const uint32_t q_base = smem_u32(smem), ring = smem_u32(smem + Geo::RING);
+      uint32_t n = 0, pn[2] = {0, 0}, items = 0, cleaned = 0;
+      bool ok = true;
+      auto slot_ready = [&](uint32_t k) { return mbar_wait(&full[k % NS], (k / NS) & 1); };
+      auto qk = [&](int t, uint32_t k) {
+        const uint32_t qa = q_base + t * Geo::TILE, ka = ring + (k % NS) * Geo::TILE;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t at = (kk >> 2) * 16384 + (kk & 3) * 32;
+          umma::mma_f16_ss(umma::taddr(tmem, 0, Geo::S_COL + t * 128), umma::desc_kmajor_sw128(qa + at),
+                           umma::desc_kmajor_sw128(ka + at), id_qk, kk > 0);
+        }
+        umma::commit(&s_full[t]);
+      };
+      for (int i = i0; i <= i1 && ok; ++i) {
+        const RowItem it = load_item(p.items + i);
+        if (it.nblk == 0) continue;
+        const int nt[2] = {tile_blocks(p, it, 0), tile_blocks(p, it, 1)};
+        const int nb = max(nt[0], nt[1]);
+        const bool clean = (it.k1 - it.k0) % kKeyBlock != 0;
+        ok = mbar_wait(&q_full, items & 1) && slot_ready(n);
+        if (!ok) break;
+        umma::fence_after_sync();
+        if (nt[0] > 0) qk(0, n);
+        if (nt[1] > 0) qk(1, n);
+        if (nb == 1) umma::commit(&q_empty);
+        umma::commit(&empty[n % NS]);
+        for (int j = 0; j < nb && ok; ++j) {
+          const uint32_t kv = n + 2 * j + 1, kn = kv + 1;  // this block's V, the next block's K
+          bool v_in = false, k_in = false;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= nt[t]) continue;
+            if (!v_in) {
+              ok = ok && slot_ready(kv);
+              // the last block's V is zeroed past the last key while the softmax works on the block
+              if (ok && clean && j == nb - 1) mbar_arrive(&c_req);
+            }
+            ok = ok && mbar_wait(&p_full[t], pn[t] & 1);
+            if (!v_in && clean && j == nb - 1) ok = ok && mbar_wait(&v_clean, cleaned++ & 1);
+            v_in = true;
+            if (!ok) break;
+            ++pn[t];
+            umma::fence_after_sync();
+            const uint32_t va = ring + (kv % NS) * Geo::TILE;
+#pragma unroll
+            for (int kk = 0; kk < kKeyBlock / 16; ++kk)
+              umma::mma_f16_ts(umma::taddr(tmem, 0, Geo::O_COL + t * D),
+                               umma::taddr(tmem, 0, Geo::S_COL + t * 128 + kk * 8),
+                               umma::desc_mnmajor_sw128(va + kk * 2048, 16384), id_pv, j > 0 || kk > 0);
+            if (j == nt[t] - 1) {
+              umma::commit(&o_full[t]);
+            } else {
+              if (!k_in) {
+                ok = slot_ready(kn);
+                k_in = true;
+                if (!ok) break;
+                umma::fence_after_sync();
+              }
+              qk(t, kn);
+            }
+          }
+          if (!ok) break;
+          umma::commit(&empty[kv % NS]);
+          if (j + 1 < nb) {
+            umma::commit(&empty[kn % NS]);
+            if (j + 2 == nb) umma::commit(&q_empty);
+          }
+        }
+        n += 2 * nb;
+        ++items;
+      }
+      if (!ok) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      umma::commit(&fin);
+      (void)mbar_wait(&fin, 0);
+    }
+    __syncwarp();
+  } else if (warp == 10) {
+    // ------------------------------------------------------------ query rows and limits
+    constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte chunks of a row, rows a step
+    const uint32_t q_base = smem_u32(smem);
+    uint32_t items = 0;
+    for (int i = i0; i <= i1; ++i) {
+      const RowItem it = load_item(p.items + i);
+      if (it.nblk == 0) continue;
+      const int tiles = it.vt0 + p.tpt < it.n_vt ? 2 : 1;
+      if (items > 0 && !warp_wait(&q_empty, (items - 1) & 1)) {
+        if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+        break;
+      }
+      for (int base = 0; base < tiles * kRowTile; base += 32) {
+        const int t = base / kRowTile, r = base % kRowTile + lane;
+        const int tok = r / p.n_rep, vt = it.vt0 + t * p.tpt + tok;
+        int64_t off = -1;
+        int limit = 0;
+        if (tok < p.tpt && vt < it.n_vt) {
+          int row = -1;
+          if (it.src >= 0) {
+            row = it.row0 + vt;
+            limit = min(it.first + vt + 1, it.k1);
+          } else {
+            const int m = vt / p.q_max, e = vt - m * p.q_max;
+            const int2 mr = p.member_row[it.member0 + m];
+            if (e < mr.y) {
+              row = mr.x + e;
+              limit = it.k1;
+            }
+          }
+          if (row >= 0)
+            off = static_cast<int64_t>(row) * p.q_st +
+                  static_cast<int64_t>(it.head * p.n_rep + r - tok * p.n_rep) * p.q_sh;
+        }
+        s_limit[base + lane] = limit;
+#pragma unroll 4
+        for (int e = 0; e < 32; e += RP) {
+          const int64_t o = __shfl_sync(0xffffffffu, off, e + lane / CH);
+          const int rr = base % kRowTile + e + lane / CH, ch = lane % CH;
+          const uint32_t dst =
+              q_base + t * Geo::TILE + (ch >> 3) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
+          cp_async16(dst, p.q + (o < 0 ? 0 : o + ch * 8), o < 0 ? 0u : 16u);
+        }
+      }
+      cp_async_wait_all();
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+      ++items;
+    }
+    cp_async_wait_all();
+  } else if (warp == 11) {
+    // ------------------------------------------------------------ V rows past the last key
+    uint32_t n = 0, cleaned = 0;
+    for (int i = i0; i <= i1; ++i) {
+      const RowItem it = load_item(p.items + i);
+      if (it.nblk == 0) continue;
+      const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+      const int rem = (it.k1 - it.k0) % kKeyBlock;
+      if (rem != 0) {
+        const uint32_t k = n + 2 * nb - 1;
+        // asked for by the MMA warp, which has seen the block arrive and waits for the answer
+        if (!warp_wait(&c_req, cleaned & 1)) {
+          if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+          break;
+        }
+        uint8_t* v = smem + Geo::RING + (k % NS) * Geo::TILE;
+#pragma unroll
+        for (int x = 0; x < KH; ++x)
+          for (int o = rem * 128 + lane * 16; o < 16384; o += 512)
+            *reinterpret_cast<uint4*>(v + x * 16384 + o) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_clean);
+        ++cleaned;
+      }
+      n += 2 * nb;
+    }
+  } else {
+    // ------------------------------------------------------------ softmax and epilogue: a thread a row
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 5;
+    const uint32_t s_ta = umma::taddr(tmem, lanes, Geo::S_COL + t * 128);
+    const uint32_t o_ta = umma::taddr(tmem, lanes, Geo::O_COL + t * D);
+    const float scale = p.scale_log2;
+    const float grow = kRowRescaleLog2 / scale;
+    uint32_t sn = 0, items = 0, on = 0;
+    bool ok = true;
+    for (int i = i0; i <= i1 && ok; ++i) {
+      const RowItem it = load_item(p.items + i);
+      if (it.nblk == 0) continue;
+      ok = warp_wait(&q_full, items & 1);
+      if (!ok) break;
+      ++items;
+      const int limit = s_limit[t * kRowTile + row];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty);
+      const int nb = tile_blocks(p, it, t);
+      if (nb == 0) {  // no tile, or a piece past the tile's keys: the row's other pieces are all of it
+        if (it.slot >= 0 && it.vt0 + t * p.tpt < it.n_vt && limit > 0)
+          p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
+        continue;
+      }
+      const bool any_row = __any_sync(0xffffffffu, limit > 0);
+      const int least = __reduce_min_sync(0xffffffffu, limit > 0 ? limit : 0x7fffffff);
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < nb; ++j, ++sn) {
+        ok = warp_wait(&s_full[t], sn & 1);
+        if (!ok) break;
+        umma::fence_after_sync();
+        if (any_row) {
+          float s[128];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) umma::tmem_ld32(s_ta + 32 * c, s + 32 * c);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) umma::tmem_wait_ld32(s + 32 * c);
+          const int key0 = it.k0 + j * kKeyBlock;
+          if (least < key0 + kKeyBlock) {
+            const int vis = limit - key0;
+#pragma unroll
+            for (int c = 0; c < 128; ++c) s[c] = c < vis ? s[c] : -INFINITY;
+          }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int c = 4; c < 124; c += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(s[c + e], s[c + 4 + e]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[124 + e]);
+          const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          if (j == 0) {
+            m = bm;
+          } else {
+            const bool need = bm > m + grow;
+            if (__any_sync(0xffffffffu, need)) {
+              const float alpha = need ? fast_exp2((m - bm) * scale) : 1.f;
+              if (need) m = bm;
+              l *= alpha;
+#pragma unroll
+              for (int c = 0; c < D; c += 32) {
+                float o[32];
+                umma::tmem_ld32(o_ta + c, o);
+                umma::tmem_wait_ld32(o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] *= alpha;
+                umma::tmem_st16(o_ta + c, reinterpret_cast<const float(&)[16]>(o[0]));
+                umma::tmem_st16(o_ta + c + 16, reinterpret_cast<const float(&)[16]>(o[16]));
+              }
+            }
+          }
+          const float neg = m == -INFINITY ? 0.f : -m * scale;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float a = fast_exp2(fmaf(s[32 * c + 2 * e], scale, neg));
+              const float b = fast_exp2(fmaf(s[32 * c + 2 * e + 1], scale, neg));
+              sum[(2 * e) & 3] += a;
+              sum[(2 * e + 1) & 3] += b;
+              w[e] = pack_bf16(a, b);
+            }
+            umma::tmem_st16_words(s_ta + 16 * c, w);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          umma::tmem_wait_st();
+        }
+        umma::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      ok = warp_wait(&o_full[t], on & 1);
+      if (!ok) break;
+      ++on;
+      umma::fence_after_sync();
+      if (any_row) {
+        const int tok = row / p.n_rep;
+        if (it.slot < 0) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const int64_t at = static_cast<int64_t>(it.row0 + it.vt0 + t * p.tpt + tok) * p.o_st +
+                             static_cast<int64_t>(it.head * p.n_rep + row - tok * p.n_rep) * p.o_sh;
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            umma::tmem_ld32(o_ta + c, o);
+            umma::tmem_wait_ld32(o);
+            if (limit > 0) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8)
+                *reinterpret_cast<uint4*>(p.out + at + c + e) =
+                    make_uint4(pack_bf16(o[e] * inv, o[e + 1] * inv), pack_bf16(o[e + 2] * inv, o[e + 3] * inv),
+                               pack_bf16(o[e + 4] * inv, o[e + 5] * inv), pack_bf16(o[e + 6] * inv, o[e + 7] * inv));
+            }
+          }
+        } else {
+          const int64_t at = it.slot + t * kRowTile + row;
+          if (limit > 0) p.part_ml[at] = make_float2(m * scale, l);
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            umma::tmem_ld32(o_ta + c, o);
+            umma::tmem_wait_ld32(o);
+            if (limit > 0) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4*>(p.part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+          }
+        }
+      }
+    }
+    if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  if (warp == 9) {
+    umma::fence_after_sync();
+    umma::tmem_dealloc(tmem, Geo::TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- joining partial rows
+// One warp a row: the pieces of up to two units, each a run of slots.  A piece that saw no key of the row has
+// sum 0 and maximum -inf and weighs nothing.
+struct Pieces {
+  int64_t row;  // workspace row of the first piece
+  int n, cap;
+  bool compact;
+  SD_DEV int64_t at(int i) const { return row + static_cast<int64_t>(compact && i > 0 ? 2 * i - 1 : i) * cap; }
+};
+template <int D>
+SD_DEV void join_row(const RowParams& p, const Pieces& a, const Pieces& b, __nv_bfloat16* out, int lane) {
+  constexpr int PER = D / 32;
+  const int n = a.n + b.n;
+  auto at = [&](int i) { return i < a.n ? a.at(i) : b.at(i - a.n); };
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 32) {
+    const float x = p.part_ml[at(i)].x;
+    m = (x > m || x != x) ? x : m;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float x = __shfl_xor_sync(0xffffffffu, m, o);
+    m = (x > m || x != x) ? x : m;
+  }
+  const float mu = m == -INFINITY ? 0.f : m;
+  float acc[PER] = {}, l = 0.f;
+  for (int base = 0; base < n; base += 32) {
+    const int i = base + lane;
+    float w = 0.f;
+    int64_t r = 0;
+    if (i < n) {
+      r = at(i);
+      const float2 ml = p.part_ml[r];
+      w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : fast_exp2(ml.x - mu);
+      l += w * ml.y;
+    }
+    const int k = min(32, n - base);
+#pragma unroll 4
+    for (int e = 0; e < k; ++e) {
+      const float we = __shfl_sync(0xffffffffu, w, e);
+      const int64_t re = __shfl_sync(0xffffffffu, r, e);
+      if (we == 0.f) continue;
+      if (PER == 4) {
+        const float4 x = reinterpret_cast<const float4*>(p.part_o + re * D)[lane];
+        acc[0] += we * x.x;
+        acc[1] += we * x.y;
+        acc[PER > 2 ? 2 : 0] += we * x.z;
+        acc[PER > 2 ? 3 : 0] += we * x.w;
+      } else {
+        const float2 x = reinterpret_cast<const float2*>(p.part_o + re * D)[lane];
+        acc[0] += we * x.x;
+        acc[1] += we * x.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (PER == 4)
+    reinterpret_cast<uint2*>(out)[lane] = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv),
+                                                     pack_bf16(acc[PER > 2 ? 2 : 0] * inv, acc[PER > 2 ? 3 : 0] * inv));
+  else
+    reinterpret_cast<uint32_t*>(out)[lane] = pack_bf16(acc[0] * inv, acc[1] * inv);
+}
+
+// rows of the units that a CTA boundary cuts (no groups): block (c, y) takes a share of the unit that is cut in CTA c
+template <int D>
+__global__ void __launch_bounds__(256) join_cut_kernel(const RowParams p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int c = blockIdx.x, u = p.cut_unit[c];
+  if (u < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int2 info = p.unit_info[u];
+  const RowItem it = load_item(p.items + u + c);
+  for (int r = blockIdx.y * 8 + warp; r < kUnitRows; r += gridDim.y * 8) {
+    const int t = r / kRowTile, e = r % kRowTile, tok = e / p.n_rep, vt = it.vt0 + t * p.tpt + tok;
+    if (tok >= p.tpt || vt >= it.n_vt) continue;
+    const Pieces a{info.x + r, info.y, p.cap_seq, p.compact != 0}, none{0, 0, 0, false};
+    join_row<D>(p, a, none,
+                p.out + static_cast<int64_t>(it.row0 + vt) * p.o_st +
+                    static_cast<int64_t>(it.head * p.n_rep + e - tok * p.n_rep) * p.o_sh,
+                lane);
+  }
+}
+
+// rows of every sequence: its group's pieces and its own
+template <int D>
+__global__ void __launch_bounds__(256) join_rows_kernel(const RowParams p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int h = static_cast<int>(w % p.H);
+  const int64_t bi = w / p.H;
+  const int i = static_cast<int>(bi % p.q_max), b = static_cast<int>(bi / p.q_max);
+  if (b >= p.B || i >= p.valid_len[b]) return;
+  const int kvh = h / p.n_rep, rep = h - kvh * p.n_rep;
+  auto pieces = [&](int part, int vt, int cap) {
+    const int2 info = p.unit_info[p.part_units[part] + vt / (2 * p.tpt) * p.KV + kvh];
+    const int in = vt % (2 * p.tpt), t = in / p.tpt;
+    return Pieces{info.x + t * kRowTile + (in - t * p.tpt) * p.n_rep + rep, info.y, cap, p.compact != 0};
+  };
+  Pieces own = pieces(p.G + b, i, p.cap_seq), pre{0, 0, 0, false};
+  const int g = p.seq_group[b];
+  if (g >= 0 && p.prefix[g] > 0)
+    pre = pieces(g, p.seq_vt[b] + i, p.cap_group);
+  else if (own.n == 1)
+    return;  // written already
+  join_row<D>(p, pre, own,
+              p.out + static_cast<int64_t>(p.q_row0[b] + i) * p.o_st + static_cast<int64_t>(h) * p.o_sh, lane);
+}
+
+// ---------------------------------------------------------------- host side
+struct RowShape {
+  int B, H, KV, D, q_max, G, M, sms;
+};
+struct RowSpace {
+  size_t first, last, cut, cost, units, valid, member, group, vt, prefix, table, mrow, info, items, ml, o, bytes;
+  int cap_seq, cap_group;
+  int64_t group_rows, rows;
+};
+
+static int row_sms(int requested) {
+  const int dev = device_sm_count();
+  return requested > 0 && requested < dev ? requested : dev;
+}
+
+static RowSpace row_space(const RowShape& s) {
+  RowSpace w;
+  const int n_rep = s.H / s.KV, tpt = kRowTile / n_rep;
+  auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const int64_t seq_units = s.B * up(s.q_max, 2 * tpt) * s.KV;
+  // groups' members: every group rounds its own rows up
+  const int64_t group_units = s.G > 0 ? (up(static_cast<int64_t>(s.M) * s.q_max, 2 * tpt) + s.G) * s.KV : 0;
+  auto cap = [&](int64_t tokens) {
+    return static_cast<int>(tokens <= tpt ? up(tokens * n_rep, 8) * 8 : kUnitRows);
+  };
+  w.cap_seq = cap(s.q_max);
+  w.cap_group = s.G > 0 ? cap(static_cast<int64_t>(s.M) * s.q_max) : 0;
+  w.group_rows = s.G > 0 ? (group_units + s.sms) * w.cap_group : 0;
+  // without groups a slot is taken by cut units only, two a CTA; else by every unit and one more a CTA
+  w.rows = w.group_rows + (s.G > 0 ? group_units + seq_units + s.sms + 1 : 2 * static_cast<int64_t>(s.sms) + 2) * w.cap_seq;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t o = at;
+    at = align_up(at + n, 256);
+    return o;
+  };
+  w.first = take(4 * s.sms);
+  w.last = take(4 * s.sms);
+  w.cut = take(4 * s.sms);
+  w.cost = take(8 * (s.G + s.B + 1));
+  w.units = take(4 * (s.G + s.B + 1));
+  w.valid = take(4 * s.B);
+  w.member = take(4 * s.B);
+  w.group = take(4 * s.B);
+  w.vt = take(4 * s.B);
+  w.prefix = take(4 * (s.G + 1));
+  w.table = take(4 * (s.G + 1));
+  w.mrow = take(8 * (s.M + 1));
+  w.info = take(8 * (seq_units + group_units));
+  w.items = take(sizeof(RowItem) * (seq_units + group_units + s.sms));
+  w.ml = take(8 * w.rows);
+  w.o = take(4 * w.rows * s.D);
+  w.bytes = at;
+  return w;
+}
+
+static bool row_shape_ok(const RowShape& s) {
+  return s.B > 0 && s.H > 0 && s.KV > 0 && s.H % s.KV == 0 && s.H / s.KV <= kRowTile && (s.D == 64 || s.D == 128) &&
+         s.q_max > 0 && s.G >= 0 && s.M >= 0;
+}
+
+static int check_shape(const RowShape& s) {
+  if (s.B <= 0 || s.H <= 0 || s.KV <= 0)
+    return fail(SPECDEC_ERR_INVALID, "num_seqs, num_q_heads and num_kv_heads must be positive");
+  if (s.H % s.KV != 0) return fail(SPECDEC_ERR_INVALID, "query heads must divide KV heads");
+  if (s.H / s.KV > kRowTile) return fail(SPECDEC_ERR_UNSUPPORTED, "at most 128 query heads per KV head");
+  if (s.D != 64 && s.D != 128) return fail(SPECDEC_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (s.q_max <= 0) return fail(SPECDEC_ERR_INVALID, "max_q_len must be positive");
+  if (s.G < 0 || s.M < 0 || (s.G == 0 && s.M != 0)) return fail(SPECDEC_ERR_INVALID, "bad group or member count");
+  // item, slot and cost numbers are 32-bit
+  const RowSpace w = row_space(s);
+  if (w.rows > 0x7fffffff || static_cast<int64_t>(s.M) * s.q_max > (1 << 30) || w.bytes > (size_t(1) << 40))
+    return fail(SPECDEC_ERR_UNSUPPORTED, "batch of %d sequences x %d tokens is too large for one call", s.B, s.q_max);
+  return SPECDEC_OK;
+}
+
+static int check_rows(const void* q, const void* out, int64_t qs, int64_t qh, int64_t os, int64_t oh) {
+  if (!q || !out) return fail(SPECDEC_ERR_INVALID, "q and out must be device pointers");
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u)
+    return fail(SPECDEC_ERR_INVALID, "q/out must be 16-byte aligned");
+  if ((qs | qh | os | oh) & 7) return fail(SPECDEC_ERR_INVALID, "q/out strides must be multiples of 8 elements");
+  return SPECDEC_OK;
+}
+
+static int fill_row_params(RowParams& p, const RowShape& s, void* ws, size_t ws_bytes, float sm_scale) {
+  if (!(sm_scale > 0.f) || sm_scale > 1e30f) return fail(SPECDEC_ERR_INVALID, "sm_scale must be positive and finite");
+  const RowSpace w = row_space(s);
+  if (!ws || ws_bytes < w.bytes)
+    return fail(SPECDEC_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, w.bytes);
+  if (reinterpret_cast<uintptr_t>(ws) & 255u) return fail(SPECDEC_ERR_INVALID, "workspace must be 256-byte aligned");
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  p.B = s.B;
+  p.H = s.H;
+  p.KV = s.KV;
+  p.n_rep = s.H / s.KV;
+  p.tpt = kRowTile / p.n_rep;
+  p.q_max = s.q_max;
+  p.G = s.G;
+  p.M = s.M;
+  p.grid = s.sms;
+  p.compact = s.G == 0;
+  p.cap_seq = w.cap_seq;
+  p.cap_group = w.cap_group;
+  p.group_rows = static_cast<int32_t>(w.group_rows);
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.cta_first = reinterpret_cast<int32_t*>(base + w.first);
+  p.cta_last = reinterpret_cast<int32_t*>(base + w.last);
+  p.cut_unit = reinterpret_cast<int32_t*>(base + w.cut);
+  p.part_cost = reinterpret_cast<int64_t*>(base + w.cost);
+  p.part_units = reinterpret_cast<int32_t*>(base + w.units);
+  p.valid_len = reinterpret_cast<int32_t*>(base + w.valid);
+  p.first_member = reinterpret_cast<int32_t*>(base + w.member);
+  p.seq_group = reinterpret_cast<int32_t*>(base + w.group);
+  p.seq_vt = reinterpret_cast<int32_t*>(base + w.vt);
+  p.prefix = reinterpret_cast<int32_t*>(base + w.prefix);
+  p.group_table = reinterpret_cast<int32_t*>(base + w.table);
+  p.member_row = reinterpret_cast<int2*>(base + w.mrow);
+  p.unit_info = reinterpret_cast<int2*>(base + w.info);
+  p.items = reinterpret_cast<RowItem*>(base + w.items);
+  p.part_ml = reinterpret_cast<float2*>(base + w.ml);
+  p.part_o = reinterpret_cast<float*>(base + w.o);
+  return SPECDEC_OK;
+}
+
+template <int D, int SRC>
+static int launch_row_attention(const RowParams& p, const CUtensorMap& kmap, const CUtensorMap& vmap, bool reuse_plan,
+                                cudaStream_t st) {
+  // the attribute belongs to the function on each device; setting it again is cheap and needs no state of its own
+  const cudaError_t e = cudaFuncSetAttribute(row_attention_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             RowGeom<D>::SMEM);
+  if (e != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "row_attention_kernel: %s", cudaGetErrorString(e));
+  if (!reuse_plan)
+    if (int rc = launch_pdl("row_plan_kernel", row_plan_kernel, dim3(1), dim3(1024), 0, st, p)) return rc;
+  if (int rc = launch_pdl("row_attention_kernel", row_attention_kernel<D, SRC>, dim3(p.grid), dim3(kRowThreads),
+                          RowGeom<D>::SMEM, st, p, kmap, vmap))
+    return rc;
+  if (p.G == 0)
+    return launch_pdl("join_cut_kernel", join_cut_kernel<D>, dim3(p.grid, kMergeParts), dim3(256), 0, st, p);
+  const int64_t warps = static_cast<int64_t>(p.B) * p.q_max * p.H;
+  return launch_pdl("join_rows_kernel", join_rows_kernel<D>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256),
+                    0, st, p);
+}
+
+// 3-D map {D, heads, rows} over packed rows with a {64, 1, 128} box and 128-byte swizzle; rows past the end read as zero
+static int encode_packed_map(CUtensorMap* map, const void* base, int64_t rows, int heads, int D, int64_t st, int64_t sh) {
+  auto fn = get_encode_fn();
+  if (!fn) return fail(SPECDEC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(st) * 2};
+  cuuint32_t box[3] = {64, 1, kKeyBlock};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SPECDEC_ERR_INVALID, "cuTensorMapEncodeTiled (packed) failed (%d)", static_cast<int>(r));
+  return SPECDEC_OK;
+}
+
+}  // namespace sd
+
+using namespace sd;
+
+extern "C" size_t specdec_prompt_workspace_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                                                 int32_t head_dim, int32_t max_q_len, int32_t num_sms) {
+  const RowShape s{num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_len, 0, 0, row_sms(num_sms)};
+  return row_shape_ok(s) ? row_space(s).bytes : 0;
+}
+
+extern "C" int specdec_prompt_attention(const SpecdecPromptArgs* a, specdec_stream_t stream) {
+  if (!a) return fail(SPECDEC_ERR_INVALID, "args is NULL");
+  const SpecdecBatch& bt = a->batch;
+  const RowShape s{bt.num_seqs, bt.num_q_heads, a->num_kv_heads, a->head_dim, bt.max_q_len, 0, 0, row_sms(a->num_sms)};
+  if (int rc = check_shape(s)) return rc;
+  if (int rc = check_rows(a->q, a->out, a->q_stride_tok, a->q_stride_head, a->o_stride_tok, a->o_stride_head)) return rc;
+  if (!a->k || !a->v) return fail(SPECDEC_ERR_INVALID, "k and v must be device pointers");
+  if (!bt.q_row0 || !bt.q_len || !bt.ctx_len || !a->kv_row0) return fail(SPECDEC_ERR_INVALID, "batch arrays must be set");
+  if (a->q_rows <= 0 || a->kv_rows <= 0 || a->q_rows > 0x7fffffff || a->kv_rows > 0x7fffffff)
+    return fail(SPECDEC_ERR_INVALID, "row counts out of range");
+  if ((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) & 15u)
+    return fail(SPECDEC_ERR_INVALID, "k/v must be 16-byte aligned");
+  const int64_t strides[4] = {a->k_stride_tok, a->k_stride_head, a->v_stride_tok, a->v_stride_head};
+  for (const int64_t x : strides)
+    if (x <= 0 || x % 8 || x >= (int64_t(1) << 38))
+      return fail(SPECDEC_ERR_INVALID, "k/v strides must be positive multiples of 8 elements");
+  RowParams p = {};
+  if (int rc = fill_row_params(p, s, a->workspace, a->workspace_bytes, a->sm_scale)) return rc;
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.out = static_cast<__nv_bfloat16*>(a->out);
+  p.q_st = a->q_stride_tok;
+  p.q_sh = a->q_stride_head;
+  p.o_st = a->o_stride_tok;
+  p.o_sh = a->o_stride_head;
+  p.q_row0 = bt.q_row0;
+  p.q_len = bt.q_len;
+  p.ctx_len = bt.ctx_len;
+  p.kv_row0 = a->kv_row0;
+  p.q_rows = a->q_rows;
+  p.kv_rows = a->kv_rows;
+  p.status = a->status;
+  CUtensorMap km, vm;
+  if (int rc = encode_packed_map(&km, a->k, a->kv_rows, s.KV, s.D, a->k_stride_tok, a->k_stride_head)) return rc;
+  if (int rc = encode_packed_map(&vm, a->v, a->kv_rows, s.KV, s.D, a->v_stride_tok, a->v_stride_head)) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return s.D == 128 ? launch_row_attention<128, kPacked>(p, km, vm, a->reuse_plan != 0, st)
+                    : launch_row_attention<64, kPacked>(p, km, vm, a->reuse_plan != 0, st);
+}
+
+extern "C" size_t specdec_shared_prefix_workspace_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                                                        int32_t head_dim, int32_t max_q_len, int32_t num_groups,
+                                                        int32_t num_members, int32_t num_sms) {
+  const RowShape s{num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_len, num_groups, num_members, row_sms(num_sms)};
+  return row_shape_ok(s) ? row_space(s).bytes : 0;
+}
+
+extern "C" int specdec_shared_prefix_attention(const SpecdecSharedPrefixArgs* a, specdec_stream_t stream) {
+  if (!a) return fail(SPECDEC_ERR_INVALID, "args is NULL");
+  const SpecdecBatch& bt = a->batch;
+  const SpecdecPagedKV& kv = a->kv;
+  const RowShape s{bt.num_seqs, bt.num_q_heads, kv.num_kv_heads, kv.head_dim, bt.max_q_len, a->num_groups,
+                   a->num_members, row_sms(a->num_sms)};
+  if (int rc = check_shape(s)) return rc;
+  if (int rc = check_rows(a->q, a->out, a->q_stride_tok, a->q_stride_head, a->o_stride_tok, a->o_stride_head)) return rc;
+  if (!bt.q_row0 || !bt.q_len || !bt.ctx_len) return fail(SPECDEC_ERR_INVALID, "batch arrays must be set");
+  if (s.G > 0 && (!a->group_start || !a->prefix_len || (s.M > 0 && !a->members)))
+    return fail(SPECDEC_ERR_INVALID, "group arrays must be set");
+  if (!kv.k_pool || !kv.v_pool || !kv.page_table) return fail(SPECDEC_ERR_INVALID, "kv pool pointers must be set");
+  if (kv.num_pages <= 0 || kv.max_pages_per_seq <= 0) return fail(SPECDEC_ERR_INVALID, "empty page pool");
+  if ((reinterpret_cast<uintptr_t>(kv.k_pool) | reinterpret_cast<uintptr_t>(kv.v_pool)) & 15u)
+    return fail(SPECDEC_ERR_INVALID, "pool pointers must be 16-byte aligned");
+  if (kv.v_dtype != SPECDEC_BF16) return fail(SPECDEC_ERR_UNSUPPORTED, "v_dtype must be SPECDEC_BF16");
+  if (a->q_rows <= 0 || a->q_rows > 0x7fffffff) return fail(SPECDEC_ERR_INVALID, "row counts out of range");
+  const int64_t page_rows = static_cast<int64_t>(kv.num_pages) * s.KV * (s.D / 64);
+  if (page_rows > 0x7fffffff || static_cast<int64_t>(kv.max_pages_per_seq) * kPage > 0x7fffffff)
+    return fail(SPECDEC_ERR_UNSUPPORTED, "page pool too large");
+  RowParams p = {};
+  if (int rc = fill_row_params(p, s, a->workspace, a->workspace_bytes, a->sm_scale)) return rc;
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.out = static_cast<__nv_bfloat16*>(a->out);
+  p.q_st = a->q_stride_tok;
+  p.q_sh = a->q_stride_head;
+  p.o_st = a->o_stride_tok;
+  p.o_sh = a->o_stride_head;
+  p.q_row0 = bt.q_row0;
+  p.q_len = bt.q_len;
+  p.ctx_len = bt.ctx_len;
+  p.group_start = a->group_start;
+  p.members = a->members;
+  p.prefix_len = a->prefix_len;
+  p.page_table = kv.page_table;
+  p.num_pages = kv.num_pages;
+  p.max_pages = kv.max_pages_per_seq;
+  p.paged = 1;
+  p.q_rows = a->q_rows;
+  p.status = a->status;
+  CUtensorMap km, vm;
+  if (int rc = encode_rows_map(&km, kv.k_pool, static_cast<uint64_t>(page_rows), 2048)) return rc;
+  if (int rc = encode_rows_map(&vm, kv.v_pool, static_cast<uint64_t>(page_rows), 2048)) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return s.D == 128 ? launch_row_attention<128, kPaged>(p, km, vm, a->reuse_plan != 0, st)
+                    : launch_row_attention<64, kPaged>(p, km, vm, a->reuse_plan != 0, st);
+}

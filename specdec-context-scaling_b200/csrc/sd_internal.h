@@ -1,6 +1,8 @@
 // sd_internal.h -- host-side helpers shared by the translation units of the library.
 #pragma once
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -19,6 +21,11 @@ int after_launch(const char* what, int n = 1);
 uint64_t wait_limit_ns();
 // SM count of the current device (cached per device).
 int device_sm_count();
+
+// cuTensorMapEncodeTiled of the driver (NULL when it is unavailable), and the 2-D map over contiguous rows whose
+// box is one row: the shape tile::gather4 loads fetch four rows of.
+PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn();
+int encode_rows_map(CUtensorMap* map, const void* base, uint64_t n_rows, uint32_t row_bytes);
 
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 

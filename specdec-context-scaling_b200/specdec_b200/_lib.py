@@ -30,6 +30,7 @@ STATUS_TRIM_RANGE = 0x8
 STATUS_TIMEOUT = 0x10
 STATUS_ACCEPT_RANGE = 0x20
 STATUS_PLAN_MISMATCH = 0x40
+STATUS_BAD_GROUP = 0x80
 
 STATUS_NAMES = {
     STATUS_BAD_LENGTH: "bad length (ctx_len < q_len or q_len > max_q_len)",
@@ -39,6 +40,7 @@ STATUS_NAMES = {
     STATUS_TIMEOUT: "bounded device wait timed out",
     STATUS_ACCEPT_RANGE: "accept row/candidate count out of range",
     STATUS_PLAN_MISMATCH: "reused plan was built for another launch shape (cluster choice or SM budget)",
+    STATUS_BAD_GROUP: "prefix group with a bad start, length or member (out of range, or listed twice)",
 }
 
 _vp = ctypes.c_void_p
@@ -151,6 +153,60 @@ class RopeAppendArgs(ctypes.Structure):
     ]
 
 
+class PromptArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp),
+        ("k", _vp),
+        ("v", _vp),
+        ("out", _vp),
+        ("q_stride_tok", _i64),
+        ("q_stride_head", _i64),
+        ("k_stride_tok", _i64),
+        ("k_stride_head", _i64),
+        ("v_stride_tok", _i64),
+        ("v_stride_head", _i64),
+        ("o_stride_tok", _i64),
+        ("o_stride_head", _i64),
+        ("batch", Batch),
+        ("kv_row0", _vp),
+        ("q_rows", _i64),
+        ("kv_rows", _i64),
+        ("num_kv_heads", _i32),
+        ("head_dim", _i32),
+        ("sm_scale", ctypes.c_float),
+        ("workspace", _vp),
+        ("workspace_bytes", _sz),
+        ("status", _vp),
+        ("reuse_plan", _i32),
+        ("num_sms", _i32),
+    ]
+
+
+class SharedPrefixArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp),
+        ("out", _vp),
+        ("q_stride_tok", _i64),
+        ("q_stride_head", _i64),
+        ("o_stride_tok", _i64),
+        ("o_stride_head", _i64),
+        ("batch", Batch),
+        ("kv", PagedKV),
+        ("group_start", _vp),
+        ("members", _vp),
+        ("prefix_len", _vp),
+        ("num_groups", _i32),
+        ("num_members", _i32),
+        ("q_rows", _i64),
+        ("sm_scale", ctypes.c_float),
+        ("workspace", _vp),
+        ("workspace_bytes", _sz),
+        ("status", _vp),
+        ("reuse_plan", _i32),
+        ("num_sms", _i32),
+    ]
+
+
 class AcceptArgs(ctypes.Structure):
     _fields_ = [
         ("logits", _vp),
@@ -206,6 +262,10 @@ SIGNATURES = {
     "specdec_lmhead_workspace_bytes": (_sz, [_i32]),
     "specdec_attention_fp8v": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _sz,
                                               _vp]),
+    "specdec_prompt_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "specdec_prompt_attention": (ctypes.c_int, [ctypes.POINTER(PromptArgs), _vp]),
+    "specdec_shared_prefix_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "specdec_shared_prefix_attention": (ctypes.c_int, [ctypes.POINTER(SharedPrefixArgs), _vp]),
     "specdec_lmhead_argmax": (ctypes.c_int, [_vp, _vp]),
     "specdec_quantize_int8": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _vp]),
     "specdec_rmsnorm_int8": (

@@ -77,6 +77,7 @@ class PagedKVCache:
     lengths: torch.Tensor  # int32 [num_seqs]
     host_lengths: list[int] | None = field(default_factory=list)
     fmt: str = "fp16"
+    page_refs: torch.Tensor | None = None  # int32 [num_pages] sequences that hold a page; None: static pages
 
     @classmethod
     def allocate(
@@ -137,6 +138,48 @@ class PagedKVCache:
             fmt="v_fp8" if v_dtype == "e4m3" else "fp16",
         )
 
+    @classmethod
+    def from_pools(cls, k_pools, v_pools, v_scales, page_table: torch.Tensor, lengths: torch.Tensor, head_dim: int, *,
+                   page_refs: torch.Tensor | None = None) -> "PagedKVCache":
+        """A cache over existing pools: one K and one V pool a layer in the layout above (bf16, or uint8 V with its
+        f32 scales), an int32 page table (num_seqs, max_pages) and int32 lengths (num_seqs,)."""
+        if not k_pools or len(k_pools) != len(v_pools) or (v_scales is not None and len(v_scales) != len(k_pools)):
+            raise ValueError("one K and one V pool (and scale pool) a layer")
+        if head_dim not in (64, 128):
+            raise ValueError("head_dim must be 64 or 128")
+        pages, kv = k_pools[0].shape[:2]
+        shape, like = (pages, kv, PAGE * head_dim), k_pools[0]
+        v_type = torch.bfloat16 if v_scales is None else torch.uint8
+        for group, dtype, want in ((k_pools, torch.bfloat16, shape), (v_pools, v_type, shape),
+                                   (v_scales or (), torch.float32, (pages, kv, PAGE))):
+            for t in group:
+                if t.dtype != dtype or tuple(t.shape) != want or not t.is_contiguous() or t.device != like.device:
+                    raise ValueError(f"pools must be contiguous {dtype} {want} on one device")
+        if v_scales is not None and head_dim != 128:
+            raise ValueError("E4M3 V needs head_dim 128 (one scale group per head, GROUP_V = 128)")
+        n = page_table.shape[0]
+        for t, want, what in ((page_table, (n, page_table.shape[1]), "page_table"), (lengths, (n,), "lengths"),
+                              (page_refs, (pages,), "page_refs")):
+            if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != want or not t.is_contiguous()
+                                  or t.device != like.device):
+                raise ValueError(f"{what} must be contiguous int32 {want} on the pools' device")
+        scales = v_scales if v_scales is not None else [None] * len(k_pools)
+        return cls(
+            num_layers=len(k_pools),
+            num_seqs=n,
+            num_kv_heads=int(kv),
+            head_dim=head_dim,
+            capacity=int(page_table.shape[1]) * PAGE,
+            v_dtype="bf16" if v_scales is None else "e4m3",
+            device=like.device,
+            pools=[LayerPool(k, v, s) for k, v, s in zip(k_pools, v_pools, scales)],
+            page_table=page_table,
+            lengths=lengths,
+            host_lengths=None,
+            fmt="fp16" if v_scales is None else "v_fp8",
+            page_refs=page_refs,
+        )
+
     # ------------------------------------------------------------------ views
     @property
     def num_pages(self) -> int:
@@ -161,6 +204,7 @@ class PagedKVCache:
             lengths=lengths,
             host_lengths=None if host_lengths is None else list(host_lengths),
             fmt=self.fmt,
+            page_refs=self.page_refs,
         )
 
     def set_host_lengths(self, lens: list[int]) -> None:

@@ -553,6 +553,198 @@ def trim_lengths(cur_len, new_len, out=None, status=None):
     return out
 
 
+# ---------------------------------------------------------------------------- prompts and shared prefixes
+def _call(t: torch.Tensor):
+    """(library, device index, its current stream) for a call on ``t``, whose device has to be the current one."""
+    return _int8_call(t)
+
+
+def _head_rows(t: torch.Tensor, what: str, D: int | None = None):
+    """(rows, heads, head_dim) of packed bf16 rows with contiguous 16-byte aligned heads."""
+    if t.dtype is not torch.bfloat16 or t.dim() != 3:
+        raise ValueError(f"{what} must be bf16 (rows, heads, head_dim)")
+    rows, heads, dim = t.shape
+    if D is not None and dim != D:
+        raise ValueError(f"{what} must share q's head_dim")
+    st, sh, sd = t.stride()
+    if sd != 1 or st % 8 or sh % 8 or st < 0 or sh < 0 or t.data_ptr() & 15:
+        raise ValueError(f"{what} heads must be contiguous and start on 16-byte boundaries")
+    return rows, heads, dim
+
+
+def _batch_struct(batch: "RaggedBatch", heads: int, dev: int):
+    """The C batch after a check of its arrays; rows that a call would read on the host stay unchecked."""
+    n = batch.num_seqs
+    for name in ("q_row0", "q_len", "ctx_len"):
+        _check_i32(getattr(batch, name), dev, n, name)
+    return _lib.Batch(q_row0=batch.q_row0.data_ptr(), q_len=batch.q_len.data_ptr(), ctx_len=batch.ctx_len.data_ptr(),
+                      num_seqs=n, num_q_heads=heads, max_q_len=batch.max_q_len, max_ctx_len=batch.max_ctx_len)
+
+
+def _check_i32(t, dev: int, n: int, what: str) -> None:
+    if t.get_device() != dev:
+        raise RuntimeError("tensors must be CUDA, all on one device")
+    if t.dtype is not torch.int32 or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous int32 ({n},)")
+
+
+def _row_out(q, out, dev: int):
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _on_device(dev, out)
+    if out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    _head_rows(out, "out")
+    return out
+
+
+def _check_status(status, dev: int) -> None:
+    if status is not None:
+        _on_device(dev, status)
+        if status.dtype is not torch.int32 or status.numel() < 1:
+            raise ValueError("status must be int32")
+
+
+def _row_workspace(workspace, nbytes: int, like, dev: int, reuse_plan: bool):
+    if nbytes == 0:
+        raise ValueError("invalid batch geometry")
+    if workspace is None:
+        if reuse_plan:
+            raise ValueError("reuse_plan needs the workspace that holds the plan")
+        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    _on_device(dev, workspace)
+    if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous uint8")
+    return workspace
+
+
+def prompt_workspace(batch: RaggedBatch, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                     device="cuda") -> torch.Tensor:
+    """Workspace of ``prompt_attention`` for a batch of this shape (any contents)."""
+    n = _lib_handle().specdec_prompt_workspace_bytes(batch.num_seqs, num_q_heads, num_kv_heads, head_dim,
+                                                     batch.max_q_len, 0)
+    if n == 0:
+        raise ValueError("invalid batch geometry")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def prompt_attention(q, k, v, batch: RaggedBatch, *, kv_row0=None, out=None, workspace=None, sm_scale=None,
+                     status=None, reuse_plan: bool = False):
+    """Causal attention of packed prompts: q (rows, H, D), k and v (key rows, KV, D) bf16, D 64 or 128.
+
+    Row i of sequence b is packed row ``q_row0[b] + i`` and sees keys j <= i + ctx_len[b] - q_len[b], key j being row
+    ``kv_row0[b] + j`` of k and v (``kv_row0``: int32 (num_seqs,); None where the prompts are whole, so that their
+    keys lie where their queries do).  What other sequences, later tokens or rows behind the last one hold reaches no
+    output.  Rows that belong to no sequence are left as they were.
+    ``reuse_plan``: ``workspace`` holds the plan of an earlier call with the same batch (the layers of one pass)."""
+    lib, dev, stream = _call(q)
+    rows, H, D = _head_rows(q, "q")
+    kv_rows, KV, _ = _head_rows(k, "k", D)
+    if v.shape != k.shape:
+        raise ValueError("k and v must have one shape")
+    _head_rows(v, "v", D)
+    _on_device(dev, k, v)
+    out = _row_out(q, out, dev)
+    if kv_row0 is None:
+        kv_row0 = batch.q_row0
+    b = _batch_struct(batch, H, dev)
+    _check_i32(kv_row0, dev, batch.num_seqs, "kv_row0")
+    _check_status(status, dev)
+    if rows == 0 or batch.num_seqs == 0:
+        return out
+    nbytes = lib.specdec_prompt_workspace_bytes(batch.num_seqs, H, KV, D, batch.max_q_len, 0)
+    workspace = _row_workspace(workspace, nbytes, q, dev, reuse_plan)
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    args = _lib.PromptArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0],
+        os[1], b, kv_row0.data_ptr(), rows, kv_rows, KV, D,
+        1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), workspace.data_ptr(), workspace.numel(),
+        _ptr(status), 1 if reuse_plan else 0, 0)
+    rc = lib.specdec_prompt_attention(ctypes.byref(args), stream)
+    if rc:
+        _lib.check(rc, "prompt_attention")
+    return out
+
+
+@dataclass
+class SharedPrefix:
+    """Groups of sequences whose first pages are the same.
+
+    Group g is the sequences ``members[group_start[g] : group_start[g + 1]]``, which share their first
+    ``prefix_len[g]`` tokens (their page tables begin with the same page ids).  A sequence is in one group at most."""
+
+    group_start: torch.Tensor  # int32 (num_groups + 1,)
+    members: torch.Tensor  # int32 (num_members,)
+    prefix_len: torch.Tensor  # int32 (num_groups,)
+    num_groups: int
+    num_members: int
+
+    @classmethod
+    def from_groups(cls, groups, device="cuda") -> "SharedPrefix":
+        """``groups``: (member sequences, shared tokens) of every group."""
+        start, members, lens = [0], [], []
+        for seqs, n in groups:
+            members += [int(b) for b in seqs]
+            start.append(len(members))
+            lens.append(int(n))
+            if int(n) < 0:
+                raise ValueError("a shared prefix has 0 or more tokens")
+        if len(set(members)) != len(members) or any(b < 0 for b in members):
+            raise ValueError("a sequence is in one group at most")
+        t = torch.tensor(start + members + lens, dtype=torch.int32).to(device)
+        a, b = len(start), len(start) + len(members)
+        return cls(t[:a], t[a:b], t[b:], len(lens), len(members))
+
+
+def shared_prefix_workspace(batch: RaggedBatch, prefix: SharedPrefix, num_q_heads: int,
+                            cache: PagedKVCache) -> torch.Tensor:
+    """Workspace of ``shared_prefix_attention`` for a batch of this shape (any contents)."""
+    n = _lib_handle().specdec_shared_prefix_workspace_bytes(batch.num_seqs, num_q_heads, cache.num_kv_heads,
+                                                            cache.head_dim, batch.max_q_len, prefix.num_groups,
+                                                            prefix.num_members, 0)
+    if n == 0:
+        raise ValueError("invalid batch geometry")
+    return torch.empty(n, dtype=torch.uint8, device=cache.device)
+
+
+def shared_prefix_attention(q, cache: PagedKVCache, layer: int, batch: RaggedBatch, prefix: SharedPrefix, *, out=None,
+                            workspace=None, sm_scale=None, status=None, reuse_plan: bool = False):
+    """``paged_attention`` for a batch in which groups of sequences share their first pages: the same rows, mask and
+    answer, the pages of a group's prefix read once for all of its members.
+
+    Of ``prefix_len`` the whole pages that every row of the group sees are shared; they are read from the table of the
+    group's first member that has rows.  ``reuse_plan``: ``workspace`` holds the plan of an earlier call with the same
+    batch and prefix (the layers of one step)."""
+    lib, dev, stream = _call(q)
+    rows, H, D = _head_rows(q, "q")
+    if D != cache.head_dim:
+        raise ValueError("q head_dim differs from the cache")
+    out = _row_out(q, out, dev)
+    _on_device(dev, cache.page_table)
+    b = _batch_struct(batch, H, dev)
+    if batch.num_seqs > cache.num_seqs:
+        raise ValueError("the batch has more sequences than the cache")
+    _check_i32(prefix.group_start, dev, prefix.num_groups + 1, "group_start")
+    _check_i32(prefix.members, dev, prefix.num_members, "members")
+    _check_i32(prefix.prefix_len, dev, prefix.num_groups, "prefix_len")
+    _check_status(status, dev)
+    if rows == 0 or batch.num_seqs == 0:
+        return out
+    nbytes = lib.specdec_shared_prefix_workspace_bytes(batch.num_seqs, H, cache.num_kv_heads, D, batch.max_q_len,
+                                                       prefix.num_groups, prefix.num_members, 0)
+    workspace = _row_workspace(workspace, nbytes, q, dev, reuse_plan)
+    qs, os = q.stride(), out.stride()
+    args = _lib.SharedPrefixArgs(
+        q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], b, _paged_kv(cache, layer),
+        prefix.group_start.data_ptr(), prefix.members.data_ptr(), prefix.prefix_len.data_ptr(), prefix.num_groups,
+        prefix.num_members, rows, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), workspace.data_ptr(),
+        workspace.numel(), _ptr(status), 1 if reuse_plan else 0, 0)
+    rc = lib.specdec_shared_prefix_attention(ctypes.byref(args), stream)
+    if rc:
+        _lib.check(rc, "shared_prefix_attention")
+    return out
+
+
 # ---------------------------------------------------------------------------- 8-bit linear path
 # These calls take a few microseconds of GPU time each in a decode step, so their checks read every
 # attribute once and the library and stream are looked up directly.
