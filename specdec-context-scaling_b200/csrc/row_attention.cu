@@ -22,6 +22,8 @@
 //   warp 10         query rows of the next item into shared memory, and each row's key limit
 //   warp 11         zeroes the V rows past an item's last key, so that a masked key's zero probability
 //                   never meets what lies behind a sequence (its next one, a page's old contents; NaN x 0)
+//   warps 12-15     (E4M3 V only) widen a block's codes, times their token's scale, to the bf16 block that the
+//                   MMAs read (the values that dequantising the cache gives), zeroes past the last key
 // Per block j and tile t:  S_t = Q_t K_j^T (TMEM, fp32) -> P_t = exp2(S_t - m) as bf16 over the same columns
 // -> O_t += P_t V_j (A operand from TMEM).  The two tiles alternate, so one's softmax runs under the other's MMAs.
 // The running maximum moves only when a row's grows by more than 2^8 (then O is rescaled in place); S_t(j) is complete
@@ -36,13 +38,21 @@ namespace sd {
 constexpr int kRowTile = 128;      // rows of a tile: TMEM lanes
 constexpr int kUnitRows = 256;     // two tiles
 constexpr int kKeyBlock = 128;     // keys of a block
-constexpr int kRowThreads = 384;
 constexpr int kUnitCost = 2;       // what a unit costs beside its blocks (query load, epilogue), in blocks
 constexpr int kMinQuota = 4;       // smallest range of a CTA, in blocks
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
 constexpr float kRowRescaleLog2 = 8.f;
 
-enum RowSource { kPacked = 0, kPaged = 1 };
+enum RowSource { kPacked = 0, kPaged = 1, kPagedE4M3 = 2 };
+// Threads, and registers a thread of the softmax warps and of the others: the launch's own are what
+// __launch_bounds__ leaves (168, 128), and the shares add up to them.
+template <int SRC>
+struct RowRoles {
+  static constexpr bool V8 = SRC == kPagedE4M3;
+  static constexpr int THREADS = V8 ? 512 : 384;
+  static constexpr int SOFTMAX_REGS = V8 ? 176 : 200, OTHER_REGS = V8 ? 80 : 104;
+  static_assert(256 * SOFTMAX_REGS + (THREADS - 256) * OTHER_REGS <= THREADS * (V8 ? 128 : 168), "register shares");
+};
 
 struct alignas(16) RowItem {
   int32_t src;     // sequence, or ~group
@@ -66,6 +76,7 @@ struct RowParams {
   const int32_t *q_row0, *q_len, *ctx_len, *kv_row0;
   const int32_t *group_start, *members, *prefix_len;
   const int32_t* page_table;
+  const float* v_scale;
   int64_t q_rows, kv_rows;
   int32_t B, H, KV, n_rep, tpt, q_max, G, M;
   int32_t num_pages, max_pages, paged;
@@ -326,13 +337,16 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
 }
 
 // ---------------------------------------------------------------- geometry
-template <int D>
+template <int D, bool V8>
 struct RowGeom {
+  static_assert(!V8 || D == 128, "E4M3 V needs head_dim 128");
   static constexpr int KH = D / 64;               // 128-byte dim halves
   static constexpr int TILE = 16384 * KH;         // one K or V block, one query tile
-  static constexpr int NS = D == 128 ? 5 : 12;    // ring slots (a K or a V block each)
+  // ring slots (a K or a V block each; E4M3: an even number, so that a slot is always one or the other's)
+  static constexpr int NS = V8 ? 4 : D == 128 ? 5 : 12;
   static constexpr int RING = 2 * TILE;           // the ring lies behind the two query tiles
-  static constexpr int SMEM = RING + NS * TILE + 1024;
+  static constexpr int RAW = RING + NS * TILE;    // E4M3: two blocks of codes
+  static constexpr int SMEM = RAW + (V8 ? 2 * 16384 : 0) + 1024;
   static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
   static_assert(SMEM <= 227 * 1024 - 2048, "shared memory budget, 2 KB of static variables aside");
 };
@@ -376,28 +390,36 @@ SD_DEV void tma_rows4(void* dst, const CUtensorMap* map, int32_t r0, int32_t r1,
 }
 
 // ---------------------------------------------------------------- main kernel
+template <int N>
+SD_DEV void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+SD_DEV void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 template <int D, int SRC>
-__global__ void __launch_bounds__(kRowThreads, 1) row_attention_kernel(const RowParams p,
+__global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kernel(const RowParams p,
                                                                        const __grid_constant__ CUtensorMap kmap,
                                                                        const __grid_constant__ CUtensorMap vmap) {
-  using Geo = RowGeom<D>;
+  constexpr bool V8 = RowRoles<SRC>::V8;
+  using Geo = RowGeom<D, V8>;
   constexpr int NS = Geo::NS, KH = Geo::KH;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[NS], empty[NS];
+  __shared__ uint64_t full[NS], empty[NS], raw_full[2], raw_empty[2];
   __shared__ uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], c_req, v_clean, fin;
   __shared__ int32_t s_limit[kUnitRows];
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], V8 && (s & 1) ? 4 : 1);  // a TMA block, or the four widening warps
       mbar_init(&empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
+      mbar_init(&raw_full[t], 1);
+      mbar_init(&raw_empty[t], 4);
     }
     mbar_init(&q_full, 1);
     mbar_init(&q_empty, 1 + 8);
@@ -421,228 +443,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_attention_kernel(const Row
   umma::fence_after_sync();
   const uint32_t tmem = s_tmem;
   const int i0 = p.cta_first[blockIdx.x], i1 = p.cta_last[blockIdx.x];
-
-  if (warp == 8) {
-    // ------------------------------------------------------------ K/V blocks
-    uint32_t n = 0;  // blocks issued (K and V each count)
-    bool ok = true;
-    for (int i = i0; i <= i1 && ok; ++i) {
-      const RowItem it = load_item(p.items + i);
-      if (it.nblk == 0) continue;
-      const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
-      int ids = 0;  // paged: lane l holds the page of keys 16 (32 (j / 4) + l) ..
-      for (int j = 0; j < nb && ok; ++j) {
-        if (SRC == kPaged && (j & 3) == 0) {
-          const int last = (it.k1 - 1) / kPage;
-          const int pg = min(it.k0 / kPage + 8 * j + lane, last);
-          ids = p.page_table[static_cast<int64_t>(it.kv) * p.max_pages + pg];
-          if (ids < 0 || ids >= p.num_pages) {
-            raise_status(p.status, SPECDEC_STATUS_BAD_PAGE);
-            ids = 0;
-          }
-        }
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++n) {
-          const uint32_t s = n % NS, round = n / NS;
-          if (round > 0 && !warp_wait(&empty[s], (round - 1) & 1)) {
-            ok = false;
-            break;
-          }
-          uint8_t* dst = smem + Geo::RING + s * Geo::TILE;
-          const CUtensorMap* map = kv ? &vmap : &kmap;
-          if (SRC == kPacked) {
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&full[s], Geo::TILE);
-#pragma unroll
-              for (int x = 0; x < KH; ++x)
-                tma_tile_3d(dst + x * 16384, map, x * 64, it.head, it.kv + it.k0 + j * kKeyBlock, &full[s]);
-            }
-          } else {
-            int pg[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) pg[e] = __shfl_sync(0xffffffffu, ids, 8 * (j & 3) + e);
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&full[s], Geo::TILE);
-#pragma unroll
-              for (int x = 0; x < KH; ++x)
-#pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                  auto row = [&](int k) { return (pg[k] * p.KV + it.head) * KH + x; };
-                  tma_rows4(dst + x * 16384 + e * 2048, map, row(e), row(e + 1), row(e + 2), row(e + 3), &full[s]);
-                }
-            }
-          }
-          __syncwarp();
-        }
-      }
-    }
-    if (!ok) {
-      if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-      // copies under way land before the CTA leaves
-      for (uint32_t k = n > NS ? n - NS : 0; k < n; ++k) (void)warp_wait(&full[k % NS], (k / NS) & 1);
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issue
-    if (lane == 0) {
-      constexpr uint32_t id_qk = umma::idesc_f16(128, kKeyBlock, true, true, false, false);
-      constexpr uint32_t id_pv = umma::idesc_f16(128, D, true, true, false, true);
-      const uint32_t q_base = smem_u32(smem), ring = smem_u32(smem + Geo::RING);
-      uint32_t n = 0, pn[2] = {0, 0}, items = 0, cleaned = 0;
-      bool ok = true;
-      auto slot_ready = [&](uint32_t k) { return mbar_wait(&full[k % NS], (k / NS) & 1); };
-      auto qk = [&](int t, uint32_t k) {
-        const uint32_t qa = q_base + t * Geo::TILE, ka = ring + (k % NS) * Geo::TILE;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t at = (kk >> 2) * 16384 + (kk & 3) * 32;
-          umma::mma_f16_ss(umma::taddr(tmem, 0, Geo::S_COL + t * 128), umma::desc_kmajor_sw128(qa + at),
-                           umma::desc_kmajor_sw128(ka + at), id_qk, kk > 0);
-        }
-        umma::commit(&s_full[t]);
-      };
-      for (int i = i0; i <= i1 && ok; ++i) {
-        const RowItem it = load_item(p.items + i);
-        if (it.nblk == 0) continue;
-        const int nt[2] = {tile_blocks(p, it, 0), tile_blocks(p, it, 1)};
-        const int nb = max(nt[0], nt[1]);
-        const bool clean = (it.k1 - it.k0) % kKeyBlock != 0;
-        ok = mbar_wait(&q_full, items & 1) && slot_ready(n);
-        if (!ok) break;
-        umma::fence_after_sync();
-        if (nt[0] > 0) qk(0, n);
-        if (nt[1] > 0) qk(1, n);
-        if (nb == 1) umma::commit(&q_empty);
-        umma::commit(&empty[n % NS]);
-        for (int j = 0; j < nb && ok; ++j) {
-          const uint32_t kv = n + 2 * j + 1, kn = kv + 1;  // this block's V, the next block's K
-          bool v_in = false, k_in = false;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (j >= nt[t]) continue;
-            if (!v_in) {
-              ok = ok && slot_ready(kv);
-              // the last block's V is zeroed past the last key while the softmax works on the block
-              if (ok && clean && j == nb - 1) mbar_arrive(&c_req);
-            }
-            ok = ok && mbar_wait(&p_full[t], pn[t] & 1);
-            if (!v_in && clean && j == nb - 1) ok = ok && mbar_wait(&v_clean, cleaned++ & 1);
-            v_in = true;
-            if (!ok) break;
-            ++pn[t];
-            umma::fence_after_sync();
-            const uint32_t va = ring + (kv % NS) * Geo::TILE;
-#pragma unroll
-            for (int kk = 0; kk < kKeyBlock / 16; ++kk)
-              umma::mma_f16_ts(umma::taddr(tmem, 0, Geo::O_COL + t * D),
-                               umma::taddr(tmem, 0, Geo::S_COL + t * 128 + kk * 8),
-                               umma::desc_mnmajor_sw128(va + kk * 2048, 16384), id_pv, j > 0 || kk > 0);
-            if (j == nt[t] - 1) {
-              umma::commit(&o_full[t]);
-            } else {
-              if (!k_in) {
-                ok = slot_ready(kn);
-                k_in = true;
-                if (!ok) break;
-                umma::fence_after_sync();
-              }
-              qk(t, kn);
-            }
-          }
-          if (!ok) break;
-          umma::commit(&empty[kv % NS]);
-          if (j + 1 < nb) {
-            umma::commit(&empty[kn % NS]);
-            if (j + 2 == nb) umma::commit(&q_empty);
-          }
-        }
-        n += 2 * nb;
-        ++items;
-      }
-      if (!ok) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-      umma::commit(&fin);
-      (void)mbar_wait(&fin, 0);
-    }
-    __syncwarp();
-  } else if (warp == 10) {
-    // ------------------------------------------------------------ query rows and limits
-    constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte chunks of a row, rows a step
-    const uint32_t q_base = smem_u32(smem);
-    uint32_t items = 0;
-    for (int i = i0; i <= i1; ++i) {
-      const RowItem it = load_item(p.items + i);
-      if (it.nblk == 0) continue;
-      const int tiles = it.vt0 + p.tpt < it.n_vt ? 2 : 1;
-      if (items > 0 && !warp_wait(&q_empty, (items - 1) & 1)) {
-        if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-        break;
-      }
-      for (int base = 0; base < tiles * kRowTile; base += 32) {
-        const int t = base / kRowTile, r = base % kRowTile + lane;
-        const int tok = r / p.n_rep, vt = it.vt0 + t * p.tpt + tok;
-        int64_t off = -1;
-        int limit = 0;
-        if (tok < p.tpt && vt < it.n_vt) {
-          int row = -1;
-          if (it.src >= 0) {
-            row = it.row0 + vt;
-            limit = min(it.first + vt + 1, it.k1);
-          } else {
-            const int m = vt / p.q_max, e = vt - m * p.q_max;
-            const int2 mr = p.member_row[it.member0 + m];
-            if (e < mr.y) {
-              row = mr.x + e;
-              limit = it.k1;
-            }
-          }
-          if (row >= 0)
-            off = static_cast<int64_t>(row) * p.q_st +
-                  static_cast<int64_t>(it.head * p.n_rep + r - tok * p.n_rep) * p.q_sh;
-        }
-        s_limit[base + lane] = limit;
-#pragma unroll 4
-        for (int e = 0; e < 32; e += RP) {
-          const int64_t o = __shfl_sync(0xffffffffu, off, e + lane / CH);
-          const int rr = base % kRowTile + e + lane / CH, ch = lane % CH;
-          const uint32_t dst =
-              q_base + t * Geo::TILE + (ch >> 3) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
-          cp_async16(dst, p.q + (o < 0 ? 0 : o + ch * 8), o < 0 ? 0u : 16u);
-        }
-      }
-      cp_async_wait_all();
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full);
-      ++items;
-    }
-    cp_async_wait_all();
-  } else if (warp == 11) {
-    // ------------------------------------------------------------ V rows past the last key
-    uint32_t n = 0, cleaned = 0;
-    for (int i = i0; i <= i1; ++i) {
-      const RowItem it = load_item(p.items + i);
-      if (it.nblk == 0) continue;
-      const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
-      const int rem = (it.k1 - it.k0) % kKeyBlock;
-      if (rem != 0) {
-        const uint32_t k = n + 2 * nb - 1;
-        // asked for by the MMA warp, which has seen the block arrive and waits for the answer
-        if (!warp_wait(&c_req, cleaned & 1)) {
-          if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-          break;
-        }
-        uint8_t* v = smem + Geo::RING + (k % NS) * Geo::TILE;
-#pragma unroll
-        for (int x = 0; x < KH; ++x)
-          for (int o = rem * 128 + lane * 16; o < 16384; o += 512)
-            *reinterpret_cast<uint4*>(v + x * 16384 + o) = make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_clean);
-        ++cleaned;
-      }
-      n += 2 * nb;
-    }
-  } else {
+  if (warp < 8) {
+    more_regs<RowRoles<SRC>::SOFTMAX_REGS>();
     // ------------------------------------------------------------ softmax and epilogue: a thread a row
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 5;
@@ -778,6 +580,305 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_attention_kernel(const Row
       }
     }
     if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+  } else {
+  fewer_regs<RowRoles<SRC>::OTHER_REGS>();
+  if (warp == 8) {
+    // ------------------------------------------------------------ K/V blocks
+    uint32_t n = 0;  // blocks issued (K and V each count)
+    bool ok = true;
+    for (int i = i0; i <= i1 && ok; ++i) {
+      const RowItem it = load_item(p.items + i);
+      if (it.nblk == 0) continue;
+      const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+      int ids = 0;  // paged: lane l holds the page of keys 16 (32 (j / 4) + l) ..
+      for (int j = 0; j < nb && ok; ++j) {
+        if (SRC != kPacked && (j & 3) == 0) {
+          const int last = (it.k1 - 1) / kPage;
+          const int pg = min(it.k0 / kPage + 8 * j + lane, last);
+          ids = p.page_table[static_cast<int64_t>(it.kv) * p.max_pages + pg];
+          if (ids < 0 || ids >= p.num_pages) {
+            raise_status(p.status, SPECDEC_STATUS_BAD_PAGE);
+            ids = 0;
+          }
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const uint32_t s = n % NS, round = n / NS;
+          if (V8 && kv) {  // codes; the widening warps take care of the block's ring slot
+            const uint32_t b = (n >> 1) & 1, r = n >> 2;
+            if (r > 0 && !warp_wait(&raw_empty[b], (r - 1) & 1)) {
+              ok = false;
+              break;
+            }
+            int pg[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pg[e] = __shfl_sync(0xffffffffu, ids, 8 * (j & 3) + e) * p.KV + it.head;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&raw_full[b], 16384);
+#pragma unroll
+              for (int e = 0; e < 8; e += 4)
+                tma_rows4(smem + Geo::RAW + b * 16384 + e * 2048, &vmap, pg[e], pg[e + 1], pg[e + 2], pg[e + 3],
+                          &raw_full[b]);
+            }
+            __syncwarp();
+            continue;
+          }
+          if (round > 0 && !warp_wait(&empty[s], (round - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = smem + Geo::RING + s * Geo::TILE;
+          const CUtensorMap* map = kv ? &vmap : &kmap;
+          if (SRC == kPacked) {
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&full[s], Geo::TILE);
+#pragma unroll
+              for (int x = 0; x < KH; ++x)
+                tma_tile_3d(dst + x * 16384, map, x * 64, it.head, it.kv + it.k0 + j * kKeyBlock, &full[s]);
+            }
+          } else {
+            int pg[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pg[e] = __shfl_sync(0xffffffffu, ids, 8 * (j & 3) + e);
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&full[s], Geo::TILE);
+#pragma unroll
+              for (int x = 0; x < KH; ++x)
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                  auto row = [&](int k) { return (pg[k] * p.KV + it.head) * KH + x; };
+                  tma_rows4(dst + x * 16384 + e * 2048, map, row(e), row(e + 1), row(e + 2), row(e + 3), &full[s]);
+                }
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (!ok) {
+      if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      // copies under way land before the CTA leaves
+      for (uint32_t k = n > NS ? n - NS : 0; k < n; ++k)
+        (void)(V8 && (k & 1) ? warp_wait(&raw_full[(k >> 1) & 1], (k >> 2) & 1) : warp_wait(&full[k % NS], (k / NS) & 1));
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issue
+    if (lane == 0) {
+      constexpr uint32_t id_qk = umma::idesc_f16(128, kKeyBlock, true, true, false, false);
+      constexpr uint32_t id_pv = umma::idesc_f16(128, D, true, true, false, true);
+      const uint32_t q_base = smem_u32(smem), ring = smem_u32(smem + Geo::RING);
+      uint32_t n = 0, pn[2] = {0, 0}, items = 0, cleaned = 0;
+      bool ok = true;
+      auto slot_ready = [&](uint32_t k) { return mbar_wait(&full[k % NS], (k / NS) & 1); };
+      auto qk = [&](int t, uint32_t k) {
+        const uint32_t qa = q_base + t * Geo::TILE, ka = ring + (k % NS) * Geo::TILE;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t at = (kk >> 2) * 16384 + (kk & 3) * 32;
+          umma::mma_f16_ss(umma::taddr(tmem, 0, Geo::S_COL + t * 128), umma::desc_kmajor_sw128(qa + at),
+                           umma::desc_kmajor_sw128(ka + at), id_qk, kk > 0);
+        }
+        umma::commit(&s_full[t]);
+      };
+      for (int i = i0; i <= i1 && ok; ++i) {
+        const RowItem it = load_item(p.items + i);
+        if (it.nblk == 0) continue;
+        const int nt[2] = {tile_blocks(p, it, 0), tile_blocks(p, it, 1)};
+        const int nb = max(nt[0], nt[1]);
+        const bool clean = !V8 && (it.k1 - it.k0) % kKeyBlock != 0;
+        ok = mbar_wait(&q_full, items & 1) && slot_ready(n);
+        if (!ok) break;
+        umma::fence_after_sync();
+        if (nt[0] > 0) qk(0, n);
+        if (nt[1] > 0) qk(1, n);
+        if (nb == 1) umma::commit(&q_empty);
+        umma::commit(&empty[n % NS]);
+        for (int j = 0; j < nb && ok; ++j) {
+          const uint32_t kv = n + 2 * j + 1, kn = kv + 1;  // this block's V, the next block's K
+          bool v_in = false, k_in = false;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= nt[t]) continue;
+            if (!v_in) {
+              ok = ok && slot_ready(kv);
+              // the last block's V is zeroed past the last key while the softmax works on the block
+              if (ok && clean && j == nb - 1) mbar_arrive(&c_req);
+            }
+            ok = ok && mbar_wait(&p_full[t], pn[t] & 1);
+            if (!v_in && clean && j == nb - 1) ok = ok && mbar_wait(&v_clean, cleaned++ & 1);
+            v_in = true;
+            if (!ok) break;
+            ++pn[t];
+            umma::fence_after_sync();
+            const uint32_t va = ring + (kv % NS) * Geo::TILE;
+#pragma unroll
+            for (int kk = 0; kk < kKeyBlock / 16; ++kk)
+              umma::mma_f16_ts(umma::taddr(tmem, 0, Geo::O_COL + t * D),
+                               umma::taddr(tmem, 0, Geo::S_COL + t * 128 + kk * 8),
+                               umma::desc_mnmajor_sw128(va + kk * 2048, 16384), id_pv, j > 0 || kk > 0);
+            if (j == nt[t] - 1) {
+              umma::commit(&o_full[t]);
+            } else {
+              if (!k_in) {
+                ok = slot_ready(kn);
+                k_in = true;
+                if (!ok) break;
+                umma::fence_after_sync();
+              }
+              qk(t, kn);
+            }
+          }
+          if (!ok) break;
+          umma::commit(&empty[kv % NS]);
+          if (j + 1 < nb) {
+            umma::commit(&empty[kn % NS]);
+            if (j + 2 == nb) umma::commit(&q_empty);
+          }
+        }
+        n += 2 * nb;
+        ++items;
+      }
+      if (!ok) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      umma::commit(&fin);
+      (void)mbar_wait(&fin, 0);
+    }
+    __syncwarp();
+  } else if (warp == 10) {
+    // ------------------------------------------------------------ query rows and limits
+    constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte chunks of a row, rows a step
+    const uint32_t q_base = smem_u32(smem);
+    uint32_t items = 0;
+    for (int i = i0; i <= i1; ++i) {
+      const RowItem it = load_item(p.items + i);
+      if (it.nblk == 0) continue;
+      const int tiles = it.vt0 + p.tpt < it.n_vt ? 2 : 1;
+      if (items > 0 && !warp_wait(&q_empty, (items - 1) & 1)) {
+        if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+        break;
+      }
+      for (int base = 0; base < tiles * kRowTile; base += 32) {
+        const int t = base / kRowTile, r = base % kRowTile + lane;
+        const int tok = r / p.n_rep, vt = it.vt0 + t * p.tpt + tok;
+        int64_t off = -1;
+        int limit = 0;
+        if (tok < p.tpt && vt < it.n_vt) {
+          int row = -1;
+          if (it.src >= 0) {
+            row = it.row0 + vt;
+            limit = min(it.first + vt + 1, it.k1);
+          } else {
+            const int m = vt / p.q_max, e = vt - m * p.q_max;
+            const int2 mr = p.member_row[it.member0 + m];
+            if (e < mr.y) {
+              row = mr.x + e;
+              limit = it.k1;
+            }
+          }
+          if (row >= 0)
+            off = static_cast<int64_t>(row) * p.q_st +
+                  static_cast<int64_t>(it.head * p.n_rep + r - tok * p.n_rep) * p.q_sh;
+        }
+        s_limit[base + lane] = limit;
+#pragma unroll 4
+        for (int e = 0; e < 32; e += RP) {
+          const int64_t o = __shfl_sync(0xffffffffu, off, e + lane / CH);
+          const int rr = base % kRowTile + e + lane / CH, ch = lane % CH;
+          const uint32_t dst =
+              q_base + t * Geo::TILE + (ch >> 3) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
+          cp_async16(dst, p.q + (o < 0 ? 0 : o + ch * 8), o < 0 ? 0u : 16u);
+        }
+      }
+      cp_async_wait_all();
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+      ++items;
+    }
+    cp_async_wait_all();
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------ E4M3: codes to bf16, a thread a key
+    if constexpr (V8) {
+      const int r = tid - 384;
+      uint32_t n = 1;
+      bool ok = true;
+      for (int i = i0; i <= i1 && ok; ++i) {
+        const RowItem it = load_item(p.items + i);
+        if (it.nblk == 0) continue;
+        const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+        // the scale of key r of block j; 0 past the last key, where the codes (clamped pages) are finite or NaN
+        auto scale_of = [&](int j) {
+          const int key = it.k0 + j * kKeyBlock + r;
+          if (key >= it.k1) return 0.f;
+          int page = p.page_table[static_cast<int64_t>(it.kv) * p.max_pages + key / kPage];
+          if (page < 0 || page >= p.num_pages) page = 0;  // the loading warp reports it
+          return p.v_scale[(static_cast<int64_t>(page) * p.KV + it.head) * kPage + key % kPage];
+        };
+        float next = scale_of(0);
+        for (int j = 0; j < nb; ++j, n += 2) {
+          const float sc = next;
+          const bool in = it.k0 + j * kKeyBlock + r < it.k1;
+          if (j + 1 < nb) next = scale_of(j + 1);
+          const uint32_t s = n % NS, b = (n >> 1) & 1;
+          ok = warp_wait(&raw_full[b], (n >> 2) & 1);
+          if (ok && n >= NS) ok = warp_wait(&empty[s], (n / NS - 1) & 1);
+          if (!ok) break;
+          const uint8_t* src = smem + Geo::RAW + b * 16384 + r * 128;
+          uint8_t* dst = smem + Geo::RING + s * Geo::TILE + r * 128;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const int ch = (c + r) & 7;  // rotated, so that neighbouring keys use different banks
+            const uint4 x = *reinterpret_cast<const uint4*>(src + ch * 16);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            uint32_t y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t h = e4m3x2_to_f16x2(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+              y[e] = in ? pack_bf16(f.x * sc, f.y * sc) : 0u;
+            }
+            uint8_t* d = dst + (ch >> 2) * 16384;
+            const int g = (ch & 3) * 2;
+            *reinterpret_cast<uint4*>(d + ((g ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(d + (((g + 1) ^ (r & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&full[s]);
+            mbar_arrive(&raw_empty[b]);
+          }
+        }
+      }
+      if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+    }
+  } else if (warp == 11 && !V8) {
+    // ------------------------------------------------------------ V rows past the last key
+    uint32_t n = 0, cleaned = 0;
+    for (int i = i0; i <= i1; ++i) {
+      const RowItem it = load_item(p.items + i);
+      if (it.nblk == 0) continue;
+      const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+      const int rem = (it.k1 - it.k0) % kKeyBlock;
+      if (rem != 0) {
+        const uint32_t k = n + 2 * nb - 1;
+        // asked for by the MMA warp, which has seen the block arrive and waits for the answer
+        if (!warp_wait(&c_req, cleaned & 1)) {
+          if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+          break;
+        }
+        uint8_t* v = smem + Geo::RING + (k % NS) * Geo::TILE;
+#pragma unroll
+        for (int x = 0; x < KH; ++x)
+          for (int o = rem * 128 + lane * 16; o < 16384; o += 512)
+            *reinterpret_cast<uint4*>(v + x * 16384 + o) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_clean);
+        ++cleaned;
+      }
+      n += 2 * nb;
+    }
+  }
   }
   umma::fence_before_sync();
   __syncthreads();
@@ -1029,12 +1130,12 @@ static int launch_row_attention(const RowParams& p, const CUtensorMap& kmap, con
                                 cudaStream_t st) {
   // the attribute belongs to the function on each device; setting it again is cheap and needs no state of its own
   const cudaError_t e = cudaFuncSetAttribute(row_attention_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             RowGeom<D>::SMEM);
+                                             RowGeom<D, RowRoles<SRC>::V8>::SMEM);
   if (e != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "row_attention_kernel: %s", cudaGetErrorString(e));
   if (!reuse_plan)
     if (int rc = launch_pdl("row_plan_kernel", row_plan_kernel, dim3(1), dim3(1024), 0, st, p)) return rc;
-  if (int rc = launch_pdl("row_attention_kernel", row_attention_kernel<D, SRC>, dim3(p.grid), dim3(kRowThreads),
-                          RowGeom<D>::SMEM, st, p, kmap, vmap))
+  if (int rc = launch_pdl("row_attention_kernel", row_attention_kernel<D, SRC>, dim3(p.grid), dim3(RowRoles<SRC>::THREADS),
+                          RowGeom<D, RowRoles<SRC>::V8>::SMEM, st, p, kmap, vmap))
     return rc;
   if (p.G == 0)
     return launch_pdl("join_cut_kernel", join_cut_kernel<D>, dim3(p.grid, kMergeParts), dim3(256), 0, st, p);
@@ -1129,7 +1230,11 @@ extern "C" int specdec_shared_prefix_attention(const SpecdecSharedPrefixArgs* a,
   if (kv.num_pages <= 0 || kv.max_pages_per_seq <= 0) return fail(SPECDEC_ERR_INVALID, "empty page pool");
   if ((reinterpret_cast<uintptr_t>(kv.k_pool) | reinterpret_cast<uintptr_t>(kv.v_pool)) & 15u)
     return fail(SPECDEC_ERR_INVALID, "pool pointers must be 16-byte aligned");
-  if (kv.v_dtype != SPECDEC_BF16) return fail(SPECDEC_ERR_UNSUPPORTED, "v_dtype must be SPECDEC_BF16");
+  if (kv.v_dtype != SPECDEC_BF16 && kv.v_dtype != SPECDEC_E4M3)
+    return fail(SPECDEC_ERR_UNSUPPORTED, "v_dtype must be SPECDEC_BF16 or SPECDEC_E4M3");
+  const bool v8 = kv.v_dtype == SPECDEC_E4M3;
+  if (v8 && s.D != 128) return fail(SPECDEC_ERR_UNSUPPORTED, "E4M3 V needs head_dim 128 (one scale group per head)");
+  if (v8 && !kv.v_scale) return fail(SPECDEC_ERR_INVALID, "E4M3 V needs v_scale");
   if (a->q_rows <= 0 || a->q_rows > 0x7fffffff) return fail(SPECDEC_ERR_INVALID, "row counts out of range");
   const int64_t page_rows = static_cast<int64_t>(kv.num_pages) * s.KV * (s.D / 64);
   if (page_rows > 0x7fffffff || static_cast<int64_t>(kv.max_pages_per_seq) * kPage > 0x7fffffff)
@@ -1152,12 +1257,14 @@ extern "C" int specdec_shared_prefix_attention(const SpecdecSharedPrefixArgs* a,
   p.num_pages = kv.num_pages;
   p.max_pages = kv.max_pages_per_seq;
   p.paged = 1;
+  p.v_scale = kv.v_scale;
   p.q_rows = a->q_rows;
   p.status = a->status;
   CUtensorMap km, vm;
   if (int rc = encode_rows_map(&km, kv.k_pool, static_cast<uint64_t>(page_rows), 2048)) return rc;
-  if (int rc = encode_rows_map(&vm, kv.v_pool, static_cast<uint64_t>(page_rows), 2048)) return rc;
+  if (int rc = encode_rows_map(&vm, kv.v_pool, static_cast<uint64_t>(v8 ? page_rows / 2 : page_rows), 2048)) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (v8) return launch_row_attention<128, kPagedE4M3>(p, km, vm, a->reuse_plan != 0, st);
   return s.D == 128 ? launch_row_attention<128, kPaged>(p, km, vm, a->reuse_plan != 0, st)
                     : launch_row_attention<64, kPaged>(p, km, vm, a->reuse_plan != 0, st);
 }
