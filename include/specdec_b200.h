@@ -67,6 +67,8 @@ typedef enum SpecdecResult {
 #define SPECDEC_STATUS_ACCEPT_RANGE 0x20 /* accept: kp outside [1, max_cands]         */
 #define SPECDEC_STATUS_PLAN_MISMATCH 0x40 /* reused plan built for another launch shape */
 #define SPECDEC_STATUS_BAD_GROUP 0x80     /* prefix group: member out of range or listed twice, bad start or length */
+#define SPECDEC_STATUS_BAD_SEQUENCE 0x100 /* page request with a sequence or a length out of range        */
+#define SPECDEC_STATUS_NO_PAGES 0x200     /* no free page left for a request                              */
 
 typedef enum SpecdecDtype { SPECDEC_F32 = 0, SPECDEC_BF16 = 1, SPECDEC_E4M3 = 2 } SpecdecDtype;
 
@@ -415,6 +417,68 @@ size_t specdec_shared_prefix_workspace_bytes(int32_t num_seqs, int32_t num_q_hea
                                              int32_t head_dim, int32_t max_q_len, int32_t num_groups,
                                              int32_t num_members, int32_t num_sms);
 int specdec_shared_prefix_attention(const SpecdecSharedPrefixArgs* args, specdec_stream_t stream);
+
+/*
+ * Pages of a cache between sequences, in all layers at once.
+ * page_refs[page] is the number of sequences that hold the page in their row of the page table; 0: it is free.  A row
+ * holds its pages in its first entries, -1 behind them.  New pages are the lowest free ids, in the order of the
+ * request.  Everything runs on the device (no host sync; it can be captured); calls that share a workspace must not
+ * overlap.  No counterpart in the reference (one sequence, caches grown with torch.cat).
+ */
+typedef struct SpecdecPagePool {
+  void* const* k_pools;   /* host arrays [num_layers] of device pools in SpecdecPagedKV's layout */
+  void* const* v_pools;
+  float* const* v_scales; /* E4M3 only */
+  int32_t num_layers;
+  int32_t num_pages;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t v_dtype;
+} SpecdecPagePool;
+
+typedef struct SpecdecPageTable {
+  int32_t* page_table; /* [num_seqs][max_pages_per_seq] */
+  int32_t* page_refs;  /* [num_pages] */
+  int32_t* lengths;    /* [num_seqs] */
+  int32_t num_seqs;
+  int32_t max_pages_per_seq;
+  void* workspace;     /* >= specdec_page_workspace_bytes(num_seqs, num_pages, n) bytes, any contents */
+  size_t workspace_bytes;
+  int32_t* status;     /* device int32, may be NULL */
+} SpecdecPageTable;
+
+/* Workspace of a call with n requests (n = 0 for reserve and compact). */
+size_t specdec_page_workspace_bytes(int32_t num_seqs, int32_t num_pages, int32_t n);
+
+/* Page src[i] to page dst[i] in every layer.  A page is a target once at most, and no source is a target (the copies
+   run at the same time).  A pair with a page out of range raises SPECDEC_STATUS_BAD_PAGE and is left out. */
+int specdec_copy_pages(const SpecdecPagePool* pool, const int32_t* src, const int32_t* dst, int32_t n, int32_t* status,
+                       specdec_stream_t stream);
+
+/* Sequence dst[i] gives up its pages and becomes the first length[i] tokens of sequence src[i]: full pages are shared
+   (their counts go up), a started one is copied to a page of its own.  All targets give up their pages before any
+   page is taken.  SPECDEC_STATUS_BAD_SEQUENCE: a sequence out of range, a length past the source's, a target
+   that is listed before or is itself a source; the request is left out.  SPECDEC_STATUS_BAD_PAGE: the source has no
+   pages for its tokens; left out.  SPECDEC_STATUS_NO_PAGES: no page for the started one; the target keeps its full
+   pages (and their tokens). */
+int specdec_fork_sequences(const SpecdecPagePool* pool, const SpecdecPageTable* table, const int32_t* src,
+                           const int32_t* dst, const int32_t* length, int32_t n, specdec_stream_t stream);
+
+/* Every sequence gets pages for tokens[b] tokens (fewer than it has: nothing happens).  Held pages that it would go on
+   writing into, from position lengths[b] on, are replaced where others hold them, too; what a started one holds is
+   copied.  SPECDEC_STATUS_NO_PAGES: a sequence, and those after it, are left as they were.
+   SPECDEC_STATUS_PAGE_OVERFLOW: more tokens than the table has entries for (the sequence is left as it was). */
+int specdec_reserve_pages(const SpecdecPagePool* pool, const SpecdecPageTable* table, const int32_t* tokens,
+                          specdec_stream_t stream);
+
+/* The sequences give up their pages; their lengths become 0.  SPECDEC_STATUS_BAD_SEQUENCE: out of range. */
+int specdec_free_sequences(const SpecdecPagePool* pool, const SpecdecPageTable* table, const int32_t* seqs, int32_t n,
+                           specdec_stream_t stream);
+
+/* Live pages move to the front of the pools, in ascending order into the free ids there; tables and counts follow.
+   n_live (device) receives their number: pages from there on are free. */
+int specdec_compact_pages(const SpecdecPagePool* pool, const SpecdecPageTable* table, int32_t* n_live,
+                          specdec_stream_t stream);
 
 /* RMSNorm over the last dim (fp32 mean of squares; the normalised value is
    rounded to the input dtype before the weight multiply, as model_self.RMSNORM). */

@@ -31,6 +31,8 @@ STATUS_TIMEOUT = 0x10
 STATUS_ACCEPT_RANGE = 0x20
 STATUS_PLAN_MISMATCH = 0x40
 STATUS_BAD_GROUP = 0x80
+STATUS_BAD_SEQUENCE = 0x100
+STATUS_NO_PAGES = 0x200
 
 STATUS_NAMES = {
     STATUS_BAD_LENGTH: "bad length (ctx_len < q_len or q_len > max_q_len)",
@@ -41,6 +43,8 @@ STATUS_NAMES = {
     STATUS_ACCEPT_RANGE: "accept row/candidate count out of range",
     STATUS_PLAN_MISMATCH: "reused plan was built for another launch shape (cluster choice or SM budget)",
     STATUS_BAD_GROUP: "prefix group with a bad start, length or member (out of range, or listed twice)",
+    STATUS_BAD_SEQUENCE: "page request with a sequence or a length out of range",
+    STATUS_NO_PAGES: "no free page left for a request",
 }
 
 _vp = ctypes.c_void_p
@@ -207,6 +211,32 @@ class SharedPrefixArgs(ctypes.Structure):
     ]
 
 
+class PagePool(ctypes.Structure):
+    _fields_ = [
+        ("k_pools", _vp),
+        ("v_pools", _vp),
+        ("v_scales", _vp),
+        ("num_layers", _i32),
+        ("num_pages", _i32),
+        ("num_kv_heads", _i32),
+        ("head_dim", _i32),
+        ("v_dtype", _i32),
+    ]
+
+
+class PageTable(ctypes.Structure):
+    _fields_ = [
+        ("page_table", _vp),
+        ("page_refs", _vp),
+        ("lengths", _vp),
+        ("num_seqs", _i32),
+        ("max_pages_per_seq", _i32),
+        ("workspace", _vp),
+        ("workspace_bytes", _sz),
+        ("status", _vp),
+    ]
+
+
 class AcceptArgs(ctypes.Structure):
     _fields_ = [
         ("logits", _vp),
@@ -266,6 +296,13 @@ SIGNATURES = {
     "specdec_prompt_attention": (ctypes.c_int, [ctypes.POINTER(PromptArgs), _vp]),
     "specdec_shared_prefix_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "specdec_shared_prefix_attention": (ctypes.c_int, [ctypes.POINTER(SharedPrefixArgs), _vp]),
+    "specdec_page_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "specdec_copy_pages": (ctypes.c_int, [ctypes.POINTER(PagePool), _vp, _vp, _i32, _vp, _vp]),
+    "specdec_fork_sequences": (
+        ctypes.c_int, [ctypes.POINTER(PagePool), ctypes.POINTER(PageTable), _vp, _vp, _vp, _i32, _vp]),
+    "specdec_reserve_pages": (ctypes.c_int, [ctypes.POINTER(PagePool), ctypes.POINTER(PageTable), _vp, _vp]),
+    "specdec_free_sequences": (ctypes.c_int, [ctypes.POINTER(PagePool), ctypes.POINTER(PageTable), _vp, _i32, _vp]),
+    "specdec_compact_pages": (ctypes.c_int, [ctypes.POINTER(PagePool), ctypes.POINTER(PageTable), _vp, _vp]),
     "specdec_lmhead_argmax": (ctypes.c_int, [_vp, _vp]),
     "specdec_quantize_int8": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _vp]),
     "specdec_rmsnorm_int8": (

@@ -745,6 +745,112 @@ def shared_prefix_attention(q, cache: PagedKVCache, layer: int, batch: RaggedBat
     return out
 
 
+# ---------------------------------------------------------------------------- pages between sequences
+def _page_pool(cache: PagedKVCache):
+    """(library, device, stream, C pool and the pointer arrays it points to) of a call on all layers of ``cache``."""
+    lib, dev, stream = _call(cache.page_table)
+    pools, n = cache.pools, cache.num_layers
+    if pools[0].k.get_device() != dev:
+        raise RuntimeError("tensors must be CUDA, all on one device")
+    array = ctypes.c_void_p * n
+    keep = [array(*[p.k.data_ptr() for p in pools]), array(*[p.v.data_ptr() for p in pools])]
+    e4m3 = cache.v_dtype == "e4m3"
+    if e4m3:
+        keep.append(array(*[p.v_scale.data_ptr() for p in pools]))
+    pool = _lib.PagePool(ctypes.addressof(keep[0]), ctypes.addressof(keep[1]),
+                         ctypes.addressof(keep[2]) if e4m3 else None, n, cache.num_pages, cache.num_kv_heads,
+                         cache.head_dim, _lib.E4M3 if e4m3 else _lib.BF16)
+    return lib, dev, stream, (pool, keep)
+
+
+def _page_table(cache: PagedKVCache, n: int, workspace, status, lib, dev: int):
+    if cache.page_refs is None:
+        raise ValueError("the cache's pages are static; allocate it with shared pages")
+    _check_status(status, dev)
+    nbytes = lib.specdec_page_workspace_bytes(cache.num_seqs, cache.num_pages, n)
+    workspace = _row_workspace(workspace, nbytes, cache.page_table, dev, False)
+    cache.host_lengths = None
+    return workspace, _lib.PageTable(cache.page_table.data_ptr(), cache.page_refs.data_ptr(),
+                                     cache.lengths.data_ptr(), cache.num_seqs, cache.max_pages, workspace.data_ptr(),
+                                     workspace.numel(), _ptr(status))
+
+
+def page_workspace(cache: PagedKVCache, requests: int = 0) -> torch.Tensor:
+    """Workspace of the page operators for up to ``requests`` sequences a call (any contents)."""
+    n = _lib_handle().specdec_page_workspace_bytes(cache.num_seqs, cache.num_pages, int(requests))
+    if n == 0:
+        raise ValueError("invalid request count")
+    return torch.empty(n, dtype=torch.uint8, device=cache.device)
+
+
+def _requests(dev: int, *arrays) -> int:
+    n = arrays[0].numel()
+    for t in arrays:
+        if t.get_device() != dev:
+            raise RuntimeError("tensors must be CUDA, all on one device")
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+            raise ValueError("requests must be contiguous int32, all of one length")
+    return n
+
+
+def copy_pages(cache: PagedKVCache, src, dst, *, status=None) -> None:
+    """Copy page ``src[i]`` to page ``dst[i]`` in every layer (K, V and scales); int32 device arrays.  A page is a
+    target once at most, and no source is a target.  Page tables and counts stay as they are."""
+    lib, dev, stream, pool = _page_pool(cache)
+    n = _requests(dev, src, dst)
+    _check_status(status, dev)
+    rc = lib.specdec_copy_pages(ctypes.byref(pool[0]), src.data_ptr(), dst.data_ptr(), n, _ptr(status), stream)
+    if rc:
+        _lib.check(rc, "copy_pages")
+
+
+def fork_sequences(cache: PagedKVCache, src, dst, length, *, workspace=None, status=None) -> None:
+    """Sequence ``dst[i]`` becomes the first ``length[i]`` tokens of sequence ``src[i]`` (int32 device arrays): full
+    pages are shared, a started one is copied.  What dst held is given up first; no source is a target."""
+    lib, dev, stream, pool = _page_pool(cache)
+    n = _requests(dev, src, dst, length)
+    workspace, table = _page_table(cache, n, workspace, status, lib, dev)
+    rc = lib.specdec_fork_sequences(ctypes.byref(pool[0]), ctypes.byref(table), src.data_ptr(), dst.data_ptr(),
+                                    length.data_ptr(), n, stream)
+    if rc:
+        _lib.check(rc, "fork_sequences")
+
+
+def reserve_pages(cache: PagedKVCache, tokens, *, workspace=None, status=None) -> None:
+    """Pages for ``tokens[b]`` tokens of every sequence (int32 (num_seqs,) on the device).  Held pages from position
+    ``cache.lengths[b]`` on that others hold, too, are replaced (a started one's contents are copied), so that what is
+    appended next reaches nobody else."""
+    lib, dev, stream, pool = _page_pool(cache)
+    if _requests(dev, tokens) != cache.num_seqs:
+        raise ValueError("one token count per sequence")
+    workspace, table = _page_table(cache, 0, workspace, status, lib, dev)
+    rc = lib.specdec_reserve_pages(ctypes.byref(pool[0]), ctypes.byref(table), tokens.data_ptr(), stream)
+    if rc:
+        _lib.check(rc, "reserve_pages")
+
+
+def free_sequences(cache: PagedKVCache, seqs, *, workspace=None, status=None) -> None:
+    """The sequences (int32 device array) give up their pages; their lengths become 0."""
+    lib, dev, stream, pool = _page_pool(cache)
+    n = _requests(dev, seqs)
+    workspace, table = _page_table(cache, n, workspace, status, lib, dev)
+    rc = lib.specdec_free_sequences(ctypes.byref(pool[0]), ctypes.byref(table), seqs.data_ptr(), n, stream)
+    if rc:
+        _lib.check(rc, "free_sequences")
+
+
+def compact_pages(cache: PagedKVCache, *, workspace=None, status=None) -> torch.Tensor:
+    """Move the live pages to the front of the pools, in every layer; tables and counts follow.  Returns their number
+    (int32, on the device): pages from there on are free."""
+    lib, dev, stream, pool = _page_pool(cache)
+    workspace, table = _page_table(cache, 0, workspace, status, lib, dev)
+    n_live = torch.empty((), dtype=torch.int32, device=cache.page_table.device)
+    rc = lib.specdec_compact_pages(ctypes.byref(pool[0]), ctypes.byref(table), n_live.data_ptr(), stream)
+    if rc:
+        _lib.check(rc, "compact_pages")
+    return n_live
+
+
 # ---------------------------------------------------------------------------- 8-bit linear path
 # These calls take a few microseconds of GPU time each in a decode step, so their checks read every
 # attribute once and the library and stream are looked up directly.
