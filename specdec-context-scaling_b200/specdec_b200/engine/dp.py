@@ -78,19 +78,23 @@ class DPResult:
 
 def run_specdec_dp(target_cfg, draft_cfg, *, total_seqs: int, prompt_len: int, max_new: int, k: int = 4,
                    seed: int = 0, world: int = 1, rank: int = 0, target_v: str = "bf16", chunk: int = 4,
-                   barrier=None, draft_is_target: bool = False, weights: str = "bf16") -> DPResult:
+                   barrier=None, draft_is_target: bool = False, weights: str = "bf16",
+                   shared_prefix: int = 0) -> DPResult:
     """One data-parallel SpecDec job on this rank's GPU (weights from ``seed``).  The
     decode time is the device time of the round-graph replays (CUDA events).
     ``draft_is_target``: the draft runs the target's weights (``draft_cfg`` is ignored), so
     nearly every candidate is accepted -- the full-accept path of every round.
-    ``weights``: "bf16" or "int8" projections, in both models."""
+    ``weights``: "bf16" or "int8" projections, in both models.
+    ``shared_prefix``: first tokens that all prompts have in common (the same on every rank), read once a rank."""
     from .model import PagedModel
     from .specdec import SpecDecEngine
 
     check_shardable(total_seqs, world)
     dev = torch.device("cuda", torch.cuda.current_device())
     s, e = shard_bounds(total_seqs, world, rank)
-    prompts = synthetic_prompts(total_seqs, prompt_len, target_cfg.vocab, seed)[s:e].to(dev)
+    prompts = synthetic_prompts(total_seqs, prompt_len, target_cfg.vocab, seed)
+    prompts[:, :shared_prefix] = prompts[:1, :shared_prefix].clone()
+    prompts = prompts[s:e].to(dev)
     if draft_is_target:
         from .model import random_state
 
@@ -100,7 +104,8 @@ def run_specdec_dp(target_cfg, draft_cfg, *, total_seqs: int, prompt_len: int, m
     else:
         target = PagedModel.random(target_cfg, seed + 1, dev, weights=weights)
         draft = PagedModel.random(draft_cfg, seed + 2, dev, weights=weights)
-    eng = SpecDecEngine(target, draft, e - s, prompt_len, max_new, k=k, target_v=target_v)
+    eng = SpecDecEngine(target, draft, e - s, prompt_len, max_new, k=k, target_v=target_v,
+                        shared_prefix=shared_prefix)
     eng.capture()  # warm-up round + graph capture on the empty state; prefill resets it
     sync = barrier or (lambda: None)
     torch.cuda.synchronize()

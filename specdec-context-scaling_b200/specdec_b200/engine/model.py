@@ -11,11 +11,12 @@ Per layer of a decode / verify step (rows = packed query rows of all sequences):
   qkv = h W_qkv^T + b_qkv                          cuBLAS (one fused GEMM)
   q = rope(q) out; rope(k) and v appended to the layer's pages (V quantised to E4M3
       for an e4m3 cache), one launch                specdec_rope_append
-  o   = paged attention of q over the layer's pages        specdec_paged_attention
+  o   = paged attention of q over the layer's pages        specdec_paged_attention, or
+      specdec_shared_prefix_attention where sequences share their first pages
   x  += o W_o^T                                    cuBLAS (residual added in place)
   x  += W_down swiglu(W_gate|up rmsnorm(x))        specdec_rmsnorm, cuBLAS, specdec_swiglu_packed
-Prefill (the whole prompt at once) uses torch's fused causal attention for the
-prompt block and appends the prompt's K/V into the pages; decode never does.
+Prefill (the whole prompt at once) attends over the prompt's own K/V rows
+(specdec_prompt_attention) and appends them into the pages.
 
 With ``weights="int8"`` the projections run on 8-bit weights and activations (one scale for
 each output channel and each token), in a decode / verify step and in the prompt pass:
@@ -35,11 +36,9 @@ reference QwenLM's weights load directly, or from a seeded random init.
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
-import torch.nn.functional as F
 
 from ..kernels import ops
 from .paged_cache import PagedKVCache
@@ -167,6 +166,27 @@ class StepLayout:
         return (self.q_row0 + self.q_len - 1).long()
 
 
+class PieceLayout(StepLayout):
+    """Rows of a step in which sequences ``seq0`` .. ``seq0 + n - 1`` of ``num_seqs`` read ``q_max`` new
+    tokens each (the next piece of their prompts) and the others none: n * q_max packed rows."""
+
+    def __init__(self, num_seqs: int, seq0: int, n: int, q_max: int, device):
+        super().__init__(num_seqs, q_max, device)
+        self.rows, self.seq0, self.n = n * q_max, seq0, n
+        seqs = torch.arange(num_seqs, dtype=torch.int32, device=device)
+        inside = (seqs >= seq0) & (seqs < seq0 + n)
+        self.q_row0.copy_((seqs - seq0).clamp(0, n - 1) * q_max)
+        self.q_len.copy_(inside.int() * q_max)
+        self.batch.total_rows = self.rows
+
+    def positions(self) -> torch.Tensor:
+        return super().positions()[self.seq0 * self.q_max:(self.seq0 + self.n) * self.q_max]
+
+    def last_rows(self) -> torch.Tensor:
+        """(n,) packed row of every reading sequence's last query row."""
+        return super().last_rows()[self.seq0:self.seq0 + self.n]
+
+
 class PagedModel:
     """Decoder weights in fused, layout-ready form plus the batched paged forward."""
 
@@ -209,10 +229,11 @@ class PagedModel:
     def random(cls, cfg: ModelConfig, seed: int, device="cuda", *, weights: str = "bf16") -> "PagedModel":
         return cls(cfg, random_state(cfg, seed, device), device, weights=weights)
 
-    def new_cache(self, num_seqs: int, capacity: int, v_dtype: str = "bf16") -> PagedKVCache:
+    def new_cache(self, num_seqs: int, capacity: int, v_dtype: str = "bf16", *, num_pages: int | None = None,
+                  on_demand: bool = False) -> PagedKVCache:
         c = self.cfg
         return PagedKVCache.allocate(c.layers, num_seqs, c.kv_heads, c.head_dim, capacity, v_dtype=v_dtype,
-                                     device=self.device)
+                                     device=self.device, num_pages=num_pages, on_demand=on_demand)
 
     # ------------------------------------------------------------------ pieces
     def _cos_sin(self, pos: torch.Tensor):
@@ -265,12 +286,14 @@ class PagedModel:
 
     # ------------------------------------------------------------------ forward passes
     def step(self, tokens: torch.Tensor, layout: StepLayout, cache: PagedKVCache, workspace: torch.Tensor,
-             *, status: torch.Tensor | None = None) -> torch.Tensor:
+             *, status: torch.Tensor | None = None, prefix: ops.SharedPrefix | None = None) -> torch.Tensor:
         """One decode / verify step of ``layout.rows`` packed query rows (token ids ``tokens``).
 
         Appends every sequence's ``q_len`` new K/V rows at positions ``pos0 ..`` of all
         layers and returns the final-norm hidden states (rows, hidden).  Rows past a
-        sequence's q_len are padding: their outputs are meaningless and never stored."""
+        sequence's q_len are padding: their outputs are meaningless and never stored.
+        ``prefix``: the groups of sequences that share their first pages, which are then read once a
+        group (``workspace`` from ``ops.shared_prefix_workspace``)."""
         c = self.cfg
         rows = layout.rows
         x = self.embed[tokens.long()]
@@ -292,8 +315,12 @@ class PagedModel:
                             max_new=layout.q_max, q_out=q, status=status)
             # layers after the first reuse layer 0's plan; the only KV the steps before write
             # is this step's new tokens, so the history may be loaded early
-            ops.paged_attention(q, cache, li, layout.batch, out=o, workspace=workspace, reuse_plan=li > 0,
-                                status=status, history_ready=li > 0)
+            if prefix is not None:
+                ops.shared_prefix_attention(q, cache, li, layout.batch, prefix, out=o, workspace=workspace,
+                                            status=status, reuse_plan=li > 0)
+            else:
+                ops.paged_attention(q, cache, li, layout.batch, out=o, workspace=workspace, reuse_plan=li > 0,
+                                    status=status, history_ready=li > 0)
             if self.int8:
                 delta = L.w_o(*ops.quantize_int8(o.view(rows, c.heads * c.head_dim)), status)
                 delta = self._mlp_int8(L, x, delta, status)
@@ -305,24 +332,31 @@ class PagedModel:
         return ops.rmsnorm(x, self.norm, c.eps)
 
     def prefill(self, ids: torch.Tensor, cache: PagedKVCache, seq0: int, *, need_logits: bool = True,
-                status: torch.Tensor | None = None) -> torch.Tensor | None:
+                status: torch.Tensor | None = None, lengths: list[int] | None = None) -> torch.Tensor | None:
         """Prompt pass of sequences seq0 .. seq0 + n - 1 (ids (n, P)): writes their K/V at
         positions 0 .. P-1 of every layer, sets their lengths to P and returns the logits
-        of each prompt's last position (n, vocab).  The causal attention inside the
-        prompt block uses torch's fused attention (prefill is not the decode path)."""
+        of each prompt's last position (n, vocab).  ``lengths``: tokens of each prompt
+        (1 .. P), the ids behind them being padding that is neither attended to nor stored."""
         c = self.cfg
         n, P = ids.shape
+        if lengths is not None and (len(lengths) != n or min(lengths) < 1 or max(lengths) > P):
+            raise ValueError(f"lengths must be {n} token counts in 1 .. {P}")
         rows = n * P
         dev = ids.device
         i32 = dict(dtype=torch.int32, device=dev)
         seqs = torch.arange(cache.num_seqs, **i32)
         inside = (seqs >= seq0) & (seqs < seq0 + n)
         row0 = torch.where(inside, (seqs - seq0) * P, torch.zeros_like(seqs))
-        n_new = torch.where(inside, torch.full_like(seqs, P), torch.zeros_like(seqs))
+        q_len = torch.full((n,), P, **i32) if lengths is None else torch.tensor(lengths, dtype=torch.int32).to(dev)
+        n_new = torch.zeros_like(seqs)
+        n_new[seq0:seq0 + n] = q_len
         pos0 = torch.zeros(cache.num_seqs, **i32)
         x = self.embed[ids.reshape(-1).long()]
         cos, sin = self._cos_sin(torch.arange(P, device=dev).repeat(n))
-        n_rep = c.heads // c.kv_heads
+        batch = ops.RaggedBatch(torch.arange(n, **i32) * P, q_len, q_len, n, P, rows, P)
+        workspace = ops.prompt_workspace(batch, c.heads, c.kv_heads, c.head_dim, dev)
+        # padding rows are written by nobody and mixed into nothing: zero, so that they stay finite
+        o = (torch.empty if lengths is None else torch.zeros)(rows, c.heads, c.head_dim, dtype=x.dtype, device=dev)
         delta = None
         for li, L in enumerate(self.layers):
             if self.int8:
@@ -336,21 +370,19 @@ class PagedModel:
                 # scales), as the reference's V-only FP8 prompt pass attends over
                 # dequantize(quantize(v)) (model_self.py:702-704)
                 v = _e4m3_round_trip(v)
-            q4 = q[0].view(c.heads, n, P, c.head_dim).transpose(0, 1)
-            k4 = k[0].view(c.kv_heads, n, P, c.head_dim).transpose(0, 1).repeat_interleave(n_rep, dim=1)
-            v4 = v.view(c.kv_heads, n, P, c.head_dim).transpose(0, 1).repeat_interleave(n_rep, dim=1)
-            o = F.scaled_dot_product_attention(q4, k4, v4, is_causal=True, scale=1.0 / math.sqrt(c.head_dim))
-            o = o.transpose(1, 2).reshape(rows, c.heads * c.head_dim)
+            ops.prompt_attention(q[0].transpose(0, 1), k[0].transpose(0, 1), v.transpose(0, 1), batch, out=o,
+                                 workspace=workspace, status=status, reuse_plan=li > 0)
+            o2 = o.view(rows, c.heads * c.head_dim)
             if self.int8:
-                delta = self._mlp_int8(L, x, L.w_o(*ops.quantize_int8(o), status), status)
+                delta = self._mlp_int8(L, x, L.w_o(*ops.quantize_int8(o2), status), status)
             else:
-                x = x + o @ L.w_o.t()
+                x = x + o2 @ L.w_o.t()
                 x = self._mlp(L, x)
-        cache.lengths.copy_(torch.where(inside, torch.full_like(seqs, P), cache.lengths))
+        cache.lengths.copy_(torch.where(inside, n_new, cache.lengths))
         cache.host_lengths = None
         if not need_logits:
             return None
         if delta is not None:
             x.add_(delta)
-        last = x.view(n, P, -1)[:, -1]
+        last = x.view(n, P, -1)[torch.arange(n, device=dev), q_len.long() - 1]
         return self.logits(ops.rmsnorm(last.contiguous(), self.norm, c.eps))

@@ -18,6 +18,10 @@ docs/design_g4_cache_api.md:8-10) is a per-layer dict of contiguous
 information in fixed pools; ``gather_layer`` returns the reference layout.
 Every page of a sequence is assigned when the cache is created (static
 capacity), so appends, rollback and attention never need the host.
+
+With ``on_demand`` pages the table starts empty (-1) and sequences take pages when they need
+them (``reserve``), share those of another one (``fork``) and give them back (``free``);
+``page_refs`` counts who holds a page.  All of it runs on the device, too.
 """
 
 from __future__ import annotations
@@ -92,6 +96,7 @@ class PagedKVCache:
         device: torch.device | str = "cuda",
         page_order_seed: int | None = None,
         num_pages: int | None = None,
+        on_demand: bool = False,
     ) -> "PagedKVCache":
         if v_dtype not in ("bf16", "e4m3"):
             raise ValueError(f"v_dtype must be 'bf16' or 'e4m3', got {v_dtype!r}")
@@ -103,9 +108,15 @@ class PagedKVCache:
         max_pages = max(1, math.ceil(capacity / PAGE))
         need = num_seqs * max_pages
         total = need if num_pages is None else int(num_pages)
-        if total < need:
+        if total < need and not on_demand:
             raise ValueError(f"pool of {total} pages cannot hold {num_seqs} x {max_pages} pages")
-        if page_order_seed is None:
+        if total < 1:
+            raise ValueError("empty page pool")
+        if on_demand:
+            if page_order_seed is not None:
+                raise ValueError("pages handed out on demand have no order of their own")
+            order = torch.full((need,), -1, dtype=torch.int32)
+        elif page_order_seed is None:
             order = torch.arange(need, dtype=torch.int32)
         else:
             g = torch.Generator().manual_seed(int(page_order_seed))
@@ -136,6 +147,7 @@ class PagedKVCache:
             lengths=torch.zeros(num_seqs, dtype=torch.int32, device=device),
             host_lengths=[0] * num_seqs,
             fmt="v_fp8" if v_dtype == "e4m3" else "fp16",
+            page_refs=torch.zeros(total, dtype=torch.int32, device=device) if on_demand else None,
         )
 
     @classmethod
@@ -220,6 +232,38 @@ class PagedKVCache:
         """Read the device lengths back (one device->host copy)."""
         self.host_lengths = [int(x) for x in self.lengths.cpu().tolist()]
         return self.host_lengths
+
+    # ------------------------------------------------------------------ pages on demand
+    def _i32(self, values) -> torch.Tensor:
+        if isinstance(values, torch.Tensor):
+            return values.to(device=self.device, dtype=torch.int32).contiguous()
+        return torch.tensor([int(v) for v in values], dtype=torch.int32).to(self.device)
+
+    def reserve(self, tokens, *, status: torch.Tensor | None = None) -> None:
+        """Pages for ``tokens[b]`` tokens of every sequence; pages that a sequence would go on writing into and others
+        hold are replaced (``ops.reserve_pages``)."""
+        from ..kernels import ops
+
+        ops.reserve_pages(self, self._i32(tokens), status=status)
+
+    def fork(self, src, dst, length, *, status: torch.Tensor | None = None) -> None:
+        """Sequence ``dst[i]`` becomes the first ``length[i]`` tokens of ``src[i]``, sharing its full pages
+        (``ops.fork_sequences``)."""
+        from ..kernels import ops
+
+        ops.fork_sequences(self, self._i32(src), self._i32(dst), self._i32(length), status=status)
+
+    def free(self, seqs, *, status: torch.Tensor | None = None) -> None:
+        """The sequences give up their pages; their lengths become 0 (``ops.free_sequences``)."""
+        from ..kernels import ops
+
+        ops.free_sequences(self, self._i32(seqs), status=status)
+
+    def compact(self, *, status: torch.Tensor | None = None) -> torch.Tensor:
+        """Live pages to the front of the pools; their number, on the device (``ops.compact_pages``)."""
+        from ..kernels import ops
+
+        return ops.compact_pages(self, status=status)
 
     # ------------------------------------------------------------------ layout helpers
     def gather_layer(self, layer: int, seq: int, length: int | None = None) -> dict:

@@ -22,6 +22,10 @@ the next round: its query lengths are 0 in every step of the round (no append, n
 attention rows), accept treats it as inactive (m = 0, lengths kept), and nothing is
 emitted for it, so its caches stop growing while slower sequences finish.
 
+With ``shared_prefix`` tokens the prompts begin alike (a system prompt): these are read once, by
+sequence 0, whose pages the others fork; what follows them is read by one step a chunk of sequences, and every
+step of a round reads the shared pages once (``ops.shared_prefix_attention``).
+
 Every step of a round is a fixed-shape device computation (the ragged q_len of
 step 1 lives in device arrays), so a round is captured once in a CUDA graph and
 replayed with no host synchronisation; the host only checks the emitted-token
@@ -34,12 +38,14 @@ from __future__ import annotations
 import torch
 
 from ..kernels import ops
-from .model import PagedModel, StepLayout
+from .model import PagedModel, PieceLayout, StepLayout
+from .paged_cache import PAGE
 
 
 class SpecDecEngine:
     def __init__(self, target: PagedModel, draft: PagedModel, num_seqs: int, prompt_len: int, max_new: int, *,
-                 k: int = 4, target_v: str = "bf16", draft_v: str = "bf16", check_every: int = 4):
+                 k: int = 4, target_v: str = "bf16", draft_v: str = "bf16", check_every: int = 4,
+                 shared_prefix: int = 0):
         if k < 1:
             raise ValueError("k must be >= 1")
         if target.cfg.vocab != draft.cfg.vocab:
@@ -52,14 +58,24 @@ class SpecDecEngine:
         # a sequence is frozen once it has max_new tokens, so its caches hold at most the
         # prompt, max_new + k emitted tokens and one verify block
         cap = prompt_len + max_new + 2 * (k + 1) + 2
-        self.tc = target.new_cache(num_seqs, cap, target_v)
-        self.dc = draft.new_cache(num_seqs, cap, draft_v)
+        if not 0 <= shared_prefix < prompt_len:
+            raise ValueError(f"shared_prefix must be in 0 .. {prompt_len - 1}: every prompt has a token of its own")
+        self.shared, self.cap = shared_prefix, cap
+        self.prefix = None
+        pages = {}
+        if shared_prefix:
+            # the prefix's full pages once, everything behind them for each sequence
+            full = shared_prefix // PAGE
+            pages = dict(on_demand=True, num_pages=full + num_seqs * (-(-cap // PAGE) - full))
+            self.prefix = ops.SharedPrefix.from_groups([(range(num_seqs), shared_prefix)], dev)
+        self.tc = target.new_cache(num_seqs, cap, target_v, **pages)
+        self.dc = draft.new_cache(num_seqs, cap, draft_v, **pages)
         self.L0 = StepLayout(num_seqs, 2, dev)
         self.L1 = StepLayout(num_seqs, 1, dev)
         self.LV = StepLayout(num_seqs, k + 1, dev)
-        self.ws0 = ops.attn_workspace(self.L0.batch, draft.cfg.heads, self.dc)
-        self.ws1 = ops.attn_workspace(self.L1.batch, draft.cfg.heads, self.dc)
-        self.wsv = ops.attn_workspace(self.LV.batch, target.cfg.heads, self.tc)
+        self.ws0 = self._workspace(self.L0, draft, self.dc)
+        self.ws1 = self._workspace(self.L1, draft, self.dc)
+        self.wsv = self._workspace(self.LV, target, self.tc)
         i32 = dict(dtype=torch.int32, device=dev)
         self.pending = torch.zeros(num_seqs, **i32)
         self.catch = torch.zeros(num_seqs, **i32)     # 1: the draft has not read the last round's ck
@@ -86,6 +102,11 @@ class SpecDecEngine:
         self.idx = torch.arange(k + 1, device=dev, dtype=torch.int32)
         self.active = torch.ones(num_seqs, **i32)   # 0: the sequence has its max_new tokens
 
+    def _workspace(self, layout: StepLayout, model: PagedModel, cache) -> torch.Tensor:
+        if self.prefix is not None:
+            return ops.shared_prefix_workspace(layout.batch, self.prefix, model.cfg.heads, cache)
+        return ops.attn_workspace(layout.batch, model.cfg.heads, cache)
+
     # ------------------------------------------------------------------ prompt
     @torch.inference_mode()
     def prefill(self, prompts: torch.Tensor, chunk: int = 4) -> None:
@@ -94,7 +115,9 @@ class SpecDecEngine:
         if tuple(prompts.shape) != (self.B, self.P):
             raise ValueError(f"prompts must be ({self.B}, {self.P})")
         self.status.zero_()
-        for s0 in range(0, self.B, chunk):
+        if self.shared:
+            self._prefill_shared(prompts, chunk)
+        for s0 in range(0, self.B if not self.shared else 0, chunk):
             ids = prompts[s0:s0 + chunk]
             lg = self.target.prefill(ids, self.tc, s0, status=self.status)
             self.pending[s0:s0 + ids.shape[0]] = lg.argmax(-1).int()
@@ -108,6 +131,28 @@ class SpecDecEngine:
         self.active_rounds.zero_()
         self.rounds = 0
 
+    def _prefill_shared(self, prompts: torch.Tensor, chunk: int) -> None:
+        """The common tokens once, in sequence 0, forked to all; then what follows, a chunk of sequences a step."""
+        n0, own = self.shared, self.P - self.shared
+        if not torch.equal(prompts[:, :n0], prompts[:1, :n0].expand(self.B, n0)):
+            raise ValueError(f"the prompts do not share their first {n0} tokens")
+        for model, cache in ((self.target, self.tc), (self.draft, self.dc)):
+            cache.free(range(self.B), status=self.status)
+            cache.reserve([n0] + [0] * (self.B - 1), status=self.status)
+            model.prefill(prompts[:1, :n0], cache, 0, need_logits=False, status=self.status)
+            if self.B > 1:
+                cache.fork([0] * (self.B - 1), range(1, self.B), [n0] * (self.B - 1), status=self.status)
+            cache.reserve([self.cap] * self.B, status=self.status)
+            for s0 in range(0, self.B, chunk):
+                n = min(chunk, self.B - s0)
+                piece = PieceLayout(self.B, s0, n, own, self.device)
+                piece.set(cache.lengths)
+                h = model.step(prompts[s0:s0 + n, n0:].reshape(-1), piece, cache, self._workspace(piece, model, cache),
+                               status=self.status, prefix=self.prefix)
+                if model is self.target:
+                    self.pending[s0:s0 + n] = model.logits(h[piece.last_rows()]).argmax(-1).int()
+                cache.lengths.add_(piece.q_len)
+
     # ------------------------------------------------------------------ one round
     def _round(self) -> None:
         k = self.k
@@ -119,18 +164,18 @@ class SpecDecEngine:
         first = torch.where(self.catch > 0, self.c_last, self.pending)
         tok0 = torch.stack([first, self.pending], dim=1).reshape(-1)
         self.L0.set(self.dc.lengths, q0)
-        h = draft.step(tok0, self.L0, self.dc, self.ws0, status=self.status)
+        h = draft.step(tok0, self.L0, self.dc, self.ws0, status=self.status, prefix=self.prefix)
         self.cands[:, 0] = draft.greedy(h[self.L0.last_rows()], self.dtok, self.lm_ws_d)
         self.dc.lengths.add_(q0)
         for i in range(1, k):
             self.L1.set(self.dc.lengths, act)
-            h = draft.step(self.cands[:, i - 1], self.L1, self.dc, self.ws1, status=self.status)
+            h = draft.step(self.cands[:, i - 1], self.L1, self.dc, self.ws1, status=self.status, prefix=self.prefix)
             self.cands[:, i] = draft.greedy(h, self.dtok, self.lm_ws_d)
             self.dc.lengths.add_(act)
         # 2. target verify of [pending, c1 .. ck]; g_j of every verify row (rows b (k+1) + j)
         vt = torch.cat([self.pending.unsqueeze(1), self.cands], dim=1).reshape(-1)
         self.LV.set(self.tc.lengths, act * (k + 1))
-        h = target.step(vt, self.LV, self.tc, self.wsv, status=self.status)
+        h = target.step(vt, self.LV, self.tc, self.wsv, status=self.status, prefix=self.prefix)
         target.greedy(h, self.g.view(-1), self.lm_ws_t)
         # 3. greedy accept from g (+ the target's rolled-back length len + 1 + m)
         ops.greedy_accept(None, row0=self.LV.q_row0, n_rows=self.LV.q_len, cands=self.cands, kp=self.kp,
@@ -161,6 +206,8 @@ class SpecDecEngine:
         """Record one round as a CUDA graph (after one eager warm-up round).  Capturing
         before ``prefill`` keeps it out of the decode: prefill resets every length and
         counter the warm-up touched."""
+        if self.shared:  # no sequence holds pages yet: a round of frozen sequences writes none
+            self.n_out.fill_(self.max_new)
         self._round()
         torch.cuda.synchronize()
         s = torch.cuda.Stream()
