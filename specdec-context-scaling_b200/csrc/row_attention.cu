@@ -42,6 +42,9 @@ constexpr int kUnitCost = 2;       // what a unit costs beside its blocks (query
 constexpr int kMinQuota = 4;       // smallest range of a CTA, in blocks
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
 constexpr float kRowRescaleLog2 = 8.f;
+constexpr int kItemsKept = 32;     // items of a CTA that it keeps in shared memory
+constexpr int kPolyPairs = 3;      // pairs of every eight whose exponentials are polynomials
+constexpr float kExpC0 = 0.999924541f, kExpC1 = 0.693136752f, kExpC2 = 0.242639482f, kExpC3 = 0.0558382832f;
 
 enum RowSource { kPacked = 0, kPaged = 1, kPagedE4M3 = 2 };
 // Threads, and registers a thread of the softmax warps and of the others: the launch's own are what
@@ -50,7 +53,7 @@ template <int SRC>
 struct RowRoles {
   static constexpr bool V8 = SRC == kPagedE4M3;
   static constexpr int THREADS = V8 ? 512 : 384;
-  static constexpr int SOFTMAX_REGS = V8 ? 176 : 200, OTHER_REGS = V8 ? 80 : 104;
+  static constexpr int SOFTMAX_REGS = V8 ? 184 : 208, OTHER_REGS = V8 ? 72 : 88;
   static_assert(256 * SOFTMAX_REGS + (THREADS - 256) * OTHER_REGS <= THREADS * (V8 ? 128 : 168), "register shares");
 };
 
@@ -394,19 +397,105 @@ template <int N>
 SD_DEV void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 SD_DEV void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// One lane of a converged warp; the loops around it stay warp-uniform, so that descriptors and counters live in
+// uniform registers.
+SD_DEV bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(ok));
+  return ok != 0;
+}
+
+// Two fp32 values in a 64-bit register: the packed arithmetic issues both at once.
+SD_DEV uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+SD_DEV void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+SD_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+SD_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SD_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+SD_DEV float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two finite x <= 8 on the FMA units: x = n + f with f in [-1/2, 1/2], 2^f by the cubic that is exact at
+// the four Chebyshev nodes of that interval (relative error below 2^-13, against the 2^-9 that P is rounded
+// to), n added to the exponent.  Below -126 it stays at 2^-126.
+SD_DEV void exp2_poly2(uint64_t x, float& a, float& b) {
+  constexpr float kRound = 12582912.f;  // 1.5 x 2^23: the sum's low mantissa bits are the nearest integer
+  float lo, hi;
+  unpack2(x, lo, hi);
+  const uint64_t xc = pack2(fmaxf(lo, -126.f), fmaxf(hi, -126.f));
+  const uint64_t t = add2(xc, pack2(kRound, kRound));
+  const uint64_t n = add2(t, pack2(-kRound, -kRound));
+  const uint64_t f = fma2(n, pack2(-1.f, -1.f), xc);
+  uint64_t y = fma2(f, pack2(kExpC3, kExpC3), pack2(kExpC2, kExpC2));
+  y = fma2(y, f, pack2(kExpC1, kExpC1));
+  y = fma2(y, f, pack2(kExpC0, kExpC0));
+  float tl, th, yl, yh;
+  unpack2(t, tl, th);
+  unpack2(y, yl, yh);
+  a = __uint_as_float((__float_as_uint(tl) << 23) + __float_as_uint(yl));
+  b = __uint_as_float((__float_as_uint(th) << 23) + __float_as_uint(yh));
+}
+
+// P of a row's 128 scores s (in registers) as bf16 over the score columns; returns the sum.  POLY: of every eight
+// pairs, kPolyPairs take the polynomial instead of the exponential unit.  `half` is called when the first 64 keys are written.
+template <bool POLY, typename Half>
+SD_DEV float row_probabilities(const float (&s)[128], float scale, float neg, uint32_t ta, Half half) {
+  const uint64_t sc = pack2(scale, scale), ng = pack2(neg, neg);
+  uint64_t sum[2] = {0, 0};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint64_t x = fma2(pack2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), sc, ng);
+      float a, b;
+      if (POLY && (e & 7) < kPolyPairs) {
+        exp2_poly2(x, a, b);
+      } else {
+        unpack2(x, a, b);
+        a = fast_exp2(a);
+        b = fast_exp2(b);
+      }
+      sum[e & 1] = add2(sum[e & 1], pack2(a, b));
+      w[e] = pack_bf16(a, b);
+    }
+    umma::tmem_st16_words(ta + 16 * c, w);
+    if (c == 1) half();
+  }
+  float a, b;
+  unpack2(add2(sum[0], sum[1]), a, b);
+  return a + b;
+}
 
 template <int D, int SRC>
-__global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kernel(const RowParams p,
-                                                                       const __grid_constant__ CUtensorMap kmap,
-                                                                       const __grid_constant__ CUtensorMap vmap) {
+__global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kernel(
+    const RowParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+    const __grid_constant__ CUtensorMap vmap) {
   constexpr bool V8 = RowRoles<SRC>::V8;
   using Geo = RowGeom<D, V8>;
   constexpr int NS = Geo::NS, KH = Geo::KH;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[NS], empty[NS], raw_full[2], raw_empty[2];
-  __shared__ uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], c_req, v_clean, fin;
-  __shared__ int32_t s_limit[kUnitRows];
+  __shared__ uint64_t q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], c_req, v_clean, fin;
+  __shared__ RowItem s_items[kItemsKept];  // the CTA's first items
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -416,13 +505,14 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
       mbar_init(&raw_full[t], 1);
       mbar_init(&raw_empty[t], 4);
     }
-    mbar_init(&q_full, 1);
-    mbar_init(&q_empty, 1 + 8);
+    mbar_init(&q_full, 2);
+    mbar_init(&q_empty, 1);
     mbar_init(&c_req, 1);
     mbar_init(&v_clean, 1);
     mbar_init(&fin, 1);
@@ -433,40 +523,56 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     umma::tmem_relinquish();
   }
   if (warp == 8 && lane == 0) {
+    prefetch_tmap(&qmap);
     prefetch_tmap(&kmap);
     prefetch_tmap(&vmap);
   }
   grid_dep_wait();
   grid_dep_launch();
+  const int i0 = p.cta_first[blockIdx.x], i1 = p.cta_last[blockIdx.x];
+  for (int e = tid; e < 3 * min(i1 - i0 + 1, kItemsKept); e += blockDim.x)
+    reinterpret_cast<int4*>(s_items)[e] = reinterpret_cast<const int4*>(p.items + i0)[e];
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = s_tmem;
-  const int i0 = p.cta_first[blockIdx.x], i1 = p.cta_last[blockIdx.x];
+  auto item_at = [&](int i) { return i - i0 < kItemsKept ? s_items[i - i0] : load_item(p.items + i); };
+
   if (warp < 8) {
     more_regs<RowRoles<SRC>::SOFTMAX_REGS>();
     // ------------------------------------------------------------ softmax and epilogue: a thread a row
     const int t = warp >> 2, row = tid & 127;
+    const int tok = row / p.n_rep, rep = row - tok * p.n_rep;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 5;
     const uint32_t s_ta = umma::taddr(tmem, lanes, Geo::S_COL + t * 128);
     const uint32_t o_ta = umma::taddr(tmem, lanes, Geo::O_COL + t * D);
     const float scale = p.scale_log2;
     const float grow = kRowRescaleLog2 / scale;
-    uint32_t sn = 0, items = 0, on = 0;
+    uint32_t sn = 0, on = 0;
     bool ok = true;
-    for (int i = i0; i <= i1 && ok; ++i) {
-      const RowItem it = load_item(p.items + i);
-      if (it.nblk == 0) continue;
-      ok = warp_wait(&q_full, items & 1);
-      if (!ok) break;
-      ++items;
-      const int limit = s_limit[t * kRowTile + row];
+    auto signal = [&](uint64_t* bar) {
+      umma::tmem_wait_st();
+      umma::fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_empty);
+      if (lane == 0) mbar_arrive(bar);
+    };
+    for (int i = i0; i <= i1 && ok; ++i) {
+      const RowItem it = item_at(i);
+      if (it.nblk == 0) continue;
+      // this row's visible keys end at `limit` (0: no row here)
+      const int vt = it.vt0 + t * p.tpt + tok;
+      int limit = 0;
+      if (tok < p.tpt && vt < it.n_vt) {
+        if (it.src >= 0) {
+          limit = min(it.first + vt + 1, it.k1);
+        } else {
+          const int mb = vt / p.q_max;
+          if (vt - mb * p.q_max < p.member_row[it.member0 + mb].y) limit = it.k1;
+        }
+      }
       const int nb = tile_blocks(p, it, t);
       if (nb == 0) {  // no tile, or a piece past the tile's keys: the row's other pieces are all of it
-        if (it.slot >= 0 && it.vt0 + t * p.tpt < it.n_vt && limit > 0)
-          p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
+        if (it.slot >= 0 && limit > 0) p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
         continue;
       }
       const bool any_row = __any_sync(0xffffffffu, limit > 0);
@@ -476,67 +582,59 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         ok = warp_wait(&s_full[t], sn & 1);
         if (!ok) break;
         umma::fence_after_sync();
-        if (any_row) {
-          float s[128];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) umma::tmem_ld32(s_ta + 32 * c, s + 32 * c);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) umma::tmem_wait_ld32(s + 32 * c);
-          const int key0 = it.k0 + j * kKeyBlock;
-          if (least < key0 + kKeyBlock) {
-            const int vis = limit - key0;
-#pragma unroll
-            for (int c = 0; c < 128; ++c) s[c] = c < vis ? s[c] : -INFINITY;
+        if (!any_row) {
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&p_half[t]);
+            mbar_arrive(&p_full[t]);
           }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int c = 4; c < 124; c += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(s[c + e], s[c + 4 + e]));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[124 + e]);
-          const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          if (j == 0) {
-            m = bm;
-          } else {
-            const bool need = bm > m + grow;
-            if (__any_sync(0xffffffffu, need)) {
-              const float alpha = need ? fast_exp2((m - bm) * scale) : 1.f;
-              if (need) m = bm;
-              l *= alpha;
-#pragma unroll
-              for (int c = 0; c < D; c += 32) {
-                float o[32];
-                umma::tmem_ld32(o_ta + c, o);
-                umma::tmem_wait_ld32(o);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= alpha;
-                umma::tmem_st16(o_ta + c, reinterpret_cast<const float(&)[16]>(o[0]));
-                umma::tmem_st16(o_ta + c + 16, reinterpret_cast<const float(&)[16]>(o[16]));
-              }
-            }
-          }
-          const float neg = m == -INFINITY ? 0.f : -m * scale;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float a = fast_exp2(fmaf(s[32 * c + 2 * e], scale, neg));
-              const float b = fast_exp2(fmaf(s[32 * c + 2 * e + 1], scale, neg));
-              sum[(2 * e) & 3] += a;
-              sum[(2 * e + 1) & 3] += b;
-              w[e] = pack_bf16(a, b);
-            }
-            umma::tmem_st16_words(s_ta + 16 * c, w);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          umma::tmem_wait_st();
+          continue;
         }
-        umma::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        float s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) umma::tmem_ld32(s_ta + 32 * c, s + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) umma::tmem_wait_ld32(s + 32 * c);
+        const int key0 = it.k0 + j * kKeyBlock;
+        const bool masked = least < key0 + kKeyBlock;
+        if (masked) {
+          const int vis = limit - key0;
+#pragma unroll
+          for (int c = 0; c < 128; ++c) s[c] = c < vis ? s[c] : -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < 124; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3_nan(mx[e], s[c + e], s[c + 4 + e]);
+        const float bm = max3_nan(max3_nan(mx[0], mx[1], s[124]), max3_nan(mx[2], mx[3], s[125]), max_nan(s[126], s[127]));
+        const bool need = j > 0 && !(bm <= m + grow);  // a NaN, too
+        if (j == 0) m = bm;
+        bool plain = masked;
+        if (__any_sync(0xffffffffu, need || !(fabsf(m) < INFINITY))) {
+          if (j > 0) {
+            const float alpha = need ? fast_exp2((m - bm) * scale) : 1.f;
+            if (need) m = bm;
+            l *= alpha;
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
+              umma::tmem_ld32(o_ta + c, o);
+              umma::tmem_wait_ld32(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= alpha;
+              umma::tmem_st16(o_ta + c, reinterpret_cast<const float(&)[16]>(o[0]));
+              umma::tmem_st16(o_ta + c + 16, reinterpret_cast<const float(&)[16]>(o[16]));
+            }
+          }
+          // infinite and NaN scores go through the exponential unit, which knows them
+          plain = plain || __any_sync(0xffffffffu, !(fabsf(m) < INFINITY));
+        }
+        const float neg = m == -INFINITY ? 0.f : -m * scale;
+        auto half = [&]() { signal(&p_half[t]); };
+        l += plain ? row_probabilities<false>(s, scale, neg, s_ta, half)
+                   : row_probabilities<true>(s, scale, neg, s_ta, half);
+        signal(&p_full[t]);
       }
       if (!ok) break;
       ok = warp_wait(&o_full[t], on & 1);
@@ -544,11 +642,10 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       ++on;
       umma::fence_after_sync();
       if (any_row) {
-        const int tok = row / p.n_rep;
         if (it.slot < 0) {
           const float inv = l == 0.f ? 0.f : 1.f / l;
-          const int64_t at = static_cast<int64_t>(it.row0 + it.vt0 + t * p.tpt + tok) * p.o_st +
-                             static_cast<int64_t>(it.head * p.n_rep + row - tok * p.n_rep) * p.o_sh;
+          const int64_t at = static_cast<int64_t>(it.row0 + vt) * p.o_st +
+                             static_cast<int64_t>(it.head * p.n_rep + rep) * p.o_sh;
 #pragma unroll
           for (int c = 0; c < D; c += 32) {
             float o[32];
@@ -577,308 +674,328 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             }
           }
         }
+        umma::fence_before_sync();  // O is read: the arrival for the next item's first block lets its MMAs write it
       }
     }
     if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
   } else {
-  fewer_regs<RowRoles<SRC>::OTHER_REGS>();
-  if (warp == 8) {
-    // ------------------------------------------------------------ K/V blocks
-    uint32_t n = 0;  // blocks issued (K and V each count)
-    bool ok = true;
-    for (int i = i0; i <= i1 && ok; ++i) {
-      const RowItem it = load_item(p.items + i);
-      if (it.nblk == 0) continue;
-      const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
-      int ids = 0;  // paged: lane l holds the page of keys 16 (32 (j / 4) + l) ..
-      for (int j = 0; j < nb && ok; ++j) {
-        if (SRC != kPacked && (j & 3) == 0) {
-          const int last = (it.k1 - 1) / kPage;
-          const int pg = min(it.k0 / kPage + 8 * j + lane, last);
-          ids = p.page_table[static_cast<int64_t>(it.kv) * p.max_pages + pg];
-          if (ids < 0 || ids >= p.num_pages) {
-            raise_status(p.status, SPECDEC_STATUS_BAD_PAGE);
-            ids = 0;
+    fewer_regs<RowRoles<SRC>::OTHER_REGS>();
+    if (warp == 8) {
+      // ---------------------------------------------------------- K/V blocks
+      uint32_t n = 0;  // blocks issued (K and V each count)
+      bool ok = true;
+      for (int i = i0; i <= i1 && ok; ++i) {
+        const RowItem it = item_at(i);
+        if (it.nblk == 0) continue;
+        const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+        int ids = 0;  // paged: lane l holds the page of keys 16 (32 (j / 4) + l) ..
+        for (int j = 0; j < nb && ok; ++j) {
+          if (SRC != kPacked && (j & 3) == 0) {
+            const int last = (it.k1 - 1) / kPage;
+            const int pg = min(it.k0 / kPage + 8 * j + lane, last);
+            ids = p.page_table[static_cast<int64_t>(it.kv) * p.max_pages + pg];
+            if (ids < 0 || ids >= p.num_pages) {
+              raise_status(p.status, SPECDEC_STATUS_BAD_PAGE);
+              ids = 0;
+            }
           }
-        }
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++n) {
-          const uint32_t s = n % NS, round = n / NS;
-          if (V8 && kv) {  // codes; the widening warps take care of the block's ring slot
-            const uint32_t b = (n >> 1) & 1, r = n >> 2;
-            if (r > 0 && !warp_wait(&raw_empty[b], (r - 1) & 1)) {
+          for (int kv = 0; kv < 2; ++kv, ++n) {
+            const uint32_t s = n % NS, round = n / NS;
+            if (V8 && kv) {  // codes; the widening warps take care of the block's ring slot
+              const uint32_t b = (n >> 1) & 1, r = n >> 2;
+              if (r > 0 && !warp_wait(&raw_empty[b], (r - 1) & 1)) {
+                ok = false;
+                break;
+              }
+              int pg[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) pg[e] = __shfl_sync(0xffffffffu, ids, 8 * (j & 3) + e) * p.KV + it.head;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&raw_full[b], 16384);
+#pragma unroll
+                for (int e = 0; e < 8; e += 4)
+                  tma_rows4(smem + Geo::RAW + b * 16384 + e * 2048, &vmap, pg[e], pg[e + 1], pg[e + 2], pg[e + 3],
+                            &raw_full[b]);
+              }
+              __syncwarp();
+              continue;
+            }
+            if (round > 0 && !warp_wait(&empty[s], (round - 1) & 1)) {
               ok = false;
               break;
             }
-            int pg[8];
+            uint8_t* dst = smem + Geo::RING + s * Geo::TILE;
+            const CUtensorMap* map = kv ? &vmap : &kmap;
+            if (SRC == kPacked) {
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&full[s], Geo::TILE);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) pg[e] = __shfl_sync(0xffffffffu, ids, 8 * (j & 3) + e) * p.KV + it.head;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&raw_full[b], 16384);
+                for (int x = 0; x < KH; ++x)
+                  tma_tile_3d(dst + x * 16384, map, x * 64, it.head, it.kv + it.k0 + j * kKeyBlock, &full[s]);
+              }
+            } else {
+              int pg[8];
 #pragma unroll
-              for (int e = 0; e < 8; e += 4)
-                tma_rows4(smem + Geo::RAW + b * 16384 + e * 2048, &vmap, pg[e], pg[e + 1], pg[e + 2], pg[e + 3],
-                          &raw_full[b]);
+              for (int e = 0; e < 8; ++e) pg[e] = __shfl_sync(0xffffffffu, ids, 8 * (j & 3) + e);
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&full[s], Geo::TILE);
+#pragma unroll
+                for (int x = 0; x < KH; ++x)
+#pragma unroll
+                  for (int e = 0; e < 8; e += 4) {
+                    auto row = [&](int k) { return (pg[k] * p.KV + it.head) * KH + x; };
+                    tma_rows4(dst + x * 16384 + e * 2048, map, row(e), row(e + 1), row(e + 2), row(e + 3), &full[s]);
+                  }
+              }
             }
             __syncwarp();
-            continue;
           }
-          if (round > 0 && !warp_wait(&empty[s], (round - 1) & 1)) {
-            ok = false;
-            break;
-          }
-          uint8_t* dst = smem + Geo::RING + s * Geo::TILE;
-          const CUtensorMap* map = kv ? &vmap : &kmap;
-          if (SRC == kPacked) {
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&full[s], Geo::TILE);
-#pragma unroll
-              for (int x = 0; x < KH; ++x)
-                tma_tile_3d(dst + x * 16384, map, x * 64, it.head, it.kv + it.k0 + j * kKeyBlock, &full[s]);
-            }
-          } else {
-            int pg[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) pg[e] = __shfl_sync(0xffffffffu, ids, 8 * (j & 3) + e);
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&full[s], Geo::TILE);
-#pragma unroll
-              for (int x = 0; x < KH; ++x)
-#pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                  auto row = [&](int k) { return (pg[k] * p.KV + it.head) * KH + x; };
-                  tma_rows4(dst + x * 16384 + e * 2048, map, row(e), row(e + 1), row(e + 2), row(e + 3), &full[s]);
-                }
-            }
-          }
-          __syncwarp();
         }
       }
-    }
-    if (!ok) {
-      if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-      // copies under way land before the CTA leaves
-      for (uint32_t k = n > NS ? n - NS : 0; k < n; ++k)
-        (void)(V8 && (k & 1) ? warp_wait(&raw_full[(k >> 1) & 1], (k >> 2) & 1) : warp_wait(&full[k % NS], (k / NS) & 1));
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issue
-    if (lane == 0) {
+      if (!ok) {
+        if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+        // copies under way land before the CTA leaves
+        for (uint32_t k = n > NS ? n - NS : 0; k < n; ++k)
+          (void)(V8 && (k & 1) ? warp_wait(&raw_full[(k >> 1) & 1], (k >> 2) & 1) : warp_wait(&full[k % NS], (k / NS) & 1));
+      }
+    } else if (warp == 9) {
+      // ---------------------------------------------------------- MMA issue
       constexpr uint32_t id_qk = umma::idesc_f16(128, kKeyBlock, true, true, false, false);
       constexpr uint32_t id_pv = umma::idesc_f16(128, D, true, true, false, true);
-      const uint32_t q_base = smem_u32(smem), ring = smem_u32(smem + Geo::RING);
-      uint32_t n = 0, pn[2] = {0, 0}, items = 0, cleaned = 0;
+      // a descriptor's low bits are the address in units of 16 bytes
+      const uint64_t q_desc = umma::desc_kmajor_sw128(smem_u32(smem));
+      const uint64_t k_desc = umma::desc_kmajor_sw128(smem_u32(smem + Geo::RING));
+      const uint64_t v_desc = umma::desc_mnmajor_sw128(smem_u32(smem + Geo::RING), 16384);
+      const uint32_t s_col[2] = {umma::taddr(tmem, 0, Geo::S_COL), umma::taddr(tmem, 0, Geo::S_COL + 128)};
+      const uint32_t o_col[2] = {umma::taddr(tmem, 0, Geo::O_COL), umma::taddr(tmem, 0, Geo::O_COL + D)};
+      uint32_t pn[2] = {0, 0}, items = 0, cleaned = 0;
+      uint32_t ks = 0, kp = 0;  // ring slot of the next K block, and its phase
       bool ok = true;
-      auto slot_ready = [&](uint32_t k) { return mbar_wait(&full[k % NS], (k / NS) & 1); };
-      auto qk = [&](int t, uint32_t k) {
-        const uint32_t qa = q_base + t * Geo::TILE, ka = ring + (k % NS) * Geo::TILE;
+      auto next = [&](uint32_t& s, uint32_t& ph) {
+        if (++s == NS) s = 0, ph ^= 1;
+      };
+      auto qk = [&](int t, uint32_t slot) {
+        if (elect_one()) {
+          const uint64_t qd = q_desc + t * (Geo::TILE >> 4), kd = k_desc + slot * (Geo::TILE >> 4);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t at = (kk >> 2) * 16384 + (kk & 3) * 32;
-          umma::mma_f16_ss(umma::taddr(tmem, 0, Geo::S_COL + t * 128), umma::desc_kmajor_sw128(qa + at),
-                           umma::desc_kmajor_sw128(ka + at), id_qk, kk > 0);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t at = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+            umma::mma_f16_ss(s_col[t], qd + at, kd + at, id_qk, kk > 0);
+          }
+          umma::commit(&s_full[t]);
         }
-        umma::commit(&s_full[t]);
+        __syncwarp();
+      };
+      auto pv = [&](int t, uint32_t slot, int h, bool acc) {  // half h of the block's keys
+        if (elect_one()) {
+          const uint64_t vd = v_desc + slot * (Geo::TILE >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kKeyBlock / 32; ++kk) {
+            const int k = h * (kKeyBlock / 32) + kk;
+            umma::mma_f16_ts(o_col[t], s_col[t] + k * 8, vd + k * (2048 >> 4), id_pv, acc || k > 0);
+          }
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) umma::commit(bar);
+        __syncwarp();
       };
       for (int i = i0; i <= i1 && ok; ++i) {
-        const RowItem it = load_item(p.items + i);
+        const RowItem it = item_at(i);
         if (it.nblk == 0) continue;
         const int nt[2] = {tile_blocks(p, it, 0), tile_blocks(p, it, 1)};
         const int nb = max(nt[0], nt[1]);
         const bool clean = !V8 && (it.k1 - it.k0) % kKeyBlock != 0;
-        ok = mbar_wait(&q_full, items & 1) && slot_ready(n);
+        ok = warp_wait(&q_full, items & 1) && warp_wait(&full[ks], kp);
         if (!ok) break;
         umma::fence_after_sync();
-        if (nt[0] > 0) qk(0, n);
-        if (nt[1] > 0) qk(1, n);
-        if (nb == 1) umma::commit(&q_empty);
-        umma::commit(&empty[n % NS]);
+        if (nt[0] > 0) qk(0, ks);
+        if (nt[1] > 0) qk(1, ks);
+        if (nb == 1) commit(&q_empty);
+        commit(&empty[ks]);
+        next(ks, kp);
         for (int j = 0; j < nb && ok; ++j) {
-          const uint32_t kv = n + 2 * j + 1, kn = kv + 1;  // this block's V, the next block's K
-          bool v_in = false, k_in = false;
+          const uint32_t vs = ks, vp = kp;  // this block's V; then the next block's K
+          next(ks, kp);
+          ok = warp_wait(&full[vs], vp);
+          const bool last = j == nb - 1, wash = clean && last;
+          // the last block's V is zeroed past the last key while the softmax works on the block
+          if (wash && ok) {
+            if (lane == 0) mbar_arrive(&c_req);
+            __syncwarp();
+          }
+          bool washed = !wash, k_in = false;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (j >= nt[t]) continue;
-            if (!v_in) {
-              ok = ok && slot_ready(kv);
-              // the last block's V is zeroed past the last key while the softmax works on the block
-              if (ok && clean && j == nb - 1) mbar_arrive(&c_req);
+            if (j >= nt[t] || !ok) continue;
+            ok = warp_wait(&p_half[t], pn[t] & 1);
+            if (!washed) {
+              ok = ok && warp_wait(&v_clean, cleaned & 1);
+              ++cleaned;
+              washed = true;
             }
-            ok = ok && mbar_wait(&p_full[t], pn[t] & 1);
-            if (!v_in && clean && j == nb - 1) ok = ok && mbar_wait(&v_clean, cleaned++ & 1);
-            v_in = true;
-            if (!ok) break;
+            if (!ok) continue;
+            umma::fence_after_sync();
+            pv(t, vs, 0, j > 0);
+            ok = warp_wait(&p_full[t], pn[t] & 1);
+            if (!ok) continue;
             ++pn[t];
             umma::fence_after_sync();
-            const uint32_t va = ring + (kv % NS) * Geo::TILE;
-#pragma unroll
-            for (int kk = 0; kk < kKeyBlock / 16; ++kk)
-              umma::mma_f16_ts(umma::taddr(tmem, 0, Geo::O_COL + t * D),
-                               umma::taddr(tmem, 0, Geo::S_COL + t * 128 + kk * 8),
-                               umma::desc_mnmajor_sw128(va + kk * 2048, 16384), id_pv, j > 0 || kk > 0);
+            pv(t, vs, 1, true);
             if (j == nt[t] - 1) {
-              umma::commit(&o_full[t]);
+              commit(&o_full[t]);
             } else {
               if (!k_in) {
-                ok = slot_ready(kn);
+                ok = warp_wait(&full[ks], kp);
+                if (!ok) continue;
                 k_in = true;
-                if (!ok) break;
                 umma::fence_after_sync();
               }
-              qk(t, kn);
+              qk(t, ks);
             }
           }
           if (!ok) break;
-          umma::commit(&empty[kv % NS]);
-          if (j + 1 < nb) {
-            umma::commit(&empty[kn % NS]);
-            if (j + 2 == nb) umma::commit(&q_empty);
+          commit(&empty[vs]);
+          if (!last) {
+            commit(&empty[ks]);
+            if (j + 2 == nb) commit(&q_empty);
+            next(ks, kp);
           }
         }
-        n += 2 * nb;
         ++items;
       }
-      if (!ok) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-      umma::commit(&fin);
-      (void)mbar_wait(&fin, 0);
-    }
-    __syncwarp();
-  } else if (warp == 10) {
-    // ------------------------------------------------------------ query rows and limits
-    constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte chunks of a row, rows a step
-    const uint32_t q_base = smem_u32(smem);
-    uint32_t items = 0;
-    for (int i = i0; i <= i1; ++i) {
-      const RowItem it = load_item(p.items + i);
-      if (it.nblk == 0) continue;
-      const int tiles = it.vt0 + p.tpt < it.n_vt ? 2 : 1;
-      if (items > 0 && !warp_wait(&q_empty, (items - 1) & 1)) {
-        if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-        break;
-      }
-      for (int base = 0; base < tiles * kRowTile; base += 32) {
-        const int t = base / kRowTile, r = base % kRowTile + lane;
-        const int tok = r / p.n_rep, vt = it.vt0 + t * p.tpt + tok;
-        int64_t off = -1;
-        int limit = 0;
-        if (tok < p.tpt && vt < it.n_vt) {
-          int row = -1;
-          if (it.src >= 0) {
-            row = it.row0 + vt;
-            limit = min(it.first + vt + 1, it.k1);
-          } else {
-            const int m = vt / p.q_max, e = vt - m * p.q_max;
-            const int2 mr = p.member_row[it.member0 + m];
-            if (e < mr.y) {
-              row = mr.x + e;
-              limit = it.k1;
-            }
-          }
-          if (row >= 0)
-            off = static_cast<int64_t>(row) * p.q_st +
-                  static_cast<int64_t>(it.head * p.n_rep + r - tok * p.n_rep) * p.q_sh;
-        }
-        s_limit[base + lane] = limit;
-#pragma unroll 4
-        for (int e = 0; e < 32; e += RP) {
-          const int64_t o = __shfl_sync(0xffffffffu, off, e + lane / CH);
-          const int rr = base % kRowTile + e + lane / CH, ch = lane % CH;
-          const uint32_t dst =
-              q_base + t * Geo::TILE + (ch >> 3) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
-          cp_async16(dst, p.q + (o < 0 ? 0 : o + ch * 8), o < 0 ? 0u : 16u);
-        }
-      }
-      cp_async_wait_all();
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full);
-      ++items;
-    }
-    cp_async_wait_all();
-  } else if (warp >= 12) {
-    // ------------------------------------------------------------ E4M3: codes to bf16, a thread a key
-    if constexpr (V8) {
-      const int r = tid - 384;
-      uint32_t n = 1;
+      if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      commit(&fin);
+      (void)warp_wait(&fin, 0);
+    } else if (warp == 10 || warp == 11) {
+      // ---------------------------------------------------------- query rows; V rows past the last key (warp 11)
+      const int t = warp - 10;
+      uint32_t items = 0, cleaned = 0, n = 0;
       bool ok = true;
       for (int i = i0; i <= i1 && ok; ++i) {
-        const RowItem it = load_item(p.items + i);
+        const RowItem it = item_at(i);
         if (it.nblk == 0) continue;
-        const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
-        // the scale of key r of block j; 0 past the last key, where the codes (clamped pages) are finite or NaN
-        auto scale_of = [&](int j) {
-          const int key = it.k0 + j * kKeyBlock + r;
-          if (key >= it.k1) return 0.f;
-          int page = p.page_table[static_cast<int64_t>(it.kv) * p.max_pages + key / kPage];
-          if (page < 0 || page >= p.num_pages) page = 0;  // the loading warp reports it
-          return p.v_scale[(static_cast<int64_t>(page) * p.KV + it.head) * kPage + key % kPage];
-        };
-        float next = scale_of(0);
-        for (int j = 0; j < nb; ++j, n += 2) {
-          const float sc = next;
-          const bool in = it.k0 + j * kKeyBlock + r < it.k1;
-          if (j + 1 < nb) next = scale_of(j + 1);
-          const uint32_t s = n % NS, b = (n >> 1) & 1;
-          ok = warp_wait(&raw_full[b], (n >> 2) & 1);
-          if (ok && n >= NS) ok = warp_wait(&empty[s], (n / NS - 1) & 1);
-          if (!ok) break;
-          const uint8_t* src = smem + Geo::RAW + b * 16384 + r * 128;
-          uint8_t* dst = smem + Geo::RING + s * Geo::TILE + r * 128;
+        const int tiles = it.vt0 + p.tpt < it.n_vt ? 2 : 1;
+        if (items > 0) ok = warp_wait(&q_empty, (items - 1) & 1);
+        if (!ok) break;
+        ++items;
+        if (it.src >= 0) {  // a sequence's rows are a box of n_rep heads x tpt tokens; rows past it meet no other row
+          if (t == 0 && lane == 0) {
+            mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(tiles * KH * 128 * p.n_rep * p.tpt));
+            for (int e = 0; e < tiles; ++e)
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const int ch = (c + r) & 7;  // rotated, so that neighbouring keys use different banks
-            const uint4 x = *reinterpret_cast<const uint4*>(src + ch * 16);
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            uint32_t y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint32_t h = e4m3x2_to_f16x2(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-              y[e] = in ? pack_bf16(f.x * sc, f.y * sc) : 0u;
-            }
-            uint8_t* d = dst + (ch >> 2) * 16384;
-            const int g = (ch & 3) * 2;
-            *reinterpret_cast<uint4*>(d + ((g ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<uint4*>(d + (((g + 1) ^ (r & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+              for (int x = 0; x < KH; ++x)
+                tma_tile_3d(smem + e * Geo::TILE + x * 16384, &qmap, x * 64, it.head * p.n_rep,
+                            it.row0 + it.vt0 + e * p.tpt, &q_full);
+          } else if (t == 1 && lane == 0) {
+            mbar_arrive(&q_full);
           }
+        } else {
+          // a group's rows are anywhere: 16 bytes a lane, tile t by warp 10 + t
+          constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte chunks of a row, rows a step
+          const uint32_t q_base = smem_u32(smem) + t * Geo::TILE;
+          for (int base = 0; base < (t < tiles ? kRowTile : 0); base += 32) {
+            const int r = base + lane, tok = r / p.n_rep, vt = it.vt0 + t * p.tpt + tok;
+            int64_t off = -1;
+            if (tok < p.tpt && vt < it.n_vt) {
+              const int mb = vt / p.q_max, e = vt - mb * p.q_max;
+              const int2 mr = p.member_row[it.member0 + mb];
+              if (e < mr.y)
+                off = static_cast<int64_t>(mr.x + e) * p.q_st +
+                      static_cast<int64_t>(it.head * p.n_rep + r - tok * p.n_rep) * p.q_sh;
+            }
+#pragma unroll 4
+            for (int e = 0; e < 32; e += RP) {
+              const int64_t o = __shfl_sync(0xffffffffu, off, e + lane / CH);
+              const int rr = base + e + lane / CH, ch = lane % CH;
+              cp_async16(q_base + (ch >> 3) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4),
+                         p.q + (o < 0 ? 0 : o + ch * 8), o < 0 ? 0u : 16u);
+            }
+          }
+          cp_async_wait_all();
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&full[s]);
-            mbar_arrive(&raw_empty[b]);
-          }
+          if (lane == 0) mbar_arrive(&q_full);
         }
+        const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+        const int rem = (it.k1 - it.k0) % kKeyBlock;
+        if (t == 1 && !V8 && rem != 0) {
+          const uint32_t k = n + 2 * nb - 1;
+          // asked for by the MMA warp, which has seen the block arrive and waits for the answer
+          ok = warp_wait(&c_req, cleaned & 1);
+          if (!ok) break;
+          uint8_t* v = smem + Geo::RING + (k % NS) * Geo::TILE;
+#pragma unroll
+          for (int x = 0; x < KH; ++x)
+            for (int o = rem * 128 + lane * 16; o < 16384; o += 512)
+              *reinterpret_cast<uint4*>(v + x * 16384 + o) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_clean);
+          ++cleaned;
+        }
+        n += 2 * nb;
       }
       if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-    }
-  } else if (warp == 11 && !V8) {
-    // ------------------------------------------------------------ V rows past the last key
-    uint32_t n = 0, cleaned = 0;
-    for (int i = i0; i <= i1; ++i) {
-      const RowItem it = load_item(p.items + i);
-      if (it.nblk == 0) continue;
-      const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
-      const int rem = (it.k1 - it.k0) % kKeyBlock;
-      if (rem != 0) {
-        const uint32_t k = n + 2 * nb - 1;
-        // asked for by the MMA warp, which has seen the block arrive and waits for the answer
-        if (!warp_wait(&c_req, cleaned & 1)) {
-          if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-          break;
-        }
-        uint8_t* v = smem + Geo::RING + (k % NS) * Geo::TILE;
+    } else {
+      // ---------------------------------------------------------- E4M3: codes to bf16, a thread a key
+      if constexpr (V8) {
+        const int r = tid - 384;
+        uint32_t n = 1;
+        bool ok = true;
+        for (int i = i0; i <= i1 && ok; ++i) {
+          const RowItem it = item_at(i);
+          if (it.nblk == 0) continue;
+          const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+          // the scale of key r of block j; 0 past the last key, where the codes (clamped pages) are finite or NaN
+          auto scale_of = [&](int j) {
+            const int key = it.k0 + j * kKeyBlock + r;
+            if (key >= it.k1) return 0.f;
+            int page = p.page_table[static_cast<int64_t>(it.kv) * p.max_pages + key / kPage];
+            if (page < 0 || page >= p.num_pages) page = 0;  // the loading warp reports it
+            return p.v_scale[(static_cast<int64_t>(page) * p.KV + it.head) * kPage + key % kPage];
+          };
+          float next = scale_of(0);
+          for (int j = 0; j < nb; ++j, n += 2) {
+            const float sc = next;
+            const bool in = it.k0 + j * kKeyBlock + r < it.k1;
+            if (j + 1 < nb) next = scale_of(j + 1);
+            const uint32_t s = n % NS, b = (n >> 1) & 1;
+            ok = warp_wait(&raw_full[b], (n >> 2) & 1);
+            if (ok && n >= NS) ok = warp_wait(&empty[s], (n / NS - 1) & 1);
+            if (!ok) break;
+            const uint8_t* src = smem + Geo::RAW + b * 16384 + r * 128;
+            uint8_t* dst = smem + Geo::RING + s * Geo::TILE + r * 128;
 #pragma unroll
-        for (int x = 0; x < KH; ++x)
-          for (int o = rem * 128 + lane * 16; o < 16384; o += 512)
-            *reinterpret_cast<uint4*>(v + x * 16384 + o) = make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_clean);
-        ++cleaned;
+            for (int c = 0; c < 8; ++c) {
+              const int ch = (c + r) & 7;  // rotated, so that neighbouring keys use different banks
+              const uint4 x = *reinterpret_cast<const uint4*>(src + ch * 16);
+              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+              uint32_t y[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t h = e4m3x2_to_f16x2(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                y[e] = in ? pack_bf16(f.x * sc, f.y * sc) : 0u;
+              }
+              uint8_t* d = dst + (ch >> 2) * 16384;
+              const int g = (ch & 3) * 2;
+              *reinterpret_cast<uint4*>(d + ((g ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+              *reinterpret_cast<uint4*>(d + (((g + 1) ^ (r & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&full[s]);
+              mbar_arrive(&raw_empty[b]);
+            }
+          }
+        }
+        if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
       }
-      n += 2 * nb;
     }
-  }
   }
   umma::fence_before_sync();
   __syncthreads();
@@ -1081,7 +1198,8 @@ static int check_rows(const void* q, const void* out, int64_t qs, int64_t qh, in
   if (!q || !out) return fail(SPECDEC_ERR_INVALID, "q and out must be device pointers");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u)
     return fail(SPECDEC_ERR_INVALID, "q/out must be 16-byte aligned");
-  if ((qs | qh | os | oh) & 7) return fail(SPECDEC_ERR_INVALID, "q/out strides must be multiples of 8 elements");
+  if ((qs | qh | os | oh) & 7 || qs <= 0 || qh <= 0 || qs >= (int64_t(1) << 38) || qh >= (int64_t(1) << 38))
+    return fail(SPECDEC_ERR_INVALID, "q/out strides must be positive multiples of 8 elements");
   return SPECDEC_OK;
 }
 
@@ -1126,8 +1244,8 @@ static int fill_row_params(RowParams& p, const RowShape& s, void* ws, size_t ws_
 }
 
 template <int D, int SRC>
-static int launch_row_attention(const RowParams& p, const CUtensorMap& kmap, const CUtensorMap& vmap, bool reuse_plan,
-                                cudaStream_t st) {
+static int launch_row_attention(const RowParams& p, const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                                bool reuse_plan, cudaStream_t st) {
   // the attribute belongs to the function on each device; setting it again is cheap and needs no state of its own
   const cudaError_t e = cudaFuncSetAttribute(row_attention_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              RowGeom<D, RowRoles<SRC>::V8>::SMEM);
@@ -1135,7 +1253,7 @@ static int launch_row_attention(const RowParams& p, const CUtensorMap& kmap, con
   if (!reuse_plan)
     if (int rc = launch_pdl("row_plan_kernel", row_plan_kernel, dim3(1), dim3(1024), 0, st, p)) return rc;
   if (int rc = launch_pdl("row_attention_kernel", row_attention_kernel<D, SRC>, dim3(p.grid), dim3(RowRoles<SRC>::THREADS),
-                          RowGeom<D, RowRoles<SRC>::V8>::SMEM, st, p, kmap, vmap))
+                          RowGeom<D, RowRoles<SRC>::V8>::SMEM, st, p, qmap, kmap, vmap))
     return rc;
   if (p.G == 0)
     return launch_pdl("join_cut_kernel", join_cut_kernel<D>, dim3(p.grid, kMergeParts), dim3(256), 0, st, p);
@@ -1144,13 +1262,15 @@ static int launch_row_attention(const RowParams& p, const CUtensorMap& kmap, con
                     0, st, p);
 }
 
-// 3-D map {D, heads, rows} over packed rows with a {64, 1, 128} box and 128-byte swizzle; rows past the end read as zero
-static int encode_packed_map(CUtensorMap* map, const void* base, int64_t rows, int heads, int D, int64_t st, int64_t sh) {
+// 3-D map {D, heads, rows} over packed rows with a {64, box_heads, box_rows} box and 128-byte swizzle; rows past the
+// end read as zero
+static int encode_packed_map(CUtensorMap* map, const void* base, int64_t rows, int heads, int D, int64_t st, int64_t sh,
+                             int box_heads, int box_rows) {
   auto fn = get_encode_fn();
   if (!fn) return fail(SPECDEC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(st) * 2};
-  cuuint32_t box[3] = {64, 1, kKeyBlock};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1200,12 +1320,13 @@ extern "C" int specdec_prompt_attention(const SpecdecPromptArgs* a, specdec_stre
   p.q_rows = a->q_rows;
   p.kv_rows = a->kv_rows;
   p.status = a->status;
-  CUtensorMap km, vm;
-  if (int rc = encode_packed_map(&km, a->k, a->kv_rows, s.KV, s.D, a->k_stride_tok, a->k_stride_head)) return rc;
-  if (int rc = encode_packed_map(&vm, a->v, a->kv_rows, s.KV, s.D, a->v_stride_tok, a->v_stride_head)) return rc;
+  CUtensorMap qm, km, vm;
+  if (int rc = encode_packed_map(&qm, a->q, a->q_rows, s.H, s.D, a->q_stride_tok, a->q_stride_head, p.n_rep, p.tpt)) return rc;
+  if (int rc = encode_packed_map(&km, a->k, a->kv_rows, s.KV, s.D, a->k_stride_tok, a->k_stride_head, 1, kKeyBlock)) return rc;
+  if (int rc = encode_packed_map(&vm, a->v, a->kv_rows, s.KV, s.D, a->v_stride_tok, a->v_stride_head, 1, kKeyBlock)) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return s.D == 128 ? launch_row_attention<128, kPacked>(p, km, vm, a->reuse_plan != 0, st)
-                    : launch_row_attention<64, kPacked>(p, km, vm, a->reuse_plan != 0, st);
+  return s.D == 128 ? launch_row_attention<128, kPacked>(p, qm, km, vm, a->reuse_plan != 0, st)
+                    : launch_row_attention<64, kPacked>(p, qm, km, vm, a->reuse_plan != 0, st);
 }
 
 extern "C" size_t specdec_shared_prefix_workspace_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
@@ -1260,11 +1381,12 @@ extern "C" int specdec_shared_prefix_attention(const SpecdecSharedPrefixArgs* a,
   p.v_scale = kv.v_scale;
   p.q_rows = a->q_rows;
   p.status = a->status;
-  CUtensorMap km, vm;
+  CUtensorMap qm, km, vm;
+  if (int rc = encode_packed_map(&qm, a->q, a->q_rows, s.H, s.D, a->q_stride_tok, a->q_stride_head, p.n_rep, p.tpt)) return rc;
   if (int rc = encode_rows_map(&km, kv.k_pool, static_cast<uint64_t>(page_rows), 2048)) return rc;
   if (int rc = encode_rows_map(&vm, kv.v_pool, static_cast<uint64_t>(v8 ? page_rows / 2 : page_rows), 2048)) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (v8) return launch_row_attention<128, kPagedE4M3>(p, km, vm, a->reuse_plan != 0, st);
-  return s.D == 128 ? launch_row_attention<128, kPaged>(p, km, vm, a->reuse_plan != 0, st)
-                    : launch_row_attention<64, kPaged>(p, km, vm, a->reuse_plan != 0, st);
+  if (v8) return launch_row_attention<128, kPagedE4M3>(p, qm, km, vm, a->reuse_plan != 0, st);
+  return s.D == 128 ? launch_row_attention<128, kPaged>(p, qm, km, vm, a->reuse_plan != 0, st)
+                    : launch_row_attention<64, kPaged>(p, qm, km, vm, a->reuse_plan != 0, st);
 }
