@@ -43,18 +43,20 @@ constexpr int kMinQuota = 4;       // smallest range of a CTA, in blocks
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
 constexpr float kRowRescaleLog2 = 8.f;
 constexpr int kItemsKept = 32;     // items of a CTA that it keeps in shared memory
-constexpr int kPolyPairs = 3;      // pairs of every eight whose exponentials are polynomials
 constexpr float kExpC0 = 0.999924541f, kExpC1 = 0.693136752f, kExpC2 = 0.242639482f, kExpC3 = 0.0558382832f;
 
 enum RowSource { kPacked = 0, kPaged = 1, kPagedE4M3 = 2 };
+constexpr int kSoftmaxWarps = 16;  // eight a row tile, four for each half of a block's keys
+constexpr int kLoadWarp = kSoftmaxWarps, kIssueWarp = kLoadWarp + 1, kQueryWarp = kLoadWarp + 2, kWidenWarp = kLoadWarp + 4;
 // Threads, and registers a thread of the softmax warps and of the others: the launch's own are what
-// __launch_bounds__ leaves (168, 128), and the shares add up to them.
+// __launch_bounds__ leaves (96, E4M3 80), and the shares add up to them.
 template <int SRC>
 struct RowRoles {
   static constexpr bool V8 = SRC == kPagedE4M3;
-  static constexpr int THREADS = V8 ? 512 : 384;
-  static constexpr int SOFTMAX_REGS = V8 ? 184 : 208, OTHER_REGS = V8 ? 72 : 88;
-  static_assert(256 * SOFTMAX_REGS + (THREADS - 256) * OTHER_REGS <= THREADS * (V8 ? 128 : 168), "register shares");
+  static constexpr int THREADS = 32 * (kSoftmaxWarps + 4 + (V8 ? 4 : 0));
+  static constexpr int SOFTMAX_REGS = V8 ? 88 : 104, OTHER_REGS = 64;
+  static_assert(32 * kSoftmaxWarps * SOFTMAX_REGS + (THREADS - 32 * kSoftmaxWarps) * OTHER_REGS <= THREADS * (V8 ? 80 : 96),
+                "register shares");
 };
 
 struct alignas(16) RowItem {
@@ -346,12 +348,15 @@ struct RowGeom {
   static constexpr int KH = D / 64;               // 128-byte dim halves
   static constexpr int TILE = 16384 * KH;         // one K or V block, one query tile
   // ring slots (a K or a V block each; E4M3: an even number, so that a slot is always one or the other's)
-  static constexpr int NS = V8 ? 4 : D == 128 ? 5 : 12;
+  static constexpr int NS = D == 128 ? 4 : 10;
+  static constexpr int NRAW = 1;                  // E4M3: blocks of codes
   static constexpr int RING = 2 * TILE;           // the ring lies behind the two query tiles
-  static constexpr int RAW = RING + NS * TILE;    // E4M3: two blocks of codes
-  static constexpr int SMEM = RAW + (V8 ? 2 * 16384 : 0) + 1024;
+  static constexpr int RAW = RING + NS * TILE;
+  static constexpr int STAGED = RAW + (V8 ? NRAW * 16384 : 0);  // rows on their way out, STAGE bytes a softmax warp
+  static constexpr int STAGE = V8 ? 512 : 1024;
+  static constexpr int SMEM = STAGED + kSoftmaxWarps * STAGE + 1024;
   static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
-  static_assert(SMEM <= 227 * 1024 - 2048, "shared memory budget, 2 KB of static variables aside");
+  static_assert(SMEM <= 227 * 1024 - 6144, "shared memory budget, 6 KB of static variables aside");
 };
 
 SD_DEV RowItem load_item(const RowItem* at) {
@@ -405,7 +410,9 @@ SD_DEV bool elect_one() {
   return ok != 0;
 }
 
-// Two fp32 values in a 64-bit register: the packed arithmetic issues both at once.
+// Two fp32 values in a 64-bit register: the packed arithmetic issues both at once.  The assembly here is volatile so
+// that it is issued in the order written: a warp issues in order, and only an order that alternates between the
+// exponential unit and the FMA units keeps both busy (scheduled by the compiler the two took turns, 1.3 times as long).
 SD_DEV uint64_t pack2(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -414,12 +421,27 @@ SD_DEV uint64_t pack2(float a, float b) {
 SD_DEV void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 SD_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 SD_DEV uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SD_DEV float fma_sat(float a, float b, float c) {  // clamped to [0, 1]
+  float r;
+  asm volatile("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+SD_DEV float exp2_unit(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+SD_DEV uint32_t round_bf16(float lo, float hi) {
+  uint32_t r;
+  asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 SD_DEV float max_nan(float a, float b) {
@@ -432,52 +454,113 @@ SD_DEV float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of two finite x <= 8 on the FMA units: x = n + f with f in [-1/2, 1/2], 2^f by the cubic that is exact at
-// the four Chebyshev nodes of that interval (relative error below 2^-13, against the 2^-9 that P is rounded
-// to), n added to the exponent.  Below -126 it stays at 2^-126.
-SD_DEV void exp2_poly2(uint64_t x, float& a, float& b) {
-  constexpr float kRound = 12582912.f;  // 1.5 x 2^23: the sum's low mantissa bits are the nearest integer
-  float lo, hi;
-  unpack2(x, lo, hi);
-  const uint64_t xc = pack2(fmaxf(lo, -126.f), fmaxf(hi, -126.f));
-  const uint64_t t = add2(xc, pack2(kRound, kRound));
-  const uint64_t n = add2(t, pack2(-kRound, -kRound));
-  const uint64_t f = fma2(n, pack2(-1.f, -1.f), xc);
-  uint64_t y = fma2(f, pack2(kExpC3, kExpC3), pack2(kExpC2, kExpC2));
-  y = fma2(y, f, pack2(kExpC1, kExpC1));
-  y = fma2(y, f, pack2(kExpC0, kExpC0));
-  float tl, th, yl, yh;
-  unpack2(t, tl, th);
-  unpack2(y, yl, yh);
-  a = __uint_as_float((__float_as_uint(tl) << 23) + __float_as_uint(yl));
-  b = __uint_as_float((__float_as_uint(th) << 23) + __float_as_uint(yh));
+
+// 2^x on the FMA units, for finite x: x = n + f with f in [-1/2, 1/2], 2^f by the cubic that is exact at the four
+// Chebyshev nodes of that interval (relative error below 2^-13, against the 2^-9 that P is rounded to), n added to
+// the exponent.  x is clamped to [-126, 10] (a score passes the reference maximum by 8 at most) as
+// z = (x + 126) / 136 in [0, 1], which costs nothing beside the scaling; z's rounding moves x by less than 2^-17.
+constexpr float kPolyLow = -126.f, kPolySpan = 136.f;
+constexpr float kRound = 12582912.f;  // 1.5 x 2^23: the low mantissa bits of x + kRound are the nearest integer
+struct Poly2 {
+  uint64_t z, t, f, y;
+  template <int STEP>
+  SD_DEV void step(float s0, float s1, float zs, float zn) {
+    if constexpr (STEP == 0) {
+      const float a = fma_sat(s0, zs, zn), b = fma_sat(s1, zs, zn);
+      z = pack2(a, b);
+    } else if constexpr (STEP == 1) {
+      t = fma2(z, pack2(kPolySpan, kPolySpan), pack2(kRound + kPolyLow, kRound + kPolyLow));
+    } else if constexpr (STEP == 2) {  // -(n - kPolyLow)
+      f = fma2(t, pack2(-1.f, -1.f), pack2(kRound + kPolyLow, kRound + kPolyLow));
+    } else if constexpr (STEP == 3) {
+      f = fma2(z, pack2(kPolySpan, kPolySpan), f);
+    } else if constexpr (STEP == 4) {
+      y = fma2(f, pack2(kExpC3, kExpC3), pack2(kExpC2, kExpC2));
+    } else if constexpr (STEP == 5) {
+      y = fma2(y, f, pack2(kExpC1, kExpC1));
+    } else {
+      y = fma2(y, f, pack2(kExpC0, kExpC0));
+    }
+  }
+  SD_DEV void result(float& a, float& b) {
+    float tl, th, yl, yh;
+    unpack2(t, tl, th);
+    unpack2(y, yl, yh);
+    a = __uint_as_float((__float_as_uint(tl) << 23) + __float_as_uint(yl));
+    b = __uint_as_float((__float_as_uint(th) << 23) + __float_as_uint(yh));
+  }
+};
+
+// Five pairs of scores at once: three take the exponential unit (6 x 8.5 clocks a warp), two the polynomial, whose
+// steps lie between the others'.  Probabilities as bf16 pairs in w[0 .. 4], their sum added to `sum`.
+SD_DEV void five_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, float zn, uint64_t (&sum)[2], uint32_t* w) {
+  Poly2 p[2];
+  float x[6], y[6], a, b;
+  unpack2(fma2(pack2(s[0], s[1]), sc, ng), x[0], x[1]);
+  y[0] = exp2_unit(x[0]);
+  p[0].step<0>(s[6], s[7], zs, zn);
+  p[1].step<0>(s[8], s[9], zs, zn);
+  unpack2(fma2(pack2(s[2], s[3]), sc, ng), x[2], x[3]);
+  y[1] = exp2_unit(x[1]);
+  p[0].step<1>(0, 0, 0, 0);
+  p[1].step<1>(0, 0, 0, 0);
+  unpack2(fma2(pack2(s[4], s[5]), sc, ng), x[4], x[5]);
+  p[0].step<2>(0, 0, 0, 0);
+  y[2] = exp2_unit(x[2]);
+  p[1].step<2>(0, 0, 0, 0);
+  p[0].step<3>(0, 0, 0, 0);
+  p[1].step<3>(0, 0, 0, 0);
+  y[3] = exp2_unit(x[3]);
+  p[0].step<4>(0, 0, 0, 0);
+  p[1].step<4>(0, 0, 0, 0);
+  sum[0] = add2(sum[0], pack2(y[0], y[1]));
+  w[0] = round_bf16(y[0], y[1]);
+  y[4] = exp2_unit(x[4]);
+  p[0].step<5>(0, 0, 0, 0);
+  p[1].step<5>(0, 0, 0, 0);
+  sum[1] = add2(sum[1], pack2(y[2], y[3]));
+  w[1] = round_bf16(y[2], y[3]);
+  y[5] = exp2_unit(x[5]);
+  p[0].step<6>(0, 0, 0, 0);
+  p[1].step<6>(0, 0, 0, 0);
+  p[0].result(a, b);
+  sum[0] = add2(sum[0], pack2(a, b));
+  w[3] = round_bf16(a, b);
+  p[1].result(a, b);
+  sum[1] = add2(sum[1], pack2(a, b));
+  w[4] = round_bf16(a, b);
+  sum[0] = add2(sum[0], pack2(y[4], y[5]));
+  w[2] = round_bf16(y[4], y[5]);
+}
+SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t ng, uint64_t& sum, uint32_t* w) {
+  float a, b;
+  unpack2(fma2(pack2(s[0], s[1]), sc, ng), a, b);
+  a = exp2_unit(a);
+  b = exp2_unit(b);
+  sum = add2(sum, pack2(a, b));
+  *w = round_bf16(a, b);
 }
 
-// P of a row's 128 scores s (in registers) as bf16 over the score columns; returns the sum.  POLY: of every eight
-// pairs, kPolyPairs take the polynomial instead of the exponential unit.  `half` is called when the first 64 keys are written.
-template <bool POLY, typename Half>
-SD_DEV float row_probabilities(const float (&s)[128], float scale, float neg, uint32_t ta, Half half) {
+// P of half a row's 64 scores s (in registers) as bf16 over the same thread's score columns; returns the sum.
+// POLY: six of every sixteen pairs by polynomial.  `first` is called when 32 keys are written.
+template <bool POLY, typename First>
+SD_DEV float row_probabilities(const float (&s)[64], float scale, float neg, uint32_t ta, First first) {
   const uint64_t sc = pack2(scale, scale), ng = pack2(neg, neg);
+  const float zs = scale * (1.f / kPolySpan), zn = (neg - kPolyLow) * (1.f / kPolySpan);
   uint64_t sum[2] = {0, 0};
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < 2; ++c) {
     uint32_t w[16];
+    if (POLY) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const uint64_t x = fma2(pack2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), sc, ng);
-      float a, b;
-      if (POLY && (e & 7) < kPolyPairs) {
-        exp2_poly2(x, a, b);
-      } else {
-        unpack2(x, a, b);
-        a = fast_exp2(a);
-        b = fast_exp2(b);
-      }
-      sum[e & 1] = add2(sum[e & 1], pack2(a, b));
-      w[e] = pack_bf16(a, b);
+      for (int e = 0; e < 3; ++e) five_pairs(s + 32 * c + 10 * e, sc, ng, zs, zn, sum, w + 5 * e);
+      one_pair(s + 32 * c + 30, sc, ng, sum[1], w + 15);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) one_pair(s + 32 * c + 2 * e, sc, ng, sum[e & 1], w + e);
     }
     umma::tmem_st16_words(ta + 16 * c, w);
-    if (c == 1) half();
+    if (c == 0) first();
   }
   float a, b;
   unpack2(add2(sum[0], sum[1]), a, b);
@@ -493,9 +576,10 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   constexpr int NS = Geo::NS, KH = Geo::KH;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[NS], empty[NS], raw_full[2], raw_empty[2];
+  __shared__ uint64_t full[NS], empty[NS], raw_full, raw_empty;
   __shared__ uint64_t q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], c_req, v_clean, fin;
   __shared__ RowItem s_items[kItemsKept];  // the CTA's first items
+  __shared__ float s_swap[2][2][2][kRowTile];  // [buffer][tile][half][row]
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -505,12 +589,12 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_half[t], 4);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&p_half[t], 8);
+      mbar_init(&p_full[t], 8);
       mbar_init(&o_full[t], 1);
-      mbar_init(&raw_full[t], 1);
-      mbar_init(&raw_empty[t], 4);
     }
+    mbar_init(&raw_full, 1);
+    mbar_init(&raw_empty, 4);
     mbar_init(&q_full, 2);
     mbar_init(&q_empty, 1);
     mbar_init(&c_req, 1);
@@ -518,11 +602,11 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     mbar_init(&fin, 1);
     fence_barrier_init();
   }
-  if (warp == 9) {
+  if (warp == kIssueWarp) {
     umma::tmem_alloc(&s_tmem, Geo::TMEM_COLS);
     umma::tmem_relinquish();
   }
-  if (warp == 8 && lane == 0) {
+  if (warp == kLoadWarp && lane == 0) {
     prefetch_tmap(&qmap);
     prefetch_tmap(&kmap);
     prefetch_tmap(&vmap);
@@ -538,18 +622,30 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   const uint32_t tmem = s_tmem;
   auto item_at = [&](int i) { return i - i0 < kItemsKept ? s_items[i - i0] : load_item(p.items + i); };
 
-  if (warp < 8) {
+  if (warp < kSoftmaxWarps) {
     more_regs<RowRoles<SRC>::SOFTMAX_REGS>();
-    // ------------------------------------------------------------ softmax and epilogue: a thread a row
-    const int t = warp >> 2, row = tid & 127;
+    // ------------------------------------------------------------ softmax and epilogue: two threads a row
+    const int t = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
     const int tok = row / p.n_rep, rep = row - tok * p.n_rep;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 5;
-    const uint32_t s_ta = umma::taddr(tmem, lanes, Geo::S_COL + t * 128);
-    const uint32_t o_ta = umma::taddr(tmem, lanes, Geo::O_COL + t * D);
+    const uint32_t s_ta = umma::taddr(tmem, lanes, Geo::S_COL + t * 128 + half * 64);
+    const uint32_t o_ta = umma::taddr(tmem, lanes, Geo::O_COL + t * D + half * (D / 2));
     const float scale = p.scale_log2;
     const float grow = kRowRescaleLog2 / scale;
-    uint32_t sn = 0, on = 0;
+    float* const mine = &s_swap[0][t][half][row];
+    const float* const theirs = &s_swap[0][t][half ^ 1][row];
+    constexpr int kSwap = 2 * 2 * kRowTile;  // floats between the two buffers of s_swap
+    const int pair_bar = 1 + (t << 2) + (warp & 3);
+    uint32_t sn = 0, on = 0, sw = 0;
     bool ok = true;
+    // the row's other thread's value; the buffers alternate, so one barrier an exchange is enough
+    auto swap = [&](float x) {
+      mine[sw * kSwap] = x;
+      named_bar_sync(pair_bar, 64);
+      const float y = theirs[sw * kSwap];
+      sw ^= 1;
+      return y;
+    };
     auto signal = [&](uint64_t* bar) {
       umma::tmem_wait_st();
       umma::fence_before_sync();
@@ -572,7 +668,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       }
       const int nb = tile_blocks(p, it, t);
       if (nb == 0) {  // no tile, or a piece past the tile's keys: the row's other pieces are all of it
-        if (it.slot >= 0 && limit > 0) p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
+        if (it.slot >= 0 && limit > 0 && half == 0)
+          p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
         continue;
       }
       const bool any_row = __any_sync(0xffffffffu, limit > 0);
@@ -590,24 +687,25 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           }
           continue;
         }
-        float s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) umma::tmem_ld32(s_ta + 32 * c, s + 32 * c);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) umma::tmem_wait_ld32(s + 32 * c);
-        const int key0 = it.k0 + j * kKeyBlock;
-        const bool masked = least < key0 + kKeyBlock;
+        float s[64];
+        umma::tmem_ld32(s_ta, s);
+        umma::tmem_ld32(s_ta + 32, s + 32);
+        umma::tmem_wait_ld32(s);
+        umma::tmem_wait_ld32(s + 32);
+        const int key0 = it.k0 + j * kKeyBlock + half * 64;
+        const bool masked = least < key0 + 64;
         if (masked) {
           const int vis = limit - key0;
 #pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = c < vis ? s[c] : -INFINITY;
+          for (int c = 0; c < 64; ++c) s[c] = c < vis ? s[c] : -INFINITY;
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < 124; c += 8)
+        for (int c = 4; c < 60; c += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx[e] = max3_nan(mx[e], s[c + e], s[c + 4 + e]);
-        const float bm = max3_nan(max3_nan(mx[0], mx[1], s[124]), max3_nan(mx[2], mx[3], s[125]), max_nan(s[126], s[127]));
+        float bm = max3_nan(max3_nan(mx[0], mx[1], s[60]), max3_nan(mx[2], mx[3], s[61]), max_nan(s[62], s[63]));
+        bm = max_nan(bm, swap(bm));
         const bool need = j > 0 && !(bm <= m + grow);  // a NaN, too
         if (j == 0) m = bm;
         bool plain = masked;
@@ -616,62 +714,87 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             const float alpha = need ? fast_exp2((m - bm) * scale) : 1.f;
             if (need) m = bm;
             l *= alpha;
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 16) {
+              float o[16];
+              umma::tmem_ld16(o_ta + c, o);
+              umma::tmem_wait_ld16(o);
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              float o[32];
-              umma::tmem_ld32(o_ta + c, o);
-              umma::tmem_wait_ld32(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= alpha;
-              umma::tmem_st16(o_ta + c, reinterpret_cast<const float(&)[16]>(o[0]));
-              umma::tmem_st16(o_ta + c + 16, reinterpret_cast<const float(&)[16]>(o[16]));
+              for (int e = 0; e < 16; ++e) o[e] *= alpha;
+              umma::tmem_st16(o_ta + c, o);
             }
           }
           // infinite and NaN scores go through the exponential unit, which knows them
           plain = plain || __any_sync(0xffffffffu, !(fabsf(m) < INFINITY));
         }
         const float neg = m == -INFINITY ? 0.f : -m * scale;
-        auto half = [&]() { signal(&p_half[t]); };
-        l += plain ? row_probabilities<false>(s, scale, neg, s_ta, half)
-                   : row_probabilities<true>(s, scale, neg, s_ta, half);
+        auto first = [&]() { signal(&p_half[t]); };
+        l += plain ? row_probabilities<false>(s, scale, neg, s_ta, first)
+                   : row_probabilities<true>(s, scale, neg, s_ta, first);
         signal(&p_full[t]);
       }
       if (!ok) break;
+      if (any_row) l += swap(l);
       ok = warp_wait(&o_full[t], on & 1);
       if (!ok) break;
       ++on;
       umma::fence_after_sync();
       if (any_row) {
-        if (it.slot < 0) {
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          const int64_t at = static_cast<int64_t>(it.row0 + vt) * p.o_st +
-                             static_cast<int64_t>(it.head * p.n_rep + rep) * p.o_sh;
-#pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            float o[32];
-            umma::tmem_ld32(o_ta + c, o);
-            umma::tmem_wait_ld32(o);
-            if (limit > 0) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 8)
-                *reinterpret_cast<uint4*>(p.out + at + c + e) =
-                    make_uint4(pack_bf16(o[e] * inv, o[e + 1] * inv), pack_bf16(o[e + 2] * inv, o[e + 3] * inv),
-                               pack_bf16(o[e + 4] * inv, o[e + 5] * inv), pack_bf16(o[e + 6] * inv, o[e + 7] * inv));
-            }
+        // Rows leave through shared memory, 32 bytes of a row at a time, so that a store covers whole sectors.
+        constexpr int RP = Geo::STAGE / 32;  // rows a pass
+        uint8_t* const stage = smem + Geo::STAGED + warp * Geo::STAGE;
+        uint8_t* const put = stage + (lane % RP) * 32;
+        const int flip = (lane >> 2) & 1;    // which of the two 16-byte places comes first: no bank conflicts
+        const bool direct = it.slot < 0;
+        const float inv = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        int64_t at = -1;  // this row's first byte
+        if (limit > 0) {
+          if (direct) {
+            at = 2 * (static_cast<int64_t>(it.row0 + vt) * p.o_st +
+                      static_cast<int64_t>(it.head * p.n_rep + rep) * p.o_sh + half * (D / 2));
+          } else {
+            const int64_t r = it.slot + t * kRowTile + row;
+            if (half == 0) p.part_ml[r] = make_float2(m * scale, l);
+            at = 4 * (r * D + half * (D / 2));
           }
-        } else {
-          const int64_t at = it.slot + t * kRowTile + row;
-          if (limit > 0) p.part_ml[at] = make_float2(m * scale, l);
+        }
+        uint8_t* const base = direct ? reinterpret_cast<uint8_t*>(p.out) : reinterpret_cast<uint8_t*>(p.part_o);
+        const int cols = direct ? 16 : 8;    // columns of a step
+        for (int c = 0; c < D / 2; c += cols) {
+          uint4 x[2];
+          if (direct) {
+            float o[16];
+            umma::tmem_ld16(o_ta + c, o);
+            umma::tmem_wait_ld16(o);
 #pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            float o[32];
-            umma::tmem_ld32(o_ta + c, o);
-            umma::tmem_wait_ld32(o);
-            if (limit > 0) {
+            for (int e = 0; e < 2; ++e)
+              x[e] = make_uint4(pack_bf16(o[8 * e] * inv, o[8 * e + 1] * inv), pack_bf16(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                pack_bf16(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
+                                pack_bf16(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+          } else {
+            float o[8];
+            umma::tmem_ld8(o_ta + c, o);
+            umma::tmem_wait_ld8(o);
 #pragma unroll
-              for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<float4*>(p.part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 2; ++e)
+              x[e] = make_uint4(__float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]), __float_as_uint(o[4 * e + 2]),
+                                __float_as_uint(o[4 * e + 3]));
+          }
+#pragma unroll
+          for (int pass = 0; pass < 32 / RP; ++pass) {
+            if (lane / RP == pass) {
+              *reinterpret_cast<uint4*>(put + (flip << 4)) = x[0];
+              *reinterpret_cast<uint4*>(put + ((flip ^ 1) << 4)) = x[1];
             }
+            __syncwarp();
+#pragma unroll
+            for (int g = 0; g < RP / 16; ++g) {
+              const int r = g * 16 + lane / 2, ch = lane & 1;
+              const int64_t to = __shfl_sync(0xffffffffu, at, pass * RP + r);
+              const uint4 y = *reinterpret_cast<const uint4*>(stage + r * 32 + ((ch ^ ((r >> 2) & 1)) << 4));
+              if (to >= 0) *reinterpret_cast<uint4*>(base + to + c * (direct ? 2 : 4) + ch * 16) = y;
+            }
+            __syncwarp();
           }
         }
         umma::fence_before_sync();  // O is read: the arrival for the next item's first block lets its MMAs write it
@@ -680,7 +803,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
   } else {
     fewer_regs<RowRoles<SRC>::OTHER_REGS>();
-    if (warp == 8) {
+    if (warp == kLoadWarp) {
       // ---------------------------------------------------------- K/V blocks
       uint32_t n = 0;  // blocks issued (K and V each count)
       bool ok = true;
@@ -703,8 +826,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           for (int kv = 0; kv < 2; ++kv, ++n) {
             const uint32_t s = n % NS, round = n / NS;
             if (V8 && kv) {  // codes; the widening warps take care of the block's ring slot
-              const uint32_t b = (n >> 1) & 1, r = n >> 2;
-              if (r > 0 && !warp_wait(&raw_empty[b], (r - 1) & 1)) {
+              const uint32_t r = n >> 1;
+              if (r > 0 && !warp_wait(&raw_empty, (r - 1) & 1)) {
                 ok = false;
                 break;
               }
@@ -712,11 +835,11 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
 #pragma unroll
               for (int e = 0; e < 8; ++e) pg[e] = __shfl_sync(0xffffffffu, ids, 8 * (j & 3) + e) * p.KV + it.head;
               if (lane == 0) {
-                mbar_arrive_expect_tx(&raw_full[b], 16384);
+                mbar_arrive_expect_tx(&raw_full, 16384);
 #pragma unroll
                 for (int e = 0; e < 8; e += 4)
-                  tma_rows4(smem + Geo::RAW + b * 16384 + e * 2048, &vmap, pg[e], pg[e + 1], pg[e + 2], pg[e + 3],
-                            &raw_full[b]);
+                  tma_rows4(smem + Geo::RAW + e * 2048, &vmap, pg[e], pg[e + 1], pg[e + 2], pg[e + 3],
+                            &raw_full);
               }
               __syncwarp();
               continue;
@@ -757,9 +880,9 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
         // copies under way land before the CTA leaves
         for (uint32_t k = n > NS ? n - NS : 0; k < n; ++k)
-          (void)(V8 && (k & 1) ? warp_wait(&raw_full[(k >> 1) & 1], (k >> 2) & 1) : warp_wait(&full[k % NS], (k / NS) & 1));
+          (void)(V8 && (k & 1) ? warp_wait(&raw_full, (k >> 1) & 1) : warp_wait(&full[k % NS], (k / NS) & 1));
       }
-    } else if (warp == 9) {
+    } else if (warp == kIssueWarp) {
       // ---------------------------------------------------------- MMA issue
       constexpr uint32_t id_qk = umma::idesc_f16(128, kKeyBlock, true, true, false, false);
       constexpr uint32_t id_pv = umma::idesc_f16(128, D, true, true, false, true);
@@ -787,13 +910,14 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         }
         __syncwarp();
       };
-      auto pv = [&](int t, uint32_t slot, int h, bool acc) {  // half h of the block's keys
+      auto pv = [&](int t, uint32_t slot, int h, bool acc) {  // keys 32 h .. and 64 + 32 h .. (32 each) of the block
         if (elect_one()) {
           const uint64_t vd = v_desc + slot * (Geo::TILE >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kKeyBlock / 32; ++kk) {
-            const int k = h * (kKeyBlock / 32) + kk;
-            umma::mma_f16_ts(o_col[t], s_col[t] + k * 8, vd + k * (2048 >> 4), id_pv, acc || k > 0);
+          for (int kk = 0; kk < 4; ++kk) {
+            const int half = kk >> 1, step = 2 * h + (kk & 1);  // 16 keys each; P of a half starts where its scores did
+            umma::mma_f16_ts(o_col[t], s_col[t] + half * 64 + step * 8, vd + (half * 4 + step) * (2048 >> 4), id_pv,
+                             acc || kk > 0);
           }
         }
         __syncwarp();
@@ -869,9 +993,9 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
       commit(&fin);
       (void)warp_wait(&fin, 0);
-    } else if (warp == 10 || warp == 11) {
-      // ---------------------------------------------------------- query rows; V rows past the last key (warp 11)
-      const int t = warp - 10;
+    } else if (warp < kWidenWarp) {
+      // ---------------------------------------------------------- query rows; V rows past the last key
+      const int t = warp - kQueryWarp;
       uint32_t items = 0, cleaned = 0, n = 0;
       bool ok = true;
       for (int i = i0; i <= i1 && ok; ++i) {
@@ -893,7 +1017,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             mbar_arrive(&q_full);
           }
         } else {
-          // a group's rows are anywhere: 16 bytes a lane, tile t by warp 10 + t
+          // a group's rows are anywhere: 16 bytes a lane, a tile a warp
           constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte chunks of a row, rows a step
           const uint32_t q_base = smem_u32(smem) + t * Geo::TILE;
           for (int base = 0; base < (t < tiles ? kRowTile : 0); base += 32) {
@@ -942,7 +1066,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     } else {
       // ---------------------------------------------------------- E4M3: codes to bf16, a thread a key
       if constexpr (V8) {
-        const int r = tid - 384;
+        const int r = tid - 32 * kWidenWarp;
         uint32_t n = 1;
         bool ok = true;
         for (int i = i0; i <= i1 && ok; ++i) {
@@ -962,11 +1086,11 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             const float sc = next;
             const bool in = it.k0 + j * kKeyBlock + r < it.k1;
             if (j + 1 < nb) next = scale_of(j + 1);
-            const uint32_t s = n % NS, b = (n >> 1) & 1;
-            ok = warp_wait(&raw_full[b], (n >> 2) & 1);
+            const uint32_t s = n % NS;
+            ok = warp_wait(&raw_full, (n >> 1) & 1);
             if (ok && n >= NS) ok = warp_wait(&empty[s], (n / NS - 1) & 1);
             if (!ok) break;
-            const uint8_t* src = smem + Geo::RAW + b * 16384 + r * 128;
+            const uint8_t* src = smem + Geo::RAW + r * 128;
             uint8_t* dst = smem + Geo::RING + s * Geo::TILE + r * 128;
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
@@ -989,7 +1113,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             __syncwarp();
             if (lane == 0) {
               mbar_arrive(&full[s]);
-              mbar_arrive(&raw_empty[b]);
+              mbar_arrive(&raw_empty);
             }
           }
         }
@@ -999,7 +1123,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   }
   umma::fence_before_sync();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kIssueWarp) {
     umma::fence_after_sync();
     umma::tmem_dealloc(tmem, Geo::TMEM_COLS);
   }
