@@ -41,21 +41,21 @@ constexpr int kKeyBlock = 128;     // keys of a block
 constexpr int kUnitCost = 2;       // what a unit costs beside its blocks (query load, epilogue), in blocks
 constexpr int kMinQuota = 4;       // smallest range of a CTA, in blocks
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
-constexpr float kRowRescaleLog2 = 8.f;
+constexpr float kGrow = 1.152921504606846976e18f;  // 2^60: a block's sum past it moves the row's reference
 constexpr int kItemsKept = 32;     // items of a CTA that it keeps in shared memory
 constexpr float kExpC0 = 0.999924541f, kExpC1 = 0.693136752f, kExpC2 = 0.242639482f, kExpC3 = 0.0558382832f;
 
 enum RowSource { kPacked = 0, kPaged = 1, kPagedE4M3 = 2 };
-constexpr int kSoftmaxWarps = 16;  // eight a row tile, four for each half of a block's keys
+constexpr int kSoftmaxWarps = 8;  // four a row tile
 constexpr int kLoadWarp = kSoftmaxWarps, kIssueWarp = kLoadWarp + 1, kQueryWarp = kLoadWarp + 2, kWidenWarp = kLoadWarp + 4;
 // Threads, and registers a thread of the softmax warps and of the others: the launch's own are what
-// __launch_bounds__ leaves (96, E4M3 80), and the shares add up to them.
+// __launch_bounds__ leaves (168, E4M3 128), and the shares add up to them.
 template <int SRC>
 struct RowRoles {
   static constexpr bool V8 = SRC == kPagedE4M3;
   static constexpr int THREADS = 32 * (kSoftmaxWarps + 4 + (V8 ? 4 : 0));
-  static constexpr int SOFTMAX_REGS = V8 ? 88 : 104, OTHER_REGS = 64;
-  static_assert(32 * kSoftmaxWarps * SOFTMAX_REGS + (THREADS - 32 * kSoftmaxWarps) * OTHER_REGS <= THREADS * (V8 ? 80 : 96),
+  static constexpr int SOFTMAX_REGS = V8 ? 184 : 208, OTHER_REGS = V8 ? 72 : 88;
+  static_assert(32 * kSoftmaxWarps * SOFTMAX_REGS + (THREADS - 32 * kSoftmaxWarps) * OTHER_REGS <= THREADS * (V8 ? 128 : 168),
                 "register shares");
 };
 
@@ -348,15 +348,15 @@ struct RowGeom {
   static constexpr int KH = D / 64;               // 128-byte dim halves
   static constexpr int TILE = 16384 * KH;         // one K or V block, one query tile
   // ring slots (a K or a V block each; E4M3: an even number, so that a slot is always one or the other's)
-  static constexpr int NS = D == 128 ? 4 : 10;
+  static constexpr int NS = D == 128 ? 4 : 11;
   static constexpr int NRAW = 1;                  // E4M3: blocks of codes
   static constexpr int RING = 2 * TILE;           // the ring lies behind the two query tiles
   static constexpr int RAW = RING + NS * TILE;
   static constexpr int STAGED = RAW + (V8 ? NRAW * 16384 : 0);  // rows on their way out, STAGE bytes a softmax warp
-  static constexpr int STAGE = V8 ? 512 : 1024;
+  static constexpr int STAGE = 2048;
   static constexpr int SMEM = STAGED + kSoftmaxWarps * STAGE + 1024;
   static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
-  static_assert(SMEM <= 227 * 1024 - 6144, "shared memory budget, 6 KB of static variables aside");
+  static_assert(SMEM <= 227 * 1024 - 2048, "shared memory budget, 2 KB of static variables aside");
 };
 
 SD_DEV RowItem load_item(const RowItem* at) {
@@ -457,9 +457,9 @@ SD_DEV float max3_nan(float a, float b, float c) {
 
 // 2^x on the FMA units, for finite x: x = n + f with f in [-1/2, 1/2], 2^f by the cubic that is exact at the four
 // Chebyshev nodes of that interval (relative error below 2^-13, against the 2^-9 that P is rounded to), n added to
-// the exponent.  x is clamped to [-126, 10] (a score passes the reference maximum by 8 at most) as
-// z = (x + 126) / 136 in [0, 1], which costs nothing beside the scaling; z's rounding moves x by less than 2^-17.
-constexpr float kPolyLow = -126.f, kPolySpan = 136.f;
+// the exponent.  x is clamped to [-126, 127] as z = (x + 126) / 253 in [0, 1], which costs nothing beside the scaling;
+// z's rounding moves x by less than 2^-16.
+constexpr float kPolyLow = -126.f, kPolySpan = 253.f;
 constexpr float kRound = 12582912.f;  // 1.5 x 2^23: the low mantissa bits of x + kRound are the nearest integer
 struct Poly2 {
   uint64_t z, t, f, y;
@@ -491,79 +491,66 @@ struct Poly2 {
   }
 };
 
-// Five pairs of scores at once: three take the exponential unit (6 x 8.5 clocks a warp), two the polynomial, whose
-// steps lie between the others'.  Probabilities as bf16 pairs in w[0 .. 4], their sum added to `sum`.
-SD_DEV void five_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, float zn, uint64_t (&sum)[2], uint32_t* w) {
-  Poly2 p[2];
-  float x[6], y[6], a, b;
-  unpack2(fma2(pack2(s[0], s[1]), sc, ng), x[0], x[1]);
-  y[0] = exp2_unit(x[0]);
-  p[0].step<0>(s[6], s[7], zs, zn);
-  p[1].step<0>(s[8], s[9], zs, zn);
-  unpack2(fma2(pack2(s[2], s[3]), sc, ng), x[2], x[3]);
-  y[1] = exp2_unit(x[1]);
-  p[0].step<1>(0, 0, 0, 0);
-  p[1].step<1>(0, 0, 0, 0);
-  unpack2(fma2(pack2(s[4], s[5]), sc, ng), x[4], x[5]);
-  p[0].step<2>(0, 0, 0, 0);
-  y[2] = exp2_unit(x[2]);
-  p[1].step<2>(0, 0, 0, 0);
-  p[0].step<3>(0, 0, 0, 0);
-  p[1].step<3>(0, 0, 0, 0);
-  y[3] = exp2_unit(x[3]);
-  p[0].step<4>(0, 0, 0, 0);
-  p[1].step<4>(0, 0, 0, 0);
-  sum[0] = add2(sum[0], pack2(y[0], y[1]));
-  w[0] = round_bf16(y[0], y[1]);
-  y[4] = exp2_unit(x[4]);
-  p[0].step<5>(0, 0, 0, 0);
-  p[1].step<5>(0, 0, 0, 0);
-  sum[1] = add2(sum[1], pack2(y[2], y[3]));
-  w[1] = round_bf16(y[2], y[3]);
-  y[5] = exp2_unit(x[5]);
-  p[0].step<6>(0, 0, 0, 0);
-  p[1].step<6>(0, 0, 0, 0);
-  p[0].result(a, b);
-  sum[0] = add2(sum[0], pack2(a, b));
-  w[3] = round_bf16(a, b);
-  p[1].result(a, b);
-  sum[1] = add2(sum[1], pack2(a, b));
-  w[4] = round_bf16(a, b);
-  sum[0] = add2(sum[0], pack2(y[4], y[5]));
-  w[2] = round_bf16(y[4], y[5]);
+// Ten pairs of scores at once, as two groups of five whose steps alternate: in a group three pairs take the
+// exponential unit (6 x 8.5 clocks a warp) and two the polynomial, whose steps lie between the others'.  Probabilities
+// as bf16 pairs in w[0 .. 9], their sums added to `sum`.
+SD_DEV void ten_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, float zn, uint64_t (&sum)[4], uint32_t* w) {
+  Poly2 p[2][2];
+  float x[2][6], y[2][6], a, b;
+#define SD_EACH(...)            \
+  _Pragma("unroll") for (int g = 0; g < 2; ++g) { \
+    [[maybe_unused]] const float* r = s + 10 * g; \
+    __VA_ARGS__                 \
+  }
+#define SD_POLY(K)                      \
+  p[g][0].step<K>(r[6], r[7], zs, zn); \
+  p[g][1].step<K>(r[8], r[9], zs, zn);
+  SD_EACH(unpack2(fma2(pack2(r[0], r[1]), sc, ng), x[g][0], x[g][1]);)
+  SD_EACH(y[g][0] = exp2_unit(x[g][0]); SD_POLY(0))
+  SD_EACH(unpack2(fma2(pack2(r[2], r[3]), sc, ng), x[g][2], x[g][3]); y[g][1] = exp2_unit(x[g][1]); SD_POLY(1))
+  SD_EACH(unpack2(fma2(pack2(r[4], r[5]), sc, ng), x[g][4], x[g][5]); y[g][2] = exp2_unit(x[g][2]); SD_POLY(2))
+  SD_EACH(y[g][3] = exp2_unit(x[g][3]); SD_POLY(3) sum[2 * g] = add2(sum[2 * g], pack2(y[g][0], y[g][1]));)
+  SD_EACH(y[g][4] = exp2_unit(x[g][4]); SD_POLY(4) w[5 * g] = round_bf16(y[g][0], y[g][1]);)
+  SD_EACH(y[g][5] = exp2_unit(x[g][5]); SD_POLY(5) sum[2 * g + 1] = add2(sum[2 * g + 1], pack2(y[g][2], y[g][3]));)
+  SD_EACH(SD_POLY(6) w[5 * g + 1] = round_bf16(y[g][2], y[g][3]);)
+  SD_EACH(p[g][0].result(a, b); sum[2 * g] = add2(sum[2 * g], pack2(a, b)); w[5 * g + 3] = round_bf16(a, b);
+          sum[2 * g + 1] = add2(sum[2 * g + 1], pack2(y[g][4], y[g][5]));
+          w[5 * g + 2] = round_bf16(y[g][4], y[g][5]);)
+  SD_EACH(p[g][1].result(a, b); sum[2 * g] = add2(sum[2 * g], pack2(a, b)); w[5 * g + 4] = round_bf16(a, b);)
+#undef SD_POLY
+#undef SD_EACH
 }
 SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t ng, uint64_t& sum, uint32_t* w) {
   float a, b;
   unpack2(fma2(pack2(s[0], s[1]), sc, ng), a, b);
-  a = exp2_unit(a);
-  b = exp2_unit(b);
+  // scores beyond 2^30 miss the reference by more than an exponent holds (their own rounding); NaN stays
+  a = exp2_unit(a > 60.f ? 60.f : a);
+  b = exp2_unit(b > 60.f ? 60.f : b);
   sum = add2(sum, pack2(a, b));
   *w = round_bf16(a, b);
 }
 
-// P of half a row's 64 scores s (in registers) as bf16 over the same thread's score columns; returns the sum.
-// POLY: six of every sixteen pairs by polynomial.  `first` is called when 32 keys are written.
-template <bool POLY, typename First>
-SD_DEV float row_probabilities(const float (&s)[64], float scale, float neg, uint32_t ta, First first) {
+// P = 2^(s scale + neg) of 64 scores as bf16 in 32 TMEM columns; returns the sum.  POLY: twelve of the 32 pairs by
+// polynomial.
+template <bool POLY>
+SD_DEV float row_probabilities(const float* s, float scale, float neg, uint32_t ta) {
   const uint64_t sc = pack2(scale, scale), ng = pack2(neg, neg);
   const float zs = scale * (1.f / kPolySpan), zn = (neg - kPolyLow) * (1.f / kPolySpan);
-  uint64_t sum[2] = {0, 0};
+  uint64_t sum[4] = {0, 0, 0, 0};
+  uint32_t w[32];
+  if (POLY) {
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t w[16];
-    if (POLY) {
+    for (int e = 0; e < 3; ++e) ten_pairs(s + 20 * e, sc, ng, zs, zn, sum, w + 10 * e);
 #pragma unroll
-      for (int e = 0; e < 3; ++e) five_pairs(s + 32 * c + 10 * e, sc, ng, zs, zn, sum, w + 5 * e);
-      one_pair(s + 32 * c + 30, sc, ng, sum[1], w + 15);
-    } else {
+    for (int e = 30; e < 32; ++e) one_pair(s + 2 * e, sc, ng, sum[e & 3], w + e);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) one_pair(s + 32 * c + 2 * e, sc, ng, sum[e & 1], w + e);
-    }
-    umma::tmem_st16_words(ta + 16 * c, w);
-    if (c == 0) first();
+    for (int e = 0; e < 32; ++e) one_pair(s + 2 * e, sc, ng, sum[e & 3], w + e);
   }
+  umma::tmem_st16_words(ta, reinterpret_cast<const uint32_t(&)[16]>(w[0]));
+  umma::tmem_st16_words(ta + 16, reinterpret_cast<const uint32_t(&)[16]>(w[16]));
   float a, b;
-  unpack2(add2(sum[0], sum[1]), a, b);
+  unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
   return a + b;
 }
 
@@ -577,9 +564,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[NS], empty[NS], raw_full, raw_empty;
-  __shared__ uint64_t q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], c_req, v_clean, fin;
+  __shared__ uint64_t q_full, q_empty, s_full[2], p_half[2], pv_half[2], p_full[2], o_full[2], c_req, v_clean, fin;
   __shared__ RowItem s_items[kItemsKept];  // the CTA's first items
-  __shared__ float s_swap[2][2][2][kRowTile];  // [buffer][tile][half][row]
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -589,8 +575,9 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_half[t], 8);
-      mbar_init(&p_full[t], 8);
+      mbar_init(&p_half[t], 4);
+      mbar_init(&pv_half[t], 1);
+      mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
     }
     mbar_init(&raw_full, 1);
@@ -624,28 +611,15 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
 
   if (warp < kSoftmaxWarps) {
     more_regs<RowRoles<SRC>::SOFTMAX_REGS>();
-    // ------------------------------------------------------------ softmax and epilogue: two threads a row
-    const int t = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+    // ------------------------------------------------------------ softmax and epilogue: a thread a row
+    const int t = warp >> 2, row = tid & 127;
     const int tok = row / p.n_rep, rep = row - tok * p.n_rep;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 5;
-    const uint32_t s_ta = umma::taddr(tmem, lanes, Geo::S_COL + t * 128 + half * 64);
-    const uint32_t o_ta = umma::taddr(tmem, lanes, Geo::O_COL + t * D + half * (D / 2));
+    const uint32_t s_ta = umma::taddr(tmem, lanes, Geo::S_COL + t * 128);
+    const uint32_t o_ta = umma::taddr(tmem, lanes, Geo::O_COL + t * D);
     const float scale = p.scale_log2;
-    const float grow = kRowRescaleLog2 / scale;
-    float* const mine = &s_swap[0][t][half][row];
-    const float* const theirs = &s_swap[0][t][half ^ 1][row];
-    constexpr int kSwap = 2 * 2 * kRowTile;  // floats between the two buffers of s_swap
-    const int pair_bar = 1 + (t << 2) + (warp & 3);
-    uint32_t sn = 0, on = 0, sw = 0;
+    uint32_t sn = 0, on = 0;
     bool ok = true;
-    // the row's other thread's value; the buffers alternate, so one barrier an exchange is enough
-    auto swap = [&](float x) {
-      mine[sw * kSwap] = x;
-      named_bar_sync(pair_bar, 64);
-      const float y = theirs[sw * kSwap];
-      sw ^= 1;
-      return y;
-    };
     auto signal = [&](uint64_t* bar) {
       umma::tmem_wait_st();
       umma::fence_before_sync();
@@ -668,8 +642,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       }
       const int nb = tile_blocks(p, it, t);
       if (nb == 0) {  // no tile, or a piece past the tile's keys: the row's other pieces are all of it
-        if (it.slot >= 0 && limit > 0 && half == 0)
-          p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
+        if (it.slot >= 0 && limit > 0) p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
         continue;
       }
       const bool any_row = __any_sync(0xffffffffu, limit > 0);
@@ -687,115 +660,125 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           }
           continue;
         }
-        float s[64];
-        umma::tmem_ld32(s_ta, s);
-        umma::tmem_ld32(s_ta + 32, s + 32);
-        umma::tmem_wait_ld32(s);
-        umma::tmem_wait_ld32(s + 32);
-        const int key0 = it.k0 + j * kKeyBlock + half * 64;
-        const bool masked = least < key0 + 64;
+        float s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) umma::tmem_ld32(s_ta + 32 * c, s + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) umma::tmem_wait_ld32(s + 32 * c);
+        const int key0 = it.k0 + j * kKeyBlock;
+        const bool masked = least < key0 + kKeyBlock;
         if (masked) {
           const int vis = limit - key0;
 #pragma unroll
-          for (int c = 0; c < 64; ++c) s[c] = c < vis ? s[c] : -INFINITY;
+          for (int c = 0; c < 128; ++c) s[c] = c < vis ? s[c] : -INFINITY;
         }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
+        auto row_max = [&]() {
+          float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < 60; c += 8)
+          for (int c = 4; c < 124; c += 8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = max3_nan(mx[e], s[c + e], s[c + 4 + e]);
-        float bm = max3_nan(max3_nan(mx[0], mx[1], s[60]), max3_nan(mx[2], mx[3], s[61]), max_nan(s[62], s[63]));
-        bm = max_nan(bm, swap(bm));
-        const bool need = j > 0 && !(bm <= m + grow);  // a NaN, too
-        if (j == 0) m = bm;
-        bool plain = masked;
-        if (__any_sync(0xffffffffu, need || !(fabsf(m) < INFINITY))) {
-          if (j > 0) {
-            const float alpha = need ? fast_exp2((m - bm) * scale) : 1.f;
-            if (need) m = bm;
-            l *= alpha;
-#pragma unroll 1
-            for (int c = 0; c < D / 2; c += 16) {
-              float o[16];
-              umma::tmem_ld16(o_ta + c, o);
-              umma::tmem_wait_ld16(o);
+            for (int e = 0; e < 4; ++e) mx[e] = max3_nan(mx[e], s[c + e], s[c + 4 + e]);
+          return max3_nan(max3_nan(mx[0], mx[1], s[124]), max3_nan(mx[2], mx[3], s[125]), max_nan(s[126], s[127]));
+        };
+        if (j == 0) m = row_max();
+        // infinite and NaN scores go through the exponential unit, which knows them
+        bool fast = !masked && __all_sync(0xffffffffu, fabsf(m) < INFINITY);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] *= alpha;
-              umma::tmem_st16(o_ta + c, o);
+        for (int h = 0; h < 2; ++h) {
+          float sum;
+          for (bool again = false;; again = true) {
+            const float neg = m == -INFINITY ? 0.f : -m * scale;
+            sum = fast ? row_probabilities<true>(s + 64 * h, scale, neg, s_ta + 32 * h)
+                       : row_probabilities<false>(s + 64 * h, scale, neg, s_ta + 32 * h);
+            // Past the reference by more than 2^60 (or no reference yet, every key so far being masked): the
+            // reference becomes the block's maximum, O and l are rescaled and this half is done again, once.  A
+            // NaN stays one; a row without a key so far has none to refer to.
+            const bool move = (!(sum < kGrow) || (m == -INFINITY && sum > 0.f)) && m == m && m < INFINITY;
+            if (again || !__any_sync(0xffffffffu, move)) break;
+            if (h == 1) {  // the MMAs over the first half add to O
+              ok = warp_wait(&pv_half[t], sn & 1);
+              if (!ok) break;
+              umma::fence_after_sync();
             }
+            const float bm = row_max();
+            const float alpha = move ? fast_exp2(((m == -INFINITY ? bm : m) - bm) * scale) : 1.f;
+            if (move) m = bm;
+            l *= alpha;
+            if (j > 0 || h == 1) {
+#pragma unroll 1
+              for (int c = 0; c < D; c += 16) {
+                float o[16];
+                umma::tmem_ld16(o_ta + c, o);
+                umma::tmem_wait_ld16(o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                umma::tmem_st16(o_ta + c, o);
+              }
+            }
+            fast = false;
           }
-          // infinite and NaN scores go through the exponential unit, which knows them
-          plain = plain || __any_sync(0xffffffffu, !(fabsf(m) < INFINITY));
+          if (!ok) break;
+          l += sum;
+          signal(h == 0 ? &p_half[t] : &p_full[t]);
         }
-        const float neg = m == -INFINITY ? 0.f : -m * scale;
-        auto first = [&]() { signal(&p_half[t]); };
-        l += plain ? row_probabilities<false>(s, scale, neg, s_ta, first)
-                   : row_probabilities<true>(s, scale, neg, s_ta, first);
-        signal(&p_full[t]);
+        if (!ok) break;
       }
       if (!ok) break;
-      if (any_row) l += swap(l);
       ok = warp_wait(&o_full[t], on & 1);
       if (!ok) break;
       ++on;
       umma::fence_after_sync();
       if (any_row) {
-        // Rows leave through shared memory, 32 bytes of a row at a time, so that a store covers whole sectors.
-        constexpr int RP = Geo::STAGE / 32;  // rows a pass
+        // Rows leave through shared memory, 64 bytes of a row at a time, so that a store covers whole sectors.
         uint8_t* const stage = smem + Geo::STAGED + warp * Geo::STAGE;
-        uint8_t* const put = stage + (lane % RP) * 32;
-        const int flip = (lane >> 2) & 1;    // which of the two 16-byte places comes first: no bank conflicts
         const bool direct = it.slot < 0;
         const float inv = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         int64_t at = -1;  // this row's first byte
         if (limit > 0) {
           if (direct) {
             at = 2 * (static_cast<int64_t>(it.row0 + vt) * p.o_st +
-                      static_cast<int64_t>(it.head * p.n_rep + rep) * p.o_sh + half * (D / 2));
+                      static_cast<int64_t>(it.head * p.n_rep + rep) * p.o_sh);
           } else {
             const int64_t r = it.slot + t * kRowTile + row;
-            if (half == 0) p.part_ml[r] = make_float2(m * scale, l);
-            at = 4 * (r * D + half * (D / 2));
+            p.part_ml[r] = make_float2(m * scale, l);
+            at = 4 * r * D;
           }
         }
         uint8_t* const base = direct ? reinterpret_cast<uint8_t*>(p.out) : reinterpret_cast<uint8_t*>(p.part_o);
-        const int cols = direct ? 16 : 8;    // columns of a step
-        for (int c = 0; c < D / 2; c += cols) {
-          uint4 x[2];
+        const int cols = direct ? 32 : 16;    // columns of a step
+        for (int c = 0; c < D; c += cols) {
+          uint4 x[4];
           if (direct) {
-            float o[16];
-            umma::tmem_ld16(o_ta + c, o);
-            umma::tmem_wait_ld16(o);
+            float o[32];
+            umma::tmem_ld32(o_ta + c, o);
+            umma::tmem_wait_ld32(o);
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 4; ++e)
               x[e] = make_uint4(pack_bf16(o[8 * e] * inv, o[8 * e + 1] * inv), pack_bf16(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
                                 pack_bf16(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
                                 pack_bf16(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
           } else {
-            float o[8];
-            umma::tmem_ld8(o_ta + c, o);
-            umma::tmem_wait_ld8(o);
+            float o[16];
+            umma::tmem_ld16(o_ta + c, o);
+            umma::tmem_wait_ld16(o);
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 4; ++e)
               x[e] = make_uint4(__float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]), __float_as_uint(o[4 * e + 2]),
                                 __float_as_uint(o[4 * e + 3]));
           }
+          // 16-byte chunk e of row r lies at place e ^ (r / 2 % 4): no bank conflicts either way
 #pragma unroll
-          for (int pass = 0; pass < 32 / RP; ++pass) {
-            if (lane / RP == pass) {
-              *reinterpret_cast<uint4*>(put + (flip << 4)) = x[0];
-              *reinterpret_cast<uint4*>(put + ((flip ^ 1) << 4)) = x[1];
-            }
-            __syncwarp();
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) = x[e];
+          __syncwarp();
 #pragma unroll
-            for (int g = 0; g < RP / 16; ++g) {
-              const int r = g * 16 + lane / 2, ch = lane & 1;
-              const int64_t to = __shfl_sync(0xffffffffu, at, pass * RP + r);
-              const uint4 y = *reinterpret_cast<const uint4*>(stage + r * 32 + ((ch ^ ((r >> 2) & 1)) << 4));
-              if (to >= 0) *reinterpret_cast<uint4*>(base + to + c * (direct ? 2 : 4) + ch * 16) = y;
-            }
-            __syncwarp();
+          for (int g = 0; g < 4; ++g) {
+            const int r = g * 8 + lane / 4, ch = lane & 3;
+            const int64_t to = __shfl_sync(0xffffffffu, at, r);
+            const uint4 y = *reinterpret_cast<const uint4*>(stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4));
+            if (to >= 0) *reinterpret_cast<uint4*>(base + to + c * (direct ? 2 : 4) + ch * 16) = y;
           }
+          __syncwarp();
         }
         umma::fence_before_sync();  // O is read: the arrival for the next item's first block lets its MMAs write it
       }
@@ -910,15 +893,13 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         }
         __syncwarp();
       };
-      auto pv = [&](int t, uint32_t slot, int h, bool acc) {  // keys 32 h .. and 64 + 32 h .. (32 each) of the block
+      auto pv = [&](int t, uint32_t slot, int h, bool acc) {  // keys 64 h .. of the block
         if (elect_one()) {
           const uint64_t vd = v_desc + slot * (Geo::TILE >> 4);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const int half = kk >> 1, step = 2 * h + (kk & 1);  // 16 keys each; P of a half starts where its scores did
-            umma::mma_f16_ts(o_col[t], s_col[t] + half * 64 + step * 8, vd + (half * 4 + step) * (2048 >> 4), id_pv,
-                             acc || kk > 0);
-          }
+          for (int kk = 0; kk < 4; ++kk)
+            umma::mma_f16_ts(o_col[t], s_col[t] + (4 * h + kk) * 8, vd + (4 * h + kk) * (2048 >> 4), id_pv, acc || kk > 0);
+          if (h == 0) umma::commit(&pv_half[t]);
         }
         __syncwarp();
       };
