@@ -46,8 +46,8 @@ constexpr int kItemsKept = 32;     // items of a CTA that it keeps in shared mem
 constexpr float kExpC0 = 0.999924541f, kExpC1 = 0.693136752f, kExpC2 = 0.242639482f, kExpC3 = 0.0558382832f;
 
 enum RowSource { kPacked = 0, kPaged = 1, kPagedE4M3 = 2 };
+constexpr int kLoadWarp = 0, kIssueWarp = 1, kQueryWarp = 3, kSoftmaxWarp = 4, kWidenWarp = 12;
 constexpr int kSoftmaxWarps = 8;  // four a row tile
-constexpr int kLoadWarp = kSoftmaxWarps, kIssueWarp = kLoadWarp + 1, kQueryWarp = kLoadWarp + 2, kWidenWarp = kLoadWarp + 4;
 // Threads, and registers a thread of the softmax warps and of the others: the launch's own are what
 // __launch_bounds__ leaves (168, E4M3 128), and the shares add up to them.
 template <int SRC>
@@ -347,8 +347,8 @@ struct RowGeom {
   static_assert(!V8 || D == 128, "E4M3 V needs head_dim 128");
   static constexpr int KH = D / 64;               // 128-byte dim halves
   static constexpr int TILE = 16384 * KH;         // one K or V block, one query tile
-  // ring slots (a K or a V block each; E4M3: an even number, so that a slot is always one or the other's)
-  static constexpr int NS = D == 128 ? 4 : 11;
+  // ring slots, a K or a V block each: K in 0 and 2, V in 1 and 3
+  static constexpr int NS = 4;
   static constexpr int NRAW = 1;                  // E4M3: blocks of codes
   static constexpr int RING = 2 * TILE;           // the ring lies behind the two query tiles
   static constexpr int RAW = RING + NS * TILE;
@@ -367,19 +367,38 @@ SD_DEV RowItem load_item(const RowItem* at) {
   for (int i = 0; i < 3; ++i) d[i] = s[i];
   return it;
 }
-// blocks of row tile t of an item
-SD_DEV int tile_blocks(const RowParams& p, const RowItem& it, int t) {
+// half blocks (64 keys) of row tile t of an item
+SD_DEV int tile_halves(const RowParams& p, const RowItem& it, int t) {
   const int v0 = it.vt0 + t * p.tpt;
   if (v0 >= it.n_vt) return 0;
-  if (it.src < 0) return it.nblk;
-  const int end = min(it.first + min(v0 + p.tpt, it.n_vt), it.k1);
-  return end <= it.k0 ? 0 : (end - it.k0 + kKeyBlock - 1) / kKeyBlock;
+  const int end = it.src < 0 ? it.k1 : min(it.first + min(v0 + p.tpt, it.n_vt), it.k1);
+  return end <= it.k0 ? 0 : (end - it.k0 + kKeyBlock / 2 - 1) / (kKeyBlock / 2);
 }
 
-SD_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// Bounded waits of this kernel's warps, most of which wait most of the time: the hint lets the hardware put a warp
+// to sleep for up to a millisecond instead of having it poll beside the softmax warps.
+SD_DEV bool mbar_try_sleep(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
 }
-SD_DEV void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+SD_DEV bool row_wait(uint64_t* bar, uint32_t parity) {
+  bool got = mbar_try_sleep(bar, parity);
+  if (!got) {
+    const uint64_t t0 = globaltimer_ns();
+    do {
+      got = mbar_try_sleep(bar, parity);
+    } while (!got && globaltimer_ns() - t0 < kWaitLimitNs);
+  }
+  return __all_sync(0xffffffffu, got);
+}
+
 // 3-D tiled load that stays in L2 as the hardware sees fit (K/V blocks are read again by other CTAs)
 SD_DEV void tma_tile_3d(void* dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2, uint64_t* bar) {
   asm volatile(
@@ -556,37 +575,39 @@ SD_DEV float row_probabilities(const float* s, float scale, float neg, uint32_t 
 
 template <int D, int SRC>
 __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kernel(
-    const RowParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-    const __grid_constant__ CUtensorMap vmap) {
+    const RowParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap tmap,
+    const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   constexpr bool V8 = RowRoles<SRC>::V8;
   using Geo = RowGeom<D, V8>;
   constexpr int NS = Geo::NS, KH = Geo::KH;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[NS], empty[NS], raw_full, raw_empty;
-  __shared__ uint64_t q_full, q_empty, s_full[2], p_half[2], pv_half[2], p_full[2], o_full[2], c_req, v_clean, fin;
+  __shared__ uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], pv_done[2], o_full[2], c_req, v_clean, fin[2];
   __shared__ RowItem s_items[kItemsKept];  // the CTA's first items
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], V8 && (s & 1) ? 4 : 1);  // a TMA block, or the four widening warps
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);  // both MMA warps have read it
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_half[t], 4);
-      mbar_init(&pv_half[t], 1);
-      mbar_init(&p_full[t], 4);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&s_full[t][h], 1);
+        mbar_init(&p_full[t][h], 4);
+      }
+      mbar_init(&pv_done[t], 1);
       mbar_init(&o_full[t], 1);
     }
     mbar_init(&raw_full, 1);
     mbar_init(&raw_empty, 4);
-    mbar_init(&q_full, 2);
-    mbar_init(&q_empty, 1);
-    mbar_init(&c_req, 1);
+    mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 2);
+    mbar_init(&c_req, 2);
     mbar_init(&v_clean, 1);
-    mbar_init(&fin, 1);
+    mbar_init(&fin[0], 1);
+    mbar_init(&fin[1], 1);
     fence_barrier_init();
   }
   if (warp == kIssueWarp) {
@@ -595,6 +616,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   }
   if (warp == kLoadWarp && lane == 0) {
     prefetch_tmap(&qmap);
+    if (p.G > 0) prefetch_tmap(&tmap);
     prefetch_tmap(&kmap);
     prefetch_tmap(&vmap);
   }
@@ -609,23 +631,17 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   const uint32_t tmem = s_tmem;
   auto item_at = [&](int i) { return i - i0 < kItemsKept ? s_items[i - i0] : load_item(p.items + i); };
 
-  if (warp < kSoftmaxWarps) {
+  if (warp >= kSoftmaxWarp && warp < kWidenWarp) {
     more_regs<RowRoles<SRC>::SOFTMAX_REGS>();
     // ------------------------------------------------------------ softmax and epilogue: a thread a row
-    const int t = warp >> 2, row = tid & 127;
+    const int t = (warp - kSoftmaxWarp) >> 2, row = tid & 127;
     const int tok = row / p.n_rep, rep = row - tok * p.n_rep;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 5;
     const uint32_t s_ta = umma::taddr(tmem, lanes, Geo::S_COL + t * 128);
     const uint32_t o_ta = umma::taddr(tmem, lanes, Geo::O_COL + t * D);
     const float scale = p.scale_log2;
-    uint32_t sn = 0, on = 0;
+    uint32_t sn = 0, pv = 0, on = 0;  // phase bits of s_full; halves handed over
     bool ok = true;
-    auto signal = [&](uint64_t* bar) {
-      umma::tmem_wait_st();
-      umma::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
     for (int i = i0; i <= i1 && ok; ++i) {
       const RowItem it = item_at(i);
       if (it.nblk == 0) continue;
@@ -640,97 +656,97 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           if (vt - mb * p.q_max < p.member_row[it.member0 + mb].y) limit = it.k1;
         }
       }
-      const int nb = tile_blocks(p, it, t);
-      if (nb == 0) {  // no tile, or a piece past the tile's keys: the row's other pieces are all of it
+      const int nh = tile_halves(p, it, t);
+      if (nh == 0) {  // no tile, or a piece past the tile's keys: the row's other pieces are all of it
         if (it.slot >= 0 && limit > 0) p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
         continue;
       }
       const bool any_row = __any_sync(0xffffffffu, limit > 0);
       const int least = __reduce_min_sync(0xffffffffu, limit > 0 ? limit : 0x7fffffff);
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < nb; ++j, ++sn) {
-        ok = warp_wait(&s_full[t], sn & 1);
+      for (int k = 0; k < nh; ++k) {
+        const int h = k & 1;
+        ok = row_wait(&s_full[t][h], (sn >> h) & 1);
         if (!ok) break;
+        sn ^= 1u << h;
         umma::fence_after_sync();
         if (!any_row) {
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&p_half[t]);
-            mbar_arrive(&p_full[t]);
-          }
+          if (lane == 0) mbar_arrive(&p_full[t][h]);
+          ++pv;
           continue;
         }
-        float s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) umma::tmem_ld32(s_ta + 32 * c, s + 32 * c);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) umma::tmem_wait_ld32(s + 32 * c);
-        const int key0 = it.k0 + j * kKeyBlock;
-        const bool masked = least < key0 + kKeyBlock;
+        float s[64];
+        umma::tmem_ld32(s_ta + 64 * h, s);
+        umma::tmem_ld32(s_ta + 64 * h + 32, s + 32);
+        umma::tmem_wait_ld32(s);
+        umma::tmem_wait_ld32(s + 32);
+        const int key0 = it.k0 + k * (kKeyBlock / 2);
+        const bool masked = least < key0 + kKeyBlock / 2;
         if (masked) {
           const int vis = limit - key0;
 #pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = c < vis ? s[c] : -INFINITY;
+          for (int c = 0; c < 64; ++c) s[c] = c < vis ? s[c] : -INFINITY;
         }
         auto row_max = [&]() {
           float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int c = 4; c < 124; c += 8)
+          for (int c = 4; c < 60; c += 8)
 #pragma unroll
             for (int e = 0; e < 4; ++e) mx[e] = max3_nan(mx[e], s[c + e], s[c + 4 + e]);
-          return max3_nan(max3_nan(mx[0], mx[1], s[124]), max3_nan(mx[2], mx[3], s[125]), max_nan(s[126], s[127]));
+          return max3_nan(max3_nan(mx[0], mx[1], s[60]), max3_nan(mx[2], mx[3], s[61]), max_nan(s[62], s[63]));
         };
-        if (j == 0) m = row_max();
+        if (k == 0) m = row_max();
         // infinite and NaN scores go through the exponential unit, which knows them
         bool fast = !masked && __all_sync(0xffffffffu, fabsf(m) < INFINITY);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float sum;
-          for (bool again = false;; again = true) {
-            const float neg = m == -INFINITY ? 0.f : -m * scale;
-            sum = fast ? row_probabilities<true>(s + 64 * h, scale, neg, s_ta + 32 * h)
-                       : row_probabilities<false>(s + 64 * h, scale, neg, s_ta + 32 * h);
-            // Past the reference by more than 2^60 (or no reference yet, every key so far being masked): the
-            // reference becomes the block's maximum, O and l are rescaled and this half is done again, once.  A
-            // NaN stays one; a row without a key so far has none to refer to.
-            const bool move = (!(sum < kGrow) || (m == -INFINITY && sum > 0.f)) && m == m && m < INFINITY;
-            if (again || !__any_sync(0xffffffffu, move)) break;
-            if (h == 1) {  // the MMAs over the first half add to O
-              ok = warp_wait(&pv_half[t], sn & 1);
-              if (!ok) break;
-              umma::fence_after_sync();
-            }
-            const float bm = row_max();
-            const float alpha = move ? fast_exp2(((m == -INFINITY ? bm : m) - bm) * scale) : 1.f;
-            if (move) m = bm;
-            l *= alpha;
-            if (j > 0 || h == 1) {
-#pragma unroll 1
-              for (int c = 0; c < D; c += 16) {
-                float o[16];
-                umma::tmem_ld16(o_ta + c, o);
-                umma::tmem_wait_ld16(o);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] *= alpha;
-                umma::tmem_st16(o_ta + c, o);
-              }
-            }
-            fast = false;
+        float sum;
+        for (bool again = false;; again = true) {
+          const float neg = m == -INFINITY ? 0.f : -m * scale;
+          sum = fast ? row_probabilities<true>(s, scale, neg, s_ta + 64 * h)
+                     : row_probabilities<false>(s, scale, neg, s_ta + 64 * h);
+          // Past the reference by more than 2^60 (or no reference yet, every key so far being masked): the
+          // reference becomes this half block's maximum, O and l are rescaled and it is done again, once.  A NaN
+          // stays one; a row without a key so far has none to refer to.
+          const bool move = (!(sum < kGrow) || (m == -INFINITY && sum > 0.f)) && m == m && m < INFINITY;
+          if (again || !__any_sync(0xffffffffu, move)) break;
+          if (k > 0) {  // the MMAs over the half before this add to O
+            ok = row_wait(&pv_done[t], (pv - 1) & 1);
+            if (!ok) break;
+            umma::fence_after_sync();
           }
-          if (!ok) break;
-          l += sum;
-          signal(h == 0 ? &p_half[t] : &p_full[t]);
+          const float bm = row_max();
+          const float alpha = move ? fast_exp2(((m == -INFINITY ? bm : m) - bm) * scale) : 1.f;
+          if (move) m = bm;
+          l *= alpha;
+          if (k > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              umma::tmem_ld16(o_ta + c, o);
+              umma::tmem_wait_ld16(o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= alpha;
+              umma::tmem_st16(o_ta + c, o);
+            }
+          }
+          fast = false;
         }
         if (!ok) break;
+        l += sum;
+        ++pv;
+        umma::tmem_wait_st();
+        umma::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t][h]);
       }
       if (!ok) break;
-      ok = warp_wait(&o_full[t], on & 1);
+      ok = row_wait(&o_full[t], on & 1);
       if (!ok) break;
       ++on;
       umma::fence_after_sync();
       if (any_row) {
         // Rows leave through shared memory, 64 bytes of a row at a time, so that a store covers whole sectors.
-        uint8_t* const stage = smem + Geo::STAGED + warp * Geo::STAGE;
+        uint8_t* const stage = smem + Geo::STAGED + (warp - kSoftmaxWarp) * Geo::STAGE;
         const bool direct = it.slot < 0;
         const float inv = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         int64_t at = -1;  // this row's first byte
@@ -793,7 +809,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       for (int i = i0; i <= i1 && ok; ++i) {
         const RowItem it = item_at(i);
         if (it.nblk == 0) continue;
-        const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+        const int nb = (max(tile_halves(p, it, 0), tile_halves(p, it, 1)) + 1) / 2;
         int ids = 0;  // paged: lane l holds the page of keys 16 (32 (j / 4) + l) ..
         for (int j = 0; j < nb && ok; ++j) {
           if (SRC != kPacked && (j & 3) == 0) {
@@ -810,7 +826,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             const uint32_t s = n % NS, round = n / NS;
             if (V8 && kv) {  // codes; the widening warps take care of the block's ring slot
               const uint32_t r = n >> 1;
-              if (r > 0 && !warp_wait(&raw_empty, (r - 1) & 1)) {
+              if (r > 0 && !row_wait(&raw_empty, (r - 1) & 1)) {
                 ok = false;
                 break;
               }
@@ -827,7 +843,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
               __syncwarp();
               continue;
             }
-            if (round > 0 && !warp_wait(&empty[s], (round - 1) & 1)) {
+            if (round > 0 && !row_wait(&empty[s], (round - 1) & 1)) {
               ok = false;
               break;
             }
@@ -863,43 +879,46 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
         // copies under way land before the CTA leaves
         for (uint32_t k = n > NS ? n - NS : 0; k < n; ++k)
-          (void)(V8 && (k & 1) ? warp_wait(&raw_full, (k >> 1) & 1) : warp_wait(&full[k % NS], (k / NS) & 1));
+          (void)(V8 && (k & 1) ? row_wait(&raw_full, (k >> 1) & 1) : row_wait(&full[k % NS], (k / NS) & 1));
       }
-    } else if (warp == kIssueWarp) {
-      // ---------------------------------------------------------- MMA issue
-      constexpr uint32_t id_qk = umma::idesc_f16(128, kKeyBlock, true, true, false, false);
+    } else if (warp < kQueryWarp) {
+      // ---------------------------------------------------------- MMA issue, a warp a row tile
+      // What such a warp does between two products is time that its tile waits for, and the tensor cores hold few
+      // products ahead: one warp for both tiles was the bound (4300 clocks a block against 2600 of products).
+      const int t = warp - kIssueWarp;
+      constexpr uint32_t id_qk = umma::idesc_f16(128, kKeyBlock / 2, true, true, false, false);
       constexpr uint32_t id_pv = umma::idesc_f16(128, D, true, true, false, true);
-      // a descriptor's low bits are the address in units of 16 bytes
-      const uint64_t q_desc = umma::desc_kmajor_sw128(smem_u32(smem));
-      const uint64_t k_desc = umma::desc_kmajor_sw128(smem_u32(smem + Geo::RING));
-      const uint64_t v_desc = umma::desc_mnmajor_sw128(smem_u32(smem + Geo::RING), 16384);
-      const uint32_t s_col[2] = {umma::taddr(tmem, 0, Geo::S_COL), umma::taddr(tmem, 0, Geo::S_COL + 128)};
-      const uint32_t o_col[2] = {umma::taddr(tmem, 0, Geo::O_COL), umma::taddr(tmem, 0, Geo::O_COL + D)};
-      uint32_t pn[2] = {0, 0}, items = 0, cleaned = 0;
-      uint32_t ks = 0, kp = 0;  // ring slot of the next K block, and its phase
+      constexpr uint32_t high = umma::desc_high(1024, umma::kSwizzle128B);
+      const uint32_t q_low = umma::desc_low(smem_u32(smem) + t * Geo::TILE, 16);
+      const uint32_t k_low = umma::desc_low(smem_u32(smem + Geo::RING), 16);
+      const uint32_t v_low = umma::desc_low(smem_u32(smem + Geo::RING), 16384);
+      const uint32_t s_col = tmem + Geo::S_COL + t * 128, o_col = tmem + Geo::O_COL + t * D;
+      uint32_t pn = 0, items = 0, cleaned = 0;  // pn: phase bits of p_full
+      uint32_t ks = 0, kp = 0;  // ring slot of the next block in the ring, and its phase
       bool ok = true;
       auto next = [&](uint32_t& s, uint32_t& ph) {
         if (++s == NS) s = 0, ph ^= 1;
       };
-      auto qk = [&](int t, uint32_t slot) {
+      auto qk = [&](int h, uint32_t slot) {  // keys 64 h .. of the block
+        const uint32_t kl = k_low + slot * (Geo::TILE >> 4);
         if (elect_one()) {
-          const uint64_t qd = q_desc + t * (Geo::TILE >> 4), kd = k_desc + slot * (Geo::TILE >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t at = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
-            umma::mma_f16_ss(s_col[t], qd + at, kd + at, id_qk, kk > 0);
+            umma::mma_f16_ss_low<id_qk, high>(s_col + 64 * h, q_low, at, kl, h * (8192 >> 4) + at, kk > 0);
           }
-          umma::commit(&s_full[t]);
+          umma::commit(&s_full[t][h]);
         }
         __syncwarp();
       };
-      auto pv = [&](int t, uint32_t slot, int h, bool acc) {  // keys 64 h .. of the block
+      auto pv = [&](int h, uint32_t slot, bool acc) {
+        const uint32_t vl = v_low + slot * (Geo::TILE >> 4);
         if (elect_one()) {
-          const uint64_t vd = v_desc + slot * (Geo::TILE >> 4);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma::mma_f16_ts(o_col[t], s_col[t] + (4 * h + kk) * 8, vd + (4 * h + kk) * (2048 >> 4), id_pv, acc || kk > 0);
-          if (h == 0) umma::commit(&pv_half[t]);
+            umma::mma_f16_ts_low<id_pv, high>(o_col, s_col, 64 * h + kk * 8, vl, h * (8192 >> 4) + kk * (2048 >> 4),
+                                              acc || kk > 0);
+          umma::commit(&pv_done[t]);
         }
         __syncwarp();
       };
@@ -910,55 +929,44 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       for (int i = i0; i <= i1 && ok; ++i) {
         const RowItem it = item_at(i);
         if (it.nblk == 0) continue;
-        const int nt[2] = {tile_blocks(p, it, 0), tile_blocks(p, it, 1)};
-        const int nb = max(nt[0], nt[1]);
+        // (a reduction's result is known to be the same in all lanes: loops and descriptors stay in uniform registers)
+        const int nh = __reduce_max_sync(0xffffffffu, tile_halves(p, it, t));
+        const int nb = (max(nh, __reduce_max_sync(0xffffffffu, tile_halves(p, it, t ^ 1))) + 1) / 2;
         const bool clean = !V8 && (it.k1 - it.k0) % kKeyBlock != 0;
-        ok = warp_wait(&q_full, items & 1) && warp_wait(&full[ks], kp);
+        ok = row_wait(&q_full, items & 1) && row_wait(&full[ks], kp);
         if (!ok) break;
         umma::fence_after_sync();
-        if (nt[0] > 0) qk(0, ks);
-        if (nt[1] > 0) qk(1, ks);
+        if (nh > 0) qk(0, ks);
+        if (nh > 1) qk(1, ks);
         if (nb == 1) commit(&q_empty);
         commit(&empty[ks]);
         next(ks, kp);
-        for (int j = 0; j < nb && ok; ++j) {
+        for (int j = 0; j < nb; ++j) {
           const uint32_t vs = ks, vp = kp;  // this block's V; then the next block's K
           next(ks, kp);
-          ok = warp_wait(&full[vs], vp);
-          const bool last = j == nb - 1, wash = clean && last;
-          // the last block's V is zeroed past the last key while the softmax works on the block
-          if (wash && ok) {
+          const bool last = j == nb - 1;
+          ok = row_wait(&full[vs], vp);
+          if (!last) ok = ok && row_wait(&full[ks], kp);
+          if (!ok) break;
+          umma::fence_after_sync();
+          if (clean && last) {
+            // the last block's V is zeroed past the last key while the softmax works on the block
             if (lane == 0) mbar_arrive(&c_req);
             __syncwarp();
+            if (2 * j < nh) ok = row_wait(&v_clean, cleaned & 1);
+            ++cleaned;
           }
-          bool washed = !wash, k_in = false;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (j >= nt[t] || !ok) continue;
-            ok = warp_wait(&p_half[t], pn[t] & 1);
-            if (!washed) {
-              ok = ok && warp_wait(&v_clean, cleaned & 1);
-              ++cleaned;
-              washed = true;
-            }
-            if (!ok) continue;
-            umma::fence_after_sync();
-            pv(t, vs, 0, j > 0);
-            ok = warp_wait(&p_full[t], pn[t] & 1);
-            if (!ok) continue;
-            ++pn[t];
-            umma::fence_after_sync();
-            pv(t, vs, 1, true);
-            if (j == nt[t] - 1) {
-              commit(&o_full[t]);
-            } else {
-              if (!k_in) {
-                ok = warp_wait(&full[ks], kp);
-                if (!ok) continue;
-                k_in = true;
-                umma::fence_after_sync();
-              }
-              qk(t, ks);
+          for (int h = 0; h < 2; ++h) {
+            const int k = 2 * j + h;
+            if (k < nh) {
+              ok = ok && row_wait(&p_full[t][h], (pn >> h) & 1);
+              if (!ok) break;
+              pn ^= 1u << h;
+              umma::fence_after_sync();
+              pv(h, vs, k > 0);
+              if (k == nh - 1) commit(&o_full[t]);
+              if (k + 2 < nh) qk(h, ks);
             }
           }
           if (!ok) break;
@@ -972,64 +980,60 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         ++items;
       }
       if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-      commit(&fin);
-      (void)warp_wait(&fin, 0);
-    } else if (warp < kWidenWarp) {
+      commit(&fin[t]);
+      (void)row_wait(&fin[t], 0);
+    } else if (warp == kQueryWarp) {
       // ---------------------------------------------------------- query rows; V rows past the last key
-      const int t = warp - kQueryWarp;
       uint32_t items = 0, cleaned = 0, n = 0;
       bool ok = true;
       for (int i = i0; i <= i1 && ok; ++i) {
         const RowItem it = item_at(i);
         if (it.nblk == 0) continue;
         const int tiles = it.vt0 + p.tpt < it.n_vt ? 2 : 1;
-        if (items > 0) ok = warp_wait(&q_empty, (items - 1) & 1);
+        if (items > 0) ok = row_wait(&q_empty, (items - 1) & 1);
         if (!ok) break;
         ++items;
-        if (it.src >= 0) {  // a sequence's rows are a box of n_rep heads x tpt tokens; rows past it meet no other row
-          if (t == 0 && lane == 0) {
+        if (it.src >= 0) {
+          // a sequence's rows are a box of n_rep heads x tpt tokens a tile; rows past it meet no other row
+          if (lane == 0) {
             mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(tiles * KH * 128 * p.n_rep * p.tpt));
             for (int e = 0; e < tiles; ++e)
 #pragma unroll
               for (int x = 0; x < KH; ++x)
                 tma_tile_3d(smem + e * Geo::TILE + x * 16384, &qmap, x * 64, it.head * p.n_rep,
                             it.row0 + it.vt0 + e * p.tpt, &q_full);
-          } else if (t == 1 && lane == 0) {
-            mbar_arrive(&q_full);
           }
         } else {
-          // a group's rows are anywhere: 16 bytes a lane, a tile a warp
-          constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte chunks of a row, rows a step
-          const uint32_t q_base = smem_u32(smem) + t * Geo::TILE;
-          for (int base = 0; base < (t < tiles ? kRowTile : 0); base += 32) {
-            const int r = base + lane, tok = r / p.n_rep, vt = it.vt0 + t * p.tpt + tok;
-            int64_t off = -1;
-            if (tok < p.tpt && vt < it.n_vt) {
-              const int mb = vt / p.q_max, e = vt - mb * p.q_max;
-              const int2 mr = p.member_row[it.member0 + mb];
-              if (e < mr.y)
-                off = static_cast<int64_t>(mr.x + e) * p.q_st +
-                      static_cast<int64_t>(it.head * p.n_rep + r - tok * p.n_rep) * p.q_sh;
-            }
-#pragma unroll 4
-            for (int e = 0; e < 32; e += RP) {
-              const int64_t o = __shfl_sync(0xffffffffu, off, e + lane / CH);
-              const int rr = base + e + lane / CH, ch = lane % CH;
-              cp_async16(q_base + (ch >> 3) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4),
-                         p.q + (o < 0 ? 0 : o + ch * 8), o < 0 ? 0u : 16u);
-            }
+          // a group's rows are anywhere: a box of n_rep heads a token (the swizzle goes by the address, so that a
+          // token may start in the middle of its pattern)
+          const int tokens = min(2 * p.tpt, it.n_vt - it.vt0);
+          int mine = 0;
+          for (int base = 0; base < tokens; base += 32) {
+            const int vt = it.vt0 + base + lane, mb = vt / p.q_max;
+            if (base + lane < tokens) mine += vt - mb * p.q_max < p.member_row[it.member0 + mb].y;
           }
-          cp_async_wait_all();
-          fence_proxy_async();
+          mine = __reduce_add_sync(0xffffffffu, mine);
+          if (lane == 0) mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(mine * KH * 128 * p.n_rep));
           __syncwarp();
-          if (lane == 0) mbar_arrive(&q_full);
+          for (int base = 0; base < tokens; base += 32) {
+            const int in = base + lane, vt = it.vt0 + in, mb = vt / p.q_max, e = vt - mb * p.q_max;
+            if (in >= tokens) continue;
+            const int2 mr = p.member_row[it.member0 + mb];
+            if (e >= mr.y) continue;
+            const int tile = in / p.tpt;
+            uint8_t* dst = smem + tile * Geo::TILE + (in - tile * p.tpt) * p.n_rep * 128;
+#pragma unroll
+            for (int x = 0; x < KH; ++x)
+              tma_tile_3d(dst + x * 16384, &tmap, x * 64, it.head * p.n_rep, mr.x + e, &q_full);
+          }
         }
-        const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+        __syncwarp();
+        const int nb = (max(tile_halves(p, it, 0), tile_halves(p, it, 1)) + 1) / 2;
         const int rem = (it.k1 - it.k0) % kKeyBlock;
-        if (t == 1 && !V8 && rem != 0) {
+        if (!V8 && rem != 0) {
           const uint32_t k = n + 2 * nb - 1;
-          // asked for by the MMA warp, which has seen the block arrive and waits for the answer
-          ok = warp_wait(&c_req, cleaned & 1);
+          // asked for by the MMA warps, which have seen the block arrive and wait for the answer
+          ok = row_wait(&c_req, cleaned & 1);
           if (!ok) break;
           uint8_t* v = smem + Geo::RING + (k % NS) * Geo::TILE;
 #pragma unroll
@@ -1053,7 +1057,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         for (int i = i0; i <= i1 && ok; ++i) {
           const RowItem it = item_at(i);
           if (it.nblk == 0) continue;
-          const int nb = max(tile_blocks(p, it, 0), tile_blocks(p, it, 1));
+          const int nb = (max(tile_halves(p, it, 0), tile_halves(p, it, 1)) + 1) / 2;
           // the scale of key r of block j; 0 past the last key, where the codes (clamped pages) are finite or NaN
           auto scale_of = [&](int j) {
             const int key = it.k0 + j * kKeyBlock + r;
@@ -1068,8 +1072,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             const bool in = it.k0 + j * kKeyBlock + r < it.k1;
             if (j + 1 < nb) next = scale_of(j + 1);
             const uint32_t s = n % NS;
-            ok = warp_wait(&raw_full, (n >> 1) & 1);
-            if (ok && n >= NS) ok = warp_wait(&empty[s], (n / NS - 1) & 1);
+            ok = row_wait(&raw_full, (n >> 1) & 1);
+            if (ok && n >= NS) ok = row_wait(&empty[s], (n / NS - 1) & 1);
             if (!ok) break;
             const uint8_t* src = smem + Geo::RAW + r * 128;
             uint8_t* dst = smem + Geo::RING + s * Geo::TILE + r * 128;
@@ -1349,7 +1353,8 @@ static int fill_row_params(RowParams& p, const RowShape& s, void* ws, size_t ws_
 }
 
 template <int D, int SRC>
-static int launch_row_attention(const RowParams& p, const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap,
+static int launch_row_attention(const RowParams& p, const CUtensorMap& qmap, const CUtensorMap& tmap, const CUtensorMap& kmap,
+                                const CUtensorMap& vmap,
                                 bool reuse_plan, cudaStream_t st) {
   // the attribute belongs to the function on each device; setting it again is cheap and needs no state of its own
   const cudaError_t e = cudaFuncSetAttribute(row_attention_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1358,7 +1363,7 @@ static int launch_row_attention(const RowParams& p, const CUtensorMap& qmap, con
   if (!reuse_plan)
     if (int rc = launch_pdl("row_plan_kernel", row_plan_kernel, dim3(1), dim3(1024), 0, st, p)) return rc;
   if (int rc = launch_pdl("row_attention_kernel", row_attention_kernel<D, SRC>, dim3(p.grid), dim3(RowRoles<SRC>::THREADS),
-                          RowGeom<D, RowRoles<SRC>::V8>::SMEM, st, p, qmap, kmap, vmap))
+                          RowGeom<D, RowRoles<SRC>::V8>::SMEM, st, p, qmap, tmap, kmap, vmap))
     return rc;
   if (p.G == 0)
     return launch_pdl("join_cut_kernel", join_cut_kernel<D>, dim3(p.grid, kMergeParts), dim3(256), 0, st, p);
@@ -1425,13 +1430,14 @@ extern "C" int specdec_prompt_attention(const SpecdecPromptArgs* a, specdec_stre
   p.q_rows = a->q_rows;
   p.kv_rows = a->kv_rows;
   p.status = a->status;
-  CUtensorMap qm, km, vm;
+  CUtensorMap qm, tm, km, vm;
   if (int rc = encode_packed_map(&qm, a->q, a->q_rows, s.H, s.D, a->q_stride_tok, a->q_stride_head, p.n_rep, p.tpt)) return rc;
+  tm = qm;  // whole prompts have no groups
   if (int rc = encode_packed_map(&km, a->k, a->kv_rows, s.KV, s.D, a->k_stride_tok, a->k_stride_head, 1, kKeyBlock)) return rc;
   if (int rc = encode_packed_map(&vm, a->v, a->kv_rows, s.KV, s.D, a->v_stride_tok, a->v_stride_head, 1, kKeyBlock)) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return s.D == 128 ? launch_row_attention<128, kPacked>(p, qm, km, vm, a->reuse_plan != 0, st)
-                    : launch_row_attention<64, kPacked>(p, qm, km, vm, a->reuse_plan != 0, st);
+  return s.D == 128 ? launch_row_attention<128, kPacked>(p, qm, tm, km, vm, a->reuse_plan != 0, st)
+                    : launch_row_attention<64, kPacked>(p, qm, tm, km, vm, a->reuse_plan != 0, st);
 }
 
 extern "C" size_t specdec_shared_prefix_workspace_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
@@ -1486,12 +1492,13 @@ extern "C" int specdec_shared_prefix_attention(const SpecdecSharedPrefixArgs* a,
   p.v_scale = kv.v_scale;
   p.q_rows = a->q_rows;
   p.status = a->status;
-  CUtensorMap qm, km, vm;
+  CUtensorMap qm, tm, km, vm;
   if (int rc = encode_packed_map(&qm, a->q, a->q_rows, s.H, s.D, a->q_stride_tok, a->q_stride_head, p.n_rep, p.tpt)) return rc;
+  if (int rc = encode_packed_map(&tm, a->q, a->q_rows, s.H, s.D, a->q_stride_tok, a->q_stride_head, p.n_rep, 1)) return rc;
   if (int rc = encode_rows_map(&km, kv.k_pool, static_cast<uint64_t>(page_rows), 2048)) return rc;
   if (int rc = encode_rows_map(&vm, kv.v_pool, static_cast<uint64_t>(v8 ? page_rows / 2 : page_rows), 2048)) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (v8) return launch_row_attention<128, kPagedE4M3>(p, qm, km, vm, a->reuse_plan != 0, st);
-  return s.D == 128 ? launch_row_attention<128, kPaged>(p, qm, km, vm, a->reuse_plan != 0, st)
-                    : launch_row_attention<64, kPaged>(p, qm, km, vm, a->reuse_plan != 0, st);
+  if (v8) return launch_row_attention<128, kPagedE4M3>(p, qm, tm, km, vm, a->reuse_plan != 0, st);
+  return s.D == 128 ? launch_row_attention<128, kPaged>(p, qm, tm, km, vm, a->reuse_plan != 0, st)
+                    : launch_row_attention<64, kPaged>(p, qm, tm, km, vm, a->reuse_plan != 0, st);
 }

@@ -64,16 +64,32 @@ SD_DEV void mma_f16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(no_mask), "r"(no_mask), "r"(no_mask), "r"(no_mask)
       : "memory");
 }
+// The same with descriptors as a low word in a register (address and leading offset) plus a constant, and a constant
+// high word: a run of MMAs over one operand then needs two or three registers, and little is between a wait and it.
+SD_DEV constexpr uint32_t desc_high(uint32_t sbo_bytes, uint32_t layout) {
+  return (sbo_bytes >> 4) | (1u << 14) | (layout << 29);
+}
+SD_DEV uint32_t desc_low(uint32_t saddr, uint32_t lbo_bytes) { return ((saddr >> 4) & 0x3FFFu) | ((lbo_bytes >> 4) << 16); }
+template <uint32_t IDESC, uint32_t HIGH>
+SD_DEV void mma_f16_ss_low(uint32_t d_tmem, uint32_t a_low, uint32_t a_plus, uint32_t b_low, uint32_t b_plus, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y, i, h;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tadd.u32 x, %1, %2;\n\tadd.u32 y, %3, %4;\n\tmov.b32 i, %6;\n\tmov.b32 h, %7;\n\t"
+      "mov.b64 a, {x, h};\n\tmov.b64 b, {y, h};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, i, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_low), "r"(a_plus), "r"(b_low), "r"(b_plus), "r"(acc ? 1u : 0u), "n"(IDESC), "n"(HIGH)
+      : "memory");
+}
 // D[tmem] (+)= A[tmem] * B[smem]^T: A is M x 16 in tensor memory, lane = row, two consecutive
 // K values in a 32-bit column (the even one in its low half), eight columns a K = 16 step.
-SD_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, bool accumulate) {
-  const uint32_t acc = accumulate ? 1u : 0u;
-  const uint32_t no_mask = 0u;
+template <uint32_t IDESC, uint32_t HIGH>
+SD_DEV void mma_f16_ts_low(uint32_t d_tmem, uint32_t a_tmem, uint32_t a_plus, uint32_t b_low, uint32_t b_plus, bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc), "r"(no_mask), "r"(no_mask), "r"(no_mask), "r"(no_mask)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t.reg .b32 x, y, i, h;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tadd.u32 x, %1, %2;\n\tadd.u32 y, %3, %4;\n\tmov.b32 i, %6;\n\tmov.b32 h, %7;\n\t"
+      "mov.b64 b, {y, h};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, i, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(a_plus), "r"(b_low), "r"(b_plus), "r"(acc ? 1u : 0u), "n"(IDESC), "n"(HIGH)
       : "memory");
 }
 // Arrive (once) on `bar` when every tcgen05 operation this thread issued so far has completed.
