@@ -85,74 +85,142 @@ struct RowParams {
   int64_t q_rows, kv_rows;
   int32_t B, H, KV, n_rep, tpt, q_max, G, M;
   int32_t num_pages, max_pages, paged;
-  int32_t grid, compact;        // CTAs of the plan; compact: slots only for cut units
+  int32_t grid, min_quota, compact;  // CTAs of the plan, its smallest range; compact: slots only for cut units
   int32_t cap_seq, cap_group;   // workspace rows of a sequence's / a group's slot
   int32_t group_rows;           // workspace rows before the sequences' slots
   float scale_log2;
   int32_t* status;
   // workspace
   int32_t *cta_first, *cta_last, *cut_unit;     // [grid]
-  int64_t* part_cost;                           // [G + B] starts
-  int32_t* part_units;
-  int32_t *valid_len, *first_member, *seq_group, *seq_vt;  // [B]
-  int32_t *prefix, *group_table;                // [G]
+  int32_t* part_units;                          // [G + B] starts
+  int32_t *valid_len, *seq_group, *seq_vt;      // [B]
+  int32_t* prefix;                              // [G]
   int2* member_row;                             // [M] {first query row, tokens}
   int2* unit_info;                              // [units] {first slot row, pieces}
   RowItem* items;                               // [units + grid]
   float2* part_ml;                              // [slot rows] {max (log2), sum}
-  float* part_o;                                // [slot rows][D]
+  float4* part_o;                               // [slot rows / 32][D / 4][32]: a warp stores 32 rows' four columns at once
 };
 
 // ---------------------------------------------------------------- plan
-struct PartInfo {
-  int n_vt, k0, first, causal;  // keys k0 .. first + i (causal) or k0 .. first - 1
+// One CTA.  Everything it works on lies in shared memory, a thread a sequence or member, so that its time is that of a
+// few round trips to L2; parts of many units (long prompts, prefixes) get a warp each.
+constexpr int kPlanMost = 4096;  // sequences, members or groups of a call
+struct PlanSpace {
+  int64_t* cost;  // [G + B] starts
+  int32_t *units, *len, *first, *group, *vt, *listed, *prefix, *table;
+  __host__ __device__ static size_t bytes(int B, int G) {
+    return sizeof(int64_t) * (G + B) + sizeof(int32_t) * (G + B + 5 * static_cast<size_t>(B) + 2 * G);
+  }
+  SD_DEV PlanSpace(uint8_t* at, int B, int G) {
+    cost = reinterpret_cast<int64_t*>(at);
+    units = reinterpret_cast<int32_t*>(cost + G + B);
+    len = units + G + B;
+    first = len + B;
+    group = first + B;
+    vt = group + B;
+    listed = vt + B;
+    prefix = listed + B;
+    table = prefix + G;
+  }
 };
-SD_DEV PartInfo part_info(const RowParams& p, int part) {
+struct PartInfo {
+  int n_vt, k0, first, rows;  // tokens; keys k0 .. first + i (a sequence's token i) or k0 .. first - 1; rows of units
+  bool group;
+};
+SD_DEV PartInfo part_info(const RowParams& p, const PlanSpace& w, int part) {
   PartInfo f;
-  if (part < p.G) {
+  f.group = part < p.G;
+  if (f.group) {
     f.k0 = 0;
-    f.first = p.prefix[part];  // 0 where the group is empty or its start bad
+    f.first = w.prefix[part];  // 0 where the group is empty or its start bad
     f.n_vt = f.first > 0 ? (p.group_start[part + 1] - p.group_start[part]) * p.q_max : 0;
-    f.causal = 0;
   } else {
     const int b = part - p.G;
-    f.n_vt = p.valid_len[b];
-    f.first = f.n_vt > 0 ? p.ctx_len[b] - f.n_vt : 0;
-    const int g = f.n_vt > 0 ? p.seq_group[b] : -1;
-    f.k0 = g >= 0 ? p.prefix[g] : 0;
-    f.causal = 1;
+    f.n_vt = w.len[b];
+    f.first = w.first[b];
+    const int g = f.n_vt > 0 ? w.group[b] : -1;
+    f.k0 = g >= 0 ? w.prefix[g] : 0;
   }
+  f.rows = (f.n_vt + 2 * p.tpt - 1) / (2 * p.tpt);
   return f;
 }
-// blocks of the part's unit row r (units of one row have as many for every KV head)
+// last key + 1 and blocks of the part's unit row r (its units have as many for every KV head)
+SD_DEV int unit_end(const RowParams& p, const PartInfo& f, int r) {
+  return f.group ? f.first : f.first + min((r + 1) * 2 * p.tpt, f.n_vt);
+}
 SD_DEV int unit_blocks(const RowParams& p, const PartInfo& f, int r) {
-  const int end = f.causal ? f.first + min((r + 1) * 2 * p.tpt, f.n_vt) : f.first;
-  return (end - f.k0 + kKeyBlock - 1) / kKeyBlock;
+  return (unit_end(p, f, r) - f.k0 + kKeyBlock - 1) / kKeyBlock;
+}
+constexpr int kShortPart = 4;  // unit rows up to which a part is one thread's work
+
+struct PlanTotals {
+  int64_t total, quota;
+  // costs pass 32 bits only for prompts of millions of tokens
+  SD_DEV int cta_of(int64_t at) const {
+    return total < 0x7fffffff ? static_cast<int>(at) / static_cast<int>(quota) : static_cast<int>(at / quota);
+  }
+};
+// the items of one unit row (all KV heads), whose costs start at `start`
+SD_DEV void emit_row(const RowParams& p, const PlanTotals& q, const PartInfo& f, int part, int r, int64_t start, int ubase,
+                     RowItem it) {
+  const int nb = unit_blocks(p, f, r), cost = nb + kUnitCost, end = unit_end(p, f, r);
+  const int cap = f.group ? p.cap_group : p.cap_seq;
+  it.vt0 = r * 2 * p.tpt;
+  for (int h = 0; h < p.KV; ++h) {
+    const int u = ubase + r * p.KV + h;
+    const int64_t us = start + static_cast<int64_t>(h) * cost, ue = us + cost;
+    const int c0 = q.cta_of(us), c1 = q.cta_of(ue - 1);
+    it.head = h;
+    // pieces that hold blocks: a CTA whose range ends in the unit's own cost has none
+    const int cb = q.cta_of(us + kUnitCost);  // first CTA with a block
+    const int pieces = c1 - cb + 1;
+    const int slot0 = p.compact ? 2 * cb + 1 : u + cb;
+    const int64_t row0 = (f.group ? 0 : p.group_rows) + static_cast<int64_t>(slot0) * cap;
+    // a sequence without shared keys writes its uncut rows itself
+    const bool direct = !f.group && f.k0 == 0 && pieces == 1;
+    p.unit_info[u] = make_int2(static_cast<int>(row0), pieces);
+    if (pieces > 1) p.cut_unit[cb] = u;
+    for (int c = c0; c <= c1; ++c) {
+      const int64_t from = c * q.quota, to = from + q.quota;
+      const int a = static_cast<int>(max(from - us - kUnitCost, static_cast<int64_t>(0)));
+      const int e = static_cast<int>(min(to - us - kUnitCost, static_cast<int64_t>(nb)));
+      const int step = c - cb;
+      it.nblk = max(e - a, 0);
+      it.k0 = f.k0 + a * kKeyBlock;
+      it.k1 = min(f.k0 + e * kKeyBlock, end);
+      it.slot = direct ? -1 : static_cast<int>(row0 + static_cast<int64_t>(p.compact && step > 0 ? 2 * step - 1 : step) * cap);
+      p.items[u + c] = it;
+      const int64_t hi = min(to, q.total) - 1;
+      if (from >= us && from < ue) p.cta_first[c] = u + c;
+      if (hi >= us && hi < ue) p.cta_last[c] = u + c;
+    }
+  }
 }
 
 __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
+  extern __shared__ __align__(16) uint8_t plan_smem[];
+  const PlanSpace w(plan_smem, p.B, p.G);
+  __shared__ int64_t s_warp[2][32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nthr = blockDim.x;
   grid_dep_wait();
   grid_dep_launch();
-  __shared__ int64_t s_warp[2][32];
-  __shared__ int64_t s_run[2];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nthr = blockDim.x;
   for (int b = tid; b < p.B; b += nthr) {
-    const int n = p.q_len[b], c = p.ctx_len[b], r0 = p.q_row0[b];
+    const int n = p.q_len[b], c = p.ctx_len[b], r0 = p.q_row0[b], k0 = p.paged ? 0 : p.kv_row0[b];
     int bad = 0;
     if (n < 0 || n > p.q_max || (n > 0 && (c < n || r0 < 0 || static_cast<int64_t>(r0) + n > p.q_rows)))
       bad = SPECDEC_STATUS_BAD_LENGTH;
     else if (n > 0 && p.paged && c > static_cast<int64_t>(p.max_pages) * kPage)
       bad = SPECDEC_STATUS_PAGE_OVERFLOW;
-    else if (n > 0 && !p.paged && (p.kv_row0[b] < 0 || static_cast<int64_t>(p.kv_row0[b]) + c > p.kv_rows))
+    else if (n > 0 && !p.paged && (k0 < 0 || static_cast<int64_t>(k0) + c > p.kv_rows))
       bad = SPECDEC_STATUS_BAD_LENGTH;
     if (bad) raise_status(p.status, bad);
-    p.valid_len[b] = bad ? 0 : n;
-    if (p.G > 0) {
-      p.first_member[b] = 0x7fffffff;
-      p.seq_group[b] = -1;
-    } else {
-      p.seq_group[b] = -1;
-    }
+    const int v = bad ? 0 : n;
+    w.len[b] = v;
+    w.first[b] = v > 0 ? c - v : 0;
+    w.group[b] = -1;
+    w.listed[b] = 0x7fffffff;
+    p.valid_len[b] = v;
   }
   for (int c = tid; c < p.grid; c += nthr) {
     p.cta_first[c] = 0;
@@ -165,8 +233,8 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
       const int n = p.prefix_len[g], a = p.group_start[g], e = p.group_start[g + 1];
       bad |= a < 0 || e < a || e > p.M;
       if (n < 0) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
-      p.prefix[g] = max(n, 0);
-      p.group_table[g] = 0x7fffffff;
+      w.prefix[g] = max(n, 0);
+      w.table[g] = 0x7fffffff;
     }
     // starts that do not ascend within the member list: nobody is in a group, everything is attended to alone
     bad = __syncthreads_or(bad);
@@ -177,14 +245,14 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
       if (b < 0 || b >= p.B)
         raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
       else
-        atomicMin(&p.first_member[b], i);  // a sequence listed twice counts where it is listed first
+        atomicMin(&w.listed[b], i);  // a sequence listed twice counts where it is listed first
     }
     __syncthreads();
     for (int i = tid; i < M; i += nthr) {
       const int b = p.members[i];
       int2 mr = make_int2(0, 0);
       if (b >= 0 && b < p.B) {
-        if (p.first_member[b] != i) {
+        if (w.listed[b] != i) {
           raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
         } else {
           int lo = 0, hi = p.G;  // the last group that starts at or before i, and holds it
@@ -194,14 +262,13 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
           }
           const int gs = p.group_start[lo], ge = p.group_start[lo + 1];
           if (i >= gs && i < ge) {
-            const int n = p.valid_len[b];
-            p.seq_group[b] = lo;
-            p.seq_vt[b] = (i - gs) * p.q_max;
+            const int n = w.len[b];
+            w.group[b] = lo;
+            w.vt[b] = (i - gs) * p.q_max;
             mr = make_int2(p.q_row0[b], n);
             if (n > 0) {
-              // keys that all of the group's rows see
-              atomicMin(&p.prefix[lo], p.ctx_len[b] - n);
-              atomicMin(&p.group_table[lo], i);
+              atomicMin(&w.prefix[lo], w.first[b]);  // keys that all of the group's rows see
+              atomicMin(&w.table[lo], i);
             }
           }
         }
@@ -210,31 +277,47 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
     }
     __syncthreads();
     for (int g = tid; g < p.G; g += nthr) {
-      const int i = p.group_table[g];
-      p.prefix[g] = i == 0x7fffffff ? 0 : p.prefix[g] / kPage * kPage;  // whole pages
-      p.group_table[g] = i == 0x7fffffff ? 0 : p.members[i];
+      const int i = w.table[g];
+      const int n = i == 0x7fffffff ? 0 : w.prefix[g] / kPage * kPage;  // whole pages
+      w.prefix[g] = n;
+      w.table[g] = i == 0x7fffffff ? 0 : p.members[i];
+      p.prefix[g] = n;
     }
   }
   __syncthreads();
   // cost and unit count of every part
   const int parts = p.G + p.B;
-  for (int part = warp; part < parts; part += nthr / 32) {
-    const PartInfo f = part_info(p, part);
-    const int rows = (f.n_vt + 2 * p.tpt - 1) / (2 * p.tpt);
+  for (int part = tid; part < parts; part += nthr) {
+    const PartInfo f = part_info(p, w, part);
     int64_t sum = 0;
-    for (int r = lane; r < rows; r += 32) sum += unit_blocks(p, f, r) + kUnitCost;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-      p.part_cost[part] = sum * p.KV;
-      p.part_units[part] = rows * p.KV;
+    if (f.group)
+      sum = static_cast<int64_t>(f.rows) * (unit_blocks(p, f, 0) + kUnitCost);
+    else if (f.rows <= kShortPart)
+      for (int r = 0; r < f.rows; ++r) sum += unit_blocks(p, f, r) + kUnitCost;
+    else
+      sum = -1;
+    w.cost[part] = sum * p.KV;
+    w.units[part] = f.rows * p.KV;
+    if (!f.group) {
+      p.seq_group[part - p.G] = w.group[part - p.G];
+      p.seq_vt[part - p.G] = w.group[part - p.G] >= 0 ? w.vt[part - p.G] : 0;
     }
   }
-  if (tid == 0) s_run[0] = s_run[1] = 0;
   __syncthreads();
+  for (int part = warp; part < parts; part += nthr / 32) {
+    if (w.cost[part] >= 0) continue;
+    const PartInfo f = part_info(p, w, part);
+    int64_t sum = 0;
+    for (int r = lane; r < f.rows; r += 32) sum += unit_blocks(p, f, r) + kUnitCost;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) w.cost[part] = sum * p.KV;
+  }
+  __syncthreads();
+  int64_t run[2] = {0, 0};
   for (int base = 0; base < parts; base += nthr) {  // exclusive scans, in place
     const int i = base + tid;
-    int64_t v[2] = {i < parts ? p.part_cost[i] : 0, i < parts ? p.part_units[i] : 0}, x[2];
+    int64_t v[2] = {i < parts ? w.cost[i] : 0, i < parts ? w.units[i] : 0}, x[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       x[q] = v[q];
@@ -247,96 +330,64 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
     }
     __syncthreads();
     if (warp < 2) {
-      int64_t w = s_warp[warp][lane];
+      int64_t t = s_warp[warp][lane];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += y;
+        const int64_t y = __shfl_up_sync(0xffffffffu, t, o);
+        if (lane >= o) t += y;
       }
-      s_warp[warp][lane] = w;
+      s_warp[warp][lane] = t;
     }
     __syncthreads();
-    const int64_t run0 = s_run[0], run1 = s_run[1];
     if (i < parts) {
-      p.part_cost[i] = run0 + (warp ? s_warp[0][warp - 1] : 0) + x[0] - v[0];
-      p.part_units[i] = static_cast<int>(run1 + (warp ? s_warp[1][warp - 1] : 0) + x[1] - v[1]);
+      w.cost[i] = run[0] + (warp ? s_warp[0][warp - 1] : 0) + x[0] - v[0];
+      w.units[i] = static_cast<int>(run[1] + (warp ? s_warp[1][warp - 1] : 0) + x[1] - v[1]);
+      p.part_units[i] = w.units[i];
     }
-    __syncthreads();
-    if (tid == 0) {
-      s_run[0] += s_warp[0][31];
-      s_run[1] += s_warp[1][31];
-    }
+    run[0] += s_warp[0][31];
+    run[1] += s_warp[1][31];
     __syncthreads();
   }
-  const int64_t total = s_run[0];
-  const int64_t quota = max((total + p.grid - 1) / p.grid, static_cast<int64_t>(kMinQuota));
-  // costs pass 32 bits only for prompts of millions of tokens
-  auto cta_of = [&](int64_t at) {
-    return total < 0x7fffffff ? static_cast<int>(at) / static_cast<int>(quota) : static_cast<int>(at / quota);
-  };
-  // items
-  for (int part = warp; part < parts; part += nthr / 32) {
-    const PartInfo f = part_info(p, part);
-    const int rows = (f.n_vt + 2 * p.tpt - 1) / (2 * p.tpt);
-    int64_t start = p.part_cost[part];
-    const int ubase = p.part_units[part];
-    const bool group = part < p.G;
+  PlanTotals q;
+  q.total = run[0];
+  q.quota = max((q.total + p.grid - 1) / p.grid, static_cast<int64_t>(p.min_quota));
+  auto item_of = [&](const PartInfo& f, int part) {
+    RowItem it = {};
     const int b = part - p.G;
-    RowItem it;
-    it.src = group ? ~part : b;
+    it.src = f.group ? ~part : b;
     it.n_vt = f.n_vt;
-    it.row0 = group ? 0 : p.q_row0[b];
+    it.row0 = f.group ? 0 : p.q_row0[b];
     it.first = f.first;
-    it.kv = group ? p.group_table[part] : (p.paged ? b : p.kv_row0[b]);
-    it.member0 = group ? p.group_start[part] : 0;
-    // a sequence without shared keys writes its uncut rows itself
-    const bool alone = !group && f.k0 == 0;
-    for (int r0 = 0; r0 < rows; r0 += 32) {
+    it.kv = f.group ? w.table[part] : (p.paged ? b : p.kv_row0[b]);
+    it.member0 = f.group ? p.group_start[part] : 0;
+    return it;
+  };
+  for (int part = tid; part < parts; part += nthr) {
+    const PartInfo f = part_info(p, w, part);
+    if (f.rows == 0 || f.rows > kShortPart || f.group) continue;
+    const RowItem it = item_of(f, part);
+    int64_t start = w.cost[part];
+    for (int r = 0; r < f.rows; ++r) {
+      emit_row(p, q, f, part, r, start, w.units[part], it);
+      start += static_cast<int64_t>(unit_blocks(p, f, r) + kUnitCost) * p.KV;
+    }
+  }
+  for (int part = warp; part < parts; part += nthr / 32) {
+    const PartInfo f = part_info(p, w, part);
+    if (f.rows == 0 || (f.rows <= kShortPart && !f.group)) continue;
+    const RowItem it = item_of(f, part);
+    int64_t start = w.cost[part];
+    for (int r0 = 0; r0 < f.rows; r0 += 32) {
       const int r = r0 + lane;
-      const int nb = r < rows ? unit_blocks(p, f, r) : 0;
-      const int cost = r < rows ? nb + kUnitCost : 0;
-      int64_t x = static_cast<int64_t>(cost) * p.KV;
+      const int64_t cost = r < f.rows ? static_cast<int64_t>(unit_blocks(p, f, r) + kUnitCost) * p.KV : 0;
+      int64_t x = cost;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      const int64_t before = x - static_cast<int64_t>(cost) * p.KV;
-      const int64_t chunk = __shfl_sync(0xffffffffu, x, 31);
-      if (r < rows) {
-        it.vt0 = r * 2 * p.tpt;
-        const int end = f.causal ? f.first + min(it.vt0 + 2 * p.tpt, f.n_vt) : f.first;
-        for (int h = 0; h < p.KV; ++h) {
-          const int u = ubase + r * p.KV + h;
-          const int64_t us = start + before + static_cast<int64_t>(h) * cost, ue = us + cost;
-          const int c0 = cta_of(us), c1 = cta_of(ue - 1);
-          it.head = h;
-          // pieces that hold blocks: a CTA whose range ends in the unit's own cost has none
-          const int cb = cta_of(us + kUnitCost);  // first CTA with a block
-          const int pieces = c1 - cb + 1;
-          const int cap = group ? p.cap_group : p.cap_seq;
-          const int slot0 = p.compact ? 2 * cb + 1 : u + cb;
-          const int64_t row0 = (group ? 0 : p.group_rows) + static_cast<int64_t>(slot0) * cap;
-          const bool direct = alone && pieces == 1;
-          p.unit_info[u] = make_int2(static_cast<int>(row0), pieces);
-          if (pieces > 1) p.cut_unit[cb] = u;
-          for (int c = c0; c <= c1; ++c) {
-            const int64_t from = c * quota, to = from + quota;
-            const int a = static_cast<int>(max(from - us - kUnitCost, static_cast<int64_t>(0)));
-            const int e = static_cast<int>(min(to - us - kUnitCost, static_cast<int64_t>(nb)));
-            const int step = c - cb;
-            it.nblk = max(e - a, 0);
-            it.k0 = f.k0 + a * kKeyBlock;
-            it.k1 = min(f.k0 + e * kKeyBlock, end);
-            it.slot = direct ? -1 : static_cast<int>(row0 + static_cast<int64_t>(p.compact && step > 0 ? 2 * step - 1 : step) * cap);
-            p.items[u + c] = it;
-            const int64_t hi = min(to, total) - 1;
-            if (from >= us && from < ue) p.cta_first[c] = u + c;
-            if (hi >= us && hi < ue) p.cta_last[c] = u + c;
-          }
-        }
-      }
-      start += chunk;
+      if (r < f.rows) emit_row(p, q, f, part, r, start + x - cost, w.units[part], it);
+      start += __shfl_sync(0xffffffffu, x, 31);
     }
   }
 }
@@ -505,39 +556,50 @@ struct Poly2 {
     float tl, th, yl, yh;
     unpack2(t, tl, th);
     unpack2(y, yl, yh);
-    a = __uint_as_float((__float_as_uint(tl) << 23) + __float_as_uint(yl));
-    b = __uint_as_float((__float_as_uint(th) << 23) + __float_as_uint(yh));
+    // (one multiply-add: the compiler's shift and addition are two instructions)
+    uint32_t ra, rb;
+    asm volatile("mad.lo.u32 %0, %1, 8388608, %2;" : "=r"(ra) : "r"(__float_as_uint(tl)), "r"(__float_as_uint(yl)));
+    asm volatile("mad.lo.u32 %0, %1, 8388608, %2;" : "=r"(rb) : "r"(__float_as_uint(th)), "r"(__float_as_uint(yh)));
+    a = __uint_as_float(ra);
+    b = __uint_as_float(rb);
   }
 };
 
-// Ten pairs of scores at once, as two groups of five whose steps alternate: in a group three pairs take the
-// exponential unit (6 x 8.5 clocks a warp) and two the polynomial, whose steps lie between the others'.  Probabilities
-// as bf16 pairs in w[0 .. 9], their sums added to `sum`.
-SD_DEV void ten_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, float zn, uint64_t (&sum)[4], uint32_t* w) {
-  Poly2 p[2][2];
-  float x[2][6], y[2][6], a, b;
-#define SD_EACH(...)            \
-  _Pragma("unroll") for (int g = 0; g < 2; ++g) { \
-    [[maybe_unused]] const float* r = s + 10 * g; \
-    __VA_ARGS__                 \
-  }
-#define SD_POLY(K)                      \
-  p[g][0].step<K>(r[6], r[7], zs, zn); \
-  p[g][1].step<K>(r[8], r[9], zs, zn);
-  SD_EACH(unpack2(fma2(pack2(r[0], r[1]), sc, ng), x[g][0], x[g][1]);)
-  SD_EACH(y[g][0] = exp2_unit(x[g][0]); SD_POLY(0))
-  SD_EACH(unpack2(fma2(pack2(r[2], r[3]), sc, ng), x[g][2], x[g][3]); y[g][1] = exp2_unit(x[g][1]); SD_POLY(1))
-  SD_EACH(unpack2(fma2(pack2(r[4], r[5]), sc, ng), x[g][4], x[g][5]); y[g][2] = exp2_unit(x[g][2]); SD_POLY(2))
-  SD_EACH(y[g][3] = exp2_unit(x[g][3]); SD_POLY(3) sum[2 * g] = add2(sum[2 * g], pack2(y[g][0], y[g][1]));)
-  SD_EACH(y[g][4] = exp2_unit(x[g][4]); SD_POLY(4) w[5 * g] = round_bf16(y[g][0], y[g][1]);)
-  SD_EACH(y[g][5] = exp2_unit(x[g][5]); SD_POLY(5) sum[2 * g + 1] = add2(sum[2 * g + 1], pack2(y[g][2], y[g][3]));)
-  SD_EACH(SD_POLY(6) w[5 * g + 1] = round_bf16(y[g][2], y[g][3]);)
-  SD_EACH(p[g][0].result(a, b); sum[2 * g] = add2(sum[2 * g], pack2(a, b)); w[5 * g + 3] = round_bf16(a, b);
-          sum[2 * g + 1] = add2(sum[2 * g + 1], pack2(y[g][4], y[g][5]));
-          w[5 * g + 2] = round_bf16(y[g][4], y[g][5]);)
-  SD_EACH(p[g][1].result(a, b); sum[2 * g] = add2(sum[2 * g], pack2(a, b)); w[5 * g + 4] = round_bf16(a, b);)
-#undef SD_POLY
-#undef SD_EACH
+// Eight pairs of scores at once: six take the exponential unit (12 x 8.5 clocks a warp), two the polynomial, whose
+// steps lie between the others'.  A pair costs about 8 issue slots by the unit and 24 by the polynomial, so a quarter
+// of the pairs balances the two.  Probabilities as bf16 pairs in w[0 .. 7], their sums added to `sum`.
+SD_DEV void eight_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, float zn, uint64_t (&sum)[4], uint32_t* w) {
+  Poly2 p[2];
+  float x[12], y[12], a, b;
+#define SD_X(E) unpack2(fma2(pack2(s[2 * (E)], s[2 * (E) + 1]), sc, ng), x[2 * (E)], x[2 * (E) + 1]);
+#define SD_Y(E) y[E] = exp2_unit(x[E]);
+#define SD_P(I, K) p[I].step<K>(s[12 + 2 * (I)], s[13 + 2 * (I)], zs, zn);
+#define SD_W(E)                                              \
+  sum[(E) & 3] = add2(sum[(E) & 3], pack2(y[2 * (E)], y[2 * (E) + 1])); \
+  w[E] = round_bf16(y[2 * (E)], y[2 * (E) + 1]);
+  SD_X(0) SD_Y(0) SD_P(0, 0)
+  SD_Y(1) SD_X(1) SD_P(1, 0)
+  SD_Y(2) SD_P(0, 1) SD_X(2)
+  SD_Y(3) SD_P(1, 1) SD_P(0, 2)
+  SD_Y(4) SD_W(0) SD_P(1, 2) SD_X(3)
+  SD_Y(5) SD_P(0, 3) SD_P(1, 3)
+  SD_Y(6) SD_W(1) SD_X(4) SD_P(0, 4)
+  SD_Y(7) SD_P(1, 4) SD_X(5)
+  SD_Y(8) SD_W(2) SD_P(0, 5) SD_P(1, 5)
+  SD_Y(9) SD_W(3) SD_P(0, 6) SD_P(1, 6)
+  SD_Y(10)
+  p[0].result(a, b);
+  sum[2] = add2(sum[2], pack2(a, b));
+  w[6] = round_bf16(a, b);
+  SD_Y(11)
+  p[1].result(a, b);
+  sum[3] = add2(sum[3], pack2(a, b));
+  w[7] = round_bf16(a, b);
+  SD_W(4) SD_W(5)
+#undef SD_X
+#undef SD_Y
+#undef SD_P
+#undef SD_W
 }
 SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t ng, uint64_t& sum, uint32_t* w) {
   float a, b;
@@ -549,7 +611,7 @@ SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t ng, uint64_t& sum, ui
   *w = round_bf16(a, b);
 }
 
-// P = 2^(s scale + neg) of 64 scores as bf16 in 32 TMEM columns; returns the sum.  POLY: twelve of the 32 pairs by
+// P = 2^(s scale + neg) of 64 scores as bf16 in 32 TMEM columns; returns the sum.  POLY: eight of the 32 pairs by
 // polynomial.
 template <bool POLY>
 SD_DEV float row_probabilities(const float* s, float scale, float neg, uint32_t ta) {
@@ -559,9 +621,7 @@ SD_DEV float row_probabilities(const float* s, float scale, float neg, uint32_t 
   uint32_t w[32];
   if (POLY) {
 #pragma unroll
-    for (int e = 0; e < 3; ++e) ten_pairs(s + 20 * e, sc, ng, zs, zn, sum, w + 10 * e);
-#pragma unroll
-    for (int e = 30; e < 32; ++e) one_pair(s + 2 * e, sc, ng, sum[e & 3], w + e);
+    for (int e = 0; e < 4; ++e) eight_pairs(s + 16 * e, sc, ng, zs, zn, sum, w + 8 * e);
   } else {
 #pragma unroll
     for (int e = 0; e < 32; ++e) one_pair(s + 2 * e, sc, ng, sum[e & 3], w + e);
@@ -745,56 +805,60 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       ++on;
       umma::fence_after_sync();
       if (any_row) {
-        // Rows leave through shared memory, 64 bytes of a row at a time, so that a store covers whole sectors.
-        uint8_t* const stage = smem + Geo::STAGED + (warp - kSoftmaxWarp) * Geo::STAGE;
-        const bool direct = it.slot < 0;
-        const float inv = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-        int64_t at = -1;  // this row's first byte
-        if (limit > 0) {
-          if (direct) {
-            at = 2 * (static_cast<int64_t>(it.row0 + vt) * p.o_st +
-                      static_cast<int64_t>(it.head * p.n_rep + rep) * p.o_sh);
-          } else {
-            const int64_t r = it.slot + t * kRowTile + row;
-            p.part_ml[r] = make_float2(m * scale, l);
-            at = 4 * r * D;
+        if (it.slot >= 0) {
+          const int64_t r = it.slot + t * kRowTile + row;
+          if (limit > 0) p.part_ml[r] = make_float2(m * scale, l);
+          // (a slot has room for whole warps of the rows that there may be)
+          if (t * kRowTile + (row & ~31) < (it.src < 0 ? p.cap_group : p.cap_seq)) {
+            float4* const to = p.part_o + (r >> 5) * (8 * D) + lane;
+#pragma unroll
+            for (int c = 0; c < D; c += 64) {
+              float o[64];
+              umma::tmem_ld32(o_ta + c, o);
+              umma::tmem_ld32(o_ta + c + 32, o + 32);
+              umma::tmem_wait_ld32(o);
+              umma::tmem_wait_ld32(o + 32);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) to[(c / 4 + e) * 32] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
           }
-        }
-        uint8_t* const base = direct ? reinterpret_cast<uint8_t*>(p.out) : reinterpret_cast<uint8_t*>(p.part_o);
-        const int cols = direct ? 32 : 16;    // columns of a step
-        for (int c = 0; c < D; c += cols) {
-          uint4 x[4];
-          if (direct) {
-            float o[32];
+        } else {
+          // Rows leave through shared memory, 64 bytes of a row at a time, so that a store covers whole sectors.
+          uint8_t* const stage = smem + Geo::STAGED + (warp - kSoftmaxWarp) * Geo::STAGE;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          int64_t at = -1;  // this row's first value
+          if (limit > 0)
+            at = static_cast<int64_t>(it.row0 + vt) * p.o_st + static_cast<int64_t>(it.head * p.n_rep + rep) * p.o_sh;
+          int64_t to[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) to[g] = __shfl_sync(0xffffffffu, at, g * 8 + lane / 4);
+          uint32_t x[D / 2];
+#pragma unroll
+          for (int c = 0; c < D; c += 64) {
+            float o[64];
             umma::tmem_ld32(o_ta + c, o);
+            umma::tmem_ld32(o_ta + c + 32, o + 32);
             umma::tmem_wait_ld32(o);
+            umma::tmem_wait_ld32(o + 32);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[c / 2 + e] = pack_bf16(o[2 * e] * inv, o[2 * e + 1] * inv);
+          }
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            // 16-byte chunk e of row r lies at place e ^ (r / 2 % 4): no bank conflicts either way
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              x[e] = make_uint4(pack_bf16(o[8 * e] * inv, o[8 * e + 1] * inv), pack_bf16(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                pack_bf16(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
-                                pack_bf16(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
-          } else {
-            float o[16];
-            umma::tmem_ld16(o_ta + c, o);
-            umma::tmem_wait_ld16(o);
+              *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
+                  make_uint4(x[16 * c + 4 * e], x[16 * c + 4 * e + 1], x[16 * c + 4 * e + 2], x[16 * c + 4 * e + 3]);
+            __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              x[e] = make_uint4(__float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]), __float_as_uint(o[4 * e + 2]),
-                                __float_as_uint(o[4 * e + 3]));
+            for (int g = 0; g < 4; ++g) {
+              const int r = g * 8 + lane / 4, ch = lane & 3;
+              const uint4 y = *reinterpret_cast<const uint4*>(stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4));
+              if (to[g] >= 0) *reinterpret_cast<uint4*>(p.out + to[g] + c * 32 + ch * 8) = y;
+            }
+            __syncwarp();
           }
-          // 16-byte chunk e of row r lies at place e ^ (r / 2 % 4): no bank conflicts either way
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) = x[e];
-          __syncwarp();
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int r = g * 8 + lane / 4, ch = lane & 3;
-            const int64_t to = __shfl_sync(0xffffffffu, at, r);
-            const uint4 y = *reinterpret_cast<const uint4*>(stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4));
-            if (to >= 0) *reinterpret_cast<uint4*>(base + to + c * (direct ? 2 : 4) + ch * 16) = y;
-          }
-          __syncwarp();
         }
         umma::fence_before_sync();  // O is read: the arrival for the next item's first block lets its MMAs write it
       }
@@ -1115,33 +1179,30 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
 }
 
 // ---------------------------------------------------------------- joining partial rows
-// One warp a row: the pieces of up to two units, each a run of slots.  A piece that saw no key of the row has
-// sum 0 and maximum -inf and weighs nothing.
+// One warp two rows that lie next to each other in their slots (a lane pair reads a whole sector): the pieces of up
+// to two units, each a run of slots.  A piece that saw no key of the row has sum 0 and maximum -inf and weighs nothing.
 struct Pieces {
   int64_t row;  // workspace row of the first piece
   int n, cap;
   bool compact;
   SD_DEV int64_t at(int i) const { return row + static_cast<int64_t>(compact && i > 0 ? 2 * i - 1 : i) * cap; }
 };
+// Lane l: row l % 2 of the pair, columns 4 (l / 2) .. + 3, and 64 further.  `out` NULL: no such row.
 template <int D>
-SD_DEV void join_row(const RowParams& p, const Pieces& a, const Pieces& b, __nv_bfloat16* out, int lane) {
-  constexpr int PER = D / 32;
-  const int n = a.n + b.n;
+SD_DEV void join_pair(const RowParams& p, const Pieces& a, const Pieces& b, __nv_bfloat16* out, int lane) {
+  constexpr int PER = D / 64;
+  const int n = out ? a.n + b.n : 0, c = lane >> 1;
   auto at = [&](int i) { return i < a.n ? a.at(i) : b.at(i - a.n); };
+  const int most = max(n, __shfl_xor_sync(0xffffffffu, n, 1));
   float m = -INFINITY;
-  for (int i = lane; i < n; i += 32) {
-    const float x = p.part_ml[at(i)].x;
-    m = (x > m || x != x) ? x : m;
-  }
+  for (int i = c; i < n; i += 16) m = max_nan(m, p.part_ml[at(i)].x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float x = __shfl_xor_sync(0xffffffffu, m, o);
-    m = (x > m || x != x) ? x : m;
-  }
+  for (int o = 16; o > 1; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float mu = m == -INFINITY ? 0.f : m;
-  float acc[PER] = {}, l = 0.f;
-  for (int base = 0; base < n; base += 32) {
-    const int i = base + lane;
+  float4 acc[PER] = {};
+  float l = 0.f;
+  for (int base = 0; base < most; base += 16) {
+    const int i = base + c;
     float w = 0.f;
     int64_t r = 0;
     if (i < n) {
@@ -1150,33 +1211,32 @@ SD_DEV void join_row(const RowParams& p, const Pieces& a, const Pieces& b, __nv_
       w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : fast_exp2(ml.x - mu);
       l += w * ml.y;
     }
-    const int k = min(32, n - base);
+    const int k = min(16, most - base);
 #pragma unroll 4
     for (int e = 0; e < k; ++e) {
-      const float we = __shfl_sync(0xffffffffu, w, e);
-      const int64_t re = __shfl_sync(0xffffffffu, r, e);
+      const float we = __shfl_sync(0xffffffffu, w, 2 * e + (lane & 1));
+      const int64_t re = __shfl_sync(0xffffffffu, r, 2 * e + (lane & 1));
       if (we == 0.f) continue;
-      if (PER == 4) {
-        const float4 x = reinterpret_cast<const float4*>(p.part_o + re * D)[lane];
-        acc[0] += we * x.x;
-        acc[1] += we * x.y;
-        acc[PER > 2 ? 2 : 0] += we * x.z;
-        acc[PER > 2 ? 3 : 0] += we * x.w;
-      } else {
-        const float2 x = reinterpret_cast<const float2*>(p.part_o + re * D)[lane];
-        acc[0] += we * x.x;
-        acc[1] += we * x.y;
+      const float4* from = p.part_o + (re >> 5) * (8 * D) + (re & 31);
+#pragma unroll
+      for (int x = 0; x < PER; ++x) {
+        const float4 v = from[(c + 16 * x) * 32];
+        acc[x].x += we * v.x;
+        acc[x].y += we * v.y;
+        acc[x].z += we * v.z;
+        acc[x].w += we * v.w;
       }
     }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  for (int o = 16; o > 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (PER == 4)
-    reinterpret_cast<uint2*>(out)[lane] = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv),
-                                                     pack_bf16(acc[PER > 2 ? 2 : 0] * inv, acc[PER > 2 ? 3 : 0] * inv));
-  else
-    reinterpret_cast<uint32_t*>(out)[lane] = pack_bf16(acc[0] * inv, acc[1] * inv);
+  if (out) {
+#pragma unroll
+    for (int x = 0; x < PER; ++x)
+      reinterpret_cast<uint2*>(out)[c + 16 * x] = make_uint2(pack_bf16(acc[x].x * inv, acc[x].y * inv),
+                                                             pack_bf16(acc[x].z * inv, acc[x].w * inv));
+  }
 }
 
 // rows of the units that a CTA boundary cuts (no groups): block (c, y) takes a share of the unit that is cut in CTA c
@@ -1189,14 +1249,17 @@ __global__ void __launch_bounds__(256) join_cut_kernel(const RowParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int2 info = p.unit_info[u];
   const RowItem it = load_item(p.items + u + c);
-  for (int r = blockIdx.y * 8 + warp; r < kUnitRows; r += gridDim.y * 8) {
+  for (int r2 = (blockIdx.y * 8 + warp) * 2; r2 < kUnitRows; r2 += gridDim.y * 16) {
+    const int r = r2 + (lane & 1);
     const int t = r / kRowTile, e = r % kRowTile, tok = e / p.n_rep, vt = it.vt0 + t * p.tpt + tok;
-    if (tok >= p.tpt || vt >= it.n_vt) continue;
+    const bool in = tok < p.tpt && vt < it.n_vt;
+    if (!__any_sync(0xffffffffu, in)) continue;
     const Pieces a{info.x + r, info.y, p.cap_seq, p.compact != 0}, none{0, 0, 0, false};
-    join_row<D>(p, a, none,
-                p.out + static_cast<int64_t>(it.row0 + vt) * p.o_st +
-                    static_cast<int64_t>(it.head * p.n_rep + e - tok * p.n_rep) * p.o_sh,
-                lane);
+    join_pair<D>(p, a, none,
+                 in ? p.out + static_cast<int64_t>(it.row0 + vt) * p.o_st +
+                          static_cast<int64_t>(it.head * p.n_rep + e - tok * p.n_rep) * p.o_sh
+                    : nullptr,
+                 lane);
   }
 }
 
@@ -1205,13 +1268,13 @@ template <int D>
 __global__ void __launch_bounds__(256) join_rows_kernel(const RowParams p) {
   grid_dep_wait();
   grid_dep_launch();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, pairs = (p.n_rep + 1) / 2;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int h = static_cast<int>(w % p.H);
-  const int64_t bi = w / p.H;
-  const int i = static_cast<int>(bi % p.q_max), b = static_cast<int>(bi / p.q_max);
+  const int64_t bi = w / (p.KV * pairs);
+  const int hp = static_cast<int>(w - bi * (p.KV * pairs)), kvh = hp / pairs;
+  const int rep = (hp - kvh * pairs) * 2 + (lane & 1);
+  const int b = static_cast<int>(bi / p.q_max), i = static_cast<int>(bi - static_cast<int64_t>(b) * p.q_max);
   if (b >= p.B || i >= p.valid_len[b]) return;
-  const int kvh = h / p.n_rep, rep = h - kvh * p.n_rep;
   auto pieces = [&](int part, int vt, int cap) {
     const int2 info = p.unit_info[p.part_units[part] + vt / (2 * p.tpt) * p.KV + kvh];
     const int in = vt % (2 * p.tpt), t = in / p.tpt;
@@ -1223,8 +1286,11 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const RowParams p) {
     pre = pieces(g, p.seq_vt[b] + i, p.cap_group);
   else if (own.n == 1)
     return;  // written already
-  join_row<D>(p, pre, own,
-              p.out + static_cast<int64_t>(p.q_row0[b] + i) * p.o_st + static_cast<int64_t>(h) * p.o_sh, lane);
+  join_pair<D>(p, pre, own,
+               rep < p.n_rep ? p.out + static_cast<int64_t>(p.q_row0[b] + i) * p.o_st +
+                                   static_cast<int64_t>(kvh * p.n_rep + rep) * p.o_sh
+                             : nullptr,
+               lane);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1232,7 +1298,7 @@ struct RowShape {
   int B, H, KV, D, q_max, G, M, sms;
 };
 struct RowSpace {
-  size_t first, last, cut, cost, units, valid, member, group, vt, prefix, table, mrow, info, items, ml, o, bytes;
+  size_t first, last, cut, units, valid, group, vt, prefix, mrow, info, items, ml, o, bytes;
   int cap_seq, cap_group;
   int64_t group_rows, rows;
 };
@@ -1250,7 +1316,7 @@ static RowSpace row_space(const RowShape& s) {
   // groups' members: every group rounds its own rows up
   const int64_t group_units = s.G > 0 ? (up(static_cast<int64_t>(s.M) * s.q_max, 2 * tpt) + s.G) * s.KV : 0;
   auto cap = [&](int64_t tokens) {
-    return static_cast<int>(tokens <= tpt ? up(tokens * n_rep, 8) * 8 : kUnitRows);
+    return static_cast<int>(tokens <= tpt ? up(tokens * n_rep, 32) * 32 : kUnitRows);
   };
   w.cap_seq = cap(s.q_max);
   w.cap_group = s.G > 0 ? cap(static_cast<int64_t>(s.M) * s.q_max) : 0;
@@ -1266,14 +1332,11 @@ static RowSpace row_space(const RowShape& s) {
   w.first = take(4 * s.sms);
   w.last = take(4 * s.sms);
   w.cut = take(4 * s.sms);
-  w.cost = take(8 * (s.G + s.B + 1));
   w.units = take(4 * (s.G + s.B + 1));
   w.valid = take(4 * s.B);
-  w.member = take(4 * s.B);
   w.group = take(4 * s.B);
   w.vt = take(4 * s.B);
   w.prefix = take(4 * (s.G + 1));
-  w.table = take(4 * (s.G + 1));
   w.mrow = take(8 * (s.M + 1));
   w.info = take(8 * (seq_units + group_units));
   w.items = take(sizeof(RowItem) * (seq_units + group_units + s.sms));
@@ -1285,7 +1348,7 @@ static RowSpace row_space(const RowShape& s) {
 
 static bool row_shape_ok(const RowShape& s) {
   return s.B > 0 && s.H > 0 && s.KV > 0 && s.H % s.KV == 0 && s.H / s.KV <= kRowTile && (s.D == 64 || s.D == 128) &&
-         s.q_max > 0 && s.G >= 0 && s.M >= 0;
+         s.q_max > 0 && s.G >= 0 && s.M >= 0 && s.B <= kPlanMost && s.G <= kPlanMost && s.M <= kPlanMost;
 }
 
 static int check_shape(const RowShape& s) {
@@ -1296,7 +1359,9 @@ static int check_shape(const RowShape& s) {
   if (s.D != 64 && s.D != 128) return fail(SPECDEC_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
   if (s.q_max <= 0) return fail(SPECDEC_ERR_INVALID, "max_q_len must be positive");
   if (s.G < 0 || s.M < 0 || (s.G == 0 && s.M != 0)) return fail(SPECDEC_ERR_INVALID, "bad group or member count");
-  // item, slot and cost numbers are 32-bit
+  if (s.B > kPlanMost || s.G > kPlanMost || s.M > kPlanMost)
+    return fail(SPECDEC_ERR_UNSUPPORTED, "at most %d sequences, groups or members a call", kPlanMost);
+  // item and slot numbers are 32-bit
   const RowSpace w = row_space(s);
   if (w.rows > 0x7fffffff || static_cast<int64_t>(s.M) * s.q_max > (1 << 30) || w.bytes > (size_t(1) << 40))
     return fail(SPECDEC_ERR_UNSUPPORTED, "batch of %d sequences x %d tokens is too large for one call", s.B, s.q_max);
@@ -1329,6 +1394,7 @@ static int fill_row_params(RowParams& p, const RowShape& s, void* ws, size_t ws_
   p.M = s.M;
   p.grid = s.sms;
   p.compact = s.G == 0;
+  p.min_quota = kMinQuota;
   p.cap_seq = w.cap_seq;
   p.cap_group = w.cap_group;
   p.group_rows = static_cast<int32_t>(w.group_rows);
@@ -1336,19 +1402,16 @@ static int fill_row_params(RowParams& p, const RowShape& s, void* ws, size_t ws_
   p.cta_first = reinterpret_cast<int32_t*>(base + w.first);
   p.cta_last = reinterpret_cast<int32_t*>(base + w.last);
   p.cut_unit = reinterpret_cast<int32_t*>(base + w.cut);
-  p.part_cost = reinterpret_cast<int64_t*>(base + w.cost);
   p.part_units = reinterpret_cast<int32_t*>(base + w.units);
   p.valid_len = reinterpret_cast<int32_t*>(base + w.valid);
-  p.first_member = reinterpret_cast<int32_t*>(base + w.member);
   p.seq_group = reinterpret_cast<int32_t*>(base + w.group);
   p.seq_vt = reinterpret_cast<int32_t*>(base + w.vt);
   p.prefix = reinterpret_cast<int32_t*>(base + w.prefix);
-  p.group_table = reinterpret_cast<int32_t*>(base + w.table);
   p.member_row = reinterpret_cast<int2*>(base + w.mrow);
   p.unit_info = reinterpret_cast<int2*>(base + w.info);
   p.items = reinterpret_cast<RowItem*>(base + w.items);
   p.part_ml = reinterpret_cast<float2*>(base + w.ml);
-  p.part_o = reinterpret_cast<float*>(base + w.o);
+  p.part_o = reinterpret_cast<float4*>(base + w.o);
   return SPECDEC_OK;
 }
 
@@ -1360,14 +1423,21 @@ static int launch_row_attention(const RowParams& p, const CUtensorMap& qmap, con
   const cudaError_t e = cudaFuncSetAttribute(row_attention_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              RowGeom<D, RowRoles<SRC>::V8>::SMEM);
   if (e != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "row_attention_kernel: %s", cudaGetErrorString(e));
-  if (!reuse_plan)
-    if (int rc = launch_pdl("row_plan_kernel", row_plan_kernel, dim3(1), dim3(1024), 0, st, p)) return rc;
+  if (!reuse_plan) {
+    const size_t smem = PlanSpace::bytes(p.B, p.G);
+    if (smem > 48 * 1024) {
+      const cudaError_t pe = cudaFuncSetAttribute(row_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                  static_cast<int>(PlanSpace::bytes(kPlanMost, kPlanMost)));
+      if (pe != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "row_plan_kernel: %s", cudaGetErrorString(pe));
+    }
+    if (int rc = launch_pdl("row_plan_kernel", row_plan_kernel, dim3(1), dim3(1024), smem, st, p)) return rc;
+  }
   if (int rc = launch_pdl("row_attention_kernel", row_attention_kernel<D, SRC>, dim3(p.grid), dim3(RowRoles<SRC>::THREADS),
                           RowGeom<D, RowRoles<SRC>::V8>::SMEM, st, p, qmap, tmap, kmap, vmap))
     return rc;
   if (p.G == 0)
     return launch_pdl("join_cut_kernel", join_cut_kernel<D>, dim3(p.grid, kMergeParts), dim3(256), 0, st, p);
-  const int64_t warps = static_cast<int64_t>(p.B) * p.q_max * p.H;
+  const int64_t warps = static_cast<int64_t>(p.B) * p.q_max * p.KV * ((p.n_rep + 1) / 2);
   return launch_pdl("join_rows_kernel", join_rows_kernel<D>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256),
                     0, st, p);
 }
