@@ -29,6 +29,8 @@
 // The running maximum moves only when a row's grows by more than 2^8 (then O is rescaled in place); S_t(j) is complete
 // only after O_t(j - 1), both being issued in this order by one lane, so the rescale needs no wait of its own.
 // P is rounded to bf16 (2^-9 of each weight, independent between keys); sums, maxima and O stay fp32.
+#include <type_traits>
+
 #include "sd_common.cuh"
 #include "sd_internal.h"
 #include "umma.cuh"
@@ -54,7 +56,7 @@ template <int SRC>
 struct RowRoles {
   static constexpr bool V8 = SRC == kPagedE4M3;
   static constexpr int THREADS = 32 * (kSoftmaxWarps + 4 + (V8 ? 4 : 0));
-  static constexpr int SOFTMAX_REGS = V8 ? 184 : 208, OTHER_REGS = V8 ? 72 : 88;
+  static constexpr int SOFTMAX_REGS = V8 ? 200 : 208, OTHER_REGS = V8 ? 56 : 88;
   static_assert(32 * kSoftmaxWarps * SOFTMAX_REGS + (THREADS - 32 * kSoftmaxWarps) * OTHER_REGS <= THREADS * (V8 ? 128 : 168),
                 "register shares");
 };
@@ -450,6 +452,19 @@ SD_DEV bool row_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, got);
 }
 
+// A wait whose failure is looked at later: most of these barriers are complete when their turn comes, and a vote a wait
+// would be most of its cost.
+SD_DEV void lazy_wait(uint64_t* bar, uint32_t parity, bool& dead) {
+  if (mbar_try_sleep(bar, parity) || dead) return;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_sleep(bar, parity)) {
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      dead = true;
+      break;
+    }
+  }
+}
+
 // 3-D tiled load that stays in L2 as the hardware sees fit (K/V blocks are read again by other CTAs)
 SD_DEV void tma_tile_3d(void* dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2, uint64_t* bar) {
   asm volatile(
@@ -612,21 +627,24 @@ SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t ng, uint64_t& sum, ui
 }
 
 // P = 2^(s scale + neg) of 64 scores as bf16 in 32 TMEM columns; returns the sum.  POLY: eight of the 32 pairs by
-// polynomial.
-template <bool POLY>
-SD_DEV float row_probabilities(const float* s, float scale, float neg, uint32_t ta) {
+// polynomial.  `before_last` is called when a quarter is left.
+template <bool POLY, typename Hook>
+SD_DEV float row_probabilities(const float* s, float scale, float neg, uint32_t ta, Hook before_last) {
   const uint64_t sc = pack2(scale, scale), ng = pack2(neg, neg);
   const float zs = scale * (1.f / kPolySpan), zn = (neg - kPolyLow) * (1.f / kPolySpan);
   uint64_t sum[4] = {0, 0, 0, 0};
   uint32_t w[32];
-  if (POLY) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) eight_pairs(s + 16 * e, sc, ng, zs, zn, sum, w + 8 * e);
-  } else {
+  for (int q = 0; q < 4; ++q) {
+    if (q == 3) before_last();
+    if (POLY) {
+      eight_pairs(s + 16 * q, sc, ng, zs, zn, sum, w + 8 * q);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) one_pair(s + 2 * e, sc, ng, sum[e & 3], w + e);
+      for (int e = 0; e < 8; ++e) one_pair(s + 16 * q + 2 * e, sc, ng, sum[e & 3], w + 8 * q + e);
+    }
+    if (q == 1) umma::tmem_st16_words(ta, reinterpret_cast<const uint32_t(&)[16]>(w[0]));
   }
-  umma::tmem_st16_words(ta, reinterpret_cast<const uint32_t(&)[16]>(w[0]));
   umma::tmem_st16_words(ta + 16, reinterpret_cast<const uint32_t(&)[16]>(w[16]));
   float a, b;
   unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
@@ -701,7 +719,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     const uint32_t o_ta = umma::taddr(tmem, lanes, Geo::O_COL + t * D);
     const float scale = p.scale_log2;
     uint32_t sn = 0, pv = 0, on = 0;  // phase bits of s_full; halves handed over
-    bool ok = true;
+    bool ok = true, dead = false;
     for (int i = i0; i <= i1 && ok; ++i) {
       const RowItem it = item_at(i);
       if (it.nblk == 0) continue;
@@ -724,81 +742,99 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       const bool any_row = __any_sync(0xffffffffu, limit > 0);
       const int least = __reduce_min_sync(0xffffffffu, limit > 0 ? limit : 0x7fffffff);
       float m = -INFINITY, l = 0.f;
-      for (int k = 0; k < nh; ++k) {
-        const int h = k & 1;
-        ok = row_wait(&s_full[t][h], (sn >> h) & 1);
-        if (!ok) break;
-        sn ^= 1u << h;
+      bool usual = false;  // every row's reference is finite
+      float s[2][64];      // one half's scores are loaded while the other's are worked on
+      auto load = [&](auto half) {
+        constexpr int H = decltype(half)::value;
+        lazy_wait(&s_full[t][H], (sn >> H) & 1, dead);
+        sn ^= 1u << H;
         umma::fence_after_sync();
+        if (any_row) {
+          umma::tmem_ld32(s_ta + 64 * H, s[H]);
+          umma::tmem_ld32(s_ta + 64 * H + 32, s[H] + 32);
+        }
+      };
+      auto work = [&](auto half, int k) {
+        constexpr int H = decltype(half)::value;
+        constexpr std::integral_constant<int, 1 - H> other{};
+        const bool more = k + 1 < nh;
         if (!any_row) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[t][h]);
-          ++pv;
-          continue;
-        }
-        float s[64];
-        umma::tmem_ld32(s_ta + 64 * h, s);
-        umma::tmem_ld32(s_ta + 64 * h + 32, s + 32);
-        umma::tmem_wait_ld32(s);
-        umma::tmem_wait_ld32(s + 32);
-        const int key0 = it.k0 + k * (kKeyBlock / 2);
-        const bool masked = least < key0 + kKeyBlock / 2;
-        if (masked) {
-          const int vis = limit - key0;
+          if (more) load(other);
+        } else {
+          float(&x)[64] = s[H];
+          umma::tmem_wait_ld32(x);
+          umma::tmem_wait_ld32(x + 32);
+          const int key0 = it.k0 + k * (kKeyBlock / 2);
+          const bool masked = least < key0 + kKeyBlock / 2;
+          if (masked) {
+            const int vis = limit - key0;
 #pragma unroll
-          for (int c = 0; c < 64; ++c) s[c] = c < vis ? s[c] : -INFINITY;
-        }
-        auto row_max = [&]() {
-          float mx[4] = {s[0], s[1], s[2], s[3]};
+            for (int c = 0; c < 64; ++c) x[c] = c < vis ? x[c] : -INFINITY;
+          }
+          auto row_max = [&]() {
+            float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-          for (int c = 4; c < 60; c += 8)
+            for (int c = 4; c < 60; c += 8)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = max3_nan(mx[e], s[c + e], s[c + 4 + e]);
-          return max3_nan(max3_nan(mx[0], mx[1], s[60]), max3_nan(mx[2], mx[3], s[61]), max_nan(s[62], s[63]));
-        };
-        if (k == 0) m = row_max();
-        // infinite and NaN scores go through the exponential unit, which knows them
-        bool fast = !masked && __all_sync(0xffffffffu, fabsf(m) < INFINITY);
-        float sum;
-        for (bool again = false;; again = true) {
-          const float neg = m == -INFINITY ? 0.f : -m * scale;
-          sum = fast ? row_probabilities<true>(s, scale, neg, s_ta + 64 * h)
-                     : row_probabilities<false>(s, scale, neg, s_ta + 64 * h);
+              for (int e = 0; e < 4; ++e) mx[e] = max3_nan(mx[e], x[c + e], x[c + 4 + e]);
+            return max3_nan(max3_nan(mx[0], mx[1], x[60]), max3_nan(mx[2], mx[3], x[61]), max_nan(x[62], x[63]));
+          };
+          if (k == 0) {
+            m = row_max();
+            usual = __all_sync(0xffffffffu, fabsf(m) < INFINITY);
+          }
+          float neg = m == -INFINITY ? 0.f : -m * scale;
+          // (head_dim 128: the next half's products are not done by then, and a warp that waits here works on nothing)
+          auto next = [&]() {
+            if (D == 64 && more) load(other);
+          };
+          // infinite and NaN scores go through the exponential unit, which knows them
+          float sum = usual && !masked ? row_probabilities<true>(x, scale, neg, s_ta + 64 * H, next)
+                                       : row_probabilities<false>(x, scale, neg, s_ta + 64 * H, next);
           // Past the reference by more than 2^60 (or no reference yet, every key so far being masked): the
           // reference becomes this half block's maximum, O and l are rescaled and it is done again, once.  A NaN
           // stays one; a row without a key so far has none to refer to.
           const bool move = (!(sum < kGrow) || (m == -INFINITY && sum > 0.f)) && m == m && m < INFINITY;
-          if (again || !__any_sync(0xffffffffu, move)) break;
-          if (k > 0) {  // the MMAs over the half before this add to O
-            ok = row_wait(&pv_done[t], (pv - 1) & 1);
-            if (!ok) break;
-            umma::fence_after_sync();
-          }
-          const float bm = row_max();
-          const float alpha = move ? fast_exp2(((m == -INFINITY ? bm : m) - bm) * scale) : 1.f;
-          if (move) m = bm;
-          l *= alpha;
-          if (k > 0) {
+          if (__any_sync(0xffffffffu, move)) {
+            const float bm = row_max();
+            const float alpha = move ? fast_exp2(((m == -INFINITY ? bm : m) - bm) * scale) : 1.f;
+            if (move) m = bm;
+            l *= alpha;
+            if (k > 0) {
+              lazy_wait(&pv_done[t], (pv - 1) & 1, dead);  // the MMAs over the half before this add to O
+              umma::fence_after_sync();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              float o[16];
-              umma::tmem_ld16(o_ta + c, o);
-              umma::tmem_wait_ld16(o);
+              for (int c = 0; c < D; c += 16) {
+                float o[16];
+                umma::tmem_ld16(o_ta + c, o);
+                umma::tmem_wait_ld16(o);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] *= alpha;
-              umma::tmem_st16(o_ta + c, o);
+                for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                umma::tmem_st16(o_ta + c, o);
+              }
             }
+            neg = m == -INFINITY ? 0.f : -m * scale;
+            sum = row_probabilities<false>(x, scale, neg, s_ta + 64 * H, []() {});
+            usual = __all_sync(0xffffffffu, fabsf(m) < INFINITY);
           }
-          fast = false;
+          l += sum;
+          umma::tmem_wait_st();
         }
-        if (!ok) break;
-        l += sum;
         ++pv;
-        umma::tmem_wait_st();
         umma::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t][h]);
+        if (lane == 0) mbar_arrive(&p_full[t][H]);
+        if (D != 64 && any_row && more) load(other);
+      };
+      constexpr std::integral_constant<int, 0> even{};
+      constexpr std::integral_constant<int, 1> odd{};
+      load(even);
+      for (int k = 0; k < nh; k += 2) {
+        work(even, k);
+        if (k + 1 < nh) work(odd, k + 1);
+        if (__any_sync(0xffffffffu, dead)) break;
       }
+      ok = !__any_sync(0xffffffffu, dead);
       if (!ok) break;
       ok = row_wait(&o_full[t], on & 1);
       if (!ok) break;
@@ -811,15 +847,13 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           // (a slot has room for whole warps of the rows that there may be)
           if (t * kRowTile + (row & ~31) < (it.src < 0 ? p.cap_group : p.cap_seq)) {
             float4* const to = p.part_o + (r >> 5) * (8 * D) + lane;
-#pragma unroll
-            for (int c = 0; c < D; c += 64) {
-              float o[64];
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
               umma::tmem_ld32(o_ta + c, o);
-              umma::tmem_ld32(o_ta + c + 32, o + 32);
               umma::tmem_wait_ld32(o);
-              umma::tmem_wait_ld32(o + 32);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) to[(c / 4 + e) * 32] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              for (int e = 0; e < 8; ++e) to[(c / 4 + e) * 32] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
           }
         } else {
@@ -832,24 +866,20 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           int64_t to[4];
 #pragma unroll
           for (int g = 0; g < 4; ++g) to[g] = __shfl_sync(0xffffffffu, at, g * 8 + lane / 4);
-          uint32_t x[D / 2];
-#pragma unroll
-          for (int c = 0; c < D; c += 64) {
-            float o[64];
-            umma::tmem_ld32(o_ta + c, o);
-            umma::tmem_ld32(o_ta + c + 32, o + 32);
-            umma::tmem_wait_ld32(o);
-            umma::tmem_wait_ld32(o + 32);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[c / 2 + e] = pack_bf16(o[2 * e] * inv, o[2 * e + 1] * inv);
-          }
+          float o[2][32];
+          umma::tmem_ld32(o_ta, o[0]);
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
+            umma::tmem_wait_ld32(o[c & 1]);
+            if (c + 1 < D / 32) umma::tmem_ld32(o_ta + 32 * (c + 1), o[(c + 1) & 1]);
+            const float* v = o[c & 1];
             // 16-byte chunk e of row r lies at place e ^ (r / 2 % 4): no bank conflicts either way
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
-                  make_uint4(x[16 * c + 4 * e], x[16 * c + 4 * e + 1], x[16 * c + 4 * e + 2], x[16 * c + 4 * e + 3]);
+                  make_uint4(pack_bf16(v[8 * e] * inv, v[8 * e + 1] * inv), pack_bf16(v[8 * e + 2] * inv, v[8 * e + 3] * inv),
+                             pack_bf16(v[8 * e + 4] * inv, v[8 * e + 5] * inv),
+                             pack_bf16(v[8 * e + 6] * inv, v[8 * e + 7] * inv));
             __syncwarp();
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
