@@ -44,7 +44,7 @@ constexpr int kUnitCost = 2;       // what a unit costs beside its blocks (query
 constexpr int kMinQuota = 4;       // smallest range of a CTA, in blocks
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
 constexpr float kGrow = 1.152921504606846976e18f;  // 2^60: a block's sum past it moves the row's reference
-constexpr int kItemsKept = 32;     // items of a CTA that it keeps in shared memory
+constexpr int kItemsKept = 24;     // items of a CTA that it keeps in shared memory
 constexpr float kExpC0 = 0.999924541f, kExpC1 = 0.693136752f, kExpC2 = 0.242639482f, kExpC3 = 0.0558382832f;
 
 enum RowSource { kPacked = 0, kPaged = 1, kPagedE4M3 = 2 };
@@ -87,6 +87,7 @@ struct RowParams {
   int64_t q_rows, kv_rows;
   int32_t B, H, KV, n_rep, tpt, q_max, G, M;
   int32_t num_pages, max_pages, paged;
+  int32_t plan;                 // 1: work the plan out, 0: it is in the workspace
   int32_t grid, min_quota, compact;  // CTAs of the plan, its smallest range; compact: slots only for cut units
   int32_t cap_seq, cap_group;   // workspace rows of a sequence's / a group's slot
   int32_t group_rows;           // workspace rows before the sequences' slots
@@ -105,13 +106,15 @@ struct RowParams {
 };
 
 // ---------------------------------------------------------------- plan
-// One CTA.  Everything it works on lies in shared memory, a thread a sequence or member, so that its time is that of a
-// few round trips to L2; parts of many units (long prompts, prefixes) get a warp each.
-constexpr int kPlanMost = 4096;  // sequences, members or groups of a call
+// Every CTA of the attention kernel works the plan out for itself before it starts, in the shared memory that its
+// blocks will take, and writes down its own items (the workspace then serves the next layers, and the join): a few
+// round trips to L2, where a kernel of its own before this one took 5 to 10 us.  A thread a sequence or member; parts
+// of many units (long prompts, prefixes) a warp each.
+constexpr int kPlanMost = 2048;  // sequences, members or groups of a call
 struct PlanSpace {
   int64_t* cost;  // [G + B] starts
   int32_t *units, *len, *first, *group, *vt, *listed, *prefix, *table;
-  __host__ __device__ static size_t bytes(int B, int G) {
+  __host__ __device__ static constexpr size_t bytes(int B, int G) {
     return sizeof(int64_t) * (G + B) + sizeof(int32_t) * (G + B + 5 * static_cast<size_t>(B) + 2 * G);
   }
   SD_DEV PlanSpace(uint8_t* at, int B, int G) {
@@ -163,50 +166,50 @@ struct PlanTotals {
     return total < 0x7fffffff ? static_cast<int>(at) / static_cast<int>(quota) : static_cast<int>(at / quota);
   }
 };
-// the items of one unit row (all KV heads), whose costs start at `start`
+// this CTA's items of one unit row (all KV heads), whose costs start at `start`; first and last are their numbers
 SD_DEV void emit_row(const RowParams& p, const PlanTotals& q, const PartInfo& f, int part, int r, int64_t start, int ubase,
-                     RowItem it) {
-  const int nb = unit_blocks(p, f, r), cost = nb + kUnitCost, end = unit_end(p, f, r);
+                     RowItem it, int* first, int* last) {
+  const int nb = unit_blocks(p, f, r), cost = nb + kUnitCost, end = unit_end(p, f, r), c = blockIdx.x;
+  const int64_t from = c * q.quota, to = min(from + q.quota, q.total);
+  if (start >= to || start + static_cast<int64_t>(cost) * p.KV <= from) return;
   const int cap = f.group ? p.cap_group : p.cap_seq;
   it.vt0 = r * 2 * p.tpt;
   for (int h = 0; h < p.KV; ++h) {
     const int u = ubase + r * p.KV + h;
     const int64_t us = start + static_cast<int64_t>(h) * cost, ue = us + cost;
-    const int c0 = q.cta_of(us), c1 = q.cta_of(ue - 1);
+    if (us >= to || ue <= from) continue;
     it.head = h;
     // pieces that hold blocks: a CTA whose range ends in the unit's own cost has none
     const int cb = q.cta_of(us + kUnitCost);  // first CTA with a block
-    const int pieces = c1 - cb + 1;
+    const int pieces = q.cta_of(ue - 1) - cb + 1;
     const int slot0 = p.compact ? 2 * cb + 1 : u + cb;
     const int64_t row0 = (f.group ? 0 : p.group_rows) + static_cast<int64_t>(slot0) * cap;
     // a sequence without shared keys writes its uncut rows itself
     const bool direct = !f.group && f.k0 == 0 && pieces == 1;
-    p.unit_info[u] = make_int2(static_cast<int>(row0), pieces);
-    if (pieces > 1) p.cut_unit[cb] = u;
-    for (int c = c0; c <= c1; ++c) {
-      const int64_t from = c * q.quota, to = from + q.quota;
-      const int a = static_cast<int>(max(from - us - kUnitCost, static_cast<int64_t>(0)));
-      const int e = static_cast<int>(min(to - us - kUnitCost, static_cast<int64_t>(nb)));
-      const int step = c - cb;
-      it.nblk = max(e - a, 0);
-      it.k0 = f.k0 + a * kKeyBlock;
-      it.k1 = min(f.k0 + e * kKeyBlock, end);
-      it.slot = direct ? -1 : static_cast<int>(row0 + static_cast<int64_t>(p.compact && step > 0 ? 2 * step - 1 : step) * cap);
-      p.items[u + c] = it;
-      const int64_t hi = min(to, q.total) - 1;
-      if (from >= us && from < ue) p.cta_first[c] = u + c;
-      if (hi >= us && hi < ue) p.cta_last[c] = u + c;
+    if (c == cb) {
+      p.unit_info[u] = make_int2(static_cast<int>(row0), pieces);
+      if (pieces > 1) p.cut_unit[cb] = u;
     }
+    const int a = static_cast<int>(max(from - us - kUnitCost, static_cast<int64_t>(0)));
+    const int e = static_cast<int>(min(to - us - kUnitCost, static_cast<int64_t>(nb)));
+    const int step = c - cb;
+    it.nblk = max(e - a, 0);
+    it.k0 = f.k0 + a * kKeyBlock;
+    it.k1 = min(f.k0 + e * kKeyBlock, end);
+    it.slot = direct ? -1 : static_cast<int>(row0 + static_cast<int64_t>(p.compact && step > 0 ? 2 * step - 1 : step) * cap);
+    p.items[u + c] = it;
+    if (from >= us) *first = u + c;
+    if (to <= ue) *last = u + c;
   }
 }
 
-__global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
-  extern __shared__ __align__(16) uint8_t plan_smem[];
-  const PlanSpace w(plan_smem, p.B, p.G);
-  __shared__ int64_t s_warp[2][32];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nthr = blockDim.x;
-  grid_dep_wait();
-  grid_dep_launch();
+// All threads of the CTA; `at`: PlanSpace::bytes() of shared memory.  Returns the numbers of this CTA's first and last
+// item in range[0 .. 1] (shared), after a barrier.  What the calls after this one read is written by CTA 0.
+SD_DEV void make_plan(const RowParams& p, uint8_t* at, int64_t (*s_warp)[32], int* range) {
+  const PlanSpace w(at, p.B, p.G);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nthr = blockDim.x, warps = nthr / 32;
+  const bool writes = blockIdx.x == 0;
+  if (tid < 2) range[tid] = -tid;  // 0, -1: no items
   for (int b = tid; b < p.B; b += nthr) {
     const int n = p.q_len[b], c = p.ctx_len[b], r0 = p.q_row0[b], k0 = p.paged ? 0 : p.kv_row0[b];
     int bad = 0;
@@ -216,47 +219,41 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
       bad = SPECDEC_STATUS_PAGE_OVERFLOW;
     else if (n > 0 && !p.paged && (k0 < 0 || static_cast<int64_t>(k0) + c > p.kv_rows))
       bad = SPECDEC_STATUS_BAD_LENGTH;
-    if (bad) raise_status(p.status, bad);
+    if (bad && writes) raise_status(p.status, bad);
     const int v = bad ? 0 : n;
     w.len[b] = v;
     w.first[b] = v > 0 ? c - v : 0;
     w.group[b] = -1;
     w.listed[b] = 0x7fffffff;
-    p.valid_len[b] = v;
+    if (writes) p.valid_len[b] = v;
   }
-  for (int c = tid; c < p.grid; c += nthr) {
-    p.cta_first[c] = 0;
-    p.cta_last[c] = -1;
-    p.cut_unit[c] = -1;
-  }
+  if (tid == 0) p.cut_unit[blockIdx.x] = -1;
   if (p.G > 0) {
     int bad = 0;
     for (int g = tid; g < p.G; g += nthr) {
       const int n = p.prefix_len[g], a = p.group_start[g], e = p.group_start[g + 1];
       bad |= a < 0 || e < a || e > p.M;
-      if (n < 0) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
+      if (n < 0 && writes) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
       w.prefix[g] = max(n, 0);
       w.table[g] = 0x7fffffff;
     }
     // starts that do not ascend within the member list: nobody is in a group, everything is attended to alone
     bad = __syncthreads_or(bad);
-    if (bad && tid == 0) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
+    if (bad && tid == 0 && writes) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
     const int M = bad ? 0 : p.M;
     for (int i = tid; i < M; i += nthr) {
       const int b = p.members[i];
-      if (b < 0 || b >= p.B)
-        raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
-      else
+      if (b >= 0 && b < p.B)
         atomicMin(&w.listed[b], i);  // a sequence listed twice counts where it is listed first
     }
     __syncthreads();
     for (int i = tid; i < M; i += nthr) {
       const int b = p.members[i];
       int2 mr = make_int2(0, 0);
-      if (b >= 0 && b < p.B) {
-        if (w.listed[b] != i) {
-          raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
-        } else {
+      if (b < 0 || b >= p.B || w.listed[b] != i) {
+        if (writes) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
+      } else {
+        {
           int lo = 0, hi = p.G;  // the last group that starts at or before i, and holds it
           while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
@@ -275,7 +272,7 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
           }
         }
       }
-      p.member_row[i] = mr;
+      if (writes) p.member_row[i] = mr;
     }
     __syncthreads();
     for (int g = tid; g < p.G; g += nthr) {
@@ -283,7 +280,7 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
       const int n = i == 0x7fffffff ? 0 : w.prefix[g] / kPage * kPage;  // whole pages
       w.prefix[g] = n;
       w.table[g] = i == 0x7fffffff ? 0 : p.members[i];
-      p.prefix[g] = n;
+      if (writes) p.prefix[g] = n;
     }
   }
   __syncthreads();
@@ -300,13 +297,13 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
       sum = -1;
     w.cost[part] = sum * p.KV;
     w.units[part] = f.rows * p.KV;
-    if (!f.group) {
+    if (!f.group && writes) {
       p.seq_group[part - p.G] = w.group[part - p.G];
       p.seq_vt[part - p.G] = w.group[part - p.G] >= 0 ? w.vt[part - p.G] : 0;
     }
   }
   __syncthreads();
-  for (int part = warp; part < parts; part += nthr / 32) {
+  for (int part = warp; part < parts; part += warps) {
     if (w.cost[part] >= 0) continue;
     const PartInfo f = part_info(p, w, part);
     int64_t sum = 0;
@@ -332,7 +329,7 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
     }
     __syncthreads();
     if (warp < 2) {
-      int64_t t = s_warp[warp][lane];
+      int64_t t = lane < warps ? s_warp[warp][lane] : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t y = __shfl_up_sync(0xffffffffu, t, o);
@@ -344,7 +341,7 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
     if (i < parts) {
       w.cost[i] = run[0] + (warp ? s_warp[0][warp - 1] : 0) + x[0] - v[0];
       w.units[i] = static_cast<int>(run[1] + (warp ? s_warp[1][warp - 1] : 0) + x[1] - v[1]);
-      p.part_units[i] = w.units[i];
+      if (writes) p.part_units[i] = w.units[i];
     }
     run[0] += s_warp[0][31];
     run[1] += s_warp[1][31];
@@ -353,6 +350,7 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
   PlanTotals q;
   q.total = run[0];
   q.quota = max((q.total + p.grid - 1) / p.grid, static_cast<int64_t>(p.min_quota));
+  const int64_t from = blockIdx.x * q.quota, to = min(from + q.quota, q.total);
   auto item_of = [&](const PartInfo& f, int part) {
     RowItem it = {};
     const int b = part - p.G;
@@ -367,18 +365,20 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
   for (int part = tid; part < parts; part += nthr) {
     const PartInfo f = part_info(p, w, part);
     if (f.rows == 0 || f.rows > kShortPart || f.group) continue;
-    const RowItem it = item_of(f, part);
     int64_t start = w.cost[part];
+    if (start >= to || (part + 1 < parts ? w.cost[part + 1] : q.total) <= from) continue;
+    const RowItem it = item_of(f, part);
     for (int r = 0; r < f.rows; ++r) {
-      emit_row(p, q, f, part, r, start, w.units[part], it);
+      emit_row(p, q, f, part, r, start, w.units[part], it, &range[0], &range[1]);
       start += static_cast<int64_t>(unit_blocks(p, f, r) + kUnitCost) * p.KV;
     }
   }
-  for (int part = warp; part < parts; part += nthr / 32) {
+  for (int part = warp; part < parts; part += warps) {
     const PartInfo f = part_info(p, w, part);
     if (f.rows == 0 || (f.rows <= kShortPart && !f.group)) continue;
-    const RowItem it = item_of(f, part);
     int64_t start = w.cost[part];
+    if (start >= to || (part + 1 < parts ? w.cost[part + 1] : q.total) <= from) continue;
+    const RowItem it = item_of(f, part);
     for (int r0 = 0; r0 < f.rows; r0 += 32) {
       const int r = r0 + lane;
       const int64_t cost = r < f.rows ? static_cast<int64_t>(unit_blocks(p, f, r) + kUnitCost) * p.KV : 0;
@@ -388,9 +388,14 @@ __global__ void __launch_bounds__(1024) row_plan_kernel(const RowParams p) {
         const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      if (r < f.rows) emit_row(p, q, f, part, r, start + x - cost, w.units[part], it);
+      if (r < f.rows) emit_row(p, q, f, part, r, start + x - cost, w.units[part], it, &range[0], &range[1]);
       start += __shfl_sync(0xffffffffu, x, 31);
     }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    p.cta_first[blockIdx.x] = range[0];
+    p.cta_last[blockIdx.x] = range[1];
   }
 }
 
@@ -409,6 +414,7 @@ struct RowGeom {
   static constexpr int STAGE = 2048;
   static constexpr int SMEM = STAGED + kSoftmaxWarps * STAGE + 1024;
   static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
+  static_assert(PlanSpace::bytes(kPlanMost, kPlanMost) <= SMEM - 1024, "a plan fits");
   static_assert(SMEM <= 227 * 1024 - 2048, "shared memory budget, 2 KB of static variables aside");
 };
 
@@ -663,6 +669,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   __shared__ uint64_t full[NS], empty[NS], raw_full, raw_empty;
   __shared__ uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], pv_done[2], o_full[2], c_req, v_clean, fin[2];
   __shared__ RowItem s_items[kItemsKept];  // the CTA's first items
+  __shared__ int64_t s_plan[2][32];
+  __shared__ int s_range[2];
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -700,7 +708,17 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   }
   grid_dep_wait();
   grid_dep_launch();
-  const int i0 = p.cta_first[blockIdx.x], i1 = p.cta_last[blockIdx.x];
+  if (p.plan) {
+    __syncthreads();
+    make_plan(p, smem, s_plan, s_range);
+  } else if (tid == 0) {
+    s_range[0] = p.cta_first[blockIdx.x];
+    s_range[1] = p.cta_last[blockIdx.x];
+  }
+  // (the plan's generic writes are over before the copies into the same memory begin)
+  fence_proxy_async();
+  __syncthreads();
+  const int i0 = s_range[0], i1 = s_range[1];
   for (int e = tid; e < 3 * min(i1 - i0 + 1, kItemsKept); e += blockDim.x)
     reinterpret_cast<int4*>(s_items)[e] = reinterpret_cast<const int4*>(p.items + i0)[e];
   umma::fence_before_sync();
@@ -1446,22 +1464,14 @@ static int fill_row_params(RowParams& p, const RowShape& s, void* ws, size_t ws_
 }
 
 template <int D, int SRC>
-static int launch_row_attention(const RowParams& p, const CUtensorMap& qmap, const CUtensorMap& tmap, const CUtensorMap& kmap,
+static int launch_row_attention(RowParams& p, const CUtensorMap& qmap, const CUtensorMap& tmap, const CUtensorMap& kmap,
                                 const CUtensorMap& vmap,
                                 bool reuse_plan, cudaStream_t st) {
+  p.plan = reuse_plan ? 0 : 1;
   // the attribute belongs to the function on each device; setting it again is cheap and needs no state of its own
   const cudaError_t e = cudaFuncSetAttribute(row_attention_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              RowGeom<D, RowRoles<SRC>::V8>::SMEM);
   if (e != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "row_attention_kernel: %s", cudaGetErrorString(e));
-  if (!reuse_plan) {
-    const size_t smem = PlanSpace::bytes(p.B, p.G);
-    if (smem > 48 * 1024) {
-      const cudaError_t pe = cudaFuncSetAttribute(row_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                  static_cast<int>(PlanSpace::bytes(kPlanMost, kPlanMost)));
-      if (pe != cudaSuccess) return fail(SPECDEC_ERR_CUDA, "row_plan_kernel: %s", cudaGetErrorString(pe));
-    }
-    if (int rc = launch_pdl("row_plan_kernel", row_plan_kernel, dim3(1), dim3(1024), smem, st, p)) return rc;
-  }
   if (int rc = launch_pdl("row_attention_kernel", row_attention_kernel<D, SRC>, dim3(p.grid), dim3(RowRoles<SRC>::THREADS),
                           RowGeom<D, RowRoles<SRC>::V8>::SMEM, st, p, qmap, tmap, kmap, vmap))
     return rc;
