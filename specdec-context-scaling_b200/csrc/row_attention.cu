@@ -56,7 +56,7 @@ template <int SRC>
 struct RowRoles {
   static constexpr bool V8 = SRC == kPagedE4M3;
   static constexpr int THREADS = 32 * (kSoftmaxWarps + 4 + (V8 ? 4 : 0));
-  static constexpr int SOFTMAX_REGS = V8 ? 200 : 208, OTHER_REGS = V8 ? 56 : 88;
+  static constexpr int SOFTMAX_REGS = V8 ? 176 : 208, OTHER_REGS = V8 ? 80 : 88;
   static_assert(32 * kSoftmaxWarps * SOFTMAX_REGS + (THREADS - 32 * kSoftmaxWarps) * OTHER_REGS <= THREADS * (V8 ? 128 : 168),
                 "register shares");
 };
@@ -69,8 +69,8 @@ struct alignas(16) RowItem {
   int32_t k0, k1;  // keys of this item
   int32_t slot;    // first workspace row of the partial, or -1: the output itself
   int32_t nblk;    // blocks (0: nothing to do)
-  int32_t row0;    // sequence: first query row
-  int32_t first;   // sequence: keys before its first new token; group: the prefix
+  int32_t row0;    // query row of token 0 (group: -1 where its members' rows do not follow one another)
+  int32_t first;   // sequence: keys before its first new token; group: not 0 if every member has q_max tokens
   int32_t kv;      // packed: first key row; paged: sequence whose page table is read
   int32_t member0; // group: first member
 };
@@ -107,30 +107,31 @@ struct RowParams {
 
 // ---------------------------------------------------------------- plan
 // Every CTA of the attention kernel works the plan out for itself before it starts, in the shared memory that its
-// blocks will take, and writes down its own items (the workspace then serves the next layers, and the join): a few
-// round trips to L2, where a kernel of its own before this one took 5 to 10 us.  A thread a sequence or member; parts
-// of many units (long prompts, prefixes) a warp each.
+// blocks will take, and keeps its own items (they are written down, too: the workspace then serves the next layers,
+// and the join).  That is a round trip to L2, some barriers and two scans; a kernel of its own before this one took 5 to
+// 10 us.  A thread a sequence, member or unit row.
 constexpr int kPlanMost = 2048;  // sequences, members or groups of a call
 struct PlanSpace {
-  int64_t* cost;  // [G + B] starts
-  int32_t *units, *len, *first, *group, *vt, *listed, *prefix, *table;
+  int32_t *rows, *len, *first, *group, *vt, *listed, *prefix, *table, *flags;
   __host__ __device__ static constexpr size_t bytes(int B, int G) {
-    return sizeof(int64_t) * (G + B) + sizeof(int32_t) * (G + B + 5 * static_cast<size_t>(B) + 2 * G);
+    return sizeof(int32_t) * (static_cast<size_t>(G) + B + 1 + 5 * static_cast<size_t>(B) + 3 * static_cast<size_t>(G));
   }
   SD_DEV PlanSpace(uint8_t* at, int B, int G) {
-    cost = reinterpret_cast<int64_t*>(at);
-    units = reinterpret_cast<int32_t*>(cost + G + B);
-    len = units + G + B;
-    first = len + B;
+    rows = reinterpret_cast<int32_t*>(at);  // [G + B + 1] first unit row of a part
+    len = rows + G + B + 1;                 // [B] valid new tokens
+    first = len + B;                        // keys before them
     group = first + B;
-    vt = group + B;
-    listed = vt + B;
-    prefix = listed + B;
-    table = prefix + G;
+    vt = group + B;                         // first token in its group's part
+    listed = vt + B;                        // where a sequence is listed first
+    prefix = listed + B;                    // [G]
+    table = prefix + G;                     // first member with rows
+    flags = table + G;                      // kGroupRows, kGroupFull
   }
 };
+constexpr int kGroupRows = 1;  // the members' rows follow one another: token vt is row (first member's row) + vt
+constexpr int kGroupFull = 2;  // and every token is one: no member has fewer than q_max
 struct PartInfo {
-  int n_vt, k0, first, rows;  // tokens; keys k0 .. first + i (a sequence's token i) or k0 .. first - 1; rows of units
+  int n_vt, k0, first;  // tokens; keys k0 .. first + i (a sequence's token i) or k0 .. first - 1
   bool group;
 };
 SD_DEV PartInfo part_info(const RowParams& p, const PlanSpace& w, int part) {
@@ -147,69 +148,54 @@ SD_DEV PartInfo part_info(const RowParams& p, const PlanSpace& w, int part) {
     const int g = f.n_vt > 0 ? w.group[b] : -1;
     f.k0 = g >= 0 ? w.prefix[g] : 0;
   }
-  f.rows = (f.n_vt + 2 * p.tpt - 1) / (2 * p.tpt);
   return f;
 }
-// last key + 1 and blocks of the part's unit row r (its units have as many for every KV head)
+// last key + 1 of the part's unit row r (all KV heads alike)
 SD_DEV int unit_end(const RowParams& p, const PartInfo& f, int r) {
   return f.group ? f.first : f.first + min((r + 1) * 2 * p.tpt, f.n_vt);
 }
 SD_DEV int unit_blocks(const RowParams& p, const PartInfo& f, int r) {
   return (unit_end(p, f, r) - f.k0 + kKeyBlock - 1) / kKeyBlock;
 }
-constexpr int kShortPart = 4;  // unit rows up to which a part is one thread's work
-
-struct PlanTotals {
-  int64_t total, quota;
-  // costs pass 32 bits only for prompts of millions of tokens
-  SD_DEV int cta_of(int64_t at) const {
-    return total < 0x7fffffff ? static_cast<int>(at) / static_cast<int>(quota) : static_cast<int>(at / quota);
+// Sum of v over the threads before this one, and over all.  `tot`: two sets of [32], used in turn.
+SD_DEV int64_t plan_scan(int64_t v, int64_t& all, int64_t (*tot)[32], int& turn) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
-};
-// this CTA's items of one unit row (all KV heads), whose costs start at `start`; first and last are their numbers
-SD_DEV void emit_row(const RowParams& p, const PlanTotals& q, const PartInfo& f, int part, int r, int64_t start, int ubase,
-                     RowItem it, int* first, int* last) {
-  const int nb = unit_blocks(p, f, r), cost = nb + kUnitCost, end = unit_end(p, f, r), c = blockIdx.x;
-  const int64_t from = c * q.quota, to = min(from + q.quota, q.total);
-  if (start >= to || start + static_cast<int64_t>(cost) * p.KV <= from) return;
-  const int cap = f.group ? p.cap_group : p.cap_seq;
-  it.vt0 = r * 2 * p.tpt;
-  for (int h = 0; h < p.KV; ++h) {
-    const int u = ubase + r * p.KV + h;
-    const int64_t us = start + static_cast<int64_t>(h) * cost, ue = us + cost;
-    if (us >= to || ue <= from) continue;
-    it.head = h;
-    // pieces that hold blocks: a CTA whose range ends in the unit's own cost has none
-    const int cb = q.cta_of(us + kUnitCost);  // first CTA with a block
-    const int pieces = q.cta_of(ue - 1) - cb + 1;
-    const int slot0 = p.compact ? 2 * cb + 1 : u + cb;
-    const int64_t row0 = (f.group ? 0 : p.group_rows) + static_cast<int64_t>(slot0) * cap;
-    // a sequence without shared keys writes its uncut rows itself
-    const bool direct = !f.group && f.k0 == 0 && pieces == 1;
-    if (c == cb) {
-      p.unit_info[u] = make_int2(static_cast<int>(row0), pieces);
-      if (pieces > 1) p.cut_unit[cb] = u;
-    }
-    const int a = static_cast<int>(max(from - us - kUnitCost, static_cast<int64_t>(0)));
-    const int e = static_cast<int>(min(to - us - kUnitCost, static_cast<int64_t>(nb)));
-    const int step = c - cb;
-    it.nblk = max(e - a, 0);
-    it.k0 = f.k0 + a * kKeyBlock;
-    it.k1 = min(f.k0 + e * kKeyBlock, end);
-    it.slot = direct ? -1 : static_cast<int>(row0 + static_cast<int64_t>(p.compact && step > 0 ? 2 * step - 1 : step) * cap);
-    p.items[u + c] = it;
-    if (from >= us) *first = u + c;
-    if (to <= ue) *last = u + c;
+  if (lane == 31) tot[turn][warp] = x;
+  __syncthreads();
+  int64_t before = 0;
+  all = 0;
+  for (int i = 0; i < warps; ++i) {
+    const int64_t t = tot[turn][i];
+    if (i < warp) before += t;
+    all += t;
   }
+  turn ^= 1;
+  return before + x - v;
 }
 
-// All threads of the CTA; `at`: PlanSpace::bytes() of shared memory.  Returns the numbers of this CTA's first and last
-// item in range[0 .. 1] (shared), after a barrier.  What the calls after this one read is written by CTA 0.
-SD_DEV void make_plan(const RowParams& p, uint8_t* at, int64_t (*s_warp)[32], int* range) {
+// All threads of the CTA; `at`: PlanSpace::bytes() of shared memory.  range[0 .. 1] (shared): numbers of this CTA's first
+// and last item; kept[i % kItemsKept] holds them where that is all of them (returns whether).
+SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* range, RowItem* kept) {
   const PlanSpace w(at, p.B, p.G);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nthr = blockDim.x, warps = nthr / 32;
-  const bool writes = blockIdx.x == 0;
+  const int tid = threadIdx.x, nthr = blockDim.x;
+  const bool writes = blockIdx.x == 0;  // what the join and later calls read of the whole batch
+  int turn = 0;
   if (tid < 2) range[tid] = -tid;  // 0, -1: no items
+  if (tid == 2) p.cut_unit[blockIdx.x] = -1;
+  // the first loads of everything, under way together
+  const int member = tid < p.M ? p.members[tid] : 0;
+  int start = 0, stop = 0, share = 0;
+  if (tid < p.G) {
+    start = p.group_start[tid];
+    stop = p.group_start[tid + 1];
+    share = p.prefix_len[tid];
+  }
   for (int b = tid; b < p.B; b += nthr) {
     const int n = p.q_len[b], c = p.ctx_len[b], r0 = p.q_row0[b], k0 = p.paged ? 0 : p.kv_row0[b];
     int bad = 0;
@@ -225,54 +211,52 @@ SD_DEV void make_plan(const RowParams& p, uint8_t* at, int64_t (*s_warp)[32], in
     w.first[b] = v > 0 ? c - v : 0;
     w.group[b] = -1;
     w.listed[b] = 0x7fffffff;
-    if (writes) p.valid_len[b] = v;
   }
-  if (tid == 0) p.cut_unit[blockIdx.x] = -1;
   if (p.G > 0) {
     int bad = 0;
     for (int g = tid; g < p.G; g += nthr) {
-      const int n = p.prefix_len[g], a = p.group_start[g], e = p.group_start[g + 1];
-      bad |= a < 0 || e < a || e > p.M;
-      if (n < 0 && writes) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
-      w.prefix[g] = max(n, 0);
+      if (g != tid) start = p.group_start[g], stop = p.group_start[g + 1], share = p.prefix_len[g];
+      bad |= start < 0 || stop < start || stop > p.M;
+      if (share < 0 && writes) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
+      w.prefix[g] = max(share, 0);
       w.table[g] = 0x7fffffff;
+      w.flags[g] = kGroupRows | kGroupFull;
     }
     // starts that do not ascend within the member list: nobody is in a group, everything is attended to alone
     bad = __syncthreads_or(bad);
     if (bad && tid == 0 && writes) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
     const int M = bad ? 0 : p.M;
     for (int i = tid; i < M; i += nthr) {
-      const int b = p.members[i];
-      if (b >= 0 && b < p.B)
-        atomicMin(&w.listed[b], i);  // a sequence listed twice counts where it is listed first
+      const int b = i == tid ? member : p.members[i];
+      if (b >= 0 && b < p.B) atomicMin(&w.listed[b], i);  // a sequence listed twice counts where it is listed first
     }
     __syncthreads();
     for (int i = tid; i < M; i += nthr) {
-      const int b = p.members[i];
+      const int b = i == tid ? member : p.members[i];
+      int lo = 0, hi = p.G;  // the last group that starts at or before i, and holds it
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (p.group_start[mid] <= i) lo = mid; else hi = mid;
+      }
+      const int gs = p.group_start[lo], ge = p.group_start[lo + 1];
       int2 mr = make_int2(0, 0);
       if (b < 0 || b >= p.B || w.listed[b] != i) {
         if (writes) raise_status(p.status, SPECDEC_STATUS_BAD_GROUP);
-      } else {
-        {
-          int lo = 0, hi = p.G;  // the last group that starts at or before i, and holds it
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (p.group_start[mid] <= i) lo = mid; else hi = mid;
-          }
-          const int gs = p.group_start[lo], ge = p.group_start[lo + 1];
-          if (i >= gs && i < ge) {
-            const int n = w.len[b];
-            w.group[b] = lo;
-            w.vt[b] = (i - gs) * p.q_max;
-            mr = make_int2(p.q_row0[b], n);
-            if (n > 0) {
-              atomicMin(&w.prefix[lo], w.first[b]);  // keys that all of the group's rows see
-              atomicMin(&w.table[lo], i);
-            }
-          }
+        if (i >= gs && i < ge) atomicAnd(&w.flags[lo], 0);
+      } else if (i >= gs && i < ge) {
+        const int n = w.len[b], lead = p.members[gs];
+        w.group[b] = lo;
+        w.vt[b] = (i - gs) * p.q_max;
+        mr = make_int2(p.q_row0[b], n);
+        const bool follows = lead >= 0 && lead < p.B && mr.x >= 0 && mr.x == p.q_row0[lead] + (i - gs) * p.q_max;
+        const int keep = (follows ? kGroupRows : 0) | (n == p.q_max ? kGroupFull : 0);
+        if (keep != (kGroupRows | kGroupFull)) atomicAnd(&w.flags[lo], keep);
+        if (n > 0) {
+          atomicMin(&w.prefix[lo], w.first[b]);  // keys that all of the group's rows see
+          atomicMin(&w.table[lo], i);
         }
       }
-      if (writes) p.member_row[i] = mr;
+      p.member_row[i] = mr;  // (by every CTA, the same: each reads it from here on)
     }
     __syncthreads();
     for (int g = tid; g < p.G; g += nthr) {
@@ -284,119 +268,127 @@ SD_DEV void make_plan(const RowParams& p, uint8_t* at, int64_t (*s_warp)[32], in
     }
   }
   __syncthreads();
-  // cost and unit count of every part
+  // first unit row of every part
   const int parts = p.G + p.B;
-  for (int part = tid; part < parts; part += nthr) {
-    const PartInfo f = part_info(p, w, part);
-    int64_t sum = 0;
-    if (f.group)
-      sum = static_cast<int64_t>(f.rows) * (unit_blocks(p, f, 0) + kUnitCost);
-    else if (f.rows <= kShortPart)
-      for (int r = 0; r < f.rows; ++r) sum += unit_blocks(p, f, r) + kUnitCost;
-    else
-      sum = -1;
-    w.cost[part] = sum * p.KV;
-    w.units[part] = f.rows * p.KV;
-    if (!f.group && writes) {
-      p.seq_group[part - p.G] = w.group[part - p.G];
-      p.seq_vt[part - p.G] = w.group[part - p.G] >= 0 ? w.vt[part - p.G] : 0;
-    }
-  }
-  __syncthreads();
-  for (int part = warp; part < parts; part += warps) {
-    if (w.cost[part] >= 0) continue;
-    const PartInfo f = part_info(p, w, part);
-    int64_t sum = 0;
-    for (int r = lane; r < f.rows; r += 32) sum += unit_blocks(p, f, r) + kUnitCost;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) w.cost[part] = sum * p.KV;
-  }
-  __syncthreads();
-  int64_t run[2] = {0, 0};
-  for (int base = 0; base < parts; base += nthr) {  // exclusive scans, in place
-    const int i = base + tid;
-    int64_t v[2] = {i < parts ? w.cost[i] : 0, i < parts ? w.units[i] : 0}, x[2];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      x[q] = v[q];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x[q], o);
-        if (lane >= o) x[q] += y;
+  int rows = 0;
+  for (int base = 0; base < parts; base += nthr) {
+    const int part = base + tid;
+    int n = 0;
+    if (part < parts) n = (part_info(p, w, part).n_vt + 2 * p.tpt - 1) / (2 * p.tpt);
+    int64_t all;
+    const int at_row = rows + static_cast<int>(plan_scan(n, all, tot, turn));
+    if (part < parts) {
+      w.rows[part] = at_row;
+      if (writes) {
+        p.part_units[part] = at_row * p.KV;
+        if (part >= p.G) {
+          const int b = part - p.G;
+          p.valid_len[b] = w.len[b];
+          p.seq_group[b] = w.group[b];
+          p.seq_vt[b] = w.group[b] >= 0 ? w.vt[b] : 0;
+        }
       }
-      if (lane == 31) s_warp[q][warp] = x[q];
     }
-    __syncthreads();
-    if (warp < 2) {
-      int64_t t = lane < warps ? s_warp[warp][lane] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, t, o);
-        if (lane >= o) t += y;
-      }
-      s_warp[warp][lane] = t;
+    rows += static_cast<int>(all);
+  }
+  if (tid == 0) w.rows[parts] = rows;
+  __syncthreads();
+  auto part_of = [&](int row) {  // the last part that starts at or before the row and has rows
+    int lo = 0, hi = parts;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (w.rows[mid] <= row) lo = mid; else hi = mid;
     }
-    __syncthreads();
-    if (i < parts) {
-      w.cost[i] = run[0] + (warp ? s_warp[0][warp - 1] : 0) + x[0] - v[0];
-      w.units[i] = static_cast<int>(run[1] + (warp ? s_warp[1][warp - 1] : 0) + x[1] - v[1]);
-      if (writes) p.part_units[i] = w.units[i];
+    return lo;
+  };
+  // a unit row's cost (one KV head's unit); rows beyond the threads are counted first, for the total
+  int64_t total = 0, all;
+  if (rows > nthr) {
+    int64_t sum = 0;
+    for (int row = tid; row < rows; row += nthr) {
+      const int part = part_of(row);
+      sum += unit_blocks(p, part_info(p, w, part), row - w.rows[part]) + kUnitCost;
     }
-    run[0] += s_warp[0][31];
-    run[1] += s_warp[1][31];
+    (void)plan_scan(sum * p.KV, total, tot, turn);
     __syncthreads();
   }
-  PlanTotals q;
-  q.total = run[0];
-  q.quota = max((q.total + p.grid - 1) / p.grid, static_cast<int64_t>(p.min_quota));
-  const int64_t from = blockIdx.x * q.quota, to = min(from + q.quota, q.total);
-  auto item_of = [&](const PartInfo& f, int part) {
+  int64_t run = 0, quota = 0, from = 0, to = 0;
+  bool direct_items = false;
+  for (int base = 0; base < rows; base += nthr) {
+    const int row = base + tid;
+    int part = 0, r = 0, nb = 0, cost = 0;
+    PartInfo f = {};
+    if (row < rows) {
+      part = part_of(row);
+      r = row - w.rows[part];
+      f = part_info(p, w, part);
+      nb = unit_blocks(p, f, r);
+      cost = nb + kUnitCost;
+    }
+    const int64_t us0 = run + plan_scan(static_cast<int64_t>(cost) * p.KV, all, tot, turn);
+    run += all;
+    if (base == 0) {
+      if (rows <= nthr) total = all;
+      // (costs pass 32 bits only for prompts of millions of tokens)
+      quota = total < 0x7fffffff ? (static_cast<int>(total) + p.grid - 1) / p.grid : (total + p.grid - 1) / p.grid;
+      quota = max(quota, static_cast<int64_t>(p.min_quota));
+      from = blockIdx.x * quota;
+      to = min(from + quota, total);
+      direct_items = quota <= (1 + kUnitCost) * (kItemsKept - 2);
+    }
+    if (row >= rows || us0 >= to || us0 + static_cast<int64_t>(cost) * p.KV <= from) continue;
+    auto cta_of = [&](int64_t x) {
+      return total < 0x7fffffff ? static_cast<int>(x) / static_cast<int>(quota) : static_cast<int>(x / quota);
+    };
+    const int c = blockIdx.x, b = part - p.G, end = unit_end(p, f, r), cap = f.group ? p.cap_group : p.cap_seq;
     RowItem it = {};
-    const int b = part - p.G;
     it.src = f.group ? ~part : b;
     it.n_vt = f.n_vt;
-    it.row0 = f.group ? 0 : p.q_row0[b];
-    it.first = f.first;
-    it.kv = f.group ? w.table[part] : (p.paged ? b : p.kv_row0[b]);
-    it.member0 = f.group ? p.group_start[part] : 0;
-    return it;
-  };
-  for (int part = tid; part < parts; part += nthr) {
-    const PartInfo f = part_info(p, w, part);
-    if (f.rows == 0 || f.rows > kShortPart || f.group) continue;
-    int64_t start = w.cost[part];
-    if (start >= to || (part + 1 < parts ? w.cost[part + 1] : q.total) <= from) continue;
-    const RowItem it = item_of(f, part);
-    for (int r = 0; r < f.rows; ++r) {
-      emit_row(p, q, f, part, r, start, w.units[part], it, &range[0], &range[1]);
-      start += static_cast<int64_t>(unit_blocks(p, f, r) + kUnitCost) * p.KV;
+    it.vt0 = r * 2 * p.tpt;
+    if (f.group) {
+      it.member0 = p.group_start[part];
+      it.row0 = w.flags[part] & kGroupRows ? p.q_row0[p.members[it.member0]] : -1;
+      it.first = w.flags[part] & kGroupFull;
+      it.kv = w.table[part];
+    } else {
+      it.row0 = p.q_row0[b];
+      it.first = f.first;
+      it.kv = p.paged ? b : p.kv_row0[b];
     }
-  }
-  for (int part = warp; part < parts; part += warps) {
-    const PartInfo f = part_info(p, w, part);
-    if (f.rows == 0 || (f.rows <= kShortPart && !f.group)) continue;
-    int64_t start = w.cost[part];
-    if (start >= to || (part + 1 < parts ? w.cost[part + 1] : q.total) <= from) continue;
-    const RowItem it = item_of(f, part);
-    for (int r0 = 0; r0 < f.rows; r0 += 32) {
-      const int r = r0 + lane;
-      const int64_t cost = r < f.rows ? static_cast<int64_t>(unit_blocks(p, f, r) + kUnitCost) * p.KV : 0;
-      int64_t x = cost;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+    for (int h = 0; h < p.KV; ++h) {
+      const int u = row * p.KV + h;
+      const int64_t us = us0 + static_cast<int64_t>(h) * cost, ue = us + cost;
+      if (us >= to || ue <= from) continue;
+      it.head = h;
+      // pieces that hold blocks: a CTA whose range ends in the unit's own cost has none
+      const int cb = cta_of(us + kUnitCost);  // first CTA with a block
+      const int pieces = cta_of(ue - 1) - cb + 1;
+      const int slot0 = p.compact ? 2 * cb + 1 : u + cb;
+      const int64_t row0 = (f.group ? 0 : p.group_rows) + static_cast<int64_t>(slot0) * cap;
+      // a sequence without shared keys writes its uncut rows itself
+      const bool direct = !f.group && f.k0 == 0 && pieces == 1;
+      if (c == cb) {
+        p.unit_info[u] = make_int2(static_cast<int>(row0), pieces);
+        if (pieces > 1) p.cut_unit[cb] = u;
       }
-      if (r < f.rows) emit_row(p, q, f, part, r, start + x - cost, w.units[part], it, &range[0], &range[1]);
-      start += __shfl_sync(0xffffffffu, x, 31);
+      const int a = static_cast<int>(max(from - us - kUnitCost, static_cast<int64_t>(0)));
+      const int e = static_cast<int>(min(to - us - kUnitCost, static_cast<int64_t>(nb)));
+      const int step = c - cb;
+      it.nblk = max(e - a, 0);
+      it.k0 = f.k0 + a * kKeyBlock;
+      it.k1 = min(f.k0 + e * kKeyBlock, end);
+      it.slot = direct ? -1 : static_cast<int>(row0 + static_cast<int64_t>(p.compact && step > 0 ? 2 * step - 1 : step) * cap);
+      p.items[u + c] = it;
+      if (direct_items) kept[(u + c) % kItemsKept] = it;
+      if (from >= us) range[0] = p.cta_first[c] = u + c;
+      if (to <= ue) range[1] = p.cta_last[c] = u + c;
     }
   }
-  __syncthreads();
-  if (tid == 0) {
-    p.cta_first[blockIdx.x] = range[0];
-    p.cta_last[blockIdx.x] = range[1];
+  if (tid == 0 && from >= total) {  // nothing for this CTA
+    p.cta_first[blockIdx.x] = 0;
+    p.cta_last[blockIdx.x] = -1;
   }
+  return direct_items;
 }
 
 // ---------------------------------------------------------------- geometry
@@ -708,24 +700,24 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   }
   grid_dep_wait();
   grid_dep_launch();
+  bool have_items = false;
   if (p.plan) {
-    __syncthreads();
-    make_plan(p, smem, s_plan, s_range);
+    have_items = make_plan(p, smem, s_plan, s_range, s_items);
+    fence_proxy_async();  // its generic writes are over before the copies into the same memory begin
   } else if (tid == 0) {
     s_range[0] = p.cta_first[blockIdx.x];
     s_range[1] = p.cta_last[blockIdx.x];
   }
-  // (the plan's generic writes are over before the copies into the same memory begin)
-  fence_proxy_async();
   __syncthreads();
   const int i0 = s_range[0], i1 = s_range[1];
-  for (int e = tid; e < 3 * min(i1 - i0 + 1, kItemsKept); e += blockDim.x)
-    reinterpret_cast<int4*>(s_items)[e] = reinterpret_cast<const int4*>(p.items + i0)[e];
+  if (!have_items)
+    for (int e = tid; e < 3 * min(i1 - i0 + 1, kItemsKept); e += blockDim.x)
+      reinterpret_cast<int4*>(s_items + (i0 + e / 3) % kItemsKept)[e % 3] = reinterpret_cast<const int4*>(p.items + i0)[e];
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = s_tmem;
-  auto item_at = [&](int i) { return i - i0 < kItemsKept ? s_items[i - i0] : load_item(p.items + i); };
+  auto item_at = [&](int i) { return i - i0 < kItemsKept ? s_items[i % kItemsKept] : load_item(p.items + i); };
 
   if (warp >= kSoftmaxWarp && warp < kWidenWarp) {
     more_regs<RowRoles<SRC>::SOFTMAX_REGS>();
@@ -747,6 +739,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       if (tok < p.tpt && vt < it.n_vt) {
         if (it.src >= 0) {
           limit = min(it.first + vt + 1, it.k1);
+        } else if (it.first) {
+          limit = it.k1;
         } else {
           const int mb = vt / p.q_max;
           if (vt - mb * p.q_max < p.member_row[it.member0 + mb].y) limit = it.k1;
@@ -761,25 +755,29 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       const int least = __reduce_min_sync(0xffffffffu, limit > 0 ? limit : 0x7fffffff);
       float m = -INFINITY, l = 0.f;
       bool usual = false;  // every row's reference is finite
-      float s[2][64];      // one half's scores are loaded while the other's are worked on
+      // At head_dim 64 one half's scores are loaded while the other's are worked on; at 128 the next half's products
+      // are not done by then, and a warp that waits for them works on nothing.
+      constexpr bool AHEAD = D == 64;
+      float s[AHEAD ? 2 : 1][64];
       auto load = [&](auto half) {
         constexpr int H = decltype(half)::value;
         lazy_wait(&s_full[t][H], (sn >> H) & 1, dead);
         sn ^= 1u << H;
         umma::fence_after_sync();
         if (any_row) {
-          umma::tmem_ld32(s_ta + 64 * H, s[H]);
-          umma::tmem_ld32(s_ta + 64 * H + 32, s[H] + 32);
+          umma::tmem_ld32(s_ta + 64 * H, s[AHEAD ? H : 0]);
+          umma::tmem_ld32(s_ta + 64 * H + 32, s[AHEAD ? H : 0] + 32);
         }
       };
       auto work = [&](auto half, int k) {
         constexpr int H = decltype(half)::value;
         constexpr std::integral_constant<int, 1 - H> other{};
         const bool more = k + 1 < nh;
+        if (!AHEAD) load(half);
         if (!any_row) {
-          if (more) load(other);
+          if (AHEAD && more) load(other);
         } else {
-          float(&x)[64] = s[H];
+          float(&x)[64] = s[AHEAD ? H : 0];
           umma::tmem_wait_ld32(x);
           umma::tmem_wait_ld32(x + 32);
           const int key0 = it.k0 + k * (kKeyBlock / 2);
@@ -802,9 +800,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             usual = __all_sync(0xffffffffu, fabsf(m) < INFINITY);
           }
           float neg = m == -INFINITY ? 0.f : -m * scale;
-          // (head_dim 128: the next half's products are not done by then, and a warp that waits here works on nothing)
           auto next = [&]() {
-            if (D == 64 && more) load(other);
+            if (AHEAD && more) load(other);
           };
           // infinite and NaN scores go through the exponential unit, which knows them
           float sum = usual && !masked ? row_probabilities<true>(x, scale, neg, s_ta + 64 * H, next)
@@ -842,11 +839,10 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         umma::fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t][H]);
-        if (D != 64 && any_row && more) load(other);
       };
       constexpr std::integral_constant<int, 0> even{};
       constexpr std::integral_constant<int, 1> odd{};
-      load(even);
+      if (AHEAD) load(even);
       for (int k = 0; k < nh; k += 2) {
         work(even, k);
         if (k + 1 < nh) work(odd, k + 1);
@@ -1105,8 +1101,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         if (items > 0) ok = row_wait(&q_empty, (items - 1) & 1);
         if (!ok) break;
         ++items;
-        if (it.src >= 0) {
-          // a sequence's rows are a box of n_rep heads x tpt tokens a tile; rows past it meet no other row
+        if (it.row0 >= 0) {
+          // rows that follow one another are a box of n_rep heads x tpt tokens a tile; rows past them meet no other row
           if (lane == 0) {
             mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(tiles * KH * 128 * p.n_rep * p.tpt));
             for (int e = 0; e < tiles; ++e)
@@ -1116,7 +1112,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
                             it.row0 + it.vt0 + e * p.tpt, &q_full);
           }
         } else {
-          // a group's rows are anywhere: a box of n_rep heads a token (the swizzle goes by the address, so that a
+          // a group's rows may be anywhere: a box of n_rep heads a token (the swizzle goes by the address, so that a
           // token may start in the middle of its pattern)
           const int tokens = min(2 * p.tpt, it.n_vt - it.vt0);
           int mine = 0;
