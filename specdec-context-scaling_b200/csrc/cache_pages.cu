@@ -5,9 +5,9 @@
 // them.  New pages are always the lowest free ids, in the order of the request, so the same calls give the same
 // tables whatever ran at the same time on the GPU.
 //
-// Bookkeeping is one CTA's work (counts and scans over the tables in L2; a few microseconds); it leaves a list of
-// (from, to) page pairs, and a second kernel moves those pages in all layers, 16 bytes a load, every load of a
-// thread under way before its first store.  Copies are bound by HBM.
+// What takes an order (which page is free next) is one CTA's work: counts and scans over the tables in L2, a few
+// microseconds.  It leaves a list of (from, to) page pairs, and a last kernel moves those pages in all layers: a warp
+// takes 2 KB at a time, four 16-byte loads a lane under way before the first store.  Copies are bound by HBM.
 #include "sd_common.cuh"
 #include "sd_internal.h"
 
@@ -17,42 +17,45 @@ constexpr int kPoolsPerLaunch = 192;  // K, V and scale pools (64 layers of thre
 
 struct PagePools {
   uint8_t* base[kPoolsPerLaunch];
-  int32_t bytes[3];  // a page of K, V, scales
-  int32_t kinds;     // 2 or 3 pools a layer
-  int32_t pools;
+  int32_t bytes[3];   // a page of K, V, scales
+  int32_t pieces[4];  // first 2 KB piece of each of them in a layer's page, and the number of all
+  int32_t kinds;      // 2 or 3 pools a layer
+  int32_t layers;
 };
+constexpr int kPiece = 2048;
 
 // ---------------------------------------------------------------- moving pages
-// Block (x, pool): pairs x, x + gridDim.x, ... of the list, in one pool.  Both pages of a pair lie in the pool, or
-// the pair is left out (and reported by whoever made the list, or here for a caller's own list).
+// A warp a (pair, layer, 2 KB piece).  Both pages of a pair lie in the pool, or the pair is left out and reported.
 __global__ void __launch_bounds__(256) move_pages_kernel(const __grid_constant__ PagePools pools, const int32_t* src,
                                                          const int32_t* dst, const int32_t* count, int32_t n,
                                                          int32_t num_pages, int32_t* status) {
   grid_dep_wait();
   grid_dep_launch();
-  const int total = count != nullptr ? min(*count, n) : n;
-  const int pool = blockIdx.y;
-  const int bytes = pools.bytes[pool % pools.kinds];
-  uint8_t* base = pools.base[pool];
-  for (int i = blockIdx.x; i < total; i += gridDim.x) {
+  const int pairs = count != nullptr ? min(*count, n) : n;
+  const int lane = threadIdx.x & 31, per_page = pools.pieces[3] * pools.layers;
+  const int64_t all = static_cast<int64_t>(pairs) * per_page, step = static_cast<int64_t>(gridDim.x) * 8;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); u < all; u += step) {
+    const int i = static_cast<int>(u / per_page), rest = static_cast<int>(u - static_cast<int64_t>(i) * per_page);
     const int a = src[i], b = dst[i];
     if (a < 0 || a >= num_pages || b < 0 || b >= num_pages) {
-      if (threadIdx.x == 0 && pool == 0) raise_status(status, SPECDEC_STATUS_BAD_PAGE);
+      if (lane == 0 && rest == 0) raise_status(status, SPECDEC_STATUS_BAD_PAGE);
       continue;
     }
     if (a == b) continue;
+    const int layer = rest / pools.pieces[3], piece = rest - layer * pools.pieces[3];
+    const int kind = piece >= pools.pieces[2] ? 2 : piece >= pools.pieces[1] ? 1 : 0;
+    const int bytes = pools.bytes[kind], at = (piece - pools.pieces[kind]) * kPiece;
+    uint8_t* base = pools.base[layer * pools.kinds + kind] + at;
     const uint4* from = reinterpret_cast<const uint4*>(base + static_cast<int64_t>(a) * bytes);
     uint4* to = reinterpret_cast<uint4*>(base + static_cast<int64_t>(b) * bytes);
-    const int words = bytes / 16;
-    for (int o = threadIdx.x; o < words; o += 4 * blockDim.x) {
-      uint4 x[4];
+    const int words = min(bytes - at, kPiece) / 16;
+    uint4 x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (o + e * static_cast<int>(blockDim.x) < words) x[e] = from[o + e * blockDim.x];
+    for (int e = 0; e < 4; ++e)
+      if (lane + 32 * e < words) x[e] = from[lane + 32 * e];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (o + e * static_cast<int>(blockDim.x) < words) to[o + e * blockDim.x] = x[e];
-    }
+    for (int e = 0; e < 4; ++e)
+      if (lane + 32 * e < words) to[lane + 32 * e] = x[e];
   }
 }
 
@@ -122,68 +125,74 @@ SD_DEV bool page_ok(const PageBook& p, int page) { return page >= 0 && page < p.
 // Row s of the table gives up its pages from entry `keep` on.
 SD_DEV void drop_row(const PageBook& p, int s, int keep, int lane) {
   int32_t* row = p.table + static_cast<int64_t>(s) * p.max_pages;
-  for (int j = keep + lane; j < p.max_pages; j += 32) {
-    const int page = row[j];
-    if (page_ok(p, page)) atomicSub(&p.refs[page], 1);
-    row[j] = -1;
+  for (int base = keep + lane; base < p.max_pages; base += 8 * 32) {
+    int page[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) page[e] = base + 32 * e < p.max_pages ? row[base + 32 * e] : -1;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (page_ok(p, page[e])) atomicSub(&p.refs[page[e]], 1);
+      if (base + 32 * e < p.max_pages) row[base + 32 * e] = -1;
+    }
   }
 }
 
 // Fork: target d = b[i] gives up its pages, takes over the full pages of source s = a[i]'s first c[i] tokens, and
-// gets a page of its own for the started one.
-__global__ void __launch_bounds__(kBookThreads) fork_kernel(const PageBook p) {
+// gets a page of its own for the started one.  A CTA a request does all but the last, taking eight entries a thread at
+// a time; fork_pages_kernel then hands out the started ones' pages, in the order of the requests.
+constexpr int kForkThreads = 256;
+__global__ void __launch_bounds__(kForkThreads) fork_kernel(const PageBook p) {
   grid_dep_wait();
   grid_dep_launch();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int32_t* mark = p.scratch;               // [num_seqs]: bit 31 a source, else the first request with this target
-  int32_t* ok = mark + p.num_seqs;         // [n]
-  int32_t* fresh = ok + p.n;               // [n] free pages
-  for (int s = threadIdx.x; s < p.num_seqs; s += kBookThreads) mark[s] = 0x3fffffff;
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.n; i += kBookThreads) {
-    const int s = p.a[i], d = p.b[i], len = p.c[i];
-    const bool fine = s >= 0 && s < p.num_seqs && d >= 0 && d < p.num_seqs && s != d;
-    if (fine) atomicMin(&mark[d], i);
-    ok[i] = fine && len >= 0 && len <= p.lengths[s] && len <= p.max_pages * kPage;
-  }
-  __syncthreads();
+  const int i = blockIdx.x, tid = threadIdx.x;
+  const int s = p.a[i], d = p.b[i], len = p.c[i];
+  auto in_range = [&](int x) { return x >= 0 && x < p.num_seqs; };
+  const bool fine = in_range(s) && in_range(d) && s != d;
   // a sequence that is forked from stays as it is: it is no target in the same call, and a target is one once
-  for (int i = threadIdx.x; i < p.n; i += kBookThreads) {
-    const int s = p.a[i], d = p.b[i];
-    if (ok[i] && (mark[d] != i || mark[s] != 0x3fffffff)) ok[i] = 0;
-    if (!ok[i]) raise_status(p.status, SPECDEC_STATUS_BAD_SEQUENCE);
+  int bad = !fine || len < 0 || len > p.max_pages * kPage;
+  if (!bad) bad = len > p.lengths[s];
+  for (int k = tid; k < p.n && fine; k += kForkThreads) {
+    const int ks = p.a[k], kd = p.b[k];
+    const bool other = in_range(ks) && in_range(kd) && ks != kd;
+    bad |= other && ((kd == d && k < i) || kd == s);
   }
-  __syncthreads();
-  // the pages that a source's tokens need are there
-  for (int i = warp; i < p.n; i += kBookThreads / 32) {
-    if (!ok[i]) continue;
-    const int32_t* row = p.table + static_cast<int64_t>(p.a[i]) * p.max_pages;
-    const int need = (p.c[i] + kPage - 1) / kPage;
-    bool bad = false;
-    for (int j = lane; j < need; j += 32) bad |= !page_ok(p, row[j]);
-    bad = __any_sync(0xffffffffu, bad);
-    if (bad && lane == 0) {
-      ok[i] = 0;
-      raise_status(p.status, SPECDEC_STATUS_BAD_PAGE);
+  bad = __syncthreads_or(bad);
+  const int32_t* from = p.table + static_cast<int64_t>(fine ? s : 0) * p.max_pages;
+  const int need = (len + kPage - 1) / kPage, full = len / kPage;
+  int lost = 0;
+  for (int j = tid; !bad && j < need; j += kForkThreads) lost |= !page_ok(p, from[j]);
+  lost = __syncthreads_or(lost);
+  if (tid == 0) {
+    p.scratch[i] = !bad && !lost;
+    if (bad) raise_status(p.status, SPECDEC_STATUS_BAD_SEQUENCE);
+    if (lost) raise_status(p.status, SPECDEC_STATUS_BAD_PAGE);
+  }
+  if (bad || lost) return;
+  int32_t* to = p.table + static_cast<int64_t>(d) * p.max_pages;
+  for (int base = tid; base < p.max_pages; base += 8 * kForkThreads) {
+    int old[8], now[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int j = base + e * kForkThreads;
+      old[e] = j < p.max_pages ? to[j] : -1;
+      now[e] = j < full ? from[j] : -1;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int j = base + e * kForkThreads;
+      if (page_ok(p, old[e])) atomicSub(&p.refs[old[e]], 1);
+      if (now[e] >= 0) atomicAdd(&p.refs[now[e]], 1);
+      if (j < p.max_pages) to[j] = now[e];
     }
   }
-  __syncthreads();
-  for (int i = warp; i < p.n; i += kBookThreads / 32)
-    if (ok[i]) drop_row(p, p.b[i], 0, lane);
-  __syncthreads();
-  for (int i = warp; i < p.n; i += kBookThreads / 32) {
-    if (!ok[i]) continue;
-    const int32_t* from = p.table + static_cast<int64_t>(p.a[i]) * p.max_pages;
-    int32_t* to = p.table + static_cast<int64_t>(p.b[i]) * p.max_pages;
-    for (int j = lane; j < p.c[i] / kPage; j += 32) {
-      const int page = from[j];
-      to[j] = page;
-      atomicAdd(&p.refs[page], 1);
-    }
-    if (lane == 0) p.lengths[p.b[i]] = p.c[i];
-  }
-  __syncthreads();
-  // started pages, in the order of the requests
+  if (tid == 0) p.lengths[d] = len;
+}
+
+__global__ void __launch_bounds__(kBookThreads) fork_pages_kernel(const PageBook p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int32_t* ok = p.scratch;
+  int32_t* fresh = p.scratch + p.n;  // [n] free pages
   int want = 0;
   for (int base = 0; base < p.n; base += kBookThreads) {
     const int i = base + threadIdx.x;
@@ -426,19 +435,22 @@ static int move_pages(const SpecdecPagePool* a, const int32_t* src, const int32_
   const int k_bytes = a->num_kv_heads * kPage * a->head_dim * 2;
   pp.bytes[0] = k_bytes;
   pp.bytes[1] = v8 ? k_bytes / 2 : k_bytes;
-  pp.bytes[2] = a->num_kv_heads * kPage * 4;
+  pp.bytes[2] = v8 ? a->num_kv_heads * kPage * 4 : 0;
+  pp.pieces[0] = 0;
+  for (int k = 0; k < 3; ++k) pp.pieces[k + 1] = pp.pieces[k] + (pp.bytes[k] + kPiece - 1) / kPiece;
   const int layers_a_launch = kPoolsPerLaunch / 3;
   for (int l0 = 0; l0 < a->num_layers; l0 += layers_a_launch) {
-    const int nl = a->num_layers - l0 < layers_a_launch ? a->num_layers - l0 : layers_a_launch;
-    for (int l = 0; l < nl; ++l) {
+    pp.layers = a->num_layers - l0 < layers_a_launch ? a->num_layers - l0 : layers_a_launch;
+    for (int l = 0; l < pp.layers; ++l) {
       pp.base[l * pp.kinds] = static_cast<uint8_t*>(a->k_pools[l0 + l]);
       pp.base[l * pp.kinds + 1] = static_cast<uint8_t*>(a->v_pools[l0 + l]);
       if (v8) pp.base[l * pp.kinds + 2] = reinterpret_cast<uint8_t*>(a->v_scales[l0 + l]);
     }
-    pp.pools = nl * pp.kinds;
-    const int grid_x = n < 1024 ? n : 1024;
-    if (int rc = launch_pdl("move_pages_kernel", move_pages_kernel, dim3(grid_x, pp.pools), dim3(256), 0, st, pp, src,
-                            dst, count, n, a->num_pages, status))
+    // every warp of the device a piece, and up to four more in turn
+    const int64_t blocks = (static_cast<int64_t>(n) * pp.layers * pp.pieces[3] + 7) / 8;
+    const int64_t most = static_cast<int64_t>(device_sm_count()) * 8 * 4;
+    if (int rc = launch_pdl("move_pages_kernel", move_pages_kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)),
+                            dim3(256), 0, st, pp, src, dst, count, n, a->num_pages, status))
       return rc;
   }
   return SPECDEC_OK;
@@ -505,7 +517,8 @@ extern "C" int specdec_fork_sequences(const SpecdecPagePool* pool, const Specdec
   p.b = dst;
   p.c = length;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (int rc = launch_pdl("fork_kernel", fork_kernel, dim3(1), dim3(kBookThreads), 0, st, p)) return rc;
+  if (int rc = launch_pdl("fork_kernel", fork_kernel, dim3(n), dim3(kForkThreads), 0, st, p)) return rc;
+  if (int rc = launch_pdl("fork_pages_kernel", fork_pages_kernel, dim3(1), dim3(kBookThreads), 0, st, p)) return rc;
   const int most = n < pool->num_pages ? n : pool->num_pages;
   return move_pages(pool, p.from, p.to, p.count, most, p.status, st);
 }
