@@ -44,7 +44,7 @@ constexpr int kUnitCost = 2;       // what a unit costs beside its blocks (query
 constexpr int kMinQuota = 4;       // smallest range of a CTA, in blocks
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
 constexpr float kGrow = 1.152921504606846976e18f;  // 2^60: a block's sum past it moves the row's reference
-constexpr int kItemsKept = 24;     // items of a CTA that it keeps in shared memory
+constexpr int kItemsKept = 12;     // items of a CTA that it keeps in shared memory
 constexpr float kExpC0 = 0.999924541f, kExpC1 = 0.693136752f, kExpC2 = 0.242639482f, kExpC3 = 0.0558382832f;
 
 enum RowSource { kPacked = 0, kPaged = 1, kPagedE4M3 = 2 };
@@ -84,6 +84,8 @@ struct RowParams {
   const int32_t *group_start, *members, *prefix_len;
   const int32_t* page_table;
   const float* v_scale;
+  const uint8_t* v_pool;         // paged: V blocks; packed: V rows, strides in elements
+  int64_t v_st, v_sh;
   int64_t q_rows, kv_rows;
   int32_t B, H, KV, n_rep, tpt, q_max, G, M;
   int32_t num_pages, max_pages, paged;
@@ -418,6 +420,16 @@ SD_DEV RowItem load_item(const RowItem* at) {
   for (int i = 0; i < 3; ++i) d[i] = s[i];
   return it;
 }
+// Keys from here on are hidden from some of the unit's rows (its first row sees those before).
+SD_DEV int first_hidden(const RowItem& it) { return it.src < 0 ? it.k1 : min(it.first + it.vt0 + 1, it.k1); }
+// First block of the item with keys that some row does not see or that do not exist (none: past the last block).
+SD_DEV int first_washed(const RowItem& it) { return max(first_hidden(it) - it.k0, 0) / kKeyBlock; }
+// The halves of a bf16 pair that are infinite or NaN, as a mask of ones over them.
+SD_DEV uint32_t not_finite(uint32_t w) {
+  const uint32_t hi = ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+  return (hi >> 15) * 0xffffu;
+}
+
 // half blocks (64 keys) of row tile t of an item
 SD_DEV int tile_halves(const RowParams& p, const RowItem& it, int t) {
   const int v0 = it.vt0 + t * p.tpt;
@@ -659,7 +671,10 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[NS], empty[NS], raw_full, raw_empty;
-  __shared__ uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], pv_done[2], o_full[2], c_req, v_clean, fin[2];
+  __shared__ uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], pv_done[2], o_full[2], v_clean[2], bad_read[2][2], fin[2];
+  // [tile][its item % 2]: keys past first_hidden whose V holds an infinity or a NaN.  A tile's items here are those in
+  // which it has work and some row does not see all keys: only those are waited for by both sides.
+  __shared__ uint32_t s_bad[2][2][4][8];  // (a washing warp its own eight words)
   __shared__ RowItem s_items[kItemsKept];  // the CTA's first items
   __shared__ int64_t s_plan[2][32];
   __shared__ int s_range[2];
@@ -677,13 +692,14 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       }
       mbar_init(&pv_done[t], 1);
       mbar_init(&o_full[t], 1);
+      mbar_init(&v_clean[t], 4);
+      mbar_init(&bad_read[t][0], 4);
+      mbar_init(&bad_read[t][1], 4);
     }
     mbar_init(&raw_full, 1);
     mbar_init(&raw_empty, 4);
     mbar_init(&q_full, 1);
     mbar_init(&q_empty, 2);
-    mbar_init(&c_req, 2);
-    mbar_init(&v_clean, 1);
     mbar_init(&fin[0], 1);
     mbar_init(&fin[1], 1);
     fence_barrier_init();
@@ -728,7 +744,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     const uint32_t s_ta = umma::taddr(tmem, lanes, Geo::S_COL + t * 128);
     const uint32_t o_ta = umma::taddr(tmem, lanes, Geo::O_COL + t * D);
     const float scale = p.scale_log2;
-    uint32_t sn = 0, pv = 0, on = 0;  // phase bits of s_full; halves handed over
+    uint32_t sn = 0, pv = 0, on = 0;  // sn: phase bits of s_full; pv: halves handed over
+    uint32_t blk = 0, rd[2] = {0, 0};  // blocks before this item; items of each tile that read s_bad
     bool ok = true, dead = false;
     for (int i = i0; i <= i1 && ok; ++i) {
       const RowItem it = item_at(i);
@@ -746,7 +763,13 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           if (vt - mb * p.q_max < p.member_row[it.member0 + mb].y) limit = it.k1;
         }
       }
-      const int nh = tile_halves(p, it, t);
+      const int nh = tile_halves(p, it, t), nh_other = tile_halves(p, it, t ^ 1);
+      const int hidden = first_hidden(it), blk0 = blk;
+      blk += (max(nh, nh_other) + 1) / 2;
+      const bool reads = hidden < it.k1 && nh > 0, other_reads = hidden < it.k1 && nh_other > 0;
+      const uint32_t rd_mine = rd[t] & 1, rd_other = rd[t ^ 1];
+      rd[t] += reads;
+      rd[t ^ 1] += other_reads;
       if (nh == 0) {  // no tile, or a piece past the tile's keys: the row's other pieces are all of it
         if (it.slot >= 0 && limit > 0) p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
         continue;
@@ -769,10 +792,60 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           umma::tmem_ld32(s_ta + 64 * H + 32, s[AHEAD ? H : 0] + 32);
         }
       };
+      // Washing: what a masked key's zero probability meets must be finite.  V rows past the last key (the next
+      // sequence's, a page's old contents) become zero; an infinity or a NaN in a key that only some rows see becomes
+      // zero, too, and its key is noted for the rows that do see it (add_bad_keys).  The tile that has work in every
+      // block does it, a quarter of the rows a warp; the MMA warps wait for it.  (E4M3: the widening warps do.)
+      const int wash = V8 || nh < nh_other || (nh == nh_other && t == 1) ? 0x7fffffff : first_washed(it);
+      auto wash_block = [&](int j) {
+        uint32_t* const bad = s_bad[t][rd_mine][warp & 3];
+        uint32_t* const bad_other = s_bad[t ^ 1][rd_other & 1][warp & 3];
+        if (j == first_washed(it)) {
+          if (other_reads && rd_other >= 2) lazy_wait(&bad_read[t ^ 1][rd_other & 1], (rd_other / 2 - 1) & 1, dead);
+          if (lane < 8 && reads) bad[lane] = 0;
+          if (lane < 8 && other_reads) bad_other[lane] = 0;
+          __syncwarp();
+        }
+        const uint32_t slot = ((blk0 + j) & 1) * 2 + 1;
+        lazy_wait(&full[slot], ((blk0 + j) >> 1) & 1, dead);
+        uint8_t* const v = smem + Geo::RING + slot * Geo::TILE;
+        const int key0 = it.k0 + j * kKeyBlock;
+        const int r0 = max(hidden - key0, 0), r1 = min(it.k1 - key0, kKeyBlock);
+        // a warp every fourth 512 bytes, four of them under way
+#pragma unroll
+        for (int x = 0; x < KH; ++x) {
+          for (int base = r0 * 128 + (warp & 3) * 512 + lane * 16; base < r1 * 128; base += 4 * 2048) {
+            uint4 w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int o = base + e * 2048;
+              w[e] = o < r1 * 128 ? *reinterpret_cast<const uint4*>(v + x * 16384 + o) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint4 b = make_uint4(not_finite(w[e].x), not_finite(w[e].y), not_finite(w[e].z), not_finite(w[e].w));
+              if (b.x | b.y | b.z | b.w) {
+                const int o = base + e * 2048, bit = key0 + o / 128 - hidden;
+                *reinterpret_cast<uint4*>(v + x * 16384 + o) =
+                    make_uint4(w[e].x & ~b.x, w[e].y & ~b.y, w[e].z & ~b.z, w[e].w & ~b.w);
+                if (reads) atomicOr(&bad[bit >> 5], 1u << (bit & 31));
+                if (other_reads) atomicOr(&bad_other[bit >> 5], 1u << (bit & 31));
+              }
+            }
+          }
+#pragma unroll 4
+          for (int o = r1 * 128 + (warp & 3) * 512 + lane * 16; o < 16384; o += 2048)
+            *reinterpret_cast<uint4*>(v + x * 16384 + o) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_clean[slot >> 1]);
+      };
       auto work = [&](auto half, int k) {
         constexpr int H = decltype(half)::value;
         constexpr std::integral_constant<int, 1 - H> other{};
         const bool more = k + 1 < nh;
+        if (H == 0 && k / 2 >= wash) wash_block(k / 2);
         if (!AHEAD) load(half);
         if (!any_row) {
           if (AHEAD && more) load(other);
@@ -854,6 +927,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       if (!ok) break;
       ++on;
       umma::fence_after_sync();
+      // keys whose V is not finite and that some row does not see: the MMAs had zeros for it
+      const bool any_bad = reads && __any_sync(0xffffffffu, (&s_bad[t][rd_mine][0][0])[lane] != 0);
       if (any_row) {
         if (it.slot >= 0) {
           const int64_t r = it.slot + t * kRowTile + row;
@@ -905,6 +980,56 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           }
         }
         umma::fence_before_sync();  // O is read: the arrival for the next item's first block lets its MMAs write it
+        if (any_bad) {
+          // A row that sees such a key gets its infinities and NaNs here, added to what has just been stored (weighed
+          // by anything above zero they stay what they are).
+          __threadfence_block();
+          __syncwarp();
+          for (int w = 0; w < 32 && limit > 0; ++w) {
+            for (uint32_t bits = (&s_bad[t][rd_mine][0][0])[w]; bits != 0; bits &= bits - 1) {
+              const int key = hidden + 32 * (w & 7) + __ffs(bits) - 1;
+              if (key >= limit) continue;
+              int64_t at = 0;  // packed: the row's first value; paged: the block
+              float vs = 1.f;
+              if (SRC == kPacked) {
+                at = (it.kv + static_cast<int64_t>(key)) * p.v_st + it.head * p.v_sh;
+              } else {
+                int page = p.page_table[static_cast<int64_t>(it.kv) * p.max_pages + key / kPage];
+                if (page < 0 || page >= p.num_pages) page = 0;
+                at = static_cast<int64_t>(page) * p.KV + it.head;
+                if (SRC == kPagedE4M3) vs = p.v_scale[at * kPage + key % kPage];
+              }
+#pragma unroll 1
+              for (int d = 0; d < D; ++d) {
+                float v;
+                if (SRC == kPacked) {
+                  v = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.v_pool)[at + d]);
+                } else if (SRC == kPaged) {
+                  v = __bfloat162float(
+                      *reinterpret_cast<const __nv_bfloat16*>(p.v_pool + at * (kPage * D * 2) + kblock_offset(key % kPage, d)));
+                } else {
+                  const uint32_t h = e4m3x2_to_f16x2(p.v_pool[at * (kPage * D) + key % kPage * D + d]);
+                  v = __half2float(__ushort_as_half(static_cast<unsigned short>(h & 0xffffu))) * vs;
+                  v = __bfloat162float(__float2bfloat16(v));
+                }
+                if (fabsf(v) < INFINITY) continue;
+                if (it.slot >= 0) {
+                  const int64_t r = it.slot + t * kRowTile + row;
+                  float* const o = reinterpret_cast<float*>(p.part_o + (r >> 5) * (8 * D) + d / 4 * 32 + lane) + d % 4;
+                  *o += v;
+                } else {
+                  __nv_bfloat16* const o = p.out + static_cast<int64_t>(it.row0 + vt) * p.o_st +
+                                           static_cast<int64_t>(it.head * p.n_rep + rep) * p.o_sh + d;
+                  *o = __float2bfloat16(__bfloat162float(*o) + v);
+                }
+              }
+            }
+          }
+        }
+      }
+      if (reads) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bad_read[t][rd_mine]);
       }
     }
     if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
@@ -1001,7 +1126,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       const uint32_t k_low = umma::desc_low(smem_u32(smem + Geo::RING), 16);
       const uint32_t v_low = umma::desc_low(smem_u32(smem + Geo::RING), 16384);
       const uint32_t s_col = tmem + Geo::S_COL + t * 128, o_col = tmem + Geo::O_COL + t * D;
-      uint32_t pn = 0, items = 0, cleaned = 0;  // pn: phase bits of p_full
+      uint32_t pn = 0, items = 0, cleaned = 0;  // pn, cleaned: phase bits of p_full, v_clean
       uint32_t ks = 0, kp = 0;  // ring slot of the next block in the ring, and its phase
       bool ok = true;
       auto next = [&](uint32_t& s, uint32_t& ph) {
@@ -1040,7 +1165,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         // (a reduction's result is known to be the same in all lanes: loops and descriptors stay in uniform registers)
         const int nh = __reduce_max_sync(0xffffffffu, tile_halves(p, it, t));
         const int nb = (max(nh, __reduce_max_sync(0xffffffffu, tile_halves(p, it, t ^ 1))) + 1) / 2;
-        const bool clean = !V8 && (it.k1 - it.k0) % kKeyBlock != 0;
+        const int wash = V8 ? 0x7fffffff : __reduce_max_sync(0xffffffffu, first_washed(it));
         ok = row_wait(&q_full, items & 1) && row_wait(&full[ks], kp);
         if (!ok) break;
         umma::fence_after_sync();
@@ -1057,12 +1182,9 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           if (!last) ok = ok && row_wait(&full[ks], kp);
           if (!ok) break;
           umma::fence_after_sync();
-          if (clean && last) {
-            // the last block's V is zeroed past the last key while the softmax works on the block
-            if (lane == 0) mbar_arrive(&c_req);
-            __syncwarp();
-            if (2 * j < nh) ok = row_wait(&v_clean, cleaned & 1);
-            ++cleaned;
+          if (j >= wash) {  // the softmax warps wash this block's V
+            ok = row_wait(&v_clean[vs >> 1], (cleaned >> (vs >> 1)) & 1);
+            cleaned ^= 1u << (vs >> 1);
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -1091,8 +1213,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       commit(&fin[t]);
       (void)row_wait(&fin[t], 0);
     } else if (warp == kQueryWarp) {
-      // ---------------------------------------------------------- query rows; V rows past the last key
-      uint32_t items = 0, cleaned = 0, n = 0;
+      // ---------------------------------------------------------- query rows
+      uint32_t items = 0;
       bool ok = true;
       for (int i = i0; i <= i1 && ok; ++i) {
         const RowItem it = item_at(i);
@@ -1136,31 +1258,13 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           }
         }
         __syncwarp();
-        const int nb = (max(tile_halves(p, it, 0), tile_halves(p, it, 1)) + 1) / 2;
-        const int rem = (it.k1 - it.k0) % kKeyBlock;
-        if (!V8 && rem != 0) {
-          const uint32_t k = n + 2 * nb - 1;
-          // asked for by the MMA warps, which have seen the block arrive and wait for the answer
-          ok = row_wait(&c_req, cleaned & 1);
-          if (!ok) break;
-          uint8_t* v = smem + Geo::RING + (k % NS) * Geo::TILE;
-#pragma unroll
-          for (int x = 0; x < KH; ++x)
-            for (int o = rem * 128 + lane * 16; o < 16384; o += 512)
-              *reinterpret_cast<uint4*>(v + x * 16384 + o) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_clean);
-          ++cleaned;
-        }
-        n += 2 * nb;
       }
       if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
     } else {
       // ---------------------------------------------------------- E4M3: codes to bf16, a thread a key
       if constexpr (V8) {
         const int r = tid - 32 * kWidenWarp;
-        uint32_t n = 1;
+        uint32_t n = 1, rd[2] = {0, 0};
         bool ok = true;
         for (int i = i0; i <= i1 && ok; ++i) {
           const RowItem it = item_at(i);
@@ -1174,10 +1278,24 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             if (page < 0 || page >= p.num_pages) page = 0;  // the loading warp reports it
             return p.v_scale[(static_cast<int64_t>(page) * p.KV + it.head) * kPage + key % kPage];
           };
+          // (washing, as the softmax warps do it for bf16)
+          const int hidden = first_hidden(it);
+          bool reads[2];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            reads[t] = hidden < it.k1 && tile_halves(p, it, t) > 0;
+            if (!reads[t]) continue;
+            if (rd[t] >= 2) ok = ok && row_wait(&bad_read[t][rd[t] & 1], (rd[t] / 2 - 1) & 1);
+            if (lane < 8) s_bad[t][rd[t] & 1][r >> 5][lane] = 0;
+          }
+          __syncwarp();
+          if (!ok) break;
           float next = scale_of(0);
           for (int j = 0; j < nb; ++j, n += 2) {
             const float sc = next;
-            const bool in = it.k0 + j * kKeyBlock + r < it.k1;
+            const int key = it.k0 + j * kKeyBlock + r;
+            const bool in = key < it.k1;
+            uint32_t bad = 0;
             if (j + 1 < nb) next = scale_of(j + 1);
             const uint32_t s = n % NS;
             ok = row_wait(&raw_full, (n >> 1) & 1);
@@ -1197,10 +1315,23 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
                 y[e] = in ? pack_bf16(f.x * sc, f.y * sc) : 0u;
               }
+              if (key >= hidden) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const uint32_t b = not_finite(y[e]);
+                  bad |= b;
+                  y[e] &= ~b;
+                }
+              }
               uint8_t* d = dst + (ch >> 2) * 16384;
               const int g = (ch & 3) * 2;
               *reinterpret_cast<uint4*>(d + ((g ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
               *reinterpret_cast<uint4*>(d + (((g + 1) ^ (r & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+            }
+            if (bad) {
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+                if (reads[t]) atomicOr(&s_bad[t][rd[t] & 1][r >> 5][(key - hidden) >> 5], 1u << ((key - hidden) & 31));
             }
             fence_proxy_async();
             __syncwarp();
@@ -1209,6 +1340,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
               mbar_arrive(&raw_empty);
             }
           }
+          rd[0] += reads[0];
+          rd[1] += reads[1];
         }
         if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
       }
@@ -1533,6 +1666,9 @@ extern "C" int specdec_prompt_attention(const SpecdecPromptArgs* a, specdec_stre
   p.q_len = bt.q_len;
   p.ctx_len = bt.ctx_len;
   p.kv_row0 = a->kv_row0;
+  p.v_pool = static_cast<const uint8_t*>(a->v);
+  p.v_st = a->v_stride_tok;
+  p.v_sh = a->v_stride_head;
   p.q_rows = a->q_rows;
   p.kv_rows = a->kv_rows;
   p.status = a->status;
@@ -1596,6 +1732,7 @@ extern "C" int specdec_shared_prefix_attention(const SpecdecSharedPrefixArgs* a,
   p.max_pages = kv.max_pages_per_seq;
   p.paged = 1;
   p.v_scale = kv.v_scale;
+  p.v_pool = static_cast<const uint8_t*>(kv.v_pool);
   p.q_rows = a->q_rows;
   p.status = a->status;
   CUtensorMap qm, tm, km, vm;
