@@ -45,7 +45,7 @@ constexpr int kMinQuota = 4;       // smallest range of a CTA, in blocks
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
 constexpr float kGrow = 1.152921504606846976e18f;  // 2^60: a block's sum past it moves the row's reference
 constexpr int kItemsKept = 12;     // items of a CTA that it keeps in shared memory
-constexpr float kExpC0 = 0.999924541f, kExpC1 = 0.693136752f, kExpC2 = 0.242639482f, kExpC3 = 0.0558382832f;
+constexpr float kExpC1 = 0.693282962f, kExpC2 = 0.242210999f, kExpC3 = 0.0550089143f;
 
 enum RowSource { kPacked = 0, kPaged = 1, kPagedE4M3 = 2 };
 constexpr int kLoadWarp = 0, kIssueWarp = 1, kQueryWarp = 3, kSoftmaxWarp = 4, kWidenWarp = 12;
@@ -331,17 +331,17 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
     run += all;
     if (base == 0) {
       if (rows <= nthr) total = all;
-      // (costs pass 32 bits only for prompts of millions of tokens)
-      quota = total < 0x7fffffff ? (static_cast<int>(total) + p.grid - 1) / p.grid : (total + p.grid - 1) / p.grid;
-      quota = max(quota, static_cast<int64_t>(p.min_quota));
+      if (total >= 0x7fffffff) {  // 2^31 blocks are half a minute of this device's tensor cores
+        if (writes && tid == 0) raise_status(p.status, SPECDEC_STATUS_BAD_LENGTH);
+        total = 0;
+      }
+      quota = max((static_cast<int>(total) + p.grid - 1) / p.grid, p.min_quota);
       from = blockIdx.x * quota;
       to = min(from + quota, total);
       direct_items = quota <= (1 + kUnitCost) * (kItemsKept - 2);
     }
-    if (row >= rows || us0 >= to || us0 + static_cast<int64_t>(cost) * p.KV <= from) continue;
-    auto cta_of = [&](int64_t x) {
-      return total < 0x7fffffff ? static_cast<int>(x) / static_cast<int>(quota) : static_cast<int>(x / quota);
-    };
+    if (row >= rows || total == 0 || us0 >= to || us0 + static_cast<int64_t>(cost) * p.KV <= from) continue;
+    auto cta_of = [&](int64_t x) { return static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(quota)); };
     const int c = blockIdx.x, b = part - p.G, end = unit_end(p, f, r), cap = f.group ? p.cap_group : p.cap_seq;
     RowItem it = {};
     it.src = f.group ? ~part : b;
@@ -550,11 +550,12 @@ SD_DEV float max3_nan(float a, float b, float c) {
   return r;
 }
 
-// 2^x on the FMA units, for finite x: x = n + f with f in [-1/2, 1/2], 2^f by the cubic that is exact at the four
-// Chebyshev nodes of that interval (relative error below 2^-13, against the 2^-9 that P is rounded to), n added to
-// the exponent.  x is clamped to [-126, 127] as z = (x + 126) / 253 in [0, 1], which costs nothing beside the scaling;
-// z's rounding moves x by less than 2^-16.
-constexpr float kPolyLow = -126.f, kPolySpan = 253.f;
+// 2^x on the FMA units: x = n + f with f in [-1/2, 1/2], 2^f by the cubic through 1 at 0 with the least largest relative
+// error on that interval (1.0e-04, against the 2^-9 that P is rounded to), n added to the exponent.  x is clamped to
+// [-127, 127] as z = (x + 127) / 254 in [0, 1], which costs nothing beside the scaling; z's rounding moves x by less
+// than 2^-16.  At -127 the exponent and the mantissa of 1 cancel: masked keys and all that is smaller give exactly 0.
+// (The clamp hides a NaN: the caller looks for one.)
+constexpr float kPolyLow = -127.f, kPolySpan = 254.f;
 constexpr float kRound = 12582912.f;  // 1.5 x 2^23: the low mantissa bits of x + kRound are the nearest integer
 struct Poly2 {
   uint64_t z, t, f, y;
@@ -574,7 +575,7 @@ struct Poly2 {
     } else if constexpr (STEP == 5) {
       y = fma2(y, f, pack2(kExpC1, kExpC1));
     } else {
-      y = fma2(y, f, pack2(kExpC0, kExpC0));
+      y = fma2(y, f, pack2(1.f, 1.f));
     }
   }
   SD_DEV void result(float& a, float& b) {
@@ -593,17 +594,20 @@ struct Poly2 {
 // Eight pairs of scores at once: six take the exponential unit (12 x 8.5 clocks a warp), two the polynomial, whose
 // steps lie between the others'.  A pair costs about 8 issue slots by the unit and 24 by the polynomial, so a quarter
 // of the pairs balances the two.  Probabilities as bf16 pairs in w[0 .. 7], their sums added to `sum`.
-SD_DEV void eight_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, float zn, uint64_t (&sum)[4], uint32_t* w) {
+SD_DEV void eight_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, float zn, uint64_t (&sum)[2], float& seen,
+                        uint32_t* w) {
   Poly2 p[2];
   float x[12], y[12], a, b;
 #define SD_X(E) unpack2(fma2(pack2(s[2 * (E)], s[2 * (E) + 1]), sc, ng), x[2 * (E)], x[2 * (E) + 1]);
 #define SD_Y(E) y[E] = exp2_unit(x[E]);
 #define SD_P(I, K) p[I].step<K>(s[12 + 2 * (I)], s[13 + 2 * (I)], zs, zn);
 #define SD_W(E)                                              \
-  sum[(E) & 3] = add2(sum[(E) & 3], pack2(y[2 * (E)], y[2 * (E) + 1])); \
+  sum[(E) & 1] = add2(sum[(E) & 1], pack2(y[2 * (E)], y[2 * (E) + 1])); \
   w[E] = round_bf16(y[2 * (E)], y[2 * (E) + 1]);
   SD_X(0) SD_Y(0) SD_P(0, 0)
+  seen = max3_nan(seen, s[12], s[13]);
   SD_Y(1) SD_X(1) SD_P(1, 0)
+  seen = max3_nan(seen, s[14], s[15]);
   SD_Y(2) SD_P(0, 1) SD_X(2)
   SD_Y(3) SD_P(1, 1) SD_P(0, 2)
   SD_Y(4) SD_W(0) SD_P(1, 2) SD_X(3)
@@ -614,11 +618,11 @@ SD_DEV void eight_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, floa
   SD_Y(9) SD_W(3) SD_P(0, 6) SD_P(1, 6)
   SD_Y(10)
   p[0].result(a, b);
-  sum[2] = add2(sum[2], pack2(a, b));
+  sum[0] = add2(sum[0], pack2(a, b));
   w[6] = round_bf16(a, b);
   SD_Y(11)
   p[1].result(a, b);
-  sum[3] = add2(sum[3], pack2(a, b));
+  sum[1] = add2(sum[1], pack2(a, b));
   w[7] = round_bf16(a, b);
   SD_W(4) SD_W(5)
 #undef SD_X
@@ -636,28 +640,30 @@ SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t ng, uint64_t& sum, ui
   *w = round_bf16(a, b);
 }
 
-// P = 2^(s scale + neg) of 64 scores as bf16 in 32 TMEM columns; returns the sum.  POLY: eight of the 32 pairs by
-// polynomial.  `before_last` is called when a quarter is left.
+// P = 2^(s scale + neg) of 64 scores as bf16 in 32 TMEM columns; returns the sum, and in `seen` a NaN if there is one
+// among the scores that took the polynomial.  POLY: eight of the 32 pairs do.  `before_last` is called when a quarter
+// is left.
 template <bool POLY, typename Hook>
-SD_DEV float row_probabilities(const float* s, float scale, float neg, uint32_t ta, Hook before_last) {
+SD_DEV float row_probabilities(const float* s, float scale, float neg, uint32_t ta, float& seen, Hook before_last) {
   const uint64_t sc = pack2(scale, scale), ng = pack2(neg, neg);
   const float zs = scale * (1.f / kPolySpan), zn = (neg - kPolyLow) * (1.f / kPolySpan);
-  uint64_t sum[4] = {0, 0, 0, 0};
+  uint64_t sum[2] = {0, 0};
   uint32_t w[32];
+  seen = -INFINITY;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     if (q == 3) before_last();
     if (POLY) {
-      eight_pairs(s + 16 * q, sc, ng, zs, zn, sum, w + 8 * q);
+      eight_pairs(s + 16 * q, sc, ng, zs, zn, sum, seen, w + 8 * q);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) one_pair(s + 16 * q + 2 * e, sc, ng, sum[e & 3], w + 8 * q + e);
+      for (int e = 0; e < 8; ++e) one_pair(s + 16 * q + 2 * e, sc, ng, sum[e & 1], w + 8 * q + e);
     }
     if (q == 1) umma::tmem_st16_words(ta, reinterpret_cast<const uint32_t(&)[16]>(w[0]));
   }
   umma::tmem_st16_words(ta + 16, reinterpret_cast<const uint32_t(&)[16]>(w[16]));
   float a, b;
-  unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
+  unpack2(add2(sum[0], sum[1]), a, b);
   return a + b;
 }
 
@@ -777,7 +783,6 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       const bool any_row = __any_sync(0xffffffffu, limit > 0);
       const int least = __reduce_min_sync(0xffffffffu, limit > 0 ? limit : 0x7fffffff);
       float m = -INFINITY, l = 0.f;
-      bool usual = false;  // every row's reference is finite
       // At head_dim 64 one half's scores are loaded while the other's are worked on; at 128 the next half's products
       // are not done by then, and a warp that waits for them works on nothing.
       constexpr bool AHEAD = D == 64;
@@ -810,32 +815,26 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         lazy_wait(&full[slot], ((blk0 + j) >> 1) & 1, dead);
         uint8_t* const v = smem + Geo::RING + slot * Geo::TILE;
         const int key0 = it.k0 + j * kKeyBlock;
-        const int r0 = max(hidden - key0, 0), r1 = min(it.k1 - key0, kKeyBlock);
-        // a warp every fourth 512 bytes, four of them under way
-#pragma unroll
+        // (the MMAs take 16 keys a step, and none of the steps past the last key's)
+        const int o0 = max(hidden - key0, 0) * 128, o1 = min(it.k1 - key0, kKeyBlock) * 128;
+        // (small code: what runs once an item is bound by fetching its instructions)
+#pragma unroll 1
         for (int x = 0; x < KH; ++x) {
-          for (int base = r0 * 128 + (warp & 3) * 512 + lane * 16; base < r1 * 128; base += 4 * 2048) {
-            uint4 w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int o = base + e * 2048;
-              w[e] = o < r1 * 128 ? *reinterpret_cast<const uint4*>(v + x * 16384 + o) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+          for (int o = o0 + (warp & 3) * 512 + lane * 16; o < ((o1 + 2047) & ~2047); o += 2048) {
+            uint4* const chunk = reinterpret_cast<uint4*>(v + x * 16384 + o);
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (o < o1) {
+              w = *chunk;
+              const uint4 b = make_uint4(not_finite(w.x), not_finite(w.y), not_finite(w.z), not_finite(w.w));
+              if (!(b.x | b.y | b.z | b.w)) continue;
+              w = make_uint4(w.x & ~b.x, w.y & ~b.y, w.z & ~b.z, w.w & ~b.w);
+              const int bit = key0 + o / 128 - hidden;
+              if (reads) atomicOr(&bad[bit >> 5], 1u << (bit & 31));
+              if (other_reads) atomicOr(&bad_other[bit >> 5], 1u << (bit & 31));
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint4 b = make_uint4(not_finite(w[e].x), not_finite(w[e].y), not_finite(w[e].z), not_finite(w[e].w));
-              if (b.x | b.y | b.z | b.w) {
-                const int o = base + e * 2048, bit = key0 + o / 128 - hidden;
-                *reinterpret_cast<uint4*>(v + x * 16384 + o) =
-                    make_uint4(w[e].x & ~b.x, w[e].y & ~b.y, w[e].z & ~b.z, w[e].w & ~b.w);
-                if (reads) atomicOr(&bad[bit >> 5], 1u << (bit & 31));
-                if (other_reads) atomicOr(&bad_other[bit >> 5], 1u << (bit & 31));
-              }
-            }
+            *chunk = w;
           }
-#pragma unroll 4
-          for (int o = r1 * 128 + (warp & 3) * 512 + lane * 16; o < 16384; o += 2048)
-            *reinterpret_cast<uint4*>(v + x * 16384 + o) = make_uint4(0u, 0u, 0u, 0u);
         }
         fence_proxy_async();
         __syncwarp();
@@ -868,23 +867,20 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
               for (int e = 0; e < 4; ++e) mx[e] = max3_nan(mx[e], x[c + e], x[c + 4 + e]);
             return max3_nan(max3_nan(mx[0], mx[1], x[60]), max3_nan(mx[2], mx[3], x[61]), max_nan(x[62], x[63]));
           };
-          if (k == 0) {
-            m = row_max();
-            usual = __all_sync(0xffffffffu, fabsf(m) < INFINITY);
-          }
-          float neg = m == -INFINITY ? 0.f : -m * scale;
+          if (k == 0) m = row_max();
+          float neg = m == -INFINITY ? 0.f : -m * scale, seen;
           auto next = [&]() {
             if (AHEAD && more) load(other);
           };
-          // infinite and NaN scores go through the exponential unit, which knows them
-          float sum = usual && !masked ? row_probabilities<true>(x, scale, neg, s_ta + 64 * H, next)
-                                       : row_probabilities<false>(x, scale, neg, s_ta + 64 * H, next);
+          float sum = row_probabilities<true>(x, scale, neg, s_ta + 64 * H, seen, next);
           // Past the reference by more than 2^60 (or no reference yet, every key so far being masked): the
-          // reference becomes this half block's maximum, O and l are rescaled and it is done again, once.  A NaN
-          // stays one; a row without a key so far has none to refer to.
-          const bool move = (!(sum < kGrow) || (m == -INFINITY && sum > 0.f)) && m == m && m < INFINITY;
-          if (__any_sync(0xffffffffu, move)) {
+          // reference becomes this half block's maximum, O and l are rescaled and it is done again, once.  Infinite
+          // and NaN scores and references go through the exponential unit, which knows them; a NaN stays one.
+          // (Rows of the tile that are no token's hold anything; rows that see nothing here add nothing.)
+          const bool redo = limit > key0 && (!(sum < kGrow) || seen != seen || !(fabsf(m) < INFINITY));
+          if (__any_sync(0xffffffffu, redo)) {
             const float bm = row_max();
+            const bool move = redo && m < INFINITY && bm != m;
             const float alpha = move ? fast_exp2(((m == -INFINITY ? bm : m) - bm) * scale) : 1.f;
             if (move) m = bm;
             l *= alpha;
@@ -902,8 +898,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
               }
             }
             neg = m == -INFINITY ? 0.f : -m * scale;
-            sum = row_probabilities<false>(x, scale, neg, s_ta + 64 * H, []() {});
-            usual = __all_sync(0xffffffffu, fabsf(m) < INFINITY);
+            sum = row_probabilities<false>(x, scale, neg, s_ta + 64 * H, seen, []() {});
           }
           l += sum;
           umma::tmem_wait_st();
@@ -955,26 +950,25 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           int64_t to[4];
 #pragma unroll
           for (int g = 0; g < 4; ++g) to[g] = __shfl_sync(0xffffffffu, at, g * 8 + lane / 4);
-          float o[2][32];
-          umma::tmem_ld32(o_ta, o[0]);
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            umma::tmem_wait_ld32(o[c & 1]);
-            if (c + 1 < D / 32) umma::tmem_ld32(o_ta + 32 * (c + 1), o[(c + 1) & 1]);
-            const float* v = o[c & 1];
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            umma::tmem_ld32(o_ta + c, o);
+            umma::tmem_wait_ld32(o);
             // 16-byte chunk e of row r lies at place e ^ (r / 2 % 4): no bank conflicts either way
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
-                  make_uint4(pack_bf16(v[8 * e] * inv, v[8 * e + 1] * inv), pack_bf16(v[8 * e + 2] * inv, v[8 * e + 3] * inv),
-                             pack_bf16(v[8 * e + 4] * inv, v[8 * e + 5] * inv),
-                             pack_bf16(v[8 * e + 6] * inv, v[8 * e + 7] * inv));
+                  make_uint4(pack_bf16(o[8 * e] * inv, o[8 * e + 1] * inv), pack_bf16(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                             pack_bf16(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
+                             pack_bf16(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
             __syncwarp();
+            const int ch = lane & 3;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              const int r = g * 8 + lane / 4, ch = lane & 3;
+              const int r = g * 8 + lane / 4;
               const uint4 y = *reinterpret_cast<const uint4*>(stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4));
-              if (to[g] >= 0) *reinterpret_cast<uint4*>(p.out + to[g] + c * 32 + ch * 8) = y;
+              if (to[g] >= 0) *reinterpret_cast<uint4*>(p.out + to[g] + c + ch * 8) = y;
             }
             __syncwarp();
           }
@@ -1144,12 +1138,13 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         }
         __syncwarp();
       };
-      auto pv = [&](int h, uint32_t slot, bool acc) {
+      auto pv = [&](int h, uint32_t slot, bool acc, int steps) {  // steps of 16 keys
         const uint32_t vl = v_low + slot * (Geo::TILE >> 4);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma::mma_f16_ts_low<id_pv, high>(o_col, s_col, 64 * h + kk * 8, vl, h * (8192 >> 4) + kk * (2048 >> 4),
+            if (kk < steps)
+              umma::mma_f16_ts_low<id_pv, high>(o_col, s_col, 64 * h + kk * 8, vl, h * (8192 >> 4) + kk * (2048 >> 4),
                                               acc || kk > 0);
           umma::commit(&pv_done[t]);
         }
@@ -1165,6 +1160,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         // (a reduction's result is known to be the same in all lanes: loops and descriptors stay in uniform registers)
         const int nh = __reduce_max_sync(0xffffffffu, tile_halves(p, it, t));
         const int nb = (max(nh, __reduce_max_sync(0xffffffffu, tile_halves(p, it, t ^ 1))) + 1) / 2;
+        const int last_key = __reduce_max_sync(0xffffffffu, it.k1 - it.k0);
         const int wash = V8 ? 0x7fffffff : __reduce_max_sync(0xffffffffu, first_washed(it));
         ok = row_wait(&q_full, items & 1) && row_wait(&full[ks], kp);
         if (!ok) break;
@@ -1194,7 +1190,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
               if (!ok) break;
               pn ^= 1u << h;
               umma::fence_after_sync();
-              pv(h, vs, k > 0);
+              pv(h, vs, k > 0, (last_key - k * (kKeyBlock / 2) + 15) / 16);
               if (k == nh - 1) commit(&o_full[t]);
               if (k + 2 < nh) qk(h, ks);
             }
