@@ -32,6 +32,12 @@
  *   specdec_lmhead_argmax        <- logits = x @ embed_tokens.weight.T (model_self.py:857)
  *                                   followed by the executors' argmax (spec_dec.py:230-236,
  *                                   fast_spec_dec.py:246-249), fused: no logits are written
+ *   specdec_prompt_attention     <- the prompt pass's attention in SelfAttention.forward,
+ *                                   specdec/engine/model_self.py:715-775, for packed prompts of any lengths
+ *   specdec_shared_prefix_attention, specdec_copy_pages, specdec_fork_sequences,
+ *   specdec_reserve_pages, specdec_free_sequences, specdec_compact_pages
+ *                                <- no counterpart (the reference runs batch 1): a prefix that sequences
+ *                                   share is read once, and pages pass between sequences
  *   specdec_*_int8               <- no counterpart (the reference's linear layers are bf16):
  *                                   8-bit activations and weights for the decoder's projections
  */
@@ -352,7 +358,9 @@ int specdec_attention_fp8v(const void* q, const void* k, const void* v_codes, co
  * reference's prompt pass (specdec/engine/model_self.py:715-775).
  * q, k, v, out 16-byte aligned, strides multiples of 8 elements; sm_scale positive.
  * reuse_plan 1: the workspace holds the plan of an earlier call with the same batch (lengths, rows, heads,
- * num_sms): the layers of one prompt pass.  Calls that share a workspace must not overlap.
+ * num_sms): the layers of one prompt pass.  A workspace without a plan for these shapes is refused on the device
+ * (SPECDEC_STATUS_PLAN_MISMATCH, nothing written).  Calls that share a workspace must not overlap, and out overlaps
+ * none of q, k and v.  Up to 2048 sequences a call (and as many groups and members below).
  */
 typedef struct SpecdecPromptArgs {
   const void* q;

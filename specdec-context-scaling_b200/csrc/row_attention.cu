@@ -29,6 +29,7 @@
 // The running maximum moves only when a row's grows by more than 2^8 (then O is rescaled in place); S_t(j) is complete
 // only after O_t(j - 1), both being issued in this order by one lane, so the rescale needs no wait of its own.
 // P is rounded to bf16 (2^-9 of each weight, independent between keys); sums, maxima and O stay fp32.
+#include <initializer_list>
 #include <type_traits>
 
 #include "sd_common.cuh"
@@ -44,6 +45,7 @@ constexpr int kUnitCost = 2;       // what a unit costs beside its blocks (query
 constexpr int kMinQuota = 4;       // smallest range of a CTA, in blocks
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
 constexpr float kGrow = 1.152921504606846976e18f;  // 2^60: a block's sum past it moves the row's reference
+constexpr float kLargeScore = 4096.f;  // in units of log2
 constexpr int kItemsKept = 12;     // items of a CTA that it keeps in shared memory
 constexpr float kExpC1 = 0.693282962f, kExpC2 = 0.242210999f, kExpC3 = 0.0550089143f;
 
@@ -94,11 +96,14 @@ struct RowParams {
   int32_t cap_seq, cap_group;   // workspace rows of a sequence's / a group's slot
   int32_t group_rows;           // workspace rows before the sequences' slots
   float scale_log2;
+  uint64_t key;                 // of this launch shape
   int32_t* status;
   // workspace
   int32_t *cta_first, *cta_last, *cut_unit;     // [grid]
   int32_t* part_units;                          // [G + B] starts
-  int32_t *valid_len, *seq_group, *seq_vt;      // [B]
+  uint64_t* plan_key;                           // the launch shape that the plan is for
+  int2* seq_rows;                               // [B] {first query row, valid tokens}
+  int32_t *seq_group, *seq_vt;                  // [B]
   int32_t* prefix;                              // [G]
   int2* member_row;                             // [M] {first query row, tokens}
   int2* unit_info;                              // [units] {first slot row, pieces}
@@ -190,6 +195,7 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
   int turn = 0;
   if (tid < 2) range[tid] = -tid;  // 0, -1: no items
   if (tid == 2) p.cut_unit[blockIdx.x] = -1;
+  if (tid == 3 && writes) *p.plan_key = p.key;
   // the first loads of everything, under way together
   const int member = tid < p.M ? p.members[tid] : 0;
   int start = 0, stop = 0, share = 0;
@@ -285,7 +291,7 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
         p.part_units[part] = at_row * p.KV;
         if (part >= p.G) {
           const int b = part - p.G;
-          p.valid_len[b] = w.len[b];
+          p.seq_rows[b] = make_int2(p.q_row0[b], w.len[b]);
           p.seq_group[b] = w.group[b];
           p.seq_vt[b] = w.group[b] >= 0 ? w.vt[b] : 0;
         }
@@ -630,21 +636,22 @@ SD_DEV void eight_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, floa
 #undef SD_P
 #undef SD_W
 }
-SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t ng, uint64_t& sum, uint32_t* w) {
+// The rare way: exact where the scores are large, whatever they are (infinities and NaNs too).
+SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t minus_m, uint64_t& sum, uint32_t* w) {
   float a, b;
-  unpack2(fma2(pack2(s[0], s[1]), sc, ng), a, b);
-  // scores beyond 2^30 miss the reference by more than an exponent holds (their own rounding); NaN stays
-  a = exp2_unit(a > 60.f ? 60.f : a);
-  b = exp2_unit(b > 60.f ? 60.f : b);
+  unpack2(fma2(add2(pack2(s[0], s[1]), minus_m), sc, pack2(0.f, 0.f)), a, b);
+  a = exp2_unit(a);
+  b = exp2_unit(b);
   sum = add2(sum, pack2(a, b));
   *w = round_bf16(a, b);
 }
 
-// P = 2^(s scale + neg) of 64 scores as bf16 in 32 TMEM columns; returns the sum, and in `seen` a NaN if there is one
-// among the scores that took the polynomial.  POLY: eight of the 32 pairs do.  `before_last` is called when a quarter
-// is left.
-template <bool POLY, typename Hook>
-SD_DEV float row_probabilities(const float* s, float scale, float neg, uint32_t ta, float& seen, Hook before_last) {
+// P = 2^((s - m) scale) of 64 scores as bf16 in 32 TMEM columns; returns the sum, and in `seen` a NaN if there is one
+// among the scores that took the polynomial.  USUAL: as s scale - m scale, eight of the 32 pairs by the polynomial.
+// `before_last` is called when a quarter is left.
+template <bool USUAL, typename Hook>
+SD_DEV float row_probabilities(const float* s, float scale, float m, uint32_t ta, float& seen, Hook before_last) {
+  const float neg = USUAL ? -m * scale : -m;
   const uint64_t sc = pack2(scale, scale), ng = pack2(neg, neg);
   const float zs = scale * (1.f / kPolySpan), zn = (neg - kPolyLow) * (1.f / kPolySpan);
   uint64_t sum[2] = {0, 0};
@@ -653,7 +660,7 @@ SD_DEV float row_probabilities(const float* s, float scale, float neg, uint32_t 
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     if (q == 3) before_last();
-    if (POLY) {
+    if (USUAL) {
       eight_pairs(s + 16 * q, sc, ng, zs, zn, sum, seen, w + 8 * q);
     } else {
 #pragma unroll
@@ -727,8 +734,10 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     have_items = make_plan(p, smem, s_plan, s_range, s_items);
     fence_proxy_async();  // its generic writes are over before the copies into the same memory begin
   } else if (tid == 0) {
-    s_range[0] = p.cta_first[blockIdx.x];
-    s_range[1] = p.cta_last[blockIdx.x];
+    const bool same = *p.plan_key == p.key;
+    if (!same && blockIdx.x == 0) raise_status(p.status, SPECDEC_STATUS_PLAN_MISMATCH);
+    s_range[0] = same ? p.cta_first[blockIdx.x] : 0;
+    s_range[1] = same ? p.cta_last[blockIdx.x] : -1;
   }
   __syncthreads();
   const int i0 = s_range[0], i1 = s_range[1];
@@ -868,21 +877,21 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             return max3_nan(max3_nan(mx[0], mx[1], x[60]), max3_nan(mx[2], mx[3], x[61]), max_nan(x[62], x[63]));
           };
           if (k == 0) m = row_max();
-          float neg = m == -INFINITY ? 0.f : -m * scale, seen;
+          float seen;
           auto next = [&]() {
             if (AHEAD && more) load(other);
           };
-          float sum = row_probabilities<true>(x, scale, neg, s_ta + 64 * H, seen, next);
+          float sum = row_probabilities<true>(x, scale, m == -INFINITY ? 0.f : m, s_ta + 64 * H, seen, next);
           // Past the reference by more than 2^60 (or no reference yet, every key so far being masked): the
-          // reference becomes this half block's maximum, O and l are rescaled and it is done again, once.  Infinite
-          // and NaN scores and references go through the exponential unit, which knows them; a NaN stays one.
+          // reference takes in this half block's maximum, O and l are rescaled and it is done again, once.  So it is
+          // for NaN and infinite scores, and where the reference is so large that the roundings of m scale and of the
+          // polynomial's argument (3 2^-24 of it) would show beside P's own.  A NaN stays one.
           // (Rows of the tile that are no token's hold anything; rows that see nothing here add nothing.)
-          const bool redo = limit > key0 && (!(sum < kGrow) || seen != seen || !(fabsf(m) < INFINITY));
+          const bool redo = limit > key0 && (!(sum < kGrow) || seen != seen || !(fabsf(m) * scale < kLargeScore));
           if (__any_sync(0xffffffffu, redo)) {
-            const float bm = row_max();
-            const bool move = redo && m < INFINITY && bm != m;
-            const float alpha = move ? fast_exp2(((m == -INFINITY ? bm : m) - bm) * scale) : 1.f;
-            if (move) m = bm;
+            const float to = redo ? max_nan(m, row_max()) : m;
+            const float alpha = to == m ? 1.f : fast_exp2((m - to) * scale);  // (no reference yet: 0 of nothing)
+            m = to;
             l *= alpha;
             if (k > 0) {
               lazy_wait(&pv_done[t], (pv - 1) & 1, dead);  // the MMAs over the half before this add to O
@@ -897,8 +906,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
                 umma::tmem_st16(o_ta + c, o);
               }
             }
-            neg = m == -INFINITY ? 0.f : -m * scale;
-            sum = row_probabilities<false>(x, scale, neg, s_ta + 64 * H, seen, []() {});
+            sum = row_probabilities<false>(x, scale, m == -INFINITY ? 0.f : m, s_ta + 64 * H, seen, []() {});
           }
           l += sum;
           umma::tmem_wait_st();
@@ -1418,7 +1426,7 @@ __global__ void __launch_bounds__(256) join_cut_kernel(const RowParams p) {
   grid_dep_wait();
   grid_dep_launch();
   const int c = blockIdx.x, u = p.cut_unit[c];
-  if (u < 0) return;
+  if (u < 0 || *p.plan_key != p.key) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int2 info = p.unit_info[u];
   const RowItem it = load_item(p.items + u + c);
@@ -1447,7 +1455,9 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const RowParams p) {
   const int hp = static_cast<int>(w - bi * (p.KV * pairs)), kvh = hp / pairs;
   const int rep = (hp - kvh * pairs) * 2 + (lane & 1);
   const int b = static_cast<int>(bi / p.q_max), i = static_cast<int>(bi - static_cast<int64_t>(b) * p.q_max);
-  if (b >= p.B || i >= p.valid_len[b]) return;
+  if (b >= p.B || *p.plan_key != p.key) return;
+  const int2 rows = p.seq_rows[b];
+  if (i >= rows.y) return;
   auto pieces = [&](int part, int vt, int cap) {
     const int2 info = p.unit_info[p.part_units[part] + vt / (2 * p.tpt) * p.KV + kvh];
     const int in = vt % (2 * p.tpt), t = in / p.tpt;
@@ -1460,7 +1470,7 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const RowParams p) {
   else if (own.n == 1)
     return;  // written already
   join_pair<D>(p, pre, own,
-               rep < p.n_rep ? p.out + static_cast<int64_t>(p.q_row0[b] + i) * p.o_st +
+               rep < p.n_rep ? p.out + static_cast<int64_t>(rows.x + i) * p.o_st +
                                    static_cast<int64_t>(kvh * p.n_rep + rep) * p.o_sh
                              : nullptr,
                lane);
@@ -1471,7 +1481,8 @@ struct RowShape {
   int B, H, KV, D, q_max, G, M, sms;
 };
 struct RowSpace {
-  size_t first, last, cut, units, valid, group, vt, prefix, mrow, info, items, ml, o, bytes;
+  int64_t units_most;
+  size_t key, first, last, cut, units, valid, group, vt, prefix, mrow, info, items, ml, o, bytes;
   int cap_seq, cap_group;
   int64_t group_rows, rows;
 };
@@ -1491,6 +1502,7 @@ static RowSpace row_space(const RowShape& s) {
   auto cap = [&](int64_t tokens) {
     return static_cast<int>(tokens <= tpt ? up(tokens * n_rep, 32) * 32 : kUnitRows);
   };
+  w.units_most = seq_units + group_units;
   w.cap_seq = cap(s.q_max);
   w.cap_group = s.G > 0 ? cap(static_cast<int64_t>(s.M) * s.q_max) : 0;
   w.group_rows = s.G > 0 ? (group_units + s.sms) * w.cap_group : 0;
@@ -1502,11 +1514,12 @@ static RowSpace row_space(const RowShape& s) {
     at = align_up(at + n, 256);
     return o;
   };
+  w.key = take(8);
   w.first = take(4 * s.sms);
   w.last = take(4 * s.sms);
   w.cut = take(4 * s.sms);
   w.units = take(4 * (s.G + s.B + 1));
-  w.valid = take(4 * s.B);
+  w.valid = take(8 * s.B);
   w.group = take(4 * s.B);
   w.vt = take(4 * s.B);
   w.prefix = take(4 * (s.G + 1));
@@ -1536,7 +1549,8 @@ static int check_shape(const RowShape& s) {
     return fail(SPECDEC_ERR_UNSUPPORTED, "at most %d sequences, groups or members a call", kPlanMost);
   // item and slot numbers are 32-bit
   const RowSpace w = row_space(s);
-  if (w.rows > 0x7fffffff || static_cast<int64_t>(s.M) * s.q_max > (1 << 30) || w.bytes > (size_t(1) << 40))
+  if (w.rows > 0x7fffffff || w.units_most > (1 << 30) || s.q_max > (1 << 30) ||
+      static_cast<int64_t>(s.M) * s.q_max > (1 << 30) || w.bytes > (size_t(1) << 40))
     return fail(SPECDEC_ERR_UNSUPPORTED, "batch of %d sequences x %d tokens is too large for one call", s.B, s.q_max);
   return SPECDEC_OK;
 }
@@ -1576,7 +1590,8 @@ static int fill_row_params(RowParams& p, const RowShape& s, void* ws, size_t ws_
   p.cta_last = reinterpret_cast<int32_t*>(base + w.last);
   p.cut_unit = reinterpret_cast<int32_t*>(base + w.cut);
   p.part_units = reinterpret_cast<int32_t*>(base + w.units);
-  p.valid_len = reinterpret_cast<int32_t*>(base + w.valid);
+  p.plan_key = reinterpret_cast<uint64_t*>(base + w.key);
+  p.seq_rows = reinterpret_cast<int2*>(base + w.valid);
   p.seq_group = reinterpret_cast<int32_t*>(base + w.group);
   p.seq_vt = reinterpret_cast<int32_t*>(base + w.vt);
   p.prefix = reinterpret_cast<int32_t*>(base + w.prefix);
@@ -1593,6 +1608,12 @@ static int launch_row_attention(RowParams& p, const CUtensorMap& qmap, const CUt
                                 const CUtensorMap& vmap,
                                 bool reuse_plan, cudaStream_t st) {
   p.plan = reuse_plan ? 0 : 1;
+  p.key = 14695981039346656037ull;  // FNV-1a over what a plan's rows, keys and places in the workspace depend on
+  for (const int64_t x : {static_cast<int64_t>(D), static_cast<int64_t>(SRC), static_cast<int64_t>(p.B),
+                          static_cast<int64_t>(p.H), static_cast<int64_t>(p.KV), static_cast<int64_t>(p.q_max),
+                          static_cast<int64_t>(p.G), static_cast<int64_t>(p.M), static_cast<int64_t>(p.grid), p.q_rows,
+                          p.kv_rows, static_cast<int64_t>(p.num_pages), static_cast<int64_t>(p.max_pages)})
+    for (int b = 0; b < 64; b += 8) p.key = (p.key ^ ((x >> b) & 255)) * 1099511628211ull;
   // the attribute belongs to the function on each device; setting it again is cheap and needs no state of its own
   const cudaError_t e = cudaFuncSetAttribute(row_attention_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              RowGeom<D, RowRoles<SRC>::V8>::SMEM);
@@ -1707,7 +1728,7 @@ extern "C" int specdec_shared_prefix_attention(const SpecdecSharedPrefixArgs* a,
   if (v8 && !kv.v_scale) return fail(SPECDEC_ERR_INVALID, "E4M3 V needs v_scale");
   if (a->q_rows <= 0 || a->q_rows > 0x7fffffff) return fail(SPECDEC_ERR_INVALID, "row counts out of range");
   const int64_t page_rows = static_cast<int64_t>(kv.num_pages) * s.KV * (s.D / 64);
-  if (page_rows > 0x7fffffff || static_cast<int64_t>(kv.max_pages_per_seq) * kPage > 0x7fffffff)
+  if (page_rows > 0x7fffffff || static_cast<int64_t>(kv.max_pages_per_seq) * kPage > (1 << 30))
     return fail(SPECDEC_ERR_UNSUPPORTED, "page pool too large");
   RowParams p = {};
   if (int rc = fill_row_params(p, s, a->workspace, a->workspace_bytes, a->sm_scale)) return rc;

@@ -8,8 +8,11 @@ C ABI -- so ``backend`` must be ``"cuda"``; any other value raises
 
 Beyond the reference's four ops this module exposes the paged decode path:
 ``paged_attention``, ``ragged_plan``, ``append_kv``, ``greedy_accept`` and
-``trim_lengths``; and the 8-bit linear path: ``rmsnorm_int8``, ``quantize_int8``,
-``swiglu_int8``, ``linear_int8`` and ``dequantize_int8``.
+``trim_lengths``; packed prompts and shared first pages: ``prompt_attention`` and
+``shared_prefix_attention``; pages between sequences: ``copy_pages``,
+``fork_sequences``, ``reserve_pages``, ``free_sequences`` and ``compact_pages``; and the
+8-bit linear path: ``rmsnorm_int8``, ``quantize_int8``, ``swiglu_int8``, ``linear_int8``
+and ``dequantize_int8``.
 """
 
 from __future__ import annotations
@@ -560,16 +563,20 @@ def _call(t: torch.Tensor):
 
 
 def _head_rows(t: torch.Tensor, what: str, D: int | None = None):
-    """(rows, heads, head_dim) of packed bf16 rows with contiguous 16-byte aligned heads."""
+    """(rows, heads, head_dim, row stride, head stride) of packed bf16 rows with contiguous 16-byte aligned heads."""
     if t.dtype is not torch.bfloat16 or t.dim() != 3:
         raise ValueError(f"{what} must be bf16 (rows, heads, head_dim)")
     rows, heads, dim = t.shape
     if D is not None and dim != D:
         raise ValueError(f"{what} must share q's head_dim")
     st, sh, sd = t.stride()
-    if sd != 1 or st % 8 or sh % 8 or st < 0 or sh < 0 or t.data_ptr() & 15:
+    if heads == 1:  # (a stride that is never taken may be anything)
+        sh = dim
+    if rows <= 1:
+        st = heads * dim
+    if sd != 1 or st % 8 or sh % 8 or st <= 0 or sh <= 0 or t.data_ptr() & 15:
         raise ValueError(f"{what} heads must be contiguous and start on 16-byte boundaries")
-    return rows, heads, dim
+    return rows, heads, dim, st, sh
 
 
 def _batch_struct(batch: "RaggedBatch", heads: int, dev: int):
@@ -589,13 +596,14 @@ def _check_i32(t, dev: int, n: int, what: str) -> None:
 
 
 def _row_out(q, out, dev: int):
+    """out (checked or new) and its strides"""
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return out, q.shape[1] * q.shape[2], q.shape[2]
     _on_device(dev, out)
     if out.shape != q.shape:
         raise ValueError("out must have q's shape")
-    _head_rows(out, "out")
-    return out
+    return (out, *_head_rows(out, "out")[3:])
 
 
 def _check_status(status, dev: int) -> None:
@@ -638,13 +646,13 @@ def prompt_attention(q, k, v, batch: RaggedBatch, *, kv_row0=None, out=None, wor
     output.  Rows that belong to no sequence are left as they were.
     ``reuse_plan``: ``workspace`` holds the plan of an earlier call with the same batch (the layers of one pass)."""
     lib, dev, stream = _call(q)
-    rows, H, D = _head_rows(q, "q")
-    kv_rows, KV, _ = _head_rows(k, "k", D)
+    rows, H, D, q_st, q_sh = _head_rows(q, "q")
+    kv_rows, KV, _, k_st, k_sh = _head_rows(k, "k", D)
     if v.shape != k.shape:
         raise ValueError("k and v must have one shape")
-    _head_rows(v, "v", D)
+    v_st, v_sh = _head_rows(v, "v", D)[3:]
     _on_device(dev, k, v)
-    out = _row_out(q, out, dev)
+    out, o_st, o_sh = _row_out(q, out, dev)
     if kv_row0 is None:
         kv_row0 = batch.q_row0
     b = _batch_struct(batch, H, dev)
@@ -654,10 +662,9 @@ def prompt_attention(q, k, v, batch: RaggedBatch, *, kv_row0=None, out=None, wor
         return out
     nbytes = lib.specdec_prompt_workspace_bytes(batch.num_seqs, H, KV, D, batch.max_q_len, 0)
     workspace = _row_workspace(workspace, nbytes, q, dev, reuse_plan)
-    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
     args = _lib.PromptArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0],
-        os[1], b, kv_row0.data_ptr(), rows, kv_rows, KV, D,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, b,
+        kv_row0.data_ptr(), rows, kv_rows, KV, D,
         1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), workspace.data_ptr(), workspace.numel(),
         _ptr(status), 1 if reuse_plan else 0, 0)
     rc = lib.specdec_prompt_attention(ctypes.byref(args), stream)
@@ -716,10 +723,10 @@ def shared_prefix_attention(q, cache: PagedKVCache, layer: int, batch: RaggedBat
     group's first member that has rows.  ``reuse_plan``: ``workspace`` holds the plan of an earlier call with the same
     batch and prefix (the layers of one step)."""
     lib, dev, stream = _call(q)
-    rows, H, D = _head_rows(q, "q")
+    rows, H, D, q_st, q_sh = _head_rows(q, "q")
     if D != cache.head_dim:
         raise ValueError("q head_dim differs from the cache")
-    out = _row_out(q, out, dev)
+    out, o_st, o_sh = _row_out(q, out, dev)
     _on_device(dev, cache.page_table)
     b = _batch_struct(batch, H, dev)
     if batch.num_seqs > cache.num_seqs:
@@ -733,9 +740,8 @@ def shared_prefix_attention(q, cache: PagedKVCache, layer: int, batch: RaggedBat
     nbytes = lib.specdec_shared_prefix_workspace_bytes(batch.num_seqs, H, cache.num_kv_heads, D, batch.max_q_len,
                                                        prefix.num_groups, prefix.num_members, 0)
     workspace = _row_workspace(workspace, nbytes, q, dev, reuse_plan)
-    qs, os = q.stride(), out.stride()
     args = _lib.SharedPrefixArgs(
-        q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], b, _paged_kv(cache, layer),
+        q.data_ptr(), out.data_ptr(), q_st, q_sh, o_st, o_sh, b, _paged_kv(cache, layer),
         prefix.group_start.data_ptr(), prefix.members.data_ptr(), prefix.prefix_len.data_ptr(), prefix.num_groups,
         prefix.num_members, rows, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), workspace.data_ptr(),
         workspace.numel(), _ptr(status), 1 if reuse_plan else 0, 0)
