@@ -44,9 +44,8 @@ constexpr int kKeyBlock = 128;     // keys of a block
 constexpr int kUnitCost = 2;       // what a unit costs beside its blocks (query load, epilogue), in blocks
 constexpr int kMinQuota = 4;       // smallest range of a CTA, in blocks
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
-constexpr float kGrow = 1.152921504606846976e18f;  // 2^60: a block's sum past it moves the row's reference
+constexpr float kGrow = 1073741824.f;  // 2^30: a half block's sum past it moves the row's reference
 constexpr float kLargeScore = 4096.f;  // in units of log2
-constexpr int kItemsKept = 12;     // items of a CTA that it keeps in shared memory
 constexpr float kExpC1 = 0.693282962f, kExpC2 = 0.242210999f, kExpC3 = 0.0550089143f;
 
 enum RowSource { kPacked = 0, kPaged = 1, kPagedE4M3 = 2 };
@@ -58,6 +57,7 @@ template <int SRC>
 struct RowRoles {
   static constexpr bool V8 = SRC == kPagedE4M3;
   static constexpr int THREADS = 32 * (kSoftmaxWarps + 4 + (V8 ? 4 : 0));
+  static constexpr int ITEMS = V8 ? 4 : 12;  // items of a CTA that it keeps in shared memory (E4M3 has less room)
   static constexpr int SOFTMAX_REGS = V8 ? 176 : 208, OTHER_REGS = V8 ? 80 : 88;
   static_assert(32 * kSoftmaxWarps * SOFTMAX_REGS + (THREADS - 32 * kSoftmaxWarps) * OTHER_REGS <= THREADS * (V8 ? 128 : 168),
                 "register shares");
@@ -187,7 +187,8 @@ SD_DEV int64_t plan_scan(int64_t v, int64_t& all, int64_t (*tot)[32], int& turn)
 }
 
 // All threads of the CTA; `at`: PlanSpace::bytes() of shared memory.  range[0 .. 1] (shared): numbers of this CTA's first
-// and last item; kept[i % kItemsKept] holds them where that is all of them (returns whether).
+// and last item; kept[i % ITEMS] holds them where that is all of them (returns whether).
+template <int ITEMS>
 SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* range, RowItem* kept) {
   const PlanSpace w(at, p.B, p.G);
   const int tid = threadIdx.x, nthr = blockDim.x;
@@ -344,7 +345,7 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
       quota = max((static_cast<int>(total) + p.grid - 1) / p.grid, p.min_quota);
       from = blockIdx.x * quota;
       to = min(from + quota, total);
-      direct_items = quota <= (1 + kUnitCost) * (kItemsKept - 2);
+      direct_items = quota <= (1 + kUnitCost) * (ITEMS - 2);
     }
     if (row >= rows || total == 0 || us0 >= to || us0 + static_cast<int64_t>(cost) * p.KV <= from) continue;
     auto cta_of = [&](int64_t x) { return static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(quota)); };
@@ -387,7 +388,7 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
       it.k1 = min(f.k0 + e * kKeyBlock, end);
       it.slot = direct ? -1 : static_cast<int>(row0 + static_cast<int64_t>(p.compact && step > 0 ? 2 * step - 1 : step) * cap);
       p.items[u + c] = it;
-      if (direct_items) kept[(u + c) % kItemsKept] = it;
+      if (direct_items) kept[(u + c) % ITEMS] = it;
       if (from >= us) range[0] = p.cta_first[c] = u + c;
       if (to <= ue) range[1] = p.cta_last[c] = u + c;
     }
@@ -414,7 +415,7 @@ struct RowGeom {
   static constexpr int STAGE = 2048;
   static constexpr int SMEM = STAGED + kSoftmaxWarps * STAGE + 1024;
   static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
-  static_assert(PlanSpace::bytes(kPlanMost, kPlanMost) <= SMEM - 1024, "a plan fits");
+  static_assert(PlanSpace::bytes(kPlanMost, kPlanMost) <= STAGED, "a plan fits");
   static_assert(SMEM <= 227 * 1024 - 2048, "shared memory budget, 2 KB of static variables aside");
 };
 
@@ -434,6 +435,16 @@ SD_DEV int first_washed(const RowItem& it) { return max(first_hidden(it) - it.k0
 SD_DEV uint32_t not_finite(uint32_t w) {
   const uint32_t hi = ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
   return (hi >> 15) * 0xffffu;
+}
+
+// Two E4M3 codes, each in the upper byte of a half, as bf16: the bits moved to bf16's exponent and mantissa are the value
+// times 2^-120 (bf16's bias is 127, E4M3's 7; subnormals are subnormals in both), and the product with 2^120 is exact.
+// (The NaN codes come out as 480.)
+SD_DEV uint32_t e4m3_bf16(uint32_t x) {
+  const uint32_t v = (x & 0x80008000u) | ((x >> 4) & 0x07f007f0u);
+  uint32_t y;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(v), "r"(0x7b807b80u));
+  return y;
 }
 
 // half blocks (64 keys) of row tile t of an item
@@ -530,6 +541,11 @@ SD_DEV uint64_t add2(uint64_t a, uint64_t b) {
   asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+SD_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm volatile("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 SD_DEV float fma_sat(float a, float b, float c) {  // clamped to [0, 1]
   float r;
   asm volatile("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -600,16 +616,30 @@ struct Poly2 {
 // Eight pairs of scores at once: six take the exponential unit (12 x 8.5 clocks a warp), two the polynomial, whose
 // steps lie between the others'.  A pair costs about 8 issue slots by the unit and 24 by the polynomial, so a quarter
 // of the pairs balances the two.  Probabilities as bf16 pairs in w[0 .. 7], their sums added to `sum`.
+template <bool V8>
 SD_DEV void eight_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, float zn, uint64_t (&sum)[2], float& seen,
-                        uint32_t* w) {
+                        const float* vs, uint32_t* w) {
   Poly2 p[2];
   float x[12], y[12], a, b;
+  // E4M3: the keys' scales, two a pair
+  ulonglong2 g[V8 ? 4 : 1];
+  if constexpr (V8) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) g[e] = reinterpret_cast<const ulonglong2*>(vs)[e];
+  }
+  auto weigh = [&](int e, float p0, float p1) {
+    uint64_t v = pack2(p0, p1);
+    sum[e & 1] = add2(sum[e & 1], v);
+    if constexpr (V8) {
+      v = mul2(v, e & 1 ? g[e >> 1].y : g[e >> 1].x);
+      unpack2(v, p0, p1);
+    }
+    w[e] = round_bf16(p0, p1);
+  };
 #define SD_X(E) unpack2(fma2(pack2(s[2 * (E)], s[2 * (E) + 1]), sc, ng), x[2 * (E)], x[2 * (E) + 1]);
 #define SD_Y(E) y[E] = exp2_unit(x[E]);
 #define SD_P(I, K) p[I].step<K>(s[12 + 2 * (I)], s[13 + 2 * (I)], zs, zn);
-#define SD_W(E)                                              \
-  sum[(E) & 1] = add2(sum[(E) & 1], pack2(y[2 * (E)], y[2 * (E) + 1])); \
-  w[E] = round_bf16(y[2 * (E)], y[2 * (E) + 1]);
+#define SD_W(E) weigh(E, y[2 * (E)], y[2 * (E) + 1]);
   SD_X(0) SD_Y(0) SD_P(0, 0)
   seen = max3_nan(seen, s[12], s[13]);
   SD_Y(1) SD_X(1) SD_P(1, 0)
@@ -624,12 +654,10 @@ SD_DEV void eight_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, floa
   SD_Y(9) SD_W(3) SD_P(0, 6) SD_P(1, 6)
   SD_Y(10)
   p[0].result(a, b);
-  sum[0] = add2(sum[0], pack2(a, b));
-  w[6] = round_bf16(a, b);
+  weigh(6, a, b);
   SD_Y(11)
   p[1].result(a, b);
-  sum[1] = add2(sum[1], pack2(a, b));
-  w[7] = round_bf16(a, b);
+  weigh(7, a, b);
   SD_W(4) SD_W(5)
 #undef SD_X
 #undef SD_Y
@@ -637,20 +665,24 @@ SD_DEV void eight_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, floa
 #undef SD_W
 }
 // The rare way: exact where the scores are large, whatever they are (infinities and NaNs too).
-SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t minus_m, uint64_t& sum, uint32_t* w) {
+template <bool V8>
+SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t minus_m, uint64_t& sum, const float* vs, uint32_t* w) {
   float a, b;
   unpack2(fma2(add2(pack2(s[0], s[1]), minus_m), sc, pack2(0.f, 0.f)), a, b);
   a = exp2_unit(a);
   b = exp2_unit(b);
   sum = add2(sum, pack2(a, b));
+  if (V8) a *= vs[0], b *= vs[1];
   *w = round_bf16(a, b);
 }
 
 // P = 2^((s - m) scale) of 64 scores as bf16 in 32 TMEM columns; returns the sum, and in `seen` a NaN if there is one
 // among the scores that took the polynomial.  USUAL: as s scale - m scale, eight of the 32 pairs by the polynomial.
+// V8: each P is rounded after a multiplication by its key's scale (the codes themselves are exact in bf16).
 // `before_last` is called when a quarter is left.
-template <bool USUAL, typename Hook>
-SD_DEV float row_probabilities(const float* s, float scale, float m, uint32_t ta, float& seen, Hook before_last) {
+template <bool USUAL, bool V8, typename Hook>
+SD_DEV float row_probabilities(const float* s, float scale, float m, uint32_t ta, float& seen, const float* vs,
+                               Hook before_last) {
   const float neg = USUAL ? -m * scale : -m;
   const uint64_t sc = pack2(scale, scale), ng = pack2(neg, neg);
   const float zs = scale * (1.f / kPolySpan), zn = (neg - kPolyLow) * (1.f / kPolySpan);
@@ -661,10 +693,10 @@ SD_DEV float row_probabilities(const float* s, float scale, float m, uint32_t ta
   for (int q = 0; q < 4; ++q) {
     if (q == 3) before_last();
     if (USUAL) {
-      eight_pairs(s + 16 * q, sc, ng, zs, zn, sum, seen, w + 8 * q);
+      eight_pairs<V8>(s + 16 * q, sc, ng, zs, zn, sum, seen, vs + 16 * q, w + 8 * q);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) one_pair(s + 16 * q + 2 * e, sc, ng, sum[e & 1], w + 8 * q + e);
+      for (int e = 0; e < 8; ++e) one_pair<V8>(s + 16 * q + 2 * e, sc, ng, sum[e & 1], vs + 16 * q + 2 * e, w + 8 * q + e);
     }
     if (q == 1) umma::tmem_st16_words(ta, reinterpret_cast<const uint32_t(&)[16]>(w[0]));
   }
@@ -680,7 +712,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   constexpr bool V8 = RowRoles<SRC>::V8;
   using Geo = RowGeom<D, V8>;
-  constexpr int NS = Geo::NS, KH = Geo::KH;
+  constexpr int NS = Geo::NS, KH = Geo::KH, ITEMS = RowRoles<SRC>::ITEMS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[NS], empty[NS], raw_full, raw_empty;
@@ -688,9 +720,9 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   // [tile][its item % 2]: keys past first_hidden whose V holds an infinity or a NaN.  A tile's items here are those in
   // which it has work and some row does not see all keys: only those are waited for by both sides.
   __shared__ uint32_t s_bad[2][2][4][8];  // (a washing warp its own eight words)
-  __shared__ RowItem s_items[kItemsKept];  // the CTA's first items
-  __shared__ int64_t s_plan[2][32];
+  __shared__ RowItem s_items[ITEMS];  // the CTA's first items
   __shared__ int s_range[2];
+  __shared__ alignas(16) float s_vs[V8 ? 2 : 1][kKeyBlock];  // E4M3: scales of the keys in V's ring slots
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -731,7 +763,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   grid_dep_launch();
   bool have_items = false;
   if (p.plan) {
-    have_items = make_plan(p, smem, s_plan, s_range, s_items);
+    have_items = make_plan<ITEMS>(p, smem, reinterpret_cast<int64_t(*)[32]>(smem + Geo::STAGED), s_range, s_items);
     fence_proxy_async();  // its generic writes are over before the copies into the same memory begin
   } else if (tid == 0) {
     const bool same = *p.plan_key == p.key;
@@ -742,13 +774,13 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   __syncthreads();
   const int i0 = s_range[0], i1 = s_range[1];
   if (!have_items)
-    for (int e = tid; e < 3 * min(i1 - i0 + 1, kItemsKept); e += blockDim.x)
-      reinterpret_cast<int4*>(s_items + (i0 + e / 3) % kItemsKept)[e % 3] = reinterpret_cast<const int4*>(p.items + i0)[e];
+    for (int e = tid; e < 3 * min(i1 - i0 + 1, ITEMS); e += blockDim.x)
+      reinterpret_cast<int4*>(s_items + (i0 + e / 3) % ITEMS)[e % 3] = reinterpret_cast<const int4*>(p.items + i0)[e];
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = s_tmem;
-  auto item_at = [&](int i) { return i - i0 < kItemsKept ? s_items[i % kItemsKept] : load_item(p.items + i); };
+  auto item_at = [&](int i) { return i - i0 < ITEMS ? s_items[i % ITEMS] : load_item(p.items + i); };
 
   if (warp >= kSoftmaxWarp && warp < kWidenWarp) {
     more_regs<RowRoles<SRC>::SOFTMAX_REGS>();
@@ -878,11 +910,17 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           };
           if (k == 0) m = row_max();
           float seen;
+          const float* vs = nullptr;
+          if constexpr (V8) {  // the block's scales are there when its codes are widened
+            const int b = blk0 + k / 2;
+            vs = s_vs[b & 1] + 64 * H;
+            if (H == 0) lazy_wait(&full[(b & 1) * 2 + 1], (b >> 1) & 1, dead);
+          }
           auto next = [&]() {
             if (AHEAD && more) load(other);
           };
-          float sum = row_probabilities<true>(x, scale, m == -INFINITY ? 0.f : m, s_ta + 64 * H, seen, next);
-          // Past the reference by more than 2^60 (or no reference yet, every key so far being masked): the
+          float sum = row_probabilities<true, V8>(x, scale, m == -INFINITY ? 0.f : m, s_ta + 64 * H, seen, vs, next);
+          // Past the reference by more than 2^30 (or no reference yet, every key so far being masked): the
           // reference takes in this half block's maximum, O and l are rescaled and it is done again, once.  So it is
           // for NaN and infinite scores, and where the reference is so large that the roundings of m scale and of the
           // polynomial's argument (3 2^-24 of it) would show beside P's own.  A NaN stays one.
@@ -906,7 +944,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
                 umma::tmem_st16(o_ta + c, o);
               }
             }
-            sum = row_probabilities<false>(x, scale, m == -INFINITY ? 0.f : m, s_ta + 64 * H, seen, []() {});
+            sum = row_probabilities<false, V8>(x, scale, m == -INFINITY ? 0.f : m, s_ta + 64 * H, seen, vs, []() {});
           }
           l += sum;
           umma::tmem_wait_st();
@@ -1012,7 +1050,6 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
                 } else {
                   const uint32_t h = e4m3x2_to_f16x2(p.v_pool[at * (kPage * D) + key % kPage * D + d]);
                   v = __half2float(__ushort_as_half(static_cast<unsigned short>(h & 0xffffu))) * vs;
-                  v = __bfloat162float(__float2bfloat16(v));
                 }
                 if (fabsf(v) < INFINITY) continue;
                 if (it.slot >= 0) {
@@ -1299,7 +1336,6 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             const float sc = next;
             const int key = it.k0 + j * kKeyBlock + r;
             const bool in = key < it.k1;
-            uint32_t bad = 0;
             if (j + 1 < nb) next = scale_of(j + 1);
             const uint32_t s = n % NS;
             ok = row_wait(&raw_full, (n >> 1) & 1);
@@ -1307,6 +1343,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             if (!ok) break;
             const uint8_t* src = smem + Geo::RAW + r * 128;
             uint8_t* dst = smem + Geo::RING + s * Geo::TILE + r * 128;
+            uint32_t nan = 0;
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
               const int ch = (c + r) & 7;  // rotated, so that neighbouring keys use different banks
@@ -1314,28 +1351,30 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
               const uint32_t w[4] = {x.x, x.y, x.z, x.w};
               uint32_t y[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const uint32_t h = e4m3x2_to_f16x2(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                y[e] = in ? pack_bf16(f.x * sc, f.y * sc) : 0u;
-              }
-              if (key >= hidden) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const uint32_t b = not_finite(y[e]);
-                  bad |= b;
-                  y[e] &= ~b;
-                }
+              for (int e = 0; e < 4; ++e) {
+                nan |= (w[e] & 0x7f7f7f7fu) + 0x01010101u;
+                y[2 * e] = in ? e4m3_bf16(__byte_perm(w[e], 0, 0x1404)) : 0u;
+                y[2 * e + 1] = in ? e4m3_bf16(__byte_perm(w[e], 0, 0x3424)) : 0u;
               }
               uint8_t* d = dst + (ch >> 2) * 16384;
               const int g = (ch & 3) * 2;
               *reinterpret_cast<uint4*>(d + ((g ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
               *reinterpret_cast<uint4*>(d + (((g + 1) ^ (r & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
             }
-            if (bad) {
+            const bool strange = in && ((nan & 0x80808080u) || !(fabsf(sc) < INFINITY));
+            // a key that some row does not see adds nothing that is not finite here
+            s_vs[s >> 1][r] = strange && key >= hidden && !(fabsf(sc) < INFINITY) ? 0.f : sc;
+            if (strange) {
+#pragma unroll 1
+              for (int d = 0; d < D; ++d)
+                if ((src[d] & 0x7f) == 0x7f)
+                  *reinterpret_cast<uint16_t*>(dst + (d >> 6) * 16384 + ((((d >> 3) & 7) ^ (r & 7)) << 4) + (d & 7) * 2) =
+                      key >= hidden ? 0 : 0x7fff;
+              if (key >= hidden) {
 #pragma unroll
-              for (int t = 0; t < 2; ++t)
-                if (reads[t]) atomicOr(&s_bad[t][rd[t] & 1][r >> 5][(key - hidden) >> 5], 1u << ((key - hidden) & 31));
+                for (int t = 0; t < 2; ++t)
+                  if (reads[t]) atomicOr(&s_bad[t][rd[t] & 1][r >> 5][(key - hidden) >> 5], 1u << ((key - hidden) & 31));
+              }
             }
             fence_proxy_async();
             __syncwarp();

@@ -1,7 +1,8 @@
 """Plain 64-bit attention of packed rows and of pages, and the tolerance of the tests that compare with it.
 
 For output o = sum_j p_j v_j with A = sum_j p_j |v_j| and S the row's largest sum of |q k| products in units of log2:
-  2^-8 A    P rounded to bf16 before the product with V, half a step of each weight (the sum l is not rounded)
+  2^-8 A    P (E4M3: P times its key's scale) rounded to bf16 before the product with V, half a step of each weight
+            (the sum l is not rounded)
   2^-12 A   the exponentials' relative error (below 2^-13), once in the weights and once in their sum
   2^-16 S A a score is D <= 128 products added in fp32, each addition off by at most 2^-23 of the largest partial sum:
             128 2^-23 S = 2^-16 S in the exponent, times ln 2 for the weight, once in the weights and once in the sum
@@ -148,7 +149,7 @@ class Pages:
         d = self.cache.gather_layer(layer, b, length)
         k, v = d["k"][0].transpose(0, 1), d["v"][0].transpose(0, 1)
         if self.v8:
-            v = (v.float() * d["v_scale"][0].transpose(0, 1)).to(torch.bfloat16)
+            v = v.double() * d["v_scale"][0].transpose(0, 1).double()
         return k, v
 
 

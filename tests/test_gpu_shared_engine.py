@@ -139,8 +139,8 @@ def test_operators_together(v8, D, H):
         row0 = [sum(new[:b]) for b in range(B)]
         ops.append_kv(k, v, c, 0, row0=i32(row0), n_new=i32(new), pos0=i32(lens), max_new=max(new), status=status)
         codes, scale = ofp8.quantize_v(v.float().cpu().transpose(0, 1).numpy()) if v8 else (None, None)
-        kept = (torch.from_numpy(ofp8.dequantize_v(codes, scale)).to(torch.bfloat16).transpose(0, 1).cuda()
-                if v8 else v)
+        # (float32: a product of a code and a scale has 4 + 24 bits, rounded by 2^-24 of it)
+        kept = torch.from_numpy(ofp8.dequantize_v(codes, scale)).float().transpose(0, 1).cuda() if v8 else v
         for b in range(B):
             at = slice(row0[b], row0[b] + new[b])
             plain[b] = (torch.cat([plain[b][0], k[at]]), torch.cat([plain[b][1], kept[at]]))

@@ -1,5 +1,5 @@
 """GPU: attention over cache pages that groups of sequences share, against a plain 64-bit form over each sequence's own
-page table (tolerance: rows_helpers; E4M3 V as the bf16 values that dequantising the cache gives)."""
+page table (tolerance: rows_helpers; E4M3 V as the unrounded products of codes and scales)."""
 
 from __future__ import annotations
 
