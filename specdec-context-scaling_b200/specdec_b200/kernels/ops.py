@@ -18,13 +18,17 @@ and ``dequantize_int8``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+import struct
 from dataclasses import dataclass
 
 import torch
 
 from .. import _lib
 from ..engine.paged_cache import PagedKVCache
+
+_BF16, _F32, _I8, _I32 = torch.bfloat16, torch.float32, torch.int8, torch.int32
 
 
 def triton_available() -> bool:
@@ -563,44 +567,59 @@ def _call(t: torch.Tensor):
     return _int8_call(t)
 
 
-def _head_rows(t: torch.Tensor, what: str, D: int | None = None):
-    """(rows, heads, head_dim, row stride, head stride) of packed bf16 rows with contiguous 16-byte aligned heads."""
-    if t.dtype is not torch.bfloat16 or t.dim() != 3:
+# These calls, too, may take less time on the GPU than a careless check takes here: every attribute is read once, and the
+# C structs are packed at once instead of field by field.
+def _head_rows(t: torch.Tensor, what: str, D: int = 0):
+    """(rows, heads, head_dim, row stride, head stride, address) of packed bf16 rows with contiguous 16-byte aligned
+    heads."""
+    shape = t.shape
+    if t.dtype is not _BF16 or len(shape) != 3:
         raise ValueError(f"{what} must be bf16 (rows, heads, head_dim)")
-    rows, heads, dim = t.shape
-    if D is not None and dim != D:
-        raise ValueError(f"{what} must share q's head_dim")
+    rows, heads, dim = shape
     st, sh, sd = t.stride()
+    at = t.data_ptr()
     if heads == 1:  # (a stride that is never taken may be anything)
         sh = dim
     if rows <= 1:
         st = heads * dim
-    if sd != 1 or st % 8 or sh % 8 or st <= 0 or sh <= 0 or t.data_ptr() & 15:
+    if sd != 1 or (st | sh) & 7 or st <= 0 or sh <= 0 or at & 15:
         raise ValueError(f"{what} heads must be contiguous and start on 16-byte boundaries")
-    return rows, heads, dim, st, sh
+    if D and dim != D:
+        raise ValueError(f"{what} must share q's head_dim")
+    return rows, heads, dim, st, sh, at
 
 
-def _batch_struct(batch: "RaggedBatch", heads: int, dev: int):
-    """The C batch after a check of its arrays; rows that a call would read on the host stay unchecked."""
-    n = batch.num_seqs
-    for name in ("q_row0", "q_len", "ctx_len"):
-        _check_i32(getattr(batch, name), dev, n, name)
-    return _lib.Batch(q_row0=batch.q_row0.data_ptr(), q_len=batch.q_len.data_ptr(), ctx_len=batch.ctx_len.data_ptr(),
-                      num_seqs=n, num_q_heads=heads, max_q_len=batch.max_q_len, max_ctx_len=batch.max_ctx_len)
+def _batch_fields(batch: "RaggedBatch", heads: int, dev: int):
+    """The fields of the C batch after a check of its arrays; rows that a call would read on the host stay unchecked."""
+    n, q_row0, q_len, ctx_len = batch.num_seqs, batch.q_row0, batch.q_len, batch.ctx_len
+    _check_i32(q_row0, dev, n, "q_row0")
+    _check_i32(q_len, dev, n, "q_len")
+    _check_i32(ctx_len, dev, n, "ctx_len")
+    return (q_row0.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), n, heads, batch.max_q_len, batch.max_ctx_len)
+
+
+_PROMPT_ARGS = struct.Struct("4Q8q3Q4iQqqiif4xQQQii")
+_SHARED_ARGS = struct.Struct("2Q4q3Q4i4Q5i4x3Qiiqf4xQQQii")
+
+
+@functools.lru_cache(maxsize=256)
+def _row_bytes(lib, name: str, dev: int, *shape) -> int:
+    return getattr(lib, name)(*shape, 0)
 
 
 def _check_i32(t, dev: int, n: int, what: str) -> None:
     if t.get_device() != dev:
         raise RuntimeError("tensors must be CUDA, all on one device")
-    if t.dtype is not torch.int32 or t.numel() < n or not t.is_contiguous():
+    if t.dtype is not _I32 or t.numel() < n or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous int32 ({n},)")
 
 
 def _row_out(q, out, dev: int):
-    """out (checked or new) and its strides"""
+    """out (checked or new), its strides and address"""
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        return out, q.shape[1] * q.shape[2], q.shape[2]
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        _, heads, dim = q.shape
+        return out, heads * dim, dim, out.data_ptr()
     _on_device(dev, out)
     if out.shape != q.shape:
         raise ValueError("out must have q's shape")
@@ -647,27 +666,26 @@ def prompt_attention(q, k, v, batch: RaggedBatch, *, kv_row0=None, out=None, wor
     output.  Rows that belong to no sequence are left as they were.
     ``reuse_plan``: ``workspace`` holds the plan of an earlier call with the same batch (the layers of one pass)."""
     lib, dev, stream = _call(q)
-    rows, H, D, q_st, q_sh = _head_rows(q, "q")
-    kv_rows, KV, _, k_st, k_sh = _head_rows(k, "k", D)
-    if v.shape != k.shape:
+    rows, H, D, q_st, q_sh, q_at = _head_rows(q, "q")
+    kv_rows, KV, _, k_st, k_sh, k_at = _head_rows(k, "k", D)
+    v_rows, v_heads, _, v_st, v_sh, v_at = _head_rows(v, "v", D)
+    if v_rows != kv_rows or v_heads != KV:
         raise ValueError("k and v must have one shape")
-    v_st, v_sh = _head_rows(v, "v", D)[3:]
     _on_device(dev, k, v)
-    out, o_st, o_sh = _row_out(q, out, dev)
+    out, o_st, o_sh, o_at = _row_out(q, out, dev)
     if kv_row0 is None:
         kv_row0 = batch.q_row0
-    b = _batch_struct(batch, H, dev)
+    b = _batch_fields(batch, H, dev)
     _check_i32(kv_row0, dev, batch.num_seqs, "kv_row0")
     _check_status(status, dev)
     if rows == 0 or batch.num_seqs == 0:
         return out
-    nbytes = lib.specdec_prompt_workspace_bytes(batch.num_seqs, H, KV, D, batch.max_q_len, 0)
+    nbytes = _row_bytes(lib, "specdec_prompt_workspace_bytes", dev, batch.num_seqs, H, KV, D, batch.max_q_len)
     workspace = _row_workspace(workspace, nbytes, q, dev, reuse_plan)
-    args = _lib.PromptArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, b,
-        kv_row0.data_ptr(), rows, kv_rows, KV, D,
-        1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), workspace.data_ptr(), workspace.numel(),
-        _ptr(status), 1 if reuse_plan else 0, 0)
+    args = _lib.PromptArgs.from_buffer_copy(_PROMPT_ARGS.pack(
+        q_at, k_at, v_at, o_at, q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, *b, kv_row0.data_ptr(), rows, kv_rows, KV,
+        D, D ** -0.5 if sm_scale is None else float(sm_scale), workspace.data_ptr(), workspace.numel(),
+        0 if status is None else status.data_ptr(), 1 if reuse_plan else 0, 0))
     rc = lib.specdec_prompt_attention(ctypes.byref(args), stream)
     if rc:
         _lib.check(rc, "prompt_attention")
@@ -724,12 +742,13 @@ def shared_prefix_attention(q, cache: PagedKVCache, layer: int, batch: RaggedBat
     group's first member that has rows.  ``reuse_plan``: ``workspace`` holds the plan of an earlier call with the same
     batch and prefix (the layers of one step)."""
     lib, dev, stream = _call(q)
-    rows, H, D, q_st, q_sh = _head_rows(q, "q")
+    rows, H, D, q_st, q_sh, q_at = _head_rows(q, "q")
     if D != cache.head_dim:
         raise ValueError("q head_dim differs from the cache")
-    out, o_st, o_sh = _row_out(q, out, dev)
-    _on_device(dev, cache.page_table)
-    b = _batch_struct(batch, H, dev)
+    out, o_st, o_sh, o_at = _row_out(q, out, dev)
+    pool, table = cache.pools[layer], cache.page_table
+    _on_device(dev, table, pool.k)
+    b = _batch_fields(batch, H, dev)
     if batch.num_seqs > cache.num_seqs:
         raise ValueError("the batch has more sequences than the cache")
     _check_i32(prefix.group_start, dev, prefix.num_groups + 1, "group_start")
@@ -738,14 +757,17 @@ def shared_prefix_attention(q, cache: PagedKVCache, layer: int, batch: RaggedBat
     _check_status(status, dev)
     if rows == 0 or batch.num_seqs == 0:
         return out
-    nbytes = lib.specdec_shared_prefix_workspace_bytes(batch.num_seqs, H, cache.num_kv_heads, D, batch.max_q_len,
-                                                       prefix.num_groups, prefix.num_members, 0)
+    KV, e4m3 = cache.num_kv_heads, pool.v_scale is not None
+    nbytes = _row_bytes(lib, "specdec_shared_prefix_workspace_bytes", dev, batch.num_seqs, H, KV, D, batch.max_q_len,
+                        prefix.num_groups, prefix.num_members)
     workspace = _row_workspace(workspace, nbytes, q, dev, reuse_plan)
-    args = _lib.SharedPrefixArgs(
-        q.data_ptr(), out.data_ptr(), q_st, q_sh, o_st, o_sh, b, _paged_kv(cache, layer),
-        prefix.group_start.data_ptr(), prefix.members.data_ptr(), prefix.prefix_len.data_ptr(), prefix.num_groups,
-        prefix.num_members, rows, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), workspace.data_ptr(),
-        workspace.numel(), _ptr(status), 1 if reuse_plan else 0, 0)
+    args = _lib.SharedPrefixArgs.from_buffer_copy(_SHARED_ARGS.pack(
+        q_at, o_at, q_st, q_sh, o_st, o_sh, *b, pool.k.data_ptr(), pool.v.data_ptr(),
+        pool.v_scale.data_ptr() if e4m3 else 0, table.data_ptr(), cache.num_pages, KV, D,
+        _lib.E4M3 if e4m3 else _lib.BF16, cache.max_pages, prefix.group_start.data_ptr(), prefix.members.data_ptr(),
+        prefix.prefix_len.data_ptr(), prefix.num_groups, prefix.num_members, rows,
+        D ** -0.5 if sm_scale is None else float(sm_scale), workspace.data_ptr(), workspace.numel(),
+        0 if status is None else status.data_ptr(), 1 if reuse_plan else 0, 0))
     rc = lib.specdec_shared_prefix_attention(ctypes.byref(args), stream)
     if rc:
         _lib.check(rc, "shared_prefix_attention")
@@ -759,13 +781,13 @@ def _page_pool(cache: PagedKVCache):
     pools, n = cache.pools, cache.num_layers
     if pools[0].k.get_device() != dev:
         raise RuntimeError("tensors must be CUDA, all on one device")
-    array = ctypes.c_void_p * n
-    keep = [array(*[p.k.data_ptr() for p in pools]), array(*[p.v.data_ptr() for p in pools])]
     e4m3 = cache.v_dtype == "e4m3"
+    at = [p.k.data_ptr() for p in pools] + [p.v.data_ptr() for p in pools]
     if e4m3:
-        keep.append(array(*[p.v_scale.data_ptr() for p in pools]))
-    pool = _lib.PagePool(ctypes.addressof(keep[0]), ctypes.addressof(keep[1]),
-                         ctypes.addressof(keep[2]) if e4m3 else None, n, cache.num_pages, cache.num_kv_heads,
+        at += [p.v_scale.data_ptr() for p in pools]
+    keep = (ctypes.c_void_p * len(at))(*at)
+    first = ctypes.addressof(keep)
+    pool = _lib.PagePool(first, first + 8 * n, first + 16 * n if e4m3 else None, n, cache.num_pages, cache.num_kv_heads,
                          cache.head_dim, _lib.E4M3 if e4m3 else _lib.BF16)
     return lib, dev, stream, (pool, keep)
 
@@ -861,7 +883,6 @@ def compact_pages(cache: PagedKVCache, *, workspace=None, status=None) -> torch.
 # ---------------------------------------------------------------------------- 8-bit linear path
 # These calls take a few microseconds of GPU time each in a decode step, so their checks read every
 # attribute once and the library and stream are looked up directly.
-_BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
 _int8_lib = None
 
 

@@ -346,7 +346,7 @@ def test_few_sms(sms):
     ws = torch.empty(n, dtype=torch.uint8, device="cuda")
     out, status = torch.full_like(q, FILL), torch.zeros(1, dtype=torch.int32, device="cuda")
     args = _lib.SharedPrefixArgs(q.data_ptr(), out.data_ptr(), H * D, D, H * D, D,
-                                 ops._batch_struct(batch, H, q.get_device()), ops._paged_kv(pages.cache, 0),
+                                 _lib.Batch(*ops._batch_fields(batch, H, q.get_device())), ops._paged_kv(pages.cache, 0),
                                  p.group_start.data_ptr(), p.members.data_ptr(), p.prefix_len.data_ptr(), 1, 3, q.shape[0],
                                  1 / math.sqrt(D), ws.data_ptr(), n, status.data_ptr(), 0, sms)
     _lib.check(lib.specdec_shared_prefix_attention(ctypes.byref(args), torch.cuda.current_stream().cuda_stream), "shared")

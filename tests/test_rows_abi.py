@@ -266,11 +266,11 @@ def test_row_shapes():
     from specdec_b200.kernels import ops
 
     x = torch.zeros(6, 4, 64, dtype=torch.bfloat16)
-    assert ops._head_rows(x, "x") == (6, 4, 64, 256, 64)
-    assert ops._head_rows(x.transpose(0, 1), "x") == (4, 6, 64, 64, 256)
+    assert ops._head_rows(x, "x") == (6, 4, 64, 256, 64, x.data_ptr())
+    assert ops._head_rows(x.transpose(0, 1), "x")[:5] == (4, 6, 64, 64, 256)
     # strides that are never taken: one row, one head
-    assert ops._head_rows(x[:, :1].as_strided((6, 1, 64), (256, 3, 1)), "x") == (6, 1, 64, 256, 64)
-    assert ops._head_rows(x.as_strided((1, 4, 64), (5, 64, 1)), "x") == (1, 4, 64, 256, 64)
+    assert ops._head_rows(x[:, :1].as_strided((6, 1, 64), (256, 3, 1)), "x")[:5] == (6, 1, 64, 256, 64)
+    assert ops._head_rows(x.as_strided((1, 4, 64), (5, 64, 1)), "x")[:5] == (1, 4, 64, 256, 64)
     bad = [x.float(), x[0], x[..., ::2], x[..., 4:], x.as_strided((6, 4, 64), (0, 64, 1)),
            x.as_strided((5, 4, 64), (260, 64, 1)), x.as_strided((6, 4, 64), (256, 0, 1))]
     for t in bad:
