@@ -78,6 +78,17 @@ struct alignas(16) RowItem {
 };
 static_assert(sizeof(RowItem) == 48, "three 16-byte loads");
 
+// What the join needs of a unit that a CTA boundary cuts / of a sequence, in as few loads as can be.
+struct alignas(16) CutUnit {
+  int32_t slot, pieces;             // pieces 0: none is cut here
+  int32_t row0, vt0, n_vt, head, pad[2];
+};
+struct alignas(16) SeqRows {
+  int32_t row0, len;                // first query row, valid tokens
+  int32_t own, pre;                 // first unit of its own part and of its group's (-1: no group, or no prefix)
+  int32_t vt, pad[3];               // its first token in the group's part
+};
+
 struct RowParams {
   const __nv_bfloat16* q;
   __nv_bfloat16* out;
@@ -99,12 +110,10 @@ struct RowParams {
   uint64_t key;                 // of this launch shape
   int32_t* status;
   // workspace
-  int32_t *cta_first, *cta_last, *cut_unit;     // [grid]
-  int32_t* part_units;                          // [G + B] starts
+  int32_t *cta_first, *cta_last;                // [grid]
+  CutUnit* cut_unit;                            // [grid]
   uint64_t* plan_key;                           // the launch shape that the plan is for
-  int2* seq_rows;                               // [B] {first query row, valid tokens}
-  int32_t *seq_group, *seq_vt;                  // [B]
-  int32_t* prefix;                              // [G]
+  SeqRows* seq_rows;                            // [B]
   int2* member_row;                             // [M] {first query row, tokens}
   int2* unit_info;                              // [units] {first slot row, pieces}
   RowItem* items;                               // [units + grid]
@@ -195,7 +204,7 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
   const bool writes = blockIdx.x == 0;  // what the join and later calls read of the whole batch
   int turn = 0;
   if (tid < 2) range[tid] = -tid;  // 0, -1: no items
-  if (tid == 2) p.cut_unit[blockIdx.x] = -1;
+  if (tid == 2) p.cut_unit[blockIdx.x].pieces = 0;
   if (tid == 3 && writes) *p.plan_key = p.key;
   // the first loads of everything, under way together
   const int member = tid < p.M ? p.members[tid] : 0;
@@ -273,7 +282,6 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
       const int n = i == 0x7fffffff ? 0 : w.prefix[g] / kPage * kPage;  // whole pages
       w.prefix[g] = n;
       w.table[g] = i == 0x7fffffff ? 0 : p.members[i];
-      if (writes) p.prefix[g] = n;
     }
   }
   __syncthreads();
@@ -286,22 +294,22 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
     if (part < parts) n = (part_info(p, w, part).n_vt + 2 * p.tpt - 1) / (2 * p.tpt);
     int64_t all;
     const int at_row = rows + static_cast<int>(plan_scan(n, all, tot, turn));
-    if (part < parts) {
-      w.rows[part] = at_row;
-      if (writes) {
-        p.part_units[part] = at_row * p.KV;
-        if (part >= p.G) {
-          const int b = part - p.G;
-          p.seq_rows[b] = make_int2(p.q_row0[b], w.len[b]);
-          p.seq_group[b] = w.group[b];
-          p.seq_vt[b] = w.group[b] >= 0 ? w.vt[b] : 0;
-        }
-      }
-    }
+    if (part < parts) w.rows[part] = at_row;
     rows += static_cast<int>(all);
   }
   if (tid == 0) w.rows[parts] = rows;
   __syncthreads();
+  if (writes)
+    for (int b = tid; b < p.B; b += nthr) {
+      const int g = w.group[b];
+      SeqRows r = {};
+      r.row0 = p.q_row0[b];
+      r.len = w.len[b];
+      r.own = w.rows[p.G + b] * p.KV;
+      r.pre = g >= 0 && w.prefix[g] > 0 ? w.rows[g] * p.KV : -1;
+      r.vt = g >= 0 ? w.vt[b] : 0;
+      p.seq_rows[b] = r;
+    }
   auto part_of = [&](int row) {  // the last part that starts at or before the row and has rows
     int lo = 0, hi = parts;
     while (hi - lo > 1) {
@@ -378,7 +386,7 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
       const bool direct = !f.group && f.k0 == 0 && pieces == 1;
       if (c == cb) {
         p.unit_info[u] = make_int2(static_cast<int>(row0), pieces);
-        if (pieces > 1) p.cut_unit[cb] = u;
+        if (pieces > 1) p.cut_unit[cb] = {static_cast<int>(row0), pieces, it.row0, it.vt0, it.n_vt, h, {}};
       }
       const int a = static_cast<int>(max(from - us - kUnitCost, static_cast<int64_t>(0)));
       const int e = static_cast<int>(min(to - us - kUnitCost, static_cast<int64_t>(nb)));
@@ -1401,6 +1409,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
 // ---------------------------------------------------------------- joining partial rows
 // One warp two rows that lie next to each other in their slots (a lane pair reads a whole sector): the pieces of up
 // to two units, each a run of slots.  A piece that saw no key of the row has sum 0 and maximum -inf and weighs nothing.
+// Bound by the latency of L2, so the loads of several pieces, sums and rows alike, are under way together.
 struct Pieces {
   int64_t row;  // workspace row of the first piece
   int n, cap;
@@ -1410,46 +1419,48 @@ struct Pieces {
 // Lane l: row l % 2 of the pair, columns 4 (l / 2) .. + 3, and 64 further.  `out` NULL: no such row.
 template <int D>
 SD_DEV void join_pair(const RowParams& p, const Pieces& a, const Pieces& b, __nv_bfloat16* out, int lane) {
-  constexpr int PER = D / 64;
+  constexpr int PER = D / 64, AT_ONCE = D == 64 ? 8 : 6;
   const int n = out ? a.n + b.n : 0, c = lane >> 1;
-  auto at = [&](int i) { return i < a.n ? a.at(i) : b.at(i - a.n); };
-  const int most = max(n, __shfl_xor_sync(0xffffffffu, n, 1));
-  float m = -INFINITY;
-  for (int i = c; i < n; i += 16) m = max_nan(m, p.part_ml[at(i)].x);
-#pragma unroll
-  for (int o = 16; o > 1; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float mu = m == -INFINITY ? 0.f : m;
   float4 acc[PER] = {};
-  float l = 0.f;
-  for (int base = 0; base < most; base += 16) {
-    const int i = base + c;
-    float w = 0.f;
-    int64_t r = 0;
-    if (i < n) {
-      r = at(i);
-      const float2 ml = p.part_ml[r];
-      w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : fast_exp2(ml.x - mu);
-      l += w * ml.y;
+  float m = -INFINITY, l = 0.f;
+  for (int base = 0; base < n; base += AT_ONCE) {
+    float2 ml[AT_ONCE];
+    float4 v[AT_ONCE][PER];
+#pragma unroll
+    for (int e = 0; e < AT_ONCE; ++e) {
+      const int i = base + e;
+      if (i >= n) {
+        ml[e] = make_float2(-INFINITY, 0.f);
+        continue;
+      }
+      const int64_t r = i < a.n ? a.at(i) : b.at(i - a.n);
+      ml[e] = p.part_ml[r];
+      const float4* from = p.part_o + (r >> 5) * (8 * D) + (r & 31);
+#pragma unroll
+      for (int x = 0; x < PER; ++x) v[e][x] = from[(c + 16 * x) * 32];
     }
-    const int k = min(16, most - base);
-#pragma unroll 4
-    for (int e = 0; e < k; ++e) {
-      const float we = __shfl_sync(0xffffffffu, w, 2 * e + (lane & 1));
-      const int64_t re = __shfl_sync(0xffffffffu, r, 2 * e + (lane & 1));
-      if (we == 0.f) continue;
-      const float4* from = p.part_o + (re >> 5) * (8 * D) + (re & 31);
+    float to = m;
+#pragma unroll
+    for (int e = 0; e < AT_ONCE; ++e) to = max_nan(to, ml[e].x);
+    const float mu = to == -INFINITY ? 0.f : to, keep = fast_exp2(m - mu);
+    m = to;
+    l *= keep;
+#pragma unroll
+    for (int x = 0; x < PER; ++x) acc[x].x *= keep, acc[x].y *= keep, acc[x].z *= keep, acc[x].w *= keep;
+#pragma unroll
+    for (int e = 0; e < AT_ONCE; ++e) {
+      const float w = ml[e].x == -INFINITY && ml[e].y == 0.f ? 0.f : fast_exp2(ml[e].x - mu);
+      if (w == 0.f) continue;  // (what such a piece's row holds may be anything)
+      l += w * ml[e].y;
 #pragma unroll
       for (int x = 0; x < PER; ++x) {
-        const float4 v = from[(c + 16 * x) * 32];
-        acc[x].x += we * v.x;
-        acc[x].y += we * v.y;
-        acc[x].z += we * v.z;
-        acc[x].w += we * v.w;
+        acc[x].x += w * v[e][x].x;
+        acc[x].y += w * v[e][x].y;
+        acc[x].z += w * v[e][x].z;
+        acc[x].w += w * v[e][x].w;
       }
     }
   }
-#pragma unroll
-  for (int o = 16; o > 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   if (out) {
 #pragma unroll
@@ -1464,20 +1475,20 @@ template <int D>
 __global__ void __launch_bounds__(256) join_cut_kernel(const RowParams p) {
   grid_dep_wait();
   grid_dep_launch();
-  const int c = blockIdx.x, u = p.cut_unit[c];
-  if (u < 0 || *p.plan_key != p.key) return;
+  const int4* from = reinterpret_cast<const int4*>(p.cut_unit + blockIdx.x);
+  const int4 x = from[0], y = from[1];
+  if (x.y == 0 || *p.plan_key != p.key) return;
+  const int slot = x.x, row0 = x.z, vt0 = x.w, n_vt = y.x, head = y.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int2 info = p.unit_info[u];
-  const RowItem it = load_item(p.items + u + c);
   for (int r2 = (blockIdx.y * 8 + warp) * 2; r2 < kUnitRows; r2 += gridDim.y * 16) {
     const int r = r2 + (lane & 1);
-    const int t = r / kRowTile, e = r % kRowTile, tok = e / p.n_rep, vt = it.vt0 + t * p.tpt + tok;
-    const bool in = tok < p.tpt && vt < it.n_vt;
+    const int t = r / kRowTile, e = r % kRowTile, tok = e / p.n_rep, vt = vt0 + t * p.tpt + tok;
+    const bool in = tok < p.tpt && vt < n_vt;
     if (!__any_sync(0xffffffffu, in)) continue;
-    const Pieces a{info.x + r, info.y, p.cap_seq, p.compact != 0}, none{0, 0, 0, false};
+    const Pieces a{slot + r, x.y, p.cap_seq, p.compact != 0}, none{0, 0, 0, false};
     join_pair<D>(p, a, none,
-                 in ? p.out + static_cast<int64_t>(it.row0 + vt) * p.o_st +
-                          static_cast<int64_t>(it.head * p.n_rep + e - tok * p.n_rep) * p.o_sh
+                 in ? p.out + static_cast<int64_t>(row0 + vt) * p.o_st +
+                          static_cast<int64_t>(head * p.n_rep + e - tok * p.n_rep) * p.o_sh
                     : nullptr,
                  lane);
   }
@@ -1494,22 +1505,23 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const RowParams p) {
   const int hp = static_cast<int>(w - bi * (p.KV * pairs)), kvh = hp / pairs;
   const int rep = (hp - kvh * pairs) * 2 + (lane & 1);
   const int b = static_cast<int>(bi / p.q_max), i = static_cast<int>(bi - static_cast<int64_t>(b) * p.q_max);
-  if (b >= p.B || *p.plan_key != p.key) return;
-  const int2 rows = p.seq_rows[b];
-  if (i >= rows.y) return;
-  auto pieces = [&](int part, int vt, int cap) {
-    const int2 info = p.unit_info[p.part_units[part] + vt / (2 * p.tpt) * p.KV + kvh];
+  if (b >= p.B) return;
+  const int4* from = reinterpret_cast<const int4*>(p.seq_rows + b);
+  const int4 rec = from[0];
+  const int first_vt = from[1].x;
+  if (*p.plan_key != p.key || i >= rec.y) return;
+  auto pieces = [&](int units, int vt, int cap) {
+    const int2 info = p.unit_info[units + vt / (2 * p.tpt) * p.KV + kvh];
     const int in = vt % (2 * p.tpt), t = in / p.tpt;
     return Pieces{info.x + t * kRowTile + (in - t * p.tpt) * p.n_rep + rep, info.y, cap, p.compact != 0};
   };
-  Pieces own = pieces(p.G + b, i, p.cap_seq), pre{0, 0, 0, false};
-  const int g = p.seq_group[b];
-  if (g >= 0 && p.prefix[g] > 0)
-    pre = pieces(g, p.seq_vt[b] + i, p.cap_group);
+  Pieces own = pieces(rec.z, i, p.cap_seq), pre{0, 0, 0, false};
+  if (rec.w >= 0)
+    pre = pieces(rec.w, first_vt + i, p.cap_group);
   else if (own.n == 1)
     return;  // written already
   join_pair<D>(p, pre, own,
-               rep < p.n_rep ? p.out + static_cast<int64_t>(rows.x + i) * p.o_st +
+               rep < p.n_rep ? p.out + static_cast<int64_t>(rec.x + i) * p.o_st +
                                    static_cast<int64_t>(kvh * p.n_rep + rep) * p.o_sh
                              : nullptr,
                lane);
@@ -1521,7 +1533,7 @@ struct RowShape {
 };
 struct RowSpace {
   int64_t units_most;
-  size_t key, first, last, cut, units, valid, group, vt, prefix, mrow, info, items, ml, o, bytes;
+  size_t key, first, last, cut, seqs, mrow, info, items, ml, o, bytes;
   int cap_seq, cap_group;
   int64_t group_rows, rows;
 };
@@ -1556,12 +1568,8 @@ static RowSpace row_space(const RowShape& s) {
   w.key = take(8);
   w.first = take(4 * s.sms);
   w.last = take(4 * s.sms);
-  w.cut = take(4 * s.sms);
-  w.units = take(4 * (s.G + s.B + 1));
-  w.valid = take(8 * s.B);
-  w.group = take(4 * s.B);
-  w.vt = take(4 * s.B);
-  w.prefix = take(4 * (s.G + 1));
+  w.cut = take(sizeof(CutUnit) * s.sms);
+  w.seqs = take(sizeof(SeqRows) * s.B);
   w.mrow = take(8 * (s.M + 1));
   w.info = take(8 * (seq_units + group_units));
   w.items = take(sizeof(RowItem) * (seq_units + group_units + s.sms));
@@ -1627,13 +1635,9 @@ static int fill_row_params(RowParams& p, const RowShape& s, void* ws, size_t ws_
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.cta_first = reinterpret_cast<int32_t*>(base + w.first);
   p.cta_last = reinterpret_cast<int32_t*>(base + w.last);
-  p.cut_unit = reinterpret_cast<int32_t*>(base + w.cut);
-  p.part_units = reinterpret_cast<int32_t*>(base + w.units);
+  p.cut_unit = reinterpret_cast<CutUnit*>(base + w.cut);
   p.plan_key = reinterpret_cast<uint64_t*>(base + w.key);
-  p.seq_rows = reinterpret_cast<int2*>(base + w.valid);
-  p.seq_group = reinterpret_cast<int32_t*>(base + w.group);
-  p.seq_vt = reinterpret_cast<int32_t*>(base + w.vt);
-  p.prefix = reinterpret_cast<int32_t*>(base + w.prefix);
+  p.seq_rows = reinterpret_cast<SeqRows*>(base + w.seqs);
   p.member_row = reinterpret_cast<int2*>(base + w.mrow);
   p.unit_info = reinterpret_cast<int2*>(base + w.info);
   p.items = reinterpret_cast<RowItem*>(base + w.items);
