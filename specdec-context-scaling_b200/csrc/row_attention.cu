@@ -10,25 +10,40 @@
 // their own with its rows only, and the results of both are joined.
 //
 // Work: parts (prefix groups, then sequences) are cut into units, a unit costs its 128-key blocks plus kUnitCost,
-// and the concatenated costs are cut into equal ranges, one a CTA (plan kernel, one CTA).  A unit that a boundary
-// cuts becomes several items, whose unnormalised rows, maxima and sums go to the workspace and are joined by
-// merge kernels; the others are written to the output at once.
+// and the concatenated costs are cut into equal ranges, one a CTA (make_plan, worked out by every CTA for itself).  A
+// unit that a boundary cuts becomes several items, whose unnormalised rows, maxima and sums go to the workspace and are
+// joined by a second kernel; the others are written to the output at once.
 //
-// One CTA an SM, 12 warps, each role walking the same items:
-//   warps 0-3, 4-7  softmax of row tile 0, 1: a thread owns a row, so maxima and sums need no exchange
-//   warp 8          K/V tiles by TMA into a ring (K 0, V 0, K 1, V 1, ...): packed rows as {64 dims, 128 rows} boxes,
+// One CTA an SM, 12 warps (E4M3 16), each role walking the same items:
+//   warp 0          K/V tiles by TMA into a ring (K 0, V 0, K 1, V 1): packed rows as {64 dims, 128 rows} boxes,
 //                   pages as four-row gathers; both give [dim half][128 keys][128 B] in the 128-byte swizzle
-//   warp 9          MMA issue (one lane), owner of the TMEM
-//   warp 10         query rows of the next item into shared memory, and each row's key limit
-//   warp 11         zeroes the V rows past an item's last key, so that a masked key's zero probability
-//                   never meets what lies behind a sequence (its next one, a page's old contents; NaN x 0)
-//   warps 12-15     (E4M3 V only) widen a block's codes, times their token's scale, to the bf16 block that the
-//                   MMAs read (the values that dequantising the cache gives), zeroes past the last key
-// Per block j and tile t:  S_t = Q_t K_j^T (TMEM, fp32) -> P_t = exp2(S_t - m) as bf16 over the same columns
-// -> O_t += P_t V_j (A operand from TMEM).  The two tiles alternate, so one's softmax runs under the other's MMAs.
-// The running maximum moves only when a row's grows by more than 2^8 (then O is rescaled in place); S_t(j) is complete
-// only after O_t(j - 1), both being issued in this order by one lane, so the rescale needs no wait of its own.
-// P is rounded to bf16 (2^-9 of each weight, independent between keys); sums, maxima and O stay fp32.
+//   warps 1, 2      MMA issue (one lane), one for each row tile
+//   warp 3          query rows of the next item, as boxes of n_rep heads x 128 / n_rep tokens (or one token, where a
+//                   group's rows do not follow one another)
+//   warps 4-7, 8-11 softmax and epilogue of row tile 0, 1: a thread owns a row, so maxima and sums need no exchange;
+//                   and the washing of V (below)
+//   warps 12-15     (E4M3 V) the block's codes to bf16 by moving bits; the keys' scales are multiplied into P
+// A block of 128 keys is two halves of 64, each with scores S_t[h] of its own in TMEM:
+//   S_t[h] = Q_t K^T  ->  P = 2^((S - m) scale) as bf16 over the same columns  ->  O_t += P V (A operand from TMEM)
+// Half h + 1's products and half h's softmax run at the same time, and so do the two tiles.
+//
+// The running maximum is a stale one: m is a row's maximum over its first half block and moves only when a half block's
+// sum passes 2^30 (2^x has the range for it), so that O is almost never rescaled.  P is rounded to bf16 (2^-8 of each weight
+// at most, independent between keys); sums, maxima, O and the joined rows stay fp32.  A quarter of the exponentials
+// are a cubic on the FMA units (relative error 1.0e-4), the rest the exponential unit's: 64 a thread and half would
+// take 544 clocks a warp there.
+//
+// What a masked key's zero probability meets in V must be finite.  The MMAs take none of the 16-key steps past an item's
+// last key, and what is left of the keys that some row does not see is washed in shared memory: an infinity or a NaN
+// becomes zero and its key is noted, and a row that does see it gets it added after the epilogue.
+//
+// Bound: the softmax warps.  A half block of both tiles takes about 1900 clocks, of which the tensor cores are busy for
+// 1290 (ncu: 53 % of the cycles; exponential unit 39 %; issue slots 42 %; DRAM 2 %): 1200 are exponentials, the rest
+// the way of the scores from TMEM and of P back.  Four prompts of 8192 tokens (12 heads over 2, 128 dims) take 810 to
+// 860 us, 960 to 1020 TFLOP/s (of 1632 measured); 16 of 1024 tokens 98 us (520); 64 x 5 rows over a shared 8192-token
+// prefix and 1024 tokens each 48 us against 78 us by paged_attention, which reads the prefix for every sequence.
+// What small calls cost: the plan 5 us (its code is fetched and run once; later layers reuse it), an item's start and
+// end 2 to 3 us (first block, epilogue), the join 3 us and up.
 #include <initializer_list>
 #include <type_traits>
 
@@ -124,8 +139,8 @@ struct RowParams {
 // ---------------------------------------------------------------- plan
 // Every CTA of the attention kernel works the plan out for itself before it starts, in the shared memory that its
 // blocks will take, and keeps its own items (they are written down, too: the workspace then serves the next layers,
-// and the join).  That is a round trip to L2, some barriers and two scans; a kernel of its own before this one took 5 to
-// 10 us.  A thread a sequence, member or unit row.
+// and the join).  That is a round trip to L2, some barriers and two scans, 3 to 6 us; a kernel of its own before this one
+// took 5 to 10.  A thread a sequence, member or unit row.
 constexpr int kPlanMost = 2048;  // sequences, members or groups of a call
 struct PlanSpace {
   int32_t *rows, *len, *first, *group, *vt, *listed, *prefix, *table, *flags;
@@ -416,10 +431,9 @@ struct RowGeom {
   static constexpr int TILE = 16384 * KH;         // one K or V block, one query tile
   // ring slots, a K or a V block each: K in 0 and 2, V in 1 and 3
   static constexpr int NS = 4;
-  static constexpr int NRAW = 1;                  // E4M3: blocks of codes
   static constexpr int RING = 2 * TILE;           // the ring lies behind the two query tiles
   static constexpr int RAW = RING + NS * TILE;
-  static constexpr int STAGED = RAW + (V8 ? NRAW * 16384 : 0);  // rows on their way out, STAGE bytes a softmax warp
+  static constexpr int STAGED = RAW + (V8 ? 16384 : 0);  // rows on their way out, STAGE bytes a softmax warp
   static constexpr int STAGE = 2048;
   static constexpr int SMEM = STAGED + kSoftmaxWarps * STAGE + 1024;
   static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
@@ -464,7 +478,8 @@ SD_DEV int tile_halves(const RowParams& p, const RowItem& it, int t) {
 }
 
 // Bounded waits of this kernel's warps, most of which wait most of the time: the hint lets the hardware put a warp
-// to sleep for up to a millisecond instead of having it poll beside the softmax warps.
+// to sleep for up to a millisecond instead of having it poll beside the softmax warps.  A wait that runs out (one second)
+// ends the CTA's work: its warps leave their loops, copies and products under way are waited for, the status says so.
 SD_DEV bool mbar_try_sleep(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -854,8 +869,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         }
       };
       // Washing: what a masked key's zero probability meets must be finite.  V rows past the last key (the next
-      // sequence's, a page's old contents) become zero; an infinity or a NaN in a key that only some rows see becomes
-      // zero, too, and its key is noted for the rows that do see it (add_bad_keys).  The tile that has work in every
+      // sequence's, a page's old contents) become zero as far as the products reach; an infinity or a NaN in a key that only some rows see becomes
+      // zero, too, and its key is noted for the rows that do see it (after the epilogue).  The tile that has work in every
       // block does it, a quarter of the rows a warp; the MMA warps wait for it.  (E4M3: the widening warps do.)
       const int wash = V8 || nh < nh_other || (nh == nh_other && t == 1) ? 0x7fffffff : first_washed(it);
       auto wash_block = [&](int j) {
