@@ -23,8 +23,9 @@ attention rows), accept treats it as inactive (m = 0, lengths kept), and nothing
 emitted for it, so its caches stop growing while slower sequences finish.
 
 With ``shared_prefix`` tokens the prompts begin alike (a system prompt): these are read once, by
-sequence 0, whose pages the others fork; what follows them is read by one step a chunk of sequences, and every
-step of a round reads the shared pages once (``ops.shared_prefix_attention``).
+sequence 0, whose pages the others fork; what follows them is read by one step a chunk of sequences.  In a large
+batch over a long prefix every step of a round, too, reads the shared pages once (``ops.shared_prefix_attention``);
+else ``ops.paged_attention`` reads them for each sequence, which is faster there.
 
 Every step of a round is a fixed-shape device computation (the ragged q_len of
 step 1 lives in device arrays), so a round is captured once in a CUDA graph and
@@ -45,7 +46,7 @@ from .paged_cache import PAGE
 class SpecDecEngine:
     def __init__(self, target: PagedModel, draft: PagedModel, num_seqs: int, prompt_len: int, max_new: int, *,
                  k: int = 4, target_v: str = "bf16", draft_v: str = "bf16", check_every: int = 4,
-                 shared_prefix: int = 0):
+                 shared_prefix: int = 0, share_reads: bool | None = None):
         if k < 1:
             raise ValueError("k must be >= 1")
         if target.cfg.vocab != draft.cfg.vocab:
@@ -68,14 +69,21 @@ class SpecDecEngine:
             full = shared_prefix // PAGE
             pages = dict(on_demand=True, num_pages=full + num_seqs * (-(-cap // PAGE) - full))
             self.prefix = ops.SharedPrefix.from_groups([(range(num_seqs), shared_prefix)], dev)
+        # One layer's attention, shared_prefix_attention against paged_attention (us; prefix + 512 tokens, 1 draft row
+        # and 5 target rows a sequence): 64 x 2048 22 against 21 and 29 against 33, 64 x 8192 27 against 41 and 43
+        # against 77; 64 x 1024 22 against 17 and 27 against 26, 256 x 1024 53 against 39 and 73 against 67, 16 x 8192
+        # 20 against 18 and 29 against 26.
+        if share_reads is None:
+            share_reads = num_seqs >= 64 and shared_prefix >= 2048
+        self.step_prefix = self.prefix if share_reads else None
         self.tc = target.new_cache(num_seqs, cap, target_v, **pages)
         self.dc = draft.new_cache(num_seqs, cap, draft_v, **pages)
         self.L0 = StepLayout(num_seqs, 2, dev)
         self.L1 = StepLayout(num_seqs, 1, dev)
         self.LV = StepLayout(num_seqs, k + 1, dev)
-        self.ws0 = self._workspace(self.L0, draft, self.dc)
-        self.ws1 = self._workspace(self.L1, draft, self.dc)
-        self.wsv = self._workspace(self.LV, target, self.tc)
+        self.ws0 = self._workspace(self.L0, draft, self.dc, self.step_prefix)
+        self.ws1 = self._workspace(self.L1, draft, self.dc, self.step_prefix)
+        self.wsv = self._workspace(self.LV, target, self.tc, self.step_prefix)
         i32 = dict(dtype=torch.int32, device=dev)
         self.pending = torch.zeros(num_seqs, **i32)
         self.catch = torch.zeros(num_seqs, **i32)     # 1: the draft has not read the last round's ck
@@ -102,9 +110,9 @@ class SpecDecEngine:
         self.idx = torch.arange(k + 1, device=dev, dtype=torch.int32)
         self.active = torch.ones(num_seqs, **i32)   # 0: the sequence has its max_new tokens
 
-    def _workspace(self, layout: StepLayout, model: PagedModel, cache) -> torch.Tensor:
-        if self.prefix is not None:
-            return ops.shared_prefix_workspace(layout.batch, self.prefix, model.cfg.heads, cache)
+    def _workspace(self, layout: StepLayout, model: PagedModel, cache, prefix) -> torch.Tensor:
+        if prefix is not None:
+            return ops.shared_prefix_workspace(layout.batch, prefix, model.cfg.heads, cache)
         return ops.attn_workspace(layout.batch, model.cfg.heads, cache)
 
     # ------------------------------------------------------------------ prompt
@@ -147,8 +155,9 @@ class SpecDecEngine:
                 n = min(chunk, self.B - s0)
                 piece = PieceLayout(self.B, s0, n, own, self.device)
                 piece.set(cache.lengths)
-                h = model.step(prompts[s0:s0 + n, n0:].reshape(-1), piece, cache, self._workspace(piece, model, cache),
-                               status=self.status, prefix=self.prefix)
+                ws = self._workspace(piece, model, cache, self.prefix)
+                h = model.step(prompts[s0:s0 + n, n0:].reshape(-1), piece, cache, ws, status=self.status,
+                               prefix=self.prefix)
                 if model is self.target:
                     self.pending[s0:s0 + n] = model.logits(h[piece.last_rows()]).argmax(-1).int()
                 cache.lengths.add_(piece.q_len)
@@ -164,18 +173,19 @@ class SpecDecEngine:
         first = torch.where(self.catch > 0, self.c_last, self.pending)
         tok0 = torch.stack([first, self.pending], dim=1).reshape(-1)
         self.L0.set(self.dc.lengths, q0)
-        h = draft.step(tok0, self.L0, self.dc, self.ws0, status=self.status, prefix=self.prefix)
+        h = draft.step(tok0, self.L0, self.dc, self.ws0, status=self.status, prefix=self.step_prefix)
         self.cands[:, 0] = draft.greedy(h[self.L0.last_rows()], self.dtok, self.lm_ws_d)
         self.dc.lengths.add_(q0)
         for i in range(1, k):
             self.L1.set(self.dc.lengths, act)
-            h = draft.step(self.cands[:, i - 1], self.L1, self.dc, self.ws1, status=self.status, prefix=self.prefix)
+            h = draft.step(self.cands[:, i - 1], self.L1, self.dc, self.ws1, status=self.status,
+                           prefix=self.step_prefix)
             self.cands[:, i] = draft.greedy(h, self.dtok, self.lm_ws_d)
             self.dc.lengths.add_(act)
         # 2. target verify of [pending, c1 .. ck]; g_j of every verify row (rows b (k+1) + j)
         vt = torch.cat([self.pending.unsqueeze(1), self.cands], dim=1).reshape(-1)
         self.LV.set(self.tc.lengths, act * (k + 1))
-        h = target.step(vt, self.LV, self.tc, self.wsv, status=self.status, prefix=self.prefix)
+        h = target.step(vt, self.LV, self.tc, self.wsv, status=self.status, prefix=self.step_prefix)
         target.greedy(h, self.g.view(-1), self.lm_ws_t)
         # 3. greedy accept from g (+ the target's rolled-back length len + 1 + m)
         ops.greedy_accept(None, row0=self.LV.q_row0, n_rows=self.LV.q_len, cands=self.cands, kp=self.kp,

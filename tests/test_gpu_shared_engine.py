@@ -51,8 +51,9 @@ def test_prompts_of_different_lengths():
 
 
 @pytest.mark.parametrize("target_v", ["bf16", "e4m3"])
-@pytest.mark.parametrize("shared,P", [(32, 48), (40, 48), (47, 48), (5, 20), (130, 131)])
-def test_shared_prompts_emit_the_same_tokens(target_v, shared, P):
+@pytest.mark.parametrize("share_reads", [True, None])
+@pytest.mark.parametrize("shared,P", [(32, 48), (40, 48), (47, 48), (5, 20), (1, 20), (130, 131)])
+def test_shared_prompts_emit_the_same_tokens(target_v, shared, P, share_reads):
     from specdec_b200.engine.model import PagedModel, random_state
     from specdec_b200.engine.specdec import SpecDecEngine
 
@@ -64,7 +65,8 @@ def test_shared_prompts_emit_the_same_tokens(target_v, shared, P):
         ref.set_kv_format("v_fp8")
     B, N = 5, 16
     prompts = _prompts(B, P, shared, tcfg.vocab, 7)
-    eng = SpecDecEngine(target, draft, B, P, N, k=4, target_v=target_v, shared_prefix=shared)
+    eng = SpecDecEngine(target, draft, B, P, N, k=4, target_v=target_v, shared_prefix=shared,
+                        share_reads=share_reads)
     eng.capture()
     for again in range(2):  # a second batch takes the first one's pages over
         eng.prefill(prompts, chunk=2)
@@ -89,7 +91,7 @@ def test_shared_engine_replay_equals_eager_rounds():
     prompts = _prompts(3, 40, 33, tcfg.vocab, 8)
     outs = []
     for use_graph in (True, False):
-        eng = SpecDecEngine(target, draft, 3, 40, 16, k=4, shared_prefix=33)
+        eng = SpecDecEngine(target, draft, 3, 40, 16, k=4, shared_prefix=33, share_reads=True)
         if use_graph:
             eng.capture()
         eng.prefill(prompts)
