@@ -362,7 +362,10 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
     if (base == 0) {
       if (rows <= nthr) total = all;
       if (total >= 0x7fffffff) {  // 2^31 blocks are half a minute of this device's tensor cores
-        if (writes && tid == 0) raise_status(p.status, SPECDEC_STATUS_BAD_LENGTH);
+        if (writes && tid == 0) {
+          raise_status(p.status, SPECDEC_STATUS_BAD_LENGTH);
+          *p.plan_key = ~p.key;  // nothing to join, and nothing to use again
+        }
         total = 0;
       }
       quota = max((static_cast<int>(total) + p.grid - 1) / p.grid, p.min_quota);
@@ -702,9 +705,10 @@ SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t minus_m, uint64_t& su
 // P = 2^((s - m) scale) of 64 scores as bf16 in 32 TMEM columns; returns the sum, and in `seen` a NaN if there is one
 // among the scores that took the polynomial.  USUAL: as s scale - m scale, eight of the 32 pairs by the polynomial.
 // V8: each P is rounded after a multiplication by its key's scale (the codes themselves are exact in bf16).
-// `before_last` is called when a quarter is left.
+// `before_last` is called when a quarter is left.  Not USUAL: what is there already stays for rows that are not `mine`,
+// so that no row's bits depend on what its neighbours' scores are.
 template <bool USUAL, bool V8, typename Hook>
-SD_DEV float row_probabilities(const float* s, float scale, float m, uint32_t ta, float& seen, const float* vs,
+SD_DEV float row_probabilities(const float* s, float scale, float m, uint32_t ta, float& seen, const float* vs, bool mine,
                                Hook before_last) {
   const float neg = USUAL ? -m * scale : -m;
   const uint64_t sc = pack2(scale, scale), ng = pack2(neg, neg);
@@ -712,6 +716,18 @@ SD_DEV float row_probabilities(const float* s, float scale, float m, uint32_t ta
   uint64_t sum[2] = {0, 0};
   uint32_t w[32];
   seen = -INFINITY;
+  auto store = [&](int at) {
+    if constexpr (!USUAL) {
+      float old[16];
+      umma::tmem_ld16(ta + at, old);
+      umma::tmem_wait_ld16(old);
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (!mine) w[at + e] = __float_as_uint(old[e]);
+    }
+    umma::tmem_st16_words(ta + at, reinterpret_cast<const uint32_t(&)[16]>(w[at]));
+  };
+  if (!USUAL) umma::tmem_wait_st();
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     if (q == 3) before_last();
@@ -721,9 +737,9 @@ SD_DEV float row_probabilities(const float* s, float scale, float m, uint32_t ta
 #pragma unroll
       for (int e = 0; e < 8; ++e) one_pair<V8>(s + 16 * q + 2 * e, sc, ng, sum[e & 1], vs + 16 * q + 2 * e, w + 8 * q + e);
     }
-    if (q == 1) umma::tmem_st16_words(ta, reinterpret_cast<const uint32_t(&)[16]>(w[0]));
+    if (q == 1) store(0);
   }
-  umma::tmem_st16_words(ta + 16, reinterpret_cast<const uint32_t(&)[16]>(w[16]));
+  store(16);
   float a, b;
   unpack2(add2(sum[0], sum[1]), a, b);
   return a + b;
@@ -948,7 +964,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           auto next = [&]() {
             if (AHEAD && more) load(std::integral_constant<int, AHEAD ? 1 - decltype(half)::value : 0>{});
           };
-          float sum = row_probabilities<true, V8>(x, scale, m == -INFINITY ? 0.f : m, s_ta + 64 * H, seen, vs, next);
+          float sum = row_probabilities<true, V8>(x, scale, m == -INFINITY ? 0.f : m, s_ta + 64 * H, seen, vs, true, next);
           // Past the reference by more than 2^30 (or no reference yet, every key so far being masked): the
           // reference takes in this half block's maximum, O and l are rescaled and it is done again, once.  So it is
           // for NaN and infinite scores, and where the reference is so large that the roundings of m scale and of the
@@ -973,7 +989,9 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
                 umma::tmem_st16(o_ta + c, o);
               }
             }
-            sum = row_probabilities<false, V8>(x, scale, m == -INFINITY ? 0.f : m, s_ta + 64 * H, seen, vs, []() {});
+            const float again = row_probabilities<false, V8>(x, scale, m == -INFINITY ? 0.f : m, s_ta + 64 * H, seen, vs,
+                                                             redo, []() {});
+            if (redo) sum = again;
           }
           l += sum;
           umma::tmem_wait_st();

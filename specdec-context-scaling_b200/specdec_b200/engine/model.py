@@ -353,8 +353,12 @@ class PagedModel:
         pos0 = torch.zeros(cache.num_seqs, **i32)
         x = self.embed[ids.reshape(-1).long()]
         cos, sin = self._cos_sin(torch.arange(P, device=dev).repeat(n))
-        batch = ops.RaggedBatch(torch.arange(n, **i32) * P, q_len, q_len, n, P, rows, P)
-        workspace = ops.prompt_workspace(batch, c.heads, c.kv_heads, c.head_dim, dev)
+        calls = []  # (rows, batch, workspace): a call takes ops.MOST_SEQUENCES prompts at most
+        for s0 in range(0, n, ops.MOST_SEQUENCES):
+            m = min(n - s0, ops.MOST_SEQUENCES)
+            batch = ops.RaggedBatch(torch.arange(m, **i32) * P, q_len[s0:s0 + m], q_len[s0:s0 + m], m, P, m * P, P)
+            calls.append((slice(s0 * P, (s0 + m) * P), batch,
+                          ops.prompt_workspace(batch, c.heads, c.kv_heads, c.head_dim, dev)))
         # padding rows are written by nobody and mixed into nothing: zero, so that they stay finite
         o = (torch.empty if lengths is None else torch.zeros)(rows, c.heads, c.head_dim, dtype=x.dtype, device=dev)
         delta = None
@@ -370,8 +374,10 @@ class PagedModel:
                 # scales), as the reference's V-only FP8 prompt pass attends over
                 # dequantize(quantize(v)) (model_self.py:702-704)
                 v = _e4m3_round_trip(v)
-            ops.prompt_attention(q[0].transpose(0, 1), k[0].transpose(0, 1), v.transpose(0, 1), batch, out=o,
-                                 workspace=workspace, status=status, reuse_plan=li > 0)
+            q, k, v = q[0].transpose(0, 1), k[0].transpose(0, 1), v.transpose(0, 1)
+            for at, batch, workspace in calls:
+                ops.prompt_attention(q[at], k[at], v[at], batch, out=o[at], workspace=workspace, status=status,
+                                     reuse_plan=li > 0)
             o2 = o.view(rows, c.heads * c.head_dim)
             if self.int8:
                 delta = self._mlp_int8(L, x, L.w_o(*ops.quantize_int8(o2), status), status)

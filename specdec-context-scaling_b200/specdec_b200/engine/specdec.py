@@ -61,7 +61,9 @@ class SpecDecEngine:
         cap = prompt_len + max_new + 2 * (k + 1) + 2
         if not 0 <= shared_prefix < prompt_len:
             raise ValueError(f"shared_prefix must be in 0 .. {prompt_len - 1}: every prompt has a token of its own")
-        self.shared, self.cap = shared_prefix, cap
+        if shared_prefix and num_seqs > ops.MOST_SEQUENCES:
+            raise ValueError(f"at most {ops.MOST_SEQUENCES} sequences share a prefix")
+        self.shared, self.cap, self.filled = shared_prefix, cap, False
         self.prefix = None
         pages = {}
         if shared_prefix:
@@ -125,6 +127,7 @@ class SpecDecEngine:
         self.status.zero_()
         if self.shared:
             self._prefill_shared(prompts, chunk)
+        self.filled = True
         for s0 in range(0, self.B if not self.shared else 0, chunk):
             ids = prompts[s0:s0 + chunk]
             lg = self.target.prefill(ids, self.tc, s0, status=self.status)
@@ -216,7 +219,7 @@ class SpecDecEngine:
         """Record one round as a CUDA graph (after one eager warm-up round).  Capturing
         before ``prefill`` keeps it out of the decode: prefill resets every length and
         counter the warm-up touched."""
-        if self.shared:  # no sequence holds pages yet: a round of frozen sequences writes none
+        if self.shared and not self.filled:  # no sequence holds pages yet: a round of frozen ones writes none
             self.n_out.fill_(self.max_new)
         self._round()
         torch.cuda.synchronize()

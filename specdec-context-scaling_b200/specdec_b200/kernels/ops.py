@@ -598,6 +598,7 @@ def _batch_fields(batch: "RaggedBatch", heads: int, dev: int):
     return (q_row0.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), n, heads, batch.max_q_len, batch.max_ctx_len)
 
 
+MOST_SEQUENCES = 2048  # sequences, groups or members of one call
 _PROMPT_ARGS = struct.Struct("4Q8q3Q4iQqqiif4xQQQii")
 _SHARED_ARGS = struct.Struct("2Q4q3Q4i4Q5i4x3Qiiqf4xQQQii")
 

@@ -274,6 +274,25 @@ def test_graph_with_changing_lengths_and_another_stream():
             assert torch.equal(out[r:r + n], beside[r:r + n])
 
 
+@pytest.mark.parametrize("H,KV,D", [(12, 2, 128), (14, 2, 64)])
+def test_a_strange_query_is_its_row_s_own(H, KV, D):
+    lens = [200, 70]
+    case = packed_case(lens, H, KV, D, 13)
+    want = _run(case, lens)
+    q = case[0].clone()
+    for r, h in ((0, 0), (77, 3), (128, H - 1), (230, 1)):
+        q[r, h, 5] = math.nan
+        q[r, (h + 1) % H, 9] = math.inf
+    got = _run((q, *case[1:]), lens)
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool)
+    for r, h in ((0, 0), (77, 3), (128, H - 1), (230, 1)):
+        hit[r, h] = hit[r, (h + 1) % H] = True
+    hit = hit.cuda()
+    assert torch.equal(got[~hit], want[~hit])
+    # the rows themselves: the formula's NaNs (a row whose only score is -inf has no weight at all and is zero)
+    check_packed(got, FILL, q, *case[1:5], lens, case[5])
+
+
 def test_same_bits_every_time():
     for D in (64, 128):
         lens = [700, 30, 1200]

@@ -100,6 +100,43 @@ def test_shared_engine_replay_equals_eager_rounds():
     assert torch.equal(*outs)
 
 
+def test_round_captured_after_the_prompts():
+    """A round recorded when the sequences hold their pages already runs as one of the decode."""
+    from specdec_b200.engine.model import PagedModel
+    from specdec_b200.engine.specdec import SpecDecEngine
+
+    tcfg, dcfg = _cfgs()
+    target, draft = PagedModel.random(tcfg, 31), PagedModel.random(dcfg, 32)
+    prompts = _prompts(3, 40, 33, tcfg.vocab, 8)
+    outs = []
+    for late in (False, True):
+        eng = SpecDecEngine(target, draft, 3, 40, 16, k=4, shared_prefix=33)
+        if not late:
+            eng.capture()
+        eng.prefill(prompts)
+        if late:
+            eng.capture()
+        eng.decode()
+        outs.append(eng.tokens().cpu())
+    assert torch.equal(*outs)
+
+
+def test_more_prompts_than_a_call_takes():
+    from specdec_b200.engine.model import ModelConfig, PagedModel
+
+    cfg = ModelConfig(vocab=100, hidden=128, heads=2, kv_heads=1, head_dim=64, intermediate=128, layers=2)
+    pm = PagedModel.random(cfg, 3)
+    n, P = 2500, 6
+    ids = _prompts(n, P, 0, cfg.vocab, 4)
+    lens = [1 + i % P for i in range(n)]
+    with torch.inference_mode():
+        cache = pm.new_cache(n, 16)
+        got = pm.prefill(ids, cache, 0, lengths=lens)
+        for s0 in (0, 1000, 2040, 2400):
+            one = pm.prefill(ids[s0:s0 + 100], pm.new_cache(100, 16), 0, lengths=lens[s0:s0 + 100])
+            _close(got[s0:s0 + 100], one, f"prompts {s0} ..", LOGIT_RTOL)
+
+
 def test_engine_refusals():
     from specdec_b200.engine.model import PagedModel
     from specdec_b200.engine.specdec import SpecDecEngine
@@ -109,6 +146,8 @@ def test_engine_refusals():
     for bad in (-1, 40, 41):
         with pytest.raises(ValueError):
             SpecDecEngine(target, draft, 3, 40, 16, shared_prefix=bad)
+    with pytest.raises(ValueError):
+        SpecDecEngine(target, draft, 2049, 40, 16, shared_prefix=33)
     eng = SpecDecEngine(target, draft, 3, 40, 16, shared_prefix=33)
     other = _prompts(3, 40, 33, tcfg.vocab, 1)
     other[2, 20] = (other[2, 20] + 1) % tcfg.vocab
