@@ -603,6 +603,15 @@ _PROMPT_ARGS = struct.Struct("4Q8q3Q4iQqqiif4xQQQii")
 _SHARED_ARGS = struct.Struct("2Q4q3Q4i4Q5i4x3Qiiqf4xQQQii")
 
 
+_PAGE_POOL = struct.Struct("3Q5i4x")
+_PAGE_TABLE = struct.Struct("3Q2i3Q")
+
+
+@functools.lru_cache(maxsize=256)
+def _page_bytes(lib, num_seqs: int, num_pages: int, requests: int) -> int:
+    return lib.specdec_page_workspace_bytes(num_seqs, num_pages, requests)
+
+
 @functools.lru_cache(maxsize=256)
 def _row_bytes(lib, name: str, dev: int, *shape) -> int:
     return getattr(lib, name)(*shape, 0)
@@ -780,7 +789,8 @@ def _page_pool(cache: PagedKVCache):
     """(library, device, stream, C pool and the pointer arrays it points to) of a call on all layers of ``cache``."""
     lib, dev, stream = _call(cache.page_table)
     pools, n = cache.pools, cache.num_layers
-    if pools[0].k.get_device() != dev:
+    k0 = pools[0].k
+    if k0.get_device() != dev:
         raise RuntimeError("tensors must be CUDA, all on one device")
     e4m3 = cache.v_dtype == "e4m3"
     at = [p.k.data_ptr() for p in pools] + [p.v.data_ptr() for p in pools]
@@ -788,8 +798,9 @@ def _page_pool(cache: PagedKVCache):
         at += [p.v_scale.data_ptr() for p in pools]
     keep = (ctypes.c_void_p * len(at))(*at)
     first = ctypes.addressof(keep)
-    pool = _lib.PagePool(first, first + 8 * n, first + 16 * n if e4m3 else None, n, cache.num_pages, cache.num_kv_heads,
-                         cache.head_dim, _lib.E4M3 if e4m3 else _lib.BF16)
+    pool = _lib.PagePool.from_buffer_copy(_PAGE_POOL.pack(
+        first, first + 8 * n, first + 16 * n if e4m3 else 0, n, k0.shape[0], cache.num_kv_heads, cache.head_dim,
+        _lib.E4M3 if e4m3 else _lib.BF16))
     return lib, dev, stream, (pool, keep)
 
 
@@ -797,12 +808,13 @@ def _page_table(cache: PagedKVCache, n: int, workspace, status, lib, dev: int):
     if cache.page_refs is None:
         raise ValueError("the cache's pages are static; allocate it with shared pages")
     _check_status(status, dev)
-    nbytes = lib.specdec_page_workspace_bytes(cache.num_seqs, cache.num_pages, n)
+    refs = cache.page_refs
+    nbytes = _page_bytes(lib, cache.num_seqs, refs.numel(), n)
     workspace = _row_workspace(workspace, nbytes, cache.page_table, dev, False)
     cache.host_lengths = None
-    return workspace, _lib.PageTable(cache.page_table.data_ptr(), cache.page_refs.data_ptr(),
-                                     cache.lengths.data_ptr(), cache.num_seqs, cache.max_pages, workspace.data_ptr(),
-                                     workspace.numel(), _ptr(status))
+    return workspace, _lib.PageTable.from_buffer_copy(_PAGE_TABLE.pack(
+        cache.page_table.data_ptr(), refs.data_ptr(), cache.lengths.data_ptr(), cache.num_seqs, cache.max_pages,
+        workspace.data_ptr(), workspace.numel(), 0 if status is None else status.data_ptr()))
 
 
 def page_workspace(cache: PagedKVCache, requests: int = 0) -> torch.Tensor:
@@ -818,7 +830,7 @@ def _requests(dev: int, *arrays) -> int:
     for t in arrays:
         if t.get_device() != dev:
             raise RuntimeError("tensors must be CUDA, all on one device")
-        if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        if t.dtype is not _I32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
             raise ValueError("requests must be contiguous int32, all of one length")
     return n
 
