@@ -137,6 +137,27 @@ def test_more_prompts_than_a_call_takes():
             _close(got[s0:s0 + 100], one, f"prompts {s0} ..", LOGIT_RTOL)
 
 
+def test_job_with_a_shared_prefix():
+    """The data-parallel job's tokens are the engine's over its prompts, the first of whose tokens are all alike."""
+    from specdec_b200.engine.dp import run_specdec_dp, synthetic_prompts
+    from specdec_b200.engine.model import PagedModel
+    from specdec_b200.engine.specdec import SpecDecEngine
+
+    tcfg, dcfg = _cfgs()
+    job = dict(total_seqs=3, prompt_len=40, max_new=12, k=4, seed=5)
+    res = run_specdec_dp(tcfg, dcfg, shared_prefix=24, **job)
+    prompts = synthetic_prompts(3, 40, tcfg.vocab, 5)
+    prompts[:, :24] = prompts[0, :24]
+    eng = SpecDecEngine(PagedModel.random(tcfg, 6), PagedModel.random(dcfg, 7), 3, 40, 12, k=4, shared_prefix=24)
+    eng.capture()
+    eng.prefill(prompts.cuda())
+    eng.decode()
+    assert torch.equal(res.tokens, eng.tokens())
+    for bad in (-1, 40):
+        with pytest.raises(ValueError):
+            run_specdec_dp(tcfg, dcfg, shared_prefix=bad, **job)
+
+
 def test_engine_refusals():
     from specdec_b200.engine.model import PagedModel
     from specdec_b200.engine.specdec import SpecDecEngine
