@@ -930,6 +930,9 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       auto work = [&](auto half, int k) {
         const int H = half;
         const bool more = k + 1 < nh;
+        // (Its slots' phases can be told apart only by a warp that is no more than one behind or ahead: a tile that had no
+        // rows in the items before may be far ahead, until the item's first scores are there.)
+        if (!AHEAD && k == 0 && wash == 0) lazy_wait(&s_full[t][0], sn & 1, dead);
         if (H == 0 && k / 2 >= wash) wash_block(k / 2);
         if (!AHEAD) load(half);
         if (!any_row) {

@@ -74,6 +74,26 @@ def test_many_sequences(H, KV, D):
         assert (out[row0[0] - 1] == FILL).all() and (out[-1] == FILL).all()
 
 
+@pytest.mark.parametrize("H,KV,D", [(12, 2, 128), (14, 2, 64), (5, 5, 128)])
+def test_second_tiles_after_items_without_them(H, KV, D):
+    """Items with rows for one tile only, then one whose second tile sees more keys than the first and washes the first
+    block: its warps wait for nobody in the items before."""
+    per = 128 // (H // KV)
+    unit = [min(5, per)] * 6 + [2 * per]
+    lens = unit * (2048 // 7 if per < 100 else 40)
+    extra = [62 - per] * len(lens) if per < 62 else [0] * len(lens)
+    case = packed_case(lens, H, KV, D, 17, extra=extra)
+    q, k, v, row0, kv0, ctx = case
+    first = _run(case, lens)
+    for _ in range(20):
+        assert torch.equal(_run(case, lens), first)
+    for b in range(6, len(lens), 21):
+        r, c = row0[b], kv0[b]
+        want, tol = plain_attention(q[r:r + lens[b]], k[c:c + ctx[b]], v[c:c + ctx[b]],
+                                    torch.arange(lens[b]) + extra[b] + 1, 1 / math.sqrt(D))
+        assert_rows(first[r:r + lens[b]], want, tol, f"sequence {b}")
+
+
 def test_long_prompts_of_mixed_lengths():
     """Units that CTA boundaries cut, at both head sizes."""
     for H, KV, D in ((12, 2, 128), (14, 2, 64)):
