@@ -456,6 +456,11 @@ SD_DEV RowItem load_item(const RowItem* at) {
 SD_DEV int first_hidden(const RowItem& it) { return it.src < 0 ? it.k1 : min(it.first + it.vt0 + 1, it.k1); }
 // First block of the item with keys that some row does not see or that do not exist (none: past the last block).
 SD_DEV int first_washed(const RowItem& it) { return max(first_hidden(it) - it.k0, 0) / kKeyBlock; }
+// Some row of a tile with `halves` half blocks of the item sees a key that another row does not see.  (A tile that ends
+// before the first such block neither waits for the washing nor looks at what it noted: it may be done before.)
+SD_DEV bool sees_washed(const RowItem& it, int halves) {
+  return first_hidden(it) < it.k1 && halves > 2 * first_washed(it);
+}
 // The halves of a bf16 pair that are infinite or NaN, as a mask of ones over them.
 SD_DEV uint32_t not_finite(uint32_t w) {
   const uint32_t hi = ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
@@ -763,8 +768,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[NS], empty[NS], raw_full, raw_empty;
   __shared__ uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], pv_done[2], o_full[2], v_clean[2], bad_read[2][2], fin[2];
-  // [tile][its item % 2]: keys past first_hidden whose V holds an infinity or a NaN.  A tile's items here are those in
-  // which it has work and some row does not see all keys: only those are waited for by both sides.
+  // [tile][its item % 2]: keys past first_hidden whose V holds an infinity or a NaN.  A tile's items here are those of
+  // sees_washed: only those are waited for by both sides.
   __shared__ uint32_t s_bad[2][2][4][8];  // (a washing warp its own eight words)
   __shared__ RowItem s_items[ITEMS];  // the CTA's first items
   __shared__ int s_range[2];
@@ -859,7 +864,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       const int nh = tile_halves(p, it, t), nh_other = tile_halves(p, it, t ^ 1);
       const int hidden = first_hidden(it), blk0 = blk;
       blk += (max(nh, nh_other) + 1) / 2;
-      const bool reads = hidden < it.k1 && nh > 0, other_reads = hidden < it.k1 && nh_other > 0;
+      const bool reads = sees_washed(it, nh), other_reads = sees_washed(it, nh_other);
       const uint32_t rd_mine = rd[t] & 1, rd_other = rd[t ^ 1];
       rd[t] += reads;
       rd[t ^ 1] += other_reads;
@@ -885,9 +890,10 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         }
       };
       // Washing: what a masked key's zero probability meets must be finite.  V rows past the last key (the next
-      // sequence's, a page's old contents) become zero as far as the products reach; an infinity or a NaN in a key that only some rows see becomes
-      // zero, too, and its key is noted for the rows that do see it (after the epilogue).  The tile that has work in every
-      // block does it, a quarter of the rows a warp; the MMA warps wait for it.  (E4M3: the widening warps do.)
+      // sequence's, a page's old contents) become zero as far as the products reach; an infinity or a NaN in a key that
+      // only some rows see becomes zero, too, and its key is noted for the rows that do see it (after the epilogue).
+      // The tile that has work in every block does it, a quarter of the rows a warp; the MMA warps wait for it.
+      // (E4M3: the widening warps do.)
       const int wash = V8 || nh < nh_other || (nh == nh_other && t == 1) ? 0x7fffffff : first_washed(it);
       auto wash_block = [&](int j) {
         uint32_t* const bad = s_bad[t][rd_mine][warp & 3];
@@ -1384,7 +1390,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           bool reads[2];
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            reads[t] = hidden < it.k1 && tile_halves(p, it, t) > 0;
+            reads[t] = sees_washed(it, tile_halves(p, it, t));
             if (!reads[t]) continue;
             if (rd[t] >= 2) ok = ok && row_wait(&bad_read[t][rd[t] & 1], (rd[t] / 2 - 1) & 1);
             if (lane < 8) s_bad[t][rd[t] & 1][r >> 5][lane] = 0;
