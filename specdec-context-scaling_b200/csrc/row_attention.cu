@@ -844,7 +844,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     const float scale = p.scale_log2;
     uint32_t sn = 0, pv = 0, on = 0;  // sn: phase bits of s_full; pv: halves handed over
     uint32_t blk = 0, rd[2] = {0, 0};  // blocks before this item; items of each tile that read s_bad
-    bool ok = true, dead = false;
+    bool ok = true, dead = false, idle = false;  // idle: no work in the item before
     for (int i = i0; i <= i1 && ok; ++i) {
       const RowItem it = item_at(i);
       if (it.nblk == 0) continue;
@@ -870,8 +870,11 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       rd[t ^ 1] += other_reads;
       if (nh == 0) {  // no tile, or a piece past the tile's keys: the row's other pieces are all of it
         if (it.slot >= 0 && limit > 0) p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
+        idle = true;
         continue;
       }
+      const bool was_idle = idle;
+      idle = false;
       const bool any_row = __any_sync(0xffffffffu, limit > 0);
       const int least = __reduce_min_sync(0xffffffffu, limit > 0 ? limit : 0x7fffffff);
       float m = -INFINITY, l = 0.f;
@@ -936,9 +939,6 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       auto work = [&](auto half, int k) {
         const int H = half;
         const bool more = k + 1 < nh;
-        // (Its slots' phases can be told apart only by a warp that is no more than one behind or ahead: a tile that had no
-        // rows in the items before may be far ahead, until the item's first scores are there.)
-        if (!AHEAD && k == 0 && wash == 0) lazy_wait(&s_full[t][0], sn & 1, dead);
         if (H == 0 && k / 2 >= wash) wash_block(k / 2);
         if (!AHEAD) load(half);
         if (!any_row) {
@@ -1012,6 +1012,9 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       };
       constexpr std::integral_constant<int, 0> even{};
       constexpr std::integral_constant<int, 1> odd{};
+      // (A slot's phases can be told apart only by a warp that is no more than one behind or ahead: a tile that had no
+      // work in the item before may be far ahead, until the item's first scores are there.)
+      if (!AHEAD && wash == 0 && was_idle) lazy_wait(&s_full[t][0], sn & 1, dead);
       if (AHEAD) load(even);
       // Pages at head_dim 128: one body for both halves, half the instructions to fetch, which items of few blocks wait for
       // (E4M3 64 requests x 5 rows 70.6 -> 64.7 us, 3 groups of 16 41.1 -> 38.4).  Long prompts are better off with two

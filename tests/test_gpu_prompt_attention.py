@@ -94,6 +94,23 @@ def test_second_tiles_after_items_without_them(H, KV, D):
         assert_rows(first[r:r + lens[b]], want, tol, f"sequence {b}")
 
 
+@pytest.mark.parametrize("KV,D", [(1, 128), (1, 64)])
+def test_last_blocks_of_second_tiles(KV, D):
+    """Two tokens a unit, the second of which sees one key past a block's end: the first tile is done with the item before
+    that block is washed."""
+    lens, extra = [2] * 1500, [127, 255, 127] * 500
+    case = packed_case(lens, 128, KV, D, 23, extra=extra)
+    q, k, v, row0, kv0, ctx = case
+    first = _run(case, lens)
+    for _ in range(20):
+        assert torch.equal(_run(case, lens), first)
+    for b in range(0, 1500, 97):
+        r, c = row0[b], kv0[b]
+        want, tol = plain_attention(q[r:r + 2], k[c:c + ctx[b]], v[c:c + ctx[b]], torch.arange(2) + extra[b] + 1,
+                                    1 / math.sqrt(D))
+        assert_rows(first[r:r + 2], want, tol, f"sequence {b}")
+
+
 def test_long_prompts_of_mixed_lengths():
     """Units that CTA boundaries cut, at both head sizes."""
     for H, KV, D in ((12, 2, 128), (14, 2, 64)):
