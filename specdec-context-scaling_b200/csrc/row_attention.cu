@@ -39,9 +39,9 @@
 //
 // Bound: the softmax warps.  A half block of both tiles takes about 1900 clocks, of which the tensor cores are busy for
 // 1290 (ncu: 53 % of the cycles; exponential unit 39 %; issue slots 42 %; DRAM 2 %): 1200 are exponentials, the rest
-// the way of the scores from TMEM and of P back.  Four prompts of 8192 tokens (12 heads over 2, 128 dims) take 810 to
-// 860 us, 960 to 1020 TFLOP/s (of 1632 measured); 16 of 1024 tokens 98 us (520); 64 x 5 rows over a shared 8192-token
-// prefix and 1024 tokens each 48 us against 78 us by paged_attention, which reads the prefix for every sequence.
+// the way of the scores from TMEM and of P back.  Four prompts of 8192 tokens (12 heads over 2, 128 dims) take 820 to
+// 870 us, 950 to 1000 TFLOP/s (of 1632 measured); 16 of 1024 tokens 99 to 105 us (500); 64 x 5 rows over a shared
+// 8192-token prefix and 1024 tokens each 48 to 54 us against 78 us by paged_attention, which reads the prefix for every sequence.
 // What small calls cost: the plan 5 us (its code is fetched and run once; later layers reuse it), an item's start and
 // end 2 to 3 us (first block, epilogue), the join 3 us and up.
 #include <initializer_list>
