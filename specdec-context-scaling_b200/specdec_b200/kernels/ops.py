@@ -383,7 +383,8 @@ def append_kv(k_new, v_new, cache: PagedKVCache, layer: int, *, row0, n_new, pos
         if t.dtype != torch.bfloat16 or t.dim() != 3 or t.stride(2) != 1:
             raise ValueError("k_new/v_new must be bf16 (rows, KV, D) with contiguous D")
     # (the stride of a dimension of one is never taken)
-    if any(a != b for a, b, n in zip(k_new.stride(), v_new.stride(), k_new.shape) if n > 1):
+    if k_new.stride() != v_new.stride() and any(
+            a != b for a, b, n in zip(k_new.stride(), v_new.stride(), k_new.shape) if n > 1):
         raise ValueError("k_new and v_new must share strides")
     args = _append_args(cache, layer, row0, n_new, pos0, max_new, len_out, status, k_new.data_ptr(),
                         v_new.data_ptr(), k_new.stride(0), k_new.stride(1))
