@@ -576,9 +576,10 @@ int specdec_umma_selftest(const void* k, const void* q, const void* v, const voi
    waited_ns (device u64, may be NULL) receives the time CTA 0 spent in its wait. */
 int specdec_wait_selftest(int32_t mode, void* counter, int32_t n_ctas, int32_t grid, int64_t limit_ns,
                           int32_t* status, void* waited_ns, specdec_stream_t stream);
-/* Limit, 0 .. 1e9 ns, of the device waits in the 8-bit kernels that the calling thread launches from here on, so
-   that their give-up paths can be tested; one second unless set.  0: linear's waits for what is to be stored give
-   up without looking, and rows that are copied ahead are not copied, so that their waits run out. */
+/* Limit, 0 .. 1e9 ns, of the device waits in the 8-bit kernels and in those of prompt_attention and
+   shared_prefix_attention that the calling thread launches from here on, so that their give-up paths can be tested;
+   one second unless set.  0: linear's waits for what is to be stored and the attention's for its scores give up
+   without looking, and rows that are copied ahead are not copied, so that their waits run out. */
 int specdec_wait_limit_selftest(int64_t limit_ns);
 const char* specdec_last_error(void);
 int specdec_abi_version(void);

@@ -123,6 +123,7 @@ struct RowParams {
   int32_t group_rows;           // workspace rows before the sequences' slots
   float scale_log2;
   uint64_t key;                 // of this launch shape
+  uint64_t wait_ns;             // limit of a wait; 0: the softmax warps give up without looking
   int32_t* status;
   // workspace
   int32_t *cta_first, *cta_last;                // [grid]
@@ -487,7 +488,8 @@ SD_DEV int tile_halves(const RowParams& p, const RowItem& it, int t) {
 
 // Bounded waits of this kernel's warps, most of which wait most of the time: the hint lets the hardware put a warp
 // to sleep for up to a millisecond instead of having it poll beside the softmax warps.  A wait that runs out (one second)
-// ends the CTA's work: its warps leave their loops, copies and products under way are waited for, the status says so.
+// ends the CTA's work: its warps leave their loops, and the status says so.  Copies and products under way are waited for
+// by the warps that issued them, whether or not a wait of their own ran out: the warp that would have used them may have left.
 SD_DEV bool mbar_try_sleep(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -499,24 +501,24 @@ SD_DEV bool mbar_try_sleep(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-SD_DEV bool row_wait(uint64_t* bar, uint32_t parity) {
+SD_DEV bool row_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
   bool got = mbar_try_sleep(bar, parity);
   if (!got) {
     const uint64_t t0 = globaltimer_ns();
     do {
       got = mbar_try_sleep(bar, parity);
-    } while (!got && globaltimer_ns() - t0 < kWaitLimitNs);
+    } while (!got && globaltimer_ns() - t0 < limit_ns);
   }
   return __all_sync(0xffffffffu, got);
 }
 
 // A wait whose failure is looked at later: most of these barriers are complete when their turn comes, and a vote a wait
 // would be most of its cost.
-SD_DEV void lazy_wait(uint64_t* bar, uint32_t parity, bool& dead) {
+SD_DEV void lazy_wait(uint64_t* bar, uint32_t parity, bool& dead, uint64_t limit_ns) {
   if (mbar_try_sleep(bar, parity) || dead) return;
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_sleep(bar, parity)) {
-    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+    if (globaltimer_ns() - t0 > limit_ns) {
       dead = true;
       break;
     }
@@ -844,7 +846,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     const float scale = p.scale_log2;
     uint32_t sn = 0, pv = 0, on = 0;  // sn: phase bits of s_full; pv: halves handed over
     uint32_t blk = 0, rd[2] = {0, 0};  // blocks before this item; items of each tile that read s_bad
-    bool ok = true, dead = false, idle = false;  // idle: no work in the item before
+    bool ok = true, dead = p.wait_ns == 0, idle = false;  // idle: no work in the item before
     for (int i = i0; i <= i1 && ok; ++i) {
       const RowItem it = item_at(i);
       if (it.nblk == 0) continue;
@@ -884,7 +886,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       float s[AHEAD ? 2 : 1][64];
       auto load = [&](auto half) {
         const int H = half;
-        lazy_wait(&s_full[t][H], (sn >> H) & 1, dead);
+        lazy_wait(&s_full[t][H], (sn >> H) & 1, dead, p.wait_ns);
         sn ^= 1u << H;
         umma::fence_after_sync();
         if (any_row) {
@@ -901,14 +903,16 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       auto wash_block = [&](int j) {
         uint32_t* const bad = s_bad[t][rd_mine][warp & 3];
         uint32_t* const bad_other = s_bad[t ^ 1][rd_other & 1][warp & 3];
+        const uint32_t slot = ((blk0 + j) & 1) * 2 + 1;
+        if (j == first_washed(it) && other_reads && rd_other >= 2)
+          lazy_wait(&bad_read[t ^ 1][rd_other & 1], (rd_other / 2 - 1) & 1, dead, p.wait_ns);
+        lazy_wait(&full[slot], ((blk0 + j) >> 1) & 1, dead, p.wait_ns);
+        if (__any_sync(0xffffffffu, dead)) return;  // what is not washed is not announced
         if (j == first_washed(it)) {
-          if (other_reads && rd_other >= 2) lazy_wait(&bad_read[t ^ 1][rd_other & 1], (rd_other / 2 - 1) & 1, dead);
           if (lane < 8 && reads) bad[lane] = 0;
           if (lane < 8 && other_reads) bad_other[lane] = 0;
           __syncwarp();
         }
-        const uint32_t slot = ((blk0 + j) & 1) * 2 + 1;
-        lazy_wait(&full[slot], ((blk0 + j) >> 1) & 1, dead);
         uint8_t* const v = smem + Geo::RING + slot * Geo::TILE;
         const int key0 = it.k0 + j * kKeyBlock;
         // (the MMAs take 16 keys a step, and none of the steps past the last key's)
@@ -968,7 +972,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           if constexpr (V8) {  // the block's scales are there when its codes are widened
             const int b = blk0 + k / 2;
             vs = s_vs[b & 1] + 64 * H;
-            if (H == 0) lazy_wait(&full[(b & 1) * 2 + 1], (b >> 1) & 1, dead);
+            if (H == 0) lazy_wait(&full[(b & 1) * 2 + 1], (b >> 1) & 1, dead, p.wait_ns);
           }
           auto next = [&]() {
             if (AHEAD && more) load(std::integral_constant<int, AHEAD ? 1 - decltype(half)::value : 0>{});
@@ -986,7 +990,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             m = to;
             l *= alpha;
             if (k > 0) {
-              lazy_wait(&pv_done[t], (pv - 1) & 1, dead);  // the MMAs over the half before this add to O
+              lazy_wait(&pv_done[t], (pv - 1) & 1, dead, p.wait_ns);  // the MMAs over the half before this add to O
               umma::fence_after_sync();
 #pragma unroll 1
               for (int c = 0; c < D; c += 16) {
@@ -1008,13 +1012,14 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         ++pv;
         umma::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t][H]);
+        // (after a wait that ran out an arrival might complete a phase that another warp's rows are missing from)
+        if (lane == 0 && !dead) mbar_arrive(&p_full[t][H]);
       };
       constexpr std::integral_constant<int, 0> even{};
       constexpr std::integral_constant<int, 1> odd{};
       // (A slot's phases can be told apart only by a warp that is no more than one behind or ahead: a tile that had no
       // work in the item before may be far ahead, until the item's first scores are there.)
-      if (!AHEAD && wash == 0 && was_idle) lazy_wait(&s_full[t][0], sn & 1, dead);
+      if (!AHEAD && wash == 0 && was_idle) lazy_wait(&s_full[t][0], sn & 1, dead, p.wait_ns);
       if (AHEAD) load(even);
       // Pages at head_dim 128: one body for both halves, half the instructions to fetch, which items of few blocks wait for
       // (E4M3 64 requests x 5 rows 70.6 -> 64.7 us, 3 groups of 16 41.1 -> 38.4).  Long prompts are better off with two
@@ -1033,7 +1038,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       }
       ok = !__any_sync(0xffffffffu, dead);
       if (!ok) break;
-      ok = row_wait(&o_full[t], on & 1);
+      ok = row_wait(&o_full[t], on & 1, p.wait_ns);
       if (!ok) break;
       ++on;
       umma::fence_after_sync();
@@ -1167,7 +1172,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             const uint32_t s = n % NS, round = n / NS;
             if (V8 && kv) {  // codes; the widening warps take care of the block's ring slot
               const uint32_t r = n >> 1;
-              if (r > 0 && !row_wait(&raw_empty, (r - 1) & 1)) {
+              if (r > 0 && !row_wait(&raw_empty, (r - 1) & 1, p.wait_ns)) {
                 ok = false;
                 break;
               }
@@ -1184,7 +1189,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
               __syncwarp();
               continue;
             }
-            if (round > 0 && !row_wait(&empty[s], (round - 1) & 1)) {
+            if (round > 0 && !row_wait(&empty[s], (round - 1) & 1, p.wait_ns)) {
               ok = false;
               break;
             }
@@ -1216,11 +1221,13 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           }
         }
       }
-      if (!ok) {
-        if (lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
-        // copies under way land before the CTA leaves
-        for (uint32_t k = n > NS ? n - NS : 0; k < n; ++k)
-          (void)(V8 && (k & 1) ? row_wait(&raw_full, (k >> 1) & 1) : row_wait(&full[k % NS], (k / NS) & 1));
+      if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      // copies under way land before the CTA leaves: the last of every slot (of the one for codes, the last)
+      for (uint32_t k = n > NS ? n - NS : 0; k < n; ++k) {
+        if (!V8 || (k & 1) == 0)
+          (void)row_wait(&full[k % NS], (k / NS) & 1, kWaitLimitNs);
+        else if (k + 2 >= n)
+          (void)row_wait(&raw_full, (k >> 1) & 1, kWaitLimitNs);
       }
     } else if (warp < kQueryWarp) {
       // ---------------------------------------------------------- MMA issue, a warp a row tile
@@ -1276,7 +1283,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         const int nb = (max(nh, __reduce_max_sync(0xffffffffu, tile_halves(p, it, t ^ 1))) + 1) / 2;
         const int last_key = __reduce_max_sync(0xffffffffu, it.k1 - it.k0);
         const int wash = V8 ? 0x7fffffff : __reduce_max_sync(0xffffffffu, first_washed(it));
-        ok = row_wait(&q_full, items & 1) && row_wait(&full[ks], kp);
+        ok = row_wait(&q_full, items & 1, p.wait_ns) && row_wait(&full[ks], kp, p.wait_ns);
         if (!ok) break;
         umma::fence_after_sync();
         if (nh > 0) qk(0, ks);
@@ -1288,19 +1295,19 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           const uint32_t vs = ks, vp = kp;  // this block's V; then the next block's K
           next(ks, kp);
           const bool last = j == nb - 1;
-          ok = row_wait(&full[vs], vp);
-          if (!last) ok = ok && row_wait(&full[ks], kp);
+          ok = row_wait(&full[vs], vp, p.wait_ns);
+          if (!last) ok = ok && row_wait(&full[ks], kp, p.wait_ns);
           if (!ok) break;
           umma::fence_after_sync();
           if (j >= wash) {  // the softmax warps wash this block's V
-            ok = row_wait(&v_clean[vs >> 1], (cleaned >> (vs >> 1)) & 1);
+            ok = row_wait(&v_clean[vs >> 1], (cleaned >> (vs >> 1)) & 1, p.wait_ns);
             cleaned ^= 1u << (vs >> 1);
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int k = 2 * j + h;
             if (k < nh) {
-              ok = ok && row_wait(&p_full[t][h], (pn >> h) & 1);
+              ok = ok && row_wait(&p_full[t][h], (pn >> h) & 1, p.wait_ns);
               if (!ok) break;
               pn ^= 1u << h;
               umma::fence_after_sync();
@@ -1321,7 +1328,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       }
       if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
       commit(&fin[t]);
-      (void)row_wait(&fin[t], 0);
+      (void)row_wait(&fin[t], 0, kWaitLimitNs);  // products under way
     } else if (warp == kQueryWarp) {
       // ---------------------------------------------------------- query rows
       uint32_t items = 0;
@@ -1330,7 +1337,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         const RowItem it = item_at(i);
         if (it.nblk == 0) continue;
         const int tiles = it.vt0 + p.tpt < it.n_vt ? 2 : 1;
-        if (items > 0) ok = row_wait(&q_empty, (items - 1) & 1);
+        if (items > 0) ok = row_wait(&q_empty, (items - 1) & 1, p.wait_ns);
         if (!ok) break;
         ++items;
         if (it.row0 >= 0) {
@@ -1370,6 +1377,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         __syncwarp();
       }
       if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+      if (items > 0) (void)row_wait(&q_full, (items - 1) & 1, kWaitLimitNs);  // the last item's rows land before the CTA leaves
     } else {
       // ---------------------------------------------------------- E4M3: codes to bf16, a thread a key
       if constexpr (V8) {
@@ -1395,7 +1403,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           for (int t = 0; t < 2; ++t) {
             reads[t] = sees_washed(it, tile_halves(p, it, t));
             if (!reads[t]) continue;
-            if (rd[t] >= 2) ok = ok && row_wait(&bad_read[t][rd[t] & 1], (rd[t] / 2 - 1) & 1);
+            if (rd[t] >= 2) ok = ok && row_wait(&bad_read[t][rd[t] & 1], (rd[t] / 2 - 1) & 1, p.wait_ns);
             if (lane < 8) s_bad[t][rd[t] & 1][r >> 5][lane] = 0;
           }
           __syncwarp();
@@ -1407,8 +1415,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             const bool in = key < it.k1;
             if (j + 1 < nb) next = scale_of(j + 1);
             const uint32_t s = n % NS;
-            ok = row_wait(&raw_full, (n >> 1) & 1);
-            if (ok && n >= NS) ok = row_wait(&empty[s], (n / NS - 1) & 1);
+            ok = row_wait(&raw_full, (n >> 1) & 1, p.wait_ns);
+            if (ok && n >= NS) ok = row_wait(&empty[s], (n / NS - 1) & 1, p.wait_ns);
             if (!ok) break;
             const uint8_t* src = smem + Geo::RAW + r * 128;
             uint8_t* dst = smem + Geo::RING + s * Geo::TILE + r * 128;
@@ -1694,6 +1702,7 @@ static int fill_row_params(RowParams& p, const RowShape& s, void* ws, size_t ws_
   p.cap_group = w.cap_group;
   p.group_rows = static_cast<int32_t>(w.group_rows);
   p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.wait_ns = wait_limit_ns();
   p.cta_first = reinterpret_cast<int32_t*>(base + w.first);
   p.cta_last = reinterpret_cast<int32_t*>(base + w.last);
   p.cut_unit = reinterpret_cast<CutUnit*>(base + w.cut);
