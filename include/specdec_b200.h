@@ -360,7 +360,8 @@ int specdec_attention_fp8v(const void* q, const void* k, const void* v_codes, co
  * reuse_plan 1: the workspace holds the plan of an earlier call with the same batch (lengths, rows, heads,
  * num_sms): the layers of one prompt pass.  A workspace without a plan for these shapes is refused on the device
  * (SPECDEC_STATUS_PLAN_MISMATCH, nothing written).  Calls that share a workspace must not overlap, and out overlaps
- * none of q, k and v.  Up to 2048 sequences a call (and as many groups and members below).
+ * none of q, k and v.  SPECDEC_STATUS_TIMEOUT: a device wait gave up after its second; the rows that it stood for are
+ * NaN.  Up to 2048 sequences a call (and as many groups and members below).
  */
 typedef struct SpecdecPromptArgs {
   const void* q;
@@ -397,8 +398,8 @@ int specdec_prompt_attention(const SpecdecPromptArgs* args, specdec_stream_t str
  * attended to alone.  The pages of a group's prefix are taken from the page table of its first member with rows; of
  * prefix_len only whole pages that every row of the group sees are shared, the rest is read from each member's own
  * table.  A member out of range or listed twice, a negative prefix or a bad group_start raises
- * SPECDEC_STATUS_BAD_GROUP (a sequence listed twice counts where it is listed first); bad lengths skip the sequence as
- * in specdec_prompt_attention.  No counterpart in the reference (batch 1).
+ * SPECDEC_STATUS_BAD_GROUP (a sequence listed twice counts where it is listed first); bad lengths skip the sequence,
+ * and a wait that gave up leaves NaN, as in specdec_prompt_attention.  No counterpart in the reference (batch 1).
  */
 typedef struct SpecdecSharedPrefixArgs {
   const void* q; /* bf16 */

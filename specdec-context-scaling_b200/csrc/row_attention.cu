@@ -488,8 +488,9 @@ SD_DEV int tile_halves(const RowParams& p, const RowItem& it, int t) {
 
 // Bounded waits of this kernel's warps, most of which wait most of the time: the hint lets the hardware put a warp
 // to sleep for up to a millisecond instead of having it poll beside the softmax warps.  A wait that runs out (one second)
-// ends the CTA's work: its warps leave their loops, and the status says so.  Copies and products under way are waited for
-// by the warps that issued them, whether or not a wait of their own ran out: the warp that would have used them may have left.
+// ends the CTA's work: its warps leave their loops, the status says so, and the rows that they stood for are NaN.  Copies
+// and products under way are waited for by the warps that issued them, whether or not a wait of their own ran out: the
+// warp that would have used them may have left.
 SD_DEV bool mbar_try_sleep(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -775,6 +776,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   __shared__ uint32_t s_bad[2][2][4][8];  // (a washing warp its own eight words)
   __shared__ RowItem s_items[ITEMS];  // the CTA's first items
   __shared__ int s_range[2];
+  __shared__ int s_lost[kSoftmaxWarps];  // first item that a softmax warp gave up on
   __shared__ alignas(16) float s_vs[V8 ? 2 : 1][kKeyBlock];  // E4M3: scales of the keys in V's ring slots
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -802,6 +804,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     mbar_init(&fin[1], 1);
     fence_barrier_init();
   }
+  if (tid < kSoftmaxWarps) s_lost[tid] = 0x7fffffff;
   if (warp == kIssueWarp) {
     umma::tmem_alloc(&s_tmem, Geo::TMEM_COLS);
     umma::tmem_relinquish();
@@ -846,8 +849,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     const float scale = p.scale_log2;
     uint32_t sn = 0, pv = 0, on = 0;  // sn: phase bits of s_full; pv: halves handed over
     uint32_t blk = 0, rd[2] = {0, 0};  // blocks before this item; items of each tile that read s_bad
-    bool ok = true, dead = p.wait_ns == 0, idle = false;  // idle: no work in the item before
-    for (int i = i0; i <= i1 && ok; ++i) {
+    bool dead = p.wait_ns == 0, idle = false;  // idle: no work in the item before
+    for (int i = i0; i <= i1; ++i) {
       const RowItem it = item_at(i);
       if (it.nblk == 0) continue;
       // this row's visible keys end at `limit` (0: no row here)
@@ -1036,10 +1039,10 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           if (__any_sync(0xffffffffu, dead)) break;
         }
       }
-      ok = !__any_sync(0xffffffffu, dead);
-      if (!ok) break;
-      ok = row_wait(&o_full[t], on & 1, p.wait_ns);
-      if (!ok) break;
+      if (__any_sync(0xffffffffu, dead) || !row_wait(&o_full[t], on & 1, p.wait_ns)) {
+        s_lost[warp - kSoftmaxWarp] = i;
+        break;
+      }
       ++on;
       umma::fence_after_sync();
       // keys whose V is not finite and that some row does not see: the MMAs had zeros for it
@@ -1145,7 +1148,6 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         if (lane == 0) mbar_arrive(&bad_read[t][rd_mine]);
       }
     }
-    if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
   } else {
     fewer_regs<RowRoles<SRC>::OTHER_REGS>();
     if (warp == kLoadWarp) {
@@ -1472,6 +1474,24 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   if (warp == kIssueWarp) {
     umma::fence_after_sync();
     umma::tmem_dealloc(tmem, Geo::TMEM_COLS);
+  }
+  // Where a wait ran out: NaN for the warp's rows of that item and of those behind it (the join hands a part's NaN on),
+  // so that nothing that the output or the workspace held before passes for a result.
+  const int lost = tid < 2 * kRowTile ? s_lost[tid >> 5] : 0x7fffffff;
+  if (lost <= i1 && (tid & 31) == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+#pragma unroll 1
+  for (int i = lost; i <= i1; ++i) {
+    const RowItem it = load_item(p.items + i);
+    const int t = tid / kRowTile, row = tid % kRowTile, tok = row / p.n_rep, vt = it.vt0 + t * p.tpt + tok;
+    if (it.nblk == 0 || tok >= p.tpt || vt >= it.n_vt) continue;
+    if (it.slot >= 0) {  // (it has these rows' places, whether or not a group's member has so many tokens)
+      p.part_ml[it.slot + tid] = make_float2(NAN, NAN);
+      continue;
+    }
+    uint4* const o = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(it.row0 + vt) * p.o_st +
+                                              static_cast<int64_t>(it.head * p.n_rep + row - tok * p.n_rep) * p.o_sh);
+#pragma unroll 1
+    for (int c = 0; c < D / 8; ++c) o[c] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
   }
 }
 

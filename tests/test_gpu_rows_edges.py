@@ -101,3 +101,31 @@ def test_waits_that_give_up_end_the_call(make, name, wait_limit):
         call()
         assert int(status) == 0
         check()
+
+
+@pytest.mark.parametrize("make,name", CALLS, ids=[n for _, n in CALLS])
+def test_what_waits_gave_up_on_is_nan(make, name, wait_limit):
+    """No row keeps what the output or the workspace held before: all are NaN where every first wait gives up, and each
+    is NaN or right where only some run out."""
+    from specdec_b200 import _lib
+
+    call, buf, status, rows, check = make(name)
+    call()
+    torch.cuda.synchronize()
+    good = buf.clone()
+    for limit in (0, 0, 1, 1000, 5000, 20_000, 50_000):
+        buf.fill_(FILL)
+        status.zero_()
+        wait_limit(limit)
+        call()
+        torch.cuda.synchronize()
+        wait_limit(1_000_000_000)
+        out = buf[1:-1]
+        here, want = out[rows], good[1:-1][rows]
+        nan = here.isnan().all(-1)
+        assert torch.equal(here[~nan], want[~nan])
+        assert nan.all() or limit > 0
+        assert int(status) == (_lib.STATUS_TIMEOUT if nan.any() else int(status) & _lib.STATUS_TIMEOUT)
+        left = torch.ones(buf.shape[0], dtype=torch.bool)
+        left[[r + 1 for r in rows]] = False
+        assert (buf[left.cuda()] == FILL).all()
