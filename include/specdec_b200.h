@@ -352,7 +352,8 @@ int specdec_attention_fp8v(const void* q, const void* k, const void* v_codes, co
  * query heads a KV head.  Row i of sequence b (query row q_row0[b] + i) sees keys j <= i + (ctx_len[b] - q_len[b]),
  * key j of sequence b being row kv_row0[b] + j of k and v: a whole prompt has ctx_len == q_len, the next piece
  * of a long one more keys than rows.  q_len[b] == 0 skips the sequence.  No value of another sequence, of a
- * later token or behind the last row reaches an output, whatever it holds.  A sequence whose lengths or rows are
+ * later token or behind the last row reaches an output, whatever it holds.  An infinity or a NaN in V of a key that a row
+ * sees leaves that value of the row not finite, whatever the key weighs (NaN or the infinity where the weight underflows).  A sequence whose lengths or rows are
  * out of range (ctx_len < q_len, q_len > max_q_len, rows past q_rows / kv_rows) raises SPECDEC_STATUS_BAD_LENGTH and
  * writes nothing; rows that belong to no sequence are left as they were.  Replaces the attention of the
  * reference's prompt pass (specdec/engine/model_self.py:715-775).

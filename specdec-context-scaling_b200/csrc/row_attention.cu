@@ -35,7 +35,9 @@
 //
 // What a masked key's zero probability meets in V must be finite.  The MMAs take none of the 16-key steps past an item's
 // last key, and what is left of the keys that some row does not see is washed in shared memory: an infinity or a NaN
-// becomes zero and its key is noted, and a row that does see it gets it added after the epilogue.
+// becomes zero and its key is noted, and a row that does see it gets it added after the epilogue.  So an infinity or a NaN
+// of a key that a row sees leaves the row's value not finite, whatever the key weighs: where the weight underflows to zero it
+// is 0 times an infinity (NaN) or the added infinity, by where the key lies.
 //
 // Bound: the softmax warps.  A half block of both tiles takes about 1900 clocks, of which the tensor cores are busy for
 // 1290 (ncu: 53 % of the cycles; exponential unit 39 %; issue slots 42 %; DRAM 2 %): 1200 are exponentials, the rest
@@ -61,6 +63,7 @@ constexpr int kMinQuota = 3;       // smallest range of a CTA, in blocks: 9, 6, 
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
 constexpr float kGrow = 1073741824.f;  // 2^30: a half block's sum past it moves the row's reference
 constexpr float kLargeScore = 4096.f;  // in units of log2
+constexpr float kNoPart = -1.f;        // sum of a partial row that was not computed
 constexpr float kExpC1 = 0.693282962f, kExpC2 = 0.242210999f, kExpC3 = 0.0550089143f;
 
 enum RowSource { kPacked = 0, kPaged = 1, kPagedE4M3 = 2 };
@@ -874,7 +877,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       rd[t] += reads;
       rd[t ^ 1] += other_reads;
       if (nh == 0) {  // no tile, or a piece past the tile's keys: the row's other pieces are all of it
-        if (it.slot >= 0 && limit > 0) p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, 0.f);
+        if (it.slot >= 0 && limit > 0) p.part_ml[it.slot + t * kRowTile + row] = make_float2(-INFINITY, kNoPart);
         idle = true;
         continue;
       }
@@ -1497,7 +1500,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
 
 // ---------------------------------------------------------------- joining partial rows
 // One warp two rows that lie next to each other in their slots (a lane pair reads a whole sector): the pieces of up
-// to two units, each a run of slots.  A piece that saw no key of the row has sum 0 and maximum -inf and weighs nothing.
+// to two units, each a run of slots.  A piece that saw no key of the row has sum 0 (kNoPart where its row was not written)
+// and maximum -inf and weighs nothing.
 // Bound by the latency of L2, so the loads of several pieces, sums and rows alike, are under way together.
 struct Pieces {
   int64_t row;  // workspace row of the first piece
@@ -1519,7 +1523,7 @@ SD_DEV void join_pair(const RowParams& p, const Pieces& a, const Pieces& b, __nv
     for (int e = 0; e < AT_ONCE; ++e) {
       const int i = base + e;
       if (i >= n) {
-        ml[e] = make_float2(-INFINITY, 0.f);
+        ml[e] = make_float2(-INFINITY, kNoPart);
         continue;
       }
       const int64_t r = i < a.n ? a.at(i) : b.at(i - a.n);
@@ -1538,8 +1542,8 @@ SD_DEV void join_pair(const RowParams& p, const Pieces& a, const Pieces& b, __nv
     for (int x = 0; x < PER; ++x) acc[x].x *= keep, acc[x].y *= keep, acc[x].z *= keep, acc[x].w *= keep;
 #pragma unroll
     for (int e = 0; e < AT_ONCE; ++e) {
-      const float w = ml[e].x == -INFINITY && ml[e].y == 0.f ? 0.f : fast_exp2(ml[e].x - mu);
-      if (w == 0.f) continue;  // (what such a piece's row holds may be anything)
+      if (ml[e].y == kNoPart) continue;  // (what such a piece's row holds may be anything)
+      const float w = fast_exp2(ml[e].x - mu);  // (0 times what is not finite stays not finite)
       l += w * ml[e].y;
 #pragma unroll
       for (int x = 0; x < PER; ++x) {

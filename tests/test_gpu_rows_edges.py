@@ -1,11 +1,14 @@
-"""GPU: prompt_attention and shared_prefix_attention at the edges of what they promise: waits that give up."""
+"""GPU: prompt_attention and shared_prefix_attention at the edges of what they promise: waits that give up, values that
+are not finite under weights of zero."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
 
-from rows_helpers import Pages, check_packed, check_pages, i32, make_batch, packed_case
+from rows_helpers import Pages, assert_rows, check_packed, check_pages, i32, make_batch, packed_case, plain_attention
 
 pytestmark = pytest.mark.gpu
 FILL = 7.0
@@ -129,3 +132,72 @@ def test_what_waits_gave_up_on_is_nan(make, name, wait_limit):
         left = torch.ones(buf.shape[0], dtype=torch.bool)
         left[[r + 1 for r in rows]] = False
         assert (buf[left.cuda()] == FILL).all()
+
+
+def _weightless(how, q, k, strong, key):
+    """Gives ``key`` no weight in any row: ``strong`` past it by more than fp32's range, or its own score -inf."""
+    q[..., 0] = 64.0
+    k[..., 0] = 0.0
+    if how == "underflow":
+        k[strong, :, 0] = 64.0  # 4096 of scale 1 / sqrt(D) and log2 e: 522 (D 64: 738)
+    else:
+        k[key, :, 0] = -math.inf
+
+
+def _check_weightless(out, q, k, v, limit, key, dim, what):
+    """Rows that see ``key``: the value at ``dim`` of its KV head is not finite, the rest is as without it."""
+    fine = torch.where(v.isfinite(), v, 0.0)
+    want, tol = plain_attention(q, torch.where(k.isfinite(), k, -1e4), fine, limit, 1 / math.sqrt(q.shape[-1]))
+    rep = q.shape[1] // k.shape[1]
+    sees = (limit > key).cuda()
+    assert not out[sees][:, :rep, dim].isfinite().any(), what
+    got = out.clone()
+    got[sees, :rep, dim] = want[sees][:, :rep, dim].to(out.dtype)
+    assert_rows(got, want, tol, what)
+
+
+# a key in front of everything, in a middle piece of a cut unit, before and behind the first key that some row does not see
+@pytest.mark.parametrize("how", ["underflow", "minus_infinity"])
+@pytest.mark.parametrize("H,KV,D", [(12, 2, 128), (14, 2, 64)])
+def test_infinite_values_without_weight_packed(H, KV, D, how):
+    for n, e in ((300, 2500), (40, 5000), (200, 0)):
+        for key in (0, e // 2, e - 1, e, e + n // 2, e + n - 1):
+            if key < 0:
+                continue
+            for strong in {key + 1, max(key - 1, 0), 0, e // 3} - {key}:
+                if strong >= e + 1:  # (every row sees it)
+                    continue
+                q, k, v, row0, kv0, ctx = packed_case([n], H, KV, D, 11, extra=[e])
+                _weightless(how, q, k, strong, key)
+                v[key, 0, 5] = math.inf
+                out = _ops().prompt_attention(q, k, v, make_batch(row0, [n], ctx, n), kv_row0=i32(kv0))
+                _check_weightless(out, q, k, v, torch.arange(n) + e + 1, key, 5, f"{n} after {e}, key {key}, {strong} strong")
+
+
+@pytest.mark.parametrize("how", ["underflow", "minus_infinity"])
+@pytest.mark.parametrize("H,KV,D", [(12, 2, 128), (14, 2, 64)])
+def test_infinite_values_without_weight_pages(H, KV, D, how):
+    """The key in the shared prefix, the strong one among the sequence's own keys, and the other way round."""
+    from specdec_b200.engine.paged_cache import kblock_index
+
+    lens, ctx, groups = [5] * 4, [2100, 2110, 2095, 2400], [([0, 1, 2, 3], 2080)]
+    idx = kblock_index(D, "cuda").view(16, D)
+    for key, strong in ((17, 2085), (2079, 2085), (2085, 17), (2092, 2079), (900, 17)):
+        pages = Pages(ctx, groups, KV, D, False, 12)
+        pool, pt = pages.cache.pools[0], pages.cache.page_table.cpu()
+        q = torch.randn(20, H, D, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+        q[..., 0] = 64.0
+        pool.k[..., idx[:, 0]] = 0.0
+        for b in range(4):
+            at = {j: (int(pt[b, j // 16]), j % 16) for j in (key, strong)}
+            if how == "underflow":
+                pool.k[at[strong][0], :, idx[at[strong][1], 0]] = 64.0
+            else:
+                pool.k[at[key][0], :, idx[at[key][1], 0]] = -math.inf
+            pool.v[at[key][0], 0, idx[at[key][1], 5]] = math.inf
+        out = _ops().shared_prefix_attention(q, pages.cache, 0, make_batch([0, 5, 10, 15], lens, ctx, 20),
+                                             _ops().SharedPrefix.from_groups(groups))
+        for b in range(4):
+            k, v = pages.kv(b)
+            _check_weightless(out[5 * b:5 * b + 5], q[5 * b:5 * b + 5], k, v, torch.arange(5) + ctx[b] - 4, key, 5,
+                              f"sequence {b}, key {key}, {strong} strong")
