@@ -22,16 +22,23 @@
 //                   group's rows do not follow one another)
 //   warps 4-7, 8-11 softmax and epilogue of row tile 0, 1: a thread owns a row, so maxima and sums need no exchange;
 //                   and the washing of V (below)
-//   warps 12-15     (E4M3 V) the block's codes to bf16 by moving bits; the keys' scales are multiplied into P
+//   warps 12-15     (E4M3 V) the block's codes to f16 by moving bits; the keys' scales are multiplied into P
 // A block of 128 keys is two halves of 64, each with scores S_t[h] of its own in TMEM:
-//   S_t[h] = Q_t K^T  ->  P = 2^((S - m) scale) as bf16 over the same columns  ->  O_t += P V (A operand from TMEM)
+//   S_t[h] = Q_t K^T  ->  P = 2^((S - m) scale) as bf16 (E4M3 f16) over the same columns  ->  O_t += P V (A operand from TMEM)
 // Half h + 1's products and half h's softmax run at the same time, and so do the two tiles.
 //
 // The running maximum is a stale one: m is a row's maximum over its first half block and moves only when a half block's
 // sum passes 2^30 (2^x has the range for it), so that O is almost never rescaled.  P is rounded to bf16 (2^-8 of each weight
-// at most, independent between keys); sums, maxima, O and the joined rows stay fp32.  A quarter of the exponentials
-// are a cubic on the FMA units (relative error 1.0e-4), the rest the exponential unit's: 64 a thread and half would
-// take 544 clocks a warp there.
+// at most, independent between keys); sums, maxima, O and the joined rows stay fp32.
+// A quarter of the exponentials are a cubic on the FMA units (relative error 1.0e-4), the rest the exponential unit's: 64 a
+// thread and half would take 544 clocks a warp there.
+//
+// E4M3: what is rounded is P times its key's scale, to f16 (2^-11), as paged_attention does it.  f16 has not bf16's
+// range: scales count in units of a power of two that puts the geometric mean of an item's first 32 keys (those that
+// all its rows see) between 2^2 and 2^3, O is multiplied by that unit at the end, and m also moves where a half block's
+// sum times the largest scale that the row sees passes 2^15, so that no weight reaches f16's end.  A weight below 2^-14
+// is off by up to 2^-25: its bits are missed only where the keys that carry a row have scales some 2^15 below that mean,
+// or 2^25 below another key's that the row sees.
 //
 // What a masked key's zero probability meets in V must be finite.  The MMAs take none of the 16-key steps past an item's
 // last key, and what is left of the keys that some row does not see is washed in shared memory: an infinity or a NaN
@@ -62,6 +69,8 @@ constexpr int kUnitCost = 2;       // what a unit costs beside its blocks (query
 constexpr int kMinQuota = 3;       // smallest range of a CTA, in blocks: 9, 6, 4 and 3 take 24.6, 20.3, 20.1 and 19.4 us for 4 decode steps
 constexpr int kMergeParts = 8;     // blocks of the cut-unit merge for each CTA of the grid
 constexpr float kGrow = 1073741824.f;  // 2^30: a half block's sum past it moves the row's reference
+constexpr float kGrowF16 = 32768.f;    // 2^15: the same of the sum times the block's largest scale (E4M3)
+constexpr int kScaleMean = 2;          // E4M3: the mean scale of an item's first keys is counted as 2^2 .. 2^3
 constexpr float kLargeScore = 4096.f;  // in units of log2
 constexpr float kNoPart = -1.f;        // sum of a partial row that was not computed
 constexpr float kExpC1 = 0.693282962f, kExpC2 = 0.242210999f, kExpC3 = 0.0550089143f;
@@ -471,13 +480,13 @@ SD_DEV uint32_t not_finite(uint32_t w) {
   return (hi >> 15) * 0xffffu;
 }
 
-// Two E4M3 codes, each in the upper byte of a half, as bf16: the bits moved to bf16's exponent and mantissa are the value
-// times 2^-120 (bf16's bias is 127, E4M3's 7; subnormals are subnormals in both), and the product with 2^120 is exact.
+// Two E4M3 codes, each in the upper byte of a half, as f16: the bits moved to f16's exponent and mantissa are the value
+// times 2^-8 (f16's bias is 15, E4M3's 7; subnormals are subnormals in both), and the product with 2^8 is exact.
 // (The NaN codes come out as 480.)
-SD_DEV uint32_t e4m3_bf16(uint32_t x) {
-  const uint32_t v = (x & 0x80008000u) | ((x >> 4) & 0x07f007f0u);
+SD_DEV uint32_t e4m3_f16(uint32_t x) {
+  const uint32_t v = (x & 0x80008000u) | ((x >> 1) & 0x3f803f80u);
   uint32_t y;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(v), "r"(0x7b807b80u));
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(v), "r"(0x5c005c00u));
   return y;
 }
 
@@ -593,9 +602,14 @@ SD_DEV float exp2_unit(float x) {
   asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-SD_DEV uint32_t round_bf16(float lo, float hi) {
+// two weights as the P V product takes them: bf16, beside E4M3 V f16
+template <bool V8>
+SD_DEV uint32_t round_weights(float lo, float hi) {
   uint32_t r;
-  asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  if constexpr (V8)
+    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 SD_DEV float max_nan(float a, float b) {
@@ -610,7 +624,7 @@ SD_DEV float max3_nan(float a, float b, float c) {
 }
 
 // 2^x on the FMA units: x = n + f with f in [-1/2, 1/2], 2^f by the cubic through 1 at 0 with the least largest relative
-// error on that interval (1.0e-04, against the 2^-9 that P is rounded to), n added to the exponent.  x is clamped to
+// error on that interval (1.0e-04, against the 2^-8, or 2^-11, that P is rounded to), n added to the exponent.  x is clamped to
 // [-127, 127] as z = (x + 127) / 254 in [0, 1], which costs nothing beside the scaling; z's rounding moves x by less
 // than 2^-16.  At -127 the exponent and the mantissa of 1 cancel: masked keys and all that is smaller give exactly 0.
 // (The clamp hides a NaN: the caller looks for one.)
@@ -652,7 +666,7 @@ struct Poly2 {
 
 // Eight pairs of scores at once: six take the exponential unit (12 x 8.5 clocks a warp), two the polynomial, whose
 // steps lie between the others'.  A pair costs about 8 issue slots by the unit and 24 by the polynomial, so a quarter
-// of the pairs balances the two.  Probabilities as bf16 pairs in w[0 .. 7], their sums added to `sum`.
+// of the pairs balances the two.  Probabilities as pairs of 16 bits in w[0 .. 7], their sums added to `sum`.
 template <bool V8>
 SD_DEV void eight_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, float zn, uint64_t (&sum)[2], float& seen,
                         const float* vs, uint32_t* w) {
@@ -671,7 +685,7 @@ SD_DEV void eight_pairs(const float* s, uint64_t sc, uint64_t ng, float zs, floa
       v = mul2(v, e & 1 ? g[e >> 1].y : g[e >> 1].x);
       unpack2(v, p0, p1);
     }
-    w[e] = round_bf16(p0, p1);
+    w[e] = round_weights<V8>(p0, p1);
   };
 #define SD_X(E) unpack2(fma2(pack2(s[2 * (E)], s[2 * (E) + 1]), sc, ng), x[2 * (E)], x[2 * (E) + 1]);
 #define SD_Y(E) y[E] = exp2_unit(x[E]);
@@ -710,12 +724,12 @@ SD_DEV void one_pair(const float* s, uint64_t sc, uint64_t minus_m, uint64_t& su
   b = exp2_unit(b);
   sum = add2(sum, pack2(a, b));
   if (V8) a *= vs[0], b *= vs[1];
-  *w = round_bf16(a, b);
+  *w = round_weights<V8>(a, b);
 }
 
-// P = 2^((s - m) scale) of 64 scores as bf16 in 32 TMEM columns; returns the sum, and in `seen` a NaN if there is one
+// P = 2^((s - m) scale) of 64 scores as bf16 (V8: f16) in 32 TMEM columns; returns the sum, and in `seen` a NaN if there is one
 // among the scores that took the polynomial.  USUAL: as s scale - m scale, eight of the 32 pairs by the polynomial.
-// V8: each P is rounded after a multiplication by its key's scale (the codes themselves are exact in bf16).
+// V8: each P is rounded after a multiplication by its key's scale (the codes themselves are exact in f16).
 // `before_last` is called when a quarter is left.  Not USUAL: what is there already stays for rows that are not `mine`,
 // so that no row's bits depend on what its neighbours' scores are.
 template <bool USUAL, bool V8, typename Hook>
@@ -779,8 +793,10 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
   __shared__ uint32_t s_bad[2][2][4][8];  // (a washing warp its own eight words)
   __shared__ RowItem s_items[ITEMS];  // the CTA's first items
   __shared__ int s_range[2];
-  __shared__ int s_lost[kSoftmaxWarps];  // first item that a softmax warp gave up on
-  __shared__ alignas(16) float s_vs[V8 ? 2 : 1][kKeyBlock];  // E4M3: scales of the keys in V's ring slots
+  __shared__ int s_lost;  // first item that a softmax warp gave up on
+  // E4M3: scales of the keys in V's ring slots, in units of s_unit, and the largest finite one of each widening warp's keys
+  __shared__ alignas(16) float s_vs[V8 ? 2 : 1][kKeyBlock], s_vs_top[V8 ? 2 : 1][4];
+  __shared__ float s_unit[2];
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -807,7 +823,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     mbar_init(&fin[1], 1);
     fence_barrier_init();
   }
-  if (tid < kSoftmaxWarps) s_lost[tid] = 0x7fffffff;
+  if (tid == 0) s_lost = 0x7fffffff;
   if (warp == kIssueWarp) {
     umma::tmem_alloc(&s_tmem, Geo::TMEM_COLS);
     umma::tmem_relinquish();
@@ -886,6 +902,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       const bool any_row = __any_sync(0xffffffffu, limit > 0);
       const int least = __reduce_min_sync(0xffffffffu, limit > 0 ? limit : 0x7fffffff);
       float m = -INFINITY, l = 0.f;
+      float unit = 1.f;  // E4M3: of the item's scales
       // At head_dim 64 one half's scores are loaded while the other's are worked on; at 128 the next half's products
       // are not done by then, and a warp that waits for them works on nothing.
       constexpr bool AHEAD = D == 64;
@@ -973,12 +990,13 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
             return max3_nan(max3_nan(mx[0], mx[1], x[60]), max3_nan(mx[2], mx[3], x[61]), max_nan(x[62], x[63]));
           };
           if (k == 0) m = row_max();
-          float seen;
+          float seen, vs_top = 0.f;  // E4M3: the block's largest scale
           const float* vs = nullptr;
           if constexpr (V8) {  // the block's scales are there when its codes are widened
             const int b = blk0 + k / 2;
             vs = s_vs[b & 1] + 64 * H;
             if (H == 0) lazy_wait(&full[(b & 1) * 2 + 1], (b >> 1) & 1, dead, p.wait_ns);
+            if (k == 0) unit = s_unit[b & 1];
           }
           auto next = [&]() {
             if (AHEAD && more) load(std::integral_constant<int, AHEAD ? 1 - decltype(half)::value : 0>{});
@@ -989,9 +1007,31 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           // for NaN and infinite scores, and where the reference is so large that the roundings of m scale and of the
           // polynomial's argument (3 2^-24 of it) would show beside P's own.  A NaN stays one.
           // (Rows of the tile that are no token's hold anything; rows that see nothing here add nothing.)
-          const bool redo = limit > key0 && (!(sum < kGrow) || seen != seen || !(fabsf(m) * scale < kLargeScore));
+          if constexpr (V8) {
+            const float4 y = *reinterpret_cast<const float4*>(s_vs_top[(blk0 + k / 2) & 1]);
+            vs_top = fmaxf(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)), kGrowF16 / kGrow);
+          }
+          // E4M3: nor may a weight pass f16's range; where the scales themselves would, the reference goes that much higher.
+          // (Whose keys' scales these are is asked only here.)
+          auto moves = [&](float scales) {
+            const bool grown = V8 ? !(sum * scales < kGrowF16) : !(sum < kGrow);
+            return limit > key0 && (grown || seen != seen || !(fabsf(m) * scale < kLargeScore));
+          };
+          bool redo = moves(vs_top);
           if (__any_sync(0xffffffffu, redo)) {
-            const float to = redo ? max_nan(m, row_max()) : m;
+            float top = row_max();
+            if constexpr (V8) {
+              float scales = vs_top;
+              if (masked) {
+                scales = kGrowF16 / kGrow;
+#pragma unroll 1
+                for (int c = 0; c < min(limit - key0, kKeyBlock / 2); ++c)
+                  if (fabsf(vs[c]) < INFINITY) scales = fmaxf(scales, fabsf(vs[c]));
+                redo = moves(scales);
+              }
+              if (scales > kGrowF16 / 2) top += __log2f(scales * (2 / kGrowF16)) / scale;
+            }
+            const float to = redo ? max_nan(m, top) : m;
             const float alpha = to == m ? 1.f : fast_exp2((m - to) * scale);  // (no reference yet: 0 of nothing)
             m = to;
             l *= alpha;
@@ -1043,7 +1083,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         }
       }
       if (__any_sync(0xffffffffu, dead) || !row_wait(&o_full[t], on & 1, p.wait_ns)) {
-        s_lost[warp - kSoftmaxWarp] = i;
+        atomicMin(&s_lost, i);
         break;
       }
       ++on;
@@ -1062,6 +1102,10 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
               float o[32];
               umma::tmem_ld32(o_ta + c, o);
               umma::tmem_wait_ld32(o);
+              if constexpr (V8) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] *= unit;
+              }
 #pragma unroll
               for (int e = 0; e < 8; ++e) to[(c / 4 + e) * 32] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
@@ -1069,7 +1113,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
         } else {
           // Rows leave through shared memory, 64 bytes of a row at a time, so that a store covers whole sectors.
           uint8_t* const stage = smem + Geo::STAGED + (warp - kSoftmaxWarp) * Geo::STAGE;
-          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const float inv = l == 0.f ? 0.f : V8 ? unit / l : 1.f / l;
           int64_t at = -1;  // this row's first value
           if (limit > 0)
             at = static_cast<int64_t>(it.row0 + vt) * p.o_st + static_cast<int64_t>(it.head * p.n_rep + rep) * p.o_sh;
@@ -1240,7 +1284,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       // products ahead: one warp for both tiles was the bound (4300 clocks a block against 2600 of products).
       const int t = warp - kIssueWarp;
       constexpr uint32_t id_qk = umma::idesc_f16(128, kKeyBlock / 2, true, true, false, false);
-      constexpr uint32_t id_pv = umma::idesc_f16(128, D, true, true, false, true);
+      constexpr uint32_t id_pv = umma::idesc_f16(128, D, !V8, !V8, false, true);
       constexpr uint32_t high = umma::desc_high(1024, umma::kSwizzle128B);
       const uint32_t q_low = umma::desc_low(smem_u32(smem) + t * Geo::TILE, 16);
       const uint32_t k_low = umma::desc_low(smem_u32(smem + Geo::RING), 16);
@@ -1384,7 +1428,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       if (!ok && lane == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
       if (items > 0) (void)row_wait(&q_full, (items - 1) & 1, kWaitLimitNs);  // the last item's rows land before the CTA leaves
     } else {
-      // ---------------------------------------------------------- E4M3: codes to bf16, a thread a key
+      // ---------------------------------------------------------- E4M3: codes to f16, a thread a key
       if constexpr (V8) {
         const int r = tid - 32 * kWidenWarp;
         uint32_t n = 1, rd[2] = {0, 0};
@@ -1393,9 +1437,9 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           const RowItem it = item_at(i);
           if (it.nblk == 0) continue;
           const int nb = (max(tile_halves(p, it, 0), tile_halves(p, it, 1)) + 1) / 2;
-          // the scale of key r of block j; 0 past the last key, where the codes (clamped pages) are finite or NaN
-          auto scale_of = [&](int j) {
-            const int key = it.k0 + j * kKeyBlock + r;
+          // the scale of the item's key x; 0 past the last key, where the codes (clamped pages) are finite or NaN
+          auto scale_of = [&](int x) {
+            const int key = it.k0 + x;
             if (key >= it.k1) return 0.f;
             int page = p.page_table[static_cast<int64_t>(it.kv) * p.max_pages + key / kPage];
             if (page < 0 || page >= p.num_pages) page = 0;  // the loading warp reports it
@@ -1413,12 +1457,15 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
           }
           __syncwarp();
           if (!ok) break;
-          float next = scale_of(0);
+          // For the unit of the item's scales every warp looks at its first 32 keys for itself, as far as all rows see them
+          // that see anything of the item.
+          float next = scale_of(r), unit = 1.f, per_unit = 1.f;
+          const float first = lane < max(hidden - it.k0, 1) ? scale_of(lane) : 0.f;
           for (int j = 0; j < nb; ++j, n += 2) {
             const float sc = next;
             const int key = it.k0 + j * kKeyBlock + r;
             const bool in = key < it.k1;
-            if (j + 1 < nb) next = scale_of(j + 1);
+            if (j + 1 < nb) next = scale_of((j + 1) * kKeyBlock + r);
             const uint32_t s = n % NS;
             ok = row_wait(&raw_full, (n >> 1) & 1, p.wait_ns);
             if (ok && n >= NS) ok = row_wait(&empty[s], (n / NS - 1) & 1, p.wait_ns);
@@ -1435,8 +1482,8 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 nan |= (w[e] & 0x7f7f7f7fu) + 0x01010101u;
-                y[2 * e] = in ? e4m3_bf16(__byte_perm(w[e], 0, 0x1404)) : 0u;
-                y[2 * e + 1] = in ? e4m3_bf16(__byte_perm(w[e], 0, 0x3424)) : 0u;
+                y[2 * e] = in ? e4m3_f16(__byte_perm(w[e], 0, 0x1404)) : 0u;
+                y[2 * e + 1] = in ? e4m3_f16(__byte_perm(w[e], 0, 0x3424)) : 0u;
               }
               uint8_t* d = dst + (ch >> 2) * 16384;
               const int g = (ch & 3) * 2;
@@ -1444,8 +1491,23 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
               *reinterpret_cast<uint4*>(d + (((g + 1) ^ (r & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
             }
             const bool strange = in && ((nan & 0x80808080u) || !(fabsf(sc) < INFINITY));
+            if (j == 0) {  // (here, so that the scales' loads and the codes' have the same time)
+              const int x = (__float_as_int(first) >> 23) & 255;
+              const bool fine = x != 0 && x != 255;
+              const int sum = __reduce_add_sync(0xffffffffu, fine ? x - 127 : 0);
+              const int of = __popc(__ballot_sync(0xffffffffu, fine));
+              // (the clamp keeps the unit, its reciprocal and their products with scales up to 2^45 away in fp32's range)
+              const int mean = of > 0 ? min(max(__float2int_rd(__fdividef(sum, of)), -80), 80) : 0;
+              unit = __int_as_float((127 + mean - kScaleMean) << 23);
+              per_unit = __int_as_float((127 - mean + kScaleMean) << 23);
+            }
             // a key that some row does not see adds nothing that is not finite here
-            s_vs[s >> 1][r] = strange && key >= hidden && !(fabsf(sc) < INFINITY) ? 0.f : sc;
+            const bool sc_fine = fabsf(sc) < INFINITY;
+            const float counted = sc_fine ? fminf(fmaxf(sc * per_unit, -3.4e38f), 3.4e38f) : key >= hidden ? 0.f : sc;
+            s_vs[s >> 1][r] = counted;
+            const uint32_t top = __reduce_max_sync(0xffffffffu, sc_fine ? __float_as_uint(fabsf(counted)) : 0u);
+            if (lane == 0) s_vs_top[s >> 1][r >> 5] = __uint_as_float(top);
+            if (r == 0) s_unit[s >> 1] = unit;
             if (strange) {
 #pragma unroll 1
               for (int d = 0; d < D; ++d)
@@ -1478,10 +1540,10 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
     umma::fence_after_sync();
     umma::tmem_dealloc(tmem, Geo::TMEM_COLS);
   }
-  // Where a wait ran out: NaN for the warp's rows of that item and of those behind it (the join hands a part's NaN on),
-  // so that nothing that the output or the workspace held before passes for a result.
-  const int lost = tid < 2 * kRowTile ? s_lost[tid >> 5] : 0x7fffffff;
-  if (lost <= i1 && (tid & 31) == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
+  // Where a wait ran out: NaN for the rows of that item and of those behind it (the join hands a part's NaN on), so that
+  // nothing that the output or the workspace held before passes for a result.
+  const int lost = tid < 2 * kRowTile ? s_lost : 0x7fffffff;
+  if (lost <= i1 && tid == 0) raise_status(p.status, SPECDEC_STATUS_TIMEOUT);
 #pragma unroll 1
   for (int i = lost; i <= i1; ++i) {
     const RowItem it = load_item(p.items + i);

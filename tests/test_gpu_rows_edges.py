@@ -1,5 +1,5 @@
 """GPU: prompt_attention and shared_prefix_attention at the edges of what they promise: waits that give up, values that
-are not finite under weights of zero."""
+are not finite under weights of zero, E4M3 scales."""
 
 from __future__ import annotations
 
@@ -201,3 +201,106 @@ def test_infinite_values_without_weight_pages(H, KV, D, how):
             k, v = pages.kv(b)
             _check_weightless(out[5 * b:5 * b + 5], q[5 * b:5 * b + 5], k, v, torch.arange(5) + ctx[b] - 4, key, 5,
                               f"sequence {b}, key {key}, {strong} strong")
+
+
+def _f16_tolerance(q, k, v, limit, scale):
+    """As rows_helpers' tolerance with weights that are rounded to f16: 2^-11 A in the place of 2^-8 A, where none of them
+    is below f16's normal range."""
+    want, tol = plain_attention(q, k, v, limit, scale)
+    A, _ = plain_attention(q, k, v.abs(), limit, scale)
+    return want, tol - A * (2.0**-8 - 2.0**-11)
+
+
+def _e4m3_pages(ctx, groups, scales, seed, zero=()):
+    """E4M3 pages, scales[b](n) the scales of sequence b's tokens; the codes of the tokens in ``zero`` are 0."""
+    pages = Pages(ctx, groups, 2, 128, True, seed)
+    pool, pt = pages.cache.pools[0], pages.cache.page_table.cpu()
+    for b, n in enumerate(ctx):
+        s = scales[b](n).cuda()
+        for j in range(n):
+            page, at = int(pt[b, j // 16]), j % 16
+            pool.v_scale[page, :, at] = s[j]
+            if j in zero:
+                pool.v[page].view(2, 16, 128)[:, at] = 0
+    return pages, pool, pt
+
+
+def test_e4m3_weights_keep_eleven_bits():
+    """Two keys of equal weight and opposite codes: what is left is the difference of their scales, and the rounding of
+    weight times scale shows at its full size."""
+    B = 60
+    g = torch.Generator().manual_seed(1)
+    pages = Pages([2] * B, [], 2, 128, True, 21)
+    pool, pt = pages.cache.pools[0], pages.cache.page_table.cpu()
+    for b in range(B):
+        codes = pool.v[int(pt[b, 0])].view(2, 16, 128)
+        codes[:, 1] = codes[:, 0] ^ 0x80
+    q = torch.zeros(B, 12, 128, dtype=torch.bfloat16, device="cuda")
+    for groups in ([], [(list(range(B)), 0)]):
+        out = _ops().shared_prefix_attention(q, pages.cache, 0, make_batch(list(range(B)), [1] * B, [2] * B, B),
+                                             _ops().SharedPrefix.from_groups(groups))
+        for b in range(B):
+            k, v = pages.kv(b)
+            assert_rows(out[b:b + 1], *_f16_tolerance(q[b:b + 1], k, v, torch.tensor([2]), 0.1), f"sequence {b}")
+
+
+# scales of a sequence's tokens; with queries of zero every weight is 1, and times its scale and the unit (2^-b where
+# the reference moves by b) stays between 2^-14 and 2^15
+SCALES = {
+    "mixed": lambda n: torch.exp2(torch.rand(n, generator=torch.Generator().manual_seed(n)) * 12 - 6),
+    "zero_tokens": lambda n: torch.where(torch.arange(n) % 100 == 3, 1.0, 2.0**-22 * 1.3),
+    "growing": lambda n: torch.where(torch.arange(n) < 128, 2.0**-20, 1.1),
+    "falling": lambda n: torch.where(torch.arange(n) < 128, 1.7, 2.0**-9),
+    "first_zero": lambda n: torch.where(torch.arange(n) == 0, 1.0, 2.0**-12 * 1.9),
+    "tiny": lambda n: torch.full((n,), 2.0**-90),
+    "huge": lambda n: torch.full((n,), 2.0**90),
+}
+
+
+@pytest.mark.parametrize("name", SCALES)
+def test_e4m3_scales_of_any_size(name):
+    lens, ctx, groups = [1, 5, 3], [1500, 700, 90], [([0, 1], 640)]
+    zero = [j for j in range(1500) if j % 100 == 3] if name == "zero_tokens" else [0] if name == "first_zero" else []
+    pages, _, _ = _e4m3_pages(ctx, groups, [SCALES[name]] * 3, 22, zero)
+    q = torch.zeros(9, 12, 128, dtype=torch.bfloat16, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for members in ([], groups):
+        out = _ops().shared_prefix_attention(q, pages.cache, 0, make_batch([0, 1, 6], lens, ctx, 9),
+                                             _ops().SharedPrefix.from_groups(members), status=status)
+        for b, r in enumerate((0, 1, 6)):
+            k, v = pages.kv(b)
+            limit = torch.arange(lens[b]) + (ctx[b] - lens[b] + 1)
+            assert_rows(out[r:r + lens[b]], *_f16_tolerance(q[r:r + lens[b]], k, v, limit, 0.1), f"sequence {b}")
+    assert int(status) == 0
+
+
+@pytest.mark.parametrize("scale", [1e30, 1e-30, 0.0, math.inf, math.nan])
+def test_e4m3_scale_of_a_later_token_reaches_no_bit(scale):
+    """The last new token's scale is anything: the rows before it keep their bits, and its own are that token's."""
+    lens, ctx = [5] * 4, [20, 131, 300, 645]
+    pages, pool, pt = _e4m3_pages(ctx, [], [lambda n: torch.rand(n, generator=torch.Generator().manual_seed(n)) + 0.5] * 4, 23)
+    q = torch.randn(20, 12, 128, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    q[:, ::3] *= 8  # (a reference that moves, too)
+
+    def run(groups):
+        return _ops().shared_prefix_attention(q, pages.cache, 0, make_batch([0, 5, 10, 15], lens, ctx, 20),
+                                              _ops().SharedPrefix.from_groups(groups))
+
+    for groups in ([], [([0, 1, 2, 3], 16)]):
+        clean = run(groups)
+        kept = []
+        for b, t in enumerate(ctx):
+            page, at = int(pt[b, (t - 1) // 16]), (t - 1) % 16
+            kept.append((page, at, pool.v_scale[page, :, at].clone()))
+            pool.v_scale[page, :, at] = scale
+        out = run(groups)
+        for b in range(4):
+            assert torch.equal(out[5 * b:5 * b + 4], clean[5 * b:5 * b + 4]), b
+            k, v = pages.kv(b)
+            if math.isfinite(scale):
+                want, tol = plain_attention(q[5 * b + 4:5 * b + 5], k, v, torch.tensor([ctx[b]]), 1 / math.sqrt(128))
+                assert_rows(out[5 * b + 4:5 * b + 5], want, tol, f"sequence {b}")
+            else:
+                assert not out[5 * b + 4].isfinite().any()
+        for page, at, s in kept:
+            pool.v_scale[page, :, at] = s
