@@ -27,7 +27,7 @@ them (``reserve``), share those of another one (``fork``) and give them back (``
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 
 import torch
 
@@ -218,6 +218,14 @@ class PagedKVCache:
             fmt=self.fmt,
             page_refs=self.page_refs,
         )
+
+    def sequences(self, seq0: int, n: int) -> "PagedKVCache":
+        """A view of sequences ``seq0`` .. ``seq0 + n - 1`` as a cache of their own: the same pools, their rows of the page
+        table and of the lengths.  Pages are taken and given back through the whole cache only."""
+        if not 0 <= seq0 < seq0 + n <= self.num_seqs:
+            raise ValueError(f"sequences {seq0} .. {seq0 + n - 1} of {self.num_seqs}")
+        return replace(self, num_seqs=n, page_table=self.page_table[seq0:seq0 + n], lengths=self.lengths[seq0:seq0 + n],
+                       host_lengths=None, page_refs=None)
 
     def set_host_lengths(self, lens: list[int]) -> None:
         if len(lens) != self.num_seqs:

@@ -39,7 +39,7 @@ from __future__ import annotations
 import torch
 
 from ..kernels import ops
-from .model import PagedModel, PieceLayout, StepLayout
+from .model import PagedModel, StepLayout
 from .paged_cache import PAGE
 
 
@@ -64,20 +64,20 @@ class SpecDecEngine:
         if shared_prefix and num_seqs > ops.MOST_SEQUENCES:
             raise ValueError(f"at most {ops.MOST_SEQUENCES} sequences share a prefix")
         self.shared, self.cap, self.filled = shared_prefix, cap, False
-        self.prefix = None
         pages = {}
         if shared_prefix:
             # the prefix's full pages once, everything behind them for each sequence
             full = shared_prefix // PAGE
             pages = dict(on_demand=True, num_pages=full + num_seqs * (-(-cap // PAGE) - full))
-            self.prefix = ops.SharedPrefix.from_groups([(range(num_seqs), shared_prefix)], dev)
         # One layer's attention, shared_prefix_attention against paged_attention (us; prefix + 512 tokens, 1 draft row
         # and 5 target rows a sequence): 64 x 2048 22 against 21 and 29 against 33, 64 x 8192 27 against 41 and 43
         # against 77; 64 x 1024 22 against 17 and 27 against 26, 256 x 1024 53 against 39 and 73 against 67, 16 x 8192
         # 20 against 18 and 29 against 26.
         if share_reads is None:
             share_reads = num_seqs >= 64 and shared_prefix >= 2048
-        self.step_prefix = self.prefix if share_reads else None
+        self.step_prefix = None
+        if shared_prefix and share_reads:
+            self.step_prefix = ops.SharedPrefix.from_groups([(range(num_seqs), shared_prefix)], dev)
         self.tc = target.new_cache(num_seqs, cap, target_v, **pages)
         self.dc = draft.new_cache(num_seqs, cap, draft_v, **pages)
         self.L0 = StepLayout(num_seqs, 2, dev)
@@ -154,16 +154,19 @@ class SpecDecEngine:
             if self.B > 1:
                 cache.fork([0] * (self.B - 1), range(1, self.B), [n0] * (self.B - 1), status=self.status)
             cache.reserve([self.cap] * self.B, status=self.status)
+            layout = prefix = ws = None
             for s0 in range(0, self.B, chunk):
                 n = min(chunk, self.B - s0)
-                piece = PieceLayout(self.B, s0, n, own, self.device)
-                piece.set(cache.lengths)
-                ws = self._workspace(piece, model, cache, self.prefix)
-                h = model.step(prompts[s0:s0 + n, n0:].reshape(-1), piece, cache, ws, status=self.status,
-                               prefix=self.prefix)
+                some = cache.sequences(s0, n)  # a batch of its own: work and workspace are the chunk's
+                if layout is None or layout.num_seqs != n:
+                    layout = StepLayout(n, own, self.device)
+                    prefix = ops.SharedPrefix.from_groups([(range(n), n0)], self.device)
+                    ws = self._workspace(layout, model, some, prefix) if ws is None else ws  # (a last, smaller one fits)
+                layout.set(some.lengths)
+                h = model.step(prompts[s0:s0 + n, n0:].reshape(-1), layout, some, ws, status=self.status, prefix=prefix)
                 if model is self.target:
-                    self.pending[s0:s0 + n] = model.logits(h[piece.last_rows()]).argmax(-1).int()
-                cache.lengths.add_(piece.q_len)
+                    self.pending[s0:s0 + n] = model.logits(h[layout.last_rows()]).argmax(-1).int()
+                some.lengths.add_(layout.q_len)
 
     # ------------------------------------------------------------------ one round
     def _round(self) -> None:
