@@ -468,7 +468,8 @@ int specdec_copy_pages(const SpecdecPagePool* pool, const int32_t* src, const in
 /* Sequence dst[i] gives up its pages and becomes the first length[i] tokens of sequence src[i]: full pages are shared
    (their counts go up), a started one is copied to a page of its own.  All targets give up their pages before any
    page is taken.  SPECDEC_STATUS_BAD_SEQUENCE: a sequence out of range, a length past the source's, a target
-   that is listed before or is itself a source; the request is left out.  SPECDEC_STATUS_BAD_PAGE: the source has no
+   that is listed before, a source that is another request's target (of (0, 1), (1, 2) the first runs); the request is
+   left out.  SPECDEC_STATUS_BAD_PAGE: the source has no
    pages for its tokens; left out.  SPECDEC_STATUS_NO_PAGES: no page for the started one; the target keeps its full
    pages (and their tokens). */
 int specdec_fork_sequences(const SpecdecPagePool* pool, const SpecdecPageTable* table, const int32_t* src,

@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(const PageBook p) {
   const int s = p.a[i], d = p.b[i], len = p.c[i];
   auto in_range = [&](int x) { return x >= 0 && x < p.num_seqs; };
   const bool fine = in_range(s) && in_range(d) && s != d;
-  // a sequence that is forked from stays as it is: it is no target in the same call, and a target is one once
+  // What is forked from stays as it is while others read it: a request whose source is another's target is left out (that
+  // other one runs), and so is one whose target was listed before.  So nobody reads a row that this block writes.
   int bad = !fine || len < 0 || len > p.max_pages * kPage;
   if (!bad) bad = len > p.lengths[s];
   for (int k = tid; k < p.n && fine; k += kForkThreads) {

@@ -849,7 +849,8 @@ def copy_pages(cache: PagedKVCache, src, dst, *, status=None) -> None:
 
 def fork_sequences(cache: PagedKVCache, src, dst, length, *, workspace=None, status=None) -> None:
     """Sequence ``dst[i]`` becomes the first ``length[i]`` tokens of sequence ``src[i]`` (int32 device arrays): full
-    pages are shared, a started one is copied.  What dst held is given up first; no source is a target."""
+    pages are shared, a started one is copied.  What dst held is given up first; no source is a target (a request whose
+    source another one's target is is reported and left out)."""
     lib, dev, stream, pool = _page_pool(cache)
     n = _requests(dev, src, dst, length)
     workspace, table = _page_table(cache, n, workspace, status, lib, dev)
