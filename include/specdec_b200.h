@@ -477,7 +477,8 @@ int specdec_fork_sequences(const SpecdecPagePool* pool, const SpecdecPageTable* 
 
 /* Every sequence gets pages for tokens[b] tokens (fewer than it has: nothing happens).  Held pages that it would go on
    writing into, from position lengths[b] on, are replaced where others hold them, too; what a started one holds is
-   copied.  SPECDEC_STATUS_NO_PAGES: a sequence, and those after it, are left as they were.
+   copied.  Who holds a page is judged by the counts before the call: where all its holders go on writing, each gets a
+   new one, and the page is free after the call.  SPECDEC_STATUS_NO_PAGES: a sequence, and those after it, are left as they were.
    SPECDEC_STATUS_PAGE_OVERFLOW: more tokens than the table has entries for (the sequence is left as it was). */
 int specdec_reserve_pages(const SpecdecPagePool* pool, const SpecdecPageTable* table, const int32_t* tokens,
                           specdec_stream_t stream);

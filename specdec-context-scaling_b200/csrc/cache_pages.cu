@@ -226,7 +226,8 @@ __global__ void __launch_bounds__(kBookThreads) fork_pages_kernel(const PageBook
 }
 
 // Reserve: row s gets pages for a[s] tokens.  Pages that it goes on writing into (from its length on) and that others
-// hold, too, are replaced by new ones, the started page's contents being copied.  Requests are met in the order of
+// hold, too, are replaced by new ones, the started page's contents being copied.  (Counts are those before the call, so
+// that no row's answer depends on another's place: a page that only writers hold is replaced for all of them.)  Requests are met in the order of
 // the sequences until the pages run out; one that cannot be met is left as it was, and so is everyone's after it.
 __global__ void __launch_bounds__(kBookThreads) reserve_kernel(const PageBook p) {
   grid_dep_wait();

@@ -60,3 +60,28 @@ def test_rings_and_doubles_of_forks():
         assert lengths == want, pairs
         held = [p for row in table for p in row if p >= 0]
         assert [held.count(p) for p in range(20)] == refs
+
+
+def test_a_page_that_all_its_holders_write_into():
+    """Both go on in a page that they share: both get new ones, judged by the counts before the call, and the page is free
+    after it; where only one new page is left the second is refused, and gets by in a second call."""
+    from specdec_b200 import _lib
+
+    for pages in (10, 2):
+        c = _cache(2, pages, 32)
+        c.reserve([16, 0])
+        c.lengths.copy_(i32([16, 0]))
+        c.fork([0], [1], [16])
+        c.lengths.copy_(i32([8, 8]))
+        first = _bytes(c)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        c.reserve([16, 16], status=status)
+        table, _, refs = _state(c)
+        if pages == 10:
+            assert int(status) == 0 and table == [[1, -1], [2, -1]] and refs[:3] == [0, 1, 1]
+            assert torch.equal(_bytes(c)[1:3], first[[0, 0]])
+        else:
+            assert int(status) == _lib.STATUS_NO_PAGES and table == [[1, -1], [0, -1]] and refs == [1, 1]
+            status.zero_()
+            c.reserve([16, 16], status=status)
+            assert int(status) == 0 and _state(c)[0] == [[1, -1], [0, -1]]
