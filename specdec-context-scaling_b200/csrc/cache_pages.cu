@@ -122,10 +122,10 @@ SD_DEV int lowest_free(const PageBook& p, int want, int32_t* list) {
 
 SD_DEV bool page_ok(const PageBook& p, int page) { return page >= 0 && page < p.num_pages; }
 
-// Row s of the table gives up its pages from entry `keep` on.
-SD_DEV void drop_row(const PageBook& p, int s, int keep, int lane) {
+// Row s of the table gives up its pages.
+SD_DEV void drop_row(const PageBook& p, int s, int lane) {
   int32_t* row = p.table + static_cast<int64_t>(s) * p.max_pages;
-  for (int base = keep + lane; base < p.max_pages; base += 8 * 32) {
+  for (int base = lane; base < p.max_pages; base += 8 * 32) {
     int page[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) page[e] = base + 32 * e < p.max_pages ? row[base + 32 * e] : -1;
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kBookThreads) free_kernel(const PageBook p) {
   for (int i = warp; i < p.n; i += kBookThreads / 32) {
     const int s = p.a[i];
     if (s < 0 || s >= p.num_seqs || mark[s] != i) continue;  // named twice: once is enough
-    drop_row(p, s, 0, lane);
+    drop_row(p, s, lane);
     if (lane == 0) p.lengths[s] = 0;
   }
 }
