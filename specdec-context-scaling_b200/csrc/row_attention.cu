@@ -381,7 +381,7 @@ SD_DEV bool make_plan(const RowParams& p, uint8_t* at, int64_t (*tot)[32], int* 
         }
         total = 0;
       }
-      quota = max((static_cast<int>(total) + p.grid - 1) / p.grid, p.min_quota);
+      quota = max(static_cast<int>((static_cast<uint32_t>(total) + p.grid - 1) / p.grid), p.min_quota);
       from = blockIdx.x * quota;
       to = min(from + quota, total);
       direct_items = quota <= (1 + kUnitCost) * (ITEMS - 2);
