@@ -304,3 +304,21 @@ def test_e4m3_scale_of_a_later_token_reaches_no_bit(scale):
                 assert not out[5 * b + 4].isfinite().any()
         for page, at, s in kept:
             pool.v_scale[page, :, at] = s
+
+
+def test_as_many_groups_as_sequences():
+    """2048 groups of one sequence each, the most of a call: values, against the 64-bit form."""
+    B, H, KV, D = 2048, 14, 2, 64
+    g = torch.Generator().manual_seed(12)
+    ctx = torch.randint(33, 80, (B,), generator=g).tolist()
+    pages = Pages(ctx, [], KV, D, False, 12)
+    q = torch.randn(B, H, D, generator=g).to(torch.bfloat16).cuda()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    order = torch.randperm(B, generator=g).tolist()
+    for groups in ([([b], 32) for b in order], [([b], 16 * (b % 3)) for b in range(B)]):
+        out = _ops().shared_prefix_attention(q, pages.cache, 0, make_batch(list(range(B)), [1] * B, ctx, B),
+                                             _ops().SharedPrefix.from_groups(groups), status=status)
+        for b in [0, 1, B - 2, B - 1, *torch.randperm(B, generator=g)[:150].tolist()]:
+            k, v = pages.kv(b)
+            assert_rows(out[b:b + 1], *plain_attention(q[b:b + 1], k, v, torch.tensor([ctx[b]]), 1 / math.sqrt(D)), f"{b}")
+    assert int(status) == 0
