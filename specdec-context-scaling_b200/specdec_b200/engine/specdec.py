@@ -24,8 +24,9 @@ emitted for it, so its caches stop growing while slower sequences finish.
 
 With ``shared_prefix`` tokens the prompts begin alike (a system prompt): these are read once, by
 sequence 0, whose pages the others fork; what follows them is read by one step a chunk of sequences.  In a large
-batch over a long prefix every step of a round, too, reads the shared pages once (``ops.shared_prefix_attention``);
-else ``ops.paged_attention`` reads them for each sequence, which is faster there.
+batch over a prefix that is long, also beside what a sequence has of its own, every step of a round reads the shared
+pages once, too (``ops.shared_prefix_attention``); else ``ops.paged_attention`` reads them for each sequence, which is
+faster there.
 
 Every step of a round is a fixed-shape device computation (the ragged q_len of
 step 1 lives in device arrays), so a round is captured once in a CUDA graph and
@@ -69,12 +70,15 @@ class SpecDecEngine:
             # the prefix's full pages once, everything behind them for each sequence
             full = shared_prefix // PAGE
             pages = dict(on_demand=True, num_pages=full + num_seqs * (-(-cap // PAGE) - full))
-        # One layer's attention, shared_prefix_attention against paged_attention (us; prefix + 512 tokens, 1 draft row
-        # and 5 target rows a sequence): 64 x 2048 22 against 21 and 29 against 33, 64 x 8192 27 against 41 and 43
-        # against 77; 64 x 1024 22 against 17 and 27 against 26, 256 x 1024 53 against 39 and 73 against 67, 16 x 8192
-        # 20 against 18 and 29 against 26.
+        # One layer's attention, shared_prefix_attention against paged_attention (us; 1 draft row and 5 target rows a
+        # sequence).  Prefix + 512 own tokens: 64 x 2048 23 against 22 and 29 against 34, 64 x 8192 27 against 42 and 43
+        # against 77, 256 x 2048 56 against 54 and 83 against 97; 64 x 1024 22 against 17 and 27 against 26, 256 x 1024
+        # 53 against 39 and 73 against 67, 16 x 8192 20 against 18 and 29 against 26.  Own tokens are the slower half: with
+        # 2048 of them 64 x 8192 48 against 48 and 64 against 90, 64 x 2048 43 against 27 and 48 against 48, 256 x 4096
+        # 146 against 104 and 183 against 202; with 6144 64 x 8192 107 against 66 and 122 against 124.  Even where the
+        # prefix is about four times as long as what a sequence has of its own.
         if share_reads is None:
-            share_reads = num_seqs >= 64 and shared_prefix >= 2048
+            share_reads = num_seqs >= 64 and shared_prefix >= max(2048, 4 * (prompt_len + max_new - shared_prefix))
         self.step_prefix = None
         if shared_prefix and share_reads:
             self.step_prefix = ops.SharedPrefix.from_groups([(range(num_seqs), shared_prefix)], dev)

@@ -90,3 +90,13 @@ def test_sequences_of_a_cache():
                   max_new=1)
     assert all((c.gather_layer(0, b, 10)["k"][0][:, 9] == 1).all() for b in (1, 2, 3))
     assert not c.gather_layer(0, 0, 10)["k"].any() and not c.gather_layer(0, 4, 10)["k"].any()
+
+
+@pytest.mark.parametrize("B,P,N,shared,want", [(64, 2304, 16, 2048, True), (64, 2544, 16, 2048, True),
+                                               (64, 2545, 16, 2048, False), (64, 2304, 400, 2048, False),
+                                               (63, 2304, 16, 2048, False), (64, 2100, 16, 2047, False)])
+def test_rounds_share_reads_where_the_prefix_outweighs_the_rest(B, P, N, shared, want):
+    """64 sequences, 2048 shared tokens and four times as many of them as a sequence has of its own; an argument decides
+    otherwise."""
+    assert (_engine(B, P, N, shared).step_prefix is not None) == want
+    assert (_engine(B, P, N, shared, share_reads=not want).step_prefix is not None) == (not want)
