@@ -1027,6 +1027,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
 #pragma unroll 1
                 for (int c = 0; c < min(limit - key0, kKeyBlock / 2); ++c)
                   if (fabsf(vs[c]) < INFINITY) scales = fmaxf(scales, fabsf(vs[c]));
+                __syncwarp();
                 redo = moves(scales);
               }
               if (scales > kGrowF16 / 2) top += __log2f(scales * (2 / kGrowF16)) / scale;
