@@ -178,6 +178,8 @@ struct PartInfo {
   int n_vt, k0, first;  // tokens; keys k0 .. first + i (a sequence's token i) or k0 .. first - 1
   bool group;
 };
+// (A group's members count q_max tokens each, whether or not they have so many: token vt is row vt % q_max of member
+// vt / q_max, with nothing to look up.)
 SD_DEV PartInfo part_info(const RowParams& p, const PlanSpace& w, int part) {
   PartInfo f;
   f.group = part < p.G;
@@ -1069,7 +1071,7 @@ __global__ void __launch_bounds__(RowRoles<SRC>::THREADS, 1) row_attention_kerne
       if (!AHEAD && wash == 0 && was_idle) lazy_wait(&s_full[t][0], sn & 1, dead, p.wait_ns);
       if (AHEAD) load(even);
       // Pages at head_dim 128: one body for both halves, half the instructions to fetch, which items of few blocks wait for
-      // (E4M3 64 requests x 5 rows 70.6 -> 64.7 us, 3 groups of 16 41.1 -> 38.4).  Long prompts are better off with two
+      // (E4M3 64 requests x 5 rows over 8192 74.6 -> 65.0 us, 3 groups of 16 43.1 -> 40.9).  Long prompts are better off with two
       // (4 x 8192 tokens 838 us against 875).
       if constexpr (AHEAD || SRC == kPacked) {
         for (int k = 0; k < nh; k += 2) {

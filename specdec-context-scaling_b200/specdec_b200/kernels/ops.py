@@ -750,7 +750,8 @@ def shared_prefix_attention(q, cache: PagedKVCache, layer: int, batch: RaggedBat
     answer, the pages of a group's prefix read once for all of its members.
 
     Of ``prefix_len`` the whole pages that every row of the group sees are shared; they are read from the table of the
-    group's first member that has rows.  ``reuse_plan``: ``workspace`` holds the plan of an earlier call with the same
+    group's first member that has rows.  A group's work and workspace go by its members times ``max_q_len``, so that
+    members without rows cost what others do (``PagedKVCache.sequences`` makes a batch of some of them).  ``reuse_plan``: ``workspace`` holds the plan of an earlier call with the same
     batch and prefix (the layers of one step)."""
     lib, dev, stream = _call(q)
     rows, H, D, q_st, q_sh, q_at = _head_rows(q, "q")
