@@ -322,3 +322,19 @@ def test_as_many_groups_as_sequences():
             k, v = pages.kv(b)
             assert_rows(out[b:b + 1], *plain_attention(q[b:b + 1], k, v, torch.tensor([ctx[b]]), 1 / math.sqrt(D)), f"{b}")
     assert int(status) == 0
+
+
+def test_groups_without_members():
+    """Groups that list nobody, and no member at all: every sequence is attended to alone."""
+    ops, (H, KV, D) = _ops(), (12, 2, 128)
+    lens, ctx = [5, 1, 0, 140], [300, 17, 9, 2000]
+    pages = Pages(ctx, [], KV, D, True, 31)
+    row0 = [0, 5, 6, 6]
+    q = torch.randn(146, H, D, generator=torch.Generator().manual_seed(8)).to(torch.bfloat16).cuda()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for groups in ([([], 16)], [([], 0), ([], 1000)], []):
+        out = torch.full_like(q, FILL)
+        ops.shared_prefix_attention(q, pages.cache, 0, make_batch(row0, lens, ctx, 146), ops.SharedPrefix.from_groups(groups),
+                                    out=out, status=status)
+        check_pages(out, FILL, q, pages, row0, lens, ctx, what=str(groups))
+    assert int(status) == 0
