@@ -274,6 +274,20 @@ def test_e4m3_scales_of_any_size(name):
     assert int(status) == 0
 
 
+@pytest.mark.parametrize("below", [10, 16, 18, 20])
+def test_e4m3_scales_far_below_the_mean_lose_bits_only(below):
+    """The first 128 tokens are zeros (scale 1), the others' scales are 2^-below: their weights count as 1.3 2^(2 - below),
+    below 2^-14 a number of f16's subnormal range, off by half of its step, 2^-25, and not by all of it."""
+    n = 600
+    pages, _, _ = _e4m3_pages([n], [], [lambda n: torch.where(torch.arange(n) < 128, 1.0, 1.3 * 2.0**-below)], 24, range(128))
+    q = torch.zeros(1, 12, 128, dtype=torch.bfloat16, device="cuda")
+    out = _ops().shared_prefix_attention(q, pages.cache, 0, make_batch([0], [1], [n], 1), _ops().SharedPrefix.from_groups([]))
+    k, v = pages.kv(0)
+    want, tol = _f16_tolerance(q, k, v, torch.tensor([n]), 0.1)
+    A, _ = plain_attention(q, k, v.abs(), torch.tensor([n]), 0.1)
+    assert_rows(out, want, tol + A * (2.0**-25 / (1.3 * 2.0**(2 - below))), f"2^-{below}")
+
+
 @pytest.mark.parametrize("scale", [1e30, 1e-30, 0.0, math.inf, math.nan])
 def test_e4m3_scale_of_a_later_token_reaches_no_bit(scale):
     """The last new token's scale is anything: the rows before it keep their bits, and its own are that token's."""
